@@ -1,0 +1,216 @@
+"""Attention of a batch over a shared prefix (yskn_b200_prefix_attention) against the formula in
+64 bits.
+
+Tolerance. With w the softmax weights and A = sum w |v|: the weights are rounded to p bits
+(bf16 8, f16 11) before they meet the values, at most 2^-p A in the sum (f16 weights below
+2^-14 of the largest lose at most 2^-24 each: 2^-24 sum |v|); scores are binary32 sums of D products, off by at most
+e = 2^-22 D scale sum |q k| (a unit for each addition, twice for truncating adders), which moves
+the quotient by at most 2 e A; the sums over n rows by 2^-23 n' A with n' the longest chain of
+additions (n at most); exponentials by 2^-21. The result is rounded once: 2^-p |out|."""
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+P_BITS = {"bf16": 8, "f16": 11}
+
+
+def run(cuda, new=(1, 1), own=(5, 40), P=100, n_qh=6, n_kvh=2, D=128, dtype="bf16", block=16, gate=False,
+        paired=False, head_major=True, pad_tokens=0, lens=None, seed=0, stream=None, scale=None, spread=1.0,
+        fill=float("nan"), max_new=None, check=True):
+    """own: each request's own rows with its new ones; lens overrides P + own."""
+    import torch
+    import yskn_b200 as Y
+    dt = {"bf16": torch.bfloat16, "f16": torch.float16}[dtype]
+    g = torch.Generator(device=cuda)
+    g.manual_seed(seed)
+    B, T = len(new), sum(new) + pad_tokens
+    lens = [P + o for o in own] if lens is None else lens
+    pre = -(-P // block)
+    held = [-(-max(n - P, 0) // block) for n in lens]
+    n_blocks = pre + sum(held) + 2
+    shape = (n_blocks, n_kvh, block, D) if head_major else (n_blocks, block, n_kvh, D)
+    # rows that no request owns hold `fill`
+    caches = [torch.full(shape, fill, dtype=dt, device=cuda) for _ in range(2)]
+    kc, vc = (c.transpose(1, 2) if head_major else c for c in caches)
+    numbers = torch.randperm(n_blocks, generator=g, device=cuda).to(torch.int32)
+    width = max(held + [1]) + 2
+    tables = torch.full((B, width + 1), 2 ** 30, dtype=torch.int32, device=cuda)[:, :width]  # unused: not a block
+    at = pre
+    rows = {}
+    for i in range(B):
+        tables[i, :held[i]] = numbers[at:at + held[i]]
+        at += held[i]
+    prefix_blocks = numbers[:pre].clone()
+
+    def put(cache, blocks, n):
+        x = (torch.randn((n, n_kvh, D), generator=g, device=cuda) * spread).to(dt)
+        j = torch.arange(n, device=cuda)
+        cache[blocks.long()[j // block], j % block] = x
+        return x
+
+    pk, pv = put(kc, prefix_blocks, P), put(vc, prefix_blocks, P)
+    for i in range(B):
+        n = max(lens[i] - P, 0)
+        rows[i] = [torch.cat([a, put(c, tables[i], n)]) for a, c in ((pk, kc), (pv, vc))]
+    q = (torch.randn((T, n_qh, D * (2 if paired else 1)), generator=g, device=cuda) * 1.5).to(dt)[:, :, :D]
+    gt = (torch.randn((T, n_qh, 2 * D), generator=g, device=cuda) * 2).to(dt)[:, :, D:] if gate else None
+    starts = np.concatenate([[0], np.cumsum(new)])
+    i32 = lambda a: torch.tensor(list(map(int, a)), dtype=torch.int32, device=cuda)  # noqa: E731
+    max_new = max(max(new), 1) if max_new is None else max_new
+    work = torch.full((Y.prefix_attention_work_bytes(T, B, max_new, n_qh, n_kvh, D),), 255, dtype=torch.uint8,
+                      device=cuda)
+    out = torch.full((T, n_qh, D), 3.0, dtype=dt, device=cuda)
+    d_lens, d_starts = i32(lens), i32(starts)
+    torch.cuda.synchronize()
+    Y.prefix_attention(q, kc, vc, tables, d_lens, d_starts, max_new, work, out, prefix_blocks=prefix_blocks,
+                       prefix_len=P, gate=gt, scale=scale, stream=stream)
+    torch.cuda.synchronize()
+    if not check:
+        return out
+    assert Y.status() == 0
+    G, sc, u = n_qh // n_kvh, D ** -0.5 if scale is None else scale, 2.0 ** -P_BITS[dtype]
+    for i in range(B):
+        for t in range(new[i]):
+            lim = max(0, lens[i] - new[i] + t + 1)
+            tok = int(starts[i]) + t
+            if lim == 0:
+                assert bool((out[tok] == 0).all())
+                continue
+            k, v = (r[:lim].double().repeat_interleave(G, 1) for r in rows[i])  # [lim][n_qh][D]
+            qd = q[tok].double()
+            s = torch.einsum("hd,lhd->hl", qd, k) * sc
+            w = torch.softmax(s, -1)
+            y, A = torch.einsum("hl,lhd->hd", w, v), torch.einsum("hl,lhd->hd", w, v.abs())
+            e = 2.0 ** -22 * D * abs(sc) * torch.einsum("hd,lhd->hl", qd.abs(), k.abs()).amax(-1)[:, None]
+            tol = (u + 2 * e + 2.0 ** -23 * lim + 2.0 ** -21) * A
+            if dtype == "f16":
+                # weights relative to the row's largest; a stale maximum scales them up, never down
+                tol = tol + 2.0 ** -24 * (v.abs().sum(0) / torch.exp(s - s.amax(-1, keepdim=True)).sum(-1)[:, None])
+            if gate:
+                sg = torch.sigmoid(gt[tok].double())
+                y, tol = y * sg, tol * sg + 2.0 ** -20 * (y * sg).abs()
+            tol = tol + u * y.abs() + 2.0 ** -25
+            d = (out[tok].double() - y).abs()
+            assert bool((d <= tol).all()), (i, t, float((d - tol).max()), float(d.max()))
+    if pad_tokens:
+        assert bool((out[T - pad_tokens:] == 0).all())
+    return out
+
+
+@pytest.mark.parametrize("P", [0, 1, 15, 16, 127, 128, 129, 1000, 5000])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_prefix_lengths(cuda, P, D):
+    run(cuda, P=P, D=D, new=(1, 1, 1), own=(1, 17, 300), seed=P + D)
+
+
+@pytest.mark.parametrize("own", [1, 2, 16, 63, 64, 65, 127, 128, 129, 600])
+def test_own_lengths(cuda, own):
+    run(cuda, own=(own, 3), P=64, seed=own)
+
+
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+@pytest.mark.parametrize("head_major", [True, False])
+def test_block_sizes_and_orders(cuda, block, head_major):
+    run(cuda, P=333, new=(2, 1, 5), own=(200, 64, 131), block=block, head_major=head_major, D=256, seed=block)
+
+
+@pytest.mark.parametrize("n_qh,n_kvh", [(1, 1), (4, 4), (24, 4), (5, 1), (16, 2), (128, 1), (14, 2), (60, 3)])
+def test_head_groups(cuda, n_qh, n_kvh):
+    run(cuda, n_qh=n_qh, n_kvh=n_kvh, new=(1, 3, 1), own=(9, 140, 1), P=200, seed=n_qh)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("gate,paired", [(True, False), (False, True), (True, True)])
+@pytest.mark.parametrize("D", [64, 256])
+def test_types_gates_and_strides(cuda, dtype, gate, paired, D):
+    run(cuda, dtype=dtype, gate=gate, paired=paired, D=D, new=(1, 4), own=(50, 200), P=150, seed=3)
+
+
+@pytest.mark.parametrize("new,own", [((130, 1, 47), (300, 1, 47)), ((300,), (300,)), ((33, 64, 2), (500, 64, 128)),
+                                     ((8,) * 19, tuple(range(8, 160, 8)))])
+@pytest.mark.parametrize("D", [128, 256])
+def test_prompt_chunks_are_causal(cuda, new, own, D):
+    run(cuda, new=new, own=own, P=70, D=D, seed=len(new))
+
+
+def test_batches_larger_than_a_tile(cuda):
+    run(cuda, new=(1,) * 70, own=tuple(1 + 5 * i % 211 for i in range(70)), n_qh=24, n_kvh=4, D=256, P=700, gate=True,
+        seed=1)
+    run(cuda, new=(1,) * 300, own=tuple(1 + i % 7 for i in range(300)), n_qh=4, n_kvh=1, D=64, P=40, seed=2)
+
+
+def test_requests_that_see_nothing_or_little(cuda):
+    """Empty, idle and short requests: a length of zero, below the prefix, below their tokens."""
+    run(cuda, new=(1, 0, 1, 3, 2, 0, 2), lens=[0, 0, 30, 2, 101, 120, 1], P=100, seed=4)
+    run(cuda, new=(2, 3), lens=[0, 0], P=0, seed=5)
+    run(cuda, new=(0, 4, 0, 0, 1, 0), lens=[0, 104, 0, 500, 260, 0], P=100, pad_tokens=5, seed=6)
+
+
+def test_padded_tokens_give_zeros(cuda):
+    run(cuda, new=(1, 1), own=(5, 40), pad_tokens=200, seed=7)
+    run(cuda, new=(0, 0), own=(5, 40), pad_tokens=3, seed=8)
+
+
+@pytest.mark.parametrize("fill", [float("inf"), float("-inf"), 3e38, 0.0])
+def test_rows_outside_hold_anything(cuda, fill):
+    """NaN (the other tests' fill), infinities and huge values in every row that no token sees."""
+    import torch
+    a = run(cuda, P=77, own=(9, 150), fill=fill, D=256, seed=9)
+    assert torch.equal(a, run(cuda, P=77, own=(9, 150), D=256, seed=9))
+
+
+def test_rising_and_large_scores(cuda):
+    run(cuda, P=900, own=(300, 7), spread=6.0, scale=1.0 / 16, D=256, seed=10)
+    run(cuda, P=900, own=(300, 7), spread=6.0, scale=1.0 / 16, D=256, dtype="f16", seed=10)
+    run(cuda, P=300, own=(30, 7), scale=-0.1, seed=11)
+    run(cuda, P=300, own=(30, 7), scale=0.0, seed=12)
+
+
+def test_same_result_twice_and_on_another_stream(cuda):
+    import torch
+    kw = dict(new=(1, 9, 1), own=(400, 129, 1), P=2000, D=256, n_qh=24, n_kvh=4, gate=True, seed=13)
+    a = run(cuda, **kw)
+    assert torch.equal(a, run(cuda, **kw)) and torch.equal(a, run(cuda, stream=torch.cuda.Stream(), **kw))
+
+
+def test_long_cache(cuda):
+    """Blocks past 2^31 elements into the cache."""
+    import torch
+    import yskn_b200 as Y
+    D, block, n_blocks = 256, 128, 70000  # 70000 * 128 * 256 > 2^31 elements
+    kc = torch.zeros((n_blocks, block, 1, D), dtype=torch.bfloat16, device=cuda)
+    vc = torch.zeros((n_blocks, block, 1, D), dtype=torch.bfloat16, device=cuda)
+    kc[-1].normal_()
+    vc[-1].normal_()
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device=cuda)  # noqa: E731
+    q = torch.randn((1, 2, D), device=cuda).to(torch.bfloat16)
+    out = torch.empty_like(q)
+    work = torch.empty(Y.prefix_attention_work_bytes(1, 1, 1, 2, 1, D), dtype=torch.uint8, device=cuda)
+    Y.prefix_attention(q, kc, vc, i32(n_blocks - 1)[None], i32(100), i32(0, 1), 1, work, out)
+    w = torch.softmax(torch.einsum("hd,ld->hl", q[0].double(), kc[-1, :100, 0].double()) / 16, -1)
+    y, A = w @ vc[-1, :100, 0].double(), w @ vc[-1, :100, 0].double().abs()
+    assert Y.status() == 0
+    assert bool(((out[0].double() - y).abs() <= 2.0 ** -8 * y.abs() + (2.0 ** -8 + 1e-2) * A).all())
+
+
+def test_blocks_outside_the_cache_are_reported(cuda):
+    import torch
+    import yskn_b200 as Y
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device=cuda)  # noqa: E731
+    c = torch.ones((4, 16, 1, 64), dtype=torch.bfloat16, device=cuda)
+    q = torch.ones((1, 1, 64), dtype=torch.bfloat16, device=cuda)
+    work = torch.empty(Y.prefix_attention_work_bytes(1, 1, 1, 1, 1, 64), dtype=torch.uint8, device=cuda)
+    for bad in (4, -1, 2 ** 30):
+        Y.prefix_attention(q, c, c, i32(0, bad)[None], i32(20), i32(0, 1), 1, work, torch.empty_like(q))
+        assert Y.status() == Y.EINVAL
+    Y.prefix_attention(q, c, c, i32(0, 9)[None], i32(16), i32(0, 1), 1, work, torch.empty_like(q))
+    assert Y.status() == 0  # an entry past the length is not looked at
+
+
+def test_more_tokens_than_promised_are_reported(cuda):
+    import yskn_b200 as Y
+    run(cuda, new=(3, 200), own=(20, 200), max_new=1, check=False)
+    assert Y.status() == Y.EINVAL
+    run(cuda, new=(3, 2), own=(20, 20), seed=1)

@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 #include <utility>
 
@@ -53,6 +54,22 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
+
+// Opts a kernel into more than 48 KB of dynamic shared memory, once per device (the attribute
+// belongs to the device's context). One static object per kernel.
+struct SmemOptIn {
+  std::atomic<uint64_t> done{0};
+  template <typename K>
+  cudaError_t operator()(K* kernel, int bytes) {
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) return e;
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+  }
+};
 
 // Thread-local error message (src/c_api.cpp:11-14 keeps one per thread as well).
 int fail(int code, const std::string& msg);

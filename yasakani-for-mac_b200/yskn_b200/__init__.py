@@ -92,6 +92,15 @@ _SIGNATURES = {
     "yskn_b200_head_merge": (_i, [_vp, _vp, _i64, _vp, _i, _i, _vp, _vp, _vp, _vp]),
     "yskn_b200_linear_from_residual": (_i, [_vp, _i, _vp, _vp, _vp, _vp, C.c_float, _i, _vp, _vp, _vp, _vp]),
     "yskn_b200_linear_rowpar_q8": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp]),
+    "yskn_b200_batch_plan": (_i, [_vp, _vp, _i, _i, _i, _vp, _i, _i64, _vp, _i, _vp, _i] + [_vp] * 7),
+    "yskn_b200_paged_prep": (_i, [_vp, _i64, _i64] * 3 + [_i, _vp, _vp, _i64, _vp, _vp, _i, _vp, _vp, C.c_float,
+                                                          _i, _i, _i, _i, _vp, _vp, _vp, _i64, _i64, _i64, _i, _i,
+                                                          _i, _vp]),
+    "yskn_b200_prefix_attention_work_bytes": (_i64, [_i] * 6),
+    "yskn_b200_prefix_attention": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i, _i, _vp, _i,
+                                        _vp, _i, _i64, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, C.c_float, _vp, _vp,
+                                        _vp]),
+    "yskn_b200_logits_adjust": (_i, [_vp, _i64, _i, _i, _vp, _i64, _i] + [_vp] * 7 + [_i, _vp, _i64, _vp, _i64, _vp]),
 }
 
 _lib = None
@@ -659,3 +668,155 @@ def kv_encode(rows, row_group, tables, gains, mults, kb, vit2, words, scales, me
     check(lib().yskn_b200_kv_encode(_ptr(rows), _ptr(row_group), rows.shape[0], _ptr(tables), _ptr(gains),
                                     _ptr(means), _ptr(has_mean), _ptr(mults), mults.shape[0], kb, int(vit2),
                                     _ptr(dest), _ptr(words), _ptr(scales), _stream(stream)), "kv_encode")
+
+
+DT_F32, DT_F16, DT_BF16 = 0, 1, 2
+_DT = {}
+
+
+def _dtype(t):
+    """YSKN_DT_* of a tensor; int16 tensors hold bf16 bits, as everywhere in this binding."""
+    if not _DT:
+        import torch
+        _DT.update({torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.int16: DT_BF16})
+    if t.dtype not in _DT:
+        raise YsknError(EINVAL, "a tensor of f32, f16, bf16 or int16 (bf16 bits) expected, not %s" % t.dtype)
+    return _DT[t.dtype]
+
+
+def _need(ok, what):
+    if not ok:
+        raise YsknError(EINVAL, what)
+
+
+def _is_i32(*tensors):
+    import torch
+    return all(t is None or t.dtype == torch.int32 for t in tensors)
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stream_address(stream):
+    import torch
+    return (torch.cuda.current_stream() if stream is None else stream).cuda_stream
+
+
+def batch_plan(lens, new_lens, block_tables, pool, free_count, block_size, lens_out, free_out, starts, slots, positions,
+               requests, prefix_len=0, stream=None):
+    """yskn_b200_batch_plan: blocks from `pool` (int32 stack of *free_count numbers) for the new
+    tokens of each request (new_lens int32 [batch]; negative: the request has ended), written
+    into block_tables (int32 [batch][width]); the new lengths and count, the served tokens
+    before each request (starts int32 [batch + 1]) and per token its slot (int64), position
+    and request (int32), -1 past the last one."""
+    B, width = block_tables.shape
+    T = slots.shape[0]
+    _need(_is_i32(lens, new_lens, block_tables, pool, free_count, lens_out, free_out, starts, positions, requests) and
+          slots.element_size() == 8 and lens.shape[0] == new_lens.shape[0] == lens_out.shape[0] == B and
+          starts.shape[0] == B + 1 and positions.shape[0] == requests.shape[0] == T and block_tables.stride(1) == 1,
+          "batch_plan: int32 arrays of the batch, int64 slots and as many positions and requests expected")
+    check(lib().yskn_b200_batch_plan(lens.data_ptr(), new_lens.data_ptr(), B, block_size, prefix_len,
+                                     block_tables.data_ptr(), width, block_tables.stride(0), pool.data_ptr(),
+                                     pool.shape[0], free_count.data_ptr(), T, lens_out.data_ptr(),
+                                     free_out.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+                                     requests.data_ptr(), _stream_address(stream)), "batch_plan")
+
+
+def paged_prep(q, k, v, slots, positions, query, k_cache, v_cache, inv_freq=None, axes=None, q_norm=None, k_norm=None,
+               eps=1e-6, stream=None):
+    """yskn_b200_paged_prep: q [T][n_qh][D], k and v [T][n_kvh][D] (f32 or the cache's type, any
+    strides with dense channels) normalised (q_norm, k_norm bf16 [D]) and rotated (inv_freq f32
+    [rot / 2], axes the position axis of each pair, positions int32 [n_axes][T] or [T]) into
+    query (dense [T][n_qh][D]) and, at `slots` (int64 [T]), k_cache and v_cache (views
+    [n_blocks][block_size][n_kvh][D] of the same strides)."""
+    T, n_qh, D = query.shape
+    n_blocks, block_size, n_kvh = k_cache.shape[:3]
+    rot = 0 if inv_freq is None else 2 * inv_freq.shape[0]
+    _need(tuple(q.shape) == (T, n_qh, D) and tuple(k.shape) == tuple(v.shape) == (T, n_kvh, D) and
+          k_cache.shape[3] == D and v_cache.shape == k_cache.shape and v_cache.stride() == k_cache.stride() and
+          k_cache.stride(3) == q.stride(2) == k.stride(2) == v.stride(2) == 1 and query.is_contiguous(),
+          "paged_prep: q, k, v of the caches' heads with dense channels, caches of one shape and strides expected")
+    _need(_dtype(q) == _dtype(k) == _dtype(v) and _dtype(query) == _dtype(k_cache) == _dtype(v_cache) and
+          slots.element_size() == 8 and slots.shape[0] == T, "paged_prep: types of q, k, v or of the caches differ")
+    packed, stride = None, 0
+    if rot:
+        axes = bytes(axes) if axes is not None else bytes(rot // 2)
+        n_axes = 1 if positions.dim() == 1 else positions.shape[0]
+        _need(_is_i32(positions) and positions.shape[-1] == T and positions.stride(-1) == 1 and
+              len(axes) == rot // 2 and max(axes) < n_axes,
+              "paged_prep: int32 positions of every token, and an axis of them for each pair expected")
+        packed, stride = axes, positions.stride(0) if positions.dim() == 2 else T
+    check(lib().yskn_b200_paged_prep(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+                                     v.data_ptr(), v.stride(0), v.stride(1), _dtype(q), slots.data_ptr(),
+                                     _address(positions), stride, _address(inv_freq), packed, rot, _address(q_norm),
+                                     _address(k_norm), eps, T, n_qh, n_kvh, D, query.data_ptr(), k_cache.data_ptr(),
+                                     v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
+                                     n_blocks, block_size, _dtype(k_cache), _stream_address(stream)), "paged_prep")
+
+
+def prefix_attention_work_bytes(tokens, batch, max_new, n_qh, n_kvh, head):
+    n = lib().yskn_b200_prefix_attention_work_bytes(tokens, batch, max_new, n_qh, n_kvh, head)
+    _need(n >= 0, "prefix_attention_work_bytes: unsupported shape")
+    return n
+
+
+def prefix_attention(q, k_cache, v_cache, block_tables, lens, starts, max_new, work, out, prefix_blocks=None,
+                     prefix_len=0, gate=None, scale=None, stream=None):
+    """yskn_b200_prefix_attention: q (and gate) [T][n_qh][D] with dense channels, the caches as
+    paged_prep, each request's own blocks in block_tables (int32 [batch][width]) and the shared
+    prefix's in prefix_blocks; lens and starts as batch_plan writes them (at most max_new tokens
+    a request) -> out (dense [T][n_qh][D]). scale defaults to 1 / sqrt(D)."""
+    T, n_qh, D = out.shape
+    n_blocks, block_size, n_kvh = k_cache.shape[:3]
+    B, width = block_tables.shape
+    dt = _dtype(q)
+    _need(tuple(q.shape) == (T, n_qh, D) and (gate is None or (gate.shape == q.shape and gate.stride(2) == 1 and
+                                                               _dtype(gate) == dt)) and
+          k_cache.shape[3] == D and v_cache.shape == k_cache.shape and v_cache.stride() == k_cache.stride() and
+          k_cache.stride(3) == q.stride(2) == 1 and out.is_contiguous() and
+          _dtype(k_cache) == _dtype(v_cache) == _dtype(out) == dt,
+          "prefix_attention: q, gate, out and caches of one type and head size with dense channels expected")
+    _need(_is_i32(block_tables, lens, starts, prefix_blocks) and lens.shape[0] == B and starts.shape[0] == B + 1 and
+          block_tables.stride(1) == 1 and
+          (prefix_len == 0 or (prefix_blocks is not None and prefix_blocks.shape[0] * block_size >= prefix_len)),
+          "prefix_attention: int32 tables, lengths and starts of one batch, and the prefix's blocks expected")
+    _need(work.numel() * work.element_size() >= prefix_attention_work_bytes(T, B, max_new, n_qh, n_kvh, D),
+          "prefix_attention: workspace too small")
+    check(lib().yskn_b200_prefix_attention(q.data_ptr(), q.stride(0), q.stride(1), _address(gate),
+                                           gate.stride(0) if gate is not None else 0,
+                                           gate.stride(1) if gate is not None else 0, k_cache.data_ptr(),
+                                           v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),
+                                           k_cache.stride(2), n_blocks, block_size,
+                                           _address(prefix_blocks) if prefix_len else None, prefix_len,
+                                           block_tables.data_ptr(), width, block_tables.stride(0), lens.data_ptr(),
+                                           starts.data_ptr(), B, T, max_new, n_qh, n_kvh, D, dt,
+                                           D ** -0.5 if scale is None else scale, work.data_ptr(), out.data_ptr(),
+                                           _stream_address(stream)), "prefix_attention")
+
+
+def logits_adjust(logits, out, history=None, history_lens=None, prompt_lens=None, repetition=None, presence=None,
+                  frequency=None, bias_ids=None, bias=None, mask=None, stream=None):
+    """yskn_b200_logits_adjust: f32 logits [M][V] (dense rows, any row stride) -> out (may be
+    logits). history int32 [M][L] with history_lens and prompt_lens int32 [M]; repetition,
+    presence, frequency f32 [M]; bias_ids int32 and bias f32 [M][n] (dense); mask int32
+    [M][>= ceil(V / 32)], a set bit for an allowed token."""
+    M, V = logits.shape
+    _need(_dtype(logits) == _dtype(out) == DT_F32 and out.shape == logits.shape and logits.stride(1) == 1 and
+          out.stride(1) == 1 and _is_i32(history, history_lens, prompt_lens, bias_ids, mask),
+          "logits_adjust: f32 logits and output of one shape, int32 history, ids and mask expected")
+    _need(all(t is None or t.shape[0] == M for t in (history, history_lens, prompt_lens, repetition, presence,
+                                                     frequency, bias_ids, bias, mask)) and
+          all(t is None or _dtype(t) == DT_F32 for t in (repetition, presence, frequency, bias)) and
+          (bias_ids is None) == (bias is None) and
+          (bias is None or (bias.shape == bias_ids.shape and bias.is_contiguous() and bias_ids.is_contiguous())) and
+          (history is None or history.stride(1) == 1) and (mask is None or mask.stride(1) == 1),
+          "logits_adjust: a row of each argument for each row of logits expected")
+    check(lib().yskn_b200_logits_adjust(logits.data_ptr(), logits.stride(0), M, V, _address(history),
+                                        history.stride(0) if history is not None else 0,
+                                        history.shape[1] if history is not None else 0, _address(history_lens),
+                                        _address(prompt_lens), _address(repetition), _address(presence),
+                                        _address(frequency), _address(bias_ids), _address(bias),
+                                        bias.shape[1] if bias is not None else 0, _address(mask),
+                                        mask.stride(0) if mask is not None else 0, out.data_ptr(), out.stride(0),
+                                        _stream_address(stream)), "logits_adjust")
