@@ -27,13 +27,10 @@
 //  Every mbarrier wait is bounded: on timeout the CTA raises YSKN_ETIMEDOUT in
 //  the device error word, stops issuing work, waits (bounded) for its own copies
 //  and frees its TMEM before returning.
-#include <cuda.h>
-
 #include <algorithm>
 #include <mutex>
 
-#include "async.cuh"
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace yskn {
 
@@ -47,38 +44,6 @@ constexpr int GM_TMEM_BUFS = 4;  // group accumulators of 128 columns: the whole
 constexpr int GM_OUT_LD = 32 + 2;  // int64 per staged output row (16 bytes of padding)
 constexpr int GM_OUT_BYTES = GM_BM * GM_OUT_LD * 8;
 constexpr int GM_SMEM = GM_STAGES * GM_STAGE_BYTES + GM_OUT_BYTES + 1024 /*align*/ + 256 /*barriers*/;
-constexpr long long GM_WAIT_LIMIT = 4000000000ll;  // clock cycles (~2 s) before a wait gives up
-
-// ------------------------------------------------------------------ PTX helpers
-// (mbarrier basics in async.cuh)
-// Bounded wait; false if this CTA aborted (timeout here or elsewhere in the CTA).
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  const long long t0 = clock64();
-  while (!mbar_try_wait(bar, parity)) {
-    if (*abort_flag) return false;
-    if (clock64() - t0 > GM_WAIT_LIMIT) {
-      *abort_flag = 1;
-      return false;
-    }
-  }
-  return true;
-}
-
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
-          smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y)
-      : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// K-major operand in 128-byte-swizzled rows: 8-row atoms of 1024 bytes (SBO), version 1.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
-  return (uint64_t)((saddr >> 4) & 0x3fff) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
 
 // kind::i8: D s32, A s8, B s8, both K-major, N = 128, M = 128.
 constexpr uint32_t GM_IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(GM_BN >> 3) << 17) |
@@ -90,23 +55,6 @@ __device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t a, uint64_t b,
           d_tmem),
       "l"(a), "l"(b), "r"(GM_IDESC), "r"(accumulate));
 }
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
-}
-
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
 // -------------------------------------------------------------- predecode
 // Codes (streaming layout, pack.cu) -> dense int8 W [phys_pad8][Kc]. One warp per
 // tile (8 rows x 256 columns); lane (n, q) decodes its 32 steps into 64 bytes of
@@ -240,7 +188,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
         // Let the copies this thread started land before the CTA leaves.
         for (int k = std::max(0, c - GM_STAGES); k < c; ++k) {
           const long long t0 = clock64();
-          while (!mbar_try_wait(&full[k % GM_STAGES], (k / GM_STAGES) & 1) && clock64() - t0 < GM_WAIT_LIMIT) {
+          while (!mbar_try_wait(&full[k % GM_STAGES], (k / GM_STAGES) & 1) && clock64() - t0 < TC_WAIT_LIMIT) {
           }
         }
       }
@@ -278,7 +226,7 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
       // Every MMA this thread issued has completed before TMEM can be freed.
       umma_commit(drained);
       const long long t0 = clock64();
-      while (!mbar_try_wait(drained, 0) && clock64() - t0 < GM_WAIT_LIMIT) {
+      while (!mbar_try_wait(drained, 0) && clock64() - t0 < TC_WAIT_LIMIT) {
       }
     }
   } else {
@@ -361,23 +309,6 @@ __global__ void __launch_bounds__(GM_THREADS, 1)
 }
 
 // ------------------------------------------------------------------ host side
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiled encode_fn() {
-  static EncodeTiled fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiled>(p);
-  });
-  return fn;
-}
-
 // 2-D int8 matrix [rows][cols] (row stride = cols bytes), box 128 x 128, 128B swizzle.
 static int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols) {
   EncodeTiled fn = encode_fn();

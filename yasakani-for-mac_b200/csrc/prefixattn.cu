@@ -7,33 +7,119 @@
 //   s_j = scale * <q, k_j>, out = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s)
 //   out *= 1 / (1 + exp(-gate))  (with a gate), rounded once. A token that sees nothing gives 0.
 // Rows at or past lim are not read into any sum, whatever the cache holds there.
+//
+// The softmax over all rows is the join of softmaxes over parts: with a part's maximum m,
+// l = sum exp(s - m) and o = sum exp(s - m) v, parts join as sum exp(m - M) o / sum
+// exp(m - M) l, M the largest m. So the work is cut into items:
+//   prefix items  128 query rows (a row is a token and one of the G query heads of a KV head;
+//                 128 / G whole tokens of the batch, whichever request they belong to) against
+//                 the P prefix rows: the prefix is read once per 128 rows, not once per request;
+//   own items     up to 128 rows of one request against that request's own rows.
+// Items are cut along their key tiles (128 rows of the cache) so that every CTA gets the same
+// number of tiles: CTA c takes tiles [c per, (c + 1) per) of all items in order. A piece of an
+// item is a segment; its unnormalised (m, l, o) goes to the workspace in binary32, at place
+// item + c, which no two segments share, and prefix_combine_kernel joins a row's segments,
+// divides, gates and rounds. Everything is summed in a fixed order: the same call gives the same
+// bits. The lengths stay on the device: every CTA forms the tile counts' prefix sum itself.
+//
+// prefix_attention_kernel: persistent, one CTA per SM, 8 warps:
+//   warp 0  brings 16 KB slots of K and V (64 channels of 128 rows; 128 KB / D rows of all
+//           channels) through a ring with TMA, box by box, each box within one block;
+//   warp 1  issues tcgen05.mma: S = Q K^T (128 x 128, K = D) into one of two TMEM tiles, then
+//           O += P V (128 x D, K = 128) with P read from TMEM, S of the next tile before P V of
+//           this one, so that the tensor cores run while the softmax does;
+//   warp 2  brings Q (TMA; a box is the G heads of whole tokens);
+//   warps 4..7  one thread per row: S from TMEM, the running maximum, P = 2^(s c - m) (c = scale
+//           log2 e) rounded to the cache's type over S's place, the row sum in binary32 of the
+//           unrounded weights. The maximum in use may lag: o and l are rescaled only when a
+//           row's maximum has grown by more than 2^8, so that a weight is at most 256 and o is
+//           seldom touched; the join uses the maximum in use, which cancels.
+// A tile's rows past the last visible one: their scores are set to -inf before the maximum, P V
+// runs over the 16-row steps that hold a visible row, and warp 1 clears the rest of the last
+// step's V rows in shared memory (a zero weight does not silence a NaN).
+// Every mbarrier wait is bounded as in gemm.cu.
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 #include "paged.cuh"
+#include "tcgen05.cuh"
 
 namespace yskn {
 
+constexpr int PA_ROWS = 128;   // query rows per item (MMA M), TMEM lanes
+constexpr int PA_KEYS = 128;   // cache rows per tile
+constexpr int PA_SLOT = 16384;  // bytes per ring slot
+constexpr int PA_THREADS = 256;
+constexpr int PA_MAX_CTAS = 148;
+constexpr int PA_MAX_SLOTS = 12;
+
+// Ring slots of K or V per tile, ring length, V rows per slot of head size D.
+template <int D>
+struct PaShape {
+  static constexpr int PER_TILE = D / 64;
+  static constexpr int RING = D == 256 ? 10 : PA_MAX_SLOTS;
+  static constexpr int V_ROWS = PA_SLOT / (2 * D);
+  static constexpr int Q_BYTES = PER_TILE * PA_SLOT;
+  static constexpr int SMEM = Q_BYTES + RING * PA_SLOT + 1024 /*align*/;
+  static constexpr int S_COL = D < 128 ? 128 : D;  // TMEM columns: O at 0, S tiles at S_COL and S_COL + 128
+};
+
+// The workspace: sizes from the host's bounds alone, so that both sides agree.
+struct PaWork {
+  int64_t base, item, pre_ml, pre_o, own_ml, own_o, bytes;  // byte offsets
+  int own_rows;                                             // rows per own segment's place
+  int64_t own_items;                                        // own items that there is room for
+};
+inline PaWork pa_work(int tokens, int batch, int max_new, int n_qh, int n_kvh, int head) {
+  auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+  const int G = n_qh / n_kvh, tpt = PA_ROWS / G;  // tokens per item
+  const int64_t pre_items = ceil_div(tokens, tpt) * n_kvh;
+  // sum of ceil(n_i / tpt) over requests with n_i > 0: at most one more than n_i / tpt each
+  const int64_t own_items = (std::min(batch, tokens) + (int64_t)tokens / tpt) * n_kvh;
+  const int64_t pre = pre_items + PA_MAX_CTAS, own = own_items + PA_MAX_CTAS;
+  PaWork w{};
+  w.own_rows = G * std::min(tpt, max_new);
+  w.own_items = own_items;
+  w.base = 256;
+  w.item = w.base + up((int64_t)batch * 4);
+  w.pre_ml = w.item + up(own_items * 8);
+  w.pre_o = w.pre_ml + up(pre * PA_ROWS * 8);
+  w.own_ml = w.pre_o + up(pre * PA_ROWS * head * 4);
+  w.own_o = w.own_ml + up(own * w.own_rows * 8);
+  w.bytes = w.own_o + up(own * w.own_rows * head * 4);
+  return w;
+}
+
 struct PrefixAttnParams {
-  const uint16_t *q, *gate;
-  int64_t q_row, q_head, gate_row, gate_head;
-  const uint16_t *k_cache, *v_cache;
-  CacheStrides cache;
-  int n_blocks, block_size;
+  const uint16_t* gate;
+  int64_t gate_row, gate_head;
   const int32_t* prefix_blocks;
-  int prefix_len;
   const int32_t* tables;
   int64_t table_stride;
-  int table_width;
   const int32_t *lens, *starts;
-  int batch, tokens, max_new, n_qh, n_kvh;
-  float scale;
+  int n_blocks, block_size, prefix_len;
+  int own_limit;  // rows that a table row can name
+  int batch, tokens, max_new, n_kvh, G, tpt;
+  int pre_tiles, pre_qtiles, pre_items;
+  float c;  // |scale| log2 e
+  uint32_t negate_q;
+  long long* work_per;    // tiles per CTA of this call, for the join
+  int32_t* work_base;     // [batch] first own item of each request
+  long long* work_item;   // [own items] first tile of each own item
+  float2 *pre_ml, *own_ml;  // (m, l) per place and row
+  float *pre_o, *own_o;
+  int own_rows;
+  long long own_items;  // more of them (starts that do not ascend) is an error: nothing is computed
   uint16_t* out;  // [tokens][n_qh][D]
   unsigned* err;
 };
 
 // The last request whose first token is at or before t (requests without tokens share a
-// start with the next one), or the batch if t is past the last token.
+// start with the next one), or the batch if t is past the last token. One token for each
+// request is the common case: looked at first.
 __device__ __forceinline__ int request_of(const int32_t* starts, int batch, int t) {
+  if (t < batch && __ldg(starts + t) == t && __ldg(starts + t + 1) == t + 1) return t;
   if (t >= __ldg(starts + batch)) return batch;
   int lo = 0, hi = batch;
   while (hi - lo > 1) {
@@ -44,70 +130,635 @@ __device__ __forceinline__ int request_of(const int32_t* starts, int batch, int 
   return lo;
 }
 
-// One warp per (token, query head); lane l holds channels V l .. V l + V - 1.
-template <int DT, int V>
-__global__ void __launch_bounds__(256) prefix_attention_kernel(const __grid_constant__ PrefixAttnParams p) {
-  constexpr int D = 32 * V;
+// Request i: its first token, its tokens (0 if there are none, or not what the host bounded)
+// and its length.
+struct PaRequest {
+  int s0, n, len;
+};
+__device__ __forceinline__ PaRequest pa_request(const PrefixAttnParams& p, int i) {
+  PaRequest r;
+  r.s0 = __ldg(p.starts + i);
+  const int n = __ldg(p.starts + i + 1) - r.s0;
+  r.len = __ldg(p.lens + i);
+  r.n = n < 0 || n > p.max_new || r.s0 < 0 || r.s0 + n > p.tokens ? 0 : n;
+  return r;
+}
+// Own rows that the last of the request's first `upto` tokens sees.
+__device__ __forceinline__ int pa_visible(const PrefixAttnParams& p, const PaRequest& r, int upto) {
+  return min(max(r.len - r.n + upto - p.prefix_len, 0), p.own_limit);
+}
+__device__ __forceinline__ int pa_own_tiles(const PrefixAttnParams& p, const PaRequest& r, int qt) {
+  return (pa_visible(p, r, min(r.n, (qt + 1) * p.tpt)) + PA_KEYS - 1) / PA_KEYS;
+}
+__device__ __forceinline__ int pa_qtiles(const PrefixAttnParams& p, const PaRequest& r) {
+  return (r.n + p.tpt - 1) / p.tpt;
+}
+
+struct PaSegment {
+  bool prefix;
+  int kvh, tok0, ntok;  // KV head, first token and whole tokens
+  int req;              // own items: the request
+  int key0, key1;       // key tiles [key0, key1)
+  int keys;             // rows on this axis that any of its tokens sees
+  int first;            // own items: rows that token tok0 sees
+  int64_t place;        // of its partial result
+};
+
+// Where a CTA's tiles begin, found by the whole CTA.
+struct PaStart {
+  long long left;  // tiles of this CTA
+  int pre_item, k0;
+  int req, item;       // own items: request and the items before it
+  long long skip;      // tiles of the request before this CTA's first
+  long long tile;      // index of the first tile
+};
+
+// The CTA's segments in order; every lane of a warp walks alike.
+struct PaWalk {
+  const PrefixAttnParams& p;
+  long long left, tile;
+  int pre_item, k0, req, item, kvh, qt;
+  PaRequest r;
+  int nq;
+  bool loaded;
+  __device__ PaWalk(const PrefixAttnParams& p_, const PaStart& s)
+      : p(p_), left(s.left), tile(s.tile), pre_item(s.pre_item), k0(s.k0), req(s.req), item(s.item), kvh(0), qt(0),
+        r{}, nq(0), loaded(false) {
+    if (s.skip > 0) {
+      load();
+      long long skip = s.skip, head = 0;
+      for (int q = 0; q < nq; ++q) head += pa_own_tiles(p, r, q);
+      kvh = (int)(skip / head);
+      skip -= kvh * head;
+      for (;; ++qt) {
+        const int kt = pa_own_tiles(p, r, qt);
+        if (skip < kt) break;
+        skip -= kt;
+      }
+      k0 = (int)skip;
+    }
+  }
+  __device__ void load() {
+    r = pa_request(p, req);
+    nq = pa_qtiles(p, r);
+    loaded = true;
+  }
+  // The next segment; tile is then the index of its first tile plus its length.
+  __device__ bool next(PaSegment& s) {
+    if (left <= 0) return false;
+    if (pre_item < p.pre_items) {
+      s.prefix = true;
+      s.kvh = pre_item / p.pre_qtiles;
+      s.tok0 = (pre_item - s.kvh * p.pre_qtiles) * p.tpt;
+      s.ntok = min(p.tpt, p.tokens - s.tok0);
+      s.req = 0;
+      s.keys = p.prefix_len;
+      s.first = 0;
+      take(s, p.pre_tiles, pre_item);
+      ++pre_item;
+      return true;
+    }
+    while (req < p.batch) {
+      if (!loaded) load();
+      for (; kvh < p.n_kvh; ++kvh, qt = 0)
+        for (; qt < nq; ++qt) {
+          const int kt = pa_own_tiles(p, r, qt);
+          if (kt == 0) continue;
+          s.prefix = false;
+          s.kvh = kvh;
+          s.tok0 = r.s0 + qt * p.tpt;
+          s.ntok = min(p.tpt, r.n - qt * p.tpt);
+          s.req = req;
+          s.keys = pa_visible(p, r, qt * p.tpt + s.ntok);
+          s.first = r.len - r.n + qt * p.tpt + 1 - p.prefix_len;
+          take(s, kt, item + kvh * nq + qt);
+          ++qt;
+          return true;
+        }
+      item += p.n_kvh * nq;
+      ++req;
+      kvh = qt = 0;
+      loaded = false;
+    }
+    return false;
+  }
+  __device__ void take(PaSegment& s, int tiles, int it) {
+    const int n = (int)min((long long)(tiles - k0), left);
+    s.key0 = k0;
+    s.key1 = k0 + n;
+    s.place = (int64_t)it + blockIdx.x;
+    left -= n;
+    tile += n;
+    k0 = 0;
+  }
+};
+
+// B operand whose N runs along the 128-byte swizzled rows (V: rows are keys, MMA K): 64-channel
+// columns `stride` bytes apart, 8-key groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr, uint32_t stride) {
+  return (uint64_t)((saddr >> 4) & 0x3fff) | ((uint64_t)(stride >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// kind::f16 with f32 accumulators, M = 128: type of both operands, N, B's major axis, A's sign.
+__device__ __forceinline__ uint32_t pa_idesc(int dt, int n, uint32_t b_mn, uint32_t negate_a) {
+  const uint32_t t = dt == YSKN_DT_BF16 ? 1u : 0u;
+  return (1u << 4) | (t << 7) | (t << 10) | (negate_a << 13) | (b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(PA_ROWS >> 4) << 24);
+}
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::
+          "r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::
+          "r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A bounded wait of a whole warp: all lanes go on or none does.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+
+template <int D, int DT>
+__global__ void __launch_bounds__(PA_THREADS, 1)
+    prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q_pre, const __grid_constant__ CUtensorMap map_q_own,
+                            const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                            const __grid_constant__ PrefixAttnParams p) {
+  using Shape = PaShape<D>;
+  constexpr int RING = Shape::RING, PT = Shape::PER_TILE, VR = Shape::V_ROWS;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;                    // [D / 64][128 rows][128 B]
+  uint8_t* ring = smem + Shape::Q_BYTES;  // [RING][16 KB]
+  __shared__ uint64_t full[RING], empty[RING];  // ring slots: landed, read
+  __shared__ uint64_t q_full, q_empty;
+  __shared__ uint64_t s_full[2], p_full[2], pv_done[2];  // by tile parity
+  __shared__ uint64_t o_free, drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  __shared__ long long s_sum[PA_THREADS / 32][2];
+  __shared__ PaStart s_start;
+  volatile int* abort_flag = &abort_word;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int s = 0; s < RING; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+    mbar_init(&q_full, 1), mbar_init(&q_empty, 1);
+    for (int b = 0; b < 2; ++b) mbar_init(&s_full[b], 1), mbar_init(&p_full[b], 4), mbar_init(&pv_done[b], 1);
+    mbar_init(&o_free, 4), mbar_init(&drained, 1);
+    abort_word = 0;
+    mbar_init_fence();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 3) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
   pdl_begin();
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (item >= (int64_t)p.tokens * p.n_qh) return;
-  const int t = (int)(item / p.n_qh), h = (int)(item - (int64_t)t * p.n_qh), kvh = h / (p.n_qh / p.n_kvh);
-  const int i = request_of(p.starts, p.batch, t);
-  int lim = 0;
-  if (i < p.batch) {
-    const int s0 = __ldg(p.starts + i), n = __ldg(p.starts + i + 1) - s0;
-    lim = max(0, __ldg(p.lens + i) - n + (t - s0) + 1);
-    if (n > p.max_new) {
-      if (lane == 0) raise_device_error(p.err, DERR_RANGE);
-      lim = 0;
+
+  // Tile counts of all requests and where this CTA begins.
+  {
+    const int per = (p.batch + PA_THREADS - 1) / PA_THREADS;
+    const int i0 = min(p.batch, tid * per), i1 = min(p.batch, i0 + per);
+    long long tiles = 0, items = 0;
+    for (int i = i0; i < i1; ++i) {
+      const PaRequest r = pa_request(p, i);
+      const int nq = pa_qtiles(p, r);
+      long long t = 0;
+      for (int q = 0; q < nq; ++q) t += pa_own_tiles(p, r, q);
+      tiles += t * p.n_kvh;
+      items += nq * p.n_kvh;
+      if (blockIdx.x == 0 && (__ldg(p.starts + i + 1) - r.s0 != r.n)) raise_device_error(p.err, DERR_RANGE);
     }
-    lim = min((int64_t)lim, (int64_t)p.prefix_len + (int64_t)p.table_width * p.block_size);
-  }
-  float q[V], o[V];
+    long long ti = tiles, it = items;
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    q[j] = Elem<DT>::to_float(p.q[t * p.q_row + h * p.q_head + lane * V + j]) * p.scale;
-    o[j] = 0.0f;
-  }
-  float top = -INFINITY, den = 0.0f;
-  for (int r = 0; r < lim; ++r) {
-    const bool shared = r < p.prefix_len;
-    const int at = shared ? r : r - p.prefix_len;
-    const int block = shared ? __ldg(p.prefix_blocks + at / p.block_size)
-                             : __ldg(p.tables + i * p.table_stride + at / p.block_size);
-    if ((unsigned)block >= (unsigned)p.n_blocks) {
-      if (lane == 0) raise_device_error(p.err, DERR_RANGE);
-      continue;
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long a = __shfl_up_sync(0xffffffffu, ti, off), b = __shfl_up_sync(0xffffffffu, it, off);
+      if (lane >= off) ti += a, it += b;
     }
-    const int64_t row = block * p.cache.block + (at % p.block_size) * p.cache.token + kvh * p.cache.head + lane * V;
-    float s = 0.0f;
-#pragma unroll
-    for (int j = 0; j < V; ++j) s = fmaf(q[j], Elem<DT>::to_float(p.k_cache[row + j]), s);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    const float next = fmaxf(top, s), keep = top == -INFINITY ? 0.0f : expf(top - next), w = expf(s - next);
-    den = fmaf(den, keep, w);
-#pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = fmaf(o[j], keep, w * Elem<DT>::to_float(p.v_cache[row + j]));
-    top = next;
+    if (lane == 31) s_sum[warp][0] = ti, s_sum[warp][1] = it;
+    __syncthreads();
+    long long before = ti - tiles, items_before = it - items, total = 0, total_items = 0;
+    for (int w = 0; w < PA_THREADS / 32; ++w) {
+      if (w < warp) before += s_sum[w][0], items_before += s_sum[w][1];
+      total += s_sum[w][0];
+      total_items += s_sum[w][1];
+    }
+    const bool sound = total_items <= p.own_items;
+    const long long pre = (long long)p.pre_items * p.pre_tiles, all = sound ? pre + total : 0;
+    const long long share = sound ? max(1ll, (all + gridDim.x - 1) / gridDim.x) : 0;
+    const long long t0 = min(all, blockIdx.x * share), t1 = min(all, t0 + share);
+    if (tid == 0) {
+      s_start = {t1 - t0, p.pre_items, 0, 0, 0, 0, t0};
+      if (t0 < pre) {
+        s_start.pre_item = (int)(t0 / p.pre_tiles);
+        s_start.k0 = (int)(t0 - (long long)s_start.pre_item * p.pre_tiles);
+      }
+      if (blockIdx.x == 0) {
+        *p.work_per = share;
+        if (!sound) raise_device_error(p.err, DERR_RANGE);
+      }
+    }
+    __syncthreads();
+    const long long at = t0 - pre;  // this CTA's first own tile
+    if (sound && ((at >= 0 && at >= before && at < before + tiles) || blockIdx.x == 0)) {
+      long long b = before;
+      int item = (int)items_before;
+      for (int i = i0; i < i1; ++i) {
+        const PaRequest r = pa_request(p, i);
+        const int nq = pa_qtiles(p, r);
+        long long t = 0;
+        for (int q = 0; q < nq; ++q) t += pa_own_tiles(p, r, q);
+        t *= p.n_kvh;
+        if (at >= b && at < b + t) s_start.req = i, s_start.item = item, s_start.skip = at - b;
+        if (blockIdx.x == 0) p.work_base[i] = item;
+        b += t;
+        item += nq * p.n_kvh;
+      }
+    }
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  PaWalk walk(p, s_start);
+  PaSegment seg;
+
+  if (warp == 0) {
+    // ---- K and V through the ring, in the order in which warp 1 uses them
+    int c = 0;
+    bool ok = true;
+    const int pages = PA_KEYS / p.block_size, box_v = min(p.block_size, VR);
+    while (ok && walk.next(seg)) {
+      const int32_t* table = seg.prefix ? p.prefix_blocks : p.tables + (int64_t)seg.req * p.table_stride;
+      const int page_end = (seg.keys + p.block_size - 1) / p.block_size;
+      auto block_of = [&](int kt) {  // lane l: the block of page l of tile kt
+        const int at = kt * pages + lane;
+        int b = 0;
+        if (lane < pages && kt < seg.key1 && at < page_end) {
+          b = __ldg(table + at);
+          if ((unsigned)b >= (unsigned)p.n_blocks) raise_device_error(p.err, DERR_RANGE);  // the copy gives zeros
+        }
+        return b;
+      };
+      auto slot = [&](uint32_t bytes) -> uint8_t* {
+        const int s = c % RING, u = c / RING;
+        if (u > 0 && !warp_wait(&empty[s], (u - 1) & 1, abort_flag)) return nullptr;
+        if (lane == 0) mbar_expect_tx(&full[s], bytes);
+        __syncwarp();
+        return ring + s * PA_SLOT;
+      };
+      auto put_k = [&](int kt, int block) {
+        const int nk = min(PA_KEYS, seg.keys - kt * PA_KEYS), n = (nk + p.block_size - 1) / p.block_size;
+        for (int d = 0; d < PT; ++d, ++c) {
+          uint8_t* to = slot(n * p.block_size * 128);
+          if (!to) return false;
+          if (lane < n) tma_load_4d(to + lane * p.block_size * 128, &map_k, &full[c % RING], d * 64, 0, seg.kvh, block);
+        }
+        return true;
+      };
+      auto put_v = [&](int kt, int block) {
+        const int nk = min(PA_KEYS, seg.keys - kt * PA_KEYS);
+        for (int v = 0; v * VR < nk; ++v, ++c) {
+          const int n = (min(VR, nk - v * VR) + box_v - 1) / box_v;  // boxes along the rows
+          uint8_t* to = slot(n * box_v * 128 * PT);
+          if (!to) return false;
+          const int rg = lane / PT, sub = lane % PT, key = v * VR + rg * box_v;
+          const int b = __shfl_sync(0xffffffffu, block, min(key / p.block_size, 31));
+          if (rg < n)
+            tma_load_4d(to + sub * VR * 128 + rg * box_v * 128, &map_v, &full[c % RING], sub * 64,
+                        key % p.block_size, seg.kvh, b);
+        }
+        return true;
+      };
+      int cur = block_of(seg.key0), nxt = block_of(seg.key0 + 1);
+      ok = put_k(seg.key0, cur);
+      for (int kt = seg.key0; ok && kt < seg.key1; ++kt) {
+        const int after = block_of(kt + 2);
+        if (kt + 1 < seg.key1) ok = put_k(kt + 1, nxt);
+        ok = ok && put_v(kt, cur);
+        cur = nxt;
+        nxt = after;
+      }
+    }
+    if (!ok && lane == 0)  // let the copies that this warp started land before the CTA leaves
+      for (int k = max(0, c - RING); k < c; ++k) {
+        const long long t0 = clock64();
+        while (!mbar_try_wait(&full[k % RING], (k / RING) & 1) && clock64() - t0 < TC_WAIT_LIMIT) {
+        }
+      }
+  } else if (warp == 1) {
+    // ---- MMAs
+    const uint32_t id_qk = pa_idesc(DT, PA_KEYS, 0, p.negate_q), id_pv = pa_idesc(DT, D, 1, 0);
+    int c = 0, g = 0, n_seg = 0;  // slots used, tiles issued, segments
+    bool ok = true;
+    auto qk = [&](int tile) {  // S of the CTA's tile number `tile`
+      const uint32_t d = tmem + Shape::S_COL + (tile & 1) * PA_KEYS;
+      for (int ch = 0; ch < PT; ++ch, ++c) {
+        const int s = c % RING;
+        if (!warp_wait(&full[s], (c / RING) & 1, abort_flag)) return false;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t a = smem_u32(sQ + ch * PA_SLOT), b = smem_u32(ring + s * PA_SLOT);
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    float y = den > 0.0f || den != den ? o[j] / den : 0.0f;
-    if (p.gate) y = y / (1.0f + expf(-Elem<DT>::to_float(p.gate[t * p.gate_row + h * p.gate_head + lane * V + j])));
-    p.out[((int64_t)t * p.n_qh + h) * D + lane * V + j] = Elem<DT>::from_float(y);
+          for (int k = 0; k < 4; ++k)
+            umma_f16_ss(d, sw128_desc(a + k * 32), sw128_desc(b + k * 32), id_qk, ch > 0 || k > 0);
+          umma_commit(&empty[s]);
+        }
+      }
+      if (lane == 0) umma_commit(&s_full[tile & 1]);
+      return true;
+    };
+    while (ok && walk.next(seg)) {
+      ok = warp_wait(&q_full, n_seg & 1, abort_flag);
+      if (!ok) break;
+      const int n = seg.key1 - seg.key0;
+      ok = qk(g);
+      for (int j = 0; ok && j < n; ++j, ++g) {
+        if (j + 1 < n) ok = qk(g + 1);
+        if (ok && j == max(0, n - 2) && lane == 0) umma_commit(&q_empty);  // after the segment's last S
+        if (ok && j == 0 && n_seg > 0) ok = warp_wait(&o_free, (n_seg - 1) & 1, abort_flag);
+        if (!ok || !(ok = warp_wait(&p_full[g & 1], (g >> 1) & 1, abort_flag))) break;
+        tc_fence_after();
+        const int nk = min(PA_KEYS, seg.keys - (seg.key0 + j) * PA_KEYS);
+        const uint32_t pt = tmem + Shape::S_COL + (g & 1) * PA_KEYS;
+        for (int v = 0; v * VR < nk; ++v, ++c) {
+          const int s = c % RING, rows = min(VR, nk - v * VR), steps = (rows + 15) / 16;
+          if (!(ok = warp_wait(&full[s], (c / RING) & 1, abort_flag))) break;
+          uint8_t* base = ring + s * PA_SLOT;
+          if (rows & 15) {  // rows up to the end of the last step: zeros
+            const int n16 = (steps * 16 - rows) * 8;
+            for (int x = lane; x < n16 * PT; x += 32) {
+              const int sub = x / n16, y = x - sub * n16;
+              *reinterpret_cast<uint4*>(base + sub * VR * 128 + rows * 128 + y * 16) = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t b = smem_u32(base);
+            for (int k = 0; k < steps; ++k)
+              umma_f16_ts(tmem, pt + (v * VR + k * 16) / 2, sw128_desc_mn(b + k * 2048, VR * 128), id_pv,
+                          j > 0 || v > 0 || k > 0);
+            umma_commit(&empty[s]);
+          }
+        }
+        if (ok && lane == 0) umma_commit(&pv_done[g & 1]);
+      }
+      ++n_seg;
+    }
+    if (lane == 0) {  // every MMA of this CTA has completed before its TMEM is freed
+      umma_commit(&drained);
+      const long long t0 = clock64();
+      while (!mbar_try_wait(&drained, 0) && clock64() - t0 < TC_WAIT_LIMIT) {
+      }
+    }
+  } else if (warp == 2) {
+    // ---- Q
+    if (lane == 0) {
+      int n_seg = 0;
+      bool ok = true;
+      for (; walk.next(seg); ++n_seg) {
+        if (n_seg > 0 && !(ok = mbar_wait(&q_empty, (n_seg - 1) & 1, abort_flag))) break;
+        const int box = seg.prefix ? p.tpt : min(p.tpt, p.max_new);
+        mbar_expect_tx(&q_full, (uint32_t)(box * p.G * 128 * PT));
+        for (int d = 0; d < PT; ++d)
+          tma_load_3d(sQ + d * PA_SLOT, seg.prefix ? &map_q_pre : &map_q_own, &q_full, d * 64, seg.kvh * p.G, seg.tok0);
+      }
+      if (!ok && n_seg > 0) {
+        const long long t0 = clock64();
+        while (!mbar_try_wait(&q_full, (n_seg - 1) & 1) && clock64() - t0 < TC_WAIT_LIMIT) {
+        }
+      }
+    }
+  } else if (warp >= 4) {
+    // ---- softmax, one row per thread, then the segment's result
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const float c = p.c;
+    int g = 0;
+    bool ok = true;
+    while (ok && walk.next(seg)) {
+      const int tl = row / p.G;  // token of the tile
+      const bool valid = tl < seg.ntok;
+      int lim = 0;  // rows on this axis that the row sees
+      if (valid) {
+        if (seg.prefix) {
+          const int i = request_of(p.starts, p.batch, seg.tok0 + tl);
+          if (i < p.batch) {
+            const PaRequest r = pa_request(p, i);
+            lim = min(max(r.len - r.n + (seg.tok0 + tl - r.s0) + 1, 0), p.prefix_len);
+          }
+        } else {
+          lim = min(max(seg.first + tl, 0), seg.keys);
+        }
+      }
+      const bool live = __any_sync(0xffffffffu, valid);  // a warp without rows only keeps the barriers going
+      const int least = __reduce_min_sync(0xffffffffu, valid ? lim : INT32_MAX);
+      float m = -INFINITY, l = 0.0f;
+      for (int kt = seg.key0; kt < seg.key1; ++kt, ++g) {
+        const int b = g & 1;
+        if (!(ok = warp_wait(&s_full[b], (g >> 1) & 1, abort_flag))) break;
+        if (live) {
+          tc_fence_after();
+          const uint32_t at = tmem + lanes + Shape::S_COL + b * PA_KEYS;
+          uint32_t s[4][32];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) tmem_ld32(at + x * 32, s[x]);
+          tmem_ld_wait();
+          const int see = lim - kt * PA_KEYS;
+          if (least < (kt + 1) * PA_KEYS) {
+#pragma unroll
+            for (int x = 0; x < 128; ++x)
+              if (x >= see) s[x >> 5][x & 31] = 0xff800000u;  // -inf
+          }
+          float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int x = 0; x < 128; ++x) t[x & 3] = fmaxf(t[x & 3], __uint_as_float(s[x >> 5][x & 31]));
+          const float top = __fmul_rn(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), c);
+          if (m == -INFINITY) m = top;  // nothing seen before: o and l are zero
+          const bool grown = top > m + 8.0f;
+          if (__any_sync(0xffffffffu, grown)) {
+            // o is complete up to the tile before; then scale it
+            if (!(ok = warp_wait(&pv_done[b ^ 1], ((g - 1) >> 1) & 1, abort_flag))) break;
+            tc_fence_after();
+            const float f = grown ? exp2_approx(m - top) : 1.0f;
+            for (int x = 0; x < D; x += 32) {
+              uint32_t o[32];
+              tmem_ld32(tmem + lanes + x, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+              tmem_st32(tmem + lanes + x, o);
+            }
+            l *= f;
+            if (grown) m = top;
+          }
+          const float base = m == -INFINITY ? 0.0f : m;
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t w[32];
+#pragma unroll
+            for (int x = 0; x < 32; ++x) {
+              const int e = h * 64 + 2 * x;
+              const float a = exp2_approx(fmaf(__uint_as_float(s[e >> 5][e & 31]), c, -base));
+              const float d = exp2_approx(fmaf(__uint_as_float(s[e >> 5][(e + 1) & 31]), c, -base));
+              sum[x & 1] += a;
+              sum[2 + (x & 1)] += d;
+              w[x] = Elem<DT>::pack(a, d);
+            }
+            tmem_st32(at + h * 32, w);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_st_wait();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[b]);
+      }
+      if (!ok || !(ok = warp_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag))) break;
+      if (live) {
+        tc_fence_after();
+        const int rows = seg.prefix ? PA_ROWS : p.own_rows;
+        float2* ml = (seg.prefix ? p.pre_ml : p.own_ml) + seg.place * rows + row;
+        float* o = (seg.prefix ? p.pre_o : p.own_o) + (seg.place * rows + row) * D;
+        if (valid) *ml = make_float2(m, l);
+        for (int x = 0; x < D; x += 32) {
+          uint32_t v[32];
+          tmem_ld32(tmem + lanes + x, v);
+          tmem_ld_wait();
+          if (valid) {
+#pragma unroll
+            for (int y = 0; y < 32; y += 4)
+              *reinterpret_cast<uint4*>(o + x + y) = make_uint4(v[y], v[y + 1], v[y + 2], v[y + 3]);
+          }
+        }
+        tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_free);
+      if (!seg.prefix && seg.key0 == 0 && row == 0)
+        p.work_item[seg.place - blockIdx.x] = walk.tile - (seg.key1 - seg.key0);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *abort_flag) raise_device_error(p.err, DERR_TIMEOUT);
+  if (warp == 3) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   }
 }
 
-template <int DT>
-static cudaError_t launch_prefix_attention(const PrefixAttnParams& p, int head, cudaStream_t st) {
-  const unsigned grid = (unsigned)ceil_div((int64_t)p.tokens * p.n_qh, 8);
-  switch (head) {
-    case 64: return launch_pdl(prefix_attention_kernel<DT, 2>, grid, 256, 0, st, p);
-    case 128: return launch_pdl(prefix_attention_kernel<DT, 4>, grid, 256, 0, st, p);
-    default: return launch_pdl(prefix_attention_kernel<DT, 8>, grid, 256, 0, st, p);
+// Joins the segments of each row: one warp per (token, query head), lane l the channels
+// V l .. V l + V - 1.
+template <int D, int DT>
+__global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_constant__ PrefixAttnParams p) {
+  constexpr int V = D / 32;
+  pdl_begin();
+  const int lane = threadIdx.x & 31, n_qh = p.n_kvh * p.G;
+  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (item >= (int64_t)p.tokens * n_qh) return;
+  const int t = (int)(item / n_qh), h = (int)(item - (int64_t)t * n_qh), kvh = h / p.G, gh = h - kvh * p.G;
+  float o[V], den = 0.0f, top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < V; ++j) o[j] = 0.0f;
+  const int i = request_of(p.starts, p.batch, t);
+  const long long per = *p.work_per;
+  const PaRequest r = i < p.batch ? pa_request(p, i) : PaRequest{};
+  if (per > 0 && t >= r.s0 && t < r.s0 + r.n) {
+    // places of the row's segments: n_pre of its prefix item, then n_own of its own item
+    int n_pre = 0, n_own = 0;
+    int64_t pre0 = 0, own0 = 0;
+    if (p.pre_tiles > 0) {
+      const int qt = t / p.tpt, it = kvh * p.pre_qtiles + qt, row = (t - qt * p.tpt) * p.G + gh;
+      const long long b = (long long)it * p.pre_tiles, c0 = b / per, c1 = (b + p.pre_tiles - 1) / per;
+      n_pre = (int)(c1 - c0) + 1;
+      pre0 = (it + c0) * PA_ROWS + row;
+    }
+    const int own_qt = (t - r.s0) / p.tpt, own_row = (t - r.s0 - own_qt * p.tpt) * p.G + gh;
+    const int kt = pa_own_tiles(p, r, own_qt);
+    if (kt > 0) {
+      const int64_t it = (int64_t)p.work_base[i] + kvh * pa_qtiles(p, r) + own_qt;
+      const long long b = p.work_item[it], c0 = b / per, c1 = (b + kt - 1) / per;
+      n_own = (int)(c1 - c0) + 1;
+      own0 = (it + c0) * p.own_rows + own_row;
+    }
+    for (int x = lane; x < n_pre + n_own; x += 32) {
+      const float2 v = x < n_pre ? p.pre_ml[pre0 + (int64_t)x * PA_ROWS] : p.own_ml[own0 + (int64_t)(x - n_pre) * p.own_rows];
+      top = fmaxf(top, v.x);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+#pragma unroll 4
+    for (int x = 0; x < n_pre + n_own; ++x) {
+      const int64_t at = x < n_pre ? pre0 + (int64_t)x * PA_ROWS : own0 + (int64_t)(x - n_pre) * p.own_rows;
+      const float2 v = (x < n_pre ? p.pre_ml : p.own_ml)[at];
+      const float* src = (x < n_pre ? p.pre_o : p.own_o) + at * D + lane * V;
+      const float w = v.x == -INFINITY ? 0.0f : exp2f(v.x - top);
+      den = fmaf(v.y, w, den);
+#pragma unroll
+      for (int j = 0; j < V; j += 2) {
+        const float2 y = *reinterpret_cast<const float2*>(src + j);
+        o[j] = fmaf(y.x, w, o[j]);
+        o[j + 1] = fmaf(y.y, w, o[j + 1]);
+      }
+    }
   }
+  const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+#pragma unroll
+  for (int j = 0; j < V; ++j) o[j] *= inv;
+  if (p.gate) {
+    const uint16_t* gate = p.gate + t * p.gate_row + h * p.gate_head + lane * V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = o[j] / (1.0f + expf(-Elem<DT>::to_float(gate[j])));
+  }
+  uint32_t* out = reinterpret_cast<uint32_t*>(p.out + item * D + lane * V);
+#pragma unroll
+  for (int j = 0; j < V; j += 2) out[j / 2] = Elem<DT>::pack(o[j], o[j + 1]);
+}
+
+template <int D, int DT>
+static int launch_prefix_attention(const CUtensorMap (&maps)[4], const PrefixAttnParams& p, int grid, cudaStream_t st) {
+  static SmemOptIn opt_in;
+  if (cudaError_t e = opt_in(prefix_attention_kernel<D, DT>, PaShape<D>::SMEM))
+    return cuda_fail(e, "prefix_attention_kernel attributes");
+  if (cudaError_t e = launch_pdl(prefix_attention_kernel<D, DT>, grid, PA_THREADS, PaShape<D>::SMEM, st, maps[0],
+                                 maps[1], maps[2], maps[3], p))
+    return cuda_fail(e, "prefix_attention_kernel");
+  const int64_t rows = (int64_t)p.tokens * p.n_kvh * p.G;
+  return cuda_fail(launch_pdl(prefix_combine_kernel<D, DT>, (unsigned)ceil_div(rows, 8), 256, 0, st, p),
+                   "prefix_combine_kernel");
+}
+
+// 16-bit tensor of 3 or 4 axes with 128B-swizzled boxes of 64 channels. Strides in elements.
+static int paged_map(CUtensorMap* map, const void* base, int dt, int rank, const int64_t* dims, const int64_t* strides,
+                     const int* box) {
+  EncodeTiled fn = encode_fn();
+  if (!fn) return fail(YSKN_ECUDA, "cuTensorMapEncodeTiled is not available");
+  cuuint64_t d[4], s[3];
+  cuuint32_t b[4], one[4] = {1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) d[i] = (cuuint64_t)dims[i], b[i] = (cuuint32_t)box[i];
+  for (int i = 0; i + 1 < rank; ++i) s[i] = (cuuint64_t)(dims[i + 1] == 1 ? dims[0] : strides[i]) * 2;
+  const CUresult r = fn(map, dt == YSKN_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                        rank, const_cast<void*>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(YSKN_EINVAL, "prefix_attention: strides that a tensor map cannot hold");
+  return YSKN_OK;
 }
 
 }  // namespace yskn
@@ -116,10 +767,10 @@ using namespace yskn;
 
 extern "C" YSKN_B200_API int64_t yskn_b200_prefix_attention_work_bytes(int tokens, int batch, int max_new, int n_qh,
                                                                       int n_kvh, int head) {
-  if (tokens < 1 || batch < 1 || max_new < 1 || n_qh < 1 || n_kvh < 1 || n_qh % n_kvh ||
+  if (tokens < 1 || batch < 1 || max_new < 1 || n_qh < 1 || n_kvh < 1 || n_qh % n_kvh || n_qh / n_kvh > PA_ROWS ||
       (head != 64 && head != 128 && head != 256))
     return -1;
-  return 256;
+  return pa_work(tokens, batch, max_new, n_qh, n_kvh, head).bytes;
 }
 
 extern "C" YSKN_B200_API int yskn_b200_prefix_attention(
@@ -147,19 +798,53 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(
       !aligned16(d_out) || (q_row | q_head | block_stride | token_stride | head_stride) % 8 ||
       (d_gate && (gate_row | gate_head) % 8))
     return fail(YSKN_EINVAL, "prefix_attention: pointers and strides are multiples of 16 bytes");
+  const int G = n_qh / n_kvh, tpt = PA_ROWS / G;
   PrefixAttnParams p{};
-  p.q = reinterpret_cast<const uint16_t*>(d_q), p.gate = reinterpret_cast<const uint16_t*>(d_gate);
-  p.q_row = q_row, p.q_head = q_head, p.gate_row = gate_row, p.gate_head = gate_head;
-  p.k_cache = reinterpret_cast<const uint16_t*>(d_k_cache), p.v_cache = reinterpret_cast<const uint16_t*>(d_v_cache);
-  p.cache = {block_stride, token_stride, head_stride};
-  p.n_blocks = n_blocks, p.block_size = block_size;
-  p.prefix_blocks = d_prefix_blocks, p.prefix_len = prefix_len;
-  p.tables = d_block_tables, p.table_stride = table_stride, p.table_width = table_width;
-  p.lens = d_lens, p.starts = d_starts, p.batch = batch, p.tokens = tokens, p.max_new = max_new;
-  p.n_qh = n_qh, p.n_kvh = n_kvh, p.scale = scale;
+  p.gate = reinterpret_cast<const uint16_t*>(d_gate);
+  p.gate_row = gate_row, p.gate_head = gate_head;
+  p.prefix_blocks = d_prefix_blocks;
+  p.tables = d_block_tables, p.table_stride = table_stride;
+  p.lens = d_lens, p.starts = d_starts;
+  p.n_blocks = n_blocks, p.block_size = block_size, p.prefix_len = prefix_len;
+  p.own_limit = (int)std::min<int64_t>((int64_t)table_width * block_size, INT32_MAX - PA_KEYS);
+  p.batch = batch, p.tokens = tokens, p.max_new = max_new, p.n_kvh = n_kvh, p.G = G, p.tpt = tpt;
+  p.pre_tiles = (int)ceil_div(prefix_len, PA_KEYS), p.pre_qtiles = (int)ceil_div(tokens, tpt);
+  const int64_t items = (int64_t)p.pre_qtiles * n_kvh;
+  if (items > INT32_MAX / 2) return fail(YSKN_EINVAL, "prefix_attention: too many rows");
+  p.pre_items = prefix_len > 0 ? (int)items : 0;
+  // a scale of zero keeps its meaning (equal weights) with a factor that leaves -inf alone
+  p.c = std::max(std::fabs(scale) * 1.4426950408889634f, 1e-30f);
+  p.negate_q = scale < 0.0f;
+  const PaWork w = pa_work(tokens, batch, max_new, n_qh, n_kvh, head);
+  uint8_t* work = reinterpret_cast<uint8_t*>(d_work);
+  p.work_per = reinterpret_cast<long long*>(work);
+  p.work_base = reinterpret_cast<int32_t*>(work + w.base);
+  p.work_item = reinterpret_cast<long long*>(work + w.item);
+  p.pre_ml = reinterpret_cast<float2*>(work + w.pre_ml), p.pre_o = reinterpret_cast<float*>(work + w.pre_o);
+  p.own_ml = reinterpret_cast<float2*>(work + w.own_ml), p.own_o = reinterpret_cast<float*>(work + w.own_o);
+  p.own_rows = w.own_rows, p.own_items = w.own_items;
   p.out = reinterpret_cast<uint16_t*>(d_out), p.err = device_error_word();
+  const int v_rows = PA_SLOT / (2 * head);
+  const int64_t q_dims[3] = {head, n_qh, tokens}, q_strides[2] = {q_head, q_row};
+  const int64_t c_dims[4] = {head, block_size, n_kvh, n_blocks}, c_strides[3] = {token_stride, head_stride, block_stride};
+  const int box_pre[3] = {64, G, tpt}, box_own[3] = {64, G, std::min(tpt, max_new)};
+  const int box_k[4] = {64, block_size, 1, 1}, box_v[4] = {64, std::min(block_size, v_rows), 1, 1};
+  CUtensorMap maps[4];
+  if (int rc = paged_map(&maps[0], d_q, dtype, 3, q_dims, q_strides, box_pre)) return rc;
+  if (int rc = paged_map(&maps[1], d_q, dtype, 3, q_dims, q_strides, box_own)) return rc;
+  if (int rc = paged_map(&maps[2], d_k_cache, dtype, 4, c_dims, c_strides, box_k)) return rc;
+  if (int rc = paged_map(&maps[3], d_v_cache, dtype, 4, c_dims, c_strides, box_v)) return rc;
+  int dev = 0, sms = PA_MAX_CTAS;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int grid = std::min(sms, PA_MAX_CTAS);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return cuda_fail(dtype == YSKN_DT_BF16 ? launch_prefix_attention<YSKN_DT_BF16>(p, head, st)
-                                         : launch_prefix_attention<YSKN_DT_F16>(p, head, st),
-                   "prefix_attention_kernel");
+  auto run = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    return dtype == YSKN_DT_BF16 ? launch_prefix_attention<D, YSKN_DT_BF16>(maps, p, grid, st)
+                                 : launch_prefix_attention<D, YSKN_DT_F16>(maps, p, grid, st);
+  };
+  if (head == 64) return run(std::integral_constant<int, 64>{});
+  if (head == 128) return run(std::integral_constant<int, 128>{});
+  return run(std::integral_constant<int, 256>{});
 }
