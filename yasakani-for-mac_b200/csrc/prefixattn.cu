@@ -22,22 +22,24 @@
 // divides, gates and rounds. Everything is summed in a fixed order: the same call gives the same
 // bits. The lengths stay on the device: every CTA forms the tile counts' prefix sum itself.
 //
-// prefix_attention_kernel: persistent, one CTA per SM, 8 warps:
-//   warp 0  brings 16 KB slots of K and V (64 channels of 128 rows; 128 KB / D rows of all
+// prefix_attention_kernel: persistent, one CTA per SM, 12 warps:
+//   warp 0  brings 16 KB slots of K and V (64 channels of 128 rows; 8192 / D rows of all
 //           channels) through a ring with TMA, box by box, each box within one block;
-//   warp 1  issues tcgen05.mma: S = Q K^T (128 x 128, K = D) into one of two TMEM tiles, then
+//   warp 1  (one thread) issues tcgen05.mma: S = Q K^T (128 x 128, K = D) into one of two TMEM tiles, then
 //           O += P V (128 x D, K = 128) with P read from TMEM, S of the next tile before P V of
 //           this one, so that the tensor cores run while the softmax does;
 //   warp 2  brings Q (TMA; a box is the G heads of whole tokens);
-//   warps 4..7  one thread per row: S from TMEM, the running maximum, P = 2^(s c - m) (c = scale
+//   warp 3  clears the V rows past a segment's last visible row (below);
+//   warps 4..11  two threads per row, one for each half of S's columns (and of O's): S from TMEM, the running maximum, P = 2^(s c - m) (c = scale
 //           log2 e) rounded to the cache's type over S's place, the row sum in binary32 of the
 //           unrounded weights. The maximum in use may lag: o and l are rescaled only when a
 //           row's maximum has grown by more than 2^8, so that a weight is at most 256 and o is
 //           seldom touched; the join uses the maximum in use, which cancels.
 // A tile's rows past the last visible one: their scores are set to -inf before the maximum, P V
-// runs over the 16-row steps that hold a visible row, and warp 1 clears the rest of the last
+// runs over the 16-row steps that hold a visible row, and warp 3 clears the rest of the last
 // step's V rows in shared memory (a zero weight does not silence a NaN).
-// Every mbarrier wait is bounded as in gemm.cu.
+// Every mbarrier wait is bounded as in gemm.cu; after a timeout the softmax warps go through
+// their remaining tiles without waiting, so that the halves' named barriers still match.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -50,7 +52,7 @@ namespace yskn {
 constexpr int PA_ROWS = 128;   // query rows per item (MMA M), TMEM lanes
 constexpr int PA_KEYS = 128;   // cache rows per tile
 constexpr int PA_SLOT = 16384;  // bytes per ring slot
-constexpr int PA_THREADS = 256;
+constexpr int PA_THREADS = 384;
 constexpr int PA_MAX_CTAS = 148;
 constexpr int PA_MAX_SLOTS = 12;
 
@@ -61,7 +63,7 @@ struct PaShape {
   static constexpr int RING = D == 256 ? 10 : PA_MAX_SLOTS;
   static constexpr int V_ROWS = PA_SLOT / (2 * D);
   static constexpr int Q_BYTES = PER_TILE * PA_SLOT;
-  static constexpr int SMEM = Q_BYTES + RING * PA_SLOT + 1024 /*align*/;
+  static constexpr int SMEM = Q_BYTES + RING * PA_SLOT + 3072 /*PaShared*/;
   static constexpr int S_COL = D < 128 ? 128 : D;  // TMEM columns: O at 0, S tiles at S_COL and S_COL + 128
 };
 
@@ -98,7 +100,7 @@ struct PrefixAttnParams {
   const int32_t* tables;
   int64_t table_stride;
   const int32_t *lens, *starts;
-  int n_blocks, block_size, prefix_len;
+  int n_blocks, block_shift, prefix_len;  // blocks of 1 << block_shift rows
   int own_limit;  // rows that a table row can name
   int batch, tokens, max_new, n_kvh, G, tpt;
   int pre_tiles, pre_qtiles, pre_items;
@@ -284,10 +286,47 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-// A bounded wait of a whole warp: all lanes go on or none does.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
 }
+// Two binary32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 y;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(y.x), "=f"(y.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return y;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 y;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(y.x), "=f"(y.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return y;
+}
+// Both warps of a row quarter.
+__device__ __forceinline__ void quarter_sync(int quarter) {
+  asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+}
+
+// Shared memory beside Q and the ring.
+struct PaShared {
+  uint64_t full[PA_MAX_SLOTS], empty[PA_MAX_SLOTS];  // ring slots: landed, read
+  uint64_t q_full, q_empty;
+  uint64_t s_full[2], p_full[2], pv_done[2];  // by tile parity
+  uint64_t o_free, drained, tail_go, tail;
+  int2 tail_at;
+  uint32_t tmem_slot;
+  int abort_word;
+  PaStart start;
+  long long sum[PA_THREADS / 32][2];
+  float half[2][2][PA_ROWS];  // tile parity, half, row: what a row's halves exchange
+};
+static_assert(sizeof(PaShared) <= 3072, "shared memory beside the ring");
 
 template <int D, int DT>
 __global__ void __launch_bounds__(PA_THREADS, 1)
@@ -296,32 +335,30 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                             const __grid_constant__ PrefixAttnParams p) {
   using Shape = PaShape<D>;
   constexpr int RING = Shape::RING, PT = Shape::PER_TILE, VR = Shape::V_ROWS;
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];  // 128B-swizzled tiles start on 1024 bytes
   uint8_t* sQ = smem;                    // [D / 64][128 rows][128 B]
   uint8_t* ring = smem + Shape::Q_BYTES;  // [RING][16 KB]
-  __shared__ uint64_t full[RING], empty[RING];  // ring slots: landed, read
-  __shared__ uint64_t q_full, q_empty;
-  __shared__ uint64_t s_full[2], p_full[2], pv_done[2];  // by tile parity
-  __shared__ uint64_t o_free, drained;
-  __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word;
-  __shared__ long long s_sum[PA_THREADS / 32][2];
-  __shared__ PaStart s_start;
-  volatile int* abort_flag = &abort_word;
+  PaShared& sh = *reinterpret_cast<PaShared*>(ring + RING * PA_SLOT);
+  uint64_t *full = sh.full, *empty = sh.empty, *s_full = sh.s_full, *p_full = sh.p_full, *pv_done = sh.pv_done;
+  uint64_t &q_full = sh.q_full, &q_empty = sh.q_empty, &o_free = sh.o_free, &drained = sh.drained, &tail_go = sh.tail_go, &tail = sh.tail;
+  float (&s_half)[2][2][PA_ROWS] = sh.half;
+  long long (&s_sum)[PA_THREADS / 32][2] = sh.sum;
+  PaStart& s_start = sh.start;
+  volatile int* abort_flag = &sh.abort_word;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
     for (int s = 0; s < RING; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
     mbar_init(&q_full, 1), mbar_init(&q_empty, 1);
-    for (int b = 0; b < 2; ++b) mbar_init(&s_full[b], 1), mbar_init(&p_full[b], 4), mbar_init(&pv_done[b], 1);
-    mbar_init(&o_free, 4), mbar_init(&drained, 1);
-    abort_word = 0;
+    for (int b = 0; b < 2; ++b) mbar_init(&s_full[b], 1), mbar_init(&p_full[b], 8), mbar_init(&pv_done[b], 1);
+    mbar_init(&o_free, 8), mbar_init(&drained, 1);
+    mbar_init(&tail_go, 1), mbar_init(&tail, 1);
+    sh.abort_word = 0;
     mbar_init_fence();
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == 3) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_slot)),
                  "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -391,18 +428,19 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = sh.tmem_slot;
   PaWalk walk(p, s_start);
   PaSegment seg;
 
   if (warp == 0) {
     // ---- K and V through the ring, in the order in which warp 1 uses them
-    int c = 0;
+    int c = 0, s = 0;  // slots filled, the ring's place
+    uint32_t turn = 1;  // parity of a place's last reading (first round: already free)
     bool ok = true;
-    const int pages = PA_KEYS / p.block_size, box_v = min(p.block_size, VR);
+    const int shift = p.block_shift, pages = PA_KEYS >> shift, box_v = min(1 << shift, VR);
     while (ok && walk.next(seg)) {
       const int32_t* table = seg.prefix ? p.prefix_blocks : p.tables + (int64_t)seg.req * p.table_stride;
-      const int page_end = (seg.keys + p.block_size - 1) / p.block_size;
+      const int page_end = (seg.keys + (1 << shift) - 1) >> shift;
       auto block_of = [&](int kt) {  // lane l: the block of page l of tile kt
         const int at = kt * pages + lane;
         int b = 0;
@@ -412,42 +450,50 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
         return b;
       };
-      auto slot = [&](uint32_t bytes) -> uint8_t* {
-        const int s = c % RING, u = c / RING;
-        if (u > 0 && !warp_wait(&empty[s], (u - 1) & 1, abort_flag)) return nullptr;
-        if (lane == 0) mbar_expect_tx(&full[s], bytes);
+      auto claim = [&](uint32_t bytes) {  // the next place of the ring, once it has been read
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], turn, abort_flag));
+        if (ok && lane == 0) mbar_expect_tx(&full[s], bytes);
         __syncwarp();
         return ring + s * PA_SLOT;
       };
+      auto advance = [&]() {
+        ++c;
+        if (++s == RING) s = 0, turn ^= 1;
+      };
       auto put_k = [&](int kt, int block) {
-        const int nk = min(PA_KEYS, seg.keys - kt * PA_KEYS), n = (nk + p.block_size - 1) / p.block_size;
-        for (int d = 0; d < PT; ++d, ++c) {
-          uint8_t* to = slot(n * p.block_size * 128);
-          if (!to) return false;
-          if (lane < n) tma_load_4d(to + lane * p.block_size * 128, &map_k, &full[c % RING], d * 64, 0, seg.kvh, block);
+        const int nk = min(PA_KEYS, seg.keys - kt * PA_KEYS), n = (nk + (1 << shift) - 1) >> shift;
+        for (int d = 0; ok && d < PT; ++d) {
+          uint8_t* to = claim((uint32_t)(n << shift) * 128);
+          if (!ok) break;
+          if (lane < n) tma_load_4d(to + (lane << shift) * 128, &map_k, &full[s], d * 64, 0, seg.kvh, block);
+          advance();
         }
-        return true;
       };
       auto put_v = [&](int kt, int block) {
         const int nk = min(PA_KEYS, seg.keys - kt * PA_KEYS);
-        for (int v = 0; v * VR < nk; ++v, ++c) {
+        for (int v = 0; ok && v * VR < nk; ++v) {
           const int n = (min(VR, nk - v * VR) + box_v - 1) / box_v;  // boxes along the rows
-          uint8_t* to = slot(n * box_v * 128 * PT);
-          if (!to) return false;
-          const int rg = lane / PT, sub = lane % PT, key = v * VR + rg * box_v;
-          const int b = __shfl_sync(0xffffffffu, block, min(key / p.block_size, 31));
-          if (rg < n)
-            tma_load_4d(to + sub * VR * 128 + rg * box_v * 128, &map_v, &full[c % RING], sub * 64,
-                        key % p.block_size, seg.kvh, b);
+          uint8_t* to = claim((uint32_t)(n * box_v) * 128 * PT);
+          if (!ok) break;
+          const int key = v * VR + lane * box_v;
+          const int b = __shfl_sync(0xffffffffu, block, (key >> shift) & 31);
+          // a box holds the rows of every 64 channels in turn; several boxes need one copy each
+          if (n == 1 && box_v == VR) {
+            if (lane == 0) tma_load_5d(to, &map_v, &full[s], 0, key & ((1 << shift) - 1), 0, seg.kvh, b);
+          } else if (lane < n) {
+            for (int d = 0; d < PT; ++d)
+              tma_load_5d(to + d * VR * 128 + lane * box_v * 128, &map_v, &full[s], 0, key & ((1 << shift) - 1), d,
+                          seg.kvh, b);
+          }
+          advance();
         }
-        return true;
       };
       int cur = block_of(seg.key0), nxt = block_of(seg.key0 + 1);
-      ok = put_k(seg.key0, cur);
+      put_k(seg.key0, cur);
       for (int kt = seg.key0; ok && kt < seg.key1; ++kt) {
         const int after = block_of(kt + 2);
-        if (kt + 1 < seg.key1) ok = put_k(kt + 1, nxt);
-        ok = ok && put_v(kt, cur);
+        if (kt + 1 < seg.key1) put_k(kt + 1, nxt);
+        if (ok) put_v(kt, cur);
         cur = nxt;
         nxt = after;
       }
@@ -459,67 +505,71 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
       }
   } else if (warp == 1) {
-    // ---- MMAs
-    const uint32_t id_qk = pa_idesc(DT, PA_KEYS, 0, p.negate_q), id_pv = pa_idesc(DT, D, 1, 0);
-    int c = 0, g = 0, n_seg = 0;  // slots used, tiles issued, segments
-    bool ok = true;
-    auto qk = [&](int tile) {  // S of the CTA's tile number `tile`
-      const uint32_t d = tmem + Shape::S_COL + (tile & 1) * PA_KEYS;
-      for (int ch = 0; ch < PT; ++ch, ++c) {
-        const int s = c % RING;
-        if (!warp_wait(&full[s], (c / RING) & 1, abort_flag)) return false;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t a = smem_u32(sQ + ch * PA_SLOT), b = smem_u32(ring + s * PA_SLOT);
+    // ---- MMAs: one thread
+    if (lane == 0) {
+      const uint32_t id_qk = pa_idesc(DT, PA_KEYS, 0, p.negate_q), id_pv = pa_idesc(DT, D, 1, 0);
+      int s = 0, g = 0, n_seg = 0;  // ring place, tiles issued, segments
+      uint32_t turn = 0, tails = 0;
+      bool ok = true;
+      const uint32_t q0 = smem_u32(sQ), r0 = smem_u32(ring);
+      auto advance = [&]() {
+        umma_commit(&empty[s]);
+        if (++s == RING) s = 0, turn ^= 1;
+      };
+      auto qk = [&](int tile) {  // S of the CTA's tile number `tile`
+        const uint32_t d = tmem + Shape::S_COL + (tile & 1) * PA_KEYS;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f16_ss(d, sw128_desc(a + k * 32), sw128_desc(b + k * 32), id_qk, ch > 0 || k > 0);
-          umma_commit(&empty[s]);
-        }
-      }
-      if (lane == 0) umma_commit(&s_full[tile & 1]);
-      return true;
-    };
-    while (ok && walk.next(seg)) {
-      ok = warp_wait(&q_full, n_seg & 1, abort_flag);
-      if (!ok) break;
-      const int n = seg.key1 - seg.key0;
-      ok = qk(g);
-      for (int j = 0; ok && j < n; ++j, ++g) {
-        if (j + 1 < n) ok = qk(g + 1);
-        if (ok && j == max(0, n - 2) && lane == 0) umma_commit(&q_empty);  // after the segment's last S
-        if (ok && j == 0 && n_seg > 0) ok = warp_wait(&o_free, (n_seg - 1) & 1, abort_flag);
-        if (!ok || !(ok = warp_wait(&p_full[g & 1], (g >> 1) & 1, abort_flag))) break;
-        tc_fence_after();
-        const int nk = min(PA_KEYS, seg.keys - (seg.key0 + j) * PA_KEYS);
-        const uint32_t pt = tmem + Shape::S_COL + (g & 1) * PA_KEYS;
-        for (int v = 0; v * VR < nk; ++v, ++c) {
-          const int s = c % RING, rows = min(VR, nk - v * VR), steps = (rows + 15) / 16;
-          if (!(ok = warp_wait(&full[s], (c / RING) & 1, abort_flag))) break;
-          uint8_t* base = ring + s * PA_SLOT;
-          if (rows & 15) {  // rows up to the end of the last step: zeros
-            const int n16 = (steps * 16 - rows) * 8;
-            for (int x = lane; x < n16 * PT; x += 32) {
-              const int sub = x / n16, y = x - sub * n16;
-              *reinterpret_cast<uint4*>(base + sub * VR * 128 + rows * 128 + y * 16) = make_uint4(0, 0, 0, 0);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-          }
+        for (int ch = 0; ch < PT; ++ch) {
+          ok = ok && mbar_wait(&full[s], turn, abort_flag);
+          if (!ok) return;
           tc_fence_after();
-          if (lane == 0) {
-            const uint32_t b = smem_u32(base);
-            for (int k = 0; k < steps; ++k)
-              umma_f16_ts(tmem, pt + (v * VR + k * 16) / 2, sw128_desc_mn(b + k * 2048, VR * 128), id_pv,
-                          j > 0 || v > 0 || k > 0);
-            umma_commit(&empty[s]);
-          }
+          const uint64_t a = sw128_desc(q0 + ch * PA_SLOT), b = sw128_desc(r0 + s * PA_SLOT);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_f16_ss(d, a + 2 * k, b + 2 * k, id_qk, ch > 0 || k > 0);
+          advance();
         }
-        if (ok && lane == 0) umma_commit(&pv_done[g & 1]);
+        umma_commit(&s_full[tile & 1]);
+      };
+      auto pv = [&](int nk, uint32_t pt, bool first) {
+#pragma unroll
+        for (int v = 0; v < PT; ++v) {
+          const int rows = nk - v * VR;
+          if (rows <= 0) break;
+          ok = ok && mbar_wait(&full[s], turn, abort_flag);
+          if (ok && rows < VR && (rows & 15)) {  // the segment's last slot: warp 3 clears its end
+            sh.tail_at = make_int2(s | (int)(turn << 8), rows);
+            mbar_arrive(&tail_go);
+            ok = mbar_wait(&tail, tails++ & 1, abort_flag);
+          }
+          if (!ok) return;
+          tc_fence_after();
+          const uint64_t b = sw128_desc_mn(r0 + s * PA_SLOT, VR * 128);
+#pragma unroll
+          for (int k = 0; k < VR / 16; ++k)
+            if (k * 16 < rows)
+              umma_f16_ts(tmem, pt + (v * VR + k * 16) / 2, b + 128 * k, id_pv, !first || v > 0 || k > 0);
+          advance();
+        }
+      };
+      for (; ok && walk.next(seg); ++n_seg) {
+        ok = mbar_wait(&q_full, n_seg & 1, abort_flag);
+        const int n = seg.key1 - seg.key0;
+        if (ok) qk(g);
+        for (int j = 0; ok && j < n; ++j, ++g) {
+          if (j + 1 < n) qk(g + 1);
+          if (ok && j == max(0, n - 2)) umma_commit(&q_empty);  // after the segment's last S
+          if (j == 0 && n_seg > 0) ok = ok && mbar_wait(&o_free, (n_seg - 1) & 1, abort_flag);
+          ok = ok && mbar_wait(&p_full[g & 1], (g >> 1) & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const int nk = min(PA_KEYS, seg.keys - (seg.key0 + j) * PA_KEYS);
+          pv(nk, tmem + Shape::S_COL + (g & 1) * PA_KEYS, j == 0);
+          if (ok) umma_commit(&pv_done[g & 1]);
+        }
       }
-      ++n_seg;
-    }
-    if (lane == 0) {  // every MMA of this CTA has completed before its TMEM is freed
+      sh.tail_at = make_int2(0, 0);  // no more of them
+      mbar_arrive(&tail_go);
+      // every MMA of this CTA has completed before its TMEM is freed
       umma_commit(&drained);
       const long long t0 = clock64();
       while (!mbar_try_wait(&drained, 0) && clock64() - t0 < TC_WAIT_LIMIT) {
@@ -543,14 +593,31 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
       }
     }
-  } else if (warp >= 4) {
-    // ---- softmax, one row per thread, then the segment's result
-    const int quarter = warp & 3, row = quarter * 32 + lane;
+  } else if (warp == 3) {
+    // ---- V rows past the last visible one, up to the end of the 16-row step, to zero: a slot that
+    // warp 1 names, once for each segment that ends inside a step
+    for (uint32_t n = 0;; ++n) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&tail_go, n & 1, abort_flag))) break;
+      const int2 t = sh.tail_at;  // ring place (its landing's parity in bit 8), rows to keep
+      if (t.y == 0) break;
+      const int s = t.x & 255, n16 = (16 - (t.y & 15)) * 8;
+      mbar_wait(&full[s], t.x >> 8, abort_flag);  // seen by warp 1; the rows are visible here too
+      uint8_t* base = ring + s * PA_SLOT + t.y * 128;
+      for (int x = lane; x < n16 * PT; x += 32) {
+        const int sub = x / n16, y = x - sub * n16;
+        *reinterpret_cast<uint4*>(base + sub * VR * 128 + y * 16) = make_uint4(0, 0, 0, 0);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tail);
+    }
+  } else {
+    // ---- softmax, a row's column halves in two threads, then the segment's result
+    const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const float c = p.c;
     int g = 0;
-    bool ok = true;
-    while (ok && walk.next(seg)) {
+    while (walk.next(seg)) {
       const int tl = row / p.G;  // token of the tile
       const bool valid = tl < seg.ntok;
       int lim = 0;  // rows on this axis that the row sees
@@ -570,32 +637,42 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       float m = -INFINITY, l = 0.0f;
       for (int kt = seg.key0; kt < seg.key1; ++kt, ++g) {
         const int b = g & 1;
-        if (!(ok = warp_wait(&s_full[b], (g >> 1) & 1, abort_flag))) break;
+        mbar_wait(&s_full[b], (g >> 1) & 1, abort_flag);
+        __syncwarp();
         if (live) {
           tc_fence_after();
           const uint32_t at = tmem + lanes + Shape::S_COL + b * PA_KEYS;
-          uint32_t s[4][32];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) tmem_ld32(at + x * 32, s[x]);
+          uint32_t s[2][32];
+          tmem_ld32(at + half * 64, s[0]);
+          tmem_ld32(at + half * 64 + 32, s[1]);
           tmem_ld_wait();
-          const int see = lim - kt * PA_KEYS;
           if (least < (kt + 1) * PA_KEYS) {
+            const int see = lim - kt * PA_KEYS - half * 64;
 #pragma unroll
-            for (int x = 0; x < 128; ++x)
+            for (int x = 0; x < 64; ++x)
               if (x >= see) s[x >> 5][x & 31] = 0xff800000u;  // -inf
           }
-          float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          auto val = [&](int x) { return __uint_as_float(s[x >> 5][x & 31]); };
+          float t[4] = {val(0), val(1), val(2), val(3)};
 #pragma unroll
-          for (int x = 0; x < 128; ++x) t[x & 3] = fmaxf(t[x & 3], __uint_as_float(s[x >> 5][x & 31]));
-          const float top = __fmul_rn(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), c);
+          for (int x = 4; x < 60; x += 8)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) t[y] = max3(t[y], val(x + 2 * y), val(x + 2 * y + 1));
+          t[0] = max3(t[0], val(60), val(61));
+          t[1] = max3(t[1], val(62), val(63));
+          const float mine = fmaxf(max3(t[0], t[1], t[2]), t[3]);
+          s_half[b][half][row] = mine;
+          quarter_sync(quarter);  // also: both halves have read S, so P may take its place
+          const float top = __fmul_rn(fmaxf(mine, s_half[b][half ^ 1][row]), c);
           if (m == -INFINITY) m = top;  // nothing seen before: o and l are zero
           const bool grown = top > m + 8.0f;
           if (__any_sync(0xffffffffu, grown)) {
             // o is complete up to the tile before; then scale it
-            if (!(ok = warp_wait(&pv_done[b ^ 1], ((g - 1) >> 1) & 1, abort_flag))) break;
+            mbar_wait(&pv_done[b ^ 1], ((g - 1) >> 1) & 1, abort_flag);
+            __syncwarp();
             tc_fence_after();
             const float f = grown ? exp2_approx(m - top) : 1.0f;
-            for (int x = 0; x < D; x += 32) {
+            for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
               uint32_t o[32];
               tmem_ld32(tmem + lanes + x, o);
               tmem_ld_wait();
@@ -606,37 +683,33 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             l *= f;
             if (grown) m = top;
           }
-          const float base = m == -INFINITY ? 0.0f : m;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const float base = m == -INFINITY ? 0.0f : -m;
+          const float2 c2 = make_float2(c, c), b2 = make_float2(base, base);
+          float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+          uint32_t w[32];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t w[32];
-#pragma unroll
-            for (int x = 0; x < 32; ++x) {
-              const int e = h * 64 + 2 * x;
-              const float a = exp2_approx(fmaf(__uint_as_float(s[e >> 5][e & 31]), c, -base));
-              const float d = exp2_approx(fmaf(__uint_as_float(s[e >> 5][(e + 1) & 31]), c, -base));
-              sum[x & 1] += a;
-              sum[2 + (x & 1)] += d;
-              w[x] = Elem<DT>::pack(a, d);
-            }
-            tmem_st32(at + h * 32, w);
+          for (int x = 0; x < 32; ++x) {
+            const float2 e = fma2(make_float2(val(2 * x), val(2 * x + 1)), c2, b2);
+            const float2 a = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+            sum[x & 1] = add2(sum[x & 1], a);
+            w[x] = Elem<DT>::pack(a.x, a.y);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_st32(at + half * 32, w);
+          sum[0] = add2(sum[0], sum[1]);
+          l += sum[0].x + sum[0].y;
           tmem_st_wait();
           tc_fence_before();
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[b]);
       }
-      if (!ok || !(ok = warp_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag))) break;
+      mbar_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag);
+      __syncwarp();
       if (live) {
         tc_fence_after();
         const int rows = seg.prefix ? PA_ROWS : p.own_rows;
-        float2* ml = (seg.prefix ? p.pre_ml : p.own_ml) + seg.place * rows + row;
         float* o = (seg.prefix ? p.pre_o : p.own_o) + (seg.place * rows + row) * D;
-        if (valid) *ml = make_float2(m, l);
-        for (int x = 0; x < D; x += 32) {
+        for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
           uint32_t v[32];
           tmem_ld32(tmem + lanes + x, v);
           tmem_ld_wait();
@@ -647,10 +720,17 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           }
         }
         tc_fence_before();
+        quarter_sync(quarter);  // the tiles' exchanges have been read
+        s_half[0][half][row] = l;
+        quarter_sync(quarter);
+        if (valid && half == 0)
+          ((seg.prefix ? p.pre_ml : p.own_ml) + seg.place * rows)[row] =
+              make_float2(m, l + s_half[0][1][row]);
+        quarter_sync(quarter);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&o_free);
-      if (!seg.prefix && seg.key0 == 0 && row == 0)
+      if (!seg.prefix && seg.key0 == 0 && row == 0 && half == 0)
         p.work_item[seg.place - blockIdx.x] = walk.tile - (seg.key1 - seg.key0);
     }
   }
@@ -744,13 +824,13 @@ static int launch_prefix_attention(const CUtensorMap (&maps)[4], const PrefixAtt
                    "prefix_combine_kernel");
 }
 
-// 16-bit tensor of 3 or 4 axes with 128B-swizzled boxes of 64 channels. Strides in elements.
+// 16-bit tensor of 3 to 5 axes with 128B-swizzled boxes of 64 channels. Strides in elements.
 static int paged_map(CUtensorMap* map, const void* base, int dt, int rank, const int64_t* dims, const int64_t* strides,
                      const int* box) {
   EncodeTiled fn = encode_fn();
   if (!fn) return fail(YSKN_ECUDA, "cuTensorMapEncodeTiled is not available");
-  cuuint64_t d[4], s[3];
-  cuuint32_t b[4], one[4] = {1, 1, 1, 1};
+  cuuint64_t d[5], s[4];
+  cuuint32_t b[5], one[5] = {1, 1, 1, 1, 1};
   for (int i = 0; i < rank; ++i) d[i] = (cuuint64_t)dims[i], b[i] = (cuuint32_t)box[i];
   for (int i = 0; i + 1 < rank; ++i) s[i] = (cuuint64_t)(dims[i + 1] == 1 ? dims[0] : strides[i]) * 2;
   const CUresult r = fn(map, dt == YSKN_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
@@ -805,7 +885,7 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(
   p.prefix_blocks = d_prefix_blocks;
   p.tables = d_block_tables, p.table_stride = table_stride;
   p.lens = d_lens, p.starts = d_starts;
-  p.n_blocks = n_blocks, p.block_size = block_size, p.prefix_len = prefix_len;
+  p.n_blocks = n_blocks, p.block_shift = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : 7, p.prefix_len = prefix_len;
   p.own_limit = (int)std::min<int64_t>((int64_t)table_width * block_size, INT32_MAX - PA_KEYS);
   p.batch = batch, p.tokens = tokens, p.max_new = max_new, p.n_kvh = n_kvh, p.G = G, p.tpt = tpt;
   p.pre_tiles = (int)ceil_div(prefix_len, PA_KEYS), p.pre_qtiles = (int)ceil_div(tokens, tpt);
@@ -828,12 +908,17 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(
   const int64_t q_dims[3] = {head, n_qh, tokens}, q_strides[2] = {q_head, q_row};
   const int64_t c_dims[4] = {head, block_size, n_kvh, n_blocks}, c_strides[3] = {token_stride, head_stride, block_stride};
   const int box_pre[3] = {64, G, tpt}, box_own[3] = {64, G, std::min(tpt, max_new)};
-  const int box_k[4] = {64, block_size, 1, 1}, box_v[4] = {64, std::min(block_size, v_rows), 1, 1};
+  // V: the 64-channel columns as an axis of their own, so that one box holds all channels of its
+  // rows in the order of the slot; where a slot takes several boxes, a box is one column
+  const int64_t v_dims[5] = {64, block_size, head / 64, n_kvh, n_blocks};
+  const int64_t v_strides[4] = {token_stride, 64, head_stride, block_stride};
+  const int box_k[4] = {64, block_size, 1, 1};
+  const int box_v[5] = {64, std::min(block_size, v_rows), block_size < v_rows ? 1 : head / 64, 1, 1};
   CUtensorMap maps[4];
   if (int rc = paged_map(&maps[0], d_q, dtype, 3, q_dims, q_strides, box_pre)) return rc;
   if (int rc = paged_map(&maps[1], d_q, dtype, 3, q_dims, q_strides, box_own)) return rc;
   if (int rc = paged_map(&maps[2], d_k_cache, dtype, 4, c_dims, c_strides, box_k)) return rc;
-  if (int rc = paged_map(&maps[3], d_v_cache, dtype, 4, c_dims, c_strides, box_v)) return rc;
+  if (int rc = paged_map(&maps[3], d_v_cache, dtype, 5, v_dims, v_strides, box_v)) return rc;
   int dev = 0, sms = PA_MAX_CTAS;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
