@@ -16,7 +16,8 @@
 //                 the P prefix rows: the prefix is read once per 128 rows, not once per request;
 //   own items     up to 128 rows of one request against that request's own rows.
 // Items are cut along their key tiles (128 rows of the cache) so that every CTA gets the same
-// number of tiles: CTA c takes tiles [c per, (c + 1) per) of all items in order. A piece of an
+// share: an item counts PA_ITEM_COST units and one per tile, and CTA c takes units
+// [c per, (c + 1) per) of all items in order. A piece of an
 // item is a segment; its unnormalised (m, l, o) goes to the workspace in binary32, at place
 // item + c, which no two segments share, and prefix_combine_kernel joins a row's segments,
 // divides, gates and rounds. Everything is summed in a fixed order: the same call gives the same
@@ -55,6 +56,7 @@ constexpr int PA_SLOT = 16384;  // bytes per ring slot
 constexpr int PA_THREADS = 384;
 constexpr int PA_MAX_CTAS = 148;
 constexpr int PA_MAX_SLOTS = 12;
+constexpr int PA_ITEM_COST = 2;  // an item's fixed cost (Q, the last P V's wait, its result) in tiles
 
 // Ring slots of K or V per tile, ring length, V rows per slot of head size D.
 template <int D>
@@ -106,10 +108,11 @@ struct PrefixAttnParams {
   int pre_tiles, pre_qtiles, pre_items;
   float c;  // |scale| log2 e
   uint32_t negate_q;
-  long long* work_per;    // tiles per CTA of this call, for the join
+  long long* work_per;    // units per CTA of this call, for the join
   int32_t* work_base;     // [batch] first own item of each request
-  long long* work_item;   // [own items] first tile of each own item
-  float2 *pre_ml, *own_ml;  // (m, l) per place and row
+  long long* work_item;   // [own items] first unit of each own item
+  // per place: (m, l) of each row; o as [D / 4][rows][4], so that a warp's rows are adjacent
+  float2 *pre_ml, *own_ml;
   float *pre_o, *own_o;
   int own_rows;
   long long own_items;  // more of them (starts that do not ascend) is an error: nothing is computed
@@ -152,6 +155,8 @@ __device__ __forceinline__ int pa_visible(const PrefixAttnParams& p, const PaReq
 __device__ __forceinline__ int pa_own_tiles(const PrefixAttnParams& p, const PaRequest& r, int qt) {
   return (pa_visible(p, r, min(r.n, (qt + 1) * p.tpt)) + PA_KEYS - 1) / PA_KEYS;
 }
+// Units of an item of so many tiles (0: nothing to do); unit u is tile u - PA_ITEM_COST.
+__host__ __device__ __forceinline__ int pa_units(int tiles) { return tiles > 0 ? tiles + PA_ITEM_COST : 0; }
 __device__ __forceinline__ int pa_qtiles(const PrefixAttnParams& p, const PaRequest& r) {
   return (r.n + p.tpt - 1) / p.tpt;
 }
@@ -164,40 +169,41 @@ struct PaSegment {
   int keys;             // rows on this axis that any of its tokens sees
   int first;            // own items: rows that token tok0 sees
   int64_t place;        // of its partial result
+  long long begin;      // the item's first unit
 };
 
-// Where a CTA's tiles begin, found by the whole CTA.
+// Where a CTA's units begin, found by the whole CTA.
 struct PaStart {
-  long long left;  // tiles of this CTA
-  int pre_item, k0;
+  long long left;  // units of this CTA
+  int pre_item, u0;    // prefix item and unit in it
   int req, item;       // own items: request and the items before it
-  long long skip;      // tiles of the request before this CTA's first
-  long long tile;      // index of the first tile
+  long long skip;      // units of the request before this CTA's first
+  long long unit;      // index of the first unit
 };
 
 // The CTA's segments in order; every lane of a warp walks alike.
 struct PaWalk {
   const PrefixAttnParams& p;
-  long long left, tile;
-  int pre_item, k0, req, item, kvh, qt;
+  long long left, unit;
+  int pre_item, u0, req, item, kvh, qt;
   PaRequest r;
   int nq;
   bool loaded;
   __device__ PaWalk(const PrefixAttnParams& p_, const PaStart& s)
-      : p(p_), left(s.left), tile(s.tile), pre_item(s.pre_item), k0(s.k0), req(s.req), item(s.item), kvh(0), qt(0),
+      : p(p_), left(s.left), unit(s.unit), pre_item(s.pre_item), u0(s.u0), req(s.req), item(s.item), kvh(0), qt(0),
         r{}, nq(0), loaded(false) {
     if (s.skip > 0) {
       load();
       long long skip = s.skip, head = 0;
-      for (int q = 0; q < nq; ++q) head += pa_own_tiles(p, r, q);
+      for (int q = 0; q < nq; ++q) head += pa_units(pa_own_tiles(p, r, q));
       kvh = (int)(skip / head);
       skip -= kvh * head;
       for (;; ++qt) {
-        const int kt = pa_own_tiles(p, r, qt);
-        if (skip < kt) break;
-        skip -= kt;
+        const int u = pa_units(pa_own_tiles(p, r, qt));
+        if (skip < u) break;
+        skip -= u;
       }
-      k0 = (int)skip;
+      u0 = (int)skip;
     }
   }
   __device__ void load() {
@@ -205,10 +211,9 @@ struct PaWalk {
     nq = pa_qtiles(p, r);
     loaded = true;
   }
-  // The next segment; tile is then the index of its first tile plus its length.
+  // The next segment; false past the last.
   __device__ bool next(PaSegment& s) {
-    if (left <= 0) return false;
-    if (pre_item < p.pre_items) {
+    while (left > 0 && pre_item < p.pre_items) {
       s.prefix = true;
       s.kvh = pre_item / p.pre_qtiles;
       s.tok0 = (pre_item - s.kvh * p.pre_qtiles) * p.tpt;
@@ -216,26 +221,24 @@ struct PaWalk {
       s.req = 0;
       s.keys = p.prefix_len;
       s.first = 0;
-      take(s, p.pre_tiles, pre_item);
       ++pre_item;
-      return true;
+      if (take(s, p.pre_tiles, pre_item - 1)) return true;
     }
-    while (req < p.batch) {
+    while (left > 0 && req < p.batch) {
       if (!loaded) load();
       for (; kvh < p.n_kvh; ++kvh, qt = 0)
-        for (; qt < nq; ++qt) {
-          const int kt = pa_own_tiles(p, r, qt);
+        while (qt < nq) {
+          const int q = qt++, kt = pa_own_tiles(p, r, q);
           if (kt == 0) continue;
           s.prefix = false;
           s.kvh = kvh;
-          s.tok0 = r.s0 + qt * p.tpt;
-          s.ntok = min(p.tpt, r.n - qt * p.tpt);
+          s.tok0 = r.s0 + q * p.tpt;
+          s.ntok = min(p.tpt, r.n - q * p.tpt);
           s.req = req;
-          s.keys = pa_visible(p, r, qt * p.tpt + s.ntok);
-          s.first = r.len - r.n + qt * p.tpt + 1 - p.prefix_len;
-          take(s, kt, item + kvh * nq + qt);
-          ++qt;
-          return true;
+          s.keys = pa_visible(p, r, q * p.tpt + s.ntok);
+          s.first = r.len - r.n + q * p.tpt + 1 - p.prefix_len;
+          if (take(s, kt, item + kvh * nq + q)) return true;
+          if (left <= 0) return false;
         }
       item += p.n_kvh * nq;
       ++req;
@@ -244,14 +247,17 @@ struct PaWalk {
     }
     return false;
   }
-  __device__ void take(PaSegment& s, int tiles, int it) {
-    const int n = (int)min((long long)(tiles - k0), left);
-    s.key0 = k0;
-    s.key1 = k0 + n;
+  // This CTA's part of an item; false if it holds no tile.
+  __device__ bool take(PaSegment& s, int tiles, int it) {
+    const int n = (int)min((long long)(tiles + PA_ITEM_COST - u0), left);
+    s.key0 = max(u0 - PA_ITEM_COST, 0);
+    s.key1 = max(u0 + n - PA_ITEM_COST, 0);
     s.place = (int64_t)it + blockIdx.x;
+    s.begin = unit - u0;
     left -= n;
-    tile += n;
-    k0 = 0;
+    unit += n;
+    u0 = 0;
+    return s.key0 < s.key1;
   }
 };
 
@@ -364,7 +370,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   }
   pdl_begin();
 
-  // Tile counts of all requests and where this CTA begins.
+  // Unit counts of all requests and where this CTA begins.
   {
     const int per = (p.batch + PA_THREADS - 1) / PA_THREADS;
     const int i0 = min(p.batch, tid * per), i1 = min(p.batch, i0 + per);
@@ -373,7 +379,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       const PaRequest r = pa_request(p, i);
       const int nq = pa_qtiles(p, r);
       long long t = 0;
-      for (int q = 0; q < nq; ++q) t += pa_own_tiles(p, r, q);
+      for (int q = 0; q < nq; ++q) t += pa_units(pa_own_tiles(p, r, q));
       tiles += t * p.n_kvh;
       items += nq * p.n_kvh;
       if (blockIdx.x == 0 && (__ldg(p.starts + i + 1) - r.s0 != r.n)) raise_device_error(p.err, DERR_RANGE);
@@ -393,14 +399,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       total_items += s_sum[w][1];
     }
     const bool sound = total_items <= p.own_items;
-    const long long pre = (long long)p.pre_items * p.pre_tiles, all = sound ? pre + total : 0;
+    const int pre_units = pa_units(p.pre_tiles);
+    const long long pre = (long long)p.pre_items * pre_units, all = sound ? pre + total : 0;
     const long long share = sound ? max(1ll, (all + gridDim.x - 1) / gridDim.x) : 0;
     const long long t0 = min(all, blockIdx.x * share), t1 = min(all, t0 + share);
     if (tid == 0) {
       s_start = {t1 - t0, p.pre_items, 0, 0, 0, 0, t0};
       if (t0 < pre) {
-        s_start.pre_item = (int)(t0 / p.pre_tiles);
-        s_start.k0 = (int)(t0 - (long long)s_start.pre_item * p.pre_tiles);
+        s_start.pre_item = (int)(t0 / pre_units);
+        s_start.u0 = (int)(t0 - (long long)s_start.pre_item * pre_units);
       }
       if (blockIdx.x == 0) {
         *p.work_per = share;
@@ -408,7 +415,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       }
     }
     __syncthreads();
-    const long long at = t0 - pre;  // this CTA's first own tile
+    const long long at = t0 - pre;  // this CTA's first own unit
     if (sound && ((at >= 0 && at >= before && at < before + tiles) || blockIdx.x == 0)) {
       long long b = before;
       int item = (int)items_before;
@@ -416,7 +423,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         const PaRequest r = pa_request(p, i);
         const int nq = pa_qtiles(p, r);
         long long t = 0;
-        for (int q = 0; q < nq; ++q) t += pa_own_tiles(p, r, q);
+        for (int q = 0; q < nq; ++q) t += pa_units(pa_own_tiles(p, r, q));
         t *= p.n_kvh;
         if (at >= b && at < b + t) s_start.req = i, s_start.item = item, s_start.skip = at - b;
         if (blockIdx.x == 0) p.work_base[i] = item;
@@ -708,7 +715,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       if (live) {
         tc_fence_after();
         const int rows = seg.prefix ? PA_ROWS : p.own_rows;
-        float* o = (seg.prefix ? p.pre_o : p.own_o) + (seg.place * rows + row) * D;
+        float4* o = reinterpret_cast<float4*>((seg.prefix ? p.pre_o : p.own_o) + seg.place * rows * D) + row;
         for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
           uint32_t v[32];
           tmem_ld32(tmem + lanes + x, v);
@@ -716,7 +723,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           if (valid) {
 #pragma unroll
             for (int y = 0; y < 32; y += 4)
-              *reinterpret_cast<uint4*>(o + x + y) = make_uint4(v[y], v[y + 1], v[y + 2], v[y + 3]);
+              o[(x + y) / 4 * rows] = make_float4(__uint_as_float(v[y]), __uint_as_float(v[y + 1]),
+                                                  __uint_as_float(v[y + 2]), __uint_as_float(v[y + 3]));
           }
         }
         tc_fence_before();
@@ -731,7 +739,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&o_free);
       if (!seg.prefix && seg.key0 == 0 && row == 0 && half == 0)
-        p.work_item[seg.place - blockIdx.x] = walk.tile - (seg.key1 - seg.key0);
+        p.work_item[seg.place - blockIdx.x] = seg.begin;
     }
   }
   tc_fence_before();
@@ -743,72 +751,90 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   }
 }
 
-// Joins the segments of each row: one warp per (token, query head), lane l the channels
-// V l .. V l + V - 1.
+// Joins the segments of each row. A warp takes 8 rows (in the order of the prefix items' rows)
+// and 64 channels: lane (r, q) row r, the channels 4 q .. 4 q + 3 of each 16, so that a load of
+// the warp is 4 runs of 128 adjacent bytes and a store 8 runs of 32.
 template <int D, int DT>
 __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_constant__ PrefixAttnParams p) {
-  constexpr int V = D / 32;
+  constexpr int PARTS = D / 64;
   pdl_begin();
-  const int lane = threadIdx.x & 31, n_qh = p.n_kvh * p.G;
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (item >= (int64_t)p.tokens * n_qh) return;
-  const int t = (int)(item / n_qh), h = (int)(item - (int64_t)t * n_qh), kvh = h / p.G, gh = h - kvh * p.G;
-  float o[V], den = 0.0f, top = -INFINITY;
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t kvh_rows = (int64_t)p.tokens * p.G, idx = unit / PARTS * 8 + (lane & 7);
+  if (idx >= kvh_rows * p.n_kvh) return;
+  const int ch = (int)(unit % PARTS) * 16 + (lane >> 3);  // of 4 channels; then every 4th
+  const int kvh = (int)(idx / kvh_rows);
+  const int64_t in_kvh = idx - kvh * kvh_rows;
+  const int t = (int)(in_kvh / p.G), gh = (int)(in_kvh - (int64_t)t * p.G);
+  float4 o[4];
+  float den = 0.0f, top = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < V; ++j) o[j] = 0.0f;
+  for (int j = 0; j < 4; ++j) o[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   const int i = request_of(p.starts, p.batch, t);
   const long long per = *p.work_per;
   const PaRequest r = i < p.batch ? pa_request(p, i) : PaRequest{};
   if (per > 0 && t >= r.s0 && t < r.s0 + r.n) {
     // places of the row's segments: n_pre of its prefix item, then n_own of its own item
-    int n_pre = 0, n_own = 0;
+    int n_pre = 0, n_own = 0, pre_row = 0;
     int64_t pre0 = 0, own0 = 0;
     if (p.pre_tiles > 0) {
-      const int qt = t / p.tpt, it = kvh * p.pre_qtiles + qt, row = (t - qt * p.tpt) * p.G + gh;
-      const long long b = (long long)it * p.pre_tiles, c0 = b / per, c1 = (b + p.pre_tiles - 1) / per;
+      const int qt = t / p.tpt, it = kvh * p.pre_qtiles + qt;
+      const long long b = (long long)it * pa_units(p.pre_tiles) + PA_ITEM_COST;
+      const long long c0 = b / per, c1 = (b + p.pre_tiles - 1) / per;
       n_pre = (int)(c1 - c0) + 1;
-      pre0 = (it + c0) * PA_ROWS + row;
+      pre0 = it + c0;
+      pre_row = (t - qt * p.tpt) * p.G + gh;
     }
     const int own_qt = (t - r.s0) / p.tpt, own_row = (t - r.s0 - own_qt * p.tpt) * p.G + gh;
     const int kt = pa_own_tiles(p, r, own_qt);
     if (kt > 0) {
       const int64_t it = (int64_t)p.work_base[i] + kvh * pa_qtiles(p, r) + own_qt;
-      const long long b = p.work_item[it], c0 = b / per, c1 = (b + kt - 1) / per;
+      const long long b = p.work_item[it] + PA_ITEM_COST, c0 = b / per, c1 = (b + kt - 1) / per;
       n_own = (int)(c1 - c0) + 1;
-      own0 = (it + c0) * p.own_rows + own_row;
+      own0 = it + c0;
     }
-    for (int x = lane; x < n_pre + n_own; x += 32) {
-      const float2 v = x < n_pre ? p.pre_ml[pre0 + (int64_t)x * PA_ROWS] : p.own_ml[own0 + (int64_t)(x - n_pre) * p.own_rows];
-      top = fmaxf(top, v.x);
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    auto ml_of = [&](int x) {
+      return x < n_pre ? p.pre_ml[(pre0 + x) * PA_ROWS + pre_row] : p.own_ml[(own0 + x - n_pre) * p.own_rows + own_row];
+    };
+#pragma unroll 4
+    for (int x = 0; x < n_pre + n_own; ++x) top = fmaxf(top, ml_of(x).x);
 #pragma unroll 4
     for (int x = 0; x < n_pre + n_own; ++x) {
-      const int64_t at = x < n_pre ? pre0 + (int64_t)x * PA_ROWS : own0 + (int64_t)(x - n_pre) * p.own_rows;
-      const float2 v = (x < n_pre ? p.pre_ml : p.own_ml)[at];
-      const float* src = (x < n_pre ? p.pre_o : p.own_o) + at * D + lane * V;
+      const float2 v = ml_of(x);
+      const bool pre = x < n_pre;
+      const int rows = pre ? PA_ROWS : p.own_rows;
+      const float4* src = reinterpret_cast<const float4*>((pre ? p.pre_o : p.own_o) +
+                                                          (pre ? pre0 + x : own0 + x - n_pre) * rows * D) +
+                          (pre ? pre_row : own_row);
+      float4 y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = src[(ch + 4 * j) * rows];
       const float w = v.x == -INFINITY ? 0.0f : exp2f(v.x - top);
       den = fmaf(v.y, w, den);
 #pragma unroll
-      for (int j = 0; j < V; j += 2) {
-        const float2 y = *reinterpret_cast<const float2*>(src + j);
-        o[j] = fmaf(y.x, w, o[j]);
-        o[j + 1] = fmaf(y.y, w, o[j + 1]);
+      for (int j = 0; j < 4; ++j) {
+        o[j].x = fmaf(y[j].x, w, o[j].x);
+        o[j].y = fmaf(y[j].y, w, o[j].y);
+        o[j].z = fmaf(y[j].z, w, o[j].z);
+        o[j].w = fmaf(y[j].w, w, o[j].w);
       }
     }
   }
+  const int h = kvh * p.G + gh;
   const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+  uint16_t* out = p.out + ((int64_t)t * p.n_kvh * p.G + h) * D;
 #pragma unroll
-  for (int j = 0; j < V; ++j) o[j] *= inv;
-  if (p.gate) {
-    const uint16_t* gate = p.gate + t * p.gate_row + h * p.gate_head + lane * V;
+  for (int j = 0; j < 4; ++j) {
+    const int at = (ch + 4 * j) * 4;
+    float v[4] = {o[j].x * inv, o[j].y * inv, o[j].z * inv, o[j].w * inv};
+    if (p.gate) {
+      const uint2 g = *reinterpret_cast<const uint2*>(p.gate + t * p.gate_row + h * p.gate_head + at);
+      const uint16_t gs[4] = {(uint16_t)g.x, (uint16_t)(g.x >> 16), (uint16_t)g.y, (uint16_t)(g.y >> 16)};
 #pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = o[j] / (1.0f + expf(-Elem<DT>::to_float(gate[j])));
+      for (int x = 0; x < 4; ++x) v[x] = v[x] / (1.0f + expf(-Elem<DT>::to_float(gs[x])));
+    }
+    *reinterpret_cast<uint2*>(out + at) = make_uint2(Elem<DT>::pack(v[0], v[1]), Elem<DT>::pack(v[2], v[3]));
   }
-  uint32_t* out = reinterpret_cast<uint32_t*>(p.out + item * D + lane * V);
-#pragma unroll
-  for (int j = 0; j < V; j += 2) out[j / 2] = Elem<DT>::pack(o[j], o[j + 1]);
 }
 
 template <int D, int DT>
@@ -819,8 +845,8 @@ static int launch_prefix_attention(const CUtensorMap (&maps)[4], const PrefixAtt
   if (cudaError_t e = launch_pdl(prefix_attention_kernel<D, DT>, grid, PA_THREADS, PaShape<D>::SMEM, st, maps[0],
                                  maps[1], maps[2], maps[3], p))
     return cuda_fail(e, "prefix_attention_kernel");
-  const int64_t rows = (int64_t)p.tokens * p.n_kvh * p.G;
-  return cuda_fail(launch_pdl(prefix_combine_kernel<D, DT>, (unsigned)ceil_div(rows, 8), 256, 0, st, p),
+  const int64_t warps = ceil_div((int64_t)p.tokens * p.n_kvh * p.G, 8) * (D / 64);
+  return cuda_fail(launch_pdl(prefix_combine_kernel<D, DT>, (unsigned)ceil_div(warps, 8), 256, 0, st, p),
                    "prefix_combine_kernel");
 }
 
