@@ -11,36 +11,45 @@
 // The softmax over all rows is the join of softmaxes over parts: with a part's maximum m,
 // l = sum exp(s - m) and o = sum exp(s - m) v, parts join as sum exp(m - M) o / sum
 // exp(m - M) l, M the largest m. So the work is cut into items:
-//   prefix items  128 query rows (a row is a token and one of the G query heads of a KV head;
-//                 128 / G whole tokens of the batch, whichever request they belong to) against
-//                 the P prefix rows: the prefix is read once per 128 rows, not once per request;
-//   own items     up to 128 rows of one request against that request's own rows.
-// Items are cut along their key tiles (128 rows of the cache) so that every CTA gets the same
-// share: an item counts PA_ITEM_COST units and one per tile, and CTA c takes units
-// [c per, (c + 1) per) of all items in order. A piece of an
-// item is a segment; its unnormalised (m, l, o) goes to the workspace in binary32, at place
-// item + c, which no two segments share, and prefix_combine_kernel joins a row's segments,
-// divides, gates and rounds. Everything is summed in a fixed order: the same call gives the same
-// bits. The lengths stay on the device: every CTA forms the tile counts' prefix sum itself.
+//   prefix items  256 query rows (a row is a token and one of the G query heads of a KV head;
+//                 2 * floor(128 / G) whole tokens of the batch, whichever request they belong
+//                 to) against the P prefix rows: the prefix is read once per 256 rows, not once
+//                 per request;
+//   own items     up to 256 rows of one request against that request's own rows.
+// Items are cut along their key tiles (128 rows of the cache) so that every pair of SMs gets the
+// same share: an item counts PA_ITEM_COST units and one per tile, and pair c takes units
+// [c per, (c + 1) per) of all items in order. A piece of an item is a segment; its unnormalised
+// (m, l, o) goes to the workspace in binary32, at place item + c, which no two segments share,
+// and prefix_combine_kernel joins a row's segments, divides, gates and rounds. Everything is
+// summed in a fixed order: the same call gives the same bits. The lengths stay on the device:
+// every CTA forms the prefix sum of the requests' units itself.
 //
-// prefix_attention_kernel: persistent, one CTA per SM, 12 warps:
-//   warp 0  brings 16 KB slots of K and V (64 channels of 128 rows; 8192 / D rows of all
-//           channels) through a ring with TMA, box by box, each box within one block;
-//   warp 1  (one thread) issues tcgen05.mma: S = Q K^T (128 x 128, K = D) into one of two TMEM tiles, then
-//           O += P V (128 x D, K = 128) with P read from TMEM, S of the next tile before P V of
-//           this one, so that the tensor cores run while the softmax does;
+// prefix_attention_kernel: persistent, clusters of two CTAs (a pair of SMs), 12 warps each. The
+// pair works on 256 rows with tcgen05.mma.cta_group::2: each CTA holds its 128 rows of Q, S, P and
+// O, and half of each K tile (64 of its 128 rows) and V tile (half of the channels). With one
+// SM per 128 rows, the operands' reads (128 KB of Q and K and 64 KB of V per tile) and the copies'
+// writes (128 KB) alone need 2560 clocks of shared memory per tile, against 2048 of the tensor
+// cores at D = 256, and twice the L2 traffic; halved K and V bring it to 1536. In each CTA:
+//   warp 0  brings 16 KB slots of K and V (64 K rows of 128 channels; 64 V rows of 128 channels or
+//           128 of 64 or 32) through a ring with TMA, each box within one block. The copies of
+//           both CTAs count on the first CTA's barriers;
+//   warp 1  (one thread of the first CTA) issues S = Q K^T (256 x 128, K = D) into one of two
+//           TMEM tiles, then O += P V (256 x D, K = 128) with P read from TMEM, S of the next tile
+//           before P V of this one, so that the tensor cores run while the softmax does;
 //   warp 2  brings Q (TMA; a box is the G heads of whole tokens);
 //   warp 3  clears the V rows past a segment's last visible row (below);
-//   warps 4..11  two threads per row, one for each half of S's columns (and of O's): S from TMEM, the running maximum, P = 2^(s c - m) (c = scale
-//           log2 e) rounded to the cache's type over S's place, the row sum in binary32 of the
-//           unrounded weights. The maximum in use may lag: o and l are rescaled only when a
-//           row's maximum has grown by more than 2^8, so that a weight is at most 256 and o is
-//           seldom touched; the join uses the maximum in use, which cancels.
+//   warps 4..11  two threads per row, one for each half of S's columns (and of O's): S from
+//           TMEM, the running maximum, P = 2^(s c - m) (c = scale log2 e) rounded to the cache's
+//           type over S's place, the row sum in binary32 of the unrounded weights. The maximum in
+//           use may lag: o and l are rescaled only when a row's maximum has grown by more than
+//           2^8, so that a weight is at most 256 and o is seldom touched; the join uses the
+//           maximum in use, which cancels.
 // A tile's rows past the last visible one: their scores are set to -inf before the maximum, P V
 // runs over the 16-row steps that hold a visible row, and warp 3 clears the rest of the last
 // step's V rows in shared memory (a zero weight does not silence a NaN).
 // Every mbarrier wait is bounded as in gemm.cu; after a timeout the softmax warps go through
-// their remaining tiles without waiting, so that the halves' named barriers still match.
+// their remaining tiles without waiting, so that the halves' named barriers still match, and
+// both CTAs meet before either leaves.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -50,21 +59,24 @@
 
 namespace yskn {
 
-constexpr int PA_ROWS = 128;   // query rows per item (MMA M), TMEM lanes
-constexpr int PA_KEYS = 128;   // cache rows per tile
+constexpr int PA_ROWS = 128;    // query rows of a CTA, TMEM lanes
+constexpr int PA_KEYS = 128;    // cache rows per tile
 constexpr int PA_SLOT = 16384;  // bytes per ring slot
 constexpr int PA_THREADS = 384;
-constexpr int PA_MAX_CTAS = 148;
+constexpr int PA_MAX_PAIRS = 74;
 constexpr int PA_MAX_SLOTS = 12;
 constexpr int PA_ITEM_COST = 2;  // an item's fixed cost (Q, the last P V's wait, its result) in tiles
 
-// Ring slots of K or V per tile, ring length, V rows per slot of head size D.
 template <int D>
 struct PaShape {
-  static constexpr int PER_TILE = D / 64;
+  static constexpr int CHUNKS = D / 64;                     // 64-channel columns of a head
+  static constexpr int SLOTS = D <= 128 ? 1 : D / 128;      // ring slots of a K or a V tile (one CTA's half)
+  static constexpr int K_CHUNKS = CHUNKS / SLOTS;           // K slot: 64 rows of so many columns
+  static constexpr int V_ROWS = PA_KEYS / SLOTS;            // V slot: so many rows
+  static constexpr int V_CHUNKS = D <= 128 ? 1 : D / 128;   // of so many columns (D = 64: half a column)
+  static constexpr int V_LINE = D == 64 ? 64 : 128;         // bytes of a V row in a column, the swizzle's span
   static constexpr int RING = D == 256 ? 10 : PA_MAX_SLOTS;
-  static constexpr int V_ROWS = PA_SLOT / (2 * D);
-  static constexpr int Q_BYTES = PER_TILE * PA_SLOT;
+  static constexpr int Q_BYTES = CHUNKS * PA_ROWS * 128;
   static constexpr int SMEM = Q_BYTES + RING * PA_SLOT + 3072 /*PaShared*/;
   static constexpr int S_COL = D < 128 ? 128 : D;  // TMEM columns: O at 0, S tiles at S_COL and S_COL + 128
 };
@@ -72,24 +84,25 @@ struct PaShape {
 // The workspace: sizes from the host's bounds alone, so that both sides agree.
 struct PaWork {
   int64_t base, item, pre_ml, pre_o, own_ml, own_o, bytes;  // byte offsets
-  int own_rows;                                             // rows per own segment's place
+  int own_half, own_rows;                                   // rows of a CTA and of the pair in an own item's place
   int64_t own_items;                                        // own items that there is room for
 };
 inline PaWork pa_work(int tokens, int batch, int max_new, int n_qh, int n_kvh, int head) {
   auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
-  const int G = n_qh / n_kvh, tpt = PA_ROWS / G;  // tokens per item
-  const int64_t pre_items = ceil_div(tokens, tpt) * n_kvh;
-  // sum of ceil(n_i / tpt) over requests with n_i > 0: at most one more than n_i / tpt each
-  const int64_t own_items = (std::min(batch, tokens) + (int64_t)tokens / tpt) * n_kvh;
-  const int64_t pre = pre_items + PA_MAX_CTAS, own = own_items + PA_MAX_CTAS;
+  const int G = n_qh / n_kvh, tpc = PA_ROWS / G, tpi = 2 * tpc;  // tokens per CTA and per item
+  const int64_t pre_items = ceil_div(tokens, tpi) * n_kvh;
+  // sum of ceil(n_i / tpi) over requests with n_i > 0: at most one more than n_i / tpi each
+  const int64_t own_items = (std::min(batch, tokens) + (int64_t)tokens / tpi) * n_kvh;
+  const int64_t pre = pre_items + PA_MAX_PAIRS, own = own_items + PA_MAX_PAIRS;
   PaWork w{};
-  w.own_rows = G * std::min(tpt, max_new);
+  w.own_half = G * std::min(tpc, max_new);
+  w.own_rows = max_new > tpc ? 2 * w.own_half : w.own_half;
   w.own_items = own_items;
   w.base = 256;
   w.item = w.base + up((int64_t)batch * 4);
   w.pre_ml = w.item + up(own_items * 8);
-  w.pre_o = w.pre_ml + up(pre * PA_ROWS * 8);
-  w.own_ml = w.pre_o + up(pre * PA_ROWS * head * 4);
+  w.pre_o = w.pre_ml + up(pre * 2 * PA_ROWS * 8);
+  w.own_ml = w.pre_o + up(pre * 2 * PA_ROWS * head * 4);
   w.own_o = w.own_ml + up(own * w.own_rows * 8);
   w.bytes = w.own_o + up(own * w.own_rows * head * 4);
   return w;
@@ -104,17 +117,18 @@ struct PrefixAttnParams {
   const int32_t *lens, *starts;
   int n_blocks, block_shift, prefix_len;  // blocks of 1 << block_shift rows
   int own_limit;  // rows that a table row can name
-  int batch, tokens, max_new, n_kvh, G, tpt;
+  int batch, tokens, max_new, n_kvh, G;
+  int tpc, tpi;  // tokens per CTA and per item
   int pre_tiles, pre_qtiles, pre_items;
   float c;  // |scale| log2 e
   uint32_t negate_q;
-  long long* work_per;    // units per CTA of this call, for the join
+  long long* work_per;    // units per pair of this call, for the join
   int32_t* work_base;     // [batch] first own item of each request
   long long* work_item;   // [own items] first unit of each own item
   // per place: (m, l) of each row; o as [D / 4][rows][4], so that a warp's rows are adjacent
   float2 *pre_ml, *own_ml;
   float *pre_o, *own_o;
-  int own_rows;
+  int own_half, own_rows;
   long long own_items;  // more of them (starts that do not ascend) is an error: nothing is computed
   uint16_t* out;  // [tokens][n_qh][D]
   unsigned* err;
@@ -153,12 +167,12 @@ __device__ __forceinline__ int pa_visible(const PrefixAttnParams& p, const PaReq
   return min(max(r.len - r.n + upto - p.prefix_len, 0), p.own_limit);
 }
 __device__ __forceinline__ int pa_own_tiles(const PrefixAttnParams& p, const PaRequest& r, int qt) {
-  return (pa_visible(p, r, min(r.n, (qt + 1) * p.tpt)) + PA_KEYS - 1) / PA_KEYS;
+  return (pa_visible(p, r, min(r.n, (qt + 1) * p.tpi)) + PA_KEYS - 1) / PA_KEYS;
 }
 // Units of an item of so many tiles (0: nothing to do); unit u is tile u - PA_ITEM_COST.
 __host__ __device__ __forceinline__ int pa_units(int tiles) { return tiles > 0 ? tiles + PA_ITEM_COST : 0; }
 __device__ __forceinline__ int pa_qtiles(const PrefixAttnParams& p, const PaRequest& r) {
-  return (r.n + p.tpt - 1) / p.tpt;
+  return (r.n + p.tpi - 1) / p.tpi;
 }
 
 struct PaSegment {
@@ -172,16 +186,16 @@ struct PaSegment {
   long long begin;      // the item's first unit
 };
 
-// Where a CTA's units begin, found by the whole CTA.
+// Where a pair's units begin, found by each of its CTAs.
 struct PaStart {
-  long long left;  // units of this CTA
+  long long left;  // units of this pair
   int pre_item, u0;    // prefix item and unit in it
   int req, item;       // own items: request and the items before it
-  long long skip;      // units of the request before this CTA's first
+  long long skip;      // units of the request before this pair's first
   long long unit;      // index of the first unit
 };
 
-// The CTA's segments in order; every lane of a warp walks alike.
+// The pair's segments in order; every lane of a warp walks alike.
 struct PaWalk {
   const PrefixAttnParams& p;
   long long left, unit;
@@ -216,8 +230,8 @@ struct PaWalk {
     while (left > 0 && pre_item < p.pre_items) {
       s.prefix = true;
       s.kvh = pre_item / p.pre_qtiles;
-      s.tok0 = (pre_item - s.kvh * p.pre_qtiles) * p.tpt;
-      s.ntok = min(p.tpt, p.tokens - s.tok0);
+      s.tok0 = (pre_item - s.kvh * p.pre_qtiles) * p.tpi;
+      s.ntok = min(p.tpi, p.tokens - s.tok0);
       s.req = 0;
       s.keys = p.prefix_len;
       s.first = 0;
@@ -232,11 +246,11 @@ struct PaWalk {
           if (kt == 0) continue;
           s.prefix = false;
           s.kvh = kvh;
-          s.tok0 = r.s0 + q * p.tpt;
-          s.ntok = min(p.tpt, r.n - q * p.tpt);
+          s.tok0 = r.s0 + q * p.tpi;
+          s.ntok = min(p.tpi, r.n - q * p.tpi);
           s.req = req;
-          s.keys = pa_visible(p, r, q * p.tpt + s.ntok);
-          s.first = r.len - r.n + q * p.tpt + 1 - p.prefix_len;
+          s.keys = pa_visible(p, r, q * p.tpi + s.ntok);
+          s.first = r.len - r.n + q * p.tpi + 1 - p.prefix_len;
           if (take(s, kt, item + kvh * nq + q)) return true;
           if (left <= 0) return false;
         }
@@ -247,12 +261,12 @@ struct PaWalk {
     }
     return false;
   }
-  // This CTA's part of an item; false if it holds no tile.
+  // This pair's part of an item; false if it holds no tile.
   __device__ bool take(PaSegment& s, int tiles, int it) {
     const int n = (int)min((long long)(tiles + PA_ITEM_COST - u0), left);
     s.key0 = max(u0 - PA_ITEM_COST, 0);
     s.key1 = max(u0 + n - PA_ITEM_COST, 0);
-    s.place = (int64_t)it + blockIdx.x;
+    s.place = (int64_t)it + (blockIdx.x >> 1);
     s.begin = unit - u0;
     left -= n;
     unit += n;
@@ -261,29 +275,76 @@ struct PaWalk {
   }
 };
 
-// B operand whose N runs along the 128-byte swizzled rows (V: rows are keys, MMA K): 64-channel
-// columns `stride` bytes apart, 8-key groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr, uint32_t stride) {
-  return (uint64_t)((saddr >> 4) & 0x3fff) | ((uint64_t)(stride >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         (1ull << 46) | (2ull << 61);
+// B operand whose N runs along the swizzled rows (V: rows are keys, MMA K), in columns of LINE
+// bytes `stride` bytes apart, 8-key groups 8 LINE bytes apart. Swizzle span 128 or 64 bytes.
+template <int LINE>
+__device__ __forceinline__ uint64_t mn_desc(uint32_t saddr, uint32_t stride) {
+  return (uint64_t)((saddr >> 4) & 0x3fff) | ((uint64_t)(stride >> 4) << 16) | ((uint64_t)(8 * LINE >> 4) << 32) |
+         (1ull << 46) | ((LINE == 128 ? 2ull : 4ull) << 61);
 }
-// kind::f16 with f32 accumulators, M = 128: type of both operands, N, B's major axis, A's sign.
+// kind::f16 with f32 accumulators, M = 256: type of both operands, N, B's major axis, A's sign.
 __device__ __forceinline__ uint32_t pa_idesc(int dt, int n, uint32_t b_mn, uint32_t negate_a) {
   const uint32_t t = dt == YSKN_DT_BF16 ? 1u : 0u;
   return (1u << 4) | (t << 7) | (t << 10) | (negate_a << 13) | (b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
-         ((uint32_t)(PA_ROWS >> 4) << 24);
+         ((uint32_t)(2 * PA_ROWS >> 4) << 24);
 }
-__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma2_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::
           "r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
 }
-__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma2_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::
           "r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+// Arrives on the barrier at this place in both CTAs once the MMAs issued so far are done.
+__device__ __forceinline__ void umma2_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+// ---- the pair: addresses and barriers of its first CTA
+__device__ __forceinline__ uint32_t first_cta(const void* p) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
+  return a;
+}
+// What these two announce is in TMEM or comes by TMA, so that they order no memory of their own
+// (cluster-scope release and acquire here cost hundreds of clocks each: 16 prompt chunks 1439 us, now 986).
+__device__ __forceinline__ void arrive_first(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void expect_first(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// After stores to this CTA's shared memory that the first CTA's MMAs read.
+__device__ __forceinline__ void release_first(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// TMA into this CTA's shared memory, counted on a barrier of the pair's first CTA.
+__device__ __forceinline__ void pair_load_3d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
+      "%5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void pair_load_5d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w,
+                                             int v) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
+      "%5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v)
+      : "memory");
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -319,12 +380,15 @@ __device__ __forceinline__ void quarter_sync(int quarter) {
   asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
 }
 
-// Shared memory beside Q and the ring.
+// Shared memory beside Q and the ring. "First": only the first CTA's copy is used.
 struct PaShared {
-  uint64_t full[PA_MAX_SLOTS], empty[PA_MAX_SLOTS];  // ring slots: landed, read
-  uint64_t q_full, q_empty;
-  uint64_t s_full[2], p_full[2], pv_done[2];  // by tile parity
-  uint64_t o_free, drained, tail_go, tail;
+  uint64_t full[PA_MAX_SLOTS];   // ring place landed in both CTAs (first)
+  uint64_t empty[PA_MAX_SLOTS];  // ring place read
+  uint64_t q_full, q_empty;      // Q landed in both CTAs (first), read
+  uint64_t s_full[2], pv_done[2];  // by tile parity: S written, P V done
+  uint64_t p_full[2];              // P written by both CTAs (first)
+  uint64_t o_free;                 // O read by both CTAs (first)
+  uint64_t drained, tail_full, tail_done;
   int2 tail_at;
   uint32_t tmem_slot;
   int abort_word;
@@ -335,42 +399,38 @@ struct PaShared {
 static_assert(sizeof(PaShared) <= 3072, "shared memory beside the ring");
 
 template <int D, int DT>
-__global__ void __launch_bounds__(PA_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
     prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q_pre, const __grid_constant__ CUtensorMap map_q_own,
                             const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                             const __grid_constant__ PrefixAttnParams p) {
   using Shape = PaShape<D>;
-  constexpr int RING = Shape::RING, PT = Shape::PER_TILE, VR = Shape::V_ROWS;
-  extern __shared__ __align__(1024) uint8_t smem[];  // 128B-swizzled tiles start on 1024 bytes
-  uint8_t* sQ = smem;                    // [D / 64][128 rows][128 B]
+  constexpr int RING = Shape::RING, SLOTS = Shape::SLOTS, VR = Shape::V_ROWS;
+  extern __shared__ __align__(1024) uint8_t smem[];  // swizzled tiles start on 1024 bytes
+  uint8_t* sQ = smem;                     // [D / 64][128 rows][128 B]
   uint8_t* ring = smem + Shape::Q_BYTES;  // [RING][16 KB]
   PaShared& sh = *reinterpret_cast<PaShared*>(ring + RING * PA_SLOT);
-  uint64_t *full = sh.full, *empty = sh.empty, *s_full = sh.s_full, *p_full = sh.p_full, *pv_done = sh.pv_done;
-  uint64_t &q_full = sh.q_full, &q_empty = sh.q_empty, &o_free = sh.o_free, &drained = sh.drained, &tail_go = sh.tail_go, &tail = sh.tail;
-  float (&s_half)[2][2][PA_ROWS] = sh.half;
-  long long (&s_sum)[PA_THREADS / 32][2] = sh.sum;
-  PaStart& s_start = sh.start;
   volatile int* abort_flag = &sh.abort_word;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   if (tid == 0) {
-    for (int s = 0; s < RING; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
-    mbar_init(&q_full, 1), mbar_init(&q_empty, 1);
-    for (int b = 0; b < 2; ++b) mbar_init(&s_full[b], 1), mbar_init(&p_full[b], 8), mbar_init(&pv_done[b], 1);
-    mbar_init(&o_free, 8), mbar_init(&drained, 1);
-    mbar_init(&tail_go, 1), mbar_init(&tail, 1);
+    for (int s = 0; s < RING; ++s) mbar_init(&sh.full[s], 2), mbar_init(&sh.empty[s], 1);
+    mbar_init(&sh.q_full, 2), mbar_init(&sh.q_empty, 1);
+    for (int b = 0; b < 2; ++b) mbar_init(&sh.s_full[b], 1), mbar_init(&sh.p_full[b], 16), mbar_init(&sh.pv_done[b], 1);
+    mbar_init(&sh.o_free, 16), mbar_init(&sh.drained, 1);
+    mbar_init(&sh.tail_full, 1), mbar_init(&sh.tail_done, 1);
     sh.abort_word = 0;
     mbar_init_fence();
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == 3) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_slot)),
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_slot)),
                  "r"(512));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
   pdl_begin();
 
-  // Unit counts of all requests and where this CTA begins.
+  // Unit counts of all requests and where this pair begins.
   {
     const int per = (p.batch + PA_THREADS - 1) / PA_THREADS;
     const int i0 = min(p.batch, tid * per), i1 = min(p.batch, i0 + per);
@@ -390,24 +450,24 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       const long long a = __shfl_up_sync(0xffffffffu, ti, off), b = __shfl_up_sync(0xffffffffu, it, off);
       if (lane >= off) ti += a, it += b;
     }
-    if (lane == 31) s_sum[warp][0] = ti, s_sum[warp][1] = it;
+    if (lane == 31) sh.sum[warp][0] = ti, sh.sum[warp][1] = it;
     __syncthreads();
     long long before = ti - tiles, items_before = it - items, total = 0, total_items = 0;
     for (int w = 0; w < PA_THREADS / 32; ++w) {
-      if (w < warp) before += s_sum[w][0], items_before += s_sum[w][1];
-      total += s_sum[w][0];
-      total_items += s_sum[w][1];
+      if (w < warp) before += sh.sum[w][0], items_before += sh.sum[w][1];
+      total += sh.sum[w][0];
+      total_items += sh.sum[w][1];
     }
     const bool sound = total_items <= p.own_items;
     const int pre_units = pa_units(p.pre_tiles);
     const long long pre = (long long)p.pre_items * pre_units, all = sound ? pre + total : 0;
-    const long long share = sound ? max(1ll, (all + gridDim.x - 1) / gridDim.x) : 0;
-    const long long t0 = min(all, blockIdx.x * share), t1 = min(all, t0 + share);
+    const long long share = sound ? max(1ll, (all + pairs - 1) / pairs) : 0;
+    const long long t0 = min(all, pair * share), t1 = min(all, t0 + share);
     if (tid == 0) {
-      s_start = {t1 - t0, p.pre_items, 0, 0, 0, 0, t0};
+      sh.start = {t1 - t0, p.pre_items, 0, 0, 0, 0, t0};
       if (t0 < pre) {
-        s_start.pre_item = (int)(t0 / pre_units);
-        s_start.u0 = (int)(t0 - (long long)s_start.pre_item * pre_units);
+        sh.start.pre_item = (int)(t0 / pre_units);
+        sh.start.u0 = (int)(t0 - (long long)sh.start.pre_item * pre_units);
       }
       if (blockIdx.x == 0) {
         *p.work_per = share;
@@ -415,7 +475,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       }
     }
     __syncthreads();
-    const long long at = t0 - pre;  // this CTA's first own unit
+    const long long at = t0 - pre;  // this pair's first own unit
     if (sound && ((at >= 0 && at >= before && at < before + tiles) || blockIdx.x == 0)) {
       long long b = before;
       int item = (int)items_before;
@@ -425,7 +485,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         long long t = 0;
         for (int q = 0; q < nq; ++q) t += pa_units(pa_own_tiles(p, r, q));
         t *= p.n_kvh;
-        if (at >= b && at < b + t) s_start.req = i, s_start.item = item, s_start.skip = at - b;
+        if (at >= b && at < b + t) sh.start.req = i, sh.start.item = item, sh.start.skip = at - b;
         if (blockIdx.x == 0) p.work_base[i] = item;
         b += t;
         item += nq * p.n_kvh;
@@ -434,17 +494,23 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync();  // both CTAs' barriers are set up
   tc_fence_after();
   const uint32_t tmem = sh.tmem_slot;
-  PaWalk walk(p, s_start);
+  PaWalk walk(p, sh.start);
   PaSegment seg;
 
   if (warp == 0) {
-    // ---- K and V through the ring, in the order in which warp 1 uses them
-    int c = 0, s = 0;  // slots filled, the ring's place
+    // ---- K and V through the ring, in the order in which the MMAs use them: this CTA's half of
+    // each tile's K rows, and of V's channels
+    int s = 0;          // the ring's place
     uint32_t turn = 1;  // parity of a place's last reading (first round: already free)
+    uint32_t tails = 0;
     bool ok = true;
-    const int shift = p.block_shift, pages = PA_KEYS >> shift, box_v = min(1 << shift, VR);
+    const int shift = p.block_shift, pages = PA_KEYS >> shift;
+    const int box_k = min(1 << shift, PA_KEYS / 2), box_v = min(1 << shift, VR);
+    const uint32_t full0 = first_cta(&sh.full[0]);
+    const int v_chunk = D == 64 ? 0 : rank * Shape::V_CHUNKS, v_x = D == 64 ? rank * 32 : 0;
     while (ok && walk.next(seg)) {
       const int32_t* table = seg.prefix ? p.prefix_blocks : p.tables + (int64_t)seg.req * p.table_stride;
       const int page_end = (seg.keys + (1 << shift) - 1) >> shift;
@@ -457,41 +523,65 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
         return b;
       };
-      auto claim = [&](uint32_t bytes) {  // the next place of the ring, once it has been read
-        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], turn, abort_flag));
-        if (ok && lane == 0) mbar_expect_tx(&full[s], bytes);
-        __syncwarp();
+      // The next place of the ring, once both CTAs' part of it has been read.
+      auto claim = [&]() {
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[s], turn, abort_flag));
         return ring + s * PA_SLOT;
       };
       auto advance = [&]() {
-        ++c;
         if (++s == RING) s = 0, turn ^= 1;
       };
+      // Rows key0 .. key0 + n * box - 1 of the tile, `chunks` columns from `chunk` on, as
+      // [column][ROWS rows][line] at `to`: one box, or one per block and column.
+      auto copy = [&](uint8_t* to, const CUtensorMap* map, uint32_t bar, int key0, int n, int box, int rows, int x,
+                      int chunk, int chunks, int line, int block) {
+        const int key = key0 + lane * box;
+        const int b = __shfl_sync(0xffffffffu, block, (key >> shift) & 31);
+        if (lane < n) {
+          const int y = key & ((1 << shift) - 1);
+          if (box == rows) pair_load_5d(to, map, bar, x, y, chunk, seg.kvh, b);
+          else
+            for (int d = 0; d < chunks; ++d)
+              pair_load_5d(to + (d * rows + lane * box) * line, map, bar, x, y, chunk + d, seg.kvh, b);
+        }
+      };
       auto put_k = [&](int kt, int block) {
-        const int nk = min(PA_KEYS, seg.keys - kt * PA_KEYS), n = (nk + (1 << shift) - 1) >> shift;
-        for (int d = 0; ok && d < PT; ++d) {
-          uint8_t* to = claim((uint32_t)(n << shift) * 128);
+        const int nk = min(max(seg.keys - kt * PA_KEYS - rank * (PA_KEYS / 2), 0), PA_KEYS / 2);
+        const int n = (nk + box_k - 1) / box_k;
+        for (int d = 0; ok && d < SLOTS; ++d) {
+          uint8_t* to = claim();
           if (!ok) break;
-          if (lane < n) tma_load_4d(to + (lane << shift) * 128, &map_k, &full[s], d * 64, 0, seg.kvh, block);
+          const uint32_t bar = full0 + 8 * s;
+          if (lane == 0) expect_first(bar, (uint32_t)(n * box_k * 128 * Shape::K_CHUNKS));
+          __syncwarp();
+          copy(to, &map_k, bar, rank * (PA_KEYS / 2), n, box_k, PA_KEYS / 2, 0, d * Shape::K_CHUNKS, Shape::K_CHUNKS,
+               128, block);
           advance();
         }
       };
       auto put_v = [&](int kt, int block) {
         const int nk = min(PA_KEYS, seg.keys - kt * PA_KEYS);
         for (int v = 0; ok && v * VR < nk; ++v) {
-          const int n = (min(VR, nk - v * VR) + box_v - 1) / box_v;  // boxes along the rows
-          uint8_t* to = claim((uint32_t)(n * box_v) * 128 * PT);
+          const int rows = min(VR, nk - v * VR), n = (rows + box_v - 1) / box_v;
+          uint8_t* to = claim();
           if (!ok) break;
-          const int key = v * VR + lane * box_v;
-          const int b = __shfl_sync(0xffffffffu, block, (key >> shift) & 31);
-          // a box holds the rows of every 64 channels in turn; several boxes need one copy each
-          if (n == 1 && box_v == VR) {
-            if (lane == 0) tma_load_5d(to, &map_v, &full[s], 0, key & ((1 << shift) - 1), 0, seg.kvh, b);
-          } else if (lane < n) {
-            for (int d = 0; d < PT; ++d)
-              tma_load_5d(to + d * VR * 128 + lane * box_v * 128, &map_v, &full[s], 0, key & ((1 << shift) - 1), d,
-                          seg.kvh, b);
+          uint32_t bar = full0 + 8 * s;
+          const uint32_t bytes = (uint32_t)(n * box_v) * Shape::V_LINE * Shape::V_CHUNKS;
+          if (rows & 15) {  // lands on this CTA's barrier; warp 3 clears the end and then arrives
+            if (tails > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.tail_done, (tails - 1) & 1, abort_flag));
+            if (!ok) break;
+            ++tails;
+            if (lane == 0) {
+              sh.tail_at = make_int2(s, rows);
+              mbar_expect_tx(&sh.tail_full, bytes);
+            }
+            bar = smem_u32(&sh.tail_full);  // of this CTA, as a cluster address
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&sh.tail_full)), "r"(rank));
+          } else if (lane == 0) {
+            expect_first(bar, bytes);
           }
+          __syncwarp();
+          copy(to, &map_v, bar, v * VR, n, box_v, VR, v_x, v_chunk, Shape::V_CHUNKS, Shape::V_LINE, block);
           advance();
         }
       };
@@ -505,128 +595,139 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         nxt = after;
       }
     }
-    if (!ok && lane == 0)  // let the copies that this warp started land before the CTA leaves
-      for (int k = max(0, c - RING); k < c; ++k) {
-        const long long t0 = clock64();
-        while (!mbar_try_wait(&full[k % RING], (k / RING) & 1) && clock64() - t0 < TC_WAIT_LIMIT) {
-        }
+    if (ok && tails > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.tail_done, (tails - 1) & 1, abort_flag));
+    if (ok && lane == 0) {
+      sh.tail_at = make_int2(0, 0);  // no more of them
+      mbar_arrive(&sh.tail_full);
+    }
+    if (!ok) {  // a copy lands within microseconds: let those that this warp started do so
+      const long long t0 = clock64();
+      while (clock64() - t0 < TC_WAIT_LIMIT / 1000) {
       }
+    }
   } else if (warp == 1) {
-    // ---- MMAs: one thread
-    if (lane == 0) {
+    // ---- MMAs: one thread of the first CTA
+    if (lane == 0 && rank == 0) {
       const uint32_t id_qk = pa_idesc(DT, PA_KEYS, 0, p.negate_q), id_pv = pa_idesc(DT, D, 1, 0);
       int s = 0, g = 0, n_seg = 0;  // ring place, tiles issued, segments
-      uint32_t turn = 0, tails = 0;
+      uint32_t turn = 0;
       bool ok = true;
       const uint32_t q0 = smem_u32(sQ), r0 = smem_u32(ring);
       auto advance = [&]() {
-        umma_commit(&empty[s]);
+        umma2_commit(&sh.empty[s]);
         if (++s == RING) s = 0, turn ^= 1;
       };
-      auto qk = [&](int tile) {  // S of the CTA's tile number `tile`
+      auto qk = [&](int tile) {  // S of the pair's tile number `tile`
         const uint32_t d = tmem + Shape::S_COL + (tile & 1) * PA_KEYS;
 #pragma unroll
-        for (int ch = 0; ch < PT; ++ch) {
-          ok = ok && mbar_wait(&full[s], turn, abort_flag);
+        for (int v = 0; v < SLOTS; ++v) {
+          ok = ok && mbar_wait(&sh.full[s], turn, abort_flag);
           if (!ok) return;
           tc_fence_after();
-          const uint64_t a = sw128_desc(q0 + ch * PA_SLOT), b = sw128_desc(r0 + s * PA_SLOT);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_f16_ss(d, a + 2 * k, b + 2 * k, id_qk, ch > 0 || k > 0);
+          for (int ch = 0; ch < Shape::K_CHUNKS; ++ch) {
+            const uint64_t a = sw128_desc(q0 + (v * Shape::K_CHUNKS + ch) * PA_ROWS * 128);
+            const uint64_t b = sw128_desc(r0 + s * PA_SLOT + ch * (PA_KEYS / 2) * 128);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) umma2_ss(d, a + 2 * k, b + 2 * k, id_qk, v > 0 || ch > 0 || k > 0);
+          }
           advance();
         }
-        umma_commit(&s_full[tile & 1]);
+        umma2_commit(&sh.s_full[tile & 1]);
       };
       auto pv = [&](int nk, uint32_t pt, bool first) {
 #pragma unroll
-        for (int v = 0; v < PT; ++v) {
+        for (int v = 0; v < SLOTS; ++v) {
           const int rows = nk - v * VR;
           if (rows <= 0) break;
-          ok = ok && mbar_wait(&full[s], turn, abort_flag);
-          if (ok && rows < VR && (rows & 15)) {  // the segment's last slot: warp 3 clears its end
-            sh.tail_at = make_int2(s | (int)(turn << 8), rows);
-            mbar_arrive(&tail_go);
-            ok = mbar_wait(&tail, tails++ & 1, abort_flag);
-          }
+          ok = ok && mbar_wait(&sh.full[s], turn, abort_flag);
           if (!ok) return;
           tc_fence_after();
-          const uint64_t b = sw128_desc_mn(r0 + s * PA_SLOT, VR * 128);
+          const uint64_t b = mn_desc<Shape::V_LINE>(r0 + s * PA_SLOT, VR * Shape::V_LINE);
 #pragma unroll
           for (int k = 0; k < VR / 16; ++k)
             if (k * 16 < rows)
-              umma_f16_ts(tmem, pt + (v * VR + k * 16) / 2, b + 128 * k, id_pv, !first || v > 0 || k > 0);
+              umma2_ts(tmem, pt + (v * VR + k * 16) / 2, b + (16 * Shape::V_LINE >> 4) * k, id_pv,
+                       !first || v > 0 || k > 0);
           advance();
         }
       };
       for (; ok && walk.next(seg); ++n_seg) {
-        ok = mbar_wait(&q_full, n_seg & 1, abort_flag);
+        ok = mbar_wait(&sh.q_full, n_seg & 1, abort_flag);
         const int n = seg.key1 - seg.key0;
         if (ok) qk(g);
         for (int j = 0; ok && j < n; ++j, ++g) {
           if (j + 1 < n) qk(g + 1);
-          if (ok && j == max(0, n - 2)) umma_commit(&q_empty);  // after the segment's last S
-          if (j == 0 && n_seg > 0) ok = ok && mbar_wait(&o_free, (n_seg - 1) & 1, abort_flag);
-          ok = ok && mbar_wait(&p_full[g & 1], (g >> 1) & 1, abort_flag);
+          if (ok && j == max(0, n - 2)) umma2_commit(&sh.q_empty);  // after the segment's last S
+          if (j == 0 && n_seg > 0) ok = ok && mbar_wait(&sh.o_free, (n_seg - 1) & 1, abort_flag);
+          ok = ok && mbar_wait(&sh.p_full[g & 1], (g >> 1) & 1, abort_flag);
           if (!ok) break;
           tc_fence_after();
           const int nk = min(PA_KEYS, seg.keys - (seg.key0 + j) * PA_KEYS);
           pv(nk, tmem + Shape::S_COL + (g & 1) * PA_KEYS, j == 0);
-          if (ok) umma_commit(&pv_done[g & 1]);
+          if (ok) umma2_commit(&sh.pv_done[g & 1]);
         }
       }
-      sh.tail_at = make_int2(0, 0);  // no more of them
-      mbar_arrive(&tail_go);
-      // every MMA of this CTA has completed before its TMEM is freed
-      umma_commit(&drained);
+      // every MMA of the pair has completed before its TMEM is freed
+      umma2_commit(&sh.drained);
       const long long t0 = clock64();
-      while (!mbar_try_wait(&drained, 0) && clock64() - t0 < TC_WAIT_LIMIT) {
+      while (!mbar_try_wait(&sh.drained, 0) && clock64() - t0 < TC_WAIT_LIMIT) {
       }
     }
   } else if (warp == 2) {
-    // ---- Q
+    // ---- Q: this CTA's tokens of each item
     if (lane == 0) {
+      const uint32_t bar = first_cta(&sh.q_full);
       int n_seg = 0;
       bool ok = true;
       for (; walk.next(seg); ++n_seg) {
-        if (n_seg > 0 && !(ok = mbar_wait(&q_empty, (n_seg - 1) & 1, abort_flag))) break;
-        const int box = seg.prefix ? p.tpt : min(p.tpt, p.max_new);
-        mbar_expect_tx(&q_full, (uint32_t)(box * p.G * 128 * PT));
-        for (int d = 0; d < PT; ++d)
-          tma_load_3d(sQ + d * PA_SLOT, seg.prefix ? &map_q_pre : &map_q_own, &q_full, d * 64, seg.kvh * p.G, seg.tok0);
+        if (n_seg > 0 && !(ok = mbar_wait(&sh.q_empty, (n_seg - 1) & 1, abort_flag))) break;
+        const int box = seg.prefix ? p.tpc : min(p.tpc, p.max_new);
+        const bool any = seg.ntok > rank * p.tpc;
+        expect_first(bar, any ? (uint32_t)(box * p.G * 128 * Shape::CHUNKS) : 0u);
+        if (any)
+          for (int d = 0; d < Shape::CHUNKS; ++d)
+            pair_load_3d(sQ + d * PA_ROWS * 128, seg.prefix ? &map_q_pre : &map_q_own, bar, d * 64, seg.kvh * p.G,
+                         seg.tok0 + rank * p.tpc);
       }
-      if (!ok && n_seg > 0) {
+      if (!ok) {
         const long long t0 = clock64();
-        while (!mbar_try_wait(&q_full, (n_seg - 1) & 1) && clock64() - t0 < TC_WAIT_LIMIT) {
+        while (clock64() - t0 < TC_WAIT_LIMIT / 1000) {
         }
       }
     }
   } else if (warp == 3) {
-    // ---- V rows past the last visible one, up to the end of the 16-row step, to zero: a slot that
-    // warp 1 names, once for each segment that ends inside a step
+    // ---- V rows past the last visible one, up to the end of the 16-row step, to zero, in the
+    // slots that warp 0 names: once for each segment that ends inside a step
+    const uint32_t full0 = first_cta(&sh.full[0]);
     for (uint32_t n = 0;; ++n) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&tail_go, n & 1, abort_flag))) break;
-      const int2 t = sh.tail_at;  // ring place (its landing's parity in bit 8), rows to keep
+      if (!__all_sync(0xffffffffu, mbar_wait(&sh.tail_full, n & 1, abort_flag))) break;
+      const int2 t = sh.tail_at;  // ring place, rows to keep
       if (t.y == 0) break;
-      const int s = t.x & 255, n16 = (16 - (t.y & 15)) * 8;
-      mbar_wait(&full[s], t.x >> 8, abort_flag);  // seen by warp 1; the rows are visible here too
-      uint8_t* base = ring + s * PA_SLOT + t.y * 128;
-      for (int x = lane; x < n16 * PT; x += 32) {
-        const int sub = x / n16, y = x - sub * n16;
-        *reinterpret_cast<uint4*>(base + sub * VR * 128 + y * 16) = make_uint4(0, 0, 0, 0);
+      constexpr int UNITS = Shape::V_LINE / 16;  // 16-byte units of a row
+      const int units = (16 - (t.y & 15)) * UNITS;
+      uint8_t* base = ring + t.x * PA_SLOT + t.y * Shape::V_LINE;
+      for (int x = lane; x < units * Shape::V_CHUNKS; x += 32) {
+        const int ch = x / units, y = x - ch * units;
+        *reinterpret_cast<uint4*>(base + ch * VR * Shape::V_LINE + y * 16) = make_uint4(0, 0, 0, 0);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tail);
+      if (lane == 0) {
+        release_first(full0 + 8 * t.x);
+        mbar_arrive(&sh.tail_done);
+      }
     }
   } else {
     // ---- softmax, a row's column halves in two threads, then the segment's result
     const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t p_full0 = first_cta(&sh.p_full[0]), o_free0 = first_cta(&sh.o_free);
     const float c = p.c;
     int g = 0;
     while (walk.next(seg)) {
-      const int tl = row / p.G;  // token of the tile
-      const bool valid = tl < seg.ntok;
+      const int tl = rank * p.tpc + row / p.G;  // token of the item
+      const bool valid = row / p.G < p.tpc && tl < seg.ntok;
       int lim = 0;  // rows on this axis that the row sees
       if (valid) {
         if (seg.prefix) {
@@ -644,7 +745,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       float m = -INFINITY, l = 0.0f;
       for (int kt = seg.key0; kt < seg.key1; ++kt, ++g) {
         const int b = g & 1;
-        mbar_wait(&s_full[b], (g >> 1) & 1, abort_flag);
+        mbar_wait(&sh.s_full[b], (g >> 1) & 1, abort_flag);
         __syncwarp();
         if (live) {
           tc_fence_after();
@@ -668,14 +769,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           t[0] = max3(t[0], val(60), val(61));
           t[1] = max3(t[1], val(62), val(63));
           const float mine = fmaxf(max3(t[0], t[1], t[2]), t[3]);
-          s_half[b][half][row] = mine;
+          sh.half[b][half][row] = mine;
           quarter_sync(quarter);  // also: both halves have read S, so P may take its place
-          const float top = __fmul_rn(fmaxf(mine, s_half[b][half ^ 1][row]), c);
+          const float top = __fmul_rn(fmaxf(mine, sh.half[b][half ^ 1][row]), c);
           if (m == -INFINITY) m = top;  // nothing seen before: o and l are zero
           const bool grown = top > m + 8.0f;
           if (__any_sync(0xffffffffu, grown)) {
             // o is complete up to the tile before; then scale it
-            mbar_wait(&pv_done[b ^ 1], ((g - 1) >> 1) & 1, abort_flag);
+            mbar_wait(&sh.pv_done[b ^ 1], ((g - 1) >> 1) & 1, abort_flag);
             __syncwarp();
             tc_fence_after();
             const float f = grown ? exp2_approx(m - top) : 1.0f;
@@ -708,14 +809,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           tc_fence_before();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[b]);
+        if (lane == 0) arrive_first(p_full0 + 8 * b);
       }
-      mbar_wait(&pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag);
+      mbar_wait(&sh.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag);
       __syncwarp();
       if (live) {
         tc_fence_after();
-        const int rows = seg.prefix ? PA_ROWS : p.own_rows;
-        float4* o = reinterpret_cast<float4*>((seg.prefix ? p.pre_o : p.own_o) + seg.place * rows * D) + row;
+        const int rows = seg.prefix ? 2 * PA_ROWS : p.own_rows;
+        const int at = rank * (seg.prefix ? PA_ROWS : p.own_half) + row;  // of the place
+        float4* o = reinterpret_cast<float4*>((seg.prefix ? p.pre_o : p.own_o) + seg.place * rows * D) + at;
         for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
           uint32_t v[32];
           tmem_ld32(tmem + lanes + x, v);
@@ -729,25 +831,26 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
         tc_fence_before();
         quarter_sync(quarter);  // the tiles' exchanges have been read
-        s_half[0][half][row] = l;
+        sh.half[0][half][row] = l;
         quarter_sync(quarter);
         if (valid && half == 0)
-          ((seg.prefix ? p.pre_ml : p.own_ml) + seg.place * rows)[row] =
-              make_float2(m, l + s_half[0][1][row]);
+          ((seg.prefix ? p.pre_ml : p.own_ml) + seg.place * rows)[at] = make_float2(m, l + sh.half[0][1][row]);
         quarter_sync(quarter);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&o_free);
-      if (!seg.prefix && seg.key0 == 0 && row == 0 && half == 0)
-        p.work_item[seg.place - blockIdx.x] = seg.begin;
+      if (lane == 0) arrive_first(o_free0);
+      if (!seg.prefix && seg.key0 == 0 && row == 0 && half == 0 && rank == 0)
+        p.work_item[seg.place - pair] = seg.begin;
     }
   }
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && *abort_flag) raise_device_error(p.err, DERR_TIMEOUT);
+  __syncwarp();
+  cluster_sync();  // neither CTA's memory is used any more
   if (warp == 3) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   }
 }
 
@@ -778,14 +881,15 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
     int n_pre = 0, n_own = 0, pre_row = 0;
     int64_t pre0 = 0, own0 = 0;
     if (p.pre_tiles > 0) {
-      const int qt = t / p.tpt, it = kvh * p.pre_qtiles + qt;
+      const int qt = t / p.tpi, it = kvh * p.pre_qtiles + qt, tl = t - qt * p.tpi, rank = tl >= p.tpc;
       const long long b = (long long)it * pa_units(p.pre_tiles) + PA_ITEM_COST;
       const long long c0 = b / per, c1 = (b + p.pre_tiles - 1) / per;
       n_pre = (int)(c1 - c0) + 1;
       pre0 = it + c0;
-      pre_row = (t - qt * p.tpt) * p.G + gh;
+      pre_row = rank * PA_ROWS + (tl - rank * p.tpc) * p.G + gh;
     }
-    const int own_qt = (t - r.s0) / p.tpt, own_row = (t - r.s0 - own_qt * p.tpt) * p.G + gh;
+    const int own_qt = (t - r.s0) / p.tpi, tl = t - r.s0 - own_qt * p.tpi, rank = tl >= p.tpc;
+    const int own_row = rank * p.own_half + (tl - rank * p.tpc) * p.G + gh;
     const int kt = pa_own_tiles(p, r, own_qt);
     if (kt > 0) {
       const int64_t it = (int64_t)p.work_base[i] + kvh * pa_qtiles(p, r) + own_qt;
@@ -794,7 +898,7 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
       own0 = it + c0;
     }
     auto ml_of = [&](int x) {
-      return x < n_pre ? p.pre_ml[(pre0 + x) * PA_ROWS + pre_row] : p.own_ml[(own0 + x - n_pre) * p.own_rows + own_row];
+      return x < n_pre ? p.pre_ml[(pre0 + x) * 2 * PA_ROWS + pre_row] : p.own_ml[(own0 + x - n_pre) * p.own_rows + own_row];
     };
 #pragma unroll 4
     for (int x = 0; x < n_pre + n_own; ++x) top = fmaxf(top, ml_of(x).x);
@@ -802,7 +906,7 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
     for (int x = 0; x < n_pre + n_own; ++x) {
       const float2 v = ml_of(x);
       const bool pre = x < n_pre;
-      const int rows = pre ? PA_ROWS : p.own_rows;
+      const int rows = pre ? 2 * PA_ROWS : p.own_rows;
       const float4* src = reinterpret_cast<const float4*>((pre ? p.pre_o : p.own_o) +
                                                           (pre ? pre0 + x : own0 + x - n_pre) * rows * D) +
                           (pre ? pre_row : own_row);
@@ -850,7 +954,7 @@ static int launch_prefix_attention(const CUtensorMap (&maps)[4], const PrefixAtt
                    "prefix_combine_kernel");
 }
 
-// 16-bit tensor of 3 to 5 axes with 128B-swizzled boxes of 64 channels. Strides in elements.
+// 16-bit tensor of 3 to 5 axes with swizzled boxes of 64 channels (128-byte lines) or 32 (64). Strides in elements.
 static int paged_map(CUtensorMap* map, const void* base, int dt, int rank, const int64_t* dims, const int64_t* strides,
                      const int* box) {
   EncodeTiled fn = encode_fn();
@@ -861,7 +965,7 @@ static int paged_map(CUtensorMap* map, const void* base, int dt, int rank, const
   for (int i = 0; i + 1 < rank; ++i) s[i] = (cuuint64_t)(dims[i + 1] == 1 ? dims[0] : strides[i]) * 2;
   const CUresult r = fn(map, dt == YSKN_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                         rank, const_cast<void*>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        box[0] == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(YSKN_EINVAL, "prefix_attention: strides that a tensor map cannot hold");
   return YSKN_OK;
@@ -904,7 +1008,7 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(
       !aligned16(d_out) || (q_row | q_head | block_stride | token_stride | head_stride) % 8 ||
       (d_gate && (gate_row | gate_head) % 8))
     return fail(YSKN_EINVAL, "prefix_attention: pointers and strides are multiples of 16 bytes");
-  const int G = n_qh / n_kvh, tpt = PA_ROWS / G;
+  const int G = n_qh / n_kvh, tpc = PA_ROWS / G;
   PrefixAttnParams p{};
   p.gate = reinterpret_cast<const uint16_t*>(d_gate);
   p.gate_row = gate_row, p.gate_head = gate_head;
@@ -913,8 +1017,9 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(
   p.lens = d_lens, p.starts = d_starts;
   p.n_blocks = n_blocks, p.block_shift = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : 7, p.prefix_len = prefix_len;
   p.own_limit = (int)std::min<int64_t>((int64_t)table_width * block_size, INT32_MAX - PA_KEYS);
-  p.batch = batch, p.tokens = tokens, p.max_new = max_new, p.n_kvh = n_kvh, p.G = G, p.tpt = tpt;
-  p.pre_tiles = (int)ceil_div(prefix_len, PA_KEYS), p.pre_qtiles = (int)ceil_div(tokens, tpt);
+  p.batch = batch, p.tokens = tokens, p.max_new = max_new, p.n_kvh = n_kvh, p.G = G;
+  p.tpc = tpc, p.tpi = 2 * tpc;
+  p.pre_tiles = (int)ceil_div(prefix_len, PA_KEYS), p.pre_qtiles = (int)ceil_div(tokens, 2 * tpc);
   const int64_t items = (int64_t)p.pre_qtiles * n_kvh;
   if (items > INT32_MAX / 2) return fail(YSKN_EINVAL, "prefix_attention: too many rows");
   p.pre_items = prefix_len > 0 ? (int)items : 0;
@@ -928,27 +1033,28 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(
   p.work_item = reinterpret_cast<long long*>(work + w.item);
   p.pre_ml = reinterpret_cast<float2*>(work + w.pre_ml), p.pre_o = reinterpret_cast<float*>(work + w.pre_o);
   p.own_ml = reinterpret_cast<float2*>(work + w.own_ml), p.own_o = reinterpret_cast<float*>(work + w.own_o);
-  p.own_rows = w.own_rows, p.own_items = w.own_items;
+  p.own_half = w.own_half, p.own_rows = w.own_rows, p.own_items = w.own_items;
   p.out = reinterpret_cast<uint16_t*>(d_out), p.err = device_error_word();
-  const int v_rows = PA_SLOT / (2 * head);
+  // The cache's 64-channel columns are an axis of their own, so that one box holds several columns
+  // of its rows in the order of the ring's slots; where a slot takes several boxes (blocks
+  // shorter than it), a box is one column.
+  const int slots = head <= 128 ? 1 : head / 128, v_rows = PA_KEYS / slots;
   const int64_t q_dims[3] = {head, n_qh, tokens}, q_strides[2] = {q_head, q_row};
-  const int64_t c_dims[4] = {head, block_size, n_kvh, n_blocks}, c_strides[3] = {token_stride, head_stride, block_stride};
-  const int box_pre[3] = {64, G, tpt}, box_own[3] = {64, G, std::min(tpt, max_new)};
-  // V: the 64-channel columns as an axis of their own, so that one box holds all channels of its
-  // rows in the order of the slot; where a slot takes several boxes, a box is one column
-  const int64_t v_dims[5] = {64, block_size, head / 64, n_kvh, n_blocks};
-  const int64_t v_strides[4] = {token_stride, 64, head_stride, block_stride};
-  const int box_k[4] = {64, block_size, 1, 1};
-  const int box_v[5] = {64, std::min(block_size, v_rows), block_size < v_rows ? 1 : head / 64, 1, 1};
+  const int64_t c_dims[5] = {64, block_size, head / 64, n_kvh, n_blocks};
+  const int64_t c_strides[4] = {token_stride, 64, head_stride, block_stride};
+  const int box_pre[3] = {64, G, tpc}, box_own[3] = {64, G, std::min(tpc, max_new)};
+  const int box_k[5] = {64, std::min(block_size, PA_KEYS / 2), block_size < PA_KEYS / 2 ? 1 : head / 64 / slots, 1, 1};
+  const int box_v[5] = {head == 64 ? 32 : 64, std::min(block_size, v_rows),
+                        block_size < v_rows || head <= 128 ? 1 : head / 128, 1, 1};
   CUtensorMap maps[4];
   if (int rc = paged_map(&maps[0], d_q, dtype, 3, q_dims, q_strides, box_pre)) return rc;
   if (int rc = paged_map(&maps[1], d_q, dtype, 3, q_dims, q_strides, box_own)) return rc;
-  if (int rc = paged_map(&maps[2], d_k_cache, dtype, 4, c_dims, c_strides, box_k)) return rc;
-  if (int rc = paged_map(&maps[3], d_v_cache, dtype, 5, v_dims, v_strides, box_v)) return rc;
-  int dev = 0, sms = PA_MAX_CTAS;
+  if (int rc = paged_map(&maps[2], d_k_cache, dtype, 5, c_dims, c_strides, box_k)) return rc;
+  if (int rc = paged_map(&maps[3], d_v_cache, dtype, 5, c_dims, c_strides, box_v)) return rc;
+  int dev = 0, sms = 2 * PA_MAX_PAIRS;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int grid = std::min(sms, PA_MAX_CTAS);
+  const int grid = 2 * std::min(sms / 2, PA_MAX_PAIRS);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   auto run = [&](auto d) {
     constexpr int D = decltype(d)::value;
