@@ -571,103 +571,136 @@ YSKN_B200_API int yskn_b200_kv_encode(const float* d_rows, const int32_t* d_row_
  * request's own rows (those after the shared prefix) in the blocks that its row of the block
  * tables names in order, the prefix's rows in blocks of its own, held once for the batch.
  * Lengths stay on the device, so a step can be one CUDA graph; host arguments that bound them
- * (max_tokens, max_new) fix the launches' shapes. */
+ * (max_tokens, max_new) fix the launches' shapes. Each call takes its arguments as a struct, read
+ * before it returns; below, a name is the struct's field. */
 #define YSKN_DT_F32 0
 #define YSKN_DT_F16 1
 #define YSKN_DT_BF16 2
 #define YSKN_PLAN_MAX_BATCH 4096
 
 /* Blocks, slots and positions of a step's new tokens. Per request i of `batch`
- * (1..YSKN_PLAN_MAX_BATCH): d_lens[i] its rows in the cache, the prefix's prefix_len counted
- * (0: none yet, not even the prefix), d_new_lens[i] its new tokens: 0 none, negative for an
+ * (1..YSKN_PLAN_MAX_BATCH): lens[i] its rows in the cache, the prefix's prefix_len counted
+ * (0: none yet, not even the prefix), new_lens[i] its new tokens: 0 none, negative for an
  * ended request, whose blocks go back onto the pool and whose length becomes 0.
- *   d_pool        int32 [pool_capacity]: stack of unused block numbers, *d_free of them, the
+ *   pool        int32 [pool_capacity]: stack of unused block numbers, *free of them, the
  *                 top last; blocks given back go on top, new ones come from the top,
  *                 requests in order;
- *   d_block_tables int32 [batch][table_stride], table_width entries used: fresh blocks are
+ *   block_tables int32 [batch][table_stride], table_width entries used: fresh blocks are
  *                 written in place, other entries stay;
  * A request is served if its rows fit its table row, and the pool and max_tokens hold it with
  * all such requests before it; else it gets no tokens and keeps its length (call again when
- * blocks are back). Written: d_lens_out [batch] and *d_free_out (arrays of their own: keep
- * two of each and swap them), d_starts [batch + 1] (served tokens before each request), and
- * per token d_slots int64 (block * block_size + place, for yskn_b200_paged_prep), d_positions
- * and d_requests int32 [max_tokens], -1 past the last served token. Lengths or a count that
+ * blocks are back). Written: lens_out [batch] and *free_out (arrays of their own: keep
+ * two of each and swap them), starts [batch + 1] (served tokens before each request), and
+ * per token slots int64 (block * block_size + place, for yskn_b200_paged_prep), positions
+ * and requests int32 [max_tokens], -1 past the last served token. Lengths or a count that
  * do not fit their arrays give YSKN_EINVAL from yskn_b200_status. One launch. */
-YSKN_B200_API int yskn_b200_batch_plan(const int32_t* d_lens, const int32_t* d_new_lens, int batch, int block_size,
-                                       int prefix_len, int32_t* d_block_tables, int table_width,
-                                       int64_t table_stride, int32_t* d_pool, int pool_capacity,
-                                       const int32_t* d_free, int max_tokens, int32_t* d_lens_out,
-                                       int32_t* d_free_out, int32_t* d_starts, int64_t* d_slots,
-                                       int32_t* d_positions, int32_t* d_requests, void* stream);
+typedef struct {
+  const int32_t *lens, *new_lens; /* [batch] */
+  int32_t* block_tables;
+  int64_t table_stride;
+  int32_t* pool;
+  const int32_t* free;
+  int32_t *lens_out, *free_out, *starts;
+  int64_t* slots;
+  int32_t *positions, *requests;
+  int batch, block_size, prefix_len, table_width, pool_capacity, max_tokens;
+} yskn_b200_batch_plan_args;
+YSKN_B200_API int yskn_b200_batch_plan(const yskn_b200_batch_plan_args* args, void* stream);
 
 /* Query and key heads normalised and rotated, new keys and values into the cache. Projection
- * rows d_q, d_k, d_v of `source` type (YSKN_DT_F32, or the cache's dtype): element (token,
- * head, channel) at token * row + head * head_stride + channel (strides in elements; a query
+ * rows q, k, v of `source` type (YSKN_DT_F32, or the cache's dtype): element (token,
+ * head, channel) at token * row + head * the head's stride + channel (strides in elements; a query
  * head inside a [query | gate] pair is a row of twice its size). Heads of `head` = 64, 128 or
  * 256 channels. In binary32, rounded once: queries and keys x * rsqrt(mean(x^2) + eps) * (1 + w)
- * (bf16 d_q_norm, d_k_norm [head]; NULL: as they are), then the first rot channels (a multiple
- * of 16; 0: none) rotated in pairs i, i + rot / 2 by float(position) * d_inv_freq[i] (f32
- * [rot / 2]), the position from axis h_axes[i] (host, 0..2) of d_positions int32
+ * (bf16 q_norm, k_norm [head]; NULL: as they are), then the first rot channels (a multiple
+ * of 16; 0: none) rotated in pairs i, i + rot / 2 by float(position) * inv_freq[i] (f32
+ * [rot / 2]), the position from axis axes[i] (0..2, below n_axes) of positions int32
  * [axes][position_stride]: one axis for text, three (time, height, width) for images and
- * video. d_query: dense [tokens][n_qh][head] of type dtype (YSKN_DT_F16 or _BF16). The caches
+ * video. query: dense [tokens][n_qh][head] of type dtype (YSKN_DT_F16 or _BF16). The caches
  * hold n_blocks blocks, element (block, place, KV head, channel) at block * block_stride +
  * place * token_stride + head * head_stride + channel for both; a token's row goes to
- * d_slots[token] (block * block_size + place). A negative slot is a padded token: no cache row,
+ * slots[token] (block * block_size + place). A negative slot is a padded token: no cache row,
  * a zero query; a slot past the cache gives YSKN_EINVAL from yskn_b200_status. Pointers and
  * strides are multiples of 16 bytes. */
-YSKN_B200_API int yskn_b200_paged_prep(const void* d_q, int64_t q_row, int64_t q_head, const void* d_k, int64_t k_row,
-                                       int64_t k_head, const void* d_v, int64_t v_row, int64_t v_head, int source,
-                                       const int64_t* d_slots, const int32_t* d_positions, int64_t position_stride,
-                                       const float* d_inv_freq, const uint8_t* h_axes, int rot,
-                                       const uint16_t* d_q_norm, const uint16_t* d_k_norm, float eps, int tokens,
-                                       int n_qh, int n_kvh, int head, void* d_query, void* d_k_cache,
-                                       void* d_v_cache, int64_t block_stride, int64_t token_stride,
-                                       int64_t head_stride, int n_blocks, int block_size, int dtype, void* stream);
+#define YSKN_MAX_PAIRS 128
+typedef struct {
+  const void *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  const int64_t* slots;       /* [tokens] */
+  const int32_t* positions;   /* [n_axes][position_stride] */
+  int64_t position_stride;
+  const float* inv_freq;      /* [rot / 2] */
+  const uint16_t *q_norm, *k_norm;
+  void *query, *k_cache, *v_cache;
+  int64_t block_stride, token_stride, head_stride;
+  int tokens, n_qh, n_kvh, head, rot, n_axes, n_blocks, block_size, source, dtype;
+  float eps;
+  uint8_t axes[YSKN_MAX_PAIRS]; /* of the first rot / 2 pairs */
+} yskn_b200_paged_prep_args;
+YSKN_B200_API int yskn_b200_paged_prep(const yskn_b200_paged_prep_args* args, void* stream);
 
 /* Attention of the batch's new tokens over the shared prefix and each request's own rows.
- * Request i's tokens are d_starts[i] .. d_starts[i + 1] - 1 of `tokens` (rows past
- * d_starts[batch] are padding), at most max_new, and the last of its d_lens[i] rows; token t of
- * n sees the first max(0, len - n + t + 1) rows: below prefix_len in d_prefix_blocks
+ * Request i's tokens are starts[i] .. starts[i + 1] - 1 of `tokens` (rows past
+ * starts[batch] are padding), at most max_new, and the last of its lens[i] rows; token t of
+ * n sees the first max(0, len - n + t + 1) rows: below prefix_len in prefix_blocks
  * int32 [ceil(prefix_len / block_size)], from there on in the request's row of
- * d_block_tables. out = softmax(scale * q k^T) v in binary32 sums, times sigmoid(gate) if
- * d_gate is given, rounded once; a token that sees nothing, padding included, gives zeros.
- * Cache rows that no token sees may hold anything. d_q, d_gate: element (token, head, channel)
- * at token * row + head * head_stride + channel; d_out dense [tokens][n_qh][head]; query head
+ * block_tables. out = softmax(scale * q k^T) v in binary32 sums, times sigmoid(gate) if
+ * gate is given, rounded once; a token that sees nothing, padding included, gives zeros.
+ * Cache rows that no token sees may hold anything. q, gate: element (token, head, channel)
+ * at token * row + head * head_stride + channel; out dense [tokens][n_qh][head]; query head
  * j reads KV head j / (n_qh / n_kvh), at most 128 query heads each. dtype YSKN_DT_F16 or
  * _BF16 for all of them (the softmax weights are rounded to it for the tensor cores); heads of
  * 64, 128 or 256 channels; blocks of 16, 32, 64 or 128 rows; the cache's strides as in
  * yskn_b200_paged_prep. Pointers and strides are multiples of 16 bytes. A block number outside
  * the cache or a request of more than max_new tokens gives YSKN_EINVAL from
- * yskn_b200_status. d_work: yskn_b200_prefix_attention_work_bytes() bytes, one call's at a time. */
+ * yskn_b200_status. work: work_bytes of
+ * memory, at least yskn_b200_prefix_attention_work_bytes(), one call's at a time. */
 YSKN_B200_API int64_t yskn_b200_prefix_attention_work_bytes(int tokens, int batch, int max_new, int n_qh, int n_kvh,
                                                             int head);
-YSKN_B200_API int yskn_b200_prefix_attention(const void* d_q, int64_t q_row, int64_t q_head, const void* d_gate,
-                                             int64_t gate_row, int64_t gate_head, const void* d_k_cache,
-                                             const void* d_v_cache, int64_t block_stride, int64_t token_stride,
-                                             int64_t head_stride, int n_blocks, int block_size,
-                                             const int32_t* d_prefix_blocks, int prefix_len,
-                                             const int32_t* d_block_tables, int table_width, int64_t table_stride,
-                                             const int32_t* d_lens, const int32_t* d_starts, int batch, int tokens,
-                                             int max_new, int n_qh, int n_kvh, int head, int dtype, float scale,
-                                             void* d_work, void* d_out, void* stream);
+typedef struct {
+  const void* q;
+  int64_t q_row, q_head;
+  const void* gate;
+  int64_t gate_row, gate_head;
+  const void *k_cache, *v_cache;
+  int64_t block_stride, token_stride, head_stride;
+  const int32_t *prefix_blocks, *block_tables;
+  int64_t table_stride;
+  const int32_t *lens, *starts; /* [batch], [batch + 1] */
+  void* work;
+  int64_t work_bytes;
+  void* out;
+  int n_blocks, block_size, prefix_len, table_width, batch, tokens, max_new, n_qh, n_kvh, head, dtype;
+  float scale;
+} yskn_b200_prefix_attention_args;
+YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_attention_args* args, void* stream);
 
 /* Penalties for repeated tokens, biases and a grammar mask on f32 logits [rows][vocab] (row
- * strides in elements; d_out may be d_logits). Per row, in binary32: a token of the history
- * (int32 d_history [rows][history_stride], d_history_lens[row] of history_width entries) has
- * its logit divided by d_repetition[row] if positive, else multiplied by it; then frequency *
- * c and, if c > 0, presence are subtracted, c its count from entry d_prompt_lens[row] on (NULL:
- * 0); then the bias of its last entry in d_bias_ids / d_bias [rows][n_bias] is added; a token
- * whose bit (bit id % 32 of word id / 32) in d_mask uint32 [rows][mask_stride] is 0 becomes
+ * strides in elements; out may be logits). Per row, in binary32: a token of the history
+ * (int32 history [rows][history_stride], history_lens[row] of history_width entries) has
+ * its logit divided by repetition[row] if positive, else multiplied by it; then frequency *
+ * c and, if c > 0, presence are subtracted, c its count from entry prompt_lens[row] on (NULL:
+ * 0); then the bias of its last entry in bias_ids / bias [rows][n_bias] is added; a token
+ * whose bit (bit id % 32 of word id / 32) in mask uint32 [rows][mask_stride] is 0 becomes
  * -inf. NULL leaves a step out; ids outside the vocabulary (padding) count for nothing. A row
  * that allows nothing is -inf throughout, for which yskn_b200_head_select answers no token.
  * rows <= 65535. A history longer than its width gives YSKN_EINVAL from yskn_b200_status. */
-YSKN_B200_API int yskn_b200_logits_adjust(const float* d_logits, int64_t logits_stride, int rows, int vocab,
-                                          const int32_t* d_history, int64_t history_stride, int history_width,
-                                          const int32_t* d_history_lens, const int32_t* d_prompt_lens,
-                                          const float* d_repetition, const float* d_presence,
-                                          const float* d_frequency, const int32_t* d_bias_ids, const float* d_bias,
-                                          int n_bias, const uint32_t* d_mask, int64_t mask_stride, float* d_out,
-                                          int64_t out_stride, void* stream);
+typedef struct {
+  const float* logits;
+  int64_t logits_stride;
+  const int32_t* history;
+  int64_t history_stride;
+  const int32_t *history_lens, *prompt_lens;
+  const float *repetition, *presence, *frequency;
+  const int32_t* bias_ids;
+  const float* bias;
+  const uint32_t* mask;
+  int64_t mask_stride;
+  float* out;
+  int64_t out_stride;
+  int rows, vocab, history_width, n_bias;
+} yskn_b200_logits_adjust_args;
+YSKN_B200_API int yskn_b200_logits_adjust(const yskn_b200_logits_adjust_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -7,17 +7,19 @@ P = 4096  # stands for a device pointer; 16-byte aligned
 
 def _check(name, good, bad):
     import yskn_b200 as Y
-    fn = getattr(Y.lib(), name)
+    fn, args_of = getattr(Y.lib(), name), Y.ARGS[name.replace("yskn_b200_", "")]
+    assert fn(None, None) == Y.EINVAL
     for i, change in enumerate(bad):
         args = dict(good, **change)
         assert list(args) == list(good)
-        assert fn(*args.values()) == Y.EINVAL, (name, i, change)
+        packed = args_of.pack(*(0 if v is None else v for v in args.values()))
+        assert fn(packed, None) == Y.EINVAL, (name, i, change)
         assert name.replace("yskn_b200_", "") in Y.last_error()
 
 
 def test_batch_plan():
-    good = dict(lens=P, new=P, batch=2, block=16, prefix=0, tables=P, width=4, stride=4, pool=P, capacity=9, free=P,
-                tokens=5, lens_out=2 * P, free_out=2 * P, starts=P, slots=P, positions=P, requests=P, stream=None)
+    good = dict(lens=P, new=P, tables=P, stride=4, pool=P, free=P, lens_out=2 * P, free_out=2 * P, starts=P, slots=P,
+                positions=P, requests=P, batch=2, block=16, prefix=0, width=4, capacity=9, tokens=5)
     _check("yskn_b200_batch_plan", good,
            [{k: None} for k in ("lens", "new", "tables", "pool", "free", "lens_out", "free_out", "starts", "slots",
                                 "positions", "requests")] +
@@ -26,32 +28,33 @@ def test_batch_plan():
 
 
 def test_paged_prep():
-    good = dict(q=P, q_row=512, q_head=128, k=P, k_row=256, k_head=128, v=P, v_row=256, v_head=128, source=0, slots=P,
-                positions=P, position_stride=4, freq=P, axes=bytes(32), rot=64, q_norm=P, k_norm=P, eps=1e-6, tokens=4,
-                n_qh=4, n_kvh=2, head=128, query=P, k_cache=P, v_cache=P, block=4096, token=128, head_stride=2048,
-                n_blocks=3, block_size=16, dtype=2, stream=None)
+    good = dict(q=P, k=P, v=P, q_row=512, q_head=128, k_row=256, k_head=128, v_row=256, v_head=128, slots=P,
+                positions=P, position_stride=4, freq=P, q_norm=P, k_norm=P, query=P, k_cache=P, v_cache=P, block=4096,
+                token=128, head_stride=2048, tokens=4, n_qh=4, n_kvh=2, head=128, rot=64, n_axes=3, n_blocks=3,
+                block_size=16, source=0, dtype=2, eps=1e-6, axes=bytes(32))
     _check("yskn_b200_paged_prep", good,
-           [{k: None} for k in ("q", "k", "v", "slots", "positions", "freq", "axes", "query", "k_cache", "v_cache")] +
+           [{k: None} for k in ("q", "k", "v", "slots", "positions", "freq", "query", "k_cache", "v_cache")] +
            [{k: P + 8} for k in ("q", "k", "v", "query", "k_cache", "v_cache", "q_norm", "k_norm")] +
            [dict(head=96), dict(head=512), dict(dtype=0), dict(dtype=3), dict(source=1), dict(source=7),
             dict(tokens=0), dict(n_qh=0), dict(n_kvh=0), dict(rot=-16), dict(rot=144), dict(rot=24),
-            dict(axes=bytes([3]) * 32), dict(q_row=514), dict(k_head=130), dict(block=4), dict(token=4),
+            dict(axes=bytes([3]) * 32, n_axes=4), dict(axes=bytes([1]) * 32, n_axes=1), dict(q_row=514), dict(k_head=130), dict(block=4), dict(token=4),
             dict(head_stride=4), dict(n_blocks=0), dict(block_size=0)])
 
 
 def test_prefix_attention():
     import yskn_b200 as Y
     good = dict(q=P, q_row=512, q_head=128, gate=None, gate_row=0, gate_head=0, k=P, v=P, block=4096, token=128,
-                head_stride=2048, n_blocks=3, block_size=16, prefix_blocks=P, prefix=20, tables=P, width=2, stride=2,
-                lens=P, starts=P, batch=2, tokens=3, max_new=2, n_qh=4, n_kvh=2, head=128, dtype=2, scale=0.1, work=P,
-                out=P, stream=None)
+                head_stride=2048, prefix_blocks=P, tables=P, stride=2, lens=P, starts=P, work=P, work_bytes=1 << 30,
+                out=P, n_blocks=3, block_size=16, prefix=20, width=2, batch=2, tokens=3, max_new=2, n_qh=4, n_kvh=2,
+                head=128, dtype=2, scale=0.1)
     _check("yskn_b200_prefix_attention", good,
            [{k: None} for k in ("q", "k", "v", "prefix_blocks", "tables", "lens", "starts", "work", "out")] +
            [{k: P + 8} for k in ("q", "gate", "k", "v", "work", "out")] +
            [dict(head=96), dict(dtype=0), dict(dtype=3), dict(tokens=0), dict(batch=0), dict(max_new=0), dict(n_kvh=0),
             dict(n_kvh=3), dict(n_qh=258), dict(prefix=-1), dict(width=0), dict(stride=1), dict(n_blocks=0),
             dict(block_size=8), dict(block_size=48), dict(block_size=256), dict(q_row=516), dict(q_head=4),
-            dict(block=4), dict(token=4), dict(head_stride=4), dict(gate=P, gate_row=4)])
+            dict(block=4), dict(token=4), dict(head_stride=4), dict(gate=P, gate_row=4),
+            dict(work_bytes=Y.prefix_attention_work_bytes(3, 2, 2, 4, 2, 128) - 1)])
     L = Y.lib()
     assert L.yskn_b200_prefix_attention_work_bytes(3, 2, 2, 4, 2, 128) > 0
     for args in [(0, 2, 2, 4, 2, 128), (3, 0, 2, 4, 2, 128), (3, 2, 0, 4, 2, 128), (3, 2, 2, 5, 2, 128),
@@ -62,9 +65,9 @@ def test_prefix_attention():
 
 
 def test_logits_adjust():
-    good = dict(logits=P, logits_stride=100, rows=2, vocab=100, history=P, history_stride=10, width=10, lens=P,
-                prompts=None, rep=P, pres=None, freq=None, ids=P, bias=P, n_bias=3, mask=P, mask_stride=4, out=P,
-                out_stride=100, stream=None)
+    good = dict(logits=P, logits_stride=100, history=P, history_stride=10, lens=P, prompts=None, rep=P, pres=None,
+                freq=None, ids=P, bias=P, mask=P, mask_stride=4, out=P, out_stride=100, rows=2, vocab=100, width=10,
+                n_bias=3)
     _check("yskn_b200_logits_adjust", good,
            [{k: None} for k in ("logits", "lens", "ids", "bias", "out")] +
            [dict(rows=0), dict(rows=65536), dict(vocab=0), dict(vocab=2 ** 31 - 1), dict(logits_stride=99),
@@ -81,9 +84,12 @@ def test_tensor_checks_of_the_binding():
     bf = lambda *s: torch.zeros(s, dtype=torch.bfloat16)  # noqa: E731
     f32 = lambda *s: torch.zeros(s)  # noqa: E731
 
+    class Stream:  # the legacy default stream; what the C entry refuses never gets to it
+        cuda_stream = 0
+
     def refused(fn, *a, **k):
         with pytest.raises(Y.YsknError) as e:
-            fn(*a, **k)
+            fn(*a, stream=Stream, **k)
         assert e.value.code == Y.EINVAL
 
     plan = lambda **k: [dict(dict(lens=i32(2), new=i32(2), tables=i32(2, 3), pool=i32(4), free=i32(1), bs=16,  # noqa: E731
@@ -106,7 +112,7 @@ def test_tensor_checks_of_the_binding():
     att = lambda **k: Y.prefix_attention(*[dict(dict(q=qa, kc=c, vc=c, tb=i32(2, 3), ln=i32(2), st=i32(3), mn=2,  # noqa: E731
                                                      wk=work, out=bf(3, 4, 64)), **k)[x]
                                            for x in ("q", "kc", "vc", "tb", "ln", "st", "mn", "wk", "out")],
-                                         **{x: y for x, y in k.items() if x in ("gate", "prefix_blocks", "prefix_len")})
+                                         **{x: y for x, y in k.items() if x in ("gate", "prefix_blocks", "prefix_len", "stream")})
     refused(att, q=qa.to(torch.float16))
     refused(att, st=i32(2))
     refused(att, tb=i64(2, 3))

@@ -67,17 +67,19 @@ struct PlanRequest {
 __device__ __forceinline__ PlanRequest plan_request(const PlanParams& p, int i) {
   PlanRequest r{};
   const int len = __ldg(p.lens + i), n = __ldg(p.new_lens + i);
+  const unsigned bs = p.block_size;
   r.len = len;
-  r.rows = max(len - p.prefix_len, 0);
-  r.held = (int)(((int64_t)r.rows + p.block_size - 1) / p.block_size);
+  r.rows = len > p.prefix_len ? len - p.prefix_len : 0;
+  r.held = (int)((unsigned)r.rows / bs + ((unsigned)r.rows % bs != 0));
   r.ended = n < 0;
   r.too_long = r.held > p.table_width;
   if (r.ended) r.back = min(r.held, p.table_width);
-  if (n > 0) {
-    const int64_t total = ((int64_t)r.rows + n + p.block_size - 1) / p.block_size;
+  if (n > 0 && r.rows <= INT32_MAX - n) {
+    const unsigned end = (unsigned)(r.rows + n);
+    const int total = (int)(end / bs + (end % bs != 0));
     if (total <= p.table_width) {
       r.n = n;
-      r.fresh = (int)total - r.held;
+      r.fresh = total - r.held;
     }
   }
   return r;
@@ -97,25 +99,32 @@ __device__ __forceinline__ int last_at_most(const int* a, int n, int v) {
 __global__ void __launch_bounds__(PLAN_THREADS) batch_plan_kernel(const __grid_constant__ PlanParams p) {
   extern __shared__ int s_plan[];
   const int B = p.batch;
-  int* s_start = s_plan;               // [B + 1] first token of each request
-  int* s_back = s_start + B + 1;       // [B + 1] blocks given back before each request
-  int* s_need = s_back + B + 1;        // [B] fresh blocks taken before each request
+  int* s_start = s_plan;               // [B + 1] tokens, then first token, of each request
+  int* s_back = s_start + B + 1;       // [B + 1] blocks given back, then those before each request
+  int* s_need = s_back + B + 1;        // [B] fresh blocks, then those taken before each request
   int* s_rows = s_need + B;            // [B]
   __shared__ Sum3 s_warp[PLAN_WARPS];
   __shared__ Sum3 s_served;            // sums over the served requests
   __shared__ int s_any_long;
   pdl_begin();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int count = __ldg(p.free_count);
+  if (tid == 0) s_served = {0, 0, 0}, s_any_long = 0;
+  __syncthreads();
+  for (int i = tid; i < B; i += PLAN_THREADS) {
+    const PlanRequest r = plan_request(p, i);
+    s_start[i] = r.n;
+    s_back[i] = r.back;
+    s_need[i] = r.fresh;
+    s_rows[i] = r.rows;
+    if (r.too_long) s_any_long = 1;
+    if (blockIdx.x == 0) p.lens_out[i] = r.ended ? 0 : r.len;  // served ones below
+  }
+  __syncthreads();
   const int per = (B + PLAN_THREADS - 1) / PLAN_THREADS;
   const int i0 = min(B, tid * per), i1 = min(B, i0 + per);
-  if (tid == 0) s_served = {0, 0, 0}, s_any_long = 0;
   Sum3 mine{0, 0, 0};
-  bool too_long = false;
-  for (int i = i0; i < i1; ++i) {
-    const PlanRequest r = plan_request(p, i);
-    mine = mine + Sum3{r.back, r.fresh, r.n};
-    too_long |= r.too_long;
-  }
+  for (int i = i0; i < i1; ++i) mine = mine + Sum3{s_back[i], s_need[i], s_start[i]};
   Sum3 incl = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -125,7 +134,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) batch_plan_kernel(const __grid_c
   }
   if (lane == 31) s_warp[warp] = incl;
   __syncthreads();
-  if (too_long) s_any_long = 1;
   Sum3 before{incl.back - mine.back, incl.need - mine.need, incl.tokens - mine.tokens};
   long long back_total = 0;
   for (int w = 0; w < PLAN_WARPS; ++w) {
@@ -133,23 +141,20 @@ __global__ void __launch_bounds__(PLAN_THREADS) batch_plan_kernel(const __grid_c
     if (w < warp) before = before + o;
     back_total += o.back;
   }
-  const int count = __ldg(p.free_count);
   const int free0 = min(max(count, 0), p.pool_capacity);
   const long long have = free0 + back_total;
   // Served requests: both sums only grow, so the last served one's end is their total.
   Sum3 run = before, end{0, 0, 0};
   for (int i = i0; i < i1; ++i) {
-    const PlanRequest r = plan_request(p, i);
-    const Sum3 next = run + Sum3{r.back, r.fresh, r.n};
-    const bool served = r.n > 0 && next.need <= have && next.tokens <= p.max_tokens;
+    const int n = s_start[i];
+    const Sum3 next = run + Sum3{s_back[i], s_need[i], n};
+    const bool served = n > 0 && next.need <= have && next.tokens <= p.max_tokens;
     if (served) end = next;
     s_back[i] = (int)run.back;
     s_need[i] = (int)min(run.need, (long long)INT32_MAX);
-    s_rows[i] = r.rows;
     s_start[i] = (int)min(run.tokens, (long long)INT32_MAX);  // cut at the served total below
-    if (blockIdx.x == 0)
-      p.lens_out[i] = r.ended ? 0 : served ? (int)min((long long)max(r.len, p.prefix_len) + r.n, (long long)INT32_MAX)
-                                           : r.len;
+    if (served && blockIdx.x == 0)
+      p.lens_out[i] = (int)min((long long)max(__ldg(p.lens + i), p.prefix_len) + n, (long long)INT32_MAX);
     run = next;
   }
   if (end.tokens > 0) {
@@ -189,8 +194,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) batch_plan_kernel(const __grid_c
     }
     const int i = last_at_most(s_start, B, t);
     const int rows = s_rows[i], row = rows + (t - s_start[i]);
-    const int held = (int)(((int64_t)rows + p.block_size - 1) / p.block_size);
-    const int b = row / p.block_size, place = row - b * p.block_size;
+    const unsigned bs = p.block_size;
+    const int held = (int)((unsigned)rows / bs + ((unsigned)rows % bs != 0));
+    const int b = (int)((unsigned)row / bs), place = row - b * (int)bs;
     int32_t* entry = p.tables + (int64_t)i * p.table_stride + b;
     int block;
     if (b < held) {
@@ -209,30 +215,26 @@ __global__ void __launch_bounds__(PLAN_THREADS) batch_plan_kernel(const __grid_c
 
 using namespace yskn;
 
-extern "C" YSKN_B200_API int yskn_b200_batch_plan(const int32_t* d_lens, const int32_t* d_new_lens, int batch,
-                                                 int block_size, int prefix_len, int32_t* d_block_tables,
-                                                 int table_width, int64_t table_stride, int32_t* d_pool,
-                                                 int pool_capacity, const int32_t* d_free, int max_tokens,
-                                                 int32_t* d_lens_out, int32_t* d_free_out, int32_t* d_starts,
-                                                 int64_t* d_slots, int32_t* d_positions, int32_t* d_requests,
-                                                 void* stream) {
-  if (!d_lens || !d_new_lens || !d_block_tables || !d_pool || !d_free || !d_lens_out || !d_free_out || !d_starts ||
-      (max_tokens > 0 && (!d_slots || !d_positions || !d_requests)))
+extern "C" YSKN_B200_API int yskn_b200_batch_plan(const yskn_b200_batch_plan_args* args, void* stream) {
+  if (!args) return fail(YSKN_EINVAL, "batch_plan: null argument");
+  const yskn_b200_batch_plan_args& a = *args;
+  if (!a.lens || !a.new_lens || !a.block_tables || !a.pool || !a.free || !a.lens_out || !a.free_out || !a.starts ||
+      (a.max_tokens > 0 && (!a.slots || !a.positions || !a.requests)))
     return fail(YSKN_EINVAL, "batch_plan: null argument");
-  if (batch < 1 || batch > YSKN_PLAN_MAX_BATCH || block_size < 1 || prefix_len < 0 || table_width < 1 ||
-      (batch > 1 && table_stride < table_width) || pool_capacity < 1 || max_tokens < 0)
+  if (a.batch < 1 || a.batch > YSKN_PLAN_MAX_BATCH || a.block_size < 1 || a.prefix_len < 0 || a.table_width < 1 ||
+      (a.batch > 1 && a.table_stride < a.table_width) || a.pool_capacity < 1 || a.max_tokens < 0)
     return fail(YSKN_EINVAL, "batch_plan: batch outside 1..4096, or a size or stride out of range");
-  if (d_lens_out == d_lens || d_free_out == d_free)
+  if (a.lens_out == a.lens || a.free_out == a.free)
     return fail(YSKN_EINVAL, "batch_plan: the new lengths and the new count need arrays of their own");
-  PlanParams p{d_lens, d_new_lens, d_block_tables, table_stride, table_width, d_pool, pool_capacity, d_free, batch,
-               block_size, prefix_len, max_tokens, d_lens_out, d_free_out, d_starts, d_slots, d_positions, d_requests,
-               device_error_word()};
-  const size_t smem = (4 * (size_t)batch + 2) * sizeof(int);
+  PlanParams p{a.lens, a.new_lens, a.block_tables, a.table_stride, a.table_width, a.pool, a.pool_capacity, a.free,
+               a.batch, a.block_size, a.prefix_len, a.max_tokens, a.lens_out, a.free_out, a.starts, a.slots,
+               a.positions, a.requests, device_error_word()};
+  const size_t smem = (4 * (size_t)a.batch + 2) * sizeof(int);
   static SmemOptIn opt_in;
   if (cudaError_t e = opt_in(batch_plan_kernel, (4 * YSKN_PLAN_MAX_BATCH + 2) * sizeof(int)))
     return cuda_fail(e, "batch_plan_kernel attributes");
-  const int64_t items = std::max<int64_t>(max_tokens, 1);
-  const int grid = (int)std::min<int64_t>(ceil_div(items, 4 * PLAN_THREADS), 296);
+  // Four tokens a thread, at most two CTAs an SM: more only repeat the prefix sums.
+  const int grid = (int)std::min<int64_t>(ceil_div(std::max(a.max_tokens, 1), 4 * PLAN_THREADS), 296);
   return cuda_fail(launch_pdl(batch_plan_kernel, grid, PLAN_THREADS, smem, reinterpret_cast<cudaStream_t>(stream), p),
                    "batch_plan_kernel");
 }

@@ -15,8 +15,9 @@
 // heads of 256 from f32). So one warp holds one head row in registers, lane l the channels
 // V l .. V l + V - 1 (V = D / 32): 16-byte accesses, the sum of squares by shuffles, and a
 // pair's other half R / 2 channels away is V-aligned in another lane, one shuffle per
-// channel. A CTA's 8 warps are 8 heads of one token: its R / 2 cosines and sines are computed
-// once (shared memory) while the rows' loads are in flight.
+// channel. A CTA's 8 warps are 8 heads of one token, or 32 (four a warp) from PP_MANY rows on:
+// the token's R / 2 cosines and sines are computed once per CTA (shared memory) while the
+// rows' loads are in flight.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -24,7 +25,8 @@
 namespace yskn {
 
 constexpr int PP_WARPS = 8;
-constexpr int PP_MAX_PAIRS = 128;
+constexpr int PP_MAX_PAIRS = YSKN_MAX_PAIRS;
+constexpr int PP_MANY = 16384;  // head rows of a call from which a warp takes four
 
 struct PagedPrepParams {
   const void *q, *k, *v;
@@ -89,26 +91,28 @@ __device__ __forceinline__ void store_row(uint16_t* p, const float (&x)[V]) {
   else *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <int SRC, int DT, int V>
+template <int SRC, int DT, int V, int R>
 __global__ void __launch_bounds__(PP_WARPS * 32) paged_prep_kernel(const __grid_constant__ PagedPrepParams p) {
   constexpr int D = 32 * V;
   __shared__ float s_cos[PP_MAX_PAIRS], s_sin[PP_MAX_PAIRS];
   pdl_begin();
   const int lane = threadIdx.x & 31;
   const int heads = p.n_qh + 2 * p.n_kvh;  // query heads, then key heads, then value heads
-  const int groups = (heads + PP_WARPS - 1) / PP_WARPS;
-  const int t = blockIdx.x / groups, h = (blockIdx.x - t * groups) * PP_WARPS + (threadIdx.x >> 5);
-  const int kind = h < p.n_qh ? 0 : (h < p.n_qh + p.n_kvh ? 1 : 2);  // query, key, value
-  const int hh = kind == 0 ? h : (kind == 1 ? h - p.n_qh : h - p.n_qh - p.n_kvh);
-  const bool live = h < heads;
-  float x[V];
+  const int groups = (heads + PP_WARPS * R - 1) / (PP_WARPS * R);
+  const int t = blockIdx.x / groups, h0 = (blockIdx.x - t * groups) * PP_WARPS * R + (threadIdx.x >> 5);
+  // kind: 0 query, 1 key, 2 value; hh the head among its kind
+  auto kind_of = [&](int h) { return h < p.n_qh ? 0 : (h < p.n_qh + p.n_kvh ? 1 : 2); };
+  auto head_of = [&](int h, int kind) { return kind == 0 ? h : (kind == 1 ? h - p.n_qh : h - p.n_qh - p.n_kvh); };
+  float x[R][V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) x[j] = 0.0f;
-  if (live) {
+  for (int r = 0; r < R; ++r) {
+    const int h = h0 + r * PP_WARPS;
+    if (h >= heads) break;
+    const int kind = kind_of(h), hh = head_of(h, kind);
     const void* src = kind == 0 ? p.q : (kind == 1 ? p.k : p.v);
     const int64_t row = kind == 0 ? p.q_row : (kind == 1 ? p.k_row : p.v_row);
     const int64_t head = kind == 0 ? p.q_head : (kind == 1 ? p.k_head : p.v_head);
-    load_row<SRC, V>(src, t * row + hh * head + lane * V, x);
+    load_row<SRC, V>(src, t * row + hh * head + lane * V, x[r]);
   }
   const int64_t slot = __ldg(p.slots + t);
   const int half = p.rot >> 1;
@@ -120,113 +124,119 @@ __global__ void __launch_bounds__(PP_WARPS * 32) paged_prep_kernel(const __grid_
     s_sin[threadIdx.x] = sn;
   }
   __syncthreads();
-  if (!live) return;
-  if (kind != 2) {
-    const uint16_t* w = kind == 0 ? p.q_norm : p.k_norm;
-    if (w) {
-      float sum = 0.0f;
+  const int lanes = half / V;  // lanes of each half of the rotated channels
+  const bool low = lane < lanes, rotated = lane < 2 * lanes;
+  const int other = rotated ? (low ? lane + lanes : lane - lanes) : lane;
+  const int i0 = rotated ? (low ? lane : lane - lanes) * V : 0;
+  const int64_t block = slot >= 0 ? slot / p.block_size : 0, place = slot - block * p.block_size;
+  const int64_t to = block * p.cache.block + place * p.cache.token + lane * V;
+  if (slot >= p.n_slots && threadIdx.x == 0) raise_device_error(p.err, DERR_RANGE);
 #pragma unroll
-      for (int j = 0; j < V; ++j) sum = fmaf(x[j], x[j], sum);
+  for (int r = 0; r < R; ++r) {
+    const int h = h0 + r * PP_WARPS;
+    if (h >= heads) break;
+    const int kind = kind_of(h), hh = head_of(h, kind);
+    if (kind != 2) {
+      const uint16_t* w = kind == 0 ? p.q_norm : p.k_norm;
+      if (w) {
+        float sum = 0.0f;
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-      const float inv = rsqrtf(sum * (1.0f / D) + p.eps);
-      float wt[V];
-      load_row<YSKN_DT_BF16, V>(w, lane * V, wt);
+        for (int j = 0; j < V; ++j) sum = fmaf(x[r][j], x[r][j], sum);
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[j] = x[j] * inv * (1.0f + wt[j]);
-    }
-    if (p.rot) {
-      const int lanes = half / V;  // lanes of each half of the rotated channels
-      const bool low = lane < lanes, rotated = lane < 2 * lanes;
-      const int other = rotated ? (low ? lane + lanes : lane - lanes) : lane;
-      const int i0 = rotated ? (low ? lane : lane - lanes) * V : 0;
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        const float inv = rsqrtf(sum * (1.0f / D) + p.eps);
+        float wt[V];
+        load_row<YSKN_DT_BF16, V>(w, lane * V, wt);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float o = __shfl_sync(0xffffffffu, x[j], other);
-        const float cs = s_cos[i0 + j], sn = s_sin[i0 + j];
-        if (rotated) x[j] = low ? fmaf(x[j], cs, -(o * sn)) : fmaf(x[j], cs, o * sn);
+        for (int j = 0; j < V; ++j) x[r][j] = x[r][j] * inv * (1.0f + wt[j]);
+      }
+      if (p.rot) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float o = __shfl_sync(0xffffffffu, x[r][j], other);
+          const float cs = s_cos[i0 + j], sn = s_sin[i0 + j];
+          if (rotated) x[r][j] = low ? fmaf(x[r][j], cs, -(o * sn)) : fmaf(x[r][j], cs, o * sn);
+        }
       }
     }
-  }
-  if (kind == 0) {
-    if (slot < 0) {
+    if (kind == 0) {
+      if (slot < 0) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[j] = 0.0f;
+        for (int j = 0; j < V; ++j) x[r][j] = 0.0f;
+      }
+      store_row<DT, V>(p.query + ((int64_t)t * p.n_qh + hh) * D + lane * V, x[r]);
+    } else if (slot >= 0 && slot < p.n_slots) {
+      store_row<DT, V>((kind == 1 ? p.k_cache : p.v_cache) + to + hh * p.cache.head, x[r]);
     }
-    store_row<DT, V>(p.query + ((int64_t)t * p.n_qh + hh) * D + lane * V, x);
-  } else if (slot >= 0) {
-    if (slot >= p.n_slots) {
-      if (lane == 0) raise_device_error(p.err, DERR_RANGE);
-      return;
-    }
-    const int64_t block = slot / p.block_size, place = slot - block * p.block_size;
-    uint16_t* cache = kind == 1 ? p.k_cache : p.v_cache;
-    store_row<DT, V>(cache + block * p.cache.block + place * p.cache.token + hh * p.cache.head + lane * V, x);
   }
 }
 
-template <int SRC, int DT>
-static cudaError_t launch_paged_prep(const PagedPrepParams& p, int head, unsigned grid, cudaStream_t st) {
+template <int SRC, int DT, int R>
+static cudaError_t launch_paged_prep(const PagedPrepParams& p, int head, cudaStream_t st) {
+  const unsigned grid = (unsigned)(p.tokens * ceil_div(p.n_qh + 2 * (int64_t)p.n_kvh, PP_WARPS * R));
   switch (head) {
-    case 64: return launch_pdl(paged_prep_kernel<SRC, DT, 2>, grid, PP_WARPS * 32, 0, st, p);
-    case 128: return launch_pdl(paged_prep_kernel<SRC, DT, 4>, grid, PP_WARPS * 32, 0, st, p);
-    default: return launch_pdl(paged_prep_kernel<SRC, DT, 8>, grid, PP_WARPS * 32, 0, st, p);
+    case 64: return launch_pdl(paged_prep_kernel<SRC, DT, 2, R>, grid, PP_WARPS * 32, 0, st, p);
+    case 128: return launch_pdl(paged_prep_kernel<SRC, DT, 4, R>, grid, PP_WARPS * 32, 0, st, p);
+    default: return launch_pdl(paged_prep_kernel<SRC, DT, 8, R>, grid, PP_WARPS * 32, 0, st, p);
   }
+}
+template <int SRC, int DT>
+static cudaError_t launch_paged_prep(const PagedPrepParams& p, int head, cudaStream_t st) {
+  const int64_t rows = p.tokens * (p.n_qh + 2 * (int64_t)p.n_kvh);
+  return rows >= PP_MANY ? launch_paged_prep<SRC, DT, 4>(p, head, st) : launch_paged_prep<SRC, DT, 1>(p, head, st);
 }
 
 }  // namespace yskn
 
 using namespace yskn;
 
-extern "C" YSKN_B200_API int yskn_b200_paged_prep(
-    const void* d_q, int64_t q_row, int64_t q_head, const void* d_k, int64_t k_row, int64_t k_head, const void* d_v,
-    int64_t v_row, int64_t v_head, int source, const int64_t* d_slots, const int32_t* d_positions,
-    int64_t position_stride, const float* d_inv_freq, const uint8_t* h_axes, int rot, const uint16_t* d_q_norm,
-    const uint16_t* d_k_norm, float eps, int tokens, int n_qh, int n_kvh, int head, void* d_query, void* d_k_cache,
-    void* d_v_cache, int64_t block_stride, int64_t token_stride, int64_t head_stride, int n_blocks, int block_size,
-    int dtype, void* stream) {
-  if (!d_q || !d_k || !d_v || !d_slots || !d_query || !d_k_cache || !d_v_cache ||
-      (rot > 0 && (!d_positions || !d_inv_freq || !h_axes)))
+extern "C" YSKN_B200_API int yskn_b200_paged_prep(const yskn_b200_paged_prep_args* args, void* stream) {
+  if (!args) return fail(YSKN_EINVAL, "paged_prep: null argument");
+  yskn_b200_paged_prep_args a = *args;
+  if (!a.q || !a.k || !a.v || !a.slots || !a.query || !a.k_cache || !a.v_cache ||
+      (a.rot > 0 && (!a.positions || !a.inv_freq)))
     return fail(YSKN_EINVAL, "paged_prep: null argument");
-  if (head != 64 && head != 128 && head != 256) return fail(YSKN_EINVAL, "paged_prep: heads of 64, 128 or 256 channels");
-  if (!is_16bit(dtype) || (source != YSKN_DT_F32 && source != dtype))
+  if (a.head != 64 && a.head != 128 && a.head != 256)
+    return fail(YSKN_EINVAL, "paged_prep: heads of 64, 128 or 256 channels");
+  if (!is_16bit(a.dtype) || (a.source != YSKN_DT_F32 && a.source != a.dtype))
     return fail(YSKN_EINVAL, "paged_prep: the cache is f16 or bf16, the projections f32 or of the cache's type");
-  if (tokens < 1 || n_qh < 1 || n_kvh < 1 || rot < 0 || rot > head || rot % 16 || n_blocks < 1 || block_size < 1)
+  if (a.tokens < 1 || a.n_qh < 1 || a.n_kvh < 1 || a.rot < 0 || a.rot > a.head || a.rot % 16 || a.n_blocks < 1 ||
+      a.block_size < 1)
     return fail(YSKN_EINVAL, "paged_prep: empty shape, or rotated channels not a multiple of 16 up to the head's");
-  for (int i = 0; i < rot / 2; ++i)
-    if (h_axes[i] > 2) return fail(YSKN_EINVAL, "paged_prep: a pair's axis is 0, 1 or 2");
-  if (tokens == 1) q_row = k_row = v_row = 0;  // strides that nothing steps over may be anything
-  if (n_qh == 1) q_head = 0;
-  if (n_kvh == 1) k_head = v_head = head_stride = 0;
-  if (block_size == 1) token_stride = 0;
-  if (n_blocks == 1) block_stride = 0;
-  const int64_t unit = source == YSKN_DT_F32 ? 4 : 8;  // elements of 16 bytes
-  if (!aligned16(d_q) || !aligned16(d_k) || !aligned16(d_v) || !aligned16(d_query) || !aligned16(d_k_cache) ||
-      !aligned16(d_v_cache) || (q_row | q_head | k_row | k_head | v_row | v_head) % unit ||
-      (block_stride | token_stride | head_stride) % 8 || (d_q_norm && !aligned16(d_q_norm)) ||
-      (d_k_norm && !aligned16(d_k_norm)))
+  for (int i = 0; i < a.rot / 2; ++i)
+    if (a.axes[i] >= a.n_axes || a.axes[i] > 2)
+      return fail(YSKN_EINVAL, "paged_prep: a pair's axis is 0, 1 or 2, and one of the positions'");
+  if (a.tokens == 1) a.q_row = a.k_row = a.v_row = 0;  // strides that nothing steps over may be anything
+  if (a.n_qh == 1) a.q_head = 0;
+  if (a.n_kvh == 1) a.k_head = a.v_head = a.head_stride = 0;
+  if (a.block_size == 1) a.token_stride = 0;
+  if (a.n_blocks == 1) a.block_stride = 0;
+  const int64_t unit = a.source == YSKN_DT_F32 ? 4 : 8;  // elements of 16 bytes
+  if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.query) || !aligned16(a.k_cache) ||
+      !aligned16(a.v_cache) || (a.q_row | a.q_head | a.k_row | a.k_head | a.v_row | a.v_head) % unit ||
+      (a.block_stride | a.token_stride | a.head_stride) % 8 || !aligned16(a.q_norm) || !aligned16(a.k_norm))
     return fail(YSKN_EINVAL, "paged_prep: pointers and strides are multiples of 16 bytes");
   PagedPrepParams p{};
-  p.q = d_q, p.k = d_k, p.v = d_v;
-  p.q_row = q_row, p.q_head = q_head, p.k_row = k_row, p.k_head = k_head, p.v_row = v_row, p.v_head = v_head;
-  p.slots = d_slots, p.positions = d_positions, p.position_stride = position_stride, p.inv_freq = d_inv_freq;
-  p.q_norm = d_q_norm, p.k_norm = d_k_norm, p.eps = eps;
-  p.tokens = tokens, p.n_qh = n_qh, p.n_kvh = n_kvh, p.rot = rot;
-  p.query = reinterpret_cast<uint16_t*>(d_query);
-  p.k_cache = reinterpret_cast<uint16_t*>(d_k_cache), p.v_cache = reinterpret_cast<uint16_t*>(d_v_cache);
-  p.cache = {block_stride, token_stride, head_stride};
-  p.block_size = block_size, p.n_slots = (int64_t)n_blocks * block_size;
+  p.q = a.q, p.k = a.k, p.v = a.v;
+  p.q_row = a.q_row, p.q_head = a.q_head, p.k_row = a.k_row, p.k_head = a.k_head, p.v_row = a.v_row, p.v_head = a.v_head;
+  p.slots = a.slots, p.positions = a.positions, p.position_stride = a.position_stride, p.inv_freq = a.inv_freq;
+  p.q_norm = a.q_norm, p.k_norm = a.k_norm, p.eps = a.eps;
+  p.tokens = a.tokens, p.n_qh = a.n_qh, p.n_kvh = a.n_kvh, p.rot = a.rot;
+  p.query = reinterpret_cast<uint16_t*>(a.query);
+  p.k_cache = reinterpret_cast<uint16_t*>(a.k_cache), p.v_cache = reinterpret_cast<uint16_t*>(a.v_cache);
+  p.cache = {a.block_stride, a.token_stride, a.head_stride};
+  p.block_size = a.block_size, p.n_slots = (int64_t)a.n_blocks * a.block_size;
   p.err = device_error_word();
-  for (int i = 0; i < rot / 2; ++i) p.axis[i] = h_axes[i];
-  const int64_t grid = (int64_t)tokens * ceil_div(n_qh + 2 * (int64_t)n_kvh, PP_WARPS);
-  if (grid > (int64_t)INT32_MAX) return fail(YSKN_EINVAL, "paged_prep: too many rows");
+  for (int i = 0; i < a.rot / 2; ++i) p.axis[i] = a.axes[i];
+  if ((int64_t)a.tokens * ceil_div(a.n_qh + 2 * (int64_t)a.n_kvh, PP_WARPS) > (int64_t)INT32_MAX)
+    return fail(YSKN_EINVAL, "paged_prep: too many rows");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (dtype == YSKN_DT_BF16)
-    e = source == YSKN_DT_F32 ? launch_paged_prep<YSKN_DT_F32, YSKN_DT_BF16>(p, head, (unsigned)grid, st)
-                              : launch_paged_prep<YSKN_DT_BF16, YSKN_DT_BF16>(p, head, (unsigned)grid, st);
+  if (a.dtype == YSKN_DT_BF16)
+    e = a.source == YSKN_DT_F32 ? launch_paged_prep<YSKN_DT_F32, YSKN_DT_BF16>(p, a.head, st)
+                                : launch_paged_prep<YSKN_DT_BF16, YSKN_DT_BF16>(p, a.head, st);
   else
-    e = source == YSKN_DT_F32 ? launch_paged_prep<YSKN_DT_F32, YSKN_DT_F16>(p, head, (unsigned)grid, st)
-                              : launch_paged_prep<YSKN_DT_F16, YSKN_DT_F16>(p, head, (unsigned)grid, st);
+    e = a.source == YSKN_DT_F32 ? launch_paged_prep<YSKN_DT_F32, YSKN_DT_F16>(p, a.head, st)
+                                : launch_paged_prep<YSKN_DT_F16, YSKN_DT_F16>(p, a.head, st);
   return cuda_fail(e, "paged_prep_kernel");
 }

@@ -100,7 +100,7 @@ inline PaWork pa_work(int tokens, int batch, int max_new, int n_qh, int n_kvh, i
   w.own_items = own_items;
   w.base = 256;
   w.item = w.base + up((int64_t)batch * 4);
-  w.pre_ml = w.item + up(own_items * 8);
+  w.pre_ml = w.item + up(own_items * 4);
   w.pre_o = w.pre_ml + up(pre * 2 * PA_ROWS * 8);
   w.own_ml = w.pre_o + up(pre * 2 * PA_ROWS * head * 4);
   w.own_o = w.own_ml + up(own * w.own_rows * 8);
@@ -122,14 +122,14 @@ struct PrefixAttnParams {
   int pre_tiles, pre_qtiles, pre_items;
   float c;  // |scale| log2 e
   uint32_t negate_q;
-  long long* work_per;    // units per pair of this call, for the join
+  int* work_per;          // units per pair of this call, for the join
   int32_t* work_base;     // [batch] first own item of each request
-  long long* work_item;   // [own items] first unit of each own item
+  int* work_item;         // [own items] first unit of each own item
   // per place: (m, l) of each row; o as [D / 4][rows][4], so that a warp's rows are adjacent
   float2 *pre_ml, *own_ml;
   float *pre_o, *own_o;
   int own_half, own_rows;
-  long long own_items;  // more of them (starts that do not ascend) is an error: nothing is computed
+  long long own_items;  // more of them (starts that do not ascend), or 2^30 own units, is an error: nothing is computed
   uint16_t* out;  // [tokens][n_qh][D]
   unsigned* err;
 };
@@ -458,7 +458,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
       total += sh.sum[w][0];
       total_items += sh.sum[w][1];
     }
-    const bool sound = total_items <= p.own_items;
+    const bool sound = total_items <= p.own_items && total <= INT32_MAX / 2;
     const int pre_units = pa_units(p.pre_tiles);
     const long long pre = (long long)p.pre_items * pre_units, all = sound ? pre + total : 0;
     const long long share = sound ? max(1ll, (all + pairs - 1) / pairs) : 0;
@@ -470,7 +470,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
         sh.start.u0 = (int)(t0 - (long long)sh.start.pre_item * pre_units);
       }
       if (blockIdx.x == 0) {
-        *p.work_per = share;
+        *p.work_per = (int)share;
         if (!sound) raise_device_error(p.err, DERR_RANGE);
       }
     }
@@ -840,7 +840,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
       __syncwarp();
       if (lane == 0) arrive_first(o_free0);
       if (!seg.prefix && seg.key0 == 0 && row == 0 && half == 0 && rank == 0)
-        p.work_item[seg.place - pair] = seg.begin;
+        p.work_item[seg.place - pair] = (int)seg.begin;
     }
   }
   tc_fence_before();
@@ -874,7 +874,7 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
 #pragma unroll
   for (int j = 0; j < 4; ++j) o[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   const int i = request_of(p.starts, p.batch, t);
-  const long long per = *p.work_per;
+  const int per = *p.work_per;
   const PaRequest r = i < p.batch ? pa_request(p, i) : PaRequest{};
   if (per > 0 && t >= r.s0 && t < r.s0 + r.n) {
     // places of the row's segments: n_pre of its prefix item, then n_own of its own item
@@ -882,9 +882,8 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
     int64_t pre0 = 0, own0 = 0;
     if (p.pre_tiles > 0) {
       const int qt = t / p.tpi, it = kvh * p.pre_qtiles + qt, tl = t - qt * p.tpi, rank = tl >= p.tpc;
-      const long long b = (long long)it * pa_units(p.pre_tiles) + PA_ITEM_COST;
-      const long long c0 = b / per, c1 = (b + p.pre_tiles - 1) / per;
-      n_pre = (int)(c1 - c0) + 1;
+      const int b = it * pa_units(p.pre_tiles) + PA_ITEM_COST, c0 = b / per;
+      n_pre = (b + p.pre_tiles - 1) / per - c0 + 1;
       pre0 = it + c0;
       pre_row = rank * PA_ROWS + (tl - rank * p.tpc) * p.G + gh;
     }
@@ -893,8 +892,8 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
     const int kt = pa_own_tiles(p, r, own_qt);
     if (kt > 0) {
       const int64_t it = (int64_t)p.work_base[i] + kvh * pa_qtiles(p, r) + own_qt;
-      const long long b = p.work_item[it] + PA_ITEM_COST, c0 = b / per, c1 = (b + kt - 1) / per;
-      n_own = (int)(c1 - c0) + 1;
+      const int b = p.work_item[it] + PA_ITEM_COST, c0 = b / per;
+      n_own = (b + kt - 1) / per - c0 + 1;
       own0 = it + c0;
     }
     auto ml_of = [&](int x) {
@@ -983,74 +982,73 @@ extern "C" YSKN_B200_API int64_t yskn_b200_prefix_attention_work_bytes(int token
   return pa_work(tokens, batch, max_new, n_qh, n_kvh, head).bytes;
 }
 
-extern "C" YSKN_B200_API int yskn_b200_prefix_attention(
-    const void* d_q, int64_t q_row, int64_t q_head, const void* d_gate, int64_t gate_row, int64_t gate_head,
-    const void* d_k_cache, const void* d_v_cache, int64_t block_stride, int64_t token_stride, int64_t head_stride,
-    int n_blocks, int block_size, const int32_t* d_prefix_blocks, int prefix_len, const int32_t* d_block_tables,
-    int table_width, int64_t table_stride, const int32_t* d_lens, const int32_t* d_starts, int batch, int tokens,
-    int max_new, int n_qh, int n_kvh, int head, int dtype, float scale, void* d_work, void* d_out, void* stream) {
-  if (!d_q || !d_k_cache || !d_v_cache || !d_block_tables || !d_lens || !d_starts || !d_work || !d_out ||
-      (prefix_len > 0 && !d_prefix_blocks))
+extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_attention_args* args, void* stream) {
+  if (!args) return fail(YSKN_EINVAL, "prefix_attention: null argument");
+  yskn_b200_prefix_attention_args a = *args;
+  if (!a.q || !a.k_cache || !a.v_cache || !a.block_tables || !a.lens || !a.starts || !a.work || !a.out ||
+      (a.prefix_len > 0 && !a.prefix_blocks))
     return fail(YSKN_EINVAL, "prefix_attention: null argument");
+  const int head = a.head, n_qh = a.n_qh, n_kvh = a.n_kvh, block_size = a.block_size, dtype = a.dtype;
   if (head != 64 && head != 128 && head != 256)
     return fail(YSKN_EINVAL, "prefix_attention: heads of 64, 128 or 256 channels");
   if (!is_16bit(dtype)) return fail(YSKN_EINVAL, "prefix_attention: queries and cache are f16 or bf16");
-  if (tokens < 1 || batch < 1 || max_new < 1 || n_kvh < 1 || n_qh < 1 || n_qh % n_kvh || n_qh / n_kvh > 128 ||
-      prefix_len < 0 || table_width < 1 || (batch > 1 && table_stride < table_width) || n_blocks < 1)
+  if (a.tokens < 1 || a.batch < 1 || a.max_new < 1 || n_kvh < 1 || n_qh < 1 || n_qh % n_kvh || n_qh / n_kvh > PA_ROWS ||
+      a.prefix_len < 0 || a.table_width < 1 || (a.batch > 1 && a.table_stride < a.table_width) || a.n_blocks < 1)
     return fail(YSKN_EINVAL, "prefix_attention: empty shape, heads not a multiple, or a stride below its width");
   if (block_size != 16 && block_size != 32 && block_size != 64 && block_size != 128)
     return fail(YSKN_EINVAL, "prefix_attention: blocks of 16, 32, 64 or 128 rows");
-  if (tokens == 1) q_row = gate_row = 0;  // strides that nothing steps over may be anything
-  if (n_qh == 1) q_head = gate_head = 0;
-  if (n_kvh == 1) head_stride = 0;
-  if (n_blocks == 1) block_stride = 0;
-  if (!aligned16(d_q) || !aligned16(d_gate) || !aligned16(d_k_cache) || !aligned16(d_v_cache) || !aligned16(d_work) ||
-      !aligned16(d_out) || (q_row | q_head | block_stride | token_stride | head_stride) % 8 ||
-      (d_gate && (gate_row | gate_head) % 8))
+  if (a.tokens == 1) a.q_row = a.gate_row = 0;  // strides that nothing steps over may be anything
+  if (n_qh == 1) a.q_head = a.gate_head = 0;
+  if (n_kvh == 1) a.head_stride = 0;
+  if (a.n_blocks == 1) a.block_stride = 0;
+  if (!aligned16(a.q) || !aligned16(a.gate) || !aligned16(a.k_cache) || !aligned16(a.v_cache) || !aligned16(a.work) ||
+      !aligned16(a.out) || (a.q_row | a.q_head | a.block_stride | a.token_stride | a.head_stride) % 8 ||
+      (a.gate && (a.gate_row | a.gate_head) % 8))
     return fail(YSKN_EINVAL, "prefix_attention: pointers and strides are multiples of 16 bytes");
+  const PaWork w = pa_work(a.tokens, a.batch, a.max_new, n_qh, n_kvh, head);
+  if (a.work_bytes < w.bytes) return fail(YSKN_EINVAL, "prefix_attention: workspace too small");
   const int G = n_qh / n_kvh, tpc = PA_ROWS / G;
   PrefixAttnParams p{};
-  p.gate = reinterpret_cast<const uint16_t*>(d_gate);
-  p.gate_row = gate_row, p.gate_head = gate_head;
-  p.prefix_blocks = d_prefix_blocks;
-  p.tables = d_block_tables, p.table_stride = table_stride;
-  p.lens = d_lens, p.starts = d_starts;
-  p.n_blocks = n_blocks, p.block_shift = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : 7, p.prefix_len = prefix_len;
-  p.own_limit = (int)std::min<int64_t>((int64_t)table_width * block_size, INT32_MAX - PA_KEYS);
-  p.batch = batch, p.tokens = tokens, p.max_new = max_new, p.n_kvh = n_kvh, p.G = G;
+  p.gate = reinterpret_cast<const uint16_t*>(a.gate);
+  p.gate_row = a.gate_row, p.gate_head = a.gate_head;
+  p.prefix_blocks = a.prefix_blocks;
+  p.tables = a.block_tables, p.table_stride = a.table_stride;
+  p.lens = a.lens, p.starts = a.starts;
+  p.n_blocks = a.n_blocks, p.block_shift = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : 7, p.prefix_len = a.prefix_len;
+  p.own_limit = (int)std::min<int64_t>((int64_t)a.table_width * block_size, INT32_MAX - PA_KEYS);
+  p.batch = a.batch, p.tokens = a.tokens, p.max_new = a.max_new, p.n_kvh = n_kvh, p.G = G;
   p.tpc = tpc, p.tpi = 2 * tpc;
-  p.pre_tiles = (int)ceil_div(prefix_len, PA_KEYS), p.pre_qtiles = (int)ceil_div(tokens, 2 * tpc);
+  p.pre_tiles = (int)ceil_div(a.prefix_len, PA_KEYS), p.pre_qtiles = (int)ceil_div(a.tokens, 2 * tpc);
   const int64_t items = (int64_t)p.pre_qtiles * n_kvh;
-  if (items > INT32_MAX / 2) return fail(YSKN_EINVAL, "prefix_attention: too many rows");
-  p.pre_items = prefix_len > 0 ? (int)items : 0;
-  // a scale of zero keeps its meaning (equal weights) with a factor that leaves -inf alone
-  p.c = std::max(std::fabs(scale) * 1.4426950408889634f, 1e-30f);
-  p.negate_q = scale < 0.0f;
-  const PaWork w = pa_work(tokens, batch, max_new, n_qh, n_kvh, head);
-  uint8_t* work = reinterpret_cast<uint8_t*>(d_work);
-  p.work_per = reinterpret_cast<long long*>(work);
+  if (items * pa_units(p.pre_tiles) > INT32_MAX / 2) return fail(YSKN_EINVAL, "prefix_attention: too much work");
+  p.pre_items = a.prefix_len > 0 ? (int)items : 0;
+  // a a.scale of zero keeps its meaning (equal weights) with a factor that leaves -inf alone
+  p.c = std::max(std::fabs(a.scale) * 1.4426950408889634f, 1e-30f);
+  p.negate_q = a.scale < 0.0f;
+  uint8_t* work = reinterpret_cast<uint8_t*>(a.work);
+  p.work_per = reinterpret_cast<int*>(work);
   p.work_base = reinterpret_cast<int32_t*>(work + w.base);
-  p.work_item = reinterpret_cast<long long*>(work + w.item);
+  p.work_item = reinterpret_cast<int*>(work + w.item);
   p.pre_ml = reinterpret_cast<float2*>(work + w.pre_ml), p.pre_o = reinterpret_cast<float*>(work + w.pre_o);
   p.own_ml = reinterpret_cast<float2*>(work + w.own_ml), p.own_o = reinterpret_cast<float*>(work + w.own_o);
   p.own_half = w.own_half, p.own_rows = w.own_rows, p.own_items = w.own_items;
-  p.out = reinterpret_cast<uint16_t*>(d_out), p.err = device_error_word();
+  p.out = reinterpret_cast<uint16_t*>(a.out), p.err = device_error_word();
   // The cache's 64-channel columns are an axis of their own, so that one box holds several columns
   // of its rows in the order of the ring's slots; where a slot takes several boxes (blocks
   // shorter than it), a box is one column.
   const int slots = head <= 128 ? 1 : head / 128, v_rows = PA_KEYS / slots;
-  const int64_t q_dims[3] = {head, n_qh, tokens}, q_strides[2] = {q_head, q_row};
-  const int64_t c_dims[5] = {64, block_size, head / 64, n_kvh, n_blocks};
-  const int64_t c_strides[4] = {token_stride, 64, head_stride, block_stride};
-  const int box_pre[3] = {64, G, tpc}, box_own[3] = {64, G, std::min(tpc, max_new)};
+  const int64_t q_dims[3] = {head, n_qh, a.tokens}, q_strides[2] = {a.q_head, a.q_row};
+  const int64_t c_dims[5] = {64, block_size, head / 64, n_kvh, a.n_blocks};
+  const int64_t c_strides[4] = {a.token_stride, 64, a.head_stride, a.block_stride};
+  const int box_pre[3] = {64, G, tpc}, box_own[3] = {64, G, std::min(tpc, a.max_new)};
   const int box_k[5] = {64, std::min(block_size, PA_KEYS / 2), block_size < PA_KEYS / 2 ? 1 : head / 64 / slots, 1, 1};
   const int box_v[5] = {head == 64 ? 32 : 64, std::min(block_size, v_rows),
                         block_size < v_rows || head <= 128 ? 1 : head / 128, 1, 1};
   CUtensorMap maps[4];
-  if (int rc = paged_map(&maps[0], d_q, dtype, 3, q_dims, q_strides, box_pre)) return rc;
-  if (int rc = paged_map(&maps[1], d_q, dtype, 3, q_dims, q_strides, box_own)) return rc;
-  if (int rc = paged_map(&maps[2], d_k_cache, dtype, 5, c_dims, c_strides, box_k)) return rc;
-  if (int rc = paged_map(&maps[3], d_v_cache, dtype, 5, c_dims, c_strides, box_v)) return rc;
+  if (int rc = paged_map(&maps[0], a.q, dtype, 3, q_dims, q_strides, box_pre)) return rc;
+  if (int rc = paged_map(&maps[1], a.q, dtype, 3, q_dims, q_strides, box_own)) return rc;
+  if (int rc = paged_map(&maps[2], a.k_cache, dtype, 5, c_dims, c_strides, box_k)) return rc;
+  if (int rc = paged_map(&maps[3], a.v_cache, dtype, 5, c_dims, c_strides, box_v)) return rc;
   int dev = 0, sms = 2 * PA_MAX_PAIRS;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

@@ -8,6 +8,7 @@ if the library has not been built; there is no fallback path.
 """
 import ctypes as C
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
@@ -92,15 +93,11 @@ _SIGNATURES = {
     "yskn_b200_head_merge": (_i, [_vp, _vp, _i64, _vp, _i, _i, _vp, _vp, _vp, _vp]),
     "yskn_b200_linear_from_residual": (_i, [_vp, _i, _vp, _vp, _vp, _vp, C.c_float, _i, _vp, _vp, _vp, _vp]),
     "yskn_b200_linear_rowpar_q8": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp]),
-    "yskn_b200_batch_plan": (_i, [_vp, _vp, _i, _i, _i, _vp, _i, _i64, _vp, _i, _vp, _i] + [_vp] * 7),
-    "yskn_b200_paged_prep": (_i, [_vp, _i64, _i64] * 3 + [_i, _vp, _vp, _i64, _vp, _vp, _i, _vp, _vp, C.c_float,
-                                                          _i, _i, _i, _i, _vp, _vp, _vp, _i64, _i64, _i64, _i, _i,
-                                                          _i, _vp]),
+    "yskn_b200_batch_plan": (_i, [C.c_char_p, _vp]),
+    "yskn_b200_paged_prep": (_i, [C.c_char_p, _vp]),
     "yskn_b200_prefix_attention_work_bytes": (_i64, [_i] * 6),
-    "yskn_b200_prefix_attention": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i, _i, _vp, _i,
-                                        _vp, _i, _i64, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, C.c_float, _vp, _vp,
-                                        _vp]),
-    "yskn_b200_logits_adjust": (_i, [_vp, _i64, _i, _i, _vp, _i64, _i] + [_vp] * 7 + [_i, _vp, _i64, _vp, _i64, _vp]),
+    "yskn_b200_prefix_attention": (_i, [C.c_char_p, _vp]),
+    "yskn_b200_logits_adjust": (_i, [C.c_char_p, _vp]),
 }
 
 _lib = None
@@ -671,17 +668,31 @@ def kv_encode(rows, row_group, tables, gains, mults, kb, vit2, words, scales, me
 
 
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
+
+# The batch operators take a struct of arguments (yskn_b200_*_args, in the header's order); packing
+# one is ten times faster than converting as many ctypes arguments.
+ARGS = {
+    "batch_plan": struct.Struct("@3PqPP3P3P6i"),
+    "paged_prep": struct.Struct("@3P6q2PqP2P3P3q10if128s"),
+    "prefix_attention": struct.Struct("@P2qP2q2P3q2Pq2PPqP11if"),
+    "logits_adjust": struct.Struct("@PqPq2P3P2PPqPq4i"),
+}
 _DT = {}
+
+
+def _types():
+    import torch
+    _DT.update({torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.int16: DT_BF16})
+    _DT["i32"] = torch.int32
+    _DT["stream"] = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
 def _dtype(t):
     """YSKN_DT_* of a tensor; int16 tensors hold bf16 bits, as everywhere in this binding."""
-    if not _DT:
-        import torch
-        _DT.update({torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.int16: DT_BF16})
-    if t.dtype not in _DT:
+    d = _DT.get(t.dtype)
+    if d is None:
         raise YsknError(EINVAL, "a tensor of f32, f16, bf16 or int16 (bf16 bits) expected, not %s" % t.dtype)
-    return _DT[t.dtype]
+    return d
 
 
 def _need(ok, what):
@@ -689,18 +700,18 @@ def _need(ok, what):
         raise YsknError(EINVAL, what)
 
 
-def _is_i32(*tensors):
-    import torch
-    return all(t is None or t.dtype == torch.int32 for t in tensors)
-
-
-def _address(t):
-    return None if t is None else t.data_ptr()
-
-
-def _stream_address(stream):
-    import torch
-    return (torch.cuda.current_stream() if stream is None else stream).cuda_stream
+def _launch(name, packed, tensor, stream):
+    """The call on `stream`, or on the current stream of the tensor's device."""
+    if stream is not None:
+        raw = stream.cuda_stream
+    elif _DT["stream"] is not None:
+        raw = _DT["stream"](tensor.get_device())
+    else:
+        import torch
+        raw = torch.cuda.current_stream().cuda_stream
+    rc = getattr(_lib or lib(), "yskn_b200_" + name)(packed, raw)
+    if rc:
+        check(rc, name)
 
 
 def batch_plan(lens, new_lens, block_tables, pool, free_count, block_size, lens_out, free_out, starts, slots, positions,
@@ -710,17 +721,21 @@ def batch_plan(lens, new_lens, block_tables, pool, free_count, block_size, lens_
     into block_tables (int32 [batch][width]); the new lengths and count, the served tokens
     before each request (starts int32 [batch + 1]) and per token its slot (int64), position
     and request (int32), -1 past the last one."""
+    if not _DT:
+        _types()
+    i32 = _DT["i32"]
     B, width = block_tables.shape
-    T = slots.shape[0]
-    _need(_is_i32(lens, new_lens, block_tables, pool, free_count, lens_out, free_out, starts, positions, requests) and
-          slots.element_size() == 8 and lens.shape[0] == new_lens.shape[0] == lens_out.shape[0] == B and
-          starts.shape[0] == B + 1 and positions.shape[0] == requests.shape[0] == T and block_tables.stride(1) == 1,
+    T, row = slots.numel(), block_tables.stride()
+    _need(lens.dtype is i32 and new_lens.dtype is i32 and block_tables.dtype is i32 and pool.dtype is i32 and
+          free_count.dtype is i32 and lens_out.dtype is i32 and free_out.dtype is i32 and starts.dtype is i32 and
+          positions.dtype is i32 and requests.dtype is i32 and slots.element_size() == 8 and lens.numel() == B and
+          new_lens.numel() == B and lens_out.numel() == B and starts.numel() == B + 1 and positions.numel() == T and
+          requests.numel() == T and row[1] == 1,
           "batch_plan: int32 arrays of the batch, int64 slots and as many positions and requests expected")
-    check(lib().yskn_b200_batch_plan(lens.data_ptr(), new_lens.data_ptr(), B, block_size, prefix_len,
-                                     block_tables.data_ptr(), width, block_tables.stride(0), pool.data_ptr(),
-                                     pool.shape[0], free_count.data_ptr(), T, lens_out.data_ptr(),
-                                     free_out.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-                                     requests.data_ptr(), _stream_address(stream)), "batch_plan")
+    _launch("batch_plan", ARGS["batch_plan"].pack(
+        lens.data_ptr(), new_lens.data_ptr(), block_tables.data_ptr(), row[0], pool.data_ptr(), free_count.data_ptr(),
+        lens_out.data_ptr(), free_out.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+        requests.data_ptr(), B, block_size, prefix_len, width, pool.numel(), T), lens, stream)
 
 
 def paged_prep(q, k, v, slots, positions, query, k_cache, v_cache, inv_freq=None, axes=None, q_norm=None, k_norm=None,
@@ -730,29 +745,35 @@ def paged_prep(q, k, v, slots, positions, query, k_cache, v_cache, inv_freq=None
     [rot / 2], axes the position axis of each pair, positions int32 [n_axes][T] or [T]) into
     query (dense [T][n_qh][D]) and, at `slots` (int64 [T]), k_cache and v_cache (views
     [n_blocks][block_size][n_kvh][D] of the same strides)."""
-    T, n_qh, D = query.shape
-    n_blocks, block_size, n_kvh = k_cache.shape[:3]
-    rot = 0 if inv_freq is None else 2 * inv_freq.shape[0]
-    _need(tuple(q.shape) == (T, n_qh, D) and tuple(k.shape) == tuple(v.shape) == (T, n_kvh, D) and
-          k_cache.shape[3] == D and v_cache.shape == k_cache.shape and v_cache.stride() == k_cache.stride() and
-          k_cache.stride(3) == q.stride(2) == k.stride(2) == v.stride(2) == 1 and query.is_contiguous(),
+    if not _DT:
+        _types()
+    shape, cache = query.shape, k_cache.shape
+    T, n_qh, D = shape
+    n_blocks, block_size, n_kvh, _ = cache
+    qs, ks, vs, cs = q.stride(), k.stride(), v.stride(), k_cache.stride()
+    src, dt = q.dtype, query.dtype
+    _need(q.shape == shape and k.shape == (T, n_kvh, D) and v.shape == (T, n_kvh, D) and cache[3] == D and
+          v_cache.shape == cache and v_cache.stride() == cs and cs[3] == 1 and qs[2] == 1 and ks[2] == 1 and
+          vs[2] == 1 and query.is_contiguous(),
           "paged_prep: q, k, v of the caches' heads with dense channels, caches of one shape and strides expected")
-    _need(_dtype(q) == _dtype(k) == _dtype(v) and _dtype(query) == _dtype(k_cache) == _dtype(v_cache) and
-          slots.element_size() == 8 and slots.shape[0] == T, "paged_prep: types of q, k, v or of the caches differ")
-    packed, stride = None, 0
-    if rot:
-        axes = bytes(axes) if axes is not None else bytes(rot // 2)
-        n_axes = 1 if positions.dim() == 1 else positions.shape[0]
-        _need(_is_i32(positions) and positions.shape[-1] == T and positions.stride(-1) == 1 and
-              len(axes) == rot // 2 and max(axes) < n_axes,
+    _need(k.dtype is src and v.dtype is src and k_cache.dtype is dt and v_cache.dtype is dt and
+          slots.element_size() == 8 and slots.numel() == T, "paged_prep: types of q, k, v or of the caches differ")
+    rot = n_axes = stride = 0
+    packed = b""
+    if inv_freq is not None:
+        rot = 2 * inv_freq.numel()
+        ps = positions.shape
+        n_axes, stride = (1, T) if len(ps) == 1 else (ps[0], positions.stride(0))
+        packed = bytes(axes) if axes is not None else bytes(rot // 2)
+        _need(positions.dtype is _DT["i32"] and ps[-1] == T and positions.stride(-1) == 1 and
+              len(packed) == rot // 2 and len(packed) <= 128,
               "paged_prep: int32 positions of every token, and an axis of them for each pair expected")
-        packed, stride = axes, positions.stride(0) if positions.dim() == 2 else T
-    check(lib().yskn_b200_paged_prep(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-                                     v.data_ptr(), v.stride(0), v.stride(1), _dtype(q), slots.data_ptr(),
-                                     _address(positions), stride, _address(inv_freq), packed, rot, _address(q_norm),
-                                     _address(k_norm), eps, T, n_qh, n_kvh, D, query.data_ptr(), k_cache.data_ptr(),
-                                     v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
-                                     n_blocks, block_size, _dtype(k_cache), _stream_address(stream)), "paged_prep")
+    _launch("paged_prep", ARGS["paged_prep"].pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], slots.data_ptr(),
+        positions.data_ptr() if rot else 0, stride, inv_freq.data_ptr() if rot else 0,
+        0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(), query.data_ptr(),
+        k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], T, n_qh, n_kvh, D, rot, n_axes, n_blocks,
+        block_size, _dtype(q), _dtype(query), eps, packed), query, stream)
 
 
 def prefix_attention_work_bytes(tokens, batch, max_new, n_qh, n_kvh, head):
@@ -766,33 +787,35 @@ def prefix_attention(q, k_cache, v_cache, block_tables, lens, starts, max_new, w
     """yskn_b200_prefix_attention: q (and gate) [T][n_qh][D] with dense channels, the caches as
     paged_prep, each request's own blocks in block_tables (int32 [batch][width]) and the shared
     prefix's in prefix_blocks; lens and starts as batch_plan writes them (at most max_new tokens
-    a request) -> out (dense [T][n_qh][D]). scale defaults to 1 / sqrt(D)."""
-    T, n_qh, D = out.shape
-    n_blocks, block_size, n_kvh = k_cache.shape[:3]
+    a request) -> out (dense [T][n_qh][D]). scale defaults to 1 / sqrt(D). work: uint8, of
+    prefix_attention_work_bytes(T, batch, max_new, n_qh, n_kvh, D) bytes."""
+    if not _DT:
+        _types()
+    i32, dt = _DT["i32"], q.dtype
+    shape, cache = out.shape, k_cache.shape
+    T, n_qh, D = shape
+    n_blocks, block_size, n_kvh, _ = cache
     B, width = block_tables.shape
-    dt = _dtype(q)
-    _need(tuple(q.shape) == (T, n_qh, D) and (gate is None or (gate.shape == q.shape and gate.stride(2) == 1 and
-                                                               _dtype(gate) == dt)) and
-          k_cache.shape[3] == D and v_cache.shape == k_cache.shape and v_cache.stride() == k_cache.stride() and
-          k_cache.stride(3) == q.stride(2) == 1 and out.is_contiguous() and
-          _dtype(k_cache) == _dtype(v_cache) == _dtype(out) == dt,
-          "prefix_attention: q, gate, out and caches of one type and head size with dense channels expected")
-    _need(_is_i32(block_tables, lens, starts, prefix_blocks) and lens.shape[0] == B and starts.shape[0] == B + 1 and
-          block_tables.stride(1) == 1 and
-          (prefix_len == 0 or (prefix_blocks is not None and prefix_blocks.shape[0] * block_size >= prefix_len)),
+    qs, cs, row = q.stride(), k_cache.stride(), block_tables.stride()
+    _need(q.shape == shape and cache[3] == D and v_cache.shape == cache and v_cache.stride() == cs and cs[3] == 1 and
+          qs[2] == 1 and out.is_contiguous() and k_cache.dtype is dt and v_cache.dtype is dt and out.dtype is dt,
+          "prefix_attention: q, out and caches of one type and head size with dense channels expected")
+    _need(block_tables.dtype is i32 and lens.dtype is i32 and starts.dtype is i32 and lens.numel() == B and
+          starts.numel() == B + 1 and row[1] == 1 and
+          (not prefix_len or (prefix_blocks is not None and prefix_blocks.dtype is i32 and
+                              prefix_blocks.numel() * block_size >= prefix_len)),
           "prefix_attention: int32 tables, lengths and starts of one batch, and the prefix's blocks expected")
-    _need(work.numel() * work.element_size() >= prefix_attention_work_bytes(T, B, max_new, n_qh, n_kvh, D),
-          "prefix_attention: workspace too small")
-    check(lib().yskn_b200_prefix_attention(q.data_ptr(), q.stride(0), q.stride(1), _address(gate),
-                                           gate.stride(0) if gate is not None else 0,
-                                           gate.stride(1) if gate is not None else 0, k_cache.data_ptr(),
-                                           v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),
-                                           k_cache.stride(2), n_blocks, block_size,
-                                           _address(prefix_blocks) if prefix_len else None, prefix_len,
-                                           block_tables.data_ptr(), width, block_tables.stride(0), lens.data_ptr(),
-                                           starts.data_ptr(), B, T, max_new, n_qh, n_kvh, D, dt,
-                                           D ** -0.5 if scale is None else scale, work.data_ptr(), out.data_ptr(),
-                                           _stream_address(stream)), "prefix_attention")
+    gs = (0, 0)
+    if gate is not None:
+        gs = gate.stride()
+        _need(gate.shape == shape and gs[2] == 1 and gate.dtype is dt,
+              "prefix_attention: a gate of the queries' shape and type with dense channels expected")
+    _launch("prefix_attention", ARGS["prefix_attention"].pack(
+        q.data_ptr(), qs[0], qs[1], 0 if gate is None else gate.data_ptr(), gs[0], gs[1], k_cache.data_ptr(),
+        v_cache.data_ptr(), cs[0], cs[1], cs[2], prefix_blocks.data_ptr() if prefix_len else 0,
+        block_tables.data_ptr(), row[0], lens.data_ptr(), starts.data_ptr(), work.data_ptr(),
+        work.numel() * work.element_size(), out.data_ptr(), n_blocks, block_size, prefix_len, width, B, T, max_new,
+        n_qh, n_kvh, D, _dtype(q), D ** -0.5 if scale is None else scale), out, stream)
 
 
 def logits_adjust(logits, out, history=None, history_lens=None, prompt_lens=None, repetition=None, presence=None,
@@ -801,22 +824,42 @@ def logits_adjust(logits, out, history=None, history_lens=None, prompt_lens=None
     logits). history int32 [M][L] with history_lens and prompt_lens int32 [M]; repetition,
     presence, frequency f32 [M]; bias_ids int32 and bias f32 [M][n] (dense); mask int32
     [M][>= ceil(V / 32)], a set bit for an allowed token."""
-    M, V = logits.shape
-    _need(_dtype(logits) == _dtype(out) == DT_F32 and out.shape == logits.shape and logits.stride(1) == 1 and
-          out.stride(1) == 1 and _is_i32(history, history_lens, prompt_lens, bias_ids, mask),
-          "logits_adjust: f32 logits and output of one shape, int32 history, ids and mask expected")
-    _need(all(t is None or t.shape[0] == M for t in (history, history_lens, prompt_lens, repetition, presence,
-                                                     frequency, bias_ids, bias, mask)) and
-          all(t is None or _dtype(t) == DT_F32 for t in (repetition, presence, frequency, bias)) and
-          (bias_ids is None) == (bias is None) and
-          (bias is None or (bias.shape == bias_ids.shape and bias.is_contiguous() and bias_ids.is_contiguous())) and
-          (history is None or history.stride(1) == 1) and (mask is None or mask.stride(1) == 1),
-          "logits_adjust: a row of each argument for each row of logits expected")
-    check(lib().yskn_b200_logits_adjust(logits.data_ptr(), logits.stride(0), M, V, _address(history),
-                                        history.stride(0) if history is not None else 0,
-                                        history.shape[1] if history is not None else 0, _address(history_lens),
-                                        _address(prompt_lens), _address(repetition), _address(presence),
-                                        _address(frequency), _address(bias_ids), _address(bias),
-                                        bias.shape[1] if bias is not None else 0, _address(mask),
-                                        mask.stride(0) if mask is not None else 0, out.data_ptr(), out.stride(0),
-                                        _stream_address(stream)), "logits_adjust")
+    if not _DT:
+        _types()
+    i32, f32 = _DT["i32"], logits.dtype
+    shape, xs, os_ = logits.shape, logits.stride(), out.stride()
+    M, V = shape
+    _need(_dtype(logits) == DT_F32 and out.dtype is f32 and out.shape == shape and xs[1] == 1 and os_[1] == 1,
+          "logits_adjust: f32 logits and output of one shape with dense rows expected")
+    hs = ms = (0, 1)
+    width = n_bias = 0
+    if history is not None:
+        hs, (rows, width) = history.stride(), history.shape
+        _need(history.dtype is i32 and rows == M and hs[1] == 1, "logits_adjust: int32 history rows expected")
+    if mask is not None:
+        ms, (rows, words) = mask.stride(), mask.shape
+        _need(mask.dtype is i32 and rows == M and ms[1] == 1 and words * 32 >= V,
+              "logits_adjust: int32 mask rows of a bit per token expected")
+    _need((bias is None) == (bias_ids is None), "logits_adjust: a bias list needs its ids and values")
+    if bias is not None:
+        rows, n_bias = bias.shape
+        _need(bias.dtype is f32 and bias_ids.dtype is i32 and bias_ids.shape == (rows, n_bias) and rows == M and
+              bias.is_contiguous() and bias_ids.is_contiguous(), "logits_adjust: dense f32 biases of int32 ids expected")
+    lp = pp = rp = ep = fp = 0
+    ok = True
+    if history_lens is not None:
+        lp, ok = history_lens.data_ptr(), history_lens.dtype is i32 and history_lens.numel() == M
+    if prompt_lens is not None:
+        pp, ok = prompt_lens.data_ptr(), ok and prompt_lens.dtype is i32 and prompt_lens.numel() == M
+    if repetition is not None:
+        rp, ok = repetition.data_ptr(), ok and repetition.dtype is f32 and repetition.numel() == M
+    if presence is not None:
+        ep, ok = presence.data_ptr(), ok and presence.dtype is f32 and presence.numel() == M
+    if frequency is not None:
+        fp, ok = frequency.data_ptr(), ok and frequency.dtype is f32 and frequency.numel() == M
+    _need(ok, "logits_adjust: a length or penalty for each row expected")
+    _launch("logits_adjust", ARGS["logits_adjust"].pack(
+        logits.data_ptr(), xs[0], 0 if history is None else history.data_ptr(), hs[0], lp, pp, rp, ep,
+        fp,
+        0 if bias is None else bias_ids.data_ptr(), 0 if bias is None else bias.data_ptr(),
+        0 if mask is None else mask.data_ptr(), ms[0], out.data_ptr(), os_[0], M, V, width, n_bias), out, stream)
