@@ -32,6 +32,9 @@ namespace yskn {
 
 constexpr int PLAN_THREADS = 512;
 constexpr int PLAN_WARPS = PLAN_THREADS / 32;
+constexpr int PLAN_PER = YSKN_PLAN_MAX_BATCH / PLAN_THREADS;  // requests of a thread, at most
+// A thread's requests are adjacent: a place in 8 left free keeps its stores off each other's banks.
+__host__ __device__ constexpr int plan_at(int i) { return i + (i >> 3); }
 
 struct PlanParams {
   const int32_t* lens;
@@ -52,11 +55,13 @@ struct PlanParams {
   unsigned* err;
 };
 
+// Sums that stop at 2^31 - 1, which no array holds.
 struct Sum3 {
-  long long back, need, tokens;
+  unsigned back, need, tokens;
 };
+__device__ __forceinline__ unsigned plan_sum(unsigned a, unsigned b) { return min(a + b, (unsigned)INT32_MAX); }
 __device__ __forceinline__ Sum3 operator+(Sum3 a, Sum3 b) {
-  return {a.back + b.back, a.need + b.need, a.tokens + b.tokens};
+  return {plan_sum(a.back, b.back), plan_sum(a.need, b.need), plan_sum(a.tokens, b.tokens)};
 }
 
 struct PlanRequest {
@@ -64,12 +69,12 @@ struct PlanRequest {
   bool ended, too_long;
 };
 
-__device__ __forceinline__ PlanRequest plan_request(const PlanParams& p, int i) {
-  PlanRequest r{};
-  const int len = __ldg(p.lens + i), n = __ldg(p.new_lens + i);
+// From r.len and the new tokens in r.n.
+__device__ __forceinline__ void plan_request(const PlanParams& p, PlanRequest& r) {
   const unsigned bs = p.block_size;
-  r.len = len;
-  r.rows = len > p.prefix_len ? len - p.prefix_len : 0;
+  const int n = r.n;
+  r.n = 0;
+  r.rows = r.len > p.prefix_len ? r.len - p.prefix_len : 0;
   r.held = (int)((unsigned)r.rows / bs + ((unsigned)r.rows % bs != 0));
   r.ended = n < 0;
   r.too_long = r.held > p.table_width;
@@ -82,16 +87,27 @@ __device__ __forceinline__ PlanRequest plan_request(const PlanParams& p, int i) 
       r.fresh = total - r.held;
     }
   }
-  return r;
 }
 
-// Last index i in [0, n) with a[i] <= v (a ascending, a[0] <= v).
-__device__ __forceinline__ int last_at_most(const int* a, int n, int v) {
-  int lo = 0, hi = n;
+// Last index i in [lo, hi) with a[plan_at(i)] <= v (ascending, the first <= v).
+__device__ __forceinline__ int last_at_most(const int* a, int lo, int hi, int v) {
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (a[mid] <= v) lo = mid;
+    if (a[plan_at(mid)] <= v) lo = mid;
     else hi = mid;
+  }
+  return lo;
+}
+// The same for a whole warp's v: 32 probes a round.
+__device__ __forceinline__ int warp_last_at_most(const int* a, int n, int v) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0;
+  while (n > 1) {
+    const int step = (n + 31) >> 5, at = lane * step;
+    const unsigned below = __ballot_sync(0xffffffffu, at < n && a[plan_at(lo + min(at, n - 1))] <= v);
+    const int k = __popc(below) - 1;
+    lo += k * step;
+    n = min(step, n - k * step);
   }
   return lo;
 }
@@ -99,32 +115,34 @@ __device__ __forceinline__ int last_at_most(const int* a, int n, int v) {
 __global__ void __launch_bounds__(PLAN_THREADS) batch_plan_kernel(const __grid_constant__ PlanParams p) {
   extern __shared__ int s_plan[];
   const int B = p.batch;
-  int* s_start = s_plan;               // [B + 1] tokens, then first token, of each request
-  int* s_back = s_start + B + 1;       // [B + 1] blocks given back, then those before each request
-  int* s_need = s_back + B + 1;        // [B] fresh blocks, then those taken before each request
-  int* s_rows = s_need + B;            // [B]
+  const int room = plan_at(B) + 1;
+  int* s_start = s_plan;         // [B + 1] first token of each request
+  int* s_back = s_start + room;  // [B + 1] blocks given back before each request
+  int* s_need = s_back + room;   // [B] fresh blocks taken before each request
+  int* s_rows = s_need + room;   // [B]
   __shared__ Sum3 s_warp[PLAN_WARPS];
-  __shared__ Sum3 s_served;            // sums over the served requests
+  __shared__ uint2 s_served[PLAN_WARPS];  // need and tokens up to each warp's last served request
   __shared__ int s_any_long;
   pdl_begin();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int count = __ldg(p.free_count);
-  if (tid == 0) s_served = {0, 0, 0}, s_any_long = 0;
-  __syncthreads();
-  for (int i = tid; i < B; i += PLAN_THREADS) {
-    const PlanRequest r = plan_request(p, i);
-    s_start[i] = r.n;
-    s_back[i] = r.back;
-    s_need[i] = r.fresh;
-    s_rows[i] = r.rows;
-    if (r.too_long) s_any_long = 1;
-    if (blockIdx.x == 0) p.lens_out[i] = r.ended ? 0 : r.len;  // served ones below
+  if (tid == 0) s_any_long = 0;
+  const int per = (B + PLAN_THREADS - 1) / PLAN_THREADS, i0 = tid * per;
+  PlanRequest r[PLAN_PER];
+#pragma unroll
+  for (int k = 0; k < PLAN_PER; ++k) {
+    r[k] = PlanRequest{};
+    if (k < per && i0 + k < B) r[k].len = __ldg(p.lens + i0 + k), r[k].n = __ldg(p.new_lens + i0 + k);
   }
-  __syncthreads();
-  const int per = (B + PLAN_THREADS - 1) / PLAN_THREADS;
-  const int i0 = min(B, tid * per), i1 = min(B, i0 + per);
   Sum3 mine{0, 0, 0};
-  for (int i = i0; i < i1; ++i) mine = mine + Sum3{s_back[i], s_need[i], s_start[i]};
+  bool too_long = false;
+#pragma unroll
+  for (int k = 0; k < PLAN_PER; ++k) {
+    if (k >= per) break;
+    plan_request(p, r[k]);
+    mine = mine + Sum3{(unsigned)r[k].back, (unsigned)r[k].fresh, (unsigned)r[k].n};
+    too_long |= r[k].too_long;
+  }
   Sum3 incl = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -134,76 +152,101 @@ __global__ void __launch_bounds__(PLAN_THREADS) batch_plan_kernel(const __grid_c
   }
   if (lane == 31) s_warp[warp] = incl;
   __syncthreads();
+  if (too_long) s_any_long = 1;
+  // a thread's own part taken off again: exact unless a sum has stopped, and then nothing fits
   Sum3 before{incl.back - mine.back, incl.need - mine.need, incl.tokens - mine.tokens};
-  long long back_total = 0;
+  unsigned back_total = 0;
+#pragma unroll
   for (int w = 0; w < PLAN_WARPS; ++w) {
     const Sum3 o = s_warp[w];
     if (w < warp) before = before + o;
-    back_total += o.back;
+    back_total = plan_sum(back_total, o.back);
   }
   const int free0 = min(max(count, 0), p.pool_capacity);
-  const long long have = free0 + back_total;
+  const unsigned have = plan_sum(free0, back_total);
   // Served requests: both sums only grow, so the last served one's end is their total.
   Sum3 run = before, end{0, 0, 0};
-  for (int i = i0; i < i1; ++i) {
-    const int n = s_start[i];
-    const Sum3 next = run + Sum3{s_back[i], s_need[i], n};
-    const bool served = n > 0 && next.need <= have && next.tokens <= p.max_tokens;
+#pragma unroll
+  for (int k = 0; k < PLAN_PER; ++k) {
+    const int i = i0 + k;
+    if (k >= per || i >= B) break;
+    const Sum3 next = run + Sum3{(unsigned)r[k].back, (unsigned)r[k].fresh, (unsigned)r[k].n};
+    const bool served = r[k].n > 0 && next.need <= have && next.tokens <= (unsigned)p.max_tokens;
     if (served) end = next;
-    s_back[i] = (int)run.back;
-    s_need[i] = (int)min(run.need, (long long)INT32_MAX);
-    s_start[i] = (int)min(run.tokens, (long long)INT32_MAX);  // cut at the served total below
-    if (served && blockIdx.x == 0)
-      p.lens_out[i] = (int)min((long long)max(__ldg(p.lens + i), p.prefix_len) + n, (long long)INT32_MAX);
+    s_back[plan_at(i)] = (int)run.back;
+    s_need[plan_at(i)] = (int)run.need;
+    s_rows[plan_at(i)] = r[k].rows;
+    s_start[plan_at(i)] = (int)run.tokens;  // cut at the served total below
+    if (blockIdx.x == 0)
+      p.lens_out[i] = r[k].ended ? 0
+                      : served   ? (int)min((long long)max(r[k].len, p.prefix_len) + r[k].n, (long long)INT32_MAX)
+                                 : r[k].len;
     run = next;
   }
-  if (end.tokens > 0) {
-    atomicMax(reinterpret_cast<unsigned long long*>(&s_served.need), (unsigned long long)end.need);
-    atomicMax(reinterpret_cast<unsigned long long*>(&s_served.tokens), (unsigned long long)end.tokens);
-  }
+  const unsigned warp_need = __reduce_max_sync(0xffffffffu, end.need);
+  const unsigned warp_tokens = __reduce_max_sync(0xffffffffu, end.tokens);
+  if (lane == 0) s_served[warp] = make_uint2(warp_need, warp_tokens);
   __syncthreads();
-  const int total = (int)s_served.tokens;
-  const int left = (int)min(have - s_served.need, (long long)INT32_MAX);
+  unsigned taken = 0, tokens = 0;
+#pragma unroll
+  for (int w = 0; w < PLAN_WARPS; ++w) taken = max(taken, s_served[w].x), tokens = max(tokens, s_served[w].y);
+  const int total = (int)tokens, left = (int)(have - taken);
   for (int i = tid; i <= B; i += PLAN_THREADS) {
-    const int st = i < B ? min(s_start[i], total) : total;
-    s_start[i] = st;
-    if (i == B) s_back[B] = (int)back_total;
+    const int st = i < B ? min(s_start[plan_at(i)], total) : total;
+    s_start[plan_at(i)] = st;
+    if (i == B) s_back[plan_at(B)] = (int)back_total;
     if (blockIdx.x == 0) p.starts[i] = st;
   }
   if (blockIdx.x == 0 && tid == 0) {
     *p.free_out = left;
-    if (s_any_long || count != free0 || have > p.pool_capacity) raise_device_error(p.err, DERR_RANGE);
+    if (s_any_long || count != free0 || have > (unsigned)p.pool_capacity) raise_device_error(p.err, DERR_RANGE);
   }
   __syncthreads();
 
-  // Block number at place v of the stack with what came back on top.
-  auto stack_at = [&](int v) -> int {
+  // Block number at place v of the stack with what came back on top; the givers lie in [lo, hi).
+  auto stack_at = [&](int v, int lo, int hi) -> int {
     if (v < free0) return __ldg(p.pool + v);
     const int k = v - free0;
-    const int g = last_at_most(s_back, B, k);  // requests that give nothing share a start with the next one
-    return p.tables[(int64_t)g * p.table_stride + (k - s_back[g])];
+    const int g = last_at_most(s_back, lo, hi, k);  // requests that give nothing share a start with the next one
+    return p.tables[(int64_t)g * p.table_stride + (k - s_back[plan_at(g)])];
   };
   const int first = blockIdx.x * PLAN_THREADS + tid, step = gridDim.x * PLAN_THREADS;
-  for (int v = free0 + first; v < min(left, p.pool_capacity); v += step) p.pool[v] = stack_at(v);
-  for (int t = first; t < p.max_tokens; t += step) {
-    if (t >= total) {
-      p.slots[t] = -1;
-      p.positions[t] = -1;
-      p.requests[t] = -1;
+  for (int v = free0 + first; v < min(left, p.pool_capacity); v += step) p.pool[v] = stack_at(v, 0, B);
+  const unsigned bs = p.block_size;
+  for (int t0 = first - lane; t0 < p.max_tokens; t0 += step) {  // a warp's 32 tokens
+    const int t = t0 + lane;
+    if (t0 >= total) {
+      if (t < p.max_tokens) p.slots[t] = -1, p.positions[t] = -1, p.requests[t] = -1;
       continue;
     }
-    const int i = last_at_most(s_start, B, t);
-    const int rows = s_rows[i], row = rows + (t - s_start[i]);
-    const unsigned bs = p.block_size;
+    // the requests of the warp's first and last token bound the others'
+    const int last = min(t0 + 31, total - 1);
+    const int lo = warp_last_at_most(s_start, B, t0);
+    const int hi = warp_last_at_most(s_start, B, last);
+    const int i = last_at_most(s_start, lo, hi + 1, min(t, last));
+    const int rows = s_rows[plan_at(i)], row = rows + (min(t, last) - s_start[plan_at(i)]);
     const int held = (int)((unsigned)rows / bs + ((unsigned)rows % bs != 0));
     const int b = (int)((unsigned)row / bs), place = row - b * (int)bs;
+    // the stack's places taken fall from token to token: the givers of the ends bound the others'
+    const int v = (int)(have - 1 - s_need[plan_at(i)]) - (b - held);
+    const bool fresh = b >= held;
+    const int v_hi = __reduce_max_sync(0xffffffffu, fresh ? v : free0), v_lo = __reduce_min_sync(0xffffffffu, fresh ? v : INT32_MAX);
+    int g_lo = 0, g_hi = 1;
+    if (v_hi >= free0 && back_total > 0) {
+      g_lo = v_lo <= free0 ? 0 : warp_last_at_most(s_back, B, v_lo - free0);
+      g_hi = warp_last_at_most(s_back, B, v_hi - free0) + 1;
+    }
+    if (t > last) {
+      if (t < p.max_tokens) p.slots[t] = -1, p.positions[t] = -1, p.requests[t] = -1;
+      continue;
+    }
     int32_t* entry = p.tables + (int64_t)i * p.table_stride + b;
     int block;
-    if (b < held) {
-      block = *entry;
-    } else {
-      block = stack_at((int)(have - 1 - s_need[i]) - (b - held));
+    if (fresh) {
+      block = stack_at(v, g_lo, g_hi);
       if (place == 0) *entry = block;
+    } else {
+      block = *entry;
     }
     p.slots[t] = (int64_t)block * p.block_size + place;
     p.positions[t] = p.prefix_len + row;
@@ -229,9 +272,9 @@ extern "C" YSKN_B200_API int yskn_b200_batch_plan(const yskn_b200_batch_plan_arg
   PlanParams p{a.lens, a.new_lens, a.block_tables, a.table_stride, a.table_width, a.pool, a.pool_capacity, a.free,
                a.batch, a.block_size, a.prefix_len, a.max_tokens, a.lens_out, a.free_out, a.starts, a.slots,
                a.positions, a.requests, device_error_word()};
-  const size_t smem = (4 * (size_t)a.batch + 2) * sizeof(int);
+  const size_t smem = 4 * (size_t)(plan_at(a.batch) + 1) * sizeof(int);
   static SmemOptIn opt_in;
-  if (cudaError_t e = opt_in(batch_plan_kernel, (4 * YSKN_PLAN_MAX_BATCH + 2) * sizeof(int)))
+  if (cudaError_t e = opt_in(batch_plan_kernel, 4 * (plan_at(YSKN_PLAN_MAX_BATCH) + 1) * sizeof(int)))
     return cuda_fail(e, "batch_plan_kernel attributes");
   // Four tokens a thread, at most two CTAs an SM: more only repeat the prefix sums.
   const int grid = (int)std::min<int64_t>(ceil_div(std::max(a.max_tokens, 1), 4 * PLAN_THREADS), 296);

@@ -15,18 +15,21 @@
 // heads of 256 from f32). So one warp holds one head row in registers, lane l the channels
 // V l .. V l + V - 1 (V = D / 32): 16-byte accesses, the sum of squares by shuffles, and a
 // pair's other half R / 2 channels away is V-aligned in another lane, one shuffle per
-// channel. A CTA's 8 warps are 8 heads of one token, or 32 (four a warp) from PP_MANY rows on:
-// the token's R / 2 cosines and sines are computed once per CTA (shared memory) while the
-// rows' loads are in flight.
+// channel. A warp takes up to PP_RUN heads of one token where there are many rows (one where
+// there are few), each row requested two rows ahead, and computes the token's R / 2 cosines and
+// sines once, one pair a lane, while its first rows arrive. No block-wide step. The cosine and
+// sine are the portable ones of the decode path's rotation (binary64 reduction).
 #include <algorithm>
 
 #include "paged.cuh"
+#include "pmath.cuh"
 
 namespace yskn {
 
 constexpr int PP_WARPS = 8;
 constexpr int PP_MAX_PAIRS = YSKN_MAX_PAIRS;
-constexpr int PP_MANY = 16384;  // head rows of a call from which a warp takes four
+constexpr int PP_RUN = 8;         // heads of a warp's run, at most
+constexpr int PP_FULL = 148 * 16;  // warps that keep the SMs busy: runs get longer beyond that
 
 struct PagedPrepParams {
   const void *q, *k, *v;
@@ -38,6 +41,7 @@ struct PagedPrepParams {
   const uint16_t *q_norm, *k_norm;  // bf16 [D] or nullptr
   float eps;
   int tokens, n_qh, n_kvh, rot;
+  int run;  // heads of one token that a warp takes
   uint16_t* query;  // [tokens][n_qh][D]
   uint16_t *k_cache, *v_cache;
   CacheStrides cache;
@@ -91,99 +95,90 @@ __device__ __forceinline__ void store_row(uint16_t* p, const float (&x)[V]) {
   else *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <int SRC, int DT, int V, int R>
+template <int SRC, int DT, int V>
 __global__ void __launch_bounds__(PP_WARPS * 32) paged_prep_kernel(const __grid_constant__ PagedPrepParams p) {
   constexpr int D = 32 * V;
-  __shared__ float s_cos[PP_MAX_PAIRS], s_sin[PP_MAX_PAIRS];
+  __shared__ float2 s_turn[PP_WARPS][PP_MAX_PAIRS];  // (cosine, sine) of the warp's token
   pdl_begin();
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int heads = p.n_qh + 2 * p.n_kvh;  // query heads, then key heads, then value heads
-  const int groups = (heads + PP_WARPS * R - 1) / (PP_WARPS * R);
-  const int t = blockIdx.x / groups, h0 = (blockIdx.x - t * groups) * PP_WARPS * R + (threadIdx.x >> 5);
-  // kind: 0 query, 1 key, 2 value; hh the head among its kind
-  auto kind_of = [&](int h) { return h < p.n_qh ? 0 : (h < p.n_qh + p.n_kvh ? 1 : 2); };
-  auto head_of = [&](int h, int kind) { return kind == 0 ? h : (kind == 1 ? h - p.n_qh : h - p.n_qh - p.n_kvh); };
-  float x[R][V];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int h = h0 + r * PP_WARPS;
-    if (h >= heads) break;
-    const int kind = kind_of(h), hh = head_of(h, kind);
-    const void* src = kind == 0 ? p.q : (kind == 1 ? p.k : p.v);
-    const int64_t row = kind == 0 ? p.q_row : (kind == 1 ? p.k_row : p.v_row);
-    const int64_t head = kind == 0 ? p.q_head : (kind == 1 ? p.k_head : p.v_head);
-    load_row<SRC, V>(src, t * row + hh * head + lane * V, x[r]);
-  }
+  const int runs = (heads + p.run - 1) / p.run;
+  const int64_t item = (int64_t)blockIdx.x * PP_WARPS + warp;
+  if (item >= (int64_t)p.tokens * runs) return;
+  const int t = (int)(item / runs), h0 = (int)(item - (int64_t)t * runs) * p.run, h1 = min(heads, h0 + p.run);
+  auto load = [&](int h, float (&x)[V]) {
+    if (h < p.n_qh) load_row<SRC, V>(p.q, t * p.q_row + h * p.q_head + lane * V, x);
+    else if (h < p.n_qh + p.n_kvh) load_row<SRC, V>(p.k, t * p.k_row + (h - p.n_qh) * p.k_head + lane * V, x);
+    else load_row<SRC, V>(p.v, t * p.v_row + (h - p.n_qh - p.n_kvh) * p.v_head + lane * V, x);
+  };
+  float x[V], next[V];
+  load(h0, x);
+  if (h0 + 1 < h1) load(h0 + 1, next);
   const int64_t slot = __ldg(p.slots + t);
   const int half = p.rot >> 1;
-  if ((int)threadIdx.x < half) {
-    const float pos = (float)__ldg(p.positions + p.axis[threadIdx.x] * p.position_stride + t);
+  for (int i = lane; i < half; i += 32) {
+    const float pos = (float)__ldg(p.positions + p.axis[i] * p.position_stride + t);
     float sn, cs;
-    sincosf(__fmul_rn(pos, __ldg(p.inv_freq + threadIdx.x)), &sn, &cs);
-    s_cos[threadIdx.x] = cs;
-    s_sin[threadIdx.x] = sn;
+    if (!pm_sincos(__fmul_rn(pos, __ldg(p.inv_freq + i)), &cs, &sn)) raise_device_error(p.err, DERR_RANGE);
+    s_turn[warp][i] = make_float2(cs, sn);
   }
-  __syncthreads();
+  __syncwarp();
   const int lanes = half / V;  // lanes of each half of the rotated channels
   const bool low = lane < lanes, rotated = lane < 2 * lanes;
   const int other = rotated ? (low ? lane + lanes : lane - lanes) : lane;
   const int i0 = rotated ? (low ? lane : lane - lanes) * V : 0;
   const int64_t block = slot >= 0 ? slot / p.block_size : 0, place = slot - block * p.block_size;
   const int64_t to = block * p.cache.block + place * p.cache.token + lane * V;
-  if (slot >= p.n_slots && threadIdx.x == 0) raise_device_error(p.err, DERR_RANGE);
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int h = h0 + r * PP_WARPS;
-    if (h >= heads) break;
-    const int kind = kind_of(h), hh = head_of(h, kind);
-    if (kind != 2) {
-      const uint16_t* w = kind == 0 ? p.q_norm : p.k_norm;
+  if (slot >= p.n_slots && lane == 0) raise_device_error(p.err, DERR_RANGE);
+  for (int h = h0; h < h1; ++h) {
+    float after[V];
+    if (h + 2 < h1) load(h + 2, after);
+    const bool query = h < p.n_qh, value = h >= p.n_qh + p.n_kvh;
+    if (!value) {
+      const uint16_t* w = query ? p.q_norm : p.k_norm;
       if (w) {
+        float wt[V];
+        load_row<YSKN_DT_BF16, V>(w, lane * V, wt);
         float sum = 0.0f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) sum = fmaf(x[r][j], x[r][j], sum);
+        for (int j = 0; j < V; ++j) sum = fmaf(x[j], x[j], sum);
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
         const float inv = rsqrtf(sum * (1.0f / D) + p.eps);
-        float wt[V];
-        load_row<YSKN_DT_BF16, V>(w, lane * V, wt);
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[r][j] = x[r][j] * inv * (1.0f + wt[j]);
+        for (int j = 0; j < V; ++j) x[j] = x[j] * inv * (1.0f + wt[j]);
       }
-      if (p.rot) {
+      if (half) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float o = __shfl_sync(0xffffffffu, x[r][j], other);
-          const float cs = s_cos[i0 + j], sn = s_sin[i0 + j];
-          if (rotated) x[r][j] = low ? fmaf(x[r][j], cs, -(o * sn)) : fmaf(x[r][j], cs, o * sn);
+          const float o = __shfl_sync(0xffffffffu, x[j], other);
+          const float2 turn = s_turn[warp][i0 + j];
+          if (rotated) x[j] = low ? fmaf(x[j], turn.x, -(o * turn.y)) : fmaf(x[j], turn.x, o * turn.y);
         }
       }
     }
-    if (kind == 0) {
+    if (query) {
       if (slot < 0) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[r][j] = 0.0f;
+        for (int j = 0; j < V; ++j) x[j] = 0.0f;
       }
-      store_row<DT, V>(p.query + ((int64_t)t * p.n_qh + hh) * D + lane * V, x[r]);
+      store_row<DT, V>(p.query + ((int64_t)t * p.n_qh + h) * D + lane * V, x);
     } else if (slot >= 0 && slot < p.n_slots) {
-      store_row<DT, V>((kind == 1 ? p.k_cache : p.v_cache) + to + hh * p.cache.head, x[r]);
+      const int kvh = value ? h - p.n_qh - p.n_kvh : h - p.n_qh;
+      store_row<DT, V>((value ? p.v_cache : p.k_cache) + to + kvh * p.cache.head, x);
     }
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = next[j], next[j] = after[j];
   }
 }
 
-template <int SRC, int DT, int R>
-static cudaError_t launch_paged_prep(const PagedPrepParams& p, int head, cudaStream_t st) {
-  const unsigned grid = (unsigned)(p.tokens * ceil_div(p.n_qh + 2 * (int64_t)p.n_kvh, PP_WARPS * R));
-  switch (head) {
-    case 64: return launch_pdl(paged_prep_kernel<SRC, DT, 2, R>, grid, PP_WARPS * 32, 0, st, p);
-    case 128: return launch_pdl(paged_prep_kernel<SRC, DT, 4, R>, grid, PP_WARPS * 32, 0, st, p);
-    default: return launch_pdl(paged_prep_kernel<SRC, DT, 8, R>, grid, PP_WARPS * 32, 0, st, p);
-  }
-}
 template <int SRC, int DT>
-static cudaError_t launch_paged_prep(const PagedPrepParams& p, int head, cudaStream_t st) {
-  const int64_t rows = p.tokens * (p.n_qh + 2 * (int64_t)p.n_kvh);
-  return rows >= PP_MANY ? launch_paged_prep<SRC, DT, 4>(p, head, st) : launch_paged_prep<SRC, DT, 1>(p, head, st);
+static cudaError_t launch_paged_prep(const PagedPrepParams& p, int head, unsigned grid, cudaStream_t st) {
+  switch (head) {
+    case 64: return launch_pdl(paged_prep_kernel<SRC, DT, 2>, grid, PP_WARPS * 32, 0, st, p);
+    case 128: return launch_pdl(paged_prep_kernel<SRC, DT, 4>, grid, PP_WARPS * 32, 0, st, p);
+    default: return launch_pdl(paged_prep_kernel<SRC, DT, 8>, grid, PP_WARPS * 32, 0, st, p);
+  }
 }
 
 }  // namespace yskn
@@ -228,15 +223,17 @@ extern "C" YSKN_B200_API int yskn_b200_paged_prep(const yskn_b200_paged_prep_arg
   p.block_size = a.block_size, p.n_slots = (int64_t)a.n_blocks * a.block_size;
   p.err = device_error_word();
   for (int i = 0; i < a.rot / 2; ++i) p.axis[i] = a.axes[i];
-  if ((int64_t)a.tokens * ceil_div(a.n_qh + 2 * (int64_t)a.n_kvh, PP_WARPS) > (int64_t)INT32_MAX)
-    return fail(YSKN_EINVAL, "paged_prep: too many rows");
+  const int heads = a.n_qh + 2 * a.n_kvh;
+  p.run = (int)std::min<int64_t>(PP_RUN, std::max<int64_t>(1, (int64_t)a.tokens * heads / PP_FULL));
+  const int64_t grid = ceil_div(a.tokens * ceil_div(heads, p.run), PP_WARPS);
+  if (grid > (int64_t)INT32_MAX) return fail(YSKN_EINVAL, "paged_prep: too many rows");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (a.dtype == YSKN_DT_BF16)
-    e = a.source == YSKN_DT_F32 ? launch_paged_prep<YSKN_DT_F32, YSKN_DT_BF16>(p, a.head, st)
-                                : launch_paged_prep<YSKN_DT_BF16, YSKN_DT_BF16>(p, a.head, st);
+    e = a.source == YSKN_DT_F32 ? launch_paged_prep<YSKN_DT_F32, YSKN_DT_BF16>(p, a.head, (unsigned)grid, st)
+                                : launch_paged_prep<YSKN_DT_BF16, YSKN_DT_BF16>(p, a.head, (unsigned)grid, st);
   else
-    e = a.source == YSKN_DT_F32 ? launch_paged_prep<YSKN_DT_F32, YSKN_DT_F16>(p, a.head, st)
-                                : launch_paged_prep<YSKN_DT_F16, YSKN_DT_F16>(p, a.head, st);
+    e = a.source == YSKN_DT_F32 ? launch_paged_prep<YSKN_DT_F32, YSKN_DT_F16>(p, a.head, (unsigned)grid, st)
+                                : launch_paged_prep<YSKN_DT_F16, YSKN_DT_F16>(p, a.head, (unsigned)grid, st);
   return cuda_fail(e, "paged_prep_kernel");
 }

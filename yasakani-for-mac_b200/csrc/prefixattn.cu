@@ -43,7 +43,9 @@
 //           type over S's place, the row sum in binary32 of the unrounded weights. The maximum in
 //           use may lag: o and l are rescaled only when a row's maximum has grown by more than
 //           2^8, so that a weight is at most 256 and o is seldom touched; the join uses the
-//           maximum in use, which cancels.
+//           maximum in use, which cancels. (Two groups that take whole tiles in turn, so that one's
+//           exponentials run beside the other's loads, measured 134 against 110 us at 64 requests
+//           behind 32k rows: with two S tiles it is a tile's latency that counts. A share of the exponentials as polynomials on the FMA pipe: 117 to 119-123 us.)
 // A tile's rows past the last visible one: their scores are set to -inf before the maximum, P V
 // runs over the 16-row steps that hold a visible row, and warp 3 clears the rest of the last
 // step's V rows in shared memory (a zero weight does not silence a NaN).
@@ -83,7 +85,7 @@ struct PaShape {
 
 // The workspace: sizes from the host's bounds alone, so that both sides agree.
 struct PaWork {
-  int64_t base, item, pre_ml, pre_o, own_ml, own_o, bytes;  // byte offsets
+  int64_t base, pre_ml, pre_o, own_ml, own_o, bytes;  // byte offsets
   int own_half, own_rows;                                   // rows of a CTA and of the pair in an own item's place
   int64_t own_items;                                        // own items that there is room for
 };
@@ -99,8 +101,7 @@ inline PaWork pa_work(int tokens, int batch, int max_new, int n_qh, int n_kvh, i
   w.own_rows = max_new > tpc ? 2 * w.own_half : w.own_half;
   w.own_items = own_items;
   w.base = 256;
-  w.item = w.base + up((int64_t)batch * 4);
-  w.pre_ml = w.item + up(own_items * 4);
+  w.pre_ml = w.base + up((int64_t)batch * 8);
   w.pre_o = w.pre_ml + up(pre * 2 * PA_ROWS * 8);
   w.own_ml = w.pre_o + up(pre * 2 * PA_ROWS * head * 4);
   w.own_o = w.own_ml + up(own * w.own_rows * 8);
@@ -123,8 +124,7 @@ struct PrefixAttnParams {
   float c;  // |scale| log2 e
   uint32_t negate_q;
   int* work_per;          // units per pair of this call, for the join
-  int32_t* work_base;     // [batch] first own item of each request
-  int* work_item;         // [own items] first unit of each own item
+  int2* work_base;        // [batch] own items, and units of all items, before each request's own
   // per place: (m, l) of each row; o as [D / 4][rows][4], so that a warp's rows are adjacent
   float2 *pre_ml, *own_ml;
   float *pre_o, *own_o;
@@ -172,7 +172,15 @@ __device__ __forceinline__ int pa_own_tiles(const PrefixAttnParams& p, const PaR
 // Units of an item of so many tiles (0: nothing to do); unit u is tile u - PA_ITEM_COST.
 __host__ __device__ __forceinline__ int pa_units(int tiles) { return tiles > 0 ? tiles + PA_ITEM_COST : 0; }
 __device__ __forceinline__ int pa_qtiles(const PrefixAttnParams& p, const PaRequest& r) {
-  return (r.n + p.tpi - 1) / p.tpi;
+  return r.n <= p.tpi ? r.n > 0 : (r.n + p.tpi - 1) / p.tpi;
+}
+// Units of a request's own items of one KV head; sums of units stop at PA_MANY, which is an error.
+constexpr unsigned PA_MANY = 1u << 30;
+__device__ __forceinline__ unsigned pa_sum(unsigned a, unsigned b) { return min(a + b, PA_MANY); }
+__device__ __forceinline__ unsigned pa_own_units(const PrefixAttnParams& p, const PaRequest& r, int nq) {
+  unsigned u = 0;
+  for (int q = 0; q < nq; ++q) u = pa_sum(u, pa_units(pa_own_tiles(p, r, q)));
+  return u;
 }
 
 struct PaSegment {
@@ -183,41 +191,37 @@ struct PaSegment {
   int keys;             // rows on this axis that any of its tokens sees
   int first;            // own items: rows that token tok0 sees
   int64_t place;        // of its partial result
-  long long begin;      // the item's first unit
 };
 
 // Where a pair's units begin, found by each of its CTAs.
 struct PaStart {
-  long long left;  // units of this pair
-  int pre_item, u0;    // prefix item and unit in it
-  int req, item;       // own items: request and the items before it
-  long long skip;      // units of the request before this pair's first
-  long long unit;      // index of the first unit
+  int left;          // units of this pair
+  int pre_item, u0;  // prefix item and unit in it
+  int req, item;     // own items: request and the items before it
+  int skip;          // units of the request before this pair's first
 };
 
 // The pair's segments in order; every lane of a warp walks alike.
 struct PaWalk {
   const PrefixAttnParams& p;
-  long long left, unit;
-  int pre_item, u0, req, item, kvh, qt;
+  int left, pre_item, u0, req, item, kvh, qt;
   PaRequest r;
   int nq;
   bool loaded;
   __device__ PaWalk(const PrefixAttnParams& p_, const PaStart& s)
-      : p(p_), left(s.left), unit(s.unit), pre_item(s.pre_item), u0(s.u0), req(s.req), item(s.item), kvh(0), qt(0),
-        r{}, nq(0), loaded(false) {
+      : p(p_), left(s.left), pre_item(s.pre_item), u0(s.u0), req(s.req), item(s.item), kvh(0), qt(0), r{}, nq(0),
+        loaded(false) {
     if (s.skip > 0) {
       load();
-      long long skip = s.skip, head = 0;
-      for (int q = 0; q < nq; ++q) head += pa_units(pa_own_tiles(p, r, q));
-      kvh = (int)(skip / head);
-      skip -= kvh * head;
+      const int head = (int)pa_own_units(p, r, nq);
+      kvh = s.skip / head;
+      int skip = s.skip - kvh * head;
       for (;; ++qt) {
         const int u = pa_units(pa_own_tiles(p, r, qt));
         if (skip < u) break;
         skip -= u;
       }
-      u0 = (int)skip;
+      u0 = skip;
     }
   }
   __device__ void load() {
@@ -263,13 +267,11 @@ struct PaWalk {
   }
   // This pair's part of an item; false if it holds no tile.
   __device__ bool take(PaSegment& s, int tiles, int it) {
-    const int n = (int)min((long long)(tiles + PA_ITEM_COST - u0), left);
+    const int n = min(tiles + PA_ITEM_COST - u0, left);
     s.key0 = max(u0 - PA_ITEM_COST, 0);
     s.key1 = max(u0 + n - PA_ITEM_COST, 0);
     s.place = (int64_t)it + (blockIdx.x >> 1);
-    s.begin = unit - u0;
     left -= n;
-    unit += n;
     u0 = 0;
     return s.key0 < s.key1;
   }
@@ -393,7 +395,7 @@ struct PaShared {
   uint32_t tmem_slot;
   int abort_word;
   PaStart start;
-  long long sum[PA_THREADS / 32][2];
+  uint2 sum[PA_THREADS / 32];
   float half[2][2][PA_ROWS];  // tile parity, half, row: what a row's halves exchange
 };
 static_assert(sizeof(PaShared) <= 3072, "shared memory beside the ring");
@@ -428,74 +430,82 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
                  "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
-  pdl_begin();
-
-  // Unit counts of all requests and where this pair begins.
-  {
-    const int per = (p.batch + PA_THREADS - 1) / PA_THREADS;
-    const int i0 = min(p.batch, tid * per), i1 = min(p.batch, i0 + per);
-    long long tiles = 0, items = 0;
-    for (int i = i0; i < i1; ++i) {
-      const PaRequest r = pa_request(p, i);
-      const int nq = pa_qtiles(p, r);
-      long long t = 0;
-      for (int q = 0; q < nq; ++q) t += pa_units(pa_own_tiles(p, r, q));
-      tiles += t * p.n_kvh;
-      items += nq * p.n_kvh;
-      if (blockIdx.x == 0 && (__ldg(p.starts + i + 1) - r.s0 != r.n)) raise_device_error(p.err, DERR_RANGE);
-    }
-    long long ti = tiles, it = items;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const long long a = __shfl_up_sync(0xffffffffu, ti, off), b = __shfl_up_sync(0xffffffffu, it, off);
-      if (lane >= off) ti += a, it += b;
-    }
-    if (lane == 31) sh.sum[warp][0] = ti, sh.sum[warp][1] = it;
-    __syncthreads();
-    long long before = ti - tiles, items_before = it - items, total = 0, total_items = 0;
-    for (int w = 0; w < PA_THREADS / 32; ++w) {
-      if (w < warp) before += sh.sum[w][0], items_before += sh.sum[w][1];
-      total += sh.sum[w][0];
-      total_items += sh.sum[w][1];
-    }
-    const bool sound = total_items <= p.own_items && total <= INT32_MAX / 2;
-    const int pre_units = pa_units(p.pre_tiles);
-    const long long pre = (long long)p.pre_items * pre_units, all = sound ? pre + total : 0;
-    const long long share = sound ? max(1ll, (all + pairs - 1) / pairs) : 0;
-    const long long t0 = min(all, pair * share), t1 = min(all, t0 + share);
-    if (tid == 0) {
-      sh.start = {t1 - t0, p.pre_items, 0, 0, 0, 0, t0};
-      if (t0 < pre) {
-        sh.start.pre_item = (int)(t0 / pre_units);
-        sh.start.u0 = (int)(t0 - (long long)sh.start.pre_item * pre_units);
-      }
-      if (blockIdx.x == 0) {
-        *p.work_per = (int)share;
-        if (!sound) raise_device_error(p.err, DERR_RANGE);
-      }
-    }
-    __syncthreads();
-    const long long at = t0 - pre;  // this pair's first own unit
-    if (sound && ((at >= 0 && at >= before && at < before + tiles) || blockIdx.x == 0)) {
-      long long b = before;
-      int item = (int)items_before;
-      for (int i = i0; i < i1; ++i) {
-        const PaRequest r = pa_request(p, i);
-        const int nq = pa_qtiles(p, r);
-        long long t = 0;
-        for (int q = 0; q < nq; ++q) t += pa_units(pa_own_tiles(p, r, q));
-        t *= p.n_kvh;
-        if (at >= b && at < b + t) sh.start.req = i, sh.start.item = item, sh.start.skip = at - b;
-        if (blockIdx.x == 0) p.work_base[i] = item;
-        b += t;
-        item += nq * p.n_kvh;
-      }
-    }
+  if (warp == 2 && lane < 4) {
+    const CUtensorMap* map = lane == 0 ? &map_q_pre : lane == 1 ? &map_q_own : lane == 2 ? &map_k : &map_v;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
   }
   tc_fence_before();
   __syncthreads();
   cluster_sync();  // both CTAs' barriers are set up
   tc_fence_after();
+  pdl_begin();
+
+  // Unit counts of all requests and where this pair begins. A thread's requests are adjacent.
+  {
+    const int per = (p.batch + PA_THREADS - 1) / PA_THREADS;
+    const int i0 = min(p.batch, tid * per), i1 = min(p.batch, i0 + per);
+    unsigned units = 0, items = 0;
+    for (int i = i0; i < i1; ++i) {
+      const PaRequest r = pa_request(p, i);
+      const int nq = pa_qtiles(p, r);
+      units = pa_sum(units, (unsigned)min((unsigned long long)pa_own_units(p, r, nq) * p.n_kvh, (unsigned long long)PA_MANY));
+      items = pa_sum(items, (unsigned)min((unsigned long long)nq * p.n_kvh, (unsigned long long)PA_MANY));
+      if (blockIdx.x == 0 && (__ldg(p.starts + i + 1) - r.s0 != r.n)) raise_device_error(p.err, DERR_RANGE);
+    }
+    unsigned ui = units, it = items;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const unsigned a = __shfl_up_sync(0xffffffffu, ui, off), b = __shfl_up_sync(0xffffffffu, it, off);
+      if (lane >= off) ui = pa_sum(ui, a), it = pa_sum(it, b);
+    }
+    if (lane == 31) sh.sum[warp] = make_uint2(ui, it);
+    __syncthreads();
+    unsigned before = 0, items_before = 0, total = 0, total_items = 0;
+#pragma unroll
+    for (int w = 0; w < PA_THREADS / 32; ++w) {
+      const uint2 o = sh.sum[w];
+      if (w < warp) before = pa_sum(before, o.x), items_before = pa_sum(items_before, o.y);
+      total = pa_sum(total, o.x);
+      total_items = pa_sum(total_items, o.y);
+    }
+    before = pa_sum(before, ui - units);
+    items_before = pa_sum(items_before, it - items);
+    const bool sound = total_items <= (unsigned)p.own_items && total < PA_MANY;
+    const int pre_units = pa_units(p.pre_tiles), pre = p.pre_items * pre_units;  // below 2^30: the host looked
+    const int all = sound ? pre + (int)total : 0, share = (all + pairs - 1) / pairs;
+    const int t0 = min(all, pair * share), t1 = min(all, t0 + share);
+    const int at = t0 - pre;  // this pair's first own unit
+    if (tid == 0) {
+      PaStart s{t1 - t0, p.pre_items, 0, 0, 0, 0};
+      if (t0 < pre) {
+        s.pre_item = t0 / pre_units;
+        s.u0 = t0 - s.pre_item * pre_units;
+      }
+      sh.start = s;
+      if (blockIdx.x == 0) {
+        *p.work_per = share;
+        if (!sound) raise_device_error(p.err, DERR_RANGE);
+      }
+    }
+    __syncthreads();
+    if (sound && ((at >= (int)before && at < (int)(before + units)) || blockIdx.x == 0)) {
+      int b = (int)before, item = (int)items_before;
+      for (int i = i0; i < i1; ++i) {
+        int u = (int)units, n = (int)items;
+        if (per > 1) {
+          const PaRequest r = pa_request(p, i);
+          n = pa_qtiles(p, r);
+          u = (int)pa_own_units(p, r, n) * p.n_kvh;
+          n *= p.n_kvh;
+        }
+        if (at >= b && at < b + u) sh.start.req = i, sh.start.item = item, sh.start.skip = at - b;
+        if (blockIdx.x == 0) p.work_base[i] = make_int2(item, pre + b);
+        b += u;
+        item += n;
+      }
+    }
+  }
+  __syncthreads();
   const uint32_t tmem = sh.tmem_slot;
   PaWalk walk(p, sh.start);
   PaSegment seg;
@@ -753,7 +763,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
           uint32_t s[2][32];
           tmem_ld32(at + half * 64, s[0]);
           tmem_ld32(at + half * 64 + 32, s[1]);
-          tmem_ld_wait();
+          tmem_ld_wait32(s[0]);
+          tmem_ld_wait32(s[1]);
           if (least < (kt + 1) * PA_KEYS) {
             const int see = lim - kt * PA_KEYS - half * 64;
 #pragma unroll
@@ -839,8 +850,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
       }
       __syncwarp();
       if (lane == 0) arrive_first(o_free0);
-      if (!seg.prefix && seg.key0 == 0 && row == 0 && half == 0 && rank == 0)
-        p.work_item[seg.place - pair] = (int)seg.begin;
     }
   }
   tc_fence_before();
@@ -855,88 +864,89 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
 }
 
 // Joins the segments of each row. A warp takes 8 rows (in the order of the prefix items' rows)
-// and 64 channels: lane (r, q) row r, the channels 4 q .. 4 q + 3 of each 16, so that a load of
-// the warp is 4 runs of 128 adjacent bytes and a store 8 runs of 32.
+// of a KV head and 64 channels: lane (r, q) row r, the channels 4 q .. 4 q + 3 of each 16, so that
+// a load of the warp is 4 runs of 128 adjacent bytes and a store 8 runs of 32. What bounds it is
+// the chain of dependent loads (lengths, places, partial results): the maximum runs along, so
+// that all of a segment's loads are independent of the segments before it.
 template <int D, int DT>
 __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_constant__ PrefixAttnParams p) {
   constexpr int PARTS = D / 64;
   pdl_begin();
   const int lane = threadIdx.x & 31;
-  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int64_t kvh_rows = (int64_t)p.tokens * p.G, idx = unit / PARTS * 8 + (lane & 7);
-  if (idx >= kvh_rows * p.n_kvh) return;
-  const int ch = (int)(unit % PARTS) * 16 + (lane >> 3);  // of 4 channels; then every 4th
-  const int kvh = (int)(idx / kvh_rows);
-  const int64_t in_kvh = idx - kvh * kvh_rows;
-  const int t = (int)(in_kvh / p.G), gh = (int)(in_kvh - (int64_t)t * p.G);
+  const int unit = blockIdx.x * 8 + (threadIdx.x >> 5), idx = unit / PARTS * 8 + (lane & 7);
+  const int kvh = blockIdx.y, t = idx / p.G, gh = idx - t * p.G;
+  if (t >= p.tokens) return;
+  const int per = *p.work_per;
+  const int ch = (unit % PARTS) * 16 + (lane >> 3);  // of 4 channels; then every 4th
+  const int h = kvh * p.G + gh;
+  uint2 gate[4];
+  if (p.gate) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      gate[j] = __ldg(reinterpret_cast<const uint2*>(p.gate + t * p.gate_row + h * p.gate_head + (ch + 4 * j) * 4));
+  }
   float4 o[4];
   float den = 0.0f, top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < 4; ++j) o[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   const int i = request_of(p.starts, p.batch, t);
-  const int per = *p.work_per;
   const PaRequest r = i < p.batch ? pa_request(p, i) : PaRequest{};
   if (per > 0 && t >= r.s0 && t < r.s0 + r.n) {
-    // places of the row's segments: n_pre of its prefix item, then n_own of its own item
-    int n_pre = 0, n_own = 0, pre_row = 0;
-    int64_t pre0 = 0, own0 = 0;
+    const int2 base = p.work_base[i];
+    auto join = [&](const float2* ml, const float* from, int rows, int64_t place, int n, int row) {
+      ml += place * rows + row;
+      const float4* src = reinterpret_cast<const float4*>(from + place * rows * D) + ch * rows + row;
+#pragma unroll 4
+      for (int x = 0; x < n; ++x, ml += rows, src += rows * (D / 4)) {
+        const float2 v = *ml;
+        float4 y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = src[4 * j * rows];
+        const float now = fmaxf(top, v.x);
+        const float w = v.x == -INFINITY ? 0.0f : exp2_approx(v.x - now);
+        const float keep = top == -INFINITY ? 0.0f : exp2_approx(top - now);
+        top = now;
+        den = fmaf(den, keep, v.y * w);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          o[j].x = fmaf(o[j].x, keep, y[j].x * w);
+          o[j].y = fmaf(o[j].y, keep, y[j].y * w);
+          o[j].z = fmaf(o[j].z, keep, y[j].z * w);
+          o[j].w = fmaf(o[j].w, keep, y[j].w * w);
+        }
+      }
+    };
     if (p.pre_tiles > 0) {
       const int qt = t / p.tpi, it = kvh * p.pre_qtiles + qt, tl = t - qt * p.tpi, rank = tl >= p.tpc;
       const int b = it * pa_units(p.pre_tiles) + PA_ITEM_COST, c0 = b / per;
-      n_pre = (b + p.pre_tiles - 1) / per - c0 + 1;
-      pre0 = it + c0;
-      pre_row = rank * PA_ROWS + (tl - rank * p.tpc) * p.G + gh;
+      join(p.pre_ml, p.pre_o, 2 * PA_ROWS, it + c0, (b + p.pre_tiles - 1) / per - c0 + 1,
+           rank * PA_ROWS + (tl - rank * p.tpc) * p.G + gh);
     }
-    const int own_qt = (t - r.s0) / p.tpi, tl = t - r.s0 - own_qt * p.tpi, rank = tl >= p.tpc;
-    const int own_row = rank * p.own_half + (tl - rank * p.tpc) * p.G + gh;
+    const int nq = pa_qtiles(p, r), own_qt = nq > 1 ? (t - r.s0) / p.tpi : 0;
     const int kt = pa_own_tiles(p, r, own_qt);
     if (kt > 0) {
-      const int64_t it = (int64_t)p.work_base[i] + kvh * pa_qtiles(p, r) + own_qt;
-      const int b = p.work_item[it] + PA_ITEM_COST, c0 = b / per;
-      n_own = (b + kt - 1) / per - c0 + 1;
-      own0 = it + c0;
-    }
-    auto ml_of = [&](int x) {
-      return x < n_pre ? p.pre_ml[(pre0 + x) * 2 * PA_ROWS + pre_row] : p.own_ml[(own0 + x - n_pre) * p.own_rows + own_row];
-    };
-#pragma unroll 4
-    for (int x = 0; x < n_pre + n_own; ++x) top = fmaxf(top, ml_of(x).x);
-#pragma unroll 4
-    for (int x = 0; x < n_pre + n_own; ++x) {
-      const float2 v = ml_of(x);
-      const bool pre = x < n_pre;
-      const int rows = pre ? 2 * PA_ROWS : p.own_rows;
-      const float4* src = reinterpret_cast<const float4*>((pre ? p.pre_o : p.own_o) +
-                                                          (pre ? pre0 + x : own0 + x - n_pre) * rows * D) +
-                          (pre ? pre_row : own_row);
-      float4 y[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = src[(ch + 4 * j) * rows];
-      const float w = v.x == -INFINITY ? 0.0f : exp2f(v.x - top);
-      den = fmaf(v.y, w, den);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        o[j].x = fmaf(y[j].x, w, o[j].x);
-        o[j].y = fmaf(y[j].y, w, o[j].y);
-        o[j].z = fmaf(y[j].z, w, o[j].z);
-        o[j].w = fmaf(y[j].w, w, o[j].w);
-      }
+      const int tl = t - r.s0 - own_qt * p.tpi, rank = tl >= p.tpc;
+      int b = base.y + kvh * (int)pa_own_units(p, r, nq) + PA_ITEM_COST;
+      for (int q = 0; q < own_qt; ++q) b += pa_units(pa_own_tiles(p, r, q));
+      const int c0 = b / per;
+      join(p.own_ml, p.own_o, p.own_rows, base.x + kvh * nq + own_qt + c0, (b + kt - 1) / per - c0 + 1,
+           rank * p.own_half + (tl - rank * p.tpc) * p.G + gh);
     }
   }
-  const int h = kvh * p.G + gh;
   const float inv = den == 0.0f ? 0.0f : 1.0f / den;
   uint16_t* out = p.out + ((int64_t)t * p.n_kvh * p.G + h) * D;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int at = (ch + 4 * j) * 4;
     float v[4] = {o[j].x * inv, o[j].y * inv, o[j].z * inv, o[j].w * inv};
     if (p.gate) {
-      const uint2 g = *reinterpret_cast<const uint2*>(p.gate + t * p.gate_row + h * p.gate_head + at);
-      const uint16_t gs[4] = {(uint16_t)g.x, (uint16_t)(g.x >> 16), (uint16_t)g.y, (uint16_t)(g.y >> 16)};
+      const uint16_t gs[4] = {(uint16_t)gate[j].x, (uint16_t)(gate[j].x >> 16), (uint16_t)gate[j].y,
+                              (uint16_t)(gate[j].y >> 16)};
 #pragma unroll
-      for (int x = 0; x < 4; ++x) v[x] = v[x] / (1.0f + expf(-Elem<DT>::to_float(gs[x])));
+      for (int x = 0; x < 4; ++x)
+        v[x] = __fdividef(v[x], 1.0f + exp2_approx(-1.44269504f * Elem<DT>::to_float(gs[x])));
     }
-    *reinterpret_cast<uint2*>(out + at) = make_uint2(Elem<DT>::pack(v[0], v[1]), Elem<DT>::pack(v[2], v[3]));
+    *reinterpret_cast<uint2*>(out + (ch + 4 * j) * 4) =
+        make_uint2(Elem<DT>::pack(v[0], v[1]), Elem<DT>::pack(v[2], v[3]));
   }
 }
 
@@ -948,8 +958,8 @@ static int launch_prefix_attention(const CUtensorMap (&maps)[4], const PrefixAtt
   if (cudaError_t e = launch_pdl(prefix_attention_kernel<D, DT>, grid, PA_THREADS, PaShape<D>::SMEM, st, maps[0],
                                  maps[1], maps[2], maps[3], p))
     return cuda_fail(e, "prefix_attention_kernel");
-  const int64_t warps = ceil_div((int64_t)p.tokens * p.n_kvh * p.G, 8) * (D / 64);
-  return cuda_fail(launch_pdl(prefix_combine_kernel<D, DT>, (unsigned)ceil_div(warps, 8), 256, 0, st, p),
+  const int64_t warps = ceil_div((int64_t)p.tokens * p.G, 8) * (D / 64);
+  return cuda_fail(launch_pdl(prefix_combine_kernel<D, DT>, dim3((unsigned)ceil_div(warps, 8), p.n_kvh), 256, 0, st, p),
                    "prefix_combine_kernel");
 }
 
@@ -1020,15 +1030,15 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   p.tpc = tpc, p.tpi = 2 * tpc;
   p.pre_tiles = (int)ceil_div(a.prefix_len, PA_KEYS), p.pre_qtiles = (int)ceil_div(a.tokens, 2 * tpc);
   const int64_t items = (int64_t)p.pre_qtiles * n_kvh;
-  if (items * pa_units(p.pre_tiles) > INT32_MAX / 2) return fail(YSKN_EINVAL, "prefix_attention: too much work");
+  if (items * pa_units(p.pre_tiles) >= (int64_t)PA_MANY || (int64_t)a.tokens * n_qh * head > INT32_MAX || n_kvh > 65535)
+    return fail(YSKN_EINVAL, "prefix_attention: too much work");
   p.pre_items = a.prefix_len > 0 ? (int)items : 0;
   // a a.scale of zero keeps its meaning (equal weights) with a factor that leaves -inf alone
   p.c = std::max(std::fabs(a.scale) * 1.4426950408889634f, 1e-30f);
   p.negate_q = a.scale < 0.0f;
   uint8_t* work = reinterpret_cast<uint8_t*>(a.work);
   p.work_per = reinterpret_cast<int*>(work);
-  p.work_base = reinterpret_cast<int32_t*>(work + w.base);
-  p.work_item = reinterpret_cast<int*>(work + w.item);
+  p.work_base = reinterpret_cast<int2*>(work + w.base);
   p.pre_ml = reinterpret_cast<float2*>(work + w.pre_ml), p.pre_o = reinterpret_cast<float*>(work + w.pre_o);
   p.own_ml = reinterpret_cast<float2*>(work + w.own_ml), p.own_o = reinterpret_cast<float*>(work + w.own_o);
   p.own_half = w.own_half, p.own_rows = w.own_rows, p.own_items = w.own_items;
