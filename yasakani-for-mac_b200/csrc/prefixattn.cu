@@ -16,11 +16,16 @@
 //                 to) against the P prefix rows: the prefix is read once per 256 rows, not once
 //                 per request;
 //   own items     up to 256 rows of one request against that request's own rows.
+// Where requests have many tokens each (prompt chunks), 256 rows of one request read the prefix as
+// well as 256 rows of several do: then an own item takes the prefix's tiles before its own and
+// there are no prefix items, so that most rows are finished in one place. Every CTA decides this
+// alike from the units that either way takes (below).
 // Items are cut along their key tiles (128 rows of the cache) so that every pair of SMs gets the
 // same share: an item counts PA_ITEM_COST units and one per tile, and pair c takes units
 // [c per, (c + 1) per) of all items in order. A piece of an item is a segment; its unnormalised
 // (m, l, o) goes to the workspace in binary32, at place item + c, which no two segments share,
-// and prefix_combine_kernel joins a row's segments, divides, gates and rounds. Everything is
+// and prefix_combine_kernel joins a row's segments, divides, gates and rounds; a segment that holds
+// all that its rows see finishes them itself. Everything is
 // summed in a fixed order: the same call gives the same bits. The lengths stay on the device:
 // every CTA forms the prefix sum of the requests' units itself.
 //
@@ -67,7 +72,7 @@ constexpr int PA_SLOT = 16384;  // bytes per ring slot
 constexpr int PA_THREADS = 384;
 constexpr int PA_MAX_PAIRS = 74;
 constexpr int PA_MAX_SLOTS = 12;
-constexpr int PA_ITEM_COST = 2;  // an item's fixed cost (Q, the last P V's wait, its result) in tiles
+constexpr int PA_ITEM_COST = 3;  // an item's fixed cost (Q, the last P V's wait, its result) in tiles
 
 template <int D>
 struct PaShape {
@@ -120,10 +125,10 @@ struct PrefixAttnParams {
   int own_limit;  // rows that a table row can name
   int batch, tokens, max_new, n_kvh, G;
   int tpc, tpi;  // tokens per CTA and per item
-  int pre_tiles, pre_qtiles, pre_items;
+  int pre_tiles, pre_qtiles, shared_items;  // prefix items, if there are any
   float c;  // |scale| log2 e
   uint32_t negate_q;
-  int* work_per;          // units per pair of this call, for the join
+  int2* work_per;         // units per pair of this call, and whether alone: for the join
   int2* work_base;        // [batch] own items, and units of all items, before each request's own
   // per place: (m, l) of each row; o as [D / 4][rows][4], so that a warp's rows are adjacent
   float2 *pre_ml, *own_ml;
@@ -174,28 +179,38 @@ __host__ __device__ __forceinline__ int pa_units(int tiles) { return tiles > 0 ?
 __device__ __forceinline__ int pa_qtiles(const PrefixAttnParams& p, const PaRequest& r) {
   return r.n <= p.tpi ? r.n > 0 : (r.n + p.tpi - 1) / p.tpi;
 }
-// Units of a request's own items of one KV head; sums of units stop at PA_MANY, which is an error.
+// Tiles of a request's item `qt`: own ones, after the prefix's where there are no prefix items.
+__device__ __forceinline__ int pa_tiles(const PrefixAttnParams& p, const PaRequest& r, int qt, bool alone) {
+  return pa_own_tiles(p, r, qt) + (alone ? p.pre_tiles : 0);
+}
+// Units of a request's items of one KV head; sums of units stop at PA_MANY, which is an error.
 constexpr unsigned PA_MANY = 1u << 30;
 __device__ __forceinline__ unsigned pa_sum(unsigned a, unsigned b) { return min(a + b, PA_MANY); }
-__device__ __forceinline__ unsigned pa_own_units(const PrefixAttnParams& p, const PaRequest& r, int nq) {
+__device__ __forceinline__ unsigned pa_own_units(const PrefixAttnParams& p, const PaRequest& r, int nq, bool alone) {
   unsigned u = 0;
-  for (int q = 0; q < nq; ++q) u = pa_sum(u, pa_units(pa_own_tiles(p, r, q)));
+  for (int q = 0; q < nq; ++q) u = pa_sum(u, pa_units(pa_tiles(p, r, q, alone)));
   return u;
 }
 
 struct PaSegment {
-  bool prefix;
+  bool prefix, whole;   // prefix item; all that its rows see
   int kvh, tok0, ntok;  // KV head, first token and whole tokens
   int req;              // own items: the request
+  int pre;              // the item's first tiles that are the prefix's
   int key0, key1;       // key tiles [key0, key1)
-  int keys;             // rows on this axis that any of its tokens sees
-  int first;            // own items: rows that token tok0 sees
+  int keys;             // own rows that any of its tokens sees
+  int first;            // own items: rows of the sequence that token tok0 sees
   int64_t place;        // of its partial result
+  // Rows of tile kt that the rows on its axis leave it.
+  __device__ int rows_of(const PrefixAttnParams& p, int kt) const {
+    return min(PA_KEYS, kt < pre ? p.prefix_len - kt * PA_KEYS : keys - (kt - pre) * PA_KEYS);
+  }
 };
 
 // Where a pair's units begin, found by each of its CTAs.
 struct PaStart {
   int left;          // units of this pair
+  int alone;         // no prefix items: each request's items take the prefix too
   int pre_item, u0;  // prefix item and unit in it
   int req, item;     // own items: request and the items before it
   int skip;          // units of the request before this pair's first
@@ -204,20 +219,21 @@ struct PaStart {
 // The pair's segments in order; every lane of a warp walks alike.
 struct PaWalk {
   const PrefixAttnParams& p;
+  const bool alone;
   int left, pre_item, u0, req, item, kvh, qt;
   PaRequest r;
   int nq;
   bool loaded;
   __device__ PaWalk(const PrefixAttnParams& p_, const PaStart& s)
-      : p(p_), left(s.left), pre_item(s.pre_item), u0(s.u0), req(s.req), item(s.item), kvh(0), qt(0), r{}, nq(0),
-        loaded(false) {
+      : p(p_), alone(s.alone), left(s.left), pre_item(s.pre_item), u0(s.u0), req(s.req), item(s.item), kvh(0), qt(0),
+        r{}, nq(0), loaded(false) {
     if (s.skip > 0) {
       load();
-      const int head = (int)pa_own_units(p, r, nq);
+      const int head = (int)pa_own_units(p, r, nq, alone);
       kvh = s.skip / head;
       int skip = s.skip - kvh * head;
       for (;; ++qt) {
-        const int u = pa_units(pa_own_tiles(p, r, qt));
+        const int u = pa_units(pa_tiles(p, r, qt, alone));
         if (skip < u) break;
         skip -= u;
       }
@@ -231,13 +247,14 @@ struct PaWalk {
   }
   // The next segment; false past the last.
   __device__ bool next(PaSegment& s) {
-    while (left > 0 && pre_item < p.pre_items) {
+    while (left > 0 && !alone && pre_item < p.shared_items) {
       s.prefix = true;
       s.kvh = pre_item / p.pre_qtiles;
       s.tok0 = (pre_item - s.kvh * p.pre_qtiles) * p.tpi;
       s.ntok = min(p.tpi, p.tokens - s.tok0);
       s.req = 0;
-      s.keys = p.prefix_len;
+      s.pre = p.pre_tiles;
+      s.keys = 0;
       s.first = 0;
       ++pre_item;
       if (take(s, p.pre_tiles, pre_item - 1)) return true;
@@ -246,15 +263,16 @@ struct PaWalk {
       if (!loaded) load();
       for (; kvh < p.n_kvh; ++kvh, qt = 0)
         while (qt < nq) {
-          const int q = qt++, kt = pa_own_tiles(p, r, q);
+          const int q = qt++, kt = pa_tiles(p, r, q, alone);
           if (kt == 0) continue;
           s.prefix = false;
           s.kvh = kvh;
           s.tok0 = r.s0 + q * p.tpi;
           s.ntok = min(p.tpi, r.n - q * p.tpi);
           s.req = req;
+          s.pre = alone ? p.pre_tiles : 0;
           s.keys = pa_visible(p, r, q * p.tpi + s.ntok);
-          s.first = r.len - r.n + q * p.tpi + 1 - p.prefix_len;
+          s.first = r.len - r.n + q * p.tpi + 1;
           if (take(s, kt, item + kvh * nq + q)) return true;
           if (left <= 0) return false;
         }
@@ -270,6 +288,7 @@ struct PaWalk {
     const int n = min(tiles + PA_ITEM_COST - u0, left);
     s.key0 = max(u0 - PA_ITEM_COST, 0);
     s.key1 = max(u0 + n - PA_ITEM_COST, 0);
+    s.whole = !s.prefix && s.key0 == 0 && s.key1 == tiles && s.pre == p.pre_tiles;
     s.place = (int64_t)it + (blockIdx.x >> 1);
     left -= n;
     u0 = 0;
@@ -377,6 +396,10 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return y;
 }
+template <int DT>
+__device__ __forceinline__ float gated(float x, uint16_t gate) {
+  return __fdividef(x, 1.0f + exp2_approx(-1.44269504f * Elem<DT>::to_float(gate)));
+}
 // Both warps of a row quarter.
 __device__ __forceinline__ void quarter_sync(int quarter) {
   asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
@@ -395,7 +418,7 @@ struct PaShared {
   uint32_t tmem_slot;
   int abort_word;
   PaStart start;
-  uint2 sum[PA_THREADS / 32];
+  uint3 sum[PA_THREADS / 32];
   float half[2][2][PA_ROWS];  // tile parity, half, row: what a row's halves exchange
 };
 static_assert(sizeof(PaShared) <= 3072, "shared memory beside the ring");
@@ -444,46 +467,60 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
   {
     const int per = (p.batch + PA_THREADS - 1) / PA_THREADS;
     const int i0 = min(p.batch, tid * per), i1 = min(p.batch, i0 + per);
-    unsigned units = 0, items = 0;
+    unsigned items = 0, units_of[2] = {0, 0};  // beside prefix items, and alone
     for (int i = i0; i < i1; ++i) {
       const PaRequest r = pa_request(p, i);
       const int nq = pa_qtiles(p, r);
-      units = pa_sum(units, (unsigned)min((unsigned long long)pa_own_units(p, r, nq) * p.n_kvh, (unsigned long long)PA_MANY));
-      items = pa_sum(items, (unsigned)min((unsigned long long)nq * p.n_kvh, (unsigned long long)PA_MANY));
+      auto times = [&](unsigned n) { return (unsigned)min((unsigned long long)n * p.n_kvh, (unsigned long long)PA_MANY); };
+      units_of[0] = pa_sum(units_of[0], times(pa_own_units(p, r, nq, false)));
+      units_of[1] = pa_sum(units_of[1], times(pa_own_units(p, r, nq, true)));
+      items = pa_sum(items, times(nq));
       if (blockIdx.x == 0 && (__ldg(p.starts + i + 1) - r.s0 != r.n)) raise_device_error(p.err, DERR_RANGE);
     }
-    unsigned ui = units, it = items;
+    unsigned ui[2] = {units_of[0], units_of[1]}, it = items;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const unsigned a = __shfl_up_sync(0xffffffffu, ui, off), b = __shfl_up_sync(0xffffffffu, it, off);
-      if (lane >= off) ui = pa_sum(ui, a), it = pa_sum(it, b);
+      const unsigned a = __shfl_up_sync(0xffffffffu, ui[0], off), b = __shfl_up_sync(0xffffffffu, ui[1], off);
+      const unsigned c = __shfl_up_sync(0xffffffffu, it, off);
+      if (lane >= off) ui[0] = pa_sum(ui[0], a), ui[1] = pa_sum(ui[1], b), it = pa_sum(it, c);
     }
-    if (lane == 31) sh.sum[warp] = make_uint2(ui, it);
+    if (lane == 31) sh.sum[warp] = make_uint3(ui[0], ui[1], it);
     __syncthreads();
-    unsigned before = 0, items_before = 0, total = 0, total_items = 0;
+    unsigned before_of[2] = {0, 0}, total_of[2] = {0, 0}, items_before = 0, total_items = 0;
 #pragma unroll
     for (int w = 0; w < PA_THREADS / 32; ++w) {
-      const uint2 o = sh.sum[w];
-      if (w < warp) before = pa_sum(before, o.x), items_before = pa_sum(items_before, o.y);
-      total = pa_sum(total, o.x);
-      total_items = pa_sum(total_items, o.y);
+      const uint3 o = sh.sum[w];
+      if (w < warp) {
+        before_of[0] = pa_sum(before_of[0], o.x);
+        before_of[1] = pa_sum(before_of[1], o.y);
+        items_before = pa_sum(items_before, o.z);
+      }
+      total_of[0] = pa_sum(total_of[0], o.x);
+      total_of[1] = pa_sum(total_of[1], o.y);
+      total_items = pa_sum(total_items, o.z);
     }
-    before = pa_sum(before, ui - units);
+    // Alone, if that is at most an eighth more: about what the join of two results per row costs
+    // (16 prompt chunks: 960 us with prefix items, ALONE us alone).
+    const int pre_units = pa_units(p.pre_tiles), pre_all = p.shared_items * pre_units;  // below 2^30: the host looked
+    const bool alone = p.shared_items > 0 && total_of[1] < PA_MANY &&
+                       8ull * total_of[1] <= 9ull * ((unsigned)pre_all + total_of[0]);
+    const unsigned units = alone ? units_of[1] : units_of[0], total = alone ? total_of[1] : total_of[0];
+    const unsigned before = pa_sum(alone ? before_of[1] : before_of[0], alone ? ui[1] - units_of[1] : ui[0] - units_of[0]);
     items_before = pa_sum(items_before, it - items);
     const bool sound = total_items <= (unsigned)p.own_items && total < PA_MANY;
-    const int pre_units = pa_units(p.pre_tiles), pre = p.pre_items * pre_units;  // below 2^30: the host looked
+    const int pre_items = alone ? 0 : p.shared_items, pre = alone ? 0 : pre_all;
     const int all = sound ? pre + (int)total : 0, share = (all + pairs - 1) / pairs;
     const int t0 = min(all, pair * share), t1 = min(all, t0 + share);
     const int at = t0 - pre;  // this pair's first own unit
     if (tid == 0) {
-      PaStart s{t1 - t0, p.pre_items, 0, 0, 0, 0};
+      PaStart s{t1 - t0, alone, pre_items, 0, 0, 0, 0};
       if (t0 < pre) {
         s.pre_item = t0 / pre_units;
         s.u0 = t0 - s.pre_item * pre_units;
       }
       sh.start = s;
       if (blockIdx.x == 0) {
-        *p.work_per = share;
+        *p.work_per = make_int2(share, alone);
         if (!sound) raise_device_error(p.err, DERR_RANGE);
       }
     }
@@ -495,7 +532,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
         if (per > 1) {
           const PaRequest r = pa_request(p, i);
           n = pa_qtiles(p, r);
-          u = (int)pa_own_units(p, r, n) * p.n_kvh;
+          u = (int)pa_own_units(p, r, n, alone) * p.n_kvh;
           n *= p.n_kvh;
         }
         if (at >= b && at < b + u) sh.start.req = i, sh.start.item = item, sh.start.skip = at - b;
@@ -522,13 +559,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
     const uint32_t full0 = first_cta(&sh.full[0]);
     const int v_chunk = D == 64 ? 0 : rank * Shape::V_CHUNKS, v_x = D == 64 ? rank * 32 : 0;
     while (ok && walk.next(seg)) {
-      const int32_t* table = seg.prefix ? p.prefix_blocks : p.tables + (int64_t)seg.req * p.table_stride;
-      const int page_end = (seg.keys + (1 << shift) - 1) >> shift;
       auto block_of = [&](int kt) {  // lane l: the block of page l of tile kt
-        const int at = kt * pages + lane;
         int b = 0;
-        if (lane < pages && kt < seg.key1 && at < page_end) {
-          b = __ldg(table + at);
+        if (kt < seg.key1 && lane < pages && (lane << shift) < seg.rows_of(p, kt)) {
+          b = __ldg(kt < seg.pre ? p.prefix_blocks + kt * pages + lane
+                                 : p.tables + (int64_t)seg.req * p.table_stride + (kt - seg.pre) * pages + lane);
           if ((unsigned)b >= (unsigned)p.n_blocks) raise_device_error(p.err, DERR_RANGE);  // the copy gives zeros
         }
         return b;
@@ -556,7 +591,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
         }
       };
       auto put_k = [&](int kt, int block) {
-        const int nk = min(max(seg.keys - kt * PA_KEYS - rank * (PA_KEYS / 2), 0), PA_KEYS / 2);
+        const int nk = min(max(seg.rows_of(p, kt) - rank * (PA_KEYS / 2), 0), PA_KEYS / 2);
         const int n = (nk + box_k - 1) / box_k;
         for (int d = 0; ok && d < SLOTS; ++d) {
           uint8_t* to = claim();
@@ -570,7 +605,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
         }
       };
       auto put_v = [&](int kt, int block) {
-        const int nk = min(PA_KEYS, seg.keys - kt * PA_KEYS);
+        const int nk = seg.rows_of(p, kt);
         for (int v = 0; ok && v * VR < nk; ++v) {
           const int rows = min(VR, nk - v * VR), n = (rows + box_v - 1) / box_v;
           uint8_t* to = claim();
@@ -673,7 +708,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
           ok = ok && mbar_wait(&sh.p_full[g & 1], (g >> 1) & 1, abort_flag);
           if (!ok) break;
           tc_fence_after();
-          const int nk = min(PA_KEYS, seg.keys - (seg.key0 + j) * PA_KEYS);
+          const int nk = seg.rows_of(p, seg.key0 + j);
           pv(nk, tmem + Shape::S_COL + (g & 1) * PA_KEYS, j == 0);
           if (ok) umma2_commit(&sh.pv_done[g & 1]);
         }
@@ -738,20 +773,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
     while (walk.next(seg)) {
       const int tl = rank * p.tpc + row / p.G;  // token of the item
       const bool valid = row / p.G < p.tpc && tl < seg.ntok;
-      int lim = 0;  // rows on this axis that the row sees
+      int lim = 0;  // rows of the sequence that the row sees
       if (valid) {
         if (seg.prefix) {
           const int i = request_of(p.starts, p.batch, seg.tok0 + tl);
           if (i < p.batch) {
             const PaRequest r = pa_request(p, i);
-            lim = min(max(r.len - r.n + (seg.tok0 + tl - r.s0) + 1, 0), p.prefix_len);
+            lim = max(r.len - r.n + (seg.tok0 + tl - r.s0) + 1, 0);
           }
         } else {
-          lim = min(max(seg.first + tl, 0), seg.keys);
+          lim = max(seg.first + tl, 0);
         }
       }
       const bool live = __any_sync(0xffffffffu, valid);  // a warp without rows only keeps the barriers going
-      const int least = __reduce_min_sync(0xffffffffu, valid ? lim : INT32_MAX);
+      // on either axis, and the least of the warp's rows
+      const int lim_pre = min(lim, p.prefix_len), lim_own = min(max(lim - p.prefix_len, 0), seg.keys);
+      const int least_pre = __reduce_min_sync(0xffffffffu, valid ? lim_pre : INT32_MAX);
+      const int least_own = __reduce_min_sync(0xffffffffu, valid ? lim_own : INT32_MAX);
       float m = -INFINITY, l = 0.0f;
       for (int kt = seg.key0; kt < seg.key1; ++kt, ++g) {
         const int b = g & 1;
@@ -765,8 +803,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
           tmem_ld32(at + half * 64 + 32, s[1]);
           tmem_ld_wait32(s[0]);
           tmem_ld_wait32(s[1]);
-          if (least < (kt + 1) * PA_KEYS) {
-            const int see = lim - kt * PA_KEYS - half * 64;
+          const bool pre = kt < seg.pre;
+          const int from = (pre ? kt : kt - seg.pre) * PA_KEYS;  // the tile's first row on its axis
+          if ((pre ? least_pre : least_own) < from + PA_KEYS) {
+            const int see = (pre ? lim_pre : lim_own) - from - half * 64;
 #pragma unroll
             for (int x = 0; x < 64; ++x)
               if (x >= see) s[x >> 5][x & 31] = 0xff800000u;  // -inf
@@ -826,27 +866,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
       __syncwarp();
       if (live) {
         tc_fence_after();
-        const int rows = seg.prefix ? 2 * PA_ROWS : p.own_rows;
-        const int at = rank * (seg.prefix ? PA_ROWS : p.own_half) + row;  // of the place
-        float4* o = reinterpret_cast<float4*>((seg.prefix ? p.pre_o : p.own_o) + seg.place * rows * D) + at;
-        for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
-          uint32_t v[32];
-          tmem_ld32(tmem + lanes + x, v);
-          tmem_ld_wait();
-          if (valid) {
-#pragma unroll
-            for (int y = 0; y < 32; y += 4)
-              o[(x + y) / 4 * rows] = make_float4(__uint_as_float(v[y]), __uint_as_float(v[y + 1]),
-                                                  __uint_as_float(v[y + 2]), __uint_as_float(v[y + 3]));
-          }
-        }
-        tc_fence_before();
         quarter_sync(quarter);  // the tiles' exchanges have been read
         sh.half[0][half][row] = l;
         quarter_sync(quarter);
-        if (valid && half == 0)
-          ((seg.prefix ? p.pre_ml : p.own_ml) + seg.place * rows)[at] = make_float2(m, l + sh.half[0][1][row]);
-        quarter_sync(quarter);
+        l += sh.half[0][half ^ 1][row];
+        if (seg.whole) {
+          const int h = seg.kvh * p.G + row % p.G;
+          const int64_t t = seg.tok0 + tl;
+          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+          uint16_t* out = p.out + (t * p.n_kvh * p.G + h) * D;
+          const uint16_t* gate = p.gate + t * p.gate_row + h * p.gate_head;
+          for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
+            uint32_t v[32];
+            tmem_ld32(tmem + lanes + x, v);
+            tmem_ld_wait32(v);
+            if (valid) {
+#pragma unroll
+              for (int y = 0; y < 32; y += 8) {
+                float z[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) z[k] = __uint_as_float(v[y + k]) * inv;
+                if (p.gate) {
+                  const uint4 g4 = __ldg(reinterpret_cast<const uint4*>(gate + x + y));
+                  const uint32_t gs[4] = {g4.x, g4.y, g4.z, g4.w};
+#pragma unroll
+                  for (int k = 0; k < 8; ++k) z[k] = gated<DT>(z[k], (uint16_t)(gs[k >> 1] >> (k & 1) * 16));
+                }
+                *reinterpret_cast<uint4*>(out + x + y) =
+                    make_uint4(Elem<DT>::pack(z[0], z[1]), Elem<DT>::pack(z[2], z[3]), Elem<DT>::pack(z[4], z[5]),
+                               Elem<DT>::pack(z[6], z[7]));
+              }
+            }
+          }
+        } else {
+          const int rows = seg.prefix ? 2 * PA_ROWS : p.own_rows;
+          const int at = rank * (seg.prefix ? PA_ROWS : p.own_half) + row;  // of the place
+          float4* o = reinterpret_cast<float4*>((seg.prefix ? p.pre_o : p.own_o) + seg.place * rows * D) + at;
+          for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
+            uint32_t v[32];
+            tmem_ld32(tmem + lanes + x, v);
+            tmem_ld_wait32(v);
+            if (valid) {
+#pragma unroll
+              for (int y = 0; y < 32; y += 4)
+                o[(x + y) / 4 * rows] = make_float4(__uint_as_float(v[y]), __uint_as_float(v[y + 1]),
+                                                    __uint_as_float(v[y + 2]), __uint_as_float(v[y + 3]));
+            }
+          }
+          if (valid && half == 0)
+            ((seg.prefix ? p.pre_ml : p.own_ml) + seg.place * rows)[at] = make_float2(m, l);
+        }
+        tc_fence_before();
+        quarter_sync(quarter);  // the halves' sums have been read
       }
       __syncwarp();
       if (lane == 0) arrive_first(o_free0);
@@ -876,7 +947,9 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
   const int unit = blockIdx.x * 8 + (threadIdx.x >> 5), idx = unit / PARTS * 8 + (lane & 7);
   const int kvh = blockIdx.y, t = idx / p.G, gh = idx - t * p.G;
   if (t >= p.tokens) return;
-  const int per = *p.work_per;
+  const int2 how = *p.work_per;
+  const int per = how.x;
+  const bool alone = how.y;
   const int ch = (unit % PARTS) * 16 + (lane >> 3);  // of 4 channels; then every 4th
   const int h = kvh * p.G + gh;
   uint2 gate[4];
@@ -916,20 +989,25 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
         }
       }
     };
-    if (p.pre_tiles > 0) {
+    const int nq = pa_qtiles(p, r), own_qt = nq > 1 ? (t - r.s0) / p.tpi : 0;
+    const int kt = pa_tiles(p, r, own_qt, alone);
+    int c0 = 0, n = 0;
+    if (kt > 0) {
+      int b = base.y + kvh * (int)pa_own_units(p, r, nq, alone) + PA_ITEM_COST;
+      for (int q = 0; q < own_qt; ++q) b += pa_units(pa_tiles(p, r, q, alone));
+      c0 = b / per;
+      n = (b + kt - 1) / per - c0 + 1;
+    }
+    if (n == 1 && (alone || p.pre_tiles == 0)) return;  // finished where it was computed
+    if (!alone && p.pre_tiles > 0) {
       const int qt = t / p.tpi, it = kvh * p.pre_qtiles + qt, tl = t - qt * p.tpi, rank = tl >= p.tpc;
-      const int b = it * pa_units(p.pre_tiles) + PA_ITEM_COST, c0 = b / per;
-      join(p.pre_ml, p.pre_o, 2 * PA_ROWS, it + c0, (b + p.pre_tiles - 1) / per - c0 + 1,
+      const int b = it * pa_units(p.pre_tiles) + PA_ITEM_COST, p0 = b / per;
+      join(p.pre_ml, p.pre_o, 2 * PA_ROWS, it + p0, (b + p.pre_tiles - 1) / per - p0 + 1,
            rank * PA_ROWS + (tl - rank * p.tpc) * p.G + gh);
     }
-    const int nq = pa_qtiles(p, r), own_qt = nq > 1 ? (t - r.s0) / p.tpi : 0;
-    const int kt = pa_own_tiles(p, r, own_qt);
-    if (kt > 0) {
+    if (n > 0) {
       const int tl = t - r.s0 - own_qt * p.tpi, rank = tl >= p.tpc;
-      int b = base.y + kvh * (int)pa_own_units(p, r, nq) + PA_ITEM_COST;
-      for (int q = 0; q < own_qt; ++q) b += pa_units(pa_own_tiles(p, r, q));
-      const int c0 = b / per;
-      join(p.own_ml, p.own_o, p.own_rows, base.x + kvh * nq + own_qt + c0, (b + kt - 1) / per - c0 + 1,
+      join(p.own_ml, p.own_o, p.own_rows, base.x + kvh * nq + own_qt + c0, n,
            rank * p.own_half + (tl - rank * p.tpc) * p.G + gh);
     }
   }
@@ -942,8 +1020,7 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
       const uint16_t gs[4] = {(uint16_t)gate[j].x, (uint16_t)(gate[j].x >> 16), (uint16_t)gate[j].y,
                               (uint16_t)(gate[j].y >> 16)};
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        v[x] = __fdividef(v[x], 1.0f + exp2_approx(-1.44269504f * Elem<DT>::to_float(gs[x])));
+      for (int x = 0; x < 4; ++x) v[x] = gated<DT>(v[x], gs[x]);
     }
     *reinterpret_cast<uint2*>(out + (ch + 4 * j) * 4) =
         make_uint2(Elem<DT>::pack(v[0], v[1]), Elem<DT>::pack(v[2], v[3]));
@@ -1032,12 +1109,12 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   const int64_t items = (int64_t)p.pre_qtiles * n_kvh;
   if (items * pa_units(p.pre_tiles) >= (int64_t)PA_MANY || (int64_t)a.tokens * n_qh * head > INT32_MAX || n_kvh > 65535)
     return fail(YSKN_EINVAL, "prefix_attention: too much work");
-  p.pre_items = a.prefix_len > 0 ? (int)items : 0;
+  p.shared_items = a.prefix_len > 0 ? (int)items : 0;
   // a a.scale of zero keeps its meaning (equal weights) with a factor that leaves -inf alone
   p.c = std::max(std::fabs(a.scale) * 1.4426950408889634f, 1e-30f);
   p.negate_q = a.scale < 0.0f;
   uint8_t* work = reinterpret_cast<uint8_t*>(a.work);
-  p.work_per = reinterpret_cast<int*>(work);
+  p.work_per = reinterpret_cast<int2*>(work);
   p.work_base = reinterpret_cast<int2*>(work + w.base);
   p.pre_ml = reinterpret_cast<float2*>(work + w.pre_ml), p.pre_o = reinterpret_cast<float*>(work + w.pre_o);
   p.own_ml = reinterpret_cast<float2*>(work + w.own_ml), p.own_o = reinterpret_cast<float*>(work + w.own_o);
