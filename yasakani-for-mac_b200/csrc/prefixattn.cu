@@ -309,17 +309,27 @@ __device__ __forceinline__ uint32_t pa_idesc(int dt, int n, uint32_t b_mn, uint3
   return (1u << 4) | (t << 7) | (t << 10) | (negate_a << 13) | (b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
          ((uint32_t)(2 * PA_ROWS >> 4) << 24);
 }
-__device__ __forceinline__ void umma2_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// A and B by the low words of their descriptors (the high words are the same throughout), which
+// leaves one 32-bit addition per operand and step to the issuing thread.
+__device__ __forceinline__ void umma2_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc,
+                                         uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::
-          "r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(accumulate));
 }
-__device__ __forceinline__ void umma2_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma2_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc,
+                                         uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::
-          "r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(accumulate));
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
 }
 // Arrives on the barrier at this place in both CTAs once the MMAs issued so far are done.
 __device__ __forceinline__ void umma2_commit(uint64_t* bar) {
@@ -435,7 +445,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
   uint8_t* ring = smem + Shape::Q_BYTES;  // [RING][16 KB]
   PaShared& sh = *reinterpret_cast<PaShared*>(ring + RING * PA_SLOT);
   volatile int* abort_flag = &sh.abort_word;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // known to be the same in all lanes
   const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   if (tid == 0) {
@@ -652,12 +663,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
     }
   } else if (warp == 1) {
     // ---- MMAs: one thread of the first CTA
-    if (lane == 0 && rank == 0) {
+    if (rank == 0 && elect_one()) {
       const uint32_t id_qk = pa_idesc(DT, PA_KEYS, 0, p.negate_q), id_pv = pa_idesc(DT, D, 1, 0);
       int s = 0, g = 0, n_seg = 0;  // ring place, tiles issued, segments
       uint32_t turn = 0;
       bool ok = true;
-      const uint32_t q0 = smem_u32(sQ), r0 = smem_u32(ring);
+      // descriptors: Q, and K or V at the ring's first place; the high words hold no address
+      const uint32_t a_lo = (uint32_t)sw128_desc(smem_u32(sQ)), b_lo = (uint32_t)sw128_desc(smem_u32(ring));
+      const uint32_t k_hi = (uint32_t)(sw128_desc(0) >> 32), v_hi = (uint32_t)(mn_desc<Shape::V_LINE>(0, 0) >> 32);
+      const uint32_t v_lo = (uint32_t)mn_desc<Shape::V_LINE>(smem_u32(ring), VR * Shape::V_LINE);
       auto advance = [&]() {
         umma2_commit(&sh.empty[s]);
         if (++s == RING) s = 0, turn ^= 1;
@@ -671,10 +685,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
           tc_fence_after();
 #pragma unroll
           for (int ch = 0; ch < Shape::K_CHUNKS; ++ch) {
-            const uint64_t a = sw128_desc(q0 + (v * Shape::K_CHUNKS + ch) * PA_ROWS * 128);
-            const uint64_t b = sw128_desc(r0 + s * PA_SLOT + ch * (PA_KEYS / 2) * 128);
+            const uint32_t a = a_lo + (v * Shape::K_CHUNKS + ch) * (PA_ROWS * 128 >> 4);
+            const uint32_t b = b_lo + s * (PA_SLOT >> 4) + ch * (PA_KEYS / 2 * 128 >> 4);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) umma2_ss(d, a + 2 * k, b + 2 * k, id_qk, v > 0 || ch > 0 || k > 0);
+            for (int k = 0; k < 4; ++k) umma2_ss(d, a + 2 * k, b + 2 * k, k_hi, id_qk, v > 0 || ch > 0 || k > 0);
           }
           advance();
         }
@@ -688,11 +702,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
           ok = ok && mbar_wait(&sh.full[s], turn, abort_flag);
           if (!ok) return;
           tc_fence_after();
-          const uint64_t b = mn_desc<Shape::V_LINE>(r0 + s * PA_SLOT, VR * Shape::V_LINE);
+          const uint32_t b = v_lo + s * (PA_SLOT >> 4);
 #pragma unroll
           for (int k = 0; k < VR / 16; ++k)
             if (k * 16 < rows)
-              umma2_ts(tmem, pt + (v * VR + k * 16) / 2, b + (16 * Shape::V_LINE >> 4) * k, id_pv,
+              umma2_ts(tmem, pt + (v * VR + k * 16) / 2, b + (16 * Shape::V_LINE >> 4) * k, v_hi, id_pv,
                        !first || v > 0 || k > 0);
           advance();
         }
