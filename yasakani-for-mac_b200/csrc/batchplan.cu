@@ -18,8 +18,8 @@
 // bytes written per token. So one launch: every CTA forms the same three prefix sums (blocks
 // given back, blocks needed, tokens) over the whole batch (at most 4096 requests, from L2)
 // in shared memory, then takes its share of the tokens and of the blocks given back, and no
-// CTA waits for another. A token finds its request by a binary search in shared memory; the
-// token in a fresh block's first place writes the table entry (a fresh block always starts
+// CTA waits for another. A warp's tokens are adjacent: it finds the first one's request by a
+// search of 32 probes a round and walks on from there; the token in a fresh block's first place writes the table entry (a fresh block always starts
 // with a new token). Nothing that any CTA reads is written in the launch: the lengths and the
 // stack's count go to other arrays, fresh table entries are never read, and the stack is
 // written only above its old count, read only below it (blocks given back in this step and
@@ -46,6 +46,7 @@ struct PlanParams {
   int pool_capacity;
   const int32_t* free_count;
   int batch, block_size, prefix_len, max_tokens;
+  int warp_tokens;  // adjacent tokens of a warp, a multiple of 32
   int32_t* lens_out;
   int32_t* free_out;
   int32_t* starts;     // [batch + 1]
@@ -112,7 +113,7 @@ __device__ __forceinline__ int warp_last_at_most(const int* a, int n, int v) {
   return lo;
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) batch_plan_kernel(const __grid_constant__ PlanParams p) {
+__global__ void __launch_bounds__(PLAN_THREADS, 2) batch_plan_kernel(const __grid_constant__ PlanParams p) {
   extern __shared__ int s_plan[];
   const int B = p.batch;
   const int room = plan_at(B) + 1;
@@ -213,44 +214,55 @@ __global__ void __launch_bounds__(PLAN_THREADS) batch_plan_kernel(const __grid_c
   const int first = blockIdx.x * PLAN_THREADS + tid, step = gridDim.x * PLAN_THREADS;
   for (int v = free0 + first; v < min(left, p.pool_capacity); v += step) p.pool[v] = stack_at(v, 0, B);
   const unsigned bs = p.block_size;
-  for (int t0 = first - lane; t0 < p.max_tokens; t0 += step) {  // a warp's 32 tokens
+  // A warp's tokens are adjacent, 32 at a time: their requests lie at or after the last ones', and
+  // the givers of the blocks they take (the stack's places fall from token to token) at or before.
+  const int t_first = (blockIdx.x * PLAN_WARPS + warp) * p.warp_tokens;
+  const int t_end = min(t_first + p.warp_tokens, p.max_tokens);
+  int lo = -1, g_hi = -1;
+  for (int t0 = t_first; t0 < t_end; t0 += 32) {
     const int t = t0 + lane;
     if (t0 >= total) {
-      if (t < p.max_tokens) p.slots[t] = -1, p.positions[t] = -1, p.requests[t] = -1;
+      if (t < t_end) p.slots[t] = -1, p.positions[t] = -1, p.requests[t] = -1;
       continue;
     }
-    // the requests of the warp's first and last token bound the others'
-    const int last = min(t0 + 31, total - 1);
-    const int lo = warp_last_at_most(s_start, B, t0);
-    const int hi = warp_last_at_most(s_start, B, last);
-    const int i = last_at_most(s_start, lo, hi + 1, min(t, last));
-    const int rows = s_rows[plan_at(i)], row = rows + (min(t, last) - s_start[plan_at(i)]);
+    const int last = min(t0 + 31, total - 1), mine = min(t, last);
+    if (lo < 0) lo = warp_last_at_most(s_start, B, t0);
+    int hi = lo;  // the last token's request
+    for (unsigned more = ~0u; more == ~0u; hi += __popc(more))
+      more = __ballot_sync(0xffffffffu, hi + 1 + lane < B && s_start[plan_at(min(hi + 1 + lane, B))] <= last);
+    const int i = last_at_most(s_start, lo, hi + 1, mine);
+    lo = hi;
+    const int rows = s_rows[plan_at(i)], row = rows + (mine - s_start[plan_at(i)]);
     const int held = (int)((unsigned)rows / bs + ((unsigned)rows % bs != 0));
     const int b = (int)((unsigned)row / bs), place = row - b * (int)bs;
-    // the stack's places taken fall from token to token: the givers of the ends bound the others'
-    const int v = (int)(have - 1 - s_need[plan_at(i)]) - (b - held);
     const bool fresh = b >= held;
-    const int v_hi = __reduce_max_sync(0xffffffffu, fresh ? v : free0), v_lo = __reduce_min_sync(0xffffffffu, fresh ? v : INT32_MAX);
-    int g_lo = 0, g_hi = 1;
-    if (v_hi >= free0 && back_total > 0) {
-      g_lo = v_lo <= free0 ? 0 : warp_last_at_most(s_back, B, v_lo - free0);
-      g_hi = warp_last_at_most(s_back, B, v_hi - free0) + 1;
-    }
-    if (t > last) {
-      if (t < p.max_tokens) p.slots[t] = -1, p.positions[t] = -1, p.requests[t] = -1;
-      continue;
+    const int v = (int)(have - 1 - s_need[plan_at(i)]) - (b - held);  // place of a fresh block in the stack
+    const int v_hi = __reduce_max_sync(0xffffffffu, fresh ? v - free0 : -1);
+    int g_lo = 0;
+    if (v_hi >= 0) {  // some come from ended requests
+      const int v_lo = __reduce_min_sync(0xffffffffu, fresh ? max(v - free0, 0) : INT32_MAX);
+      if (g_hi < 0) g_hi = warp_last_at_most(s_back, B, v_hi);
+      g_lo = g_hi;
+      for (unsigned more = ~0u; more == ~0u; g_lo -= __popc(more))
+        more = __ballot_sync(0xffffffffu, g_lo - lane >= 0 && s_back[plan_at(max(g_lo - lane, 0))] > v_lo);
     }
     int32_t* entry = p.tables + (int64_t)i * p.table_stride + b;
-    int block;
-    if (fresh) {
-      block = stack_at(v, g_lo, g_hi);
-      if (place == 0) *entry = block;
-    } else {
-      block = *entry;
+    if (t <= last) {
+      int block;
+      if (fresh) {
+        block = stack_at(v, g_lo, g_hi + 1);
+        if (place == 0) *entry = block;
+      } else {
+        block = *entry;
+      }
+      p.slots[t] = (int64_t)block * p.block_size + place;
+      p.positions[t] = p.prefix_len + row;
+      p.requests[t] = i;
+    } else if (t < t_end) {
+      p.slots[t] = -1, p.positions[t] = -1, p.requests[t] = -1;
     }
-    p.slots[t] = (int64_t)block * p.block_size + place;
-    p.positions[t] = p.prefix_len + row;
-    p.requests[t] = i;
+    if (v_hi >= 0) g_hi = g_lo;
+    __syncwarp();
   }
 }
 
@@ -270,14 +282,15 @@ extern "C" YSKN_B200_API int yskn_b200_batch_plan(const yskn_b200_batch_plan_arg
   if (a.lens_out == a.lens || a.free_out == a.free)
     return fail(YSKN_EINVAL, "batch_plan: the new lengths and the new count need arrays of their own");
   PlanParams p{a.lens, a.new_lens, a.block_tables, a.table_stride, a.table_width, a.pool, a.pool_capacity, a.free,
-               a.batch, a.block_size, a.prefix_len, a.max_tokens, a.lens_out, a.free_out, a.starts, a.slots,
+               a.batch, a.block_size, a.prefix_len, a.max_tokens, 0, a.lens_out, a.free_out, a.starts, a.slots,
                a.positions, a.requests, device_error_word()};
   const size_t smem = 4 * (size_t)(plan_at(a.batch) + 1) * sizeof(int);
   static SmemOptIn opt_in;
   if (cudaError_t e = opt_in(batch_plan_kernel, 4 * (plan_at(YSKN_PLAN_MAX_BATCH) + 1) * sizeof(int)))
     return cuda_fail(e, "batch_plan_kernel attributes");
-  // Four tokens a thread, at most two CTAs an SM: more only repeat the prefix sums.
-  const int grid = (int)std::min<int64_t>(ceil_div(std::max(a.max_tokens, 1), 4 * PLAN_THREADS), 296);
+  // A warp's tokens: at most two CTAs an SM (more only repeat the prefix sums), 32 or more a warp.
+  p.warp_tokens = (int)(ceil_div(ceil_div(std::max(a.max_tokens, 1), 2 * 148 * PLAN_WARPS), 32) * 32);
+  const int grid = (int)ceil_div(std::max(a.max_tokens, 1), (int64_t)p.warp_tokens * PLAN_WARPS);
   return cuda_fail(launch_pdl(batch_plan_kernel, grid, PLAN_THREADS, smem, reinterpret_cast<cudaStream_t>(stream), p),
                    "batch_plan_kernel");
 }

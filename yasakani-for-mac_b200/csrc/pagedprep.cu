@@ -13,23 +13,23 @@
 //
 // What bounds it: bytes (each row read once and written once; 48 KB a token at 24 + 4 + 4
 // heads of 256 from f32). So one warp holds one head row in registers, lane l the channels
-// V l .. V l + V - 1 (V = D / 32): 16-byte accesses, the sum of squares by shuffles, and a
-// pair's other half R / 2 channels away is V-aligned in another lane, one shuffle per
-// channel. A warp takes up to PP_RUN heads of one token where there are many rows (one where
-// there are few), each row requested two rows ahead, and computes the token's R / 2 cosines and
-// sines once, one pair a lane, while its first rows arrive. No block-wide step. The cosine and
-// sine are the portable ones of the decode path's rotation (binary64 reduction).
+// W l .. W l + W - 1 of each 32 W (W = 4, or 2 where D = 64): every access of the warp is one
+// run of adjacent bytes, the sum of squares comes by shuffles, and a pair's other half, R / 2 (a
+// multiple of W) channels away, by one shuffle per channel (two where pairs straddle the runs).
+// A warp takes up to PP_RUN heads of one token where there are many rows (one where there are
+// few), each row requested while the one before is worked on (two rows ahead leaves room for
+// fewer warps: 86 us for 8192 tokens, not 78; runs of 4: 84); the cosines and sines of its channels are computed
+// once, one pair a lane, while its first rows arrive, and stay in registers. No block-wide step.
 #include <algorithm>
 
 #include "paged.cuh"
-#include "pmath.cuh"
 
 namespace yskn {
 
 constexpr int PP_WARPS = 8;
 constexpr int PP_MAX_PAIRS = YSKN_MAX_PAIRS;
 constexpr int PP_RUN = 8;         // heads of a warp's run, at most
-constexpr int PP_FULL = 148 * 16;  // warps that keep the SMs busy: runs get longer beyond that
+constexpr int PP_FULL = 148 * 32;  // warps that keep the SMs busy: runs get longer beyond that
 
 struct PagedPrepParams {
   const void *q, *k, *v;
@@ -51,133 +51,195 @@ struct PagedPrepParams {
   uint8_t axis[PP_MAX_PAIRS];
 };
 
-// V consecutive channels from 16-byte aligned (or V-element aligned) memory, as f32.
-template <int SRC, int V>
-__device__ __forceinline__ void load_row(const void* base, int64_t at, float (&x)[V]) {
+// Cosine and sine of a binary32 angle: reduced by its nearest multiple of pi / 2 in binary64 (two
+// parts of pi / 2), then on [-pi / 4, pi / 4] polynomials that interpolate (sin r - r) / r^3 and
+// (cos r - 1 + r^2 / 2) / r^4 at the Chebyshev nodes in r^2, in binary32: within 8e-8 (a unit of
+// 1). (With the decode path's portable function, binary64 throughout: 81 us for 8192 tokens, not 78.)
+// False for an angle past 2^30, whose multiple is not held.
+__device__ __forceinline__ bool turn_of(float angle, float2* turn) {
+  const double v = (double)angle;
+  const int n = __double2int_rn(v * 0.63661977236758134308);
+  const double r64 = fma((double)n, -6.12323399573676603587e-17, fma((double)n, -1.57079632679489661923, v));
+  const float r = (float)r64, t = r * r;
+  const float s = fmaf(r * t, fmaf(t, fmaf(t, -1.958789088e-4f, 8.332748271e-3f), -1.666666466e-1f), r);
+  const float c = fmaf(t * t, fmaf(t, fmaf(t, 2.454794208e-5f, -1.388830304e-3f), 4.166666466e-2f), fmaf(t, -0.5f, 1.0f));
+  const float x = n & 1 ? s : c, y = n & 1 ? c : s;  // cosine and sine up to their signs
+  *turn = make_float2((n + 1) & 2 ? -x : x, n & 2 ? -y : y);
+  return fabsf(angle) < 1073741824.0f;
+}
+
+// W channels from W-element aligned memory, as f32.
+template <int SRC, int W>
+__device__ __forceinline__ void load_part(const void* base, int64_t at, float* x) {
   if constexpr (SRC == YSKN_DT_F32) {
     const float* p = reinterpret_cast<const float*>(base) + at;
-    if constexpr (V == 2) {
+    if constexpr (W == 2) {
       const float2 a = __ldg(reinterpret_cast<const float2*>(p));
       x[0] = a.x, x[1] = a.y;
     } else {
-#pragma unroll
-      for (int j = 0; j < V; j += 4) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p + j));
-        x[j] = a.x, x[j + 1] = a.y, x[j + 2] = a.z, x[j + 3] = a.w;
-      }
+      const float4 a = __ldg(reinterpret_cast<const float4*>(p));
+      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
     }
   } else {
     const uint16_t* p = reinterpret_cast<const uint16_t*>(base) + at;
-    uint32_t w[V / 2];
-    if constexpr (V == 2) w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-    else if constexpr (V == 4) {
+    uint32_t w[W / 2];
+    if constexpr (W == 2) {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    } else {
       const uint2 a = __ldg(reinterpret_cast<const uint2*>(p));
       w[0] = a.x, w[1] = a.y;
-    } else {
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-      w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
     }
 #pragma unroll
-    for (int j = 0; j < V / 2; ++j) {
+    for (int j = 0; j < W / 2; ++j) {
       x[2 * j] = Elem<SRC>::to_float((uint16_t)w[j]);
       x[2 * j + 1] = Elem<SRC>::to_float((uint16_t)(w[j] >> 16));
     }
   }
 }
 
-template <int DT, int V>
-__device__ __forceinline__ void store_row(uint16_t* p, const float (&x)[V]) {
-  uint32_t w[V / 2];
-#pragma unroll
-  for (int j = 0; j < V / 2; ++j) w[j] = Elem<DT>::pack(x[2 * j], x[2 * j + 1]);
-  if constexpr (V == 2) *reinterpret_cast<uint32_t*>(p) = w[0];
-  else if constexpr (V == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-  else *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+template <int DT, int W>
+__device__ __forceinline__ void store_part(uint16_t* p, const float* x) {
+  if constexpr (W == 2) *reinterpret_cast<uint32_t*>(p) = Elem<DT>::pack(x[0], x[1]);
+  else *reinterpret_cast<uint2*>(p) = make_uint2(Elem<DT>::pack(x[0], x[1]), Elem<DT>::pack(x[2], x[3]));
 }
 
-template <int SRC, int DT, int V>
-__global__ void __launch_bounds__(PP_WARPS * 32) paged_prep_kernel(const __grid_constant__ PagedPrepParams p) {
-  constexpr int D = 32 * V;
+template <int SRC, int DT, int D>
+__global__ void __launch_bounds__(PP_WARPS * 32, 4) paged_prep_kernel(const __grid_constant__ PagedPrepParams p) {
+  constexpr int W = D == 64 ? 2 : 4, RUN = 32 * W, C = D / RUN;  // a lane's channels: W of each of C runs
   __shared__ float2 s_turn[PP_WARPS][PP_MAX_PAIRS];  // (cosine, sine) of the warp's token
   pdl_begin();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int heads = p.n_qh + 2 * p.n_kvh;  // query heads, then key heads, then value heads
-  const int runs = (heads + p.run - 1) / p.run;
-  const int64_t item = (int64_t)blockIdx.x * PP_WARPS + warp;
-  if (item >= (int64_t)p.tokens * runs) return;
-  const int t = (int)(item / runs), h0 = (int)(item - (int64_t)t * runs) * p.run, h1 = min(heads, h0 + p.run);
-  auto load = [&](int h, float (&x)[V]) {
-    if (h < p.n_qh) load_row<SRC, V>(p.q, t * p.q_row + h * p.q_head + lane * V, x);
-    else if (h < p.n_qh + p.n_kvh) load_row<SRC, V>(p.k, t * p.k_row + (h - p.n_qh) * p.k_head + lane * V, x);
-    else load_row<SRC, V>(p.v, t * p.v_row + (h - p.n_qh - p.n_kvh) * p.v_head + lane * V, x);
+  const int t = blockIdx.x * PP_WARPS + warp;
+  if (t >= p.tokens) return;
+  const int h0 = blockIdx.y * p.run, h1 = min(heads, h0 + p.run);
+  auto load = [&](int h, float (&x)[C][W]) {
+    const void* src;
+    int64_t at;
+    if (h < p.n_qh) src = p.q, at = t * p.q_row + h * p.q_head;
+    else if (h < p.n_qh + p.n_kvh) src = p.k, at = t * p.k_row + (h - p.n_qh) * p.k_head;
+    else src = p.v, at = t * p.v_row + (h - p.n_qh - p.n_kvh) * p.v_head;
+#pragma unroll
+    for (int c = 0; c < C; ++c) load_part<SRC, W>(src, at + c * RUN + lane * W, x[c]);
   };
-  float x[V], next[V];
+  float x[C][W];
   load(h0, x);
-  if (h0 + 1 < h1) load(h0 + 1, next);
   const int64_t slot = __ldg(p.slots + t);
   const int half = p.rot >> 1;
   for (int i = lane; i < half; i += 32) {
     const float pos = (float)__ldg(p.positions + p.axis[i] * p.position_stride + t);
-    float sn, cs;
-    if (!pm_sincos(__fmul_rn(pos, __ldg(p.inv_freq + i)), &cs, &sn)) raise_device_error(p.err, DERR_RANGE);
-    s_turn[warp][i] = make_float2(cs, sn);
+    if (!turn_of(__fmul_rn(pos, __ldg(p.inv_freq + i)), &s_turn[warp][i])) raise_device_error(p.err, DERR_RANGE);
   }
   __syncwarp();
-  const int lanes = half / V;  // lanes of each half of the rotated channels
-  const bool low = lane < lanes, rotated = lane < 2 * lanes;
-  const int other = rotated ? (low ? lane + lanes : lane - lanes) : lane;
-  const int i0 = rotated ? (low ? lane : lane - lanes) * V : 0;
-  const int64_t block = slot >= 0 ? slot / p.block_size : 0, place = slot - block * p.block_size;
-  const int64_t to = block * p.cache.block + place * p.cache.token + lane * V;
+  // The turns of this lane's channels, the sine negated in a pair's first half: y = x cos + other sin;
+  // (1, 0) for channels that are not rotated. `from`: the lane that holds the other half, `far`
+  // whether it holds it in its other run.
+  float cs[C][W], sn[C][W];
+  int from[C];
+  bool far[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int ch = c * RUN + lane * W;
+    const bool rotated = ch < p.rot, low = ch < half;
+    const int other = rotated ? (low ? ch + half : ch - half) : ch;
+    from[c] = other % RUN / W;
+    far[c] = other / RUN != c;
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const float2 turn = rotated ? s_turn[warp][(low ? ch : ch - half) + j] : make_float2(1.0f, 0.0f);
+      cs[c][j] = turn.x;
+      sn[c][j] = low ? -turn.y : turn.y;
+    }
+  }
+  int64_t block, place;  // a 64-bit division takes longer than the rest of the set-up
+  if ((uint64_t)slot <= UINT32_MAX) block = (uint32_t)slot / (uint32_t)p.block_size;
+  else block = slot >= 0 ? slot / p.block_size : 0;
+  place = slot - block * p.block_size;
+  const int64_t to = block * p.cache.block + place * p.cache.token + lane * W;
   if (slot >= p.n_slots && lane == 0) raise_device_error(p.err, DERR_RANGE);
+  const uint16_t* w_of = nullptr;  // what `scale` holds 1 + w of
+  float scale[C][W];
   for (int h = h0; h < h1; ++h) {
-    float after[V];
-    if (h + 2 < h1) load(h + 2, after);
+    float after[C][W];
+    if (h + 1 < h1) load(h + 1, after);
     const bool query = h < p.n_qh, value = h >= p.n_qh + p.n_kvh;
     if (!value) {
       const uint16_t* w = query ? p.q_norm : p.k_norm;
       if (w) {
-        float wt[V];
-        load_row<YSKN_DT_BF16, V>(w, lane * V, wt);
+        if (w != w_of) {
+          w_of = w;
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            load_part<YSKN_DT_BF16, W>(w, c * RUN + lane * W, scale[c]);
+#pragma unroll
+            for (int j = 0; j < W; ++j) scale[c][j] += 1.0f;
+          }
+        }
         float sum = 0.0f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) sum = fmaf(x[j], x[j], sum);
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int j = 0; j < W; ++j) sum = fmaf(x[c][j], x[c][j], sum);
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
         const float inv = rsqrtf(sum * (1.0f / D) + p.eps);
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = x[j] * inv * (1.0f + wt[j]);
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int j = 0; j < W; ++j) x[c][j] = x[c][j] * inv * scale[c][j];
       }
       if (half) {
+        if (C == 1 || p.rot <= RUN) {  // pairs within the first run
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float o = __shfl_sync(0xffffffffu, x[j], other);
-          const float2 turn = s_turn[warp][i0 + j];
-          if (rotated) x[j] = low ? fmaf(x[j], turn.x, -(o * turn.y)) : fmaf(x[j], turn.x, o * turn.y);
+          for (int j = 0; j < W; ++j) {
+            const float o = __shfl_sync(0xffffffffu, x[0][j], from[0]);
+            x[0][j] = fmaf(x[0][j], cs[0][j], o * sn[0][j]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < W; ++j) {
+            float o[C];
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+              const float near_one = __shfl_sync(0xffffffffu, x[c][j], from[c]);
+              const float far_one = __shfl_sync(0xffffffffu, x[C - 1 - c][j], from[c]);
+              o[c] = far[c] ? far_one : near_one;
+            }
+#pragma unroll
+            for (int c = 0; c < C; ++c) x[c][j] = fmaf(x[c][j], cs[c][j], o[c] * sn[c][j]);
+          }
         }
       }
     }
     if (query) {
       if (slot < 0) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = 0.0f;
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int j = 0; j < W; ++j) x[c][j] = 0.0f;
       }
-      store_row<DT, V>(p.query + ((int64_t)t * p.n_qh + h) * D + lane * V, x);
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        store_part<DT, W>(p.query + ((int64_t)t * p.n_qh + h) * D + c * RUN + lane * W, x[c]);
     } else if (slot >= 0 && slot < p.n_slots) {
-      const int kvh = value ? h - p.n_qh - p.n_kvh : h - p.n_qh;
-      store_row<DT, V>((value ? p.v_cache : p.k_cache) + to + kvh * p.cache.head, x);
+      uint16_t* row = (value ? p.v_cache + (h - p.n_qh - p.n_kvh) * p.cache.head
+                             : p.k_cache + (h - p.n_qh) * p.cache.head) + to;
+#pragma unroll
+      for (int c = 0; c < C; ++c) store_part<DT, W>(row + c * RUN, x[c]);
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) x[j] = next[j], next[j] = after[j];
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int j = 0; j < W; ++j) x[c][j] = after[c][j];
   }
 }
 
 template <int SRC, int DT>
-static cudaError_t launch_paged_prep(const PagedPrepParams& p, int head, unsigned grid, cudaStream_t st) {
+static cudaError_t launch_paged_prep(const PagedPrepParams& p, int head, dim3 grid, cudaStream_t st) {
   switch (head) {
-    case 64: return launch_pdl(paged_prep_kernel<SRC, DT, 2>, grid, PP_WARPS * 32, 0, st, p);
-    case 128: return launch_pdl(paged_prep_kernel<SRC, DT, 4>, grid, PP_WARPS * 32, 0, st, p);
-    default: return launch_pdl(paged_prep_kernel<SRC, DT, 8>, grid, PP_WARPS * 32, 0, st, p);
+    case 64: return launch_pdl(paged_prep_kernel<SRC, DT, 64>, grid, PP_WARPS * 32, 0, st, p);
+    case 128: return launch_pdl(paged_prep_kernel<SRC, DT, 128>, grid, PP_WARPS * 32, 0, st, p);
+    default: return launch_pdl(paged_prep_kernel<SRC, DT, 256>, grid, PP_WARPS * 32, 0, st, p);
   }
 }
 
@@ -225,15 +287,16 @@ extern "C" YSKN_B200_API int yskn_b200_paged_prep(const yskn_b200_paged_prep_arg
   for (int i = 0; i < a.rot / 2; ++i) p.axis[i] = a.axes[i];
   const int heads = a.n_qh + 2 * a.n_kvh;
   p.run = (int)std::min<int64_t>(PP_RUN, std::max<int64_t>(1, (int64_t)a.tokens * heads / PP_FULL));
-  const int64_t grid = ceil_div(a.tokens * ceil_div(heads, p.run), PP_WARPS);
-  if (grid > (int64_t)INT32_MAX) return fail(YSKN_EINVAL, "paged_prep: too many rows");
+  const int64_t runs = ceil_div(heads, p.run);
+  if (heads < 0 || runs > 65535) return fail(YSKN_EINVAL, "paged_prep: too many heads");
+  const dim3 grid((unsigned)ceil_div(a.tokens, PP_WARPS), (unsigned)runs);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (a.dtype == YSKN_DT_BF16)
-    e = a.source == YSKN_DT_F32 ? launch_paged_prep<YSKN_DT_F32, YSKN_DT_BF16>(p, a.head, (unsigned)grid, st)
-                                : launch_paged_prep<YSKN_DT_BF16, YSKN_DT_BF16>(p, a.head, (unsigned)grid, st);
+    e = a.source == YSKN_DT_F32 ? launch_paged_prep<YSKN_DT_F32, YSKN_DT_BF16>(p, a.head, grid, st)
+                                : launch_paged_prep<YSKN_DT_BF16, YSKN_DT_BF16>(p, a.head, grid, st);
   else
-    e = a.source == YSKN_DT_F32 ? launch_paged_prep<YSKN_DT_F32, YSKN_DT_F16>(p, a.head, (unsigned)grid, st)
-                                : launch_paged_prep<YSKN_DT_F16, YSKN_DT_F16>(p, a.head, (unsigned)grid, st);
+    e = a.source == YSKN_DT_F32 ? launch_paged_prep<YSKN_DT_F32, YSKN_DT_F16>(p, a.head, grid, st)
+                                : launch_paged_prep<YSKN_DT_F16, YSKN_DT_F16>(p, a.head, grid, st);
   return cuda_fail(e, "paged_prep_kernel");
 }
