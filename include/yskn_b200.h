@@ -649,7 +649,8 @@ YSKN_B200_API int yskn_b200_paged_prep(const yskn_b200_paged_prep_args* args, vo
  * Cache rows that no token sees may hold anything. q, gate: element (token, head, channel)
  * at token * row + head * head_stride + channel; out dense [tokens][n_qh][head]; query head
  * j reads KV head j / (n_qh / n_kvh), at most 128 query heads each. dtype YSKN_DT_F16 or
- * _BF16 for all of them (the softmax weights are rounded to it for the tensor cores); heads of
+ * _BF16 for all of them (the softmax weights are rounded to it for the tensor cores), gate_dtype
+ * the same or YSKN_DT_F32 (the gate as a projection leaves it); heads of
  * 64, 128 or 256 channels; blocks of 16, 32, 64 or 128 rows; the cache's strides as in
  * yskn_b200_paged_prep. Pointers and strides are multiples of 16 bytes. A block number outside
  * the cache or a request of more than max_new tokens gives YSKN_EINVAL from
@@ -670,7 +671,7 @@ typedef struct {
   void* work;
   int64_t work_bytes;
   void* out;
-  int n_blocks, block_size, prefix_len, table_width, batch, tokens, max_new, n_qh, n_kvh, head, dtype;
+  int n_blocks, block_size, prefix_len, table_width, batch, tokens, max_new, n_qh, n_kvh, head, dtype, gate_dtype;
   float scale;
 } yskn_b200_prefix_attention_args;
 YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_attention_args* args, void* stream);

@@ -46,7 +46,7 @@ def test_prefix_attention():
     good = dict(q=P, q_row=512, q_head=128, gate=None, gate_row=0, gate_head=0, k=P, v=P, block=4096, token=128,
                 head_stride=2048, prefix_blocks=P, tables=P, stride=2, lens=P, starts=P, work=P, work_bytes=1 << 30,
                 out=P, n_blocks=3, block_size=16, prefix=20, width=2, batch=2, tokens=3, max_new=2, n_qh=4, n_kvh=2,
-                head=128, dtype=2, scale=0.1)
+                head=128, dtype=2, gate_dtype=2, scale=0.1)
     _check("yskn_b200_prefix_attention", good,
            [{k: None} for k in ("q", "k", "v", "prefix_blocks", "tables", "lens", "starts", "work", "out")] +
            [{k: P + 8} for k in ("q", "gate", "k", "v", "work", "out")] +
@@ -54,6 +54,7 @@ def test_prefix_attention():
             dict(n_kvh=3), dict(n_qh=258), dict(prefix=-1), dict(width=0), dict(stride=1), dict(n_blocks=0),
             dict(block_size=8), dict(block_size=48), dict(block_size=256), dict(q_row=516), dict(q_head=4),
             dict(block=4), dict(token=4), dict(head_stride=4), dict(gate=P, gate_row=4),
+            dict(gate=P, gate_dtype=1), dict(gate=P, gate_dtype=0, gate_row=2),
             dict(work_bytes=Y.prefix_attention_work_bytes(3, 2, 2, 4, 2, 128) - 1)])
     L = Y.lib()
     assert L.yskn_b200_prefix_attention_work_bytes(3, 2, 2, 4, 2, 128) > 0

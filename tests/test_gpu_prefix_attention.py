@@ -18,7 +18,7 @@ P_BITS = {"bf16": 8, "f16": 11}
 
 def run(cuda, new=(1, 1), own=(5, 40), P=100, n_qh=6, n_kvh=2, D=128, dtype="bf16", block=16, gate=False,
         paired=False, head_major=True, pad_tokens=0, lens=None, seed=0, stream=None, scale=None, spread=1.0,
-        fill=float("nan"), max_new=None, check=True):
+        fill=float("nan"), max_new=None, check=True, gate_f32=False):
     """own: each request's own rows with its new ones; lens overrides P + own."""
     import torch
     import yskn_b200 as Y
@@ -55,7 +55,7 @@ def run(cuda, new=(1, 1), own=(5, 40), P=100, n_qh=6, n_kvh=2, D=128, dtype="bf1
         n = max(lens[i] - P, 0)
         rows[i] = [torch.cat([a, put(c, tables[i], n)]) for a, c in ((pk, kc), (pv, vc))]
     q = (torch.randn((T, n_qh, D * (2 if paired else 1)), generator=g, device=cuda) * 1.5).to(dt)[:, :, :D]
-    gt = (torch.randn((T, n_qh, 2 * D), generator=g, device=cuda) * 2).to(dt)[:, :, D:] if gate else None
+    gt = (torch.randn((T, n_qh, 2 * D), generator=g, device=cuda) * 2).to(torch.float32 if gate_f32 else dt)[:, :, D:] if gate else None
     starts = np.concatenate([[0], np.cumsum(new)])
     i32 = lambda a: torch.tensor(list(map(int, a)), dtype=torch.int32, device=cuda)  # noqa: E731
     max_new = max(max(new), 1) if max_new is None else max_new
@@ -128,6 +128,12 @@ def test_types_gates_and_strides(cuda, dtype, gate, paired, D):
     run(cuda, dtype=dtype, gate=gate, paired=paired, D=D, new=(1, 4), own=(50, 200), P=150, seed=3)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("new,own,P", [((1, 4), (50, 200), 150), ((1, 1), (9, 60), 0), ((130,), (130,), 300)])
+def test_gates_in_f32(cuda, dtype, new, own, P):
+    run(cuda, dtype=dtype, gate=True, gate_f32=True, D=256, new=new, own=own, P=P, seed=14)
+
+
 @pytest.mark.parametrize("new,own", [((130, 1, 47), (300, 1, 47)), ((300,), (300,)), ((33, 64, 2), (500, 64, 128)),
                                      ((8,) * 19, tuple(range(8, 160, 8)))])
 @pytest.mark.parametrize("D", [128, 256])
@@ -146,6 +152,16 @@ def test_requests_that_see_nothing_or_little(cuda):
     run(cuda, new=(1, 0, 1, 3, 2, 0, 2), lens=[0, 0, 30, 2, 101, 120, 1], P=100, seed=4)
     run(cuda, new=(2, 3), lens=[0, 0], P=0, seed=5)
     run(cuda, new=(0, 4, 0, 0, 1, 0), lens=[0, 104, 0, 500, 260, 0], P=100, pad_tokens=5, seed=6)
+
+
+@pytest.mark.parametrize("n_qh,n_kvh,D", [(24, 4, 256), (6, 2, 128), (3, 3, 64)])
+def test_few_items_of_few_tiles(cuda, n_qh, n_kvh, D):
+    """Items that one pair of SMs finishes from end to end, empty and idle requests among them."""
+    kw = dict(n_qh=n_qh, n_kvh=n_kvh, D=D, block=16, gate=True)
+    run(cuda, new=(1, 0, 2, 1), lens=[30, 0, 2, 0], P=0, pad_tokens=3, seed=15, **kw)
+    run(cuda, new=(1, 1), own=(1, 90), P=100, pad_tokens=1, seed=16, **kw)
+    run(cuda, new=(1, 3, 1), lens=[0, 50, 101], P=100, seed=17, **kw)
+    run(cuda, new=(90, 1), own=(90, 120), P=0, seed=18, **kw)
 
 
 def test_padded_tokens_give_zeros(cuda):

@@ -72,6 +72,7 @@ constexpr int PA_SLOT = 16384;  // bytes per ring slot
 constexpr int PA_THREADS = 384;
 constexpr int PA_MAX_PAIRS = 74;
 constexpr int PA_MAX_SLOTS = 12;
+constexpr int PA_WHOLE_TILES = 2;  // tiles up to which few items are not cut
 constexpr int PA_ITEM_COST = 3;  // an item's fixed cost (Q, the last P V's wait, its result) in tiles
 
 template <int D>
@@ -115,8 +116,9 @@ inline PaWork pa_work(int tokens, int batch, int max_new, int n_qh, int n_kvh, i
 }
 
 struct PrefixAttnParams {
-  const uint16_t* gate;
+  const void* gate;  // of the queries' type, or f32
   int64_t gate_row, gate_head;
+  bool gate_f32;
   const int32_t* prefix_blocks;
   const int32_t* tables;
   int64_t table_stride;
@@ -126,7 +128,8 @@ struct PrefixAttnParams {
   int batch, tokens, max_new, n_kvh, G;
   int tpc, tpi;  // tokens per CTA and per item
   int pre_tiles, pre_qtiles, shared_items;  // prefix items, if there are any
-  float c;  // |scale| log2 e
+  bool whole;  // items are not cut: no join
+  float c;     // |scale| log2 e
   uint32_t negate_q;
   int2* work_per;         // units per pair of this call, and whether alone: for the join
   int2* work_base;        // [batch] own items, and units of all items, before each request's own
@@ -134,6 +137,7 @@ struct PrefixAttnParams {
   float2 *pre_ml, *own_ml;
   float *pre_o, *own_o;
   int own_half, own_rows;
+  unsigned many_per_head;  // PA_MANY / n_kvh
   long long own_items;  // more of them (starts that do not ascend), or 2^30 own units, is an error: nothing is computed
   uint16_t* out;  // [tokens][n_qh][D]
   unsigned* err;
@@ -174,8 +178,11 @@ __device__ __forceinline__ int pa_visible(const PrefixAttnParams& p, const PaReq
 __device__ __forceinline__ int pa_own_tiles(const PrefixAttnParams& p, const PaRequest& r, int qt) {
   return (pa_visible(p, r, min(r.n, (qt + 1) * p.tpi)) + PA_KEYS - 1) / PA_KEYS;
 }
-// Units of an item of so many tiles (0: nothing to do); unit u is tile u - PA_ITEM_COST.
-__host__ __device__ __forceinline__ int pa_units(int tiles) { return tiles > 0 ? tiles + PA_ITEM_COST : 0; }
+// Units of an item of so many tiles (0: nothing to do): unit u is tile u - PA_ITEM_COST; or the
+// whole item is one unit.
+__host__ __device__ __forceinline__ int pa_units(int tiles, bool whole) {
+  return tiles <= 0 ? 0 : whole ? 1 : tiles + PA_ITEM_COST;
+}
 __device__ __forceinline__ int pa_qtiles(const PrefixAttnParams& p, const PaRequest& r) {
   return r.n <= p.tpi ? r.n > 0 : (r.n + p.tpi - 1) / p.tpi;
 }
@@ -188,7 +195,7 @@ constexpr unsigned PA_MANY = 1u << 30;
 __device__ __forceinline__ unsigned pa_sum(unsigned a, unsigned b) { return min(a + b, PA_MANY); }
 __device__ __forceinline__ unsigned pa_own_units(const PrefixAttnParams& p, const PaRequest& r, int nq, bool alone) {
   unsigned u = 0;
-  for (int q = 0; q < nq; ++q) u = pa_sum(u, pa_units(pa_tiles(p, r, q, alone)));
+  for (int q = 0; q < nq; ++q) u = pa_sum(u, pa_units(pa_tiles(p, r, q, alone), p.whole));
   return u;
 }
 
@@ -233,7 +240,7 @@ struct PaWalk {
       kvh = s.skip / head;
       int skip = s.skip - kvh * head;
       for (;; ++qt) {
-        const int u = pa_units(pa_tiles(p, r, qt, alone));
+        const int u = pa_units(pa_tiles(p, r, qt, alone), p.whole);
         if (skip < u) break;
         skip -= u;
       }
@@ -249,7 +256,7 @@ struct PaWalk {
   __device__ bool next(PaSegment& s) {
     while (left > 0 && !alone && pre_item < p.shared_items) {
       s.prefix = true;
-      s.kvh = pre_item / p.pre_qtiles;
+      s.kvh = p.pre_qtiles == 1 ? pre_item : pre_item / p.pre_qtiles;
       s.tok0 = (pre_item - s.kvh * p.pre_qtiles) * p.tpi;
       s.ntok = min(p.tpi, p.tokens - s.tok0);
       s.req = 0;
@@ -285,9 +292,9 @@ struct PaWalk {
   }
   // This pair's part of an item; false if it holds no tile.
   __device__ bool take(PaSegment& s, int tiles, int it) {
-    const int n = min(tiles + PA_ITEM_COST - u0, left);
-    s.key0 = max(u0 - PA_ITEM_COST, 0);
-    s.key1 = max(u0 + n - PA_ITEM_COST, 0);
+    const int n = p.whole ? 1 : min(tiles + PA_ITEM_COST - u0, left);
+    s.key0 = p.whole ? 0 : max(u0 - PA_ITEM_COST, 0);
+    s.key1 = p.whole ? tiles : max(u0 + n - PA_ITEM_COST, 0);
     s.whole = !s.prefix && s.key0 == 0 && s.key1 == tiles && s.pre == p.pre_tiles;
     s.place = (int64_t)it + (blockIdx.x >> 1);
     left -= n;
@@ -406,9 +413,22 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return y;
 }
+__device__ __forceinline__ float gated(float x, float gate) {
+  return __fdividef(x, 1.0f + exp2_approx(-1.44269504f * gate));
+}
+// Four of the output gate's channels from element `at` on, as they are stored, and as f32: apart, so
+// that several loads are under way before the first is waited for.
+__device__ __forceinline__ uint4 gate_load(const PrefixAttnParams& p, int64_t at) {
+  if (p.gate_f32) return __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p.gate) + at));
+  const uint2 g = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p.gate) + at));
+  return make_uint4(g.x, g.y, 0, 0);
+}
 template <int DT>
-__device__ __forceinline__ float gated(float x, uint16_t gate) {
-  return __fdividef(x, 1.0f + exp2_approx(-1.44269504f * Elem<DT>::to_float(gate)));
+__device__ __forceinline__ float4 gate_value(const PrefixAttnParams& p, uint4 g) {
+  if (p.gate_f32)
+    return make_float4(__uint_as_float(g.x), __uint_as_float(g.y), __uint_as_float(g.z), __uint_as_float(g.w));
+  return make_float4(Elem<DT>::to_float((uint16_t)g.x), Elem<DT>::to_float((uint16_t)(g.x >> 16)),
+                     Elem<DT>::to_float((uint16_t)g.y), Elem<DT>::to_float((uint16_t)(g.y >> 16)));
 }
 // Both warps of a row quarter.
 __device__ __forceinline__ void quarter_sync(int quarter) {
@@ -476,13 +496,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
 
   // Unit counts of all requests and where this pair begins. A thread's requests are adjacent.
   {
-    const int per = (p.batch + PA_THREADS - 1) / PA_THREADS;
+    const int per = p.batch <= PA_THREADS ? 1 : (p.batch + PA_THREADS - 1) / PA_THREADS;
     const int i0 = min(p.batch, tid * per), i1 = min(p.batch, i0 + per);
     unsigned items = 0, units_of[2] = {0, 0};  // beside prefix items, and alone
     for (int i = i0; i < i1; ++i) {
       const PaRequest r = pa_request(p, i);
       const int nq = pa_qtiles(p, r);
-      auto times = [&](unsigned n) { return (unsigned)min((unsigned long long)n * p.n_kvh, (unsigned long long)PA_MANY); };
+      auto times = [&](unsigned n) { return n > p.many_per_head ? PA_MANY : n * p.n_kvh; };
       units_of[0] = pa_sum(units_of[0], times(pa_own_units(p, r, nq, false)));
       units_of[1] = pa_sum(units_of[1], times(pa_own_units(p, r, nq, true)));
       items = pa_sum(items, times(nq));
@@ -498,8 +518,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
     if (lane == 31) sh.sum[warp] = make_uint3(ui[0], ui[1], it);
     __syncthreads();
     unsigned before_of[2] = {0, 0}, total_of[2] = {0, 0}, items_before = 0, total_items = 0;
-#pragma unroll
-    for (int w = 0; w < PA_THREADS / 32; ++w) {
+    const int used = per == 1 ? p.batch : PA_THREADS;  // threads with requests
+    for (int w = 0; w * 32 < used; ++w) {
       const uint3 o = sh.sum[w];
       if (w < warp) {
         before_of[0] = pa_sum(before_of[0], o.x);
@@ -512,15 +532,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
     }
     // Alone, if that is at most an eighth more: about what the join of two results per row costs
     // (16 prompt chunks: 960 us with prefix items, ALONE us alone).
-    const int pre_units = pa_units(p.pre_tiles), pre_all = p.shared_items * pre_units;  // below 2^30: the host looked
-    const bool alone = p.shared_items > 0 && total_of[1] < PA_MANY &&
-                       8ull * total_of[1] <= 9ull * ((unsigned)pre_all + total_of[0]);
+    const int pre_units = pa_units(p.pre_tiles, false), pre_all = p.shared_items * pre_units;  // below 2^30: the host looked
+    const bool alone = p.whole || (p.shared_items > 0 && total_of[1] < PA_MANY &&
+                                   8ull * total_of[1] <= 9ull * ((unsigned)pre_all + total_of[0]));
     const unsigned units = alone ? units_of[1] : units_of[0], total = alone ? total_of[1] : total_of[0];
     const unsigned before = pa_sum(alone ? before_of[1] : before_of[0], alone ? ui[1] - units_of[1] : ui[0] - units_of[0]);
     items_before = pa_sum(items_before, it - items);
     const bool sound = total_items <= (unsigned)p.own_items && total < PA_MANY;
     const int pre_items = alone ? 0 : p.shared_items, pre = alone ? 0 : pre_all;
-    const int all = sound ? pre + (int)total : 0, share = (all + pairs - 1) / pairs;
+    const int all = sound ? pre + (int)total : 0, share = pairs == PA_MAX_PAIRS ? (all + PA_MAX_PAIRS - 1) / PA_MAX_PAIRS : (all + pairs - 1) / pairs;
     const int t0 = min(all, pair * share), t1 = min(all, t0 + share);
     const int at = t0 - pre;  // this pair's first own unit
     if (tid == 0) {
@@ -756,6 +776,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
       }
     }
   } else if (warp == 3) {
+    // ---- where there is no join: zeros for the tokens that no item holds
+    if (p.whole)
+      for (int t = blockIdx.x; t < p.tokens; t += gridDim.x) {
+        const int i = request_of(p.starts, p.batch, t);
+        const PaRequest r = i < p.batch ? pa_request(p, i) : PaRequest{};
+        if (t >= r.s0 && t < r.s0 + r.n && pa_tiles(p, r, (t - r.s0) / p.tpi, true) > 0) continue;
+        uint4* row = reinterpret_cast<uint4*>(p.out + (int64_t)t * p.n_kvh * p.G * D);
+        for (int x = lane; x < p.n_kvh * p.G * D / 8; x += 32) row[x] = make_uint4(0, 0, 0, 0);
+      }
     // ---- V rows past the last visible one, up to the end of the 16-row step, to zero, in the
     // slots that warp 0 names: once for each segment that ends inside a step
     const uint32_t full0 = first_cta(&sh.full[0]);
@@ -889,10 +918,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
           const int64_t t = seg.tok0 + tl;
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;
           uint16_t* out = p.out + (t * p.n_kvh * p.G + h) * D;
-          const uint16_t* gate = p.gate + t * p.gate_row + h * p.gate_head;
+          const int64_t gate = t * p.gate_row + h * p.gate_head;
           for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
             uint32_t v[32];
+            uint4 g[8];
             tmem_ld32(tmem + lanes + x, v);
+            if (valid && p.gate) {
+#pragma unroll
+              for (int y = 0; y < 8; ++y) g[y] = gate_load(p, gate + x + 4 * y);
+            }
             tmem_ld_wait32(v);
             if (valid) {
 #pragma unroll
@@ -901,10 +935,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
 #pragma unroll
                 for (int k = 0; k < 8; ++k) z[k] = __uint_as_float(v[y + k]) * inv;
                 if (p.gate) {
-                  const uint4 g4 = __ldg(reinterpret_cast<const uint4*>(gate + x + y));
-                  const uint32_t gs[4] = {g4.x, g4.y, g4.z, g4.w};
+                  const float4 a = gate_value<DT>(p, g[y / 4]), d = gate_value<DT>(p, g[y / 4 + 1]);
+                  const float gs[8] = {a.x, a.y, a.z, a.w, d.x, d.y, d.z, d.w};
 #pragma unroll
-                  for (int k = 0; k < 8; ++k) z[k] = gated<DT>(z[k], (uint16_t)(gs[k >> 1] >> (k & 1) * 16));
+                  for (int k = 0; k < 8; ++k) z[k] = gated(z[k], gs[k]);
                 }
                 *reinterpret_cast<uint4*>(out + x + y) =
                     make_uint4(Elem<DT>::pack(z[0], z[1]), Elem<DT>::pack(z[2], z[3]), Elem<DT>::pack(z[4], z[5]),
@@ -966,11 +1000,10 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
   const bool alone = how.y;
   const int ch = (unit % PARTS) * 16 + (lane >> 3);  // of 4 channels; then every 4th
   const int h = kvh * p.G + gh;
-  uint2 gate[4];
+  uint4 gate[4];
   if (p.gate) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      gate[j] = __ldg(reinterpret_cast<const uint2*>(p.gate + t * p.gate_row + h * p.gate_head + (ch + 4 * j) * 4));
+    for (int j = 0; j < 4; ++j) gate[j] = gate_load(p, t * p.gate_row + h * p.gate_head + (ch + 4 * j) * 4);
   }
   float4 o[4];
   float den = 0.0f, top = -INFINITY;
@@ -1008,14 +1041,14 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
     int c0 = 0, n = 0;
     if (kt > 0) {
       int b = base.y + kvh * (int)pa_own_units(p, r, nq, alone) + PA_ITEM_COST;
-      for (int q = 0; q < own_qt; ++q) b += pa_units(pa_tiles(p, r, q, alone));
+      for (int q = 0; q < own_qt; ++q) b += pa_units(pa_tiles(p, r, q, alone), p.whole);
       c0 = b / per;
       n = (b + kt - 1) / per - c0 + 1;
     }
     if (n == 1 && (alone || p.pre_tiles == 0)) return;  // finished where it was computed
     if (!alone && p.pre_tiles > 0) {
       const int qt = t / p.tpi, it = kvh * p.pre_qtiles + qt, tl = t - qt * p.tpi, rank = tl >= p.tpc;
-      const int b = it * pa_units(p.pre_tiles) + PA_ITEM_COST, p0 = b / per;
+      const int b = it * pa_units(p.pre_tiles, false) + PA_ITEM_COST, p0 = b / per;
       join(p.pre_ml, p.pre_o, 2 * PA_ROWS, it + p0, (b + p.pre_tiles - 1) / per - p0 + 1,
            rank * PA_ROWS + (tl - rank * p.tpc) * p.G + gh);
     }
@@ -1031,10 +1064,8 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
   for (int j = 0; j < 4; ++j) {
     float v[4] = {o[j].x * inv, o[j].y * inv, o[j].z * inv, o[j].w * inv};
     if (p.gate) {
-      const uint16_t gs[4] = {(uint16_t)gate[j].x, (uint16_t)(gate[j].x >> 16), (uint16_t)gate[j].y,
-                              (uint16_t)(gate[j].y >> 16)};
-#pragma unroll
-      for (int x = 0; x < 4; ++x) v[x] = gated<DT>(v[x], gs[x]);
+      const float4 g = gate_value<DT>(p, gate[j]);
+      v[0] = gated(v[0], g.x), v[1] = gated(v[1], g.y), v[2] = gated(v[2], g.z), v[3] = gated(v[3], g.w);
     }
     *reinterpret_cast<uint2*>(out + (ch + 4 * j) * 4) =
         make_uint2(Elem<DT>::pack(v[0], v[1]), Elem<DT>::pack(v[2], v[3]));
@@ -1049,6 +1080,7 @@ static int launch_prefix_attention(const CUtensorMap (&maps)[4], const PrefixAtt
   if (cudaError_t e = launch_pdl(prefix_attention_kernel<D, DT>, grid, PA_THREADS, PaShape<D>::SMEM, st, maps[0],
                                  maps[1], maps[2], maps[3], p))
     return cuda_fail(e, "prefix_attention_kernel");
+  if (p.whole) return YSKN_OK;
   const int64_t warps = ceil_div((int64_t)p.tokens * p.G, 8) * (D / 64);
   return cuda_fail(launch_pdl(prefix_combine_kernel<D, DT>, dim3((unsigned)ceil_div(warps, 8), p.n_kvh), 256, 0, st, p),
                    "prefix_combine_kernel");
@@ -1092,7 +1124,8 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   const int head = a.head, n_qh = a.n_qh, n_kvh = a.n_kvh, block_size = a.block_size, dtype = a.dtype;
   if (head != 64 && head != 128 && head != 256)
     return fail(YSKN_EINVAL, "prefix_attention: heads of 64, 128 or 256 channels");
-  if (!is_16bit(dtype)) return fail(YSKN_EINVAL, "prefix_attention: queries and cache are f16 or bf16");
+  if (!is_16bit(dtype) || (a.gate && a.gate_dtype != dtype && a.gate_dtype != YSKN_DT_F32))
+    return fail(YSKN_EINVAL, "prefix_attention: queries and cache are f16 or bf16, the gate of their type or f32");
   if (a.tokens < 1 || a.batch < 1 || a.max_new < 1 || n_kvh < 1 || n_qh < 1 || n_qh % n_kvh || n_qh / n_kvh > PA_ROWS ||
       a.prefix_len < 0 || a.table_width < 1 || (a.batch > 1 && a.table_stride < a.table_width) || a.n_blocks < 1)
     return fail(YSKN_EINVAL, "prefix_attention: empty shape, heads not a multiple, or a stride below its width");
@@ -1104,13 +1137,13 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   if (a.n_blocks == 1) a.block_stride = 0;
   if (!aligned16(a.q) || !aligned16(a.gate) || !aligned16(a.k_cache) || !aligned16(a.v_cache) || !aligned16(a.work) ||
       !aligned16(a.out) || (a.q_row | a.q_head | a.block_stride | a.token_stride | a.head_stride) % 8 ||
-      (a.gate && (a.gate_row | a.gate_head) % 8))
+      (a.gate && (a.gate_row | a.gate_head) % (a.gate_dtype == YSKN_DT_F32 ? 4 : 8)))
     return fail(YSKN_EINVAL, "prefix_attention: pointers and strides are multiples of 16 bytes");
   const PaWork w = pa_work(a.tokens, a.batch, a.max_new, n_qh, n_kvh, head);
   if (a.work_bytes < w.bytes) return fail(YSKN_EINVAL, "prefix_attention: workspace too small");
   const int G = n_qh / n_kvh, tpc = PA_ROWS / G;
   PrefixAttnParams p{};
-  p.gate = reinterpret_cast<const uint16_t*>(a.gate);
+  p.gate = a.gate, p.gate_f32 = a.gate_dtype == YSKN_DT_F32;
   p.gate_row = a.gate_row, p.gate_head = a.gate_head;
   p.prefix_blocks = a.prefix_blocks;
   p.tables = a.block_tables, p.table_stride = a.table_stride;
@@ -1121,10 +1154,16 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   p.tpc = tpc, p.tpi = 2 * tpc;
   p.pre_tiles = (int)ceil_div(a.prefix_len, PA_KEYS), p.pre_qtiles = (int)ceil_div(a.tokens, 2 * tpc);
   const int64_t items = (int64_t)p.pre_qtiles * n_kvh;
-  if (items * pa_units(p.pre_tiles) >= (int64_t)PA_MANY || (int64_t)a.tokens * n_qh * head > INT32_MAX || n_kvh > 65535)
+  if (items * pa_units(p.pre_tiles, false) >= (int64_t)PA_MANY || (int64_t)a.tokens * n_qh * head > INT32_MAX || n_kvh > 65535)
     return fail(YSKN_EINVAL, "prefix_attention: too much work");
   p.shared_items = a.prefix_len > 0 ? (int)items : 0;
-  // a a.scale of zero keeps its meaning (equal weights) with a factor that leaves -inf alone
+  // Few items of few tiles: each by one pair of SMs from end to end, which is quicker than the second
+  // launch that joins its parts (two requests of up to 64 rows: 16.4 us cut, 13.9 whole without a
+  // prefix, 15.2 and 15.4 behind 100 rows, 15.4 and 16.1 behind 256).
+  const int64_t most_tiles = p.pre_tiles + ceil_div(p.own_limit, PA_KEYS);
+  p.whole = w.own_items <= PA_MAX_PAIRS && most_tiles <= PA_WHOLE_TILES;
+  p.many_per_head = PA_MANY / (unsigned)n_kvh;
+  // a scale of zero keeps its meaning (equal weights) with a factor that leaves -inf alone
   p.c = std::max(std::fabs(a.scale) * 1.4426950408889634f, 1e-30f);
   p.negate_q = a.scale < 0.0f;
   uint8_t* work = reinterpret_cast<uint8_t*>(a.work);

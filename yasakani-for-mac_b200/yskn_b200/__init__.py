@@ -674,17 +674,19 @@ DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 ARGS = {
     "batch_plan": struct.Struct("@3PqPP3P3P6i"),
     "paged_prep": struct.Struct("@3P6q2PqP2P3P3q10if128s"),
-    "prefix_attention": struct.Struct("@P2qP2q2P3q2Pq2PPqP11if"),
+    "prefix_attention": struct.Struct("@P2qP2q2P3q2Pq2PPqP12if"),
     "logits_adjust": struct.Struct("@PqPq2P3P2PPqPq4i"),
 }
-_DT = {}
+_DT, _FN = {}, {}
 
 
 def _types():
     import torch
     _DT.update({torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.int16: DT_BF16})
     _DT["i32"] = torch.int32
-    _DT["stream"] = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+    # the raw handle at once: building a torch.cuda.Stream object around it takes longer than a launch
+    _DT["stream"] = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _dtype(t):
@@ -702,14 +704,10 @@ def _need(ok, what):
 
 def _launch(name, packed, tensor, stream):
     """The call on `stream`, or on the current stream of the tensor's device."""
-    if stream is not None:
-        raw = stream.cuda_stream
-    elif _DT["stream"] is not None:
-        raw = _DT["stream"](tensor.get_device())
-    else:
-        import torch
-        raw = torch.cuda.current_stream().cuda_stream
-    rc = getattr(_lib or lib(), "yskn_b200_" + name)(packed, raw)
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(lib(), "yskn_b200_" + name)
+    rc = fn(packed, stream.cuda_stream if stream is not None else _DT["stream"](tensor.get_device()))
     if rc:
         check(rc, name)
 
@@ -784,8 +782,8 @@ def prefix_attention_work_bytes(tokens, batch, max_new, n_qh, n_kvh, head):
 
 def prefix_attention(q, k_cache, v_cache, block_tables, lens, starts, max_new, work, out, prefix_blocks=None,
                      prefix_len=0, gate=None, scale=None, stream=None):
-    """yskn_b200_prefix_attention: q (and gate) [T][n_qh][D] with dense channels, the caches as
-    paged_prep, each request's own blocks in block_tables (int32 [batch][width]) and the shared
+    """yskn_b200_prefix_attention: q and gate (of q's type, or f32) [T][n_qh][D] with dense
+    channels, the caches as paged_prep, each request's own blocks in block_tables (int32 [batch][width]) and the shared
     prefix's in prefix_blocks; lens and starts as batch_plan writes them (at most max_new tokens
     a request) -> out (dense [T][n_qh][D]). scale defaults to 1 / sqrt(D). work: uint8, of
     prefix_attention_work_bytes(T, batch, max_new, n_qh, n_kvh, D) bytes."""
@@ -805,17 +803,17 @@ def prefix_attention(q, k_cache, v_cache, block_tables, lens, starts, max_new, w
           (not prefix_len or (prefix_blocks is not None and prefix_blocks.dtype is i32 and
                               prefix_blocks.numel() * block_size >= prefix_len)),
           "prefix_attention: int32 tables, lengths and starts of one batch, and the prefix's blocks expected")
-    gs = (0, 0)
+    gs, gd = (0, 0), 0
     if gate is not None:
-        gs = gate.stride()
-        _need(gate.shape == shape and gs[2] == 1 and gate.dtype is dt,
-              "prefix_attention: a gate of the queries' shape and type with dense channels expected")
+        gs, gd = gate.stride(), _dtype(gate)
+        _need(gate.shape == shape and gs[2] == 1,
+              "prefix_attention: a gate of the queries' shape with dense channels expected")
     _launch("prefix_attention", ARGS["prefix_attention"].pack(
         q.data_ptr(), qs[0], qs[1], 0 if gate is None else gate.data_ptr(), gs[0], gs[1], k_cache.data_ptr(),
         v_cache.data_ptr(), cs[0], cs[1], cs[2], prefix_blocks.data_ptr() if prefix_len else 0,
         block_tables.data_ptr(), row[0], lens.data_ptr(), starts.data_ptr(), work.data_ptr(),
         work.numel() * work.element_size(), out.data_ptr(), n_blocks, block_size, prefix_len, width, B, T, max_new,
-        n_qh, n_kvh, D, _dtype(q), D ** -0.5 if scale is None else scale), out, stream)
+        n_qh, n_kvh, D, _dtype(q), gd, D ** -0.5 if scale is None else scale), out, stream)
 
 
 def logits_adjust(logits, out, history=None, history_lens=None, prompt_lens=None, repetition=None, presence=None,
