@@ -127,6 +127,7 @@ struct PrefixAttnParams {
   int own_limit;  // rows that a table row can name
   int batch, tokens, max_new, n_kvh, G;
   int tpc, tpi;  // tokens per CTA and per item
+  unsigned g_magic, tpi_magic;  // ceil(2^32 / d): quotients of numbers below 2^32 / d
   int pre_tiles, pre_qtiles, shared_items;  // prefix items, if there are any
   bool whole;  // items are not cut: no join
   float c;     // |scale| log2 e
@@ -142,6 +143,9 @@ struct PrefixAttnParams {
   uint16_t* out;  // [tokens][n_qh][D]
   unsigned* err;
 };
+
+// n / d by its magic number (0 for d = 1).
+__device__ __forceinline__ int pa_quotient(int n, unsigned magic) { return magic ? (int)__umulhi((unsigned)n, magic) : n; }
 
 // The last request whose first token is at or before t (requests without tokens share a
 // start with the next one), or the batch if t is past the last token. One token for each
@@ -184,7 +188,7 @@ __host__ __device__ __forceinline__ int pa_units(int tiles, bool whole) {
   return tiles <= 0 ? 0 : whole ? 1 : tiles + PA_ITEM_COST;
 }
 __device__ __forceinline__ int pa_qtiles(const PrefixAttnParams& p, const PaRequest& r) {
-  return r.n <= p.tpi ? r.n > 0 : (r.n + p.tpi - 1) / p.tpi;
+  return r.n <= p.tpi ? r.n > 0 : pa_quotient(r.n + p.tpi - 1, p.tpi_magic);
 }
 // Tiles of a request's item `qt`: own ones, after the prefix's where there are no prefix items.
 __device__ __forceinline__ int pa_tiles(const PrefixAttnParams& p, const PaRequest& r, int qt, bool alone) {
@@ -781,7 +785,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
       for (int t = blockIdx.x; t < p.tokens; t += gridDim.x) {
         const int i = request_of(p.starts, p.batch, t);
         const PaRequest r = i < p.batch ? pa_request(p, i) : PaRequest{};
-        if (t >= r.s0 && t < r.s0 + r.n && pa_tiles(p, r, (t - r.s0) / p.tpi, true) > 0) continue;
+        if (t >= r.s0 && t < r.s0 + r.n && pa_tiles(p, r, pa_quotient(t - r.s0, p.tpi_magic), true) > 0) continue;
         uint4* row = reinterpret_cast<uint4*>(p.out + (int64_t)t * p.n_kvh * p.G * D);
         for (int x = lane; x < p.n_kvh * p.G * D / 8; x += 32) row[x] = make_uint4(0, 0, 0, 0);
       }
@@ -814,8 +818,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
     const float c = p.c;
     int g = 0;
     while (walk.next(seg)) {
-      const int tl = rank * p.tpc + row / p.G;  // token of the item
-      const bool valid = row / p.G < p.tpc && tl < seg.ntok;
+      const int row_tok = pa_quotient(row, p.g_magic), tl = rank * p.tpc + row_tok;  // token of the item
+      const bool valid = row_tok < p.tpc && tl < seg.ntok;
       int lim = 0;  // rows of the sequence that the row sees
       if (valid) {
         if (seg.prefix) {
@@ -874,6 +878,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
             __syncwarp();
             tc_fence_after();
             const float f = grown ? exp2_approx(m - top) : 1.0f;
+            // (Rolled: unrolled it is rare code that costs 800 bytes of spilled registers at D = 256.)
+#pragma unroll 1
             for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
               uint32_t o[32];
               tmem_ld32(tmem + lanes + x, o);
@@ -914,35 +920,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
         quarter_sync(quarter);
         l += sh.half[0][half ^ 1][row];
         if (seg.whole) {
-          const int h = seg.kvh * p.G + row % p.G;
+          const int h = seg.kvh * p.G + row - row_tok * p.G;
           const int64_t t = seg.tok0 + tl;
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;
           uint16_t* out = p.out + (t * p.n_kvh * p.G + h) * D;
           const int64_t gate = t * p.gate_row + h * p.gate_head;
           for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
             uint32_t v[32];
-            uint4 g[8];
             tmem_ld32(tmem + lanes + x, v);
-            if (valid && p.gate) {
-#pragma unroll
-              for (int y = 0; y < 8; ++y) g[y] = gate_load(p, gate + x + 4 * y);
-            }
             tmem_ld_wait32(v);
             if (valid) {
 #pragma unroll
-              for (int y = 0; y < 32; y += 8) {
-                float z[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) z[k] = __uint_as_float(v[y + k]) * inv;
+              for (int y0 = 0; y0 < 32; y0 += 16) {
+                uint4 g[4];
                 if (p.gate) {
-                  const float4 a = gate_value<DT>(p, g[y / 4]), d = gate_value<DT>(p, g[y / 4 + 1]);
-                  const float gs[8] = {a.x, a.y, a.z, a.w, d.x, d.y, d.z, d.w};
 #pragma unroll
-                  for (int k = 0; k < 8; ++k) z[k] = gated(z[k], gs[k]);
+                  for (int y = 0; y < 4; ++y) g[y] = gate_load(p, gate + x + y0 + 4 * y);
                 }
-                *reinterpret_cast<uint4*>(out + x + y) =
-                    make_uint4(Elem<DT>::pack(z[0], z[1]), Elem<DT>::pack(z[2], z[3]), Elem<DT>::pack(z[4], z[5]),
-                               Elem<DT>::pack(z[6], z[7]));
+#pragma unroll
+                for (int y = 0; y < 16; y += 8) {
+                  float z[8];
+#pragma unroll
+                  for (int k = 0; k < 8; ++k) z[k] = __uint_as_float(v[y0 + y + k]) * inv;
+                  if (p.gate) {
+                    const float4 a = gate_value<DT>(p, g[y / 4]), d = gate_value<DT>(p, g[y / 4 + 1]);
+                    const float gs[8] = {a.x, a.y, a.z, a.w, d.x, d.y, d.z, d.w};
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) z[k] = gated(z[k], gs[k]);
+                  }
+                  *reinterpret_cast<uint4*>(out + x + y0 + y) =
+                      make_uint4(Elem<DT>::pack(z[0], z[1]), Elem<DT>::pack(z[2], z[3]), Elem<DT>::pack(z[4], z[5]),
+                                 Elem<DT>::pack(z[6], z[7]));
+                }
               }
             }
           }
@@ -993,11 +1002,14 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
   pdl_begin();
   const int lane = threadIdx.x & 31;
   const int unit = blockIdx.x * 8 + (threadIdx.x >> 5), idx = unit / PARTS * 8 + (lane & 7);
-  const int kvh = blockIdx.y, t = idx / p.G, gh = idx - t * p.G;
+  const int kvh = blockIdx.y, t = pa_quotient(idx, p.g_magic), gh = idx - t * p.G;
   if (t >= p.tokens) return;
   const int2 how = *p.work_per;
-  const int per = how.x;
-  const bool alone = how.y;
+  // one token for each request is the common case: its request's numbers are asked for at once
+  int i = t;
+  PaRequest r{-1, 0, 0};
+  int2 base{};
+  if (t < p.batch) r = pa_request(p, t), base = p.work_base[t];
   const int ch = (unit % PARTS) * 16 + (lane >> 3);  // of 4 channels; then every 4th
   const int h = kvh * p.G + gh;
   uint4 gate[4];
@@ -1005,57 +1017,79 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
 #pragma unroll
     for (int j = 0; j < 4; ++j) gate[j] = gate_load(p, t * p.gate_row + h * p.gate_head + (ch + 4 * j) * 4);
   }
+  if (r.s0 != t || r.n != 1) {
+    i = request_of(p.starts, p.batch, t);
+    r = i < p.batch ? pa_request(p, i) : PaRequest{-1, 0, 0};
+    if (i < p.batch) base = p.work_base[i];
+  }
+  const int per = how.x;
+  const bool alone = how.y;
   float4 o[4];
   float den = 0.0f, top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < 4; ++j) o[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  const int i = request_of(p.starts, p.batch, t);
-  const PaRequest r = i < p.batch ? pa_request(p, i) : PaRequest{};
   if (per > 0 && t >= r.s0 && t < r.s0 + r.n) {
-    const int2 base = p.work_base[i];
-    auto join = [&](const float2* ml, const float* from, int rows, int64_t place, int n, int row) {
-      ml += place * rows + row;
-      const float4* src = reinterpret_cast<const float4*>(from + place * rows * D) + ch * rows + row;
-#pragma unroll 4
-      for (int x = 0; x < n; ++x, ml += rows, src += rows * (D / 4)) {
-        const float2 v = *ml;
-        float4 y[4];
+    // b / per, a pair's number: small, so that one correction makes the quotient in binary32 right
+    const float inv_per = 1.0f / (float)per;
+    auto pair_of = [&](int b) {
+      int q = (int)((float)b * inv_per);
+      q -= q * per > b;
+      return q + ((q + 1) * per <= b);
+    };
+    // segments of the row: n_pre of its prefix item, n_own of its own, from their first places on
+    int n_pre = 0, n_own = 0, pre_row = 0, own_row = 0;
+    int64_t pre0 = 0, own0 = 0;
+    const int nq = pa_qtiles(p, r), own_qt = nq > 1 ? pa_quotient(t - r.s0, p.tpi_magic) : 0;
+    const int kt = pa_tiles(p, r, own_qt, alone);
+    if (kt > 0) {
+      int b = base.y + PA_ITEM_COST;
+      if (kvh > 0) b += kvh * (int)pa_own_units(p, r, nq, alone);
+      for (int q = 0; q < own_qt; ++q) b += pa_units(pa_tiles(p, r, q, alone), false);
+      const int c0 = pair_of(b), tl = t - r.s0 - own_qt * p.tpi, rank = tl >= p.tpc;
+      n_own = pair_of(b + kt - 1) - c0 + 1;
+      own0 = base.x + kvh * nq + own_qt + c0;
+      own_row = rank * p.own_half + (tl - rank * p.tpc) * p.G + gh;
+    }
+    if (n_own == 1 && (alone || p.pre_tiles == 0)) return;  // finished where it was computed
+    if (!alone && p.pre_tiles > 0) {
+      const int qt = pa_quotient(t, p.tpi_magic), it = kvh * p.pre_qtiles + qt, tl = t - qt * p.tpi, rank = tl >= p.tpc;
+      const int b = it * pa_units(p.pre_tiles, false) + PA_ITEM_COST, c0 = pair_of(b);
+      n_pre = pair_of(b + p.pre_tiles - 1) - c0 + 1;
+      pre0 = it + c0;
+      pre_row = rank * PA_ROWS + (tl - rank * p.tpc) * p.G + gh;
+    }
+    constexpr int BATCH = 4;  // segments asked for at once
+    const int n = n_pre + n_own;
+    for (int x0 = 0; x0 < n; x0 += BATCH) {
+      float2 ml[BATCH];
+      float4 y[BATCH][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = src[4 * j * rows];
-        const float now = fmaxf(top, v.x);
-        const float w = v.x == -INFINITY ? 0.0f : exp2_approx(v.x - now);
+      for (int u = 0; u < BATCH; ++u) {
+        const int x = min(x0 + u, n - 1);
+        const bool pre = x < n_pre;
+        const int rows = pre ? 2 * PA_ROWS : p.own_rows, row = pre ? pre_row : own_row;
+        const int64_t at = (pre ? pre0 + x : own0 + x - n_pre) * rows;
+        ml[u] = (pre ? p.pre_ml : p.own_ml)[at + row];
+        const float4* src = reinterpret_cast<const float4*>((pre ? p.pre_o : p.own_o) + at * D) + ch * rows + row;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[u][j] = src[4 * j * rows];
+      }
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        if (x0 + u >= n) break;
+        const float now = fmaxf(top, ml[u].x);
+        const float w = ml[u].x == -INFINITY ? 0.0f : exp2_approx(ml[u].x - now);
         const float keep = top == -INFINITY ? 0.0f : exp2_approx(top - now);
         top = now;
-        den = fmaf(den, keep, v.y * w);
+        den = fmaf(den, keep, ml[u].y * w);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          o[j].x = fmaf(o[j].x, keep, y[j].x * w);
-          o[j].y = fmaf(o[j].y, keep, y[j].y * w);
-          o[j].z = fmaf(o[j].z, keep, y[j].z * w);
-          o[j].w = fmaf(o[j].w, keep, y[j].w * w);
+          o[j].x = fmaf(o[j].x, keep, y[u][j].x * w);
+          o[j].y = fmaf(o[j].y, keep, y[u][j].y * w);
+          o[j].z = fmaf(o[j].z, keep, y[u][j].z * w);
+          o[j].w = fmaf(o[j].w, keep, y[u][j].w * w);
         }
       }
-    };
-    const int nq = pa_qtiles(p, r), own_qt = nq > 1 ? (t - r.s0) / p.tpi : 0;
-    const int kt = pa_tiles(p, r, own_qt, alone);
-    int c0 = 0, n = 0;
-    if (kt > 0) {
-      int b = base.y + kvh * (int)pa_own_units(p, r, nq, alone) + PA_ITEM_COST;
-      for (int q = 0; q < own_qt; ++q) b += pa_units(pa_tiles(p, r, q, alone), p.whole);
-      c0 = b / per;
-      n = (b + kt - 1) / per - c0 + 1;
-    }
-    if (n == 1 && (alone || p.pre_tiles == 0)) return;  // finished where it was computed
-    if (!alone && p.pre_tiles > 0) {
-      const int qt = t / p.tpi, it = kvh * p.pre_qtiles + qt, tl = t - qt * p.tpi, rank = tl >= p.tpc;
-      const int b = it * pa_units(p.pre_tiles, false) + PA_ITEM_COST, p0 = b / per;
-      join(p.pre_ml, p.pre_o, 2 * PA_ROWS, it + p0, (b + p.pre_tiles - 1) / per - p0 + 1,
-           rank * PA_ROWS + (tl - rank * p.tpc) * p.G + gh);
-    }
-    if (n > 0) {
-      const int tl = t - r.s0 - own_qt * p.tpi, rank = tl >= p.tpc;
-      join(p.own_ml, p.own_o, p.own_rows, base.x + kvh * nq + own_qt + c0, n,
-           rank * p.own_half + (tl - rank * p.tpc) * p.G + gh);
     }
   }
   const float inv = den == 0.0f ? 0.0f : 1.0f / den;
@@ -1152,9 +1186,12 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   p.own_limit = (int)std::min<int64_t>((int64_t)a.table_width * block_size, INT32_MAX - PA_KEYS);
   p.batch = a.batch, p.tokens = a.tokens, p.max_new = a.max_new, p.n_kvh = n_kvh, p.G = G;
   p.tpc = tpc, p.tpi = 2 * tpc;
+  auto magic = [](int d) { return d == 1 ? 0u : (unsigned)(((1ull << 32) + d - 1) / d); };
+  p.g_magic = magic(G), p.tpi_magic = magic(p.tpi);
   p.pre_tiles = (int)ceil_div(a.prefix_len, PA_KEYS), p.pre_qtiles = (int)ceil_div(a.tokens, 2 * tpc);
   const int64_t items = (int64_t)p.pre_qtiles * n_kvh;
-  if (items * pa_units(p.pre_tiles, false) >= (int64_t)PA_MANY || (int64_t)a.tokens * n_qh * head > INT32_MAX || n_kvh > 65535)
+  if (items * pa_units(p.pre_tiles, false) >= (int64_t)PA_MANY || (int64_t)a.tokens * n_qh * head > INT32_MAX ||
+      a.tokens >= 1 << 24 || n_kvh > 65535)
     return fail(YSKN_EINVAL, "prefix_attention: too much work");
   p.shared_items = a.prefix_len > 0 ? (int)items : 0;
   // Few items of few tiles: each by one pair of SMs from end to end, which is quicker than the second
