@@ -19,8 +19,8 @@
 // given back, blocks needed, tokens) over the whole batch (at most 4096 requests, from L2)
 // in shared memory, then takes its share of the tokens and of the blocks given back, and no
 // CTA waits for another. A warp's tokens are adjacent: it finds the first one's request by a
-// search of 32 probes a round and walks on from there; the token in a fresh block's first place writes the table entry (a fresh block always starts
-// with a new token). Nothing that any CTA reads is written in the launch: the lengths and the
+// search of 32 probes a round and walks on from there; the token in a fresh block's first place
+// writes the table entry (a fresh block always starts with a new token). Nothing that any CTA reads is written in the launch: the lengths and the
 // stack's count go to other arrays, fresh table entries are never read, and the stack is
 // written only above its old count, read only below it (blocks given back in this step and
 // taken in it are read from the ended request's table row).

@@ -21,7 +21,8 @@
 // 81. Streaming a plain copy and adjusting the history's logits afterwards took 141: two
 // million scattered 4-byte updates.) Some of nearly every 128 neighbouring tokens are in a
 // long history, so the penalties run for nearly every warp: the quotient is the product
-// with the reciprocal, corrected by its residual (one Newton step, Markstein 1990), which rounds as the division.
+// with the reciprocal, corrected by its residual (one Newton step, Markstein 1990), which rounds
+// as the division.
 // A token's count: the top bit for a token of the prompt, the others the count after it, so that
 // a token is seen if it is not zero. Histories shorter than 32768 are counted in 16 bits (two
 // counts a word), longer ones in 32: a chunk may be as large as its counts allow, because every

@@ -18,8 +18,8 @@
 // multiple of W) channels away, by one shuffle per channel (two where pairs straddle the runs).
 // A warp takes up to PP_RUN heads of one token where there are many rows (one where there are
 // few), each row requested while the one before is worked on (two rows ahead leaves room for
-// fewer warps: 86 us for 8192 tokens, not 78; runs of 4: 84); the cosines and sines of its channels are computed
-// once, one pair a lane, while its first rows arrive, and stay in registers. No block-wide step.
+// fewer warps: 86 us for 8192 tokens, not 78; runs of 4: 84); the cosines and sines of its
+// channels are computed once, one pair a lane, while its first rows arrive, and stay in registers. No block-wide step.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -54,7 +54,8 @@ struct PagedPrepParams {
 // Cosine and sine of a binary32 angle: reduced by its nearest multiple of pi / 2 in binary64 (two
 // parts of pi / 2), then on [-pi / 4, pi / 4] polynomials that interpolate (sin r - r) / r^3 and
 // (cos r - 1 + r^2 / 2) / r^4 at the Chebyshev nodes in r^2, in binary32: within 8e-8 (a unit of
-// 1). (With the decode path's portable function, binary64 throughout: 81 us for 8192 tokens, not 78.)
+// 1). (With the decode path's portable function, binary64 throughout: 81 us for 8192 tokens,
+// not 78.)
 // False for an angle past 2^30, whose multiple is not held.
 __device__ __forceinline__ bool turn_of(float angle, float2* turn) {
   const double v = (double)angle;
@@ -62,7 +63,8 @@ __device__ __forceinline__ bool turn_of(float angle, float2* turn) {
   const double r64 = fma((double)n, -6.12323399573676603587e-17, fma((double)n, -1.57079632679489661923, v));
   const float r = (float)r64, t = r * r;
   const float s = fmaf(r * t, fmaf(t, fmaf(t, -1.958789088e-4f, 8.332748271e-3f), -1.666666466e-1f), r);
-  const float c = fmaf(t * t, fmaf(t, fmaf(t, 2.454794208e-5f, -1.388830304e-3f), 4.166666466e-2f), fmaf(t, -0.5f, 1.0f));
+  const float u = fmaf(t, fmaf(t, 2.454794208e-5f, -1.388830304e-3f), 4.166666466e-2f);
+  const float c = fmaf(t * t, u, fmaf(t, -0.5f, 1.0f));
   const float x = n & 1 ? s : c, y = n & 1 ? c : s;  // cosine and sine up to their signs
   *turn = make_float2((n + 1) & 2 ? -x : x, n & 2 ? -y : y);
   return fabsf(angle) < 1073741824.0f;

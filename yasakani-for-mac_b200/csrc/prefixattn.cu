@@ -50,7 +50,8 @@
 //           2^8, so that a weight is at most 256 and o is seldom touched; the join uses the
 //           maximum in use, which cancels. (Two groups that take whole tiles in turn, so that one's
 //           exponentials run beside the other's loads, measured 134 against 110 us at 64 requests
-//           behind 32k rows: with two S tiles it is a tile's latency that counts. A share of the exponentials as polynomials on the FMA pipe: 117 to 119-123 us.)
+//           behind 32k rows: with two S tiles it is a tile's latency that counts. A share of the
+//           exponentials as polynomials on the FMA pipe: 119 to 123 against 117 us.)
 // A tile's rows past the last visible one: their scores are set to -inf before the maximum, P V
 // runs over the 16-row steps that hold a visible row, and warp 3 clears the rest of the last
 // step's V rows in shared memory (a zero weight does not silence a NaN).
@@ -145,7 +146,9 @@ struct PrefixAttnParams {
 };
 
 // n / d by its magic number (0 for d = 1).
-__device__ __forceinline__ int pa_quotient(int n, unsigned magic) { return magic ? (int)__umulhi((unsigned)n, magic) : n; }
+__device__ __forceinline__ int pa_quotient(int n, unsigned magic) {
+  return magic ? (int)__umulhi((unsigned)n, magic) : n;
+}
 
 // The last request whose first token is at or before t (requests without tokens share a
 // start with the next one), or the batch if t is past the last token. One token for each
@@ -325,7 +328,8 @@ __device__ __forceinline__ uint32_t pa_idesc(int dt, int n, uint32_t b_mn, uint3
 __device__ __forceinline__ void umma2_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc,
                                          uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
       "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
       "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(accumulate));
 }
@@ -535,16 +539,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
       total_items = pa_sum(total_items, o.z);
     }
     // Alone, if that is at most an eighth more: about what the join of two results per row costs
-    // (16 prompt chunks: 960 us with prefix items, ALONE us alone).
-    const int pre_units = pa_units(p.pre_tiles, false), pre_all = p.shared_items * pre_units;  // below 2^30: the host looked
+    // (16 prompt chunks: 960 us with prefix items, 850 alone, at the step that added it).
+    const int pre_units = pa_units(p.pre_tiles, false);
+    const int pre_all = p.shared_items * pre_units;  // below 2^30: the host looked
     const bool alone = p.whole || (p.shared_items > 0 && total_of[1] < PA_MANY &&
                                    8ull * total_of[1] <= 9ull * ((unsigned)pre_all + total_of[0]));
     const unsigned units = alone ? units_of[1] : units_of[0], total = alone ? total_of[1] : total_of[0];
-    const unsigned before = pa_sum(alone ? before_of[1] : before_of[0], alone ? ui[1] - units_of[1] : ui[0] - units_of[0]);
+    const unsigned before =
+        alone ? pa_sum(before_of[1], ui[1] - units_of[1]) : pa_sum(before_of[0], ui[0] - units_of[0]);
     items_before = pa_sum(items_before, it - items);
     const bool sound = total_items <= (unsigned)p.own_items && total < PA_MANY;
     const int pre_items = alone ? 0 : p.shared_items, pre = alone ? 0 : pre_all;
-    const int all = sound ? pre + (int)total : 0, share = pairs == PA_MAX_PAIRS ? (all + PA_MAX_PAIRS - 1) / PA_MAX_PAIRS : (all + pairs - 1) / pairs;
+    const int all = sound ? pre + (int)total : 0;
+    const int share = pairs == PA_MAX_PAIRS ? (all + PA_MAX_PAIRS - 1) / PA_MAX_PAIRS : (all + pairs - 1) / pairs;
     const int t0 = min(all, pair * share), t1 = min(all, t0 + share);
     const int at = t0 - pre;  // this pair's first own unit
     if (tid == 0) {
@@ -1131,7 +1138,8 @@ static int paged_map(CUtensorMap* map, const void* base, int dt, int rank, const
   for (int i = 0; i + 1 < rank; ++i) s[i] = (cuuint64_t)(dims[i + 1] == 1 ? dims[0] : strides[i]) * 2;
   const CUresult r = fn(map, dt == YSKN_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                         rank, const_cast<void*>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        box[0] == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        box[0] == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(YSKN_EINVAL, "prefix_attention: strides that a tensor map cannot hold");
   return YSKN_OK;
@@ -1182,7 +1190,8 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   p.prefix_blocks = a.prefix_blocks;
   p.tables = a.block_tables, p.table_stride = a.table_stride;
   p.lens = a.lens, p.starts = a.starts;
-  p.n_blocks = a.n_blocks, p.block_shift = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : 7, p.prefix_len = a.prefix_len;
+  p.n_blocks = a.n_blocks, p.prefix_len = a.prefix_len;
+  p.block_shift = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : 7;
   p.own_limit = (int)std::min<int64_t>((int64_t)a.table_width * block_size, INT32_MAX - PA_KEYS);
   p.batch = a.batch, p.tokens = a.tokens, p.max_new = a.max_new, p.n_kvh = n_kvh, p.G = G;
   p.tpc = tpc, p.tpi = 2 * tpc;

@@ -783,8 +783,8 @@ def prefix_attention_work_bytes(tokens, batch, max_new, n_qh, n_kvh, head):
 def prefix_attention(q, k_cache, v_cache, block_tables, lens, starts, max_new, work, out, prefix_blocks=None,
                      prefix_len=0, gate=None, scale=None, stream=None):
     """yskn_b200_prefix_attention: q and gate (of q's type, or f32) [T][n_qh][D] with dense
-    channels, the caches as paged_prep, each request's own blocks in block_tables (int32 [batch][width]) and the shared
-    prefix's in prefix_blocks; lens and starts as batch_plan writes them (at most max_new tokens
+    channels, the caches as paged_prep, each request's own blocks in block_tables (int32
+    [batch][width]) and the shared prefix's in prefix_blocks; lens and starts as batch_plan writes them (at most max_new tokens
     a request) -> out (dense [T][n_qh][D]). scale defaults to 1 / sqrt(D). work: uint8, of
     prefix_attention_work_bytes(T, batch, max_new, n_qh, n_kvh, D) bytes."""
     if not _DT:
@@ -857,7 +857,6 @@ def logits_adjust(logits, out, history=None, history_lens=None, prompt_lens=None
         fp, ok = frequency.data_ptr(), ok and frequency.dtype is f32 and frequency.numel() == M
     _need(ok, "logits_adjust: a length or penalty for each row expected")
     _launch("logits_adjust", ARGS["logits_adjust"].pack(
-        logits.data_ptr(), xs[0], 0 if history is None else history.data_ptr(), hs[0], lp, pp, rp, ep,
-        fp,
+        logits.data_ptr(), xs[0], 0 if history is None else history.data_ptr(), hs[0], lp, pp, rp, ep, fp,
         0 if bias is None else bias_ids.data_ptr(), 0 if bias is None else bias.data_ptr(),
         0 if mask is None else mask.data_ptr(), ms[0], out.data_ptr(), os_[0], M, V, width, n_bias), out, stream)
