@@ -73,6 +73,15 @@ constexpr int PA_SLOT = 16384;  // bytes per ring slot
 constexpr int PA_THREADS = 384;
 constexpr int PA_MAX_PAIRS = 74;
 constexpr int PA_MAX_SLOTS = 12;
+constexpr int PA_THIN_ROWS = 8;      // rows of a thin item, at most
+constexpr int PA_THIN_SHIFT = 4;     // a thin item's tiles: 16 rows of the cache
+constexpr int PA_THIN_COST = 3;      // its fixed cost in such tiles
+constexpr int PA_THIN_WHOLE = 6;     // tiles up to which few thin items are not cut
+constexpr int PA_THIN_LEAST = 4;     // units of a warp, at least
+constexpr int PA_THIN_WARPS = 12;    // warps of a CTA: each takes thin items by itself
+constexpr int PA_THIN_STAGE = 16384; // bytes on the way to one of them
+constexpr int PA_THIN_PER_TILE = 10; // thin tiles (two CTAs) in the time of a pair's tile of 128
+constexpr int PA_MAX_THIN = 2 * PA_MAX_PAIRS * PA_THIN_WARPS;
 constexpr int PA_WHOLE_TILES = 2;  // tiles up to which few items are not cut
 constexpr int PA_ITEM_COST = 3;  // an item's fixed cost (Q, the last P V's wait, its result) in tiles
 
@@ -102,7 +111,7 @@ inline PaWork pa_work(int tokens, int batch, int max_new, int n_qh, int n_kvh, i
   const int64_t pre_items = ceil_div(tokens, tpi) * n_kvh;
   // sum of ceil(n_i / tpi) over requests with n_i > 0: at most one more than n_i / tpi each
   const int64_t own_items = (std::min(batch, tokens) + (int64_t)tokens / tpi) * n_kvh;
-  const int64_t pre = pre_items + PA_MAX_PAIRS, own = own_items + PA_MAX_PAIRS;
+  const int64_t pre = pre_items + PA_MAX_PAIRS, own = own_items + (G * max_new <= PA_THIN_ROWS ? PA_MAX_THIN : PA_MAX_PAIRS);
   PaWork w{};
   w.own_half = G * std::min(tpc, max_new);
   w.own_rows = max_new > tpc ? 2 * w.own_half : w.own_half;
@@ -130,10 +139,17 @@ struct PrefixAttnParams {
   int tpc, tpi;  // tokens per CTA and per item
   unsigned g_magic, tpi_magic;  // ceil(2^32 / d): quotients of numbers below 2^32 / d
   int pre_tiles, pre_qtiles, shared_items;  // prefix items, if there are any
+  // Own items: thin ones (below) or not, the rows of a tile as a power of two, the prefix's tiles
+  // where an own item takes them, and an item's fixed cost in tiles.
+  bool thin;
+  int tile_shift, own_pre, item_cost;
+  const uint16_t *q, *k_cache, *v_cache;  // thin items read them by address
+  int64_t q_row, q_head;
+  CacheStrides cache;
   bool whole;  // items are not cut: no join
   float c;     // |scale| log2 e
   uint32_t negate_q;
-  int2* work_per;         // units per pair of this call, and whether alone: for the join
+  int4* work_per;         // for the join: units per pair of prefix items and of own ones, whether alone
   int2* work_base;        // [batch] own items, and units of all items, before each request's own
   // per place: (m, l) of each row; o as [D / 4][rows][4], so that a warp's rows are adjacent
   float2 *pre_ml, *own_ml;
@@ -183,26 +199,26 @@ __device__ __forceinline__ int pa_visible(const PrefixAttnParams& p, const PaReq
   return min(max(r.len - r.n + upto - p.prefix_len, 0), p.own_limit);
 }
 __device__ __forceinline__ int pa_own_tiles(const PrefixAttnParams& p, const PaRequest& r, int qt) {
-  return (pa_visible(p, r, min(r.n, (qt + 1) * p.tpi)) + PA_KEYS - 1) / PA_KEYS;
+  return (pa_visible(p, r, min(r.n, (qt + 1) * p.tpi)) + (1 << p.tile_shift) - 1) >> p.tile_shift;
 }
-// Units of an item of so many tiles (0: nothing to do): unit u is tile u - PA_ITEM_COST; or the
-// whole item is one unit.
-__host__ __device__ __forceinline__ int pa_units(int tiles, bool whole) {
-  return tiles <= 0 ? 0 : whole ? 1 : tiles + PA_ITEM_COST;
+// Units of an item of so many tiles (0: nothing to do): unit u is tile u - cost; or the whole
+// item is one unit.
+__host__ __device__ __forceinline__ int pa_units(int tiles, bool whole, int cost) {
+  return tiles <= 0 ? 0 : whole ? 1 : tiles + cost;
 }
 __device__ __forceinline__ int pa_qtiles(const PrefixAttnParams& p, const PaRequest& r) {
   return r.n <= p.tpi ? r.n > 0 : pa_quotient(r.n + p.tpi - 1, p.tpi_magic);
 }
 // Tiles of a request's item `qt`: own ones, after the prefix's where there are no prefix items.
 __device__ __forceinline__ int pa_tiles(const PrefixAttnParams& p, const PaRequest& r, int qt, bool alone) {
-  return pa_own_tiles(p, r, qt) + (alone ? p.pre_tiles : 0);
+  return pa_own_tiles(p, r, qt) + (alone ? p.own_pre : 0);
 }
 // Units of a request's items of one KV head; sums of units stop at PA_MANY, which is an error.
 constexpr unsigned PA_MANY = 1u << 30;
 __device__ __forceinline__ unsigned pa_sum(unsigned a, unsigned b) { return min(a + b, PA_MANY); }
 __device__ __forceinline__ unsigned pa_own_units(const PrefixAttnParams& p, const PaRequest& r, int nq, bool alone) {
   unsigned u = 0;
-  for (int q = 0; q < nq; ++q) u = pa_sum(u, pa_units(pa_tiles(p, r, q, alone), p.whole));
+  for (int q = 0; q < nq; ++q) u = pa_sum(u, pa_units(pa_tiles(p, r, q, alone), p.whole, p.item_cost));
   return u;
 }
 
@@ -223,7 +239,9 @@ struct PaSegment {
 
 // Where a pair's units begin, found by each of its CTAs.
 struct PaStart {
-  int left;          // units of this pair
+  int who;           // this pair, or this warp of those that take thin items
+  bool thin;         // the latter
+  int left;          // its units
   int alone;         // no prefix items: each request's items take the prefix too
   int pre_item, u0;  // prefix item and unit in it
   int req, item;     // own items: request and the items before it
@@ -234,12 +252,13 @@ struct PaStart {
 struct PaWalk {
   const PrefixAttnParams& p;
   const bool alone;
+  const int who;
   int left, pre_item, u0, req, item, kvh, qt;
   PaRequest r;
   int nq;
   bool loaded;
   __device__ PaWalk(const PrefixAttnParams& p_, const PaStart& s)
-      : p(p_), alone(s.alone), left(s.left), pre_item(s.pre_item), u0(s.u0), req(s.req), item(s.item), kvh(0), qt(0),
+      : p(p_), alone(s.alone), who(s.who), left(s.left), pre_item(s.pre_item), u0(s.u0), req(s.req), item(s.item), kvh(0), qt(0),
         r{}, nq(0), loaded(false) {
     if (s.skip > 0) {
       load();
@@ -247,7 +266,7 @@ struct PaWalk {
       kvh = s.skip / head;
       int skip = s.skip - kvh * head;
       for (;; ++qt) {
-        const int u = pa_units(pa_tiles(p, r, qt, alone), p.whole);
+        const int u = pa_units(pa_tiles(p, r, qt, alone), p.whole, p.item_cost);
         if (skip < u) break;
         skip -= u;
       }
@@ -284,7 +303,7 @@ struct PaWalk {
           s.tok0 = r.s0 + q * p.tpi;
           s.ntok = min(p.tpi, r.n - q * p.tpi);
           s.req = req;
-          s.pre = alone ? p.pre_tiles : 0;
+          s.pre = alone ? p.own_pre : 0;
           s.keys = pa_visible(p, r, q * p.tpi + s.ntok);
           s.first = r.len - r.n + q * p.tpi + 1;
           if (take(s, kt, item + kvh * nq + q)) return true;
@@ -299,11 +318,12 @@ struct PaWalk {
   }
   // This pair's part of an item; false if it holds no tile.
   __device__ bool take(PaSegment& s, int tiles, int it) {
-    const int n = p.whole ? 1 : min(tiles + PA_ITEM_COST - u0, left);
-    s.key0 = p.whole ? 0 : max(u0 - PA_ITEM_COST, 0);
-    s.key1 = p.whole ? tiles : max(u0 + n - PA_ITEM_COST, 0);
-    s.whole = !s.prefix && s.key0 == 0 && s.key1 == tiles && s.pre == p.pre_tiles;
-    s.place = (int64_t)it + (blockIdx.x >> 1);
+    const int cost = s.prefix ? PA_ITEM_COST : p.item_cost;
+    const int n = p.whole ? 1 : min(tiles + cost - u0, left);
+    s.key0 = p.whole ? 0 : max(u0 - cost, 0);
+    s.key1 = p.whole ? tiles : max(u0 + n - cost, 0);
+    s.whole = !s.prefix && s.key0 == 0 && s.key1 == tiles && s.pre == p.own_pre;
+    s.place = (int64_t)it + who;
     left -= n;
     u0 = 0;
     return s.key0 < s.key1;
@@ -443,6 +463,284 @@ __device__ __forceinline__ void quarter_sync(int quarter) {
   asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
 }
 
+// Where there is no join: zeros for this CTA's share of the tokens that no item holds. One warp.
+template <int D>
+__device__ __forceinline__ void zero_unheld(const PrefixAttnParams& p, int lane) {
+  for (int t = blockIdx.x; t < p.tokens; t += gridDim.x) {
+    const int i = request_of(p.starts, p.batch, t);
+    const PaRequest r = i < p.batch ? pa_request(p, i) : PaRequest{};
+    if (t >= r.s0 && t < r.s0 + r.n && pa_tiles(p, r, pa_quotient(t - r.s0, p.tpi_magic), true) > 0) continue;
+    uint4* row = reinterpret_cast<uint4*>(p.out + (int64_t)t * p.n_kvh * p.G * D);
+    for (int x = lane; x < p.n_kvh * p.G * D / 8; x += 32) row[x] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// ---- thin items: up to 8 rows (one token of up to 8 query heads a KV head, or a few of fewer)
+// against the request's own rows. 256 rows of MMA for 6 are 2048 clocks a tile for work that the
+// memory bounds, and an item's Q, S, P, O pass through one after another (64 requests of 1 to 1024
+// own rows: 74 us for 142 MB). Here each of 8 warps keeps a softmax of its own over every 8th
+// slice of 16 cache rows, with warp-level MMAs (m16n8k16): nothing is shared until the item's end,
+// where the 8 results are joined in shared memory. What bounds it: bytes, so the copies run a ring
+// of 8 chunks (16 rows of 64 channels of K or V) ahead, across items, 128 KB an SM.
+//   S = Q K^T   A: Q, rows 0..7 (8..15 zero); B: K, of a lane (g, t) the 16 bytes 8 t of row g of a
+//               chunk's half: two steps of 16 channels, in an order that Q's registers share;
+//   O^T = V^T P^T  B: P^T, which is S as it left the first MMA (row g, keys 2t, 2t+1 and 8 on);
+//               A: V^T, of a lane the 16 bytes 8 g of those four rows: word w's two channels of
+//               two rows by one byte permutation each, rows g and g + 8 of MMA w.
+// A chunk's rows are 128 bytes; 8 lanes bring one (lanes that fetch just what they need later,
+// 64 or 32 bytes of a line a request, had the L2 answer 1.3 sectors a request: 54 us, now THINCO). The
+// 16-byte unit c of row r lies at c ^ (4 (r2 ^ r0) + 2 r1), r's low bits, where both reads find their
+// 8 lanes on 8 different units.
+template <int DT>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  if constexpr (DT == YSKN_DT_BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 16 bytes into shared memory, or zeros.
+__device__ __forceinline__ void copy16(uint32_t to, const uint16_t* from, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 stage_load(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
+// The rows that this warp's copies are at. Each segment that it comes to goes into the warp's queue in
+// shared memory, from which the arithmetic takes it: at most LEAD + 2 slices later.
+constexpr int PA_THIN_QUEUE = 8;
+struct ThinCursor {
+  const PrefixAttnParams& p;
+  PaWalk walk;
+  PaSegment seg;
+  PaSegment* queue;
+  int found;  // segments put into it
+  int kt;
+  bool live;
+  int block;  // of slice kt: asked for one slice ahead
+  const uint16_t *k, *v;  // the slice that is being copied, and how many of its rows there are
+  int rows;
+  __device__ ThinCursor(const PrefixAttnParams& p_, const PaStart& s, PaSegment* queue_)
+      : p(p_), walk(p_, s), queue(queue_), found(0), kt(0), live(true), block(0), k(nullptr), v(nullptr), rows(0) {
+    seg.key1 = 0;
+    advance();
+  }
+  __device__ void advance() {
+    if (++kt >= seg.key1 && live) {
+      live = walk.next(seg);  // a segment holds a slice
+      kt = seg.key0;
+      if (live) {
+        if ((threadIdx.x & 31) == 0) queue[found % PA_THIN_QUEUE] = seg;
+        __syncwarp();
+        ++found;
+      }
+    }
+    if (live) {
+      const int at = (kt < seg.pre ? kt : kt - seg.pre) << PA_THIN_SHIFT >> p.block_shift;
+      block = __ldg(kt < seg.pre ? p.prefix_blocks + at : p.tables + (int64_t)seg.req * p.table_stride + at);
+    }
+  }
+  // To the next slice's rows.
+  __device__ void next() {
+    rows = 0;
+    k = p.k_cache, v = p.v_cache;
+    if (!live) return;
+    const int at = (kt < seg.pre ? kt : kt - seg.pre) << PA_THIN_SHIFT;
+    if ((unsigned)block < (unsigned)p.n_blocks) {
+      rows = min(1 << PA_THIN_SHIFT, (kt < seg.pre ? p.prefix_len : seg.keys) - at);
+      const int64_t from = block * p.cache.block + (at & ((1 << p.block_shift) - 1)) * p.cache.token +
+                           seg.kvh * p.cache.head;
+      k += from, v += from;
+    } else {
+      raise_device_error(p.err, DERR_RANGE);  // the copies give zeros
+    }
+    advance();
+  }
+};
+
+template <int D, int DT>
+__device__ __forceinline__ void thin_items(const PrefixAttnParams& p, const PaStart& start, uint8_t* smem, int warp, int lane) {
+  constexpr int C = D / 64, CHUNKS = 2 * C;  // chunks of a slice's K; of K and V
+  constexpr int LEAD = 8 / CHUNKS;           // slices on the way
+  static_assert(PaShape<D>::Q_BYTES + PaShape<D>::RING * PA_SLOT >=
+                    PA_THIN_WARPS * (PA_THIN_STAGE + PA_THIN_QUEUE * (int)sizeof(PaSegment)) &&
+                    LEAD + 2 < PA_THIN_QUEUE,
+                "the warps' rings and queues");
+  const uint32_t mine = smem_u32(smem + warp * PA_THIN_STAGE);
+  const int g = lane >> 2, t = lane & 3;
+  const float c = p.negate_q ? -p.c : p.c;
+  const int64_t tok = p.cache.token;
+  PaSegment* queue = reinterpret_cast<PaSegment*>(smem + PA_THIN_WARPS * PA_THIN_STAGE) + warp * PA_THIN_QUEUE;
+  ThinCursor from(p, start, queue);
+  // Chunk x of the slice that the cursor is at, into place `at` of the ring.
+  const int row0 = lane >> 3, unit = lane & 7;
+  const uint32_t put = row0 * 128 + (unit ^ ((row0 & 1) << 2) ^ (row0 & 2)) * 16;
+  auto copy = [&](int x, uint32_t at) {
+    const uint16_t* src = (x < C ? from.k + 64 * x : from.v + 64 * (x - C)) + row0 * tok + 8 * unit;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {  // rows 4 u + row0
+      const bool valid = 4 * u + row0 < from.rows;
+      copy16(at + u * 512 + (put ^ ((u & 1) << 6)), valid ? src + 4 * u * tok : p.k_cache, valid);
+    }
+  };
+  // where this lane reads: rows g and g + 8 of K, units t and t + 4; rows 2t, 2t + 1, 2t + 8 and
+  // 2t + 9 of V, unit g
+  const uint32_t get_k = g * 128 + (t ^ (((g >> 2 ^ g) & 1) << 2) ^ (g & 2)) * 16;
+  const uint32_t get_v = 2 * t * 128 + (g ^ ((t >> 1) << 2) ^ ((t & 1) << 1)) * 16;
+  auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+  const int tl = pa_quotient(g, p.g_magic);  // row g's token
+  uint4 q[2 * C];
+  auto load_q = [&](const PaSegment& seg) {
+    const int h = seg.kvh * p.G + g - tl * p.G;
+#pragma unroll
+    for (int x = 0; x < 2 * C; ++x) {
+      q[x] = make_uint4(0, 0, 0, 0);
+      if (g < seg.ntok * p.G)
+        q[x] = __ldg(reinterpret_cast<const uint4*>(p.q + (seg.tok0 + tl) * p.q_row + h * p.q_head + 32 * x + 8 * t));
+    }
+  };
+  if (from.found > 0) load_q(queue[0]);  // ahead of the copies, behind which it would wait for microseconds
+#pragma unroll 1
+  for (int i = 0; i < LEAD; ++i) {
+    from.next();
+#pragma unroll
+    for (int x = 0; x < CHUNKS; ++x) copy(x, mine + (i * CHUNKS + x) * 2048), commit();
+  }
+  int turn = 0;  // the slice's place in the ring
+  for (int taken = 0; taken < from.found;) {
+    const PaSegment& seg = queue[taken % PA_THIN_QUEUE];
+    const int n_rows = seg.ntok * p.G, sees = seg.first + tl;  // rows of the sequence that row g sees
+    float o[C][4][4];
+#pragma unroll
+    for (int x = 0; x < C * 16; ++x) o[x / 16][x / 4 % 4][x % 4] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll 1
+    for (int kt = seg.key0, end = seg.key1; kt < end; ++kt) {
+      from.next();
+      const uint32_t at = mine + turn * (CHUNKS * 2048);
+      float s[4][4];  // 8 keys; even and odd steps apart
+#pragma unroll
+      for (int x = 0; x < 16; ++x) s[x / 4][x % 4] = 0.0f;
+#pragma unroll
+      for (int x = 0; x < C; ++x) {
+        asm volatile("cp.async.wait_group 7;" ::: "memory");
+        __syncwarp();
+        uint4 k[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) k[u] = stage_load(at + x * 2048 + (u >> 1) * 1024 + (get_k ^ ((u & 1) << 6)));
+        __syncwarp();
+        copy(x, at + x * 2048), commit();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint4 a = q[2 * x + (u & 1)];
+          mma16816<DT>(s[u >> 1], a.x, 0, a.y, 0, k[u].x, k[u].y);
+          mma16816<DT>(s[2 + (u >> 1)], a.z, 0, a.w, 0, k[u].z, k[u].w);
+        }
+      }
+      // row g, keys 2t, 2t + 1, 2t + 8, 2t + 9
+      const bool pre = kt < seg.pre;
+      const int first = (pre ? kt : kt - seg.pre) << PA_THIN_SHIFT;
+      const int seen = min((pre ? p.prefix_len : seg.keys) - first, sees - first - (pre ? 0 : p.prefix_len)) - 2 * t;
+      float z[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        z[x] = (s[x >> 1][x & 1] + s[2 + (x >> 1)][x & 1]) * c;
+        if ((x & 1) + 8 * (x >> 1) >= seen) z[x] = -INFINITY;
+      }
+      float top = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const bool grown = top > m + 8.0f;  // the maximum may lag by 2^8
+      if (__any_sync(0xffffffffu, grown)) {
+        const float f = grown ? exp2_approx(m - top) : 1.0f;
+        const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+#pragma unroll
+        for (int x = 0; x < C * 4; ++x) {
+          float(&y)[4] = o[x / 4][x % 4];
+          y[0] *= f0, y[1] *= f1, y[2] *= f0, y[3] *= f1;
+        }
+        l *= f;
+        if (grown) m = top;
+      }
+      const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) z[x] = exp2_approx(z[x] - base);
+      l += (z[0] + z[1]) + (z[2] + z[3]);
+      const uint32_t b0 = Elem<DT>::pack(z[0], z[1]), b1 = Elem<DT>::pack(z[2], z[3]);
+#pragma unroll
+      for (int x = 0; x < C; ++x) {
+        asm volatile("cp.async.wait_group 7;" ::: "memory");
+        __syncwarp();
+        uint32_t v[4][4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint4 y =
+              stage_load(at + (C + x) * 2048 + (u >> 1) * 1024 + (u & 1) * 128 + (get_v ^ ((u & 1) << 6)));
+          v[u][0] = y.x, v[u][1] = y.y, v[u][2] = y.z, v[u][3] = y.w;
+        }
+        __syncwarp();
+        copy(C + x, at + (C + x) * 2048), commit();
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          mma16816<DT>(o[x][w], __byte_perm(v[0][w], v[1][w], 0x5410), __byte_perm(v[0][w], v[1][w], 0x7632),
+                       __byte_perm(v[2][w], v[3][w], 0x5410), __byte_perm(v[2][w], v[3][w], 0x7632), b0, b1);
+      }
+      if (++turn == LEAD) turn = 0;
+    }
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (seg.whole) {
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {  // row 2t + y: channels 64 x + 8 g + 0..7
+        const int row = 2 * t + y, rt = pa_quotient(row, p.g_magic), rh = seg.kvh * p.G + row - rt * p.G;
+        const float f = __shfl_sync(0xffffffffu, inv, 8 * t + 4 * y);
+        if (row >= n_rows) continue;
+        const int64_t tk = seg.tok0 + rt;
+        uint16_t* out = p.out + (tk * p.n_kvh * p.G + rh) * D + 8 * g;
+        const int64_t gate = tk * p.gate_row + rh * p.gate_head + 8 * g;
+#pragma unroll
+        for (int x = 0; x < C; ++x) {
+          float e[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) e[k] = o[x][k / 2][y + 2 * (k % 2)] * f;
+          if (p.gate) {
+            const float4 a = gate_value<DT>(p, gate_load(p, gate + 64 * x));
+            const float4 d = gate_value<DT>(p, gate_load(p, gate + 64 * x + 4));
+            const float gs[8] = {a.x, a.y, a.z, a.w, d.x, d.y, d.z, d.w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) e[k] = gated(e[k], gs[k]);
+          }
+          *reinterpret_cast<uint4*>(out + 64 * x) = make_uint4(Elem<DT>::pack(e[0], e[1]), Elem<DT>::pack(e[2], e[3]),
+                                                               Elem<DT>::pack(e[4], e[5]), Elem<DT>::pack(e[6], e[7]));
+        }
+      }
+    } else {
+      const int64_t at = seg.place * p.own_rows;
+      if (t == 0 && g < n_rows) p.own_ml[at + g] = make_float2(m, l);
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        if (2 * t + y >= n_rows) continue;
+        float4* to = reinterpret_cast<float4*>(p.own_o + at * D) + 2 * g * p.own_rows + 2 * t + y;
+#pragma unroll
+        for (int x = 0; x < C; ++x) {
+          to[16 * x * p.own_rows] = make_float4(o[x][0][y], o[x][0][2 + y], o[x][1][y], o[x][1][2 + y]);
+          to[(16 * x + 1) * p.own_rows] = make_float4(o[x][2][y], o[x][2][2 + y], o[x][3][y], o[x][3][2 + y]);
+        }
+      }
+    }
+    if (++taken < from.found) load_q(queue[taken % PA_THIN_QUEUE]);
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
 // Shared memory beside Q and the ring. "First": only the first CTA's copy is used.
 struct PaShared {
   uint64_t full[PA_MAX_SLOTS];   // ring place landed in both CTAs (first)
@@ -455,7 +753,7 @@ struct PaShared {
   int2 tail_at;
   uint32_t tmem_slot;
   int abort_word;
-  PaStart start;
+  PaStart start[PA_THIN_WARPS];  // of the pair's walk (all alike), or of each warp's
   uint3 sum[PA_THREADS / 32];
   float half[2][2][PA_ROWS];  // tile parity, half, row: what a row's halves exchange
 };
@@ -540,34 +838,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
     }
     // Alone, if that is at most an eighth more: about what the join of two results per row costs
     // (16 prompt chunks: 960 us with prefix items, 850 alone, at the step that added it).
-    const int pre_units = pa_units(p.pre_tiles, false);
+    const int pre_units = pa_units(p.pre_tiles, false, PA_ITEM_COST);
     const int pre_all = p.shared_items * pre_units;  // below 2^30: the host looked
+    const unsigned long long pre_time = (unsigned long long)pre_all * (p.thin ? PA_THIN_PER_TILE : 1);
     const bool alone = p.whole || (p.shared_items > 0 && total_of[1] < PA_MANY &&
-                                   8ull * total_of[1] <= 9ull * ((unsigned)pre_all + total_of[0]));
+                                   8ull * total_of[1] <= 9ull * (pre_time + total_of[0]));
     const unsigned units = alone ? units_of[1] : units_of[0], total = alone ? total_of[1] : total_of[0];
     const unsigned before =
         alone ? pa_sum(before_of[1], ui[1] - units_of[1]) : pa_sum(before_of[0], ui[0] - units_of[0]);
     items_before = pa_sum(items_before, it - items);
     const bool sound = total_items <= (unsigned)p.own_items && total < PA_MANY;
-    const int pre_items = alone ? 0 : p.shared_items, pre = alone ? 0 : pre_all;
-    const int all = sound ? pre + (int)total : 0;
-    const int share = pairs == PA_MAX_PAIRS ? (all + PA_MAX_PAIRS - 1) / PA_MAX_PAIRS : (all + pairs - 1) / pairs;
-    const int t0 = min(all, pair * share), t1 = min(all, t0 + share);
-    const int at = t0 - pre;  // this pair's first own unit
-    if (tid == 0) {
-      PaStart s{t1 - t0, alone, pre_items, 0, 0, 0, 0};
-      if (t0 < pre) {
+    const int pre_items = alone ? 0 : p.shared_items, pre = alone || !sound ? 0 : pre_all;
+    const int own = sound ? (int)total : 0;
+    // Without thin items, the pairs share prefix units and then own ones as one line. With them, the
+    // first pairs take the prefix items, as many as their part of the time, and each warp of the
+    // other pairs a share of the thin ones.
+    int tc = pairs, share_pre, share_own;
+    if (!p.thin) {
+      const int all = pre + own;
+      share_pre = pairs == PA_MAX_PAIRS ? (all + PA_MAX_PAIRS - 1) / PA_MAX_PAIRS : (all + pairs - 1) / pairs;
+      share_own = share_pre;
+    } else {
+      if (pre == 0) tc = 0;
+      else if (own > 0)
+        tc = min(max((int)((float)pairs * (float)pre_time / ((float)pre_time + (float)own) + 0.5f), 1), pairs - 1);
+      const int warps = 2 * PA_THIN_WARPS * (pairs - tc);
+      share_pre = tc > 0 ? (pre + tc - 1) / tc : 0;
+      share_own = warps > 0 ? max((own + warps - 1) / warps, p.whole ? 1 : PA_THIN_LEAST) : 0;
+    }
+    const bool thin = pair >= tc;  // this pair's CTAs
+    // a CTA's first thin warp, and from each to its next (neighbours are on different SMs: where there
+    // are few units, every SM has some)
+    const int ctas = 2 * (pairs - tc), who0 = thin ? blockIdx.x - 2 * tc : pair;
+    if (tid < PA_THIN_WARPS) {
+      const int who = who0 + (thin ? tid * ctas : 0), share = thin ? share_own : share_pre;
+      const int all = thin ? own : p.thin ? pre : pre + own, t0 = min(all, who * share);
+      PaStart s{who, thin, min(all, t0 + share) - t0, alone, pre_items, 0, p.thin && !thin ? p.batch : 0, 0, 0};
+      if (!thin && t0 < pre) {
         s.pre_item = t0 / pre_units;
         s.u0 = t0 - s.pre_item * pre_units;
       }
-      sh.start = s;
-      if (blockIdx.x == 0) {
-        *p.work_per = make_int2(share, alone);
+      sh.start[tid] = s;
+      if (blockIdx.x == 0 && tid == 0) {
+        *p.work_per = make_int4(share_pre, share_own, alone, 0);
         if (!sound) raise_device_error(p.err, DERR_RANGE);
       }
     }
     __syncthreads();
-    if (sound && ((at >= (int)before && at < (int)(before + units)) || blockIdx.x == 0)) {
+    // the walks that begin inside this thread's requests: walk x begins at own unit first + x step
+    const int step = ctas * share_own;
+    const int walks = thin ? PA_THIN_WARPS : p.thin ? 0 : 1, first = who0 * share_own - (p.thin ? 0 : pre);
+    const int last = first + (walks - 1) * step;
+    if (sound && units > 0 && ((last >= (int)before && first < (int)(before + units)) || blockIdx.x == 0)) {
       int b = (int)before, item = (int)items_before;
       for (int i = i0; i < i1; ++i) {
         int u = (int)units, n = (int)items;
@@ -577,8 +899,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
           u = (int)pa_own_units(p, r, n, alone) * p.n_kvh;
           n *= p.n_kvh;
         }
-        if (at >= b && at < b + u) sh.start.req = i, sh.start.item = item, sh.start.skip = at - b;
-        if (blockIdx.x == 0) p.work_base[i] = make_int2(item, pre + b);
+        for (int x = 0; x < walks; ++x) {
+          const int at = first + x * step;
+          if (at >= b && at < b + u) {
+            PaStart& s = sh.start[thin ? x : 0];
+            s.req = i, s.item = item, s.skip = at - b;
+          }
+        }
+        if (blockIdx.x == 0) p.work_base[i] = make_int2(item, p.thin ? b : pre + b);
         b += u;
         item += n;
       }
@@ -586,9 +914,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
   }
   __syncthreads();
   const uint32_t tmem = sh.tmem_slot;
-  PaWalk walk(p, sh.start);
+  if (sh.start[0].thin) {
+    if (p.whole && warp == PA_THIN_WARPS - 1) zero_unheld<D>(p, lane);
+    thin_items<D, DT>(p, sh.start[warp], smem, warp, lane);
+  } else {
+  PaWalk walk(p, sh.start[0]);
   PaSegment seg;
-
   if (warp == 0) {
     // ---- K and V through the ring, in the order in which the MMAs use them: this CTA's half of
     // each tile's K rows, and of V's channels
@@ -787,15 +1118,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
       }
     }
   } else if (warp == 3) {
-    // ---- where there is no join: zeros for the tokens that no item holds
-    if (p.whole)
-      for (int t = blockIdx.x; t < p.tokens; t += gridDim.x) {
-        const int i = request_of(p.starts, p.batch, t);
-        const PaRequest r = i < p.batch ? pa_request(p, i) : PaRequest{};
-        if (t >= r.s0 && t < r.s0 + r.n && pa_tiles(p, r, pa_quotient(t - r.s0, p.tpi_magic), true) > 0) continue;
-        uint4* row = reinterpret_cast<uint4*>(p.out + (int64_t)t * p.n_kvh * p.G * D);
-        for (int x = lane; x < p.n_kvh * p.G * D / 8; x += 32) row[x] = make_uint4(0, 0, 0, 0);
-      }
+    if (p.whole) zero_unheld<D>(p, lane);
     // ---- V rows past the last visible one, up to the end of the 16-row step, to zero, in the
     // slots that warp 0 names: once for each segment that ends inside a step
     const uint32_t full0 = first_cta(&sh.full[0]);
@@ -987,6 +1310,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
       if (lane == 0) arrive_first(o_free0);
     }
   }
+  }
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && *abort_flag) raise_device_error(p.err, DERR_TIMEOUT);
@@ -1011,7 +1335,7 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
   const int unit = blockIdx.x * 8 + (threadIdx.x >> 5), idx = unit / PARTS * 8 + (lane & 7);
   const int kvh = blockIdx.y, t = pa_quotient(idx, p.g_magic), gh = idx - t * p.G;
   if (t >= p.tokens) return;
-  const int2 how = *p.work_per;
+  const int4 how = *p.work_per;
   // one token for each request is the common case: its request's numbers are asked for at once
   int i = t;
   PaRequest r{-1, 0, 0};
@@ -1029,17 +1353,15 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
     r = i < p.batch ? pa_request(p, i) : PaRequest{-1, 0, 0};
     if (i < p.batch) base = p.work_base[i];
   }
-  const int per = how.x;
-  const bool alone = how.y;
+  const bool alone = how.z;
   float4 o[4];
   float den = 0.0f, top = -INFINITY;
 #pragma unroll
   for (int j = 0; j < 4; ++j) o[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (per > 0 && t >= r.s0 && t < r.s0 + r.n) {
+  if ((how.x | how.y) > 0 && t >= r.s0 && t < r.s0 + r.n) {
     // b / per, a pair's number: small, so that one correction makes the quotient in binary32 right
-    const float inv_per = 1.0f / (float)per;
-    auto pair_of = [&](int b) {
-      int q = (int)((float)b * inv_per);
+    auto pair_of = [&](int b, int per) {
+      int q = (int)((float)b * (1.0f / (float)per));
       q -= q * per > b;
       return q + ((q + 1) * per <= b);
     };
@@ -1049,19 +1371,19 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
     const int nq = pa_qtiles(p, r), own_qt = nq > 1 ? pa_quotient(t - r.s0, p.tpi_magic) : 0;
     const int kt = pa_tiles(p, r, own_qt, alone);
     if (kt > 0) {
-      int b = base.y + PA_ITEM_COST;
+      int b = base.y + p.item_cost;
       if (kvh > 0) b += kvh * (int)pa_own_units(p, r, nq, alone);
-      for (int q = 0; q < own_qt; ++q) b += pa_units(pa_tiles(p, r, q, alone), false);
-      const int c0 = pair_of(b), tl = t - r.s0 - own_qt * p.tpi, rank = tl >= p.tpc;
-      n_own = pair_of(b + kt - 1) - c0 + 1;
+      for (int q = 0; q < own_qt; ++q) b += pa_units(pa_tiles(p, r, q, alone), false, p.item_cost);
+      const int c0 = pair_of(b, how.y), tl = t - r.s0 - own_qt * p.tpi, rank = tl >= p.tpc;
+      n_own = pair_of(b + kt - 1, how.y) - c0 + 1;
       own0 = base.x + kvh * nq + own_qt + c0;
       own_row = rank * p.own_half + (tl - rank * p.tpc) * p.G + gh;
     }
     if (n_own == 1 && (alone || p.pre_tiles == 0)) return;  // finished where it was computed
     if (!alone && p.pre_tiles > 0) {
       const int qt = pa_quotient(t, p.tpi_magic), it = kvh * p.pre_qtiles + qt, tl = t - qt * p.tpi, rank = tl >= p.tpc;
-      const int b = it * pa_units(p.pre_tiles, false) + PA_ITEM_COST, c0 = pair_of(b);
-      n_pre = pair_of(b + p.pre_tiles - 1) - c0 + 1;
+      const int b = it * pa_units(p.pre_tiles, false, PA_ITEM_COST) + PA_ITEM_COST, c0 = pair_of(b, how.x);
+      n_pre = pair_of(b + p.pre_tiles - 1, how.x) - c0 + 1;
       pre0 = it + c0;
       pre_row = rank * PA_ROWS + (tl - rank * p.tpc) * p.G + gh;
     }
@@ -1184,7 +1506,14 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   const PaWork w = pa_work(a.tokens, a.batch, a.max_new, n_qh, n_kvh, head);
   if (a.work_bytes < w.bytes) return fail(YSKN_EINVAL, "prefix_attention: workspace too small");
   const int G = n_qh / n_kvh, tpc = PA_ROWS / G;
+  int dev = 0, sms = 2 * PA_MAX_PAIRS;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int pairs = std::min(sms / 2, PA_MAX_PAIRS);
   PrefixAttnParams p{};
+  p.q = reinterpret_cast<const uint16_t*>(a.q), p.q_row = a.q_row, p.q_head = a.q_head;
+  p.k_cache = reinterpret_cast<const uint16_t*>(a.k_cache), p.v_cache = reinterpret_cast<const uint16_t*>(a.v_cache);
+  p.cache = {a.block_stride, a.token_stride, a.head_stride};
   p.gate = a.gate, p.gate_f32 = a.gate_dtype == YSKN_DT_F32;
   p.gate_row = a.gate_row, p.gate_head = a.gate_head;
   p.prefix_blocks = a.prefix_blocks;
@@ -1199,21 +1528,25 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   p.g_magic = magic(G), p.tpi_magic = magic(p.tpi);
   p.pre_tiles = (int)ceil_div(a.prefix_len, PA_KEYS), p.pre_qtiles = (int)ceil_div(a.tokens, 2 * tpc);
   const int64_t items = (int64_t)p.pre_qtiles * n_kvh;
-  if (items * pa_units(p.pre_tiles, false) >= (int64_t)PA_MANY || (int64_t)a.tokens * n_qh * head > INT32_MAX ||
+  if (items * pa_units(p.pre_tiles, false, PA_ITEM_COST) >= (int64_t)PA_MANY || (int64_t)a.tokens * n_qh * head > INT32_MAX ||
       a.tokens >= 1 << 24 || n_kvh > 65535)
     return fail(YSKN_EINVAL, "prefix_attention: too much work");
   p.shared_items = a.prefix_len > 0 ? (int)items : 0;
   // Few items of few tiles: each by one pair of SMs from end to end, which is quicker than the second
   // launch that joins its parts (two requests of up to 64 rows: 16.4 us cut, 13.9 whole without a
   // prefix, 15.2 and 15.4 behind 100 rows, 15.4 and 16.1 behind 256).
-  const int64_t most_tiles = p.pre_tiles + ceil_div(p.own_limit, PA_KEYS);
-  p.whole = w.own_items <= PA_MAX_PAIRS && most_tiles <= PA_WHOLE_TILES;
+  p.thin = G * a.max_new <= PA_THIN_ROWS && pairs > 1;
+  p.tile_shift = p.thin ? PA_THIN_SHIFT : 7;
+  p.own_pre = (int)ceil_div(a.prefix_len, 1 << p.tile_shift);
+  p.item_cost = p.thin ? PA_THIN_COST : PA_ITEM_COST;
+  const int64_t most_tiles = p.own_pre + ceil_div(p.own_limit, 1 << p.tile_shift);
+  p.whole = w.own_items <= (p.thin ? 2 * PA_THIN_WARPS : 1) * pairs && most_tiles <= (p.thin ? PA_THIN_WHOLE : PA_WHOLE_TILES);
   p.many_per_head = PA_MANY / (unsigned)n_kvh;
   // a scale of zero keeps its meaning (equal weights) with a factor that leaves -inf alone
   p.c = std::max(std::fabs(a.scale) * 1.4426950408889634f, 1e-30f);
   p.negate_q = a.scale < 0.0f;
   uint8_t* work = reinterpret_cast<uint8_t*>(a.work);
-  p.work_per = reinterpret_cast<int2*>(work);
+  p.work_per = reinterpret_cast<int4*>(work);
   p.work_base = reinterpret_cast<int2*>(work + w.base);
   p.pre_ml = reinterpret_cast<float2*>(work + w.pre_ml), p.pre_o = reinterpret_cast<float*>(work + w.pre_o);
   p.own_ml = reinterpret_cast<float2*>(work + w.own_ml), p.own_o = reinterpret_cast<float*>(work + w.own_o);
@@ -1235,10 +1568,7 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   if (int rc = paged_map(&maps[1], a.q, dtype, 3, q_dims, q_strides, box_own)) return rc;
   if (int rc = paged_map(&maps[2], a.k_cache, dtype, 5, c_dims, c_strides, box_k)) return rc;
   if (int rc = paged_map(&maps[3], a.v_cache, dtype, 5, c_dims, c_strides, box_v)) return rc;
-  int dev = 0, sms = 2 * PA_MAX_PAIRS;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int grid = 2 * std::min(sms / 2, PA_MAX_PAIRS);
+  const int grid = 2 * pairs;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   auto run = [&](auto d) {
     constexpr int D = decltype(d)::value;
