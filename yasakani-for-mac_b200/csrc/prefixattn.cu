@@ -80,7 +80,7 @@ constexpr int PA_THIN_WHOLE = 6;     // tiles up to which few thin items are not
 constexpr int PA_THIN_LEAST = 4;     // units of a warp, at least
 constexpr int PA_THIN_WARPS = 12;    // warps of a CTA: each takes thin items by itself
 constexpr int PA_THIN_STAGE = 16384; // bytes on the way to one of them
-constexpr int PA_THIN_PER_TILE = 10; // thin tiles (two CTAs) in the time of a pair's tile of 128
+constexpr int PA_THIN_PER_TILE = 14; // thin tiles (two CTAs) in the time of a pair's tile of 128
 constexpr int PA_MAX_THIN = 2 * PA_MAX_PAIRS * PA_THIN_WARPS;
 constexpr int PA_WHOLE_TILES = 2;  // tiles up to which few items are not cut
 constexpr int PA_ITEM_COST = 3;  // an item's fixed cost (Q, the last P V's wait, its result) in tiles
@@ -147,6 +147,7 @@ struct PrefixAttnParams {
   int64_t q_row, q_head;
   CacheStrides cache;
   bool whole;  // items are not cut: no join
+  int join_span;  // 16-channel parts of a row that a warp of the join takes
   float c;     // |scale| log2 e
   uint32_t negate_q;
   int4* work_per;         // for the join: units per pair of prefix items and of own ones, whether alone
@@ -1322,17 +1323,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
   }
 }
 
-// Joins the segments of each row. A warp takes 8 rows (in the order of the prefix items' rows)
-// of a KV head and 64 channels: lane (r, q) row r, the channels 4 q .. 4 q + 3 of each 16, so that
-// a load of the warp is 4 runs of 128 adjacent bytes and a store 8 runs of 32. What bounds it is
-// the chain of dependent loads (lengths, places, partial results): the maximum runs along, so
-// that all of a segment's loads are independent of the segments before it.
+// Joins the segments of each row. A warp takes 8 rows (in the order of the prefix items' rows) of a
+// KV head and 16 channels: lane (r, q) row r, the channels 4 q .. 4 q + 3, so that a load of the warp
+// is 4 runs of 128 adjacent bytes and a store 8 runs of 32. What bounds it is the chain of
+// dependent loads (lengths, places, partial results), so as many segments as a row has in most
+// calls are asked for at once, and a thread has few channels (16 of them and 4 segments at once: 17 us
+// of the 93 of 64 requests behind 32k rows, COMBCO so).
 template <int D, int DT>
 __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_constant__ PrefixAttnParams p) {
-  constexpr int PARTS = D / 64;
+  const int parts = D / 16 / p.join_span;
   pdl_begin();
   const int lane = threadIdx.x & 31;
-  const int unit = blockIdx.x * 8 + (threadIdx.x >> 5), idx = unit / PARTS * 8 + (lane & 7);
+  const int unit = blockIdx.x * 8 + (threadIdx.x >> 5), idx = unit / parts * 8 + (lane & 7);
   const int kvh = blockIdx.y, t = pa_quotient(idx, p.g_magic), gh = idx - t * p.G;
   if (t >= p.tokens) return;
   const int4 how = *p.work_per;
@@ -1341,23 +1343,17 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
   PaRequest r{-1, 0, 0};
   int2 base{};
   if (t < p.batch) r = pa_request(p, t), base = p.work_base[t];
-  const int ch = (unit % PARTS) * 16 + (lane >> 3);  // of 4 channels; then every 4th
+  int ch = (unit % parts) * p.join_span * 4 + (lane >> 3);  // of 4 channels; then join_span - 1 times the 4th after
   const int h = kvh * p.G + gh;
-  uint4 gate[4];
-  if (p.gate) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) gate[j] = gate_load(p, t * p.gate_row + h * p.gate_head + (ch + 4 * j) * 4);
-  }
   if (r.s0 != t || r.n != 1) {
     i = request_of(p.starts, p.batch, t);
     r = i < p.batch ? pa_request(p, i) : PaRequest{-1, 0, 0};
     if (i < p.batch) base = p.work_base[i];
   }
   const bool alone = how.z;
-  float4 o[4];
-  float den = 0.0f, top = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) o[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  // segments of the row: n_pre of its prefix item, n_own of its own, from their first places on
+  int n_pre = 0, n_own = 0, pre_row = 0, own_row = 0;
+  int64_t pre0 = 0, own0 = 0;
   if ((how.x | how.y) > 0 && t >= r.s0 && t < r.s0 + r.n) {
     // b / per, a pair's number: small, so that one correction makes the quotient in binary32 right
     auto pair_of = [&](int b, int per) {
@@ -1365,9 +1361,6 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
       q -= q * per > b;
       return q + ((q + 1) * per <= b);
     };
-    // segments of the row: n_pre of its prefix item, n_own of its own, from their first places on
-    int n_pre = 0, n_own = 0, pre_row = 0, own_row = 0;
-    int64_t pre0 = 0, own0 = 0;
     const int nq = pa_qtiles(p, r), own_qt = nq > 1 ? pa_quotient(t - r.s0, p.tpi_magic) : 0;
     const int kt = pa_tiles(p, r, own_qt, alone);
     if (kt > 0) {
@@ -1387,50 +1380,51 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
       pre0 = it + c0;
       pre_row = rank * PA_ROWS + (tl - rank * p.tpc) * p.G + gh;
     }
-    constexpr int BATCH = 4;  // segments asked for at once
-    const int n = n_pre + n_own;
+  }
+  constexpr int BATCH = 8;  // segments asked for at once
+  const int n = n_pre + n_own;
+#pragma unroll 1
+  for (int j = 0; j < p.join_span; ++j, ch += 4) {
+    const uint4 gate = p.gate ? gate_load(p, t * p.gate_row + h * p.gate_head + ch * 4) : make_uint4(0, 0, 0, 0);
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float den = 0.0f, top = -INFINITY;
+#pragma unroll 1
     for (int x0 = 0; x0 < n; x0 += BATCH) {
       float2 ml[BATCH];
-      float4 y[BATCH][4];
+      float4 y[BATCH];
+      float now = top;
 #pragma unroll
       for (int u = 0; u < BATCH; ++u) {
-        const int x = min(x0 + u, n - 1);
-        const bool pre = x < n_pre;
-        const int rows = pre ? 2 * PA_ROWS : p.own_rows, row = pre ? pre_row : own_row;
-        const int64_t at = (pre ? pre0 + x : own0 + x - n_pre) * rows;
-        ml[u] = (pre ? p.pre_ml : p.own_ml)[at + row];
-        const float4* src = reinterpret_cast<const float4*>((pre ? p.pre_o : p.own_o) + at * D) + ch * rows + row;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[u][j] = src[4 * j * rows];
-      }
-#pragma unroll
-      for (int u = 0; u < BATCH; ++u) {
-        if (x0 + u >= n) break;
-        const float now = fmaxf(top, ml[u].x);
-        const float w = ml[u].x == -INFINITY ? 0.0f : exp2_approx(ml[u].x - now);
-        const float keep = top == -INFINITY ? 0.0f : exp2_approx(top - now);
-        top = now;
-        den = fmaf(den, keep, ml[u].y * w);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          o[j].x = fmaf(o[j].x, keep, y[u][j].x * w);
-          o[j].y = fmaf(o[j].y, keep, y[u][j].y * w);
-          o[j].z = fmaf(o[j].z, keep, y[u][j].z * w);
-          o[j].w = fmaf(o[j].w, keep, y[u][j].w * w);
+        ml[u] = make_float2(-INFINITY, 0.0f), y[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const int x = x0 + u;
+        if (x < n) {
+          const bool pre = x < n_pre;
+          const int rows = pre ? 2 * PA_ROWS : p.own_rows, row = pre ? pre_row : own_row;
+          const int64_t at = (pre ? pre0 + x : own0 + x - n_pre) * rows;
+          ml[u] = (pre ? p.pre_ml : p.own_ml)[at + row];
+          y[u] = reinterpret_cast<const float4*>((pre ? p.pre_o : p.own_o) + at * D)[ch * rows + row];
         }
       }
-    }
-  }
-  const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-  uint16_t* out = p.out + ((int64_t)t * p.n_kvh * p.G + h) * D;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float v[4] = {o[j].x * inv, o[j].y * inv, o[j].z * inv, o[j].w * inv};
+      for (int u = 0; u < BATCH; ++u) now = fmaxf(now, ml[u].x);
+      const float keep = top == -INFINITY ? 0.0f : exp2_approx(top - now);
+      top = now;
+      den *= keep, o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const float w = ml[u].x == -INFINITY ? 0.0f : exp2_approx(ml[u].x - now);
+        den = fmaf(ml[u].y, w, den);
+        o.x = fmaf(y[u].x, w, o.x), o.y = fmaf(y[u].y, w, o.y);
+        o.z = fmaf(y[u].z, w, o.z), o.w = fmaf(y[u].w, w, o.w);
+      }
+    }
+    const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+    float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
     if (p.gate) {
-      const float4 g = gate_value<DT>(p, gate[j]);
+      const float4 g = gate_value<DT>(p, gate);
       v[0] = gated(v[0], g.x), v[1] = gated(v[1], g.y), v[2] = gated(v[2], g.z), v[3] = gated(v[3], g.w);
     }
-    *reinterpret_cast<uint2*>(out + (ch + 4 * j) * 4) =
+    *reinterpret_cast<uint2*>(p.out + ((int64_t)t * p.n_kvh * p.G + h) * D + ch * 4) =
         make_uint2(Elem<DT>::pack(v[0], v[1]), Elem<DT>::pack(v[2], v[3]));
   }
 }
@@ -1444,7 +1438,7 @@ static int launch_prefix_attention(const CUtensorMap (&maps)[4], const PrefixAtt
                                  maps[1], maps[2], maps[3], p))
     return cuda_fail(e, "prefix_attention_kernel");
   if (p.whole) return YSKN_OK;
-  const int64_t warps = ceil_div((int64_t)p.tokens * p.G, 8) * (D / 64);
+  const int64_t warps = ceil_div((int64_t)p.tokens * p.G, 8) * (D / 16 / p.join_span);
   return cuda_fail(launch_pdl(prefix_combine_kernel<D, DT>, dim3((unsigned)ceil_div(warps, 8), p.n_kvh), 256, 0, st, p),
                    "prefix_combine_kernel");
 }
@@ -1542,6 +1536,12 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   const int64_t most_tiles = p.own_pre + ceil_div(p.own_limit, 1 << p.tile_shift);
   p.whole = w.own_items <= (p.thin ? 2 * PA_THIN_WARPS : 1) * pairs && most_tiles <= (p.thin ? PA_THIN_WHOLE : PA_WHOLE_TILES);
   p.many_per_head = PA_MANY / (unsigned)n_kvh;
+  // A warp of the join takes 16 channels of 8 rows; or more, where there are twice the warps that the
+  // SMs hold: then few rows are left to join, or enough of them in every SM (16 prompt chunks: 945 us
+  // with 16 channels, SPANCO with all).
+  const int64_t join_rows = ceil_div((int64_t)a.tokens * G, 8) * n_kvh;
+  p.join_span = 1;
+  while (p.join_span < head / 16 && join_rows * (head / 16 / p.join_span) > 2 * 148 * 24) p.join_span *= 2;
   // a scale of zero keeps its meaning (equal weights) with a factor that leaves -inf alone
   p.c = std::max(std::fabs(a.scale) * 1.4426950408889634f, 1e-30f);
   p.negate_q = a.scale < 0.0f;
