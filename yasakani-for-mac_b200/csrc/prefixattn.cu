@@ -147,7 +147,7 @@ struct PrefixAttnParams {
   int64_t q_row, q_head;
   CacheStrides cache;
   bool whole;  // items are not cut: no join
-  int join_span;  // 16-channel parts of a row that a warp of the join takes
+  int join_span, join_split;  // 16-channel parts of a row that a warp of the join takes; warps for one part
   float c;     // |scale| log2 e
   uint32_t negate_q;
   int4* work_per;         // for the join: units per pair of prefix items and of own ones, whether alone
@@ -1331,21 +1331,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
 // of the 93 of 64 requests behind 32k rows, COMBCO so).
 template <int D, int DT>
 __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_constant__ PrefixAttnParams p) {
-  const int parts = D / 16 / p.join_span;
+  __shared__ float joined[8][6][32];
+  const int parts = D / 16 / p.join_span, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int split = p.join_split, part = warp & (split - 1);
+  const int unit = (blockIdx.x * 8 + warp) / split, idx = unit / parts * 8 + (lane & 7);
+  const int kvh = blockIdx.y, t = pa_quotient(idx, p.g_magic), gh = idx - t * p.G, h = kvh * p.G + gh;
+  int ch = (unit % parts) * p.join_span * 4 + (lane >> 3);  // of 4 channels; then every 4th, join_span in all
+  bool live = t < p.tokens;
   pdl_begin();
-  const int lane = threadIdx.x & 31;
-  const int unit = blockIdx.x * 8 + (threadIdx.x >> 5), idx = unit / parts * 8 + (lane & 7);
-  const int kvh = blockIdx.y, t = pa_quotient(idx, p.g_magic), gh = idx - t * p.G;
-  if (t >= p.tokens) return;
   const int4 how = *p.work_per;
   // one token for each request is the common case: its request's numbers are asked for at once
   int i = t;
   PaRequest r{-1, 0, 0};
   int2 base{};
   if (t < p.batch) r = pa_request(p, t), base = p.work_base[t];
-  int ch = (unit % parts) * p.join_span * 4 + (lane >> 3);  // of 4 channels; then join_span - 1 times the 4th after
-  const int h = kvh * p.G + gh;
-  if (r.s0 != t || r.n != 1) {
+  if (live && (r.s0 != t || r.n != 1)) {
     i = request_of(p.starts, p.batch, t);
     r = i < p.batch ? pa_request(p, i) : PaRequest{-1, 0, 0};
     if (i < p.batch) base = p.work_base[i];
@@ -1354,7 +1354,7 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
   // segments of the row: n_pre of its prefix item, n_own of its own, from their first places on
   int n_pre = 0, n_own = 0, pre_row = 0, own_row = 0;
   int64_t pre0 = 0, own0 = 0;
-  if ((how.x | how.y) > 0 && t >= r.s0 && t < r.s0 + r.n) {
+  if (live && (how.x | how.y) > 0 && t >= r.s0 && t < r.s0 + r.n) {
     // b / per, a pair's number: small, so that one correction makes the quotient in binary32 right
     auto pair_of = [&](int b, int per) {
       int q = (int)((float)b * (1.0f / (float)per));
@@ -1372,7 +1372,7 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
       own0 = base.x + kvh * nq + own_qt + c0;
       own_row = rank * p.own_half + (tl - rank * p.tpc) * p.G + gh;
     }
-    if (n_own == 1 && (alone || p.pre_tiles == 0)) return;  // finished where it was computed
+    if (n_own == 1 && (alone || p.pre_tiles == 0)) live = false;  // finished where it was computed
     if (!alone && p.pre_tiles > 0) {
       const int qt = pa_quotient(t, p.tpi_magic), it = kvh * p.pre_qtiles + qt, tl = t - qt * p.tpi, rank = tl >= p.tpc;
       const int b = it * pa_units(p.pre_tiles, false, PA_ITEM_COST) + PA_ITEM_COST, c0 = pair_of(b, how.x);
@@ -1383,21 +1383,23 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
   }
   constexpr int BATCH = 8;  // segments asked for at once
   const int n = n_pre + n_own;
+  if (split == 1 && !live) return;
 #pragma unroll 1
   for (int j = 0; j < p.join_span; ++j, ch += 4) {
-    const uint4 gate = p.gate ? gate_load(p, t * p.gate_row + h * p.gate_head + ch * 4) : make_uint4(0, 0, 0, 0);
+    uint4 gate = make_uint4(0, 0, 0, 0);
+    if (p.gate && live) gate = gate_load(p, t * p.gate_row + h * p.gate_head + ch * 4);
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float den = 0.0f, top = -INFINITY;
 #pragma unroll 1
-    for (int x0 = 0; x0 < n; x0 += BATCH) {
+    for (int x0 = part; x0 < n; x0 += BATCH * split) {
       float2 ml[BATCH];
       float4 y[BATCH];
       float now = top;
 #pragma unroll
       for (int u = 0; u < BATCH; ++u) {
         ml[u] = make_float2(-INFINITY, 0.0f), y[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const int x = x0 + u;
-        if (x < n) {
+        const int x = x0 + u * split;
+        if (x < n && live) {
           const bool pre = x < n_pre;
           const int rows = pre ? 2 * PA_ROWS : p.own_rows, row = pre ? pre_row : own_row;
           const int64_t at = (pre ? pre0 + x : own0 + x - n_pre) * rows;
@@ -1416,6 +1418,23 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
         den = fmaf(ml[u].y, w, den);
         o.x = fmaf(y[u].x, w, o.x), o.y = fmaf(y[u].y, w, o.y);
         o.z = fmaf(y[u].z, w, o.z), o.w = fmaf(y[u].w, w, o.w);
+      }
+    }
+    if (split > 1) {  // the parts of the row's segments, in order
+      float(&mine)[6][32] = joined[warp];
+      mine[0][lane] = top, mine[1][lane] = den;
+      mine[2][lane] = o.x, mine[3][lane] = o.y, mine[4][lane] = o.z, mine[5][lane] = o.w;
+      __syncthreads();
+      if (part > 0 || !live) return;
+      for (int x = 1; x < split; ++x) {
+        const float(&other)[6][32] = joined[warp + x];
+        const float most = other[0][lane], now = fmaxf(top, most);
+        const float keep = top == -INFINITY ? 0.0f : exp2_approx(top - now);
+        const float w = most == -INFINITY ? 0.0f : exp2_approx(most - now);
+        top = now;
+        den = den * keep + other[1][lane] * w;
+        o.x = o.x * keep + other[2][lane] * w, o.y = o.y * keep + other[3][lane] * w;
+        o.z = o.z * keep + other[4][lane] * w, o.w = o.w * keep + other[5][lane] * w;
       }
     }
     const float inv = den == 0.0f ? 0.0f : 1.0f / den;
@@ -1438,7 +1457,7 @@ static int launch_prefix_attention(const CUtensorMap (&maps)[4], const PrefixAtt
                                  maps[1], maps[2], maps[3], p))
     return cuda_fail(e, "prefix_attention_kernel");
   if (p.whole) return YSKN_OK;
-  const int64_t warps = ceil_div((int64_t)p.tokens * p.G, 8) * (D / 16 / p.join_span);
+  const int64_t warps = ceil_div((int64_t)p.tokens * p.G, 8) * (D / 16 / p.join_span) * p.join_split;
   return cuda_fail(launch_pdl(prefix_combine_kernel<D, DT>, dim3((unsigned)ceil_div(warps, 8), p.n_kvh), 256, 0, st, p),
                    "prefix_combine_kernel");
 }
@@ -1542,6 +1561,9 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   const int64_t join_rows = ceil_div((int64_t)a.tokens * G, 8) * n_kvh;
   p.join_span = 1;
   while (p.join_span < head / 16 && join_rows * (head / 16 / p.join_span) > 2 * 148 * 24) p.join_span *= 2;
+  // Few: several warps share a row's segments (SPLITCO).
+  p.join_split = 1;
+  while (p.join_split < 8 && join_rows * (head / 16) * 2 * p.join_split <= 148 * 24) p.join_split *= 2;
   // a scale of zero keeps its meaning (equal weights) with a factor that leaves -inf alone
   p.c = std::max(std::fabs(a.scale) * 1.4426950408889634f, 1e-30f);
   p.negate_q = a.scale < 0.0f;
