@@ -1352,8 +1352,10 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
   }
   const bool alone = how.z;
   // segments of the row: n_pre of its prefix item, n_own of its own, from their first places on
-  int n_pre = 0, n_own = 0, pre_row = 0, own_row = 0;
-  int64_t pre0 = 0, own0 = 0;
+  int n_pre = 0, n_own = 0;
+  const float4 *pre_o = nullptr, *own_o = nullptr;
+  const float2 *pre_ml = nullptr, *own_ml = nullptr;
+  const int pre_step = 2 * PA_ROWS, own_step = p.own_rows;  // rows from one place to the next
   if (live && (how.x | how.y) > 0 && t >= r.s0 && t < r.s0 + r.n) {
     // b / per, a pair's number: small, so that one correction makes the quotient in binary32 right
     auto pair_of = [&](int b, int per) {
@@ -1369,23 +1371,29 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
       for (int q = 0; q < own_qt; ++q) b += pa_units(pa_tiles(p, r, q, alone), false, p.item_cost);
       const int c0 = pair_of(b, how.y), tl = t - r.s0 - own_qt * p.tpi, rank = tl >= p.tpc;
       n_own = pair_of(b + kt - 1, how.y) - c0 + 1;
-      own0 = base.x + kvh * nq + own_qt + c0;
-      own_row = rank * p.own_half + (tl - rank * p.tpc) * p.G + gh;
+      const int64_t place = base.x + kvh * nq + own_qt + c0;
+      const int row = rank * p.own_half + (tl - rank * p.tpc) * p.G + gh;
+      own_ml = p.own_ml + place * own_step + row;
+      own_o = reinterpret_cast<const float4*>(p.own_o) + place * own_step * (D / 4) + ch * own_step + row;
     }
     if (n_own == 1 && (alone || p.pre_tiles == 0)) live = false;  // finished where it was computed
     if (!alone && p.pre_tiles > 0) {
       const int qt = pa_quotient(t, p.tpi_magic), it = kvh * p.pre_qtiles + qt, tl = t - qt * p.tpi, rank = tl >= p.tpc;
       const int b = it * pa_units(p.pre_tiles, false, PA_ITEM_COST) + PA_ITEM_COST, c0 = pair_of(b, how.x);
       n_pre = pair_of(b + p.pre_tiles - 1, how.x) - c0 + 1;
-      pre0 = it + c0;
-      pre_row = rank * PA_ROWS + (tl - rank * p.tpc) * p.G + gh;
+      const int64_t place = it + c0;
+      const int row = rank * PA_ROWS + (tl - rank * p.tpc) * p.G + gh;
+      pre_ml = p.pre_ml + place * pre_step + row;
+      pre_o = reinterpret_cast<const float4*>(p.pre_o) + place * pre_step * (D / 4) + ch * pre_step + row;
     }
   }
   constexpr int BATCH = 8;  // segments asked for at once
-  const int n = n_pre + n_own;
+  const int n = live ? n_pre + n_own : 0;
+  // segment x of the own ones is the row's n_pre + x
+  own_ml -= (int64_t)n_pre * own_step, own_o -= (int64_t)n_pre * own_step * (D / 4);
   if (split == 1 && !live) return;
 #pragma unroll 1
-  for (int j = 0; j < p.join_span; ++j, ch += 4) {
+  for (int j = 0; j < p.join_span; ++j, ch += 4, pre_o += 4 * pre_step, own_o += 4 * own_step) {
     uint4 gate = make_uint4(0, 0, 0, 0);
     if (p.gate && live) gate = gate_load(p, t * p.gate_row + h * p.gate_head + ch * 4);
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1399,12 +1407,11 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
       for (int u = 0; u < BATCH; ++u) {
         ml[u] = make_float2(-INFINITY, 0.0f), y[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         const int x = x0 + u * split;
-        if (x < n && live) {
+        if (x < n) {
           const bool pre = x < n_pre;
-          const int rows = pre ? 2 * PA_ROWS : p.own_rows, row = pre ? pre_row : own_row;
-          const int64_t at = (pre ? pre0 + x : own0 + x - n_pre) * rows;
-          ml[u] = (pre ? p.pre_ml : p.own_ml)[at + row];
-          y[u] = reinterpret_cast<const float4*>((pre ? p.pre_o : p.own_o) + at * D)[ch * rows + row];
+          const int64_t at = (int64_t)x * (pre ? pre_step : own_step);
+          ml[u] = (pre ? pre_ml : own_ml)[at];
+          y[u] = (pre ? pre_o : own_o)[at * (D / 4)];
         }
       }
 #pragma unroll
