@@ -111,7 +111,8 @@ inline PaWork pa_work(int tokens, int batch, int max_new, int n_qh, int n_kvh, i
   const int64_t pre_items = ceil_div(tokens, tpi) * n_kvh;
   // sum of ceil(n_i / tpi) over requests with n_i > 0: at most one more than n_i / tpi each
   const int64_t own_items = (std::min(batch, tokens) + (int64_t)tokens / tpi) * n_kvh;
-  const int64_t pre = pre_items + PA_MAX_PAIRS, own = own_items + (G * max_new <= PA_THIN_ROWS ? PA_MAX_THIN : PA_MAX_PAIRS);
+  const int64_t pre = pre_items + PA_MAX_PAIRS;
+  const int64_t own = own_items + (G * max_new <= PA_THIN_ROWS ? PA_MAX_THIN : PA_MAX_PAIRS);
   PaWork w{};
   w.own_half = G * std::min(tpc, max_new);
   w.own_rows = max_new > tpc ? 2 * w.own_half : w.own_half;
@@ -259,8 +260,8 @@ struct PaWalk {
   int nq;
   bool loaded;
   __device__ PaWalk(const PrefixAttnParams& p_, const PaStart& s)
-      : p(p_), alone(s.alone), who(s.who), left(s.left), pre_item(s.pre_item), u0(s.u0), req(s.req), item(s.item), kvh(0), qt(0),
-        r{}, nq(0), loaded(false) {
+      : p(p_), alone(s.alone), who(s.who), left(s.left), pre_item(s.pre_item), u0(s.u0), req(s.req), item(s.item),
+        kvh(0), qt(0), r{}, nq(0), loaded(false) {
     if (s.skip > 0) {
       load();
       const int head = (int)pa_own_units(p, r, nq, alone);
@@ -496,11 +497,15 @@ template <int DT>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   if constexpr (DT == YSKN_DT_BF16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+        "%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+        "%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -510,7 +515,10 @@ __device__ __forceinline__ void copy16(uint32_t to, const uint16_t* from, bool v
 }
 __device__ __forceinline__ uint4 stage_load(uint32_t at) {
   uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(at)
+               : "memory");
   return v;
 }
 
@@ -567,7 +575,8 @@ struct ThinCursor {
 };
 
 template <int D, int DT>
-__device__ __forceinline__ void thin_items(const PrefixAttnParams& p, const PaStart& start, uint8_t* smem, int warp, int lane) {
+__device__ __forceinline__ void thin_items(const PrefixAttnParams& p, const PaStart& start, uint8_t* smem, int warp,
+                                           int lane) {
   constexpr int C = D / 64, CHUNKS = 2 * C;  // chunks of a slice's K; of K and V
   constexpr int LEAD = 8 / CHUNKS;           // slices on the way
   static_assert(PaShape<D>::Q_BYTES + PaShape<D>::RING * PA_SLOT >=
@@ -919,398 +928,399 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
     if (p.whole && warp == PA_THIN_WARPS - 1) zero_unheld<D>(p, lane);
     thin_items<D, DT>(p, sh.start[warp], smem, warp, lane);
   } else {
-  PaWalk walk(p, sh.start[0]);
-  PaSegment seg;
-  if (warp == 0) {
-    // ---- K and V through the ring, in the order in which the MMAs use them: this CTA's half of
-    // each tile's K rows, and of V's channels
-    int s = 0;          // the ring's place
-    uint32_t turn = 1;  // parity of a place's last reading (first round: already free)
-    uint32_t tails = 0;
-    bool ok = true;
-    const int shift = p.block_shift, pages = PA_KEYS >> shift;
-    const int box_k = min(1 << shift, PA_KEYS / 2), box_v = min(1 << shift, VR);
-    const uint32_t full0 = first_cta(&sh.full[0]);
-    const int v_chunk = D == 64 ? 0 : rank * Shape::V_CHUNKS, v_x = D == 64 ? rank * 32 : 0;
-    while (ok && walk.next(seg)) {
-      auto block_of = [&](int kt) {  // lane l: the block of page l of tile kt
-        int b = 0;
-        if (kt < seg.key1 && lane < pages && (lane << shift) < seg.rows_of(p, kt)) {
-          b = __ldg(kt < seg.pre ? p.prefix_blocks + kt * pages + lane
-                                 : p.tables + (int64_t)seg.req * p.table_stride + (kt - seg.pre) * pages + lane);
-          if ((unsigned)b >= (unsigned)p.n_blocks) raise_device_error(p.err, DERR_RANGE);  // the copy gives zeros
-        }
-        return b;
-      };
-      // The next place of the ring, once both CTAs' part of it has been read.
-      auto claim = [&]() {
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[s], turn, abort_flag));
-        return ring + s * PA_SLOT;
-      };
-      auto advance = [&]() {
-        if (++s == RING) s = 0, turn ^= 1;
-      };
-      // Rows key0 .. key0 + n * box - 1 of the tile, `chunks` columns from `chunk` on, as
-      // [column][ROWS rows][line] at `to`: one box, or one per block and column.
-      auto copy = [&](uint8_t* to, const CUtensorMap* map, uint32_t bar, int key0, int n, int box, int rows, int x,
-                      int chunk, int chunks, int line, int block) {
-        const int key = key0 + lane * box;
-        const int b = __shfl_sync(0xffffffffu, block, (key >> shift) & 31);
-        if (lane < n) {
-          const int y = key & ((1 << shift) - 1);
-          if (box == rows) pair_load_5d(to, map, bar, x, y, chunk, seg.kvh, b);
-          else
-            for (int d = 0; d < chunks; ++d)
-              pair_load_5d(to + (d * rows + lane * box) * line, map, bar, x, y, chunk + d, seg.kvh, b);
-        }
-      };
-      auto put_k = [&](int kt, int block) {
-        const int nk = min(max(seg.rows_of(p, kt) - rank * (PA_KEYS / 2), 0), PA_KEYS / 2);
-        const int n = (nk + box_k - 1) / box_k;
-        for (int d = 0; ok && d < SLOTS; ++d) {
-          uint8_t* to = claim();
-          if (!ok) break;
-          const uint32_t bar = full0 + 8 * s;
-          if (lane == 0) expect_first(bar, (uint32_t)(n * box_k * 128 * Shape::K_CHUNKS));
-          __syncwarp();
-          copy(to, &map_k, bar, rank * (PA_KEYS / 2), n, box_k, PA_KEYS / 2, 0, d * Shape::K_CHUNKS, Shape::K_CHUNKS,
-               128, block);
-          advance();
-        }
-      };
-      auto put_v = [&](int kt, int block) {
-        const int nk = seg.rows_of(p, kt);
-        for (int v = 0; ok && v * VR < nk; ++v) {
-          const int rows = min(VR, nk - v * VR), n = (rows + box_v - 1) / box_v;
-          uint8_t* to = claim();
-          if (!ok) break;
-          uint32_t bar = full0 + 8 * s;
-          const uint32_t bytes = (uint32_t)(n * box_v) * Shape::V_LINE * Shape::V_CHUNKS;
-          if (rows & 15) {  // lands on this CTA's barrier; warp 3 clears the end and then arrives
-            if (tails > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.tail_done, (tails - 1) & 1, abort_flag));
+    PaWalk walk(p, sh.start[0]);
+    PaSegment seg;
+
+    if (warp == 0) {
+      // ---- K and V through the ring, in the order in which the MMAs use them: this CTA's half of
+      // each tile's K rows, and of V's channels
+      int s = 0;          // the ring's place
+      uint32_t turn = 1;  // parity of a place's last reading (first round: already free)
+      uint32_t tails = 0;
+      bool ok = true;
+      const int shift = p.block_shift, pages = PA_KEYS >> shift;
+      const int box_k = min(1 << shift, PA_KEYS / 2), box_v = min(1 << shift, VR);
+      const uint32_t full0 = first_cta(&sh.full[0]);
+      const int v_chunk = D == 64 ? 0 : rank * Shape::V_CHUNKS, v_x = D == 64 ? rank * 32 : 0;
+      while (ok && walk.next(seg)) {
+        auto block_of = [&](int kt) {  // lane l: the block of page l of tile kt
+          int b = 0;
+          if (kt < seg.key1 && lane < pages && (lane << shift) < seg.rows_of(p, kt)) {
+            b = __ldg(kt < seg.pre ? p.prefix_blocks + kt * pages + lane
+                                   : p.tables + (int64_t)seg.req * p.table_stride + (kt - seg.pre) * pages + lane);
+            if ((unsigned)b >= (unsigned)p.n_blocks) raise_device_error(p.err, DERR_RANGE);  // the copy gives zeros
+          }
+          return b;
+        };
+        // The next place of the ring, once both CTAs' part of it has been read.
+        auto claim = [&]() {
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.empty[s], turn, abort_flag));
+          return ring + s * PA_SLOT;
+        };
+        auto advance = [&]() {
+          if (++s == RING) s = 0, turn ^= 1;
+        };
+        // Rows key0 .. key0 + n * box - 1 of the tile, `chunks` columns from `chunk` on, as
+        // [column][ROWS rows][line] at `to`: one box, or one per block and column.
+        auto copy = [&](uint8_t* to, const CUtensorMap* map, uint32_t bar, int key0, int n, int box, int rows, int x,
+                        int chunk, int chunks, int line, int block) {
+          const int key = key0 + lane * box;
+          const int b = __shfl_sync(0xffffffffu, block, (key >> shift) & 31);
+          if (lane < n) {
+            const int y = key & ((1 << shift) - 1);
+            if (box == rows) pair_load_5d(to, map, bar, x, y, chunk, seg.kvh, b);
+            else
+              for (int d = 0; d < chunks; ++d)
+                pair_load_5d(to + (d * rows + lane * box) * line, map, bar, x, y, chunk + d, seg.kvh, b);
+          }
+        };
+        auto put_k = [&](int kt, int block) {
+          const int nk = min(max(seg.rows_of(p, kt) - rank * (PA_KEYS / 2), 0), PA_KEYS / 2);
+          const int n = (nk + box_k - 1) / box_k;
+          for (int d = 0; ok && d < SLOTS; ++d) {
+            uint8_t* to = claim();
             if (!ok) break;
-            ++tails;
-            if (lane == 0) {
-              sh.tail_at = make_int2(s, rows);
-              mbar_expect_tx(&sh.tail_full, bytes);
+            const uint32_t bar = full0 + 8 * s;
+            if (lane == 0) expect_first(bar, (uint32_t)(n * box_k * 128 * Shape::K_CHUNKS));
+            __syncwarp();
+            copy(to, &map_k, bar, rank * (PA_KEYS / 2), n, box_k, PA_KEYS / 2, 0, d * Shape::K_CHUNKS, Shape::K_CHUNKS,
+                 128, block);
+            advance();
+          }
+        };
+        auto put_v = [&](int kt, int block) {
+          const int nk = seg.rows_of(p, kt);
+          for (int v = 0; ok && v * VR < nk; ++v) {
+            const int rows = min(VR, nk - v * VR), n = (rows + box_v - 1) / box_v;
+            uint8_t* to = claim();
+            if (!ok) break;
+            uint32_t bar = full0 + 8 * s;
+            const uint32_t bytes = (uint32_t)(n * box_v) * Shape::V_LINE * Shape::V_CHUNKS;
+            if (rows & 15) {  // lands on this CTA's barrier; warp 3 clears the end and then arrives
+              if (tails > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.tail_done, (tails - 1) & 1, abort_flag));
+              if (!ok) break;
+              ++tails;
+              if (lane == 0) {
+                sh.tail_at = make_int2(s, rows);
+                mbar_expect_tx(&sh.tail_full, bytes);
+              }
+              bar = smem_u32(&sh.tail_full);  // of this CTA, as a cluster address
+              asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&sh.tail_full)), "r"(rank));
+            } else if (lane == 0) {
+              expect_first(bar, bytes);
             }
-            bar = smem_u32(&sh.tail_full);  // of this CTA, as a cluster address
-            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&sh.tail_full)), "r"(rank));
-          } else if (lane == 0) {
-            expect_first(bar, bytes);
+            __syncwarp();
+            copy(to, &map_v, bar, v * VR, n, box_v, VR, v_x, v_chunk, Shape::V_CHUNKS, Shape::V_LINE, block);
+            advance();
           }
-          __syncwarp();
-          copy(to, &map_v, bar, v * VR, n, box_v, VR, v_x, v_chunk, Shape::V_CHUNKS, Shape::V_LINE, block);
-          advance();
-        }
-      };
-      int cur = block_of(seg.key0), nxt = block_of(seg.key0 + 1);
-      put_k(seg.key0, cur);
-      for (int kt = seg.key0; ok && kt < seg.key1; ++kt) {
-        const int after = block_of(kt + 2);
-        if (kt + 1 < seg.key1) put_k(kt + 1, nxt);
-        if (ok) put_v(kt, cur);
-        cur = nxt;
-        nxt = after;
-      }
-    }
-    if (ok && tails > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.tail_done, (tails - 1) & 1, abort_flag));
-    if (ok && lane == 0) {
-      sh.tail_at = make_int2(0, 0);  // no more of them
-      mbar_arrive(&sh.tail_full);
-    }
-    if (!ok) {  // a copy lands within microseconds: let those that this warp started do so
-      const long long t0 = clock64();
-      while (clock64() - t0 < TC_WAIT_LIMIT / 1000) {
-      }
-    }
-  } else if (warp == 1) {
-    // ---- MMAs: one thread of the first CTA
-    if (rank == 0 && elect_one()) {
-      const uint32_t id_qk = pa_idesc(DT, PA_KEYS, 0, p.negate_q), id_pv = pa_idesc(DT, D, 1, 0);
-      int s = 0, g = 0, n_seg = 0;  // ring place, tiles issued, segments
-      uint32_t turn = 0;
-      bool ok = true;
-      // descriptors: Q, and K or V at the ring's first place; the high words hold no address
-      const uint32_t a_lo = (uint32_t)sw128_desc(smem_u32(sQ)), b_lo = (uint32_t)sw128_desc(smem_u32(ring));
-      const uint32_t k_hi = (uint32_t)(sw128_desc(0) >> 32), v_hi = (uint32_t)(mn_desc<Shape::V_LINE>(0, 0) >> 32);
-      const uint32_t v_lo = (uint32_t)mn_desc<Shape::V_LINE>(smem_u32(ring), VR * Shape::V_LINE);
-      auto advance = [&]() {
-        umma2_commit(&sh.empty[s]);
-        if (++s == RING) s = 0, turn ^= 1;
-      };
-      auto qk = [&](int tile) {  // S of the pair's tile number `tile`
-        const uint32_t d = tmem + Shape::S_COL + (tile & 1) * PA_KEYS;
-#pragma unroll
-        for (int v = 0; v < SLOTS; ++v) {
-          ok = ok && mbar_wait(&sh.full[s], turn, abort_flag);
-          if (!ok) return;
-          tc_fence_after();
-#pragma unroll
-          for (int ch = 0; ch < Shape::K_CHUNKS; ++ch) {
-            const uint32_t a = a_lo + (v * Shape::K_CHUNKS + ch) * (PA_ROWS * 128 >> 4);
-            const uint32_t b = b_lo + s * (PA_SLOT >> 4) + ch * (PA_KEYS / 2 * 128 >> 4);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) umma2_ss(d, a + 2 * k, b + 2 * k, k_hi, id_qk, v > 0 || ch > 0 || k > 0);
-          }
-          advance();
-        }
-        umma2_commit(&sh.s_full[tile & 1]);
-      };
-      auto pv = [&](int nk, uint32_t pt, bool first) {
-#pragma unroll
-        for (int v = 0; v < SLOTS; ++v) {
-          const int rows = nk - v * VR;
-          if (rows <= 0) break;
-          ok = ok && mbar_wait(&sh.full[s], turn, abort_flag);
-          if (!ok) return;
-          tc_fence_after();
-          const uint32_t b = v_lo + s * (PA_SLOT >> 4);
-#pragma unroll
-          for (int k = 0; k < VR / 16; ++k)
-            if (k * 16 < rows)
-              umma2_ts(tmem, pt + (v * VR + k * 16) / 2, b + (16 * Shape::V_LINE >> 4) * k, v_hi, id_pv,
-                       !first || v > 0 || k > 0);
-          advance();
-        }
-      };
-      for (; ok && walk.next(seg); ++n_seg) {
-        ok = mbar_wait(&sh.q_full, n_seg & 1, abort_flag);
-        const int n = seg.key1 - seg.key0;
-        if (ok) qk(g);
-        for (int j = 0; ok && j < n; ++j, ++g) {
-          if (j + 1 < n) qk(g + 1);
-          if (ok && j == max(0, n - 2)) umma2_commit(&sh.q_empty);  // after the segment's last S
-          if (j == 0 && n_seg > 0) ok = ok && mbar_wait(&sh.o_free, (n_seg - 1) & 1, abort_flag);
-          ok = ok && mbar_wait(&sh.p_full[g & 1], (g >> 1) & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          const int nk = seg.rows_of(p, seg.key0 + j);
-          pv(nk, tmem + Shape::S_COL + (g & 1) * PA_KEYS, j == 0);
-          if (ok) umma2_commit(&sh.pv_done[g & 1]);
+        };
+        int cur = block_of(seg.key0), nxt = block_of(seg.key0 + 1);
+        put_k(seg.key0, cur);
+        for (int kt = seg.key0; ok && kt < seg.key1; ++kt) {
+          const int after = block_of(kt + 2);
+          if (kt + 1 < seg.key1) put_k(kt + 1, nxt);
+          if (ok) put_v(kt, cur);
+          cur = nxt;
+          nxt = after;
         }
       }
-      // every MMA of the pair has completed before its TMEM is freed
-      umma2_commit(&sh.drained);
-      const long long t0 = clock64();
-      while (!mbar_try_wait(&sh.drained, 0) && clock64() - t0 < TC_WAIT_LIMIT) {
+      if (ok && tails > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.tail_done, (tails - 1) & 1, abort_flag));
+      if (ok && lane == 0) {
+        sh.tail_at = make_int2(0, 0);  // no more of them
+        mbar_arrive(&sh.tail_full);
       }
-    }
-  } else if (warp == 2) {
-    // ---- Q: this CTA's tokens of each item
-    if (lane == 0) {
-      const uint32_t bar = first_cta(&sh.q_full);
-      int n_seg = 0;
-      bool ok = true;
-      for (; walk.next(seg); ++n_seg) {
-        if (n_seg > 0 && !(ok = mbar_wait(&sh.q_empty, (n_seg - 1) & 1, abort_flag))) break;
-        const int box = seg.prefix ? p.tpc : min(p.tpc, p.max_new);
-        const bool any = seg.ntok > rank * p.tpc;
-        expect_first(bar, any ? (uint32_t)(box * p.G * 128 * Shape::CHUNKS) : 0u);
-        if (any)
-          for (int d = 0; d < Shape::CHUNKS; ++d)
-            pair_load_3d(sQ + d * PA_ROWS * 128, seg.prefix ? &map_q_pre : &map_q_own, bar, d * 64, seg.kvh * p.G,
-                         seg.tok0 + rank * p.tpc);
-      }
-      if (!ok) {
+      if (!ok) {  // a copy lands within microseconds: let those that this warp started do so
         const long long t0 = clock64();
         while (clock64() - t0 < TC_WAIT_LIMIT / 1000) {
         }
       }
-    }
-  } else if (warp == 3) {
-    if (p.whole) zero_unheld<D>(p, lane);
-    // ---- V rows past the last visible one, up to the end of the 16-row step, to zero, in the
-    // slots that warp 0 names: once for each segment that ends inside a step
-    const uint32_t full0 = first_cta(&sh.full[0]);
-    for (uint32_t n = 0;; ++n) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&sh.tail_full, n & 1, abort_flag))) break;
-      const int2 t = sh.tail_at;  // ring place, rows to keep
-      if (t.y == 0) break;
-      constexpr int UNITS = Shape::V_LINE / 16;  // 16-byte units of a row
-      const int units = (16 - (t.y & 15)) * UNITS;
-      uint8_t* base = ring + t.x * PA_SLOT + t.y * Shape::V_LINE;
-      for (int x = lane; x < units * Shape::V_CHUNKS; x += 32) {
-        const int ch = x / units, y = x - ch * units;
-        *reinterpret_cast<uint4*>(base + ch * VR * Shape::V_LINE + y * 16) = make_uint4(0, 0, 0, 0);
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) {
-        release_first(full0 + 8 * t.x);
-        mbar_arrive(&sh.tail_done);
-      }
-    }
-  } else {
-    // ---- softmax, a row's column halves in two threads, then the segment's result
-    const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const uint32_t p_full0 = first_cta(&sh.p_full[0]), o_free0 = first_cta(&sh.o_free);
-    const float c = p.c;
-    int g = 0;
-    while (walk.next(seg)) {
-      const int row_tok = pa_quotient(row, p.g_magic), tl = rank * p.tpc + row_tok;  // token of the item
-      const bool valid = row_tok < p.tpc && tl < seg.ntok;
-      int lim = 0;  // rows of the sequence that the row sees
-      if (valid) {
-        if (seg.prefix) {
-          const int i = request_of(p.starts, p.batch, seg.tok0 + tl);
-          if (i < p.batch) {
-            const PaRequest r = pa_request(p, i);
-            lim = max(r.len - r.n + (seg.tok0 + tl - r.s0) + 1, 0);
+    } else if (warp == 1) {
+      // ---- MMAs: one thread of the first CTA
+      if (rank == 0 && elect_one()) {
+        const uint32_t id_qk = pa_idesc(DT, PA_KEYS, 0, p.negate_q), id_pv = pa_idesc(DT, D, 1, 0);
+        int s = 0, g = 0, n_seg = 0;  // ring place, tiles issued, segments
+        uint32_t turn = 0;
+        bool ok = true;
+        // descriptors: Q, and K or V at the ring's first place; the high words hold no address
+        const uint32_t a_lo = (uint32_t)sw128_desc(smem_u32(sQ)), b_lo = (uint32_t)sw128_desc(smem_u32(ring));
+        const uint32_t k_hi = (uint32_t)(sw128_desc(0) >> 32), v_hi = (uint32_t)(mn_desc<Shape::V_LINE>(0, 0) >> 32);
+        const uint32_t v_lo = (uint32_t)mn_desc<Shape::V_LINE>(smem_u32(ring), VR * Shape::V_LINE);
+        auto advance = [&]() {
+          umma2_commit(&sh.empty[s]);
+          if (++s == RING) s = 0, turn ^= 1;
+        };
+        auto qk = [&](int tile) {  // S of the pair's tile number `tile`
+          const uint32_t d = tmem + Shape::S_COL + (tile & 1) * PA_KEYS;
+#pragma unroll
+          for (int v = 0; v < SLOTS; ++v) {
+            ok = ok && mbar_wait(&sh.full[s], turn, abort_flag);
+            if (!ok) return;
+            tc_fence_after();
+#pragma unroll
+            for (int ch = 0; ch < Shape::K_CHUNKS; ++ch) {
+              const uint32_t a = a_lo + (v * Shape::K_CHUNKS + ch) * (PA_ROWS * 128 >> 4);
+              const uint32_t b = b_lo + s * (PA_SLOT >> 4) + ch * (PA_KEYS / 2 * 128 >> 4);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) umma2_ss(d, a + 2 * k, b + 2 * k, k_hi, id_qk, v > 0 || ch > 0 || k > 0);
+            }
+            advance();
           }
-        } else {
-          lim = max(seg.first + tl, 0);
+          umma2_commit(&sh.s_full[tile & 1]);
+        };
+        auto pv = [&](int nk, uint32_t pt, bool first) {
+#pragma unroll
+          for (int v = 0; v < SLOTS; ++v) {
+            const int rows = nk - v * VR;
+            if (rows <= 0) break;
+            ok = ok && mbar_wait(&sh.full[s], turn, abort_flag);
+            if (!ok) return;
+            tc_fence_after();
+            const uint32_t b = v_lo + s * (PA_SLOT >> 4);
+#pragma unroll
+            for (int k = 0; k < VR / 16; ++k)
+              if (k * 16 < rows)
+                umma2_ts(tmem, pt + (v * VR + k * 16) / 2, b + (16 * Shape::V_LINE >> 4) * k, v_hi, id_pv,
+                         !first || v > 0 || k > 0);
+            advance();
+          }
+        };
+        for (; ok && walk.next(seg); ++n_seg) {
+          ok = mbar_wait(&sh.q_full, n_seg & 1, abort_flag);
+          const int n = seg.key1 - seg.key0;
+          if (ok) qk(g);
+          for (int j = 0; ok && j < n; ++j, ++g) {
+            if (j + 1 < n) qk(g + 1);
+            if (ok && j == max(0, n - 2)) umma2_commit(&sh.q_empty);  // after the segment's last S
+            if (j == 0 && n_seg > 0) ok = ok && mbar_wait(&sh.o_free, (n_seg - 1) & 1, abort_flag);
+            ok = ok && mbar_wait(&sh.p_full[g & 1], (g >> 1) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const int nk = seg.rows_of(p, seg.key0 + j);
+            pv(nk, tmem + Shape::S_COL + (g & 1) * PA_KEYS, j == 0);
+            if (ok) umma2_commit(&sh.pv_done[g & 1]);
+          }
+        }
+        // every MMA of the pair has completed before its TMEM is freed
+        umma2_commit(&sh.drained);
+        const long long t0 = clock64();
+        while (!mbar_try_wait(&sh.drained, 0) && clock64() - t0 < TC_WAIT_LIMIT) {
         }
       }
-      const bool live = __any_sync(0xffffffffu, valid);  // a warp without rows only keeps the barriers going
-      // on either axis, and the least of the warp's rows
-      const int lim_pre = min(lim, p.prefix_len), lim_own = min(max(lim - p.prefix_len, 0), seg.keys);
-      const int least_pre = __reduce_min_sync(0xffffffffu, valid ? lim_pre : INT32_MAX);
-      const int least_own = __reduce_min_sync(0xffffffffu, valid ? lim_own : INT32_MAX);
-      float m = -INFINITY, l = 0.0f;
-      for (int kt = seg.key0; kt < seg.key1; ++kt, ++g) {
-        const int b = g & 1;
-        mbar_wait(&sh.s_full[b], (g >> 1) & 1, abort_flag);
+    } else if (warp == 2) {
+      // ---- Q: this CTA's tokens of each item
+      if (lane == 0) {
+        const uint32_t bar = first_cta(&sh.q_full);
+        int n_seg = 0;
+        bool ok = true;
+        for (; walk.next(seg); ++n_seg) {
+          if (n_seg > 0 && !(ok = mbar_wait(&sh.q_empty, (n_seg - 1) & 1, abort_flag))) break;
+          const int box = seg.prefix ? p.tpc : min(p.tpc, p.max_new);
+          const bool any = seg.ntok > rank * p.tpc;
+          expect_first(bar, any ? (uint32_t)(box * p.G * 128 * Shape::CHUNKS) : 0u);
+          if (any)
+            for (int d = 0; d < Shape::CHUNKS; ++d)
+              pair_load_3d(sQ + d * PA_ROWS * 128, seg.prefix ? &map_q_pre : &map_q_own, bar, d * 64, seg.kvh * p.G,
+                           seg.tok0 + rank * p.tpc);
+        }
+        if (!ok) {
+          const long long t0 = clock64();
+          while (clock64() - t0 < TC_WAIT_LIMIT / 1000) {
+          }
+        }
+      }
+    } else if (warp == 3) {
+      if (p.whole) zero_unheld<D>(p, lane);
+      // ---- V rows past the last visible one, up to the end of the 16-row step, to zero, in the
+      // slots that warp 0 names: once for each segment that ends inside a step
+      const uint32_t full0 = first_cta(&sh.full[0]);
+      for (uint32_t n = 0;; ++n) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&sh.tail_full, n & 1, abort_flag))) break;
+        const int2 t = sh.tail_at;  // ring place, rows to keep
+        if (t.y == 0) break;
+        constexpr int UNITS = Shape::V_LINE / 16;  // 16-byte units of a row
+        const int units = (16 - (t.y & 15)) * UNITS;
+        uint8_t* base = ring + t.x * PA_SLOT + t.y * Shape::V_LINE;
+        for (int x = lane; x < units * Shape::V_CHUNKS; x += 32) {
+          const int ch = x / units, y = x - ch * units;
+          *reinterpret_cast<uint4*>(base + ch * VR * Shape::V_LINE + y * 16) = make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          release_first(full0 + 8 * t.x);
+          mbar_arrive(&sh.tail_done);
+        }
+      }
+    } else {
+      // ---- softmax, a row's column halves in two threads, then the segment's result
+      const int quarter = warp & 3, half = (warp - 4) >> 2, row = quarter * 32 + lane;
+      const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+      const uint32_t p_full0 = first_cta(&sh.p_full[0]), o_free0 = first_cta(&sh.o_free);
+      const float c = p.c;
+      int g = 0;
+      while (walk.next(seg)) {
+        const int row_tok = pa_quotient(row, p.g_magic), tl = rank * p.tpc + row_tok;  // token of the item
+        const bool valid = row_tok < p.tpc && tl < seg.ntok;
+        int lim = 0;  // rows of the sequence that the row sees
+        if (valid) {
+          if (seg.prefix) {
+            const int i = request_of(p.starts, p.batch, seg.tok0 + tl);
+            if (i < p.batch) {
+              const PaRequest r = pa_request(p, i);
+              lim = max(r.len - r.n + (seg.tok0 + tl - r.s0) + 1, 0);
+            }
+          } else {
+            lim = max(seg.first + tl, 0);
+          }
+        }
+        const bool live = __any_sync(0xffffffffu, valid);  // a warp without rows only keeps the barriers going
+        // on either axis, and the least of the warp's rows
+        const int lim_pre = min(lim, p.prefix_len), lim_own = min(max(lim - p.prefix_len, 0), seg.keys);
+        const int least_pre = __reduce_min_sync(0xffffffffu, valid ? lim_pre : INT32_MAX);
+        const int least_own = __reduce_min_sync(0xffffffffu, valid ? lim_own : INT32_MAX);
+        float m = -INFINITY, l = 0.0f;
+        for (int kt = seg.key0; kt < seg.key1; ++kt, ++g) {
+          const int b = g & 1;
+          mbar_wait(&sh.s_full[b], (g >> 1) & 1, abort_flag);
+          __syncwarp();
+          if (live) {
+            tc_fence_after();
+            const uint32_t at = tmem + lanes + Shape::S_COL + b * PA_KEYS;
+            uint32_t s[2][32];
+            tmem_ld32(at + half * 64, s[0]);
+            tmem_ld32(at + half * 64 + 32, s[1]);
+            tmem_ld_wait32(s[0]);
+            tmem_ld_wait32(s[1]);
+            const bool pre = kt < seg.pre;
+            const int from = (pre ? kt : kt - seg.pre) * PA_KEYS;  // the tile's first row on its axis
+            if ((pre ? least_pre : least_own) < from + PA_KEYS) {
+              const int see = (pre ? lim_pre : lim_own) - from - half * 64;
+#pragma unroll
+              for (int x = 0; x < 64; ++x)
+                if (x >= see) s[x >> 5][x & 31] = 0xff800000u;  // -inf
+            }
+            auto val = [&](int x) { return __uint_as_float(s[x >> 5][x & 31]); };
+            float t[4] = {val(0), val(1), val(2), val(3)};
+#pragma unroll
+            for (int x = 4; x < 60; x += 8)
+#pragma unroll
+              for (int y = 0; y < 4; ++y) t[y] = max3(t[y], val(x + 2 * y), val(x + 2 * y + 1));
+            t[0] = max3(t[0], val(60), val(61));
+            t[1] = max3(t[1], val(62), val(63));
+            const float mine = fmaxf(max3(t[0], t[1], t[2]), t[3]);
+            sh.half[b][half][row] = mine;
+            quarter_sync(quarter);  // also: both halves have read S, so P may take its place
+            const float top = __fmul_rn(fmaxf(mine, sh.half[b][half ^ 1][row]), c);
+            if (m == -INFINITY) m = top;  // nothing seen before: o and l are zero
+            const bool grown = top > m + 8.0f;
+            if (__any_sync(0xffffffffu, grown)) {
+              // o is complete up to the tile before; then scale it
+              mbar_wait(&sh.pv_done[b ^ 1], ((g - 1) >> 1) & 1, abort_flag);
+              __syncwarp();
+              tc_fence_after();
+              const float f = grown ? exp2_approx(m - top) : 1.0f;
+              // (Rolled: unrolled it is rare code that costs 800 bytes of spilled registers at D = 256.)
+#pragma unroll 1
+              for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
+                uint32_t o[32];
+                tmem_ld32(tmem + lanes + x, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+                tmem_st32(tmem + lanes + x, o);
+              }
+              l *= f;
+              if (grown) m = top;
+            }
+            const float base = m == -INFINITY ? 0.0f : -m;
+            const float2 c2 = make_float2(c, c), b2 = make_float2(base, base);
+            float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+            uint32_t w[32];
+#pragma unroll
+            for (int x = 0; x < 32; ++x) {
+              const float2 e = fma2(make_float2(val(2 * x), val(2 * x + 1)), c2, b2);
+              const float2 a = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+              sum[x & 1] = add2(sum[x & 1], a);
+              w[x] = Elem<DT>::pack(a.x, a.y);
+            }
+            tmem_st32(at + half * 32, w);
+            sum[0] = add2(sum[0], sum[1]);
+            l += sum[0].x + sum[0].y;
+            tmem_st_wait();
+            tc_fence_before();
+          }
+          __syncwarp();
+          if (lane == 0) arrive_first(p_full0 + 8 * b);
+        }
+        mbar_wait(&sh.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag);
         __syncwarp();
         if (live) {
           tc_fence_after();
-          const uint32_t at = tmem + lanes + Shape::S_COL + b * PA_KEYS;
-          uint32_t s[2][32];
-          tmem_ld32(at + half * 64, s[0]);
-          tmem_ld32(at + half * 64 + 32, s[1]);
-          tmem_ld_wait32(s[0]);
-          tmem_ld_wait32(s[1]);
-          const bool pre = kt < seg.pre;
-          const int from = (pre ? kt : kt - seg.pre) * PA_KEYS;  // the tile's first row on its axis
-          if ((pre ? least_pre : least_own) < from + PA_KEYS) {
-            const int see = (pre ? lim_pre : lim_own) - from - half * 64;
-#pragma unroll
-            for (int x = 0; x < 64; ++x)
-              if (x >= see) s[x >> 5][x & 31] = 0xff800000u;  // -inf
-          }
-          auto val = [&](int x) { return __uint_as_float(s[x >> 5][x & 31]); };
-          float t[4] = {val(0), val(1), val(2), val(3)};
-#pragma unroll
-          for (int x = 4; x < 60; x += 8)
-#pragma unroll
-            for (int y = 0; y < 4; ++y) t[y] = max3(t[y], val(x + 2 * y), val(x + 2 * y + 1));
-          t[0] = max3(t[0], val(60), val(61));
-          t[1] = max3(t[1], val(62), val(63));
-          const float mine = fmaxf(max3(t[0], t[1], t[2]), t[3]);
-          sh.half[b][half][row] = mine;
-          quarter_sync(quarter);  // also: both halves have read S, so P may take its place
-          const float top = __fmul_rn(fmaxf(mine, sh.half[b][half ^ 1][row]), c);
-          if (m == -INFINITY) m = top;  // nothing seen before: o and l are zero
-          const bool grown = top > m + 8.0f;
-          if (__any_sync(0xffffffffu, grown)) {
-            // o is complete up to the tile before; then scale it
-            mbar_wait(&sh.pv_done[b ^ 1], ((g - 1) >> 1) & 1, abort_flag);
-            __syncwarp();
-            tc_fence_after();
-            const float f = grown ? exp2_approx(m - top) : 1.0f;
-            // (Rolled: unrolled it is rare code that costs 800 bytes of spilled registers at D = 256.)
-#pragma unroll 1
+          quarter_sync(quarter);  // the tiles' exchanges have been read
+          sh.half[0][half][row] = l;
+          quarter_sync(quarter);
+          l += sh.half[0][half ^ 1][row];
+          if (seg.whole) {
+            const int h = seg.kvh * p.G + row - row_tok * p.G;
+            const int64_t t = seg.tok0 + tl;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            uint16_t* out = p.out + (t * p.n_kvh * p.G + h) * D;
+            const int64_t gate = t * p.gate_row + h * p.gate_head;
             for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
-              uint32_t o[32];
-              tmem_ld32(tmem + lanes + x, o);
-              tmem_ld_wait();
+              uint32_t v[32];
+              tmem_ld32(tmem + lanes + x, v);
+              tmem_ld_wait32(v);
+              if (valid) {
 #pragma unroll
-              for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-              tmem_st32(tmem + lanes + x, o);
-            }
-            l *= f;
-            if (grown) m = top;
-          }
-          const float base = m == -INFINITY ? 0.0f : -m;
-          const float2 c2 = make_float2(c, c), b2 = make_float2(base, base);
-          float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
-          uint32_t w[32];
-#pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            const float2 e = fma2(make_float2(val(2 * x), val(2 * x + 1)), c2, b2);
-            const float2 a = make_float2(exp2_approx(e.x), exp2_approx(e.y));
-            sum[x & 1] = add2(sum[x & 1], a);
-            w[x] = Elem<DT>::pack(a.x, a.y);
-          }
-          tmem_st32(at + half * 32, w);
-          sum[0] = add2(sum[0], sum[1]);
-          l += sum[0].x + sum[0].y;
-          tmem_st_wait();
-          tc_fence_before();
-        }
-        __syncwarp();
-        if (lane == 0) arrive_first(p_full0 + 8 * b);
-      }
-      mbar_wait(&sh.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag);
-      __syncwarp();
-      if (live) {
-        tc_fence_after();
-        quarter_sync(quarter);  // the tiles' exchanges have been read
-        sh.half[0][half][row] = l;
-        quarter_sync(quarter);
-        l += sh.half[0][half ^ 1][row];
-        if (seg.whole) {
-          const int h = seg.kvh * p.G + row - row_tok * p.G;
-          const int64_t t = seg.tok0 + tl;
-          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-          uint16_t* out = p.out + (t * p.n_kvh * p.G + h) * D;
-          const int64_t gate = t * p.gate_row + h * p.gate_head;
-          for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
-            uint32_t v[32];
-            tmem_ld32(tmem + lanes + x, v);
-            tmem_ld_wait32(v);
-            if (valid) {
-#pragma unroll
-              for (int y0 = 0; y0 < 32; y0 += 16) {
-                uint4 g[4];
-                if (p.gate) {
-#pragma unroll
-                  for (int y = 0; y < 4; ++y) g[y] = gate_load(p, gate + x + y0 + 4 * y);
-                }
-#pragma unroll
-                for (int y = 0; y < 16; y += 8) {
-                  float z[8];
-#pragma unroll
-                  for (int k = 0; k < 8; ++k) z[k] = __uint_as_float(v[y0 + y + k]) * inv;
+                for (int y0 = 0; y0 < 32; y0 += 16) {
+                  uint4 g[4];
                   if (p.gate) {
-                    const float4 a = gate_value<DT>(p, g[y / 4]), d = gate_value<DT>(p, g[y / 4 + 1]);
-                    const float gs[8] = {a.x, a.y, a.z, a.w, d.x, d.y, d.z, d.w};
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) z[k] = gated(z[k], gs[k]);
+                    for (int y = 0; y < 4; ++y) g[y] = gate_load(p, gate + x + y0 + 4 * y);
                   }
-                  *reinterpret_cast<uint4*>(out + x + y0 + y) =
-                      make_uint4(Elem<DT>::pack(z[0], z[1]), Elem<DT>::pack(z[2], z[3]), Elem<DT>::pack(z[4], z[5]),
-                                 Elem<DT>::pack(z[6], z[7]));
+#pragma unroll
+                  for (int y = 0; y < 16; y += 8) {
+                    float z[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) z[k] = __uint_as_float(v[y0 + y + k]) * inv;
+                    if (p.gate) {
+                      const float4 a = gate_value<DT>(p, g[y / 4]), d = gate_value<DT>(p, g[y / 4 + 1]);
+                      const float gs[8] = {a.x, a.y, a.z, a.w, d.x, d.y, d.z, d.w};
+#pragma unroll
+                      for (int k = 0; k < 8; ++k) z[k] = gated(z[k], gs[k]);
+                    }
+                    *reinterpret_cast<uint4*>(out + x + y0 + y) =
+                        make_uint4(Elem<DT>::pack(z[0], z[1]), Elem<DT>::pack(z[2], z[3]), Elem<DT>::pack(z[4], z[5]),
+                                   Elem<DT>::pack(z[6], z[7]));
+                  }
                 }
               }
             }
-          }
-        } else {
-          const int rows = seg.prefix ? 2 * PA_ROWS : p.own_rows;
-          const int at = rank * (seg.prefix ? PA_ROWS : p.own_half) + row;  // of the place
-          float4* o = reinterpret_cast<float4*>((seg.prefix ? p.pre_o : p.own_o) + seg.place * rows * D) + at;
-          for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
-            uint32_t v[32];
-            tmem_ld32(tmem + lanes + x, v);
-            tmem_ld_wait32(v);
-            if (valid) {
+          } else {
+            const int rows = seg.prefix ? 2 * PA_ROWS : p.own_rows;
+            const int at = rank * (seg.prefix ? PA_ROWS : p.own_half) + row;  // of the place
+            float4* o = reinterpret_cast<float4*>((seg.prefix ? p.pre_o : p.own_o) + seg.place * rows * D) + at;
+            for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
+              uint32_t v[32];
+              tmem_ld32(tmem + lanes + x, v);
+              tmem_ld_wait32(v);
+              if (valid) {
 #pragma unroll
-              for (int y = 0; y < 32; y += 4)
-                o[(x + y) / 4 * rows] = make_float4(__uint_as_float(v[y]), __uint_as_float(v[y + 1]),
-                                                    __uint_as_float(v[y + 2]), __uint_as_float(v[y + 3]));
+                for (int y = 0; y < 32; y += 4)
+                  o[(x + y) / 4 * rows] = make_float4(__uint_as_float(v[y]), __uint_as_float(v[y + 1]),
+                                                      __uint_as_float(v[y + 2]), __uint_as_float(v[y + 3]));
+              }
             }
+            if (valid && half == 0)
+              ((seg.prefix ? p.pre_ml : p.own_ml) + seg.place * rows)[at] = make_float2(m, l);
           }
-          if (valid && half == 0)
-            ((seg.prefix ? p.pre_ml : p.own_ml) + seg.place * rows)[at] = make_float2(m, l);
+          tc_fence_before();
+          quarter_sync(quarter);  // the halves' sums have been read
         }
-        tc_fence_before();
-        quarter_sync(quarter);  // the halves' sums have been read
+        __syncwarp();
+        if (lane == 0) arrive_first(o_free0);
       }
-      __syncwarp();
-      if (lane == 0) arrive_first(o_free0);
     }
-  }
   }
   tc_fence_before();
   __syncthreads();
@@ -1548,8 +1558,8 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   p.g_magic = magic(G), p.tpi_magic = magic(p.tpi);
   p.pre_tiles = (int)ceil_div(a.prefix_len, PA_KEYS), p.pre_qtiles = (int)ceil_div(a.tokens, 2 * tpc);
   const int64_t items = (int64_t)p.pre_qtiles * n_kvh;
-  if (items * pa_units(p.pre_tiles, false, PA_ITEM_COST) >= (int64_t)PA_MANY || (int64_t)a.tokens * n_qh * head > INT32_MAX ||
-      a.tokens >= 1 << 24 || n_kvh > 65535)
+  if (items * pa_units(p.pre_tiles, false, PA_ITEM_COST) >= (int64_t)PA_MANY ||
+      (int64_t)a.tokens * n_qh * head > INT32_MAX || a.tokens >= 1 << 24 || n_kvh > 65535)
     return fail(YSKN_EINVAL, "prefix_attention: too much work");
   p.shared_items = a.prefix_len > 0 ? (int)items : 0;
   // Few items of few tiles: each by one pair of SMs from end to end, which is quicker than the second
@@ -1560,7 +1570,8 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   p.own_pre = (int)ceil_div(a.prefix_len, 1 << p.tile_shift);
   p.item_cost = p.thin ? PA_THIN_COST : PA_ITEM_COST;
   const int64_t most_tiles = p.own_pre + ceil_div(p.own_limit, 1 << p.tile_shift);
-  p.whole = w.own_items <= (p.thin ? 2 * PA_THIN_WARPS : 1) * pairs && most_tiles <= (p.thin ? PA_THIN_WHOLE : PA_WHOLE_TILES);
+  p.whole = p.thin ? w.own_items <= 2 * PA_THIN_WARPS * pairs && most_tiles <= PA_THIN_WHOLE
+                   : w.own_items <= pairs && most_tiles <= PA_WHOLE_TILES;
   p.many_per_head = PA_MANY / (unsigned)n_kvh;
   // A warp of the join takes 16 channels of 8 rows; or more, where there are twice the warps that the
   // SMs hold: then few rows are left to join, or enough of them in every SM (16 prompt chunks: 945 us
