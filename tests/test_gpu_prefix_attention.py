@@ -164,6 +164,21 @@ def test_few_items_of_few_tiles(cuda, n_qh, n_kvh, D):
     run(cuda, new=(90, 1), own=(90, 120), P=0, seed=18, **kw)
 
 
+@pytest.mark.parametrize("G,n", [(1, 8), (2, 4), (3, 2), (4, 2), (8, 1), (5, 2), (9, 1)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_few_rows_a_head(cuda, G, n, D):
+    """Up to 8 rows a KV head (and just over), own rows from one slice to many, each count of tokens."""
+    kw = dict(n_qh=2 * G, n_kvh=2, D=D, gate=True)
+    run(cuda, new=(n, 1, max(1, n - 1), n, n), own=(n, 700, n + 15, 2100, n + 16), P=130, seed=21, **kw)
+    run(cuda, new=(n, 1, n), own=(n + 40, 1, 555), P=0, dtype="f16", block=64, head_major=False, seed=22, **kw)
+
+
+def test_many_short_requests(cuda):
+    """More requests than threads of a CTA, and than warps of all of them."""
+    run(cuda, new=(1,) * 500, own=tuple(1 + i % 40 for i in range(500)), n_qh=8, n_kvh=2, D=64, P=20, seed=23)
+    run(cuda, new=(1,) * 1000, own=tuple(1 + i % 5 for i in range(1000)), n_qh=6, n_kvh=3, D=64, P=0, seed=24)
+
+
 def test_padded_tokens_give_zeros(cuda):
     run(cuda, new=(1, 1), own=(5, 40), pad_tokens=200, seed=7)
     run(cuda, new=(0, 0), own=(5, 40), pad_tokens=3, seed=8)

@@ -15,19 +15,20 @@
 //                 2 * floor(128 / G) whole tokens of the batch, whichever request they belong
 //                 to) against the P prefix rows: the prefix is read once per 256 rows, not once
 //                 per request;
-//   own items     up to 256 rows of one request against that request's own rows.
+//   own items     up to 256 rows of one request against that request's own rows; thin ones, where
+//                 every request of the call has at most 8 rows a KV head (G max_new <= 8).
 // Where requests have many tokens each (prompt chunks), 256 rows of one request read the prefix as
 // well as 256 rows of several do: then an own item takes the prefix's tiles before its own and
 // there are no prefix items, so that most rows are finished in one place. Every CTA decides this
 // alike from the units that either way takes (below).
-// Items are cut along their key tiles (128 rows of the cache) so that every pair of SMs gets the
-// same share: an item counts PA_ITEM_COST units and one per tile, and pair c takes units
-// [c per, (c + 1) per) of all items in order. A piece of an item is a segment; its unnormalised
-// (m, l, o) goes to the workspace in binary32, at place item + c, which no two segments share,
-// and prefix_combine_kernel joins a row's segments, divides, gates and rounds; a segment that holds
-// all that its rows see finishes them itself. Everything is
-// summed in a fixed order: the same call gives the same bits. The lengths stay on the device:
-// every CTA forms the prefix sum of the requests' units itself.
+// Items are cut along their key tiles (128 rows of the cache; 16 for thin ones) so that every pair of
+// SMs (a warp, for thin ones, in the SMs that the prefix items leave) gets the same share: an item
+// counts a fixed cost in units and one per tile, and pair c takes units [c per, (c + 1) per) of all
+// items in order. A piece of an item is a segment; its unnormalised (m, l, o) goes to the workspace in
+// binary32, at place item + c, which no two segments share, and prefix_combine_kernel joins a row's
+// segments, divides, gates and rounds; a segment that holds all that its rows see finishes them
+// itself. Everything is summed in a fixed order: the same call gives the same bits. The lengths stay
+// on the device: every CTA forms the prefix sum of the requests' units itself.
 //
 // prefix_attention_kernel: persistent, clusters of two CTAs (a pair of SMs), 12 warps each. The
 // pair works on 256 rows with tcgen05.mma.cta_group::2: each CTA holds its 128 rows of Q, S, P and
@@ -73,17 +74,20 @@ constexpr int PA_SLOT = 16384;  // bytes per ring slot
 constexpr int PA_THREADS = 384;
 constexpr int PA_MAX_PAIRS = 74;
 constexpr int PA_MAX_SLOTS = 12;
-constexpr int PA_THIN_ROWS = 8;      // rows of a thin item, at most
-constexpr int PA_THIN_SHIFT = 4;     // a thin item's tiles: 16 rows of the cache
-constexpr int PA_THIN_COST = 3;      // its fixed cost in such tiles
-constexpr int PA_THIN_WHOLE = 6;     // tiles up to which few thin items are not cut
-constexpr int PA_THIN_LEAST = 4;     // units of a warp, at least
-constexpr int PA_THIN_WARPS = 12;    // warps of a CTA: each takes thin items by itself
-constexpr int PA_THIN_STAGE = 16384; // bytes on the way to one of them
-constexpr int PA_THIN_PER_TILE = 14; // thin tiles (two CTAs) in the time of a pair's tile of 128
+constexpr int PA_WHOLE_TILES = 1;  // tiles up to which few items are not cut
+constexpr int PA_ITEM_COST = 3;    // an item's fixed cost (Q, the last P V's wait, its result) in tiles
+// Thin items. Cost, least and time per tile as they served 64 requests best (us behind 32k rows, and
+// without a prefix): costs of 1, 3, 5: 100 and 50, 93 and 46, 81 and 41; times of 10, 14, 18 and 22:
+// 93, 89, 81, 97. A least of 2 rather than 4: two requests 13.7, not 14.8; of 1: 8 requests 17.2, not 15.7.
+constexpr int PA_THIN_ROWS = 8;       // rows of a thin item, at most
+constexpr int PA_THIN_SHIFT = 4;      // its tiles: 16 rows of the cache
+constexpr int PA_THIN_COST = 5;       // its fixed cost in such tiles
+constexpr int PA_THIN_LEAST = 2;      // units of a warp, at least
+constexpr int PA_THIN_WHOLE = 6;      // tiles up to which few thin items are not cut
+constexpr int PA_THIN_PER_TILE = 18;  // thin tiles (two CTAs) in the time of a pair's tile of 128
+constexpr int PA_THIN_WARPS = 12;     // warps of a CTA: each takes thin items by itself
+constexpr int PA_THIN_STAGE = 16384;  // bytes on the way to one of them
 constexpr int PA_MAX_THIN = 2 * PA_MAX_PAIRS * PA_THIN_WARPS;
-constexpr int PA_WHOLE_TILES = 2;  // tiles up to which few items are not cut
-constexpr int PA_ITEM_COST = 3;  // an item's fixed cost (Q, the last P V's wait, its result) in tiles
 
 template <int D>
 struct PaShape {
@@ -479,18 +483,20 @@ __device__ __forceinline__ void zero_unheld(const PrefixAttnParams& p, int lane)
 
 // ---- thin items: up to 8 rows (one token of up to 8 query heads a KV head, or a few of fewer)
 // against the request's own rows. 256 rows of MMA for 6 are 2048 clocks a tile for work that the
-// memory bounds, and an item's Q, S, P, O pass through one after another (64 requests of 1 to 1024
-// own rows: 74 us for 142 MB). Here each of 8 warps keeps a softmax of its own over every 8th
-// slice of 16 cache rows, with warp-level MMAs (m16n8k16): nothing is shared until the item's end,
-// where the 8 results are joined in shared memory. What bounds it: bytes, so the copies run a ring
-// of 8 chunks (16 rows of 64 channels of K or V) ahead, across items, 128 KB an SM.
-//   S = Q K^T   A: Q, rows 0..7 (8..15 zero); B: K, of a lane (g, t) the 16 bytes 8 t of row g of a
-//               chunk's half: two steps of 16 channels, in an order that Q's registers share;
-//   O^T = V^T P^T  B: P^T, which is S as it left the first MMA (row g, keys 2t, 2t+1 and 8 on);
-//               A: V^T, of a lane the 16 bytes 8 g of those four rows: word w's two channels of
-//               two rows by one byte permutation each, rows g and g + 8 of MMA w.
+// memory bounds, and an item's Q, S, P, O pass through one after another (64 requests of up to 1024
+// own rows, no prefix: 74 us for 142 MB; thin 41, of which the join is 7). Here each warp takes a run of
+// 16-row slices by itself, with warp-level MMAs (m16n8k16): no barrier. What bounds it: bytes, so
+// the copies run a ring of 8 chunks (16 rows of 64 channels of K or V) ahead, across items, 192 KB an SM
+// (in steady state 6.6 TB/s; the rest is the start, a warp's last slices and the join).
+//   S = Q K^T   A: Q, rows 0..7 (8..15 zero); B: K, of a lane (g, t) the 16-byte units t and t + 4 of
+//               row g in a chunk: steps of 16 channels in an order that Q's registers share;
+//   O^T = V^T P^T  B: P^T, which is S as it left the first MMA (row g, keys 2t, 2t + 1, 2t + 8 and
+//               2t + 9); A: V^T, of a lane unit g of those four rows: word w's two channels of two
+//               rows by one byte permutation each, rows g and g + 8 of MMA w.
+// (Eight warps on one item, joined in shared memory at its end: 71 us where one each takes 54, both with
+// the copies of that step; the MMAs are 5 % of it.)
 // A chunk's rows are 128 bytes; 8 lanes bring one (lanes that fetch just what they need later,
-// 64 or 32 bytes of a line a request, had the L2 answer 1.3 sectors a request: 54 us, now THINCO). The
+// 64 or 32 bytes of a line a request, had the L2 answer 1.3 sectors a request: 54 us, not 47). The
 // 16-byte unit c of row r lies at c ^ (4 (r2 ^ r0) + 2 r1), r's low bits, where both reads find their
 // 8 lanes on 8 different units.
 template <int DT>
@@ -1338,7 +1344,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
 // is 4 runs of 128 adjacent bytes and a store 8 runs of 32. What bounds it is the chain of
 // dependent loads (lengths, places, partial results), so as many segments as a row has in most
 // calls are asked for at once, and a thread has few channels (16 of them and 4 segments at once: 17 us
-// of the 93 of 64 requests behind 32k rows, COMBCO so).
+// of the 93 of 64 requests behind 32k rows, 10 so; 12 segments at once 12, 4 13).
 template <int D, int DT>
 __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_constant__ PrefixAttnParams p) {
   __shared__ float joined[8][6][32];
@@ -1562,9 +1568,10 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
       (int64_t)a.tokens * n_qh * head > INT32_MAX || a.tokens >= 1 << 24 || n_kvh > 65535)
     return fail(YSKN_EINVAL, "prefix_attention: too much work");
   p.shared_items = a.prefix_len > 0 ? (int)items : 0;
-  // Few items of few tiles: each by one pair of SMs from end to end, which is quicker than the second
-  // launch that joins its parts (two requests of up to 64 rows: 16.4 us cut, 13.9 whole without a
-  // prefix, 15.2 and 15.4 behind 100 rows, 15.4 and 16.1 behind 256).
+  // Few items of few tiles: each by one pair of SMs (a thin one by one warp) from end to end, which is
+  // quicker than the second launch that joins its parts. Two requests, us whole and cut: of two
+  // tokens and one tile 15.5, 19.2, of two tiles 17.3, 14.8; thin with up to 32 and 64 rows 10.3, 14.4
+  // and 12.1, 16.1, with 128 15.7, 13.8 (12.2 since a warp's least is 2 units).
   p.thin = G * a.max_new <= PA_THIN_ROWS && pairs > 1;
   p.tile_shift = p.thin ? PA_THIN_SHIFT : 7;
   p.own_pre = (int)ceil_div(a.prefix_len, 1 << p.tile_shift);
@@ -1575,11 +1582,12 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   p.many_per_head = PA_MANY / (unsigned)n_kvh;
   // A warp of the join takes 16 channels of 8 rows; or more, where there are twice the warps that the
   // SMs hold: then few rows are left to join, or enough of them in every SM (16 prompt chunks: 945 us
-  // with 16 channels, SPANCO with all).
+  // with 16 channels, 804 with all).
   const int64_t join_rows = ceil_div((int64_t)a.tokens * G, 8) * n_kvh;
   p.join_span = 1;
   while (p.join_span < head / 16 && join_rows * (head / 16 / p.join_span) > 2 * 148 * 24) p.join_span *= 2;
-  // Few: several warps share a row's segments (SPLITCO).
+  // Few: several warps share a row's segments (42 requests of one KV head behind 32k rows: 44.5 us by one
+  // warp, 28 by eight).
   p.join_split = 1;
   while (p.join_split < 8 && join_rows * (head / 16) * 2 * p.join_split <= 148 * 24) p.join_split *= 2;
   // a scale of zero keeps its meaning (equal weights) with a factor that leaves -inf alone
