@@ -806,7 +806,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
                  "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
-  if (warp == 2 && lane < 4) {
+  if (warp == 2 && lane < 4 && (!p.thin || p.shared_items > 0)) {
     const CUtensorMap* map = lane == 0 ? &map_q_pre : lane == 1 ? &map_q_own : lane == 2 ? &map_k : &map_v;
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
   }
@@ -1611,11 +1611,15 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   const int box_k[5] = {64, std::min(block_size, PA_KEYS / 2), block_size < PA_KEYS / 2 ? 1 : head / 64 / slots, 1, 1};
   const int box_v[5] = {head == 64 ? 32 : 64, std::min(block_size, v_rows),
                         block_size < v_rows || head <= 128 ? 1 : head / 128, 1, 1};
-  CUtensorMap maps[4];
-  if (int rc = paged_map(&maps[0], a.q, dtype, 3, q_dims, q_strides, box_pre)) return rc;
-  if (int rc = paged_map(&maps[1], a.q, dtype, 3, q_dims, q_strides, box_own)) return rc;
-  if (int rc = paged_map(&maps[2], a.k_cache, dtype, 5, c_dims, c_strides, box_k)) return rc;
-  if (int rc = paged_map(&maps[3], a.v_cache, dtype, 5, c_dims, c_strides, box_v)) return rc;
+  CUtensorMap maps[4] = {};
+  if (!p.thin || p.shared_items > 0) {  // thin items need no map
+    if (int rc = paged_map(&maps[0], a.q, dtype, 3, q_dims, q_strides, box_pre)) return rc;
+    if (int rc = paged_map(&maps[2], a.k_cache, dtype, 5, c_dims, c_strides, box_k)) return rc;
+    if (int rc = paged_map(&maps[3], a.v_cache, dtype, 5, c_dims, c_strides, box_v)) return rc;
+    maps[1] = maps[0];
+    if (!p.thin)
+      if (int rc = paged_map(&maps[1], a.q, dtype, 3, q_dims, q_strides, box_own)) return rc;
+  }
   const int grid = 2 * pairs;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   auto run = [&](auto d) {
