@@ -17,9 +17,10 @@
 // run of adjacent bytes, the sum of squares comes by shuffles, and a pair's other half, R / 2 (a
 // multiple of W) channels away, by one shuffle per channel (two where pairs straddle the runs).
 // A warp takes up to PP_RUN heads of one token where there are many rows (one where there are
-// few), each row requested while the one before is worked on (two rows ahead leaves room for
-// fewer warps: 86 us for 8192 tokens, not 78; runs of 4: 84); the cosines and sines of its
-// channels are computed once, one pair a lane, while its first rows arrive, and stay in registers. No block-wide step.
+// few: chosen with the launch), each row requested while the one before is worked on (two rows
+// ahead leaves room for fewer warps: 86 us for 8192 tokens, not 78; runs of 4: 84); the cosines and
+// sines of its channels are computed once, one pair a lane, while its first rows arrive, and stay in
+// registers. No block-wide step.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -28,8 +29,9 @@ namespace yskn {
 
 constexpr int PP_WARPS = 8;
 constexpr int PP_MAX_PAIRS = YSKN_MAX_PAIRS;
-constexpr int PP_RUN = 8;         // heads of a warp's run, at most
-constexpr int PP_FULL = 148 * 32;  // warps that keep the SMs busy: runs get longer beyond that
+constexpr int PP_RUN = 16;           // heads of a warp's run, at most
+constexpr int PP_SETUP = 3;          // a warp's set-up in the time of a head
+constexpr int PP_RESIDENT = 148 * 4;  // CTAs at a time
 
 struct PagedPrepParams {
   const void *q, *k, *v;
@@ -288,8 +290,14 @@ extern "C" YSKN_B200_API int yskn_b200_paged_prep(const yskn_b200_paged_prep_arg
   p.err = device_error_word();
   for (int i = 0; i < a.rot / 2; ++i) p.axis[i] = a.axes[i];
   const int heads = a.n_qh + 2 * a.n_kvh;
-  p.run = (int)std::min<int64_t>(PP_RUN, std::max<int64_t>(1, (int64_t)a.tokens * heads / PP_FULL));
-  const int64_t runs = ceil_div(heads, p.run);
+  // The run that takes the least time in whole rounds of resident CTAs (300 tokens of 30 heads of 128: 8.7 us
+  // with runs that just fill the SMs, 6.0 so; 1037 tokens 11.8, 10.6; 3000 of 32 heads of 256 31.1, 29.7).
+  int64_t least = INT64_MAX;
+  for (int run = 1; run <= std::min(PP_RUN, heads); ++run) {
+    const int64_t time = ceil_div(ceil_div(a.tokens, PP_WARPS) * ceil_div(heads, run), PP_RESIDENT) * (PP_SETUP + run);
+    if (time < least) least = time, p.run = run;
+  }
+  const int64_t runs = ceil_div(heads, std::max(p.run, 1));
   if (heads < 0 || runs > 65535) return fail(YSKN_EINVAL, "paged_prep: too many heads");
   const dim3 grid((unsigned)ceil_div(a.tokens, PP_WARPS), (unsigned)runs);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
