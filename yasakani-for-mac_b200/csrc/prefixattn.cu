@@ -155,7 +155,7 @@ struct PrefixAttnParams {
   int join_span, join_split;  // 16-channel parts of a row that a warp of the join takes; warps for one part
   float c;     // |scale| log2 e
   uint32_t negate_q;
-  int4* work_per;         // for the join: units per pair of prefix items and of own ones, whether alone
+  int4* work_per;         // for the join: units per pair of prefix items and of own ones, whether alone, own units
   int2* work_base;        // [batch] own items, and units of all items, before each request's own
   // per place: (m, l) of each row; o as [D / 4][rows][4], so that a warp's rows are adjacent
   float2 *pre_ml, *own_ml;
@@ -469,15 +469,22 @@ __device__ __forceinline__ void quarter_sync(int quarter) {
   asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
 }
 
-// Where there is no join: zeros for this CTA's share of the tokens that no item holds. One warp.
+// Where no join visits every row: zeros for this CTA's share of the tokens that no item holds. One
+// warp; each lane looks at a token.
 template <int D>
 __device__ __forceinline__ void zero_unheld(const PrefixAttnParams& p, int lane) {
-  for (int t = blockIdx.x; t < p.tokens; t += gridDim.x) {
-    const int i = request_of(p.starts, p.batch, t);
-    const PaRequest r = i < p.batch ? pa_request(p, i) : PaRequest{};
-    if (t >= r.s0 && t < r.s0 + r.n && pa_tiles(p, r, pa_quotient(t - r.s0, p.tpi_magic), true) > 0) continue;
-    uint4* row = reinterpret_cast<uint4*>(p.out + (int64_t)t * p.n_kvh * p.G * D);
-    for (int x = lane; x < p.n_kvh * p.G * D / 8; x += 32) row[x] = make_uint4(0, 0, 0, 0);
+  for (int t0 = blockIdx.x * 32; t0 < p.tokens; t0 += gridDim.x * 32) {
+    const int t = t0 + lane;
+    bool bare = t < p.tokens;
+    if (bare) {
+      const int i = request_of(p.starts, p.batch, t);
+      const PaRequest r = i < p.batch ? pa_request(p, i) : PaRequest{};
+      bare = t < r.s0 || t >= r.s0 + r.n || pa_tiles(p, r, pa_quotient(t - r.s0, p.tpi_magic), true) == 0;
+    }
+    for (unsigned left = __ballot_sync(0xffffffffu, bare); left; left &= left - 1) {
+      uint4* row = reinterpret_cast<uint4*>(p.out + (int64_t)(t0 + __ffs(left) - 1) * p.n_kvh * p.G * D);
+      for (int x = lane; x < p.n_kvh * p.G * D / 8; x += 32) row[x] = make_uint4(0, 0, 0, 0);
+    }
   }
 }
 
@@ -857,8 +864,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
     const int pre_units = pa_units(p.pre_tiles, false, PA_ITEM_COST);
     const int pre_all = p.shared_items * pre_units;  // below 2^30: the host looked
     const unsigned long long pre_time = (unsigned long long)pre_all * (p.thin ? PA_THIN_PER_TILE : 1);
-    const bool alone = p.whole || (p.shared_items > 0 && total_of[1] < PA_MANY &&
-                                   8ull * total_of[1] <= 9ull * (pre_time + total_of[0]));
+    const bool alone = p.whole || p.shared_items == 0 ||
+                       (total_of[1] < PA_MANY && 8ull * total_of[1] <= 9ull * (pre_time + total_of[0]));
     const unsigned units = alone ? units_of[1] : units_of[0], total = alone ? total_of[1] : total_of[0];
     const unsigned before =
         alone ? pa_sum(before_of[1], ui[1] - units_of[1]) : pa_sum(before_of[0], ui[0] - units_of[0]);
@@ -896,7 +903,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
       }
       sh.start[tid] = s;
       if (blockIdx.x == 0 && tid == 0) {
-        *p.work_per = make_int4(share_pre, share_own, alone, 0);
+        *p.work_per = make_int4(share_pre, share_own, alone, own);
         if (!sound) raise_device_error(p.err, DERR_RANGE);
       }
     }
@@ -905,7 +912,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
     const int step = ctas * share_own;
     const int walks = thin ? PA_THIN_WARPS : p.thin ? 0 : 1, first = who0 * share_own - (p.thin ? 0 : pre);
     const int last = first + (walks - 1) * step;
-    if (sound && units > 0 && ((last >= (int)before && first < (int)(before + units)) || blockIdx.x == 0)) {
+    if (sound && (blockIdx.x == 0 || (units > 0 && last >= (int)before && first < (int)(before + units)))) {
       int b = (int)before, item = (int)items_before;
       for (int i = i0; i < i1; ++i) {
         int u = (int)units, n = (int)items;
@@ -1135,7 +1142,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
         }
       }
     } else if (warp == 3) {
-      if (p.whole) zero_unheld<D>(p, lane);
+      if (walk.alone) zero_unheld<D>(p, lane);
       // ---- V rows past the last visible one, up to the end of the 16-row step, to zero, in the
       // slots that warp 0 names: once for each segment that ends inside a step
       const uint32_t full0 = first_cta(&sh.full[0]);
@@ -1345,6 +1352,139 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
 // dependent loads (lengths, places, partial results), so as many segments as a row has in most
 // calls are asked for at once, and a thread has few channels (16 of them and 4 segments at once: 17 us
 // of the 93 of 64 requests behind 32k rows, 10 so; 12 segments at once 12, 4 13).
+struct RowSum {
+  float4 o;
+  float den, top;
+};
+// Every stride-th segment of a row from `first` on: x < n_pre of its prefix item, the others of its own.
+template <int D>
+__device__ __forceinline__ RowSum join_segments(const float2* pre_ml, const float4* pre_o, const float2* own_ml,
+                                                const float4* own_o, int own_step, int n_pre, int n, int first,
+                                                int stride) {
+  constexpr int BATCH = 8;  // segments asked for at once
+  RowSum s{make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f, -INFINITY};
+#pragma unroll 1
+  for (int x0 = first; x0 < n; x0 += BATCH * stride) {
+    float2 ml[BATCH];
+    float4 y[BATCH];
+    float now = s.top;
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      ml[u] = make_float2(-INFINITY, 0.0f), y[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const int x = x0 + u * stride;
+      if (x < n) {
+        const bool pre = x < n_pre;
+        const int64_t at = pre ? (int64_t)x * (2 * PA_ROWS) : (int64_t)(x - n_pre) * own_step;
+        ml[u] = (pre ? pre_ml : own_ml)[at];
+        y[u] = (pre ? pre_o : own_o)[at * (D / 4)];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) now = fmaxf(now, ml[u].x);
+    const float keep = s.top == -INFINITY ? 0.0f : exp2_approx(s.top - now);
+    s.top = now;
+    s.den *= keep, s.o.x *= keep, s.o.y *= keep, s.o.z *= keep, s.o.w *= keep;
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const float w = ml[u].x == -INFINITY ? 0.0f : exp2_approx(ml[u].x - now);
+      s.den = fmaf(ml[u].y, w, s.den);
+      s.o.x = fmaf(y[u].x, w, s.o.x), s.o.y = fmaf(y[u].y, w, s.o.y);
+      s.o.z = fmaf(y[u].z, w, s.o.z), s.o.w = fmaf(y[u].w, w, s.o.w);
+    }
+  }
+  return s;
+}
+// A row's four channels 4 ch .. 4 ch + 3: divided, gated, rounded.
+template <int D, int DT>
+__device__ __forceinline__ void join_store(const PrefixAttnParams& p, int t, int h, int ch, const RowSum& s, uint4 gate) {
+  const float inv = s.den == 0.0f ? 0.0f : 1.0f / s.den;
+  float v[4] = {s.o.x * inv, s.o.y * inv, s.o.z * inv, s.o.w * inv};
+  if (p.gate) {
+    const float4 g = gate_value<DT>(p, gate);
+    v[0] = gated(v[0], g.x), v[1] = gated(v[1], g.y), v[2] = gated(v[2], g.z), v[3] = gated(v[3], g.w);
+  }
+  *reinterpret_cast<uint2*>(p.out + ((int64_t)t * p.n_kvh * p.G + h) * D + ch * 4) =
+      make_uint2(Elem<DT>::pack(v[0], v[1]), Elem<DT>::pack(v[2], v[3]));
+}
+__device__ __forceinline__ uint4 join_gate(const PrefixAttnParams& p, int t, int h, int ch) {
+  return p.gate ? gate_load(p, t * p.gate_row + h * p.gate_head + ch * 4) : make_uint4(0, 0, 0, 0);
+}
+// b / per, a pair's or a warp's number: small, so that one correction makes the quotient in binary32
+// right.
+__device__ __forceinline__ int pair_of(int b, int per) {
+  int q = (int)((float)b * (1.0f / (float)per));
+  q -= q * per > b;
+  return q + ((q + 1) * per <= b);
+}
+
+// Without prefix items only the items that a pair's share cuts are left to join: the warps take
+// their rows, 8 rows and 64 channels each, by the pair that the cut ends at. (16 prompt chunks, whose rows
+// were looked at one by one before: the join 45 us, 24 so, with flushed caches.)
+template <int D, int DT>
+__device__ __forceinline__ void join_cut_items(const PrefixAttnParams& p, int per, int units, int warp, int lane) {
+  const int groups = (p.own_rows + 7) / 8, each = groups * (D / 64), cuts = (units + per - 1) / per - 1;
+  const int warps = gridDim.x * gridDim.y * 8;
+  for (int w = (blockIdx.y * gridDim.x + blockIdx.x) * 8 + warp; w < cuts * each; w += warps) {
+    const int c = 1 + w / each, rest = w % each, unit = c * per;
+    int lo = 0, hi = p.batch;  // the last request whose units begin at or before this one
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (p.work_base[mid].y <= unit) lo = mid;
+      else hi = mid;
+    }
+    const int2 base = p.work_base[lo];
+    const PaRequest r = pa_request(p, lo);
+    const int nq = pa_qtiles(p, r), head = (int)pa_own_units(p, r, nq, true);
+    int u = unit - base.y, kvh = 0, qt = 0, kt = 0;
+    if (head <= 0) continue;
+    kvh = u / head, u -= kvh * head;
+    for (; qt < nq; ++qt) {
+      kt = pa_tiles(p, r, qt, true);
+      const int n = pa_units(kt, false, p.item_cost);
+      if (u < n) break;
+      u -= n;
+    }
+    if (kvh >= p.n_kvh || qt >= nq) continue;
+    const int b = unit - u + p.item_cost, c0 = pair_of(b, per), n = pair_of(b + kt - 1, per) - c0 + 1;
+    if (n < 2 || c0 != c - 1) continue;  // not cut here, or first cut before
+    const int row = rest / (D / 64) * 8 + (lane & 7), rank = row >= p.own_half, in = row - rank * p.own_half;
+    const int tl = rank * p.tpc + pa_quotient(in, p.g_magic), h = kvh * p.G + in - pa_quotient(in, p.g_magic) * p.G;
+    if (row >= p.own_rows || tl >= min(p.tpi, r.n - qt * p.tpi)) continue;
+    const int t = r.s0 + qt * p.tpi + tl;
+    const int64_t at = (int64_t)(base.x + kvh * nq + qt + c0) * p.own_rows;
+    int ch = rest % (D / 64) * 16 + (lane >> 3);
+    const float2* ml = p.own_ml + at + row;
+    const float4* o = reinterpret_cast<const float4*>(p.own_o) + at * (D / 4) + row;
+    if (n == 2) {  // the common case: everything asked for at once
+      const float2 m0 = ml[0], m1 = ml[p.own_rows];
+      const int64_t step = (int64_t)p.own_rows * (D / 4);
+      float4 y0[4], y1[4];
+      uint4 gate[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        y0[j] = o[(ch + 4 * j) * p.own_rows], y1[j] = o[(ch + 4 * j) * p.own_rows + step];
+        gate[j] = join_gate(p, t, h, ch + 4 * j);
+      }
+      const float top = fmaxf(m0.x, m1.x);
+      const float w0 = m0.x == -INFINITY ? 0.0f : exp2_approx(m0.x - top);
+      const float w1 = m1.x == -INFINITY ? 0.0f : exp2_approx(m1.x - top);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const RowSum s{make_float4(fmaf(y1[j].x, w1, y0[j].x * w0), fmaf(y1[j].y, w1, y0[j].y * w0),
+                                   fmaf(y1[j].z, w1, y0[j].z * w0), fmaf(y1[j].w, w1, y0[j].w * w0)),
+                       fmaf(m1.y, w1, m0.y * w0), top};
+        join_store<D, DT>(p, t, h, ch + 4 * j, s, gate[j]);
+      }
+      continue;
+    }
+#pragma unroll 1
+    for (int j = 0; j < 4; ++j, ch += 4) {
+      const uint4 gate = join_gate(p, t, h, ch);
+      join_store<D, DT>(p, t, h, ch, join_segments<D>(ml, o, ml, o + ch * p.own_rows, p.own_rows, 0, n, 0, 1), gate);
+    }
+  }
+}
+
 template <int D, int DT>
 __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_constant__ PrefixAttnParams p) {
   __shared__ float joined[8][6][32];
@@ -1356,29 +1496,26 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
   bool live = t < p.tokens;
   pdl_begin();
   const int4 how = *p.work_per;
+  const bool alone = how.z;
   // one token for each request is the common case: its request's numbers are asked for at once
   int i = t;
   PaRequest r{-1, 0, 0};
   int2 base{};
   if (t < p.batch) r = pa_request(p, t), base = p.work_base[t];
+  if (alone && !p.thin) {
+    if (how.y > 0) join_cut_items<D, DT>(p, how.y, how.w, warp, lane);
+    return;
+  }
   if (live && (r.s0 != t || r.n != 1)) {
     i = request_of(p.starts, p.batch, t);
     r = i < p.batch ? pa_request(p, i) : PaRequest{-1, 0, 0};
     if (i < p.batch) base = p.work_base[i];
   }
-  const bool alone = how.z;
   // segments of the row: n_pre of its prefix item, n_own of its own, from their first places on
   int n_pre = 0, n_own = 0;
   const float4 *pre_o = nullptr, *own_o = nullptr;
   const float2 *pre_ml = nullptr, *own_ml = nullptr;
-  const int pre_step = 2 * PA_ROWS, own_step = p.own_rows;  // rows from one place to the next
   if (live && (how.x | how.y) > 0 && t >= r.s0 && t < r.s0 + r.n) {
-    // b / per, a pair's number: small, so that one correction makes the quotient in binary32 right
-    auto pair_of = [&](int b, int per) {
-      int q = (int)((float)b * (1.0f / (float)per));
-      q -= q * per > b;
-      return q + ((q + 1) * per <= b);
-    };
     const int nq = pa_qtiles(p, r), own_qt = nq > 1 ? pa_quotient(t - r.s0, p.tpi_magic) : 0;
     const int kt = pa_tiles(p, r, own_qt, alone);
     if (kt > 0) {
@@ -1387,87 +1524,46 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
       for (int q = 0; q < own_qt; ++q) b += pa_units(pa_tiles(p, r, q, alone), false, p.item_cost);
       const int c0 = pair_of(b, how.y), tl = t - r.s0 - own_qt * p.tpi, rank = tl >= p.tpc;
       n_own = pair_of(b + kt - 1, how.y) - c0 + 1;
-      const int64_t place = base.x + kvh * nq + own_qt + c0;
+      const int64_t at = (int64_t)(base.x + kvh * nq + own_qt + c0) * p.own_rows;
       const int row = rank * p.own_half + (tl - rank * p.tpc) * p.G + gh;
-      own_ml = p.own_ml + place * own_step + row;
-      own_o = reinterpret_cast<const float4*>(p.own_o) + place * own_step * (D / 4) + ch * own_step + row;
+      own_ml = p.own_ml + at + row;
+      own_o = reinterpret_cast<const float4*>(p.own_o) + at * (D / 4) + ch * p.own_rows + row;
     }
-    if (n_own == 1 && (alone || p.pre_tiles == 0)) live = false;  // finished where it was computed
-    if (!alone && p.pre_tiles > 0) {
+    if (n_own == 1 && alone) live = false;  // finished where it was computed
+    if (!alone) {
       const int qt = pa_quotient(t, p.tpi_magic), it = kvh * p.pre_qtiles + qt, tl = t - qt * p.tpi, rank = tl >= p.tpc;
       const int b = it * pa_units(p.pre_tiles, false, PA_ITEM_COST) + PA_ITEM_COST, c0 = pair_of(b, how.x);
       n_pre = pair_of(b + p.pre_tiles - 1, how.x) - c0 + 1;
-      const int64_t place = it + c0;
+      const int64_t at = (int64_t)(it + c0) * (2 * PA_ROWS);
       const int row = rank * PA_ROWS + (tl - rank * p.tpc) * p.G + gh;
-      pre_ml = p.pre_ml + place * pre_step + row;
-      pre_o = reinterpret_cast<const float4*>(p.pre_o) + place * pre_step * (D / 4) + ch * pre_step + row;
+      pre_ml = p.pre_ml + at + row;
+      pre_o = reinterpret_cast<const float4*>(p.pre_o) + at * (D / 4) + ch * (2 * PA_ROWS) + row;
     }
   }
-  constexpr int BATCH = 8;  // segments asked for at once
   const int n = live ? n_pre + n_own : 0;
-  // segment x of the own ones is the row's n_pre + x
-  own_ml -= (int64_t)n_pre * own_step, own_o -= (int64_t)n_pre * own_step * (D / 4);
   if (split == 1 && !live) return;
 #pragma unroll 1
-  for (int j = 0; j < p.join_span; ++j, ch += 4, pre_o += 4 * pre_step, own_o += 4 * own_step) {
-    uint4 gate = make_uint4(0, 0, 0, 0);
-    if (p.gate && live) gate = gate_load(p, t * p.gate_row + h * p.gate_head + ch * 4);
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float den = 0.0f, top = -INFINITY;
-#pragma unroll 1
-    for (int x0 = part; x0 < n; x0 += BATCH * split) {
-      float2 ml[BATCH];
-      float4 y[BATCH];
-      float now = top;
-#pragma unroll
-      for (int u = 0; u < BATCH; ++u) {
-        ml[u] = make_float2(-INFINITY, 0.0f), y[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const int x = x0 + u * split;
-        if (x < n) {
-          const bool pre = x < n_pre;
-          const int64_t at = (int64_t)x * (pre ? pre_step : own_step);
-          ml[u] = (pre ? pre_ml : own_ml)[at];
-          y[u] = (pre ? pre_o : own_o)[at * (D / 4)];
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < BATCH; ++u) now = fmaxf(now, ml[u].x);
-      const float keep = top == -INFINITY ? 0.0f : exp2_approx(top - now);
-      top = now;
-      den *= keep, o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
-#pragma unroll
-      for (int u = 0; u < BATCH; ++u) {
-        const float w = ml[u].x == -INFINITY ? 0.0f : exp2_approx(ml[u].x - now);
-        den = fmaf(ml[u].y, w, den);
-        o.x = fmaf(y[u].x, w, o.x), o.y = fmaf(y[u].y, w, o.y);
-        o.z = fmaf(y[u].z, w, o.z), o.w = fmaf(y[u].w, w, o.w);
-      }
-    }
+  for (int j = 0; j < p.join_span; ++j, ch += 4, pre_o += 4 * 2 * PA_ROWS, own_o += 4 * p.own_rows) {
+    const uint4 gate = live ? join_gate(p, t, h, ch) : make_uint4(0, 0, 0, 0);
+    RowSum s = join_segments<D>(pre_ml, pre_o, own_ml, own_o, p.own_rows, n_pre, n, part, split);
     if (split > 1) {  // the parts of the row's segments, in order
       float(&mine)[6][32] = joined[warp];
-      mine[0][lane] = top, mine[1][lane] = den;
-      mine[2][lane] = o.x, mine[3][lane] = o.y, mine[4][lane] = o.z, mine[5][lane] = o.w;
+      mine[0][lane] = s.top, mine[1][lane] = s.den;
+      mine[2][lane] = s.o.x, mine[3][lane] = s.o.y, mine[4][lane] = s.o.z, mine[5][lane] = s.o.w;
       __syncthreads();
       if (part > 0 || !live) return;
       for (int x = 1; x < split; ++x) {
         const float(&other)[6][32] = joined[warp + x];
-        const float most = other[0][lane], now = fmaxf(top, most);
-        const float keep = top == -INFINITY ? 0.0f : exp2_approx(top - now);
+        const float most = other[0][lane], now = fmaxf(s.top, most);
+        const float keep = s.top == -INFINITY ? 0.0f : exp2_approx(s.top - now);
         const float w = most == -INFINITY ? 0.0f : exp2_approx(most - now);
-        top = now;
-        den = den * keep + other[1][lane] * w;
-        o.x = o.x * keep + other[2][lane] * w, o.y = o.y * keep + other[3][lane] * w;
-        o.z = o.z * keep + other[4][lane] * w, o.w = o.w * keep + other[5][lane] * w;
+        s.top = now;
+        s.den = s.den * keep + other[1][lane] * w;
+        s.o.x = s.o.x * keep + other[2][lane] * w, s.o.y = s.o.y * keep + other[3][lane] * w;
+        s.o.z = s.o.z * keep + other[4][lane] * w, s.o.w = s.o.w * keep + other[5][lane] * w;
       }
     }
-    const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-    float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-    if (p.gate) {
-      const float4 g = gate_value<DT>(p, gate);
-      v[0] = gated(v[0], g.x), v[1] = gated(v[1], g.y), v[2] = gated(v[2], g.z), v[3] = gated(v[3], g.w);
-    }
-    *reinterpret_cast<uint2*>(p.out + ((int64_t)t * p.n_kvh * p.G + h) * D + ch * 4) =
-        make_uint2(Elem<DT>::pack(v[0], v[1]), Elem<DT>::pack(v[2], v[3]));
+    join_store<D, DT>(p, t, h, ch, s, gate);
   }
 }
 
