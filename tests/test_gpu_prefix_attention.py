@@ -179,6 +179,16 @@ def test_many_short_requests(cuda):
     run(cuda, new=(1,) * 1000, own=tuple(1 + i % 5 for i in range(1000)), n_qh=6, n_kvh=3, D=64, P=0, seed=24)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_items_cut_in_many_places(cuda, D):
+    """Long own rows of few requests, idle and empty ones and padding among them; without a prefix, and
+    with one that each request's items take themselves."""
+    kw = dict(n_qh=10, n_kvh=2, D=D, gate=True, block=128)
+    run(cuda, new=(3, 0, 2, 4, 0), lens=[5000, 0, 2, 3000, 7], P=0, pad_tokens=40, seed=25, **kw)
+    run(cuda, new=(60, 0, 2, 55), lens=[2000, 0, 0, 900], P=0, pad_tokens=3, seed=26, **kw)
+    run(cuda, new=(130, 0, 70), lens=[900, 300, 230], P=160, pad_tokens=3, seed=27, **kw)
+
+
 def test_padded_tokens_give_zeros(cuda):
     run(cuda, new=(1, 1), own=(5, 40), pad_tokens=200, seed=7)
     run(cuda, new=(0, 0), own=(5, 40), pad_tokens=3, seed=8)

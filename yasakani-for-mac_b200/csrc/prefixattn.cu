@@ -410,8 +410,8 @@ __device__ __forceinline__ void pair_load_3d(void* dst, const CUtensorMap* map, 
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
-__device__ __forceinline__ void pair_load_5d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w,
-                                             int v) {
+__device__ __forceinline__ void pair_load_5d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z,
+                                             int w, int v) {
   asm volatile(
       "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
       "%5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
@@ -1396,7 +1396,8 @@ __device__ __forceinline__ RowSum join_segments(const float2* pre_ml, const floa
 }
 // A row's four channels 4 ch .. 4 ch + 3: divided, gated, rounded.
 template <int D, int DT>
-__device__ __forceinline__ void join_store(const PrefixAttnParams& p, int t, int h, int ch, const RowSum& s, uint4 gate) {
+__device__ __forceinline__ void join_store(const PrefixAttnParams& p, int t, int h, int ch, const RowSum& s,
+                                           uint4 gate) {
   const float inv = s.den == 0.0f ? 0.0f : 1.0f / s.den;
   float v[4] = {s.o.x * inv, s.o.y * inv, s.o.z * inv, s.o.w * inv};
   if (p.gate) {
@@ -1676,9 +1677,9 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   p.whole = p.thin ? w.own_items <= 2 * PA_THIN_WARPS * pairs && most_tiles <= PA_THIN_WHOLE
                    : w.own_items <= pairs && most_tiles <= PA_WHOLE_TILES;
   p.many_per_head = PA_MANY / (unsigned)n_kvh;
-  // A warp of the join takes 16 channels of 8 rows; or more, where there are twice the warps that the
-  // SMs hold: then few rows are left to join, or enough of them in every SM (16 prompt chunks: 945 us
-  // with 16 channels, 804 with all).
+  // A warp of the join takes 16 channels of 8 rows; or more, where that makes twice the warps that the
+  // SMs hold (128 requests of 8 tokens: 162 us with 16 channels, 141 so; 16 prompt chunks, where most
+  // warps find nothing to do, 835, 740).
   const int64_t join_rows = ceil_div((int64_t)a.tokens * G, 8) * n_kvh;
   p.join_span = 1;
   while (p.join_span < head / 16 && join_rows * (head / 16 / p.join_span) > 2 * 148 * 24) p.join_span *= 2;
