@@ -1356,12 +1356,12 @@ struct RowSum {
   float4 o;
   float den, top;
 };
-// Every stride-th segment of a row from `first` on: x < n_pre of its prefix item, the others of its own.
-template <int D>
+// Every stride-th segment of a row from `first` on: x < n_pre of its prefix item, the others of its own
+// (own_ml and own_o are where segment 0 would be). BATCH: segments asked for at once.
+template <int D, int BATCH>
 __device__ __forceinline__ RowSum join_segments(const float2* pre_ml, const float4* pre_o, const float2* own_ml,
                                                 const float4* own_o, int own_step, int n_pre, int n, int first,
                                                 int stride) {
-  constexpr int BATCH = 8;  // segments asked for at once
   RowSum s{make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f, -INFINITY};
 #pragma unroll 1
   for (int x0 = first; x0 < n; x0 += BATCH * stride) {
@@ -1374,7 +1374,7 @@ __device__ __forceinline__ RowSum join_segments(const float2* pre_ml, const floa
       const int x = x0 + u * stride;
       if (x < n) {
         const bool pre = x < n_pre;
-        const int64_t at = pre ? (int64_t)x * (2 * PA_ROWS) : (int64_t)(x - n_pre) * own_step;
+        const int64_t at = (int64_t)x * (pre ? 2 * PA_ROWS : own_step);
         ml[u] = (pre ? pre_ml : own_ml)[at];
         y[u] = (pre ? pre_o : own_o)[at * (D / 4)];
       }
@@ -1456,32 +1456,31 @@ __device__ __forceinline__ void join_cut_items(const PrefixAttnParams& p, int pe
     int ch = rest % (D / 64) * 16 + (lane >> 3);
     const float2* ml = p.own_ml + at + row;
     const float4* o = reinterpret_cast<const float4*>(p.own_o) + at * (D / 4) + row;
-    if (n == 2) {  // the common case: everything asked for at once
+    if (n == 2) {  // the common case: eight channels asked for at once
       const float2 m0 = ml[0], m1 = ml[p.own_rows];
-      const int64_t step = (int64_t)p.own_rows * (D / 4);
-      float4 y0[4], y1[4];
-      uint4 gate[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        y0[j] = o[(ch + 4 * j) * p.own_rows], y1[j] = o[(ch + 4 * j) * p.own_rows + step];
-        gate[j] = join_gate(p, t, h, ch + 4 * j);
-      }
       const float top = fmaxf(m0.x, m1.x);
       const float w0 = m0.x == -INFINITY ? 0.0f : exp2_approx(m0.x - top);
       const float w1 = m1.x == -INFINITY ? 0.0f : exp2_approx(m1.x - top);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const RowSum s{make_float4(fmaf(y1[j].x, w1, y0[j].x * w0), fmaf(y1[j].y, w1, y0[j].y * w0),
-                                   fmaf(y1[j].z, w1, y0[j].z * w0), fmaf(y1[j].w, w1, y0[j].w * w0)),
-                       fmaf(m1.y, w1, m0.y * w0), top};
-        join_store<D, DT>(p, t, h, ch + 4 * j, s, gate[j]);
+      const int step = p.own_rows * (D / 4);
+      const float4* from = o + ch * p.own_rows;
+#pragma unroll 1
+      for (int j = 0; j < 4; j += 2, ch += 8, from += 8 * p.own_rows) {
+        const float4 y0 = from[0], y1 = from[step], y2 = from[4 * p.own_rows], y3 = from[4 * p.own_rows + step];
+        const uint4 g0 = join_gate(p, t, h, ch), g1 = join_gate(p, t, h, ch + 4);
+        RowSum s{make_float4(fmaf(y1.x, w1, y0.x * w0), fmaf(y1.y, w1, y0.y * w0), fmaf(y1.z, w1, y0.z * w0),
+                             fmaf(y1.w, w1, y0.w * w0)),
+                 fmaf(m1.y, w1, m0.y * w0), top};
+        join_store<D, DT>(p, t, h, ch, s, g0);
+        s.o = make_float4(fmaf(y3.x, w1, y2.x * w0), fmaf(y3.y, w1, y2.y * w0), fmaf(y3.z, w1, y2.z * w0),
+                          fmaf(y3.w, w1, y2.w * w0));
+        join_store<D, DT>(p, t, h, ch + 4, s, g1);
       }
       continue;
     }
 #pragma unroll 1
     for (int j = 0; j < 4; ++j, ch += 4) {
       const uint4 gate = join_gate(p, t, h, ch);
-      join_store<D, DT>(p, t, h, ch, join_segments<D>(ml, o, ml, o + ch * p.own_rows, p.own_rows, 0, n, 0, 1), gate);
+      join_store<D, DT>(p, t, h, ch, join_segments<D, 4>(ml, o, ml, o + ch * p.own_rows, p.own_rows, 0, n, 0, 1), gate);
     }
   }
 }
@@ -1542,11 +1541,12 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
     }
   }
   const int n = live ? n_pre + n_own : 0;
+  own_ml -= (int64_t)n_pre * p.own_rows, own_o -= (int64_t)n_pre * p.own_rows * (D / 4);
   if (split == 1 && !live) return;
 #pragma unroll 1
   for (int j = 0; j < p.join_span; ++j, ch += 4, pre_o += 4 * 2 * PA_ROWS, own_o += 4 * p.own_rows) {
     const uint4 gate = live ? join_gate(p, t, h, ch) : make_uint4(0, 0, 0, 0);
-    RowSum s = join_segments<D>(pre_ml, pre_o, own_ml, own_o, p.own_rows, n_pre, n, part, split);
+    RowSum s = join_segments<D, 8>(pre_ml, pre_o, own_ml, own_o, p.own_rows, n_pre, n, part, split);
     if (split > 1) {  // the parts of the row's segments, in order
       float(&mine)[6][32] = joined[warp];
       mine[0][lane] = s.top, mine[1][lane] = s.den;
