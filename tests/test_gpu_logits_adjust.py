@@ -155,3 +155,31 @@ def test_history_longer_than_its_width_is_reported(cuda):
                     history_lens=torch.tensor([5], dtype=torch.int32, device=cuda),
                     presence=torch.ones(1, device=cuda))
     assert Y.status() == Y.EINVAL
+
+
+@pytest.mark.parametrize("rep", [0.5, 1.0, 1.3, 3.0, 1e-39, 1e-45, 1e-30, 2.0 ** -126, 2.0 ** 127, 3e38, 0.0, -0.7, np.inf])
+@pytest.mark.parametrize("wide", [False, True])
+def test_penalties_of_every_size_round_as_the_division(cuda, rep, wide):
+    """Infinities, NaN, the largest, the subnormal and bit patterns at random: binary32's quotient and
+    product, bit for bit (each step is rounded once, so nothing may differ)."""
+    import torch
+    import yskn_b200 as Y
+    rng = np.random.default_rng(11)
+    V = 4099
+    x = rng.integers(0, 2 ** 32, V, dtype=np.uint64).astype(np.uint32).view(np.float32)
+    x[:12] = [3e38, -3e38, 3.4028235e38, np.inf, -np.inf, np.nan, 0.0, -0.0, 1e-45, 1.1754944e-38, -1e-39, 1.0]
+    x[12:1000] = rng.standard_normal(988).astype(np.float32) * 4
+    rep = np.float32(rep)
+    L = 40000 if wide else V  # counts of 32 bits, or of 16
+    hist = np.resize(np.arange(V, dtype=np.int32), (1, L))
+    dev = lambda a: torch.from_numpy(a).to(cuda)  # noqa: E731
+    out = torch.empty((1, V), device=cuda)
+    Y.logits_adjust(dev(x[None]), out, history=dev(hist), history_lens=dev(np.array([L], np.int32)),
+                    prompt_lens=dev(np.array([L], np.int32)), repetition=dev(np.array([rep])))
+    with np.errstate(all="ignore"):
+        exp = np.where(x > 0, x / rep, x * rep)
+    got = out.cpu().numpy()[0]
+    assert Y.status() == 0
+    assert np.array_equal(np.isnan(got), np.isnan(exp))
+    bits = ~np.isnan(exp)
+    assert np.array_equal(got.view(np.uint32)[bits], exp.view(np.uint32)[bits])

@@ -20,9 +20,7 @@
 // 255 us; 16-byte accesses, counting and streaming in turn in four CTAs an SM 114; this way
 // 81. Streaming a plain copy and adjusting the history's logits afterwards took 141: two
 // million scattered 4-byte updates.) Some of nearly every 128 neighbouring tokens are in a
-// long history, so the penalties run for nearly every warp: the quotient is the product
-// with the reciprocal, corrected by its residual (one Newton step, Markstein 1990), which rounds
-// as the division.
+// long history, so the penalties run for nearly every warp: no division among them (Penalties).
 // A token's count: the top bit for a token of the prompt, the others the count after it, so that
 // a token is seen if it is not zero. Histories shorter than 32768 are counted in 16 bits (two
 // counts a word), longer ones in 32: a chunk may be as large as its counts allow, because every
@@ -98,12 +96,21 @@ struct LogitsCount {
   static constexpr uint32_t PROMPT = 1u << (BITS - 1), ALL = PROMPT | (PROMPT - 1);
 };
 
+// The quotient by the repetition penalty is the binary64 product with its binary64 reciprocal, rounded:
+// off by 2^-52 of itself before that, and a quotient of two 24-bit numbers that is normal in binary32
+// lies 2^-49 of itself or more from where binary32's rounding turns, so this is the division's result;
+// infinities, overflow and penalties of any size included. A subnormal quotient half way between two
+// numbers may fall on the other one. (256 rows of 151936: 81.5 us; the division where binary32's
+// product and one Newton step do not hold, as a rare branch, 98.)
 struct Penalties {
-  float rep, inv, pres, freq;
+  float rep, pres, freq;
+  double inv;
+  __device__ void repeated(float r) {
+    rep = r;
+    inv = 1.0 / (double)r;
+  }
   __device__ float operator()(float x, uint32_t count, uint32_t prompt) const {
-    const float q = __fmul_rn(x, inv), rest = fmaf(-q, rep, x);
-    const float quotient = rest == rest ? fmaf(rest, inv, q) : q;  // without a residual (infinities): as it is
-    float y = x > 0.0f ? quotient : __fmul_rn(x, rep);
+    float y = x > 0.0f ? (float)((double)x * inv) : __fmul_rn(x, rep);
     const float c = (float)(count & (prompt - 1));
     y = c > 0.0f ? __fsub_rn(__fsub_rn(y, __fmul_rn(freq, c)), pres) : y;
     return count ? y : x;
@@ -202,8 +209,8 @@ __global__ void __launch_bounds__(LA_THREADS) logits_adjust_kernel(const __grid_
     int k = 0;
     for (int item = blockIdx.x; item < items; item += step, ++k) {
       const LogitsItem it(p, item);
-      Penalties pen{1.0f, 1.0f, 0.0f, 0.0f};
-      if (p.repetition) pen.rep = __ldg(p.repetition + it.m), pen.inv = __fdiv_rn(1.0f, pen.rep);
+      Penalties pen{1.0f, 0.0f, 0.0f, 1.0};
+      if (p.repetition) pen.repeated(__ldg(p.repetition + it.m));
       if (p.presence) pen.pres = __ldg(p.presence + it.m);
       if (p.frequency) pen.freq = __ldg(p.frequency + it.m);
       la_stream<Count>(it, counts_of(k), pen, counted, [&]() {
