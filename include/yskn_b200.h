@@ -646,7 +646,8 @@ YSKN_B200_API int yskn_b200_paged_prep(const yskn_b200_paged_prep_args* args, vo
  * int32 [ceil(prefix_len / block_size)], from there on in the request's row of
  * block_tables. out = softmax(scale * q k^T) v in binary32 sums, times sigmoid(gate) if
  * gate is given, rounded once; a token that sees nothing, padding included, gives zeros.
- * Cache rows that no token sees may hold anything. q, gate: element (token, head, channel)
+ * Cache rows that no token sees may hold anything; one that some token of a request sees holds numbers
+ * (for the tokens that do not see it its weight is zero, and zero times infinity is NaN). q, gate: element (token, head, channel)
  * at token * row + head * head_stride + channel; out dense [tokens][n_qh][head]; query head
  * j reads KV head j / (n_qh / n_kvh), at most 128 query heads each. dtype YSKN_DT_F16 or
  * _BF16 for all of them (the softmax weights are rounded to it for the tensor cores), gate_dtype

@@ -255,3 +255,81 @@ def test_more_tokens_than_promised_are_reported(cuda):
     run(cuda, new=(3, 200), own=(20, 200), max_new=1, check=False)
     assert Y.status() == Y.EINVAL
     run(cuda, new=(3, 2), own=(20, 20), seed=1)
+
+
+def call(cuda, new, lens, P, fill, n_qh=6, n_kvh=2, D=128, block=16, gate=None, seed=0):
+    """A bf16 call without a wrapper around it: q, the rows of each request ([len][n_kvh][D] K and V), out and
+    the starts. Cache rows that no token sees hold `fill`, those of the prefix too."""
+    import torch
+    import yskn_b200 as Y
+    g = torch.Generator(device=cuda)
+    g.manual_seed(seed)
+    B, T, pre = len(new), sum(new), -(-P // block)
+    seen = [n if k else 0 for n, k in zip(lens, new)]
+    held = [-(-max(n - P, 0) // block) for n in lens]
+    n_blocks = pre + sum(held) + 1
+    kc, vc = (torch.full((n_blocks, block, n_kvh, D), fill, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    numbers = torch.randperm(n_blocks, generator=g, device=cuda).to(torch.int32)
+    tables = torch.full((B, max(held + [1])), -1, dtype=torch.int32, device=cuda)
+
+    def put(cache, blocks, n):
+        x = torch.randn((n, n_kvh, D), generator=g, device=cuda).to(torch.bfloat16)
+        j = torch.arange(n, device=cuda)
+        cache[blocks.long()[j // block], j % block] = x
+        return x
+
+    prefix, at, rows = [put(c, numbers, min(P, max(seen + [0]))) for c in (kc, vc)], pre, []
+    for i in range(B):
+        tables[i, :held[i]] = numbers[at:at + held[i]]
+        at += held[i]
+        rows.append([torch.cat([a, put(c, tables[i], max(seen[i] - P, 0))]) for a, c in zip(prefix, (kc, vc))])
+    q = (torch.randn((T, n_qh, D), generator=g, device=cuda) * 1.5).to(torch.bfloat16)
+    starts = np.concatenate([[0], np.cumsum(new)]).tolist()
+    i32 = lambda a: torch.tensor(list(map(int, a)), dtype=torch.int32, device=cuda)  # noqa: E731
+    work = torch.full((Y.prefix_attention_work_bytes(T, B, max(new), n_qh, n_kvh, D),), 255, dtype=torch.uint8,
+                      device=cuda)
+    out = torch.full((T, n_qh, D), 3.0, dtype=torch.bfloat16, device=cuda)
+    Y.prefix_attention(q, kc, vc, tables, i32(lens), i32(starts), max(new), work, out, prefix_blocks=numbers[:pre],
+                       prefix_len=P, gate=gate)
+    return q, rows, out, starts
+
+
+def near(q, rows, out, starts, new, lens):
+    """The bound at the top of the file, for bf16 without a gate."""
+    import torch
+    n_qh, D, u = q.shape[1], q.shape[2], 2.0 ** -8
+    for i, (k, v) in enumerate(rows):
+        for t in range(new[i]):
+            lim, tok = max(0, lens[i] - new[i] + t + 1), starts[i] + t
+            if lim == 0:
+                assert bool((out[tok] == 0).all()), (i, t)
+                continue
+            kd, vd = (x[:lim].double().repeat_interleave(n_qh // x.shape[1], 1) for x in (k, v))
+            qd = q[tok].double()
+            w = torch.softmax(torch.einsum("hd,lhd->hl", qd, kd) * D ** -0.5, -1)
+            y, A = torch.einsum("hl,lhd->hd", w, vd), torch.einsum("hl,lhd->hd", w, vd.abs())
+            e = 2.0 ** -22 * D ** 0.5 * torch.einsum("hd,lhd->hl", qd.abs(), kd.abs()).amax(-1)[:, None]
+            tol = (u + 2 * e + 2.0 ** -23 * lim + 2.0 ** -21) * A + u * y.abs() + 2.0 ** -25
+            assert bool(((out[tok].double() - y).abs() <= tol).all()), (i, t)
+
+
+UNSEEN = [  # new tokens, lengths and prefix: requests that end inside the prefix
+    ((1, 1, 1), (30, 100, 1), 200),  # few rows a head: each request by itself
+    ((1,) * 40, tuple(300 + 7 * i for i in range(40)), 5000),  # beside prefix items
+    ((4,) * 40, tuple(300 + 7 * i for i in range(40)), 5000),  # many rows, prefix items
+    ((150, 0, 90), (330, 900, 140), 700),  # each request by itself, an idle one sees no row
+    ((2, 3), (1, 0), 100),  # tokens that see nothing
+]
+
+
+@pytest.mark.parametrize("fill", [float("nan"), float("inf")])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("case", range(len(UNSEEN)))
+def test_prefix_rows_that_no_token_sees_hold_anything(cuda, case, D, fill):
+    import torch
+    import yskn_b200 as Y
+    new, lens, P = UNSEEN[case]
+    q, rows, out, starts = call(cuda, new, lens, P, fill, D=D, seed=case)
+    assert Y.status() == 0
+    near(q, rows, out, starts, new, lens)
+    assert torch.equal(out, call(cuda, new, lens, P, 0.0, D=D, seed=case)[2])

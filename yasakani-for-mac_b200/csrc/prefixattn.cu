@@ -6,7 +6,9 @@
 // prefix's blocks, the others in the request's. Per query head, in binary32:
 //   s_j = scale * <q, k_j>, out = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s)
 //   out *= 1 / (1 + exp(-gate))  (with a gate), rounded once. A token that sees nothing gives 0.
-// Rows at or past lim are not read into any sum, whatever the cache holds there.
+// Rows that no token of the call sees are not read into any sum, whatever the cache holds there: the
+// prefix's tiles end at the longest length, an own item's at its last token. (A row that some token of
+// an item sees has weight zero for the others, and so has to hold a number for them.)
 //
 // The softmax over all rows is the join of softmaxes over parts: with a part's maximum m,
 // l = sum exp(s - m) and o = sum exp(s - m) v, parts join as sum exp(m - M) o / sum
@@ -143,11 +145,11 @@ struct PrefixAttnParams {
   int batch, tokens, max_new, n_kvh, G;
   int tpc, tpi;  // tokens per CTA and per item
   unsigned g_magic, tpi_magic;  // ceil(2^32 / d): quotients of numbers below 2^32 / d
-  int pre_tiles, pre_qtiles, shared_items;  // prefix items, if there are any
-  // Own items: thin ones (below) or not, the rows of a tile as a power of two, the prefix's tiles
-  // where an own item takes them, and an item's fixed cost in tiles.
+  int pre_qtiles, shared_items;  // prefix items, if there are any
+  // Own items: thin ones (below) or not, the rows of a tile as a power of two, and an item's fixed
+  // cost in tiles.
   bool thin;
-  int tile_shift, own_pre, item_cost;
+  int tile_shift, item_cost;
   const uint16_t *q, *k_cache, *v_cache;  // thin items read them by address
   int64_t q_row, q_head;
   CacheStrides cache;
@@ -155,7 +157,7 @@ struct PrefixAttnParams {
   int join_span, join_split;  // 16-channel parts of a row that a warp of the join takes; warps for one part
   float c;     // |scale| log2 e
   uint32_t negate_q;
-  int4* work_per;         // for the join: units per pair of prefix items and of own ones, whether alone, own units
+  int4* work_per;  // for the join: units per pair of prefix items and of own ones, prefix tiles (-1: alone), own units
   int2* work_base;        // [batch] own items, and units of all items, before each request's own
   // per place: (m, l) of each row; o as [D / 4][rows][4], so that a warp's rows are adjacent
   float2 *pre_ml, *own_ml;
@@ -204,8 +206,9 @@ __device__ __forceinline__ PaRequest pa_request(const PrefixAttnParams& p, int i
 __device__ __forceinline__ int pa_visible(const PrefixAttnParams& p, const PaRequest& r, int upto) {
   return min(max(r.len - r.n + upto - p.prefix_len, 0), p.own_limit);
 }
-__device__ __forceinline__ int pa_own_tiles(const PrefixAttnParams& p, const PaRequest& r, int qt) {
-  return (pa_visible(p, r, min(r.n, (qt + 1) * p.tpi)) + (1 << p.tile_shift) - 1) >> p.tile_shift;
+// Rows of the prefix that it sees.
+__device__ __forceinline__ int pa_visible_prefix(const PrefixAttnParams& p, const PaRequest& r, int upto) {
+  return min(max(r.len - r.n + upto, 0), p.prefix_len);
 }
 // Units of an item of so many tiles (0: nothing to do): unit u is tile u - cost; or the whole
 // item is one unit.
@@ -217,7 +220,9 @@ __device__ __forceinline__ int pa_qtiles(const PrefixAttnParams& p, const PaRequ
 }
 // Tiles of a request's item `qt`: own ones, after the prefix's where there are no prefix items.
 __device__ __forceinline__ int pa_tiles(const PrefixAttnParams& p, const PaRequest& r, int qt, bool alone) {
-  return pa_own_tiles(p, r, qt) + (alone ? p.own_pre : 0);
+  const int upto = min(r.n, (qt + 1) * p.tpi), up = (1 << p.tile_shift) - 1;
+  const int own = (pa_visible(p, r, upto) + up) >> p.tile_shift;
+  return alone ? own + ((pa_visible_prefix(p, r, upto) + up) >> p.tile_shift) : own;
 }
 // Units of a request's items of one KV head; sums of units stop at PA_MANY, which is an error.
 constexpr unsigned PA_MANY = 1u << 30;
@@ -235,11 +240,14 @@ struct PaSegment {
   int pre;              // the item's first tiles that are the prefix's
   int key0, key1;       // key tiles [key0, key1)
   int keys;             // own rows that any of its tokens sees
-  int first;            // own items: rows of the sequence that token tok0 sees
+  int first;            // rows of the sequence that token tok0 sees, one more for each token (prefix
+                        // items: as if its last token saw what the longest request does)
   int64_t place;        // of its partial result
+  // Rows of the prefix that any of its tokens sees.
+  __device__ int pre_keys(const PrefixAttnParams& p) const { return min(first + ntok - 1, p.prefix_len); }
   // Rows of tile kt that the rows on its axis leave it.
   __device__ int rows_of(const PrefixAttnParams& p, int kt) const {
-    return min(PA_KEYS, kt < pre ? p.prefix_len - kt * PA_KEYS : keys - (kt - pre) * PA_KEYS);
+    return min(PA_KEYS, kt < pre ? pre_keys(p) - kt * PA_KEYS : keys - (kt - pre) * PA_KEYS);
   }
 };
 
@@ -249,6 +257,7 @@ struct PaStart {
   bool thin;         // the latter
   int left;          // its units
   int alone;         // no prefix items: each request's items take the prefix too
+  int pre_seen;      // rows of the prefix that any token of the call sees
   int pre_item, u0;  // prefix item and unit in it
   int req, item;     // own items: request and the items before it
   int skip;          // units of the request before this pair's first
@@ -258,13 +267,13 @@ struct PaStart {
 struct PaWalk {
   const PrefixAttnParams& p;
   const bool alone;
-  const int who;
+  const int who, pre_seen;
   int left, pre_item, u0, req, item, kvh, qt;
   PaRequest r;
   int nq;
   bool loaded;
   __device__ PaWalk(const PrefixAttnParams& p_, const PaStart& s)
-      : p(p_), alone(s.alone), who(s.who), left(s.left), pre_item(s.pre_item), u0(s.u0), req(s.req), item(s.item),
+      : p(p_), alone(s.alone), who(s.who), pre_seen(s.pre_seen), left(s.left), pre_item(s.pre_item), u0(s.u0), req(s.req), item(s.item),
         kvh(0), qt(0), r{}, nq(0), loaded(false) {
     if (s.skip > 0) {
       load();
@@ -292,11 +301,11 @@ struct PaWalk {
       s.tok0 = (pre_item - s.kvh * p.pre_qtiles) * p.tpi;
       s.ntok = min(p.tpi, p.tokens - s.tok0);
       s.req = 0;
-      s.pre = p.pre_tiles;
+      s.pre = (pre_seen + PA_KEYS - 1) / PA_KEYS;
       s.keys = 0;
-      s.first = 0;
+      s.first = pre_seen - s.ntok + 1;
       ++pre_item;
-      if (take(s, p.pre_tiles, pre_item - 1)) return true;
+      if (take(s, s.pre, pre_item - 1)) return true;
     }
     while (left > 0 && req < p.batch) {
       if (!loaded) load();
@@ -309,8 +318,8 @@ struct PaWalk {
           s.tok0 = r.s0 + q * p.tpi;
           s.ntok = min(p.tpi, r.n - q * p.tpi);
           s.req = req;
-          s.pre = alone ? p.own_pre : 0;
           s.keys = pa_visible(p, r, q * p.tpi + s.ntok);
+          s.pre = kt - ((s.keys + (1 << p.tile_shift) - 1) >> p.tile_shift);
           s.first = r.len - r.n + q * p.tpi + 1;
           if (take(s, kt, item + kvh * nq + q)) return true;
           if (left <= 0) return false;
@@ -328,7 +337,7 @@ struct PaWalk {
     const int n = p.whole ? 1 : min(tiles + cost - u0, left);
     s.key0 = p.whole ? 0 : max(u0 - cost, 0);
     s.key1 = p.whole ? tiles : max(u0 + n - cost, 0);
-    s.whole = !s.prefix && s.key0 == 0 && s.key1 == tiles && s.pre == p.own_pre;
+    s.whole = !s.prefix && s.key0 == 0 && s.key1 == tiles && alone;
     s.place = (int64_t)it + who;
     left -= n;
     u0 = 0;
@@ -576,7 +585,7 @@ struct ThinCursor {
     if (!live) return;
     const int at = (kt < seg.pre ? kt : kt - seg.pre) << PA_THIN_SHIFT;
     if ((unsigned)block < (unsigned)p.n_blocks) {
-      rows = min(1 << PA_THIN_SHIFT, (kt < seg.pre ? p.prefix_len : seg.keys) - at);
+      rows = min(1 << PA_THIN_SHIFT, (kt < seg.pre ? seg.pre_keys(p) : seg.keys) - at);
       const int64_t from = block * p.cache.block + (at & ((1 << p.block_shift) - 1)) * p.cache.token +
                            seg.kvh * p.cache.head;
       k += from, v += from;
@@ -777,7 +786,7 @@ struct PaShared {
   uint32_t tmem_slot;
   int abort_word;
   PaStart start[PA_THIN_WARPS];  // of the pair's walk (all alike), or of each warp's
-  uint3 sum[PA_THREADS / 32];
+  uint4 sum[PA_THREADS / 32];
   float half[2][2][PA_ROWS];  // tile parity, half, row: what a row's halves exchange
 };
 static_assert(sizeof(PaShared) <= 3072, "shared memory beside the ring");
@@ -827,7 +836,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
   {
     const int per = p.batch <= PA_THREADS ? 1 : (p.batch + PA_THREADS - 1) / PA_THREADS;
     const int i0 = min(p.batch, tid * per), i1 = min(p.batch, i0 + per);
-    unsigned items = 0, units_of[2] = {0, 0};  // beside prefix items, and alone
+    unsigned items = 0, units_of[2] = {0, 0}, seen = 0;  // beside prefix items, and alone; of the prefix
     for (int i = i0; i < i1; ++i) {
       const PaRequest r = pa_request(p, i);
       const int nq = pa_qtiles(p, r);
@@ -835,6 +844,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
       units_of[0] = pa_sum(units_of[0], times(pa_own_units(p, r, nq, false)));
       units_of[1] = pa_sum(units_of[1], times(pa_own_units(p, r, nq, true)));
       items = pa_sum(items, times(nq));
+      if (r.n > 0) seen = max(seen, (unsigned)pa_visible_prefix(p, r, r.n));
       if (blockIdx.x == 0 && (__ldg(p.starts + i + 1) - r.s0 != r.n)) raise_device_error(p.err, DERR_RANGE);
     }
     unsigned ui[2] = {units_of[0], units_of[1]}, it = items;
@@ -844,12 +854,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
       const unsigned c = __shfl_up_sync(0xffffffffu, it, off);
       if (lane >= off) ui[0] = pa_sum(ui[0], a), ui[1] = pa_sum(ui[1], b), it = pa_sum(it, c);
     }
-    if (lane == 31) sh.sum[warp] = make_uint3(ui[0], ui[1], it);
+    seen = __reduce_max_sync(0xffffffffu, seen);
+    if (lane == 31) sh.sum[warp] = make_uint4(ui[0], ui[1], it, seen);
     __syncthreads();
     unsigned before_of[2] = {0, 0}, total_of[2] = {0, 0}, items_before = 0, total_items = 0;
     const int used = per == 1 ? p.batch : PA_THREADS;  // threads with requests
     for (int w = 0; w * 32 < used; ++w) {
-      const uint3 o = sh.sum[w];
+      const uint4 o = sh.sum[w];
+      seen = max(seen, o.w);
       if (w < warp) {
         before_of[0] = pa_sum(before_of[0], o.x);
         before_of[1] = pa_sum(before_of[1], o.y);
@@ -861,7 +873,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
     }
     // Alone, if that is at most an eighth more: about what the join of two results per row costs
     // (16 prompt chunks: 960 us with prefix items, 850 alone, at the step that added it).
-    const int pre_units = pa_units(p.pre_tiles, false, PA_ITEM_COST);
+    const int pre_tiles = (int)(seen + PA_KEYS - 1) / PA_KEYS, pre_units = pa_units(pre_tiles, false, PA_ITEM_COST);
     const int pre_all = p.shared_items * pre_units;  // below 2^30: the host looked
     const unsigned long long pre_time = (unsigned long long)pre_all * (p.thin ? PA_THIN_PER_TILE : 1);
     const bool alone = p.whole || p.shared_items == 0 ||
@@ -896,14 +908,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
     if (tid < PA_THIN_WARPS) {
       const int who = who0 + (thin ? tid * ctas : 0), share = thin ? share_own : share_pre;
       const int all = thin ? own : p.thin ? pre : pre + own, t0 = min(all, who * share);
-      PaStart s{who, thin, min(all, t0 + share) - t0, alone, pre_items, 0, p.thin && !thin ? p.batch : 0, 0, 0};
+      PaStart s{who,       thin, min(all, t0 + share) - t0,        alone, (int)seen,
+                pre_items, 0,    p.thin && !thin ? p.batch : 0, 0,     0};
       if (!thin && t0 < pre) {
         s.pre_item = t0 / pre_units;
         s.u0 = t0 - s.pre_item * pre_units;
       }
       sh.start[tid] = s;
       if (blockIdx.x == 0 && tid == 0) {
-        *p.work_per = make_int4(share_pre, share_own, alone, own);
+        *p.work_per = make_int4(share_pre, share_own, alone ? -1 : pre_tiles, own);
         if (!sound) raise_device_error(p.err, DERR_RANGE);
       }
     }
@@ -1496,7 +1509,7 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
   bool live = t < p.tokens;
   pdl_begin();
   const int4 how = *p.work_per;
-  const bool alone = how.z;
+  const bool alone = how.z < 0;
   // one token for each request is the common case: its request's numbers are asked for at once
   int i = t;
   PaRequest r{-1, 0, 0};
@@ -1532,8 +1545,8 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
     if (n_own == 1 && alone) live = false;  // finished where it was computed
     if (!alone) {
       const int qt = pa_quotient(t, p.tpi_magic), it = kvh * p.pre_qtiles + qt, tl = t - qt * p.tpi, rank = tl >= p.tpc;
-      const int b = it * pa_units(p.pre_tiles, false, PA_ITEM_COST) + PA_ITEM_COST, c0 = pair_of(b, how.x);
-      n_pre = pair_of(b + p.pre_tiles - 1, how.x) - c0 + 1;
+      const int b = it * pa_units(how.z, false, PA_ITEM_COST) + PA_ITEM_COST, c0 = pair_of(b, how.x);
+      n_pre = pair_of(b + how.z - 1, how.x) - c0 + 1;
       const int64_t at = (int64_t)(it + c0) * (2 * PA_ROWS);
       const int row = rank * PA_ROWS + (tl - rank * p.tpc) * p.G + gh;
       pre_ml = p.pre_ml + at + row;
@@ -1659,9 +1672,10 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   p.tpc = tpc, p.tpi = 2 * tpc;
   auto magic = [](int d) { return d == 1 ? 0u : (unsigned)(((1ull << 32) + d - 1) / d); };
   p.g_magic = magic(G), p.tpi_magic = magic(p.tpi);
-  p.pre_tiles = (int)ceil_div(a.prefix_len, PA_KEYS), p.pre_qtiles = (int)ceil_div(a.tokens, 2 * tpc);
+  const int pre_tiles = (int)ceil_div(a.prefix_len, PA_KEYS);  // at most: where a request sees the whole prefix
+  p.pre_qtiles = (int)ceil_div(a.tokens, 2 * tpc);
   const int64_t items = (int64_t)p.pre_qtiles * n_kvh;
-  if (items * pa_units(p.pre_tiles, false, PA_ITEM_COST) >= (int64_t)PA_MANY ||
+  if (items * pa_units(pre_tiles, false, PA_ITEM_COST) >= (int64_t)PA_MANY ||
       (int64_t)a.tokens * n_qh * head > INT32_MAX || a.tokens >= 1 << 24 || n_kvh > 65535)
     return fail(YSKN_EINVAL, "prefix_attention: too much work");
   p.shared_items = a.prefix_len > 0 ? (int)items : 0;
@@ -1671,9 +1685,8 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   // and 12.1, 16.1, with 128 15.7, 13.8 (12.2 since a warp's least is 2 units).
   p.thin = G * a.max_new <= PA_THIN_ROWS && pairs > 1;
   p.tile_shift = p.thin ? PA_THIN_SHIFT : 7;
-  p.own_pre = (int)ceil_div(a.prefix_len, 1 << p.tile_shift);
   p.item_cost = p.thin ? PA_THIN_COST : PA_ITEM_COST;
-  const int64_t most_tiles = p.own_pre + ceil_div(p.own_limit, 1 << p.tile_shift);
+  const int64_t most_tiles = ceil_div(a.prefix_len, 1 << p.tile_shift) + ceil_div(p.own_limit, 1 << p.tile_shift);
   p.whole = p.thin ? w.own_items <= 2 * PA_THIN_WARPS * pairs && most_tiles <= PA_THIN_WHOLE
                    : w.own_items <= pairs && most_tiles <= PA_WHOLE_TILES;
   p.many_per_head = PA_MANY / (unsigned)n_kvh;
