@@ -128,3 +128,26 @@ def test_tensor_checks_of_the_binding():
     refused(Y.logits_adjust, x, x, bias=f32(2, 3), bias_ids=i32(2, 4))
     refused(Y.logits_adjust, x, x, mask=i32(1, 2))
     refused(Y.logits_adjust, f32(50, 2).t(), x)
+
+
+@pytest.mark.parametrize("name,last", [("batch_plan", "max_tokens"), ("paged_prep", "axes"),
+                                       ("prefix_attention", "scale"), ("logits_adjust", "n_bias")])
+def test_packed_arguments_are_the_whole_struct(tmp_path, name, last):
+    """The library copies the struct whole: its padding at the end has to be there too."""
+    import os
+    import shutil
+    import struct
+    import subprocess
+    import yskn_b200 as Y
+    from conftest import ROOT
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    src, exe = tmp_path / "s.c", tmp_path / "s"
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "yskn_b200.h"\nint main(void) { printf("%%zu %%zu", '
+                   'sizeof(yskn_b200_%s_args), offsetof(yskn_b200_%s_args, %s)); return 0; }' % (name, name, last))
+    subprocess.run([cc, "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    size, at = map(int, subprocess.run([str(exe)], capture_output=True, check=True).stdout.split())
+    assert Y.ARGS[name].size == size
+    unpadded = Y.ARGS[name].format.replace("0P", "")
+    assert struct.calcsize(unpadded) - (128 if last == "axes" else 4) == at

@@ -670,12 +670,13 @@ def kv_encode(rows, row_group, tables, gains, mults, kb, vit2, words, scales, me
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2
 
 # The batch operators take a struct of arguments (yskn_b200_*_args, in the header's order); packing
-# one is ten times faster than converting as many ctypes arguments.
+# one is ten times faster than converting as many ctypes arguments. The library reads the whole of it,
+# so a format ends with the padding that C adds (0P: up to a pointer's alignment).
 ARGS = {
-    "batch_plan": struct.Struct("@3PqPP3P3P6i"),
-    "paged_prep": struct.Struct("@3P6q2PqP2P3P3q10if128s"),
-    "prefix_attention": struct.Struct("@P2qP2q2P3q2Pq2PPqP12if"),
-    "logits_adjust": struct.Struct("@PqPq2P3P2PPqPq4i"),
+    "batch_plan": struct.Struct("@3PqPP3P3P6i0P"),
+    "paged_prep": struct.Struct("@3P6q2PqP2P3P3q10if128s0P"),
+    "prefix_attention": struct.Struct("@P2qP2q2P3q2Pq2PPqP12if0P"),
+    "logits_adjust": struct.Struct("@PqPq2P3P2PPqPq4i0P"),
 }
 _DT, _FN = {}, {}
 
