@@ -151,3 +151,54 @@ def test_packed_arguments_are_the_whole_struct(tmp_path, name, last):
     assert Y.ARGS[name].size == size
     unpadded = Y.ARGS[name].format.replace("0P", "")
     assert struct.calcsize(unpadded) - (128 if last == "axes" else 4) == at
+
+
+def test_arrays_that_the_library_reads_by_address_alone():
+    """Types, lengths and strides of the arrays whose layout the C entry takes for granted."""
+    import torch
+    import yskn_b200 as Y
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    i64 = lambda *s: torch.zeros(s, dtype=torch.int64)  # noqa: E731
+    bf = lambda *s: torch.zeros(s, dtype=torch.bfloat16)  # noqa: E731
+    f32 = lambda *s: torch.zeros(s)  # noqa: E731
+    every_second = lambda t: torch.stack([t, t], -1)[..., 0]  # noqa: E731
+
+    class Stream:
+        cuda_stream = 0
+
+    def refused(what, fn, good, **change):
+        args = dict(good, **change)
+        with pytest.raises(Y.YsknError, match=what) as e:
+            fn(stream=Stream, **args)
+        assert e.value.code == Y.EINVAL
+
+    plan = dict(lens=i32(2), new_lens=i32(2), block_tables=i32(2, 3), pool=i32(4), free_count=i32(1), block_size=16,
+                lens_out=i32(2), free_out=i32(1), starts=i32(3), slots=i64(4), positions=i32(4), requests=i32(4))
+    for k, v in plan.items():
+        if k not in ("block_tables", "block_size"):
+            if v.numel() > 1:
+                refused("^batch_plan: ", Y.batch_plan, plan, **{k: every_second(v)})
+            refused("^batch_plan: ", Y.batch_plan, plan, **{k: v.to(torch.float64 if k == "slots" else torch.float32)})
+    refused("^batch_plan: ", Y.batch_plan, plan, free_count=i32(0))
+
+    c = bf(5, 16, 2, 64)
+    prep = dict(q=f32(3, 4, 64), k=f32(3, 2, 64), v=f32(3, 2, 64), slots=i64(3), positions=i32(3), query=bf(3, 4, 64),
+                k_cache=c, v_cache=c, inv_freq=f32(16), q_norm=bf(64), k_norm=bf(64))
+    refused("slots", Y.paged_prep, prep, slots=f32(3).double())
+    refused("slots", Y.paged_prep, prep, slots=every_second(i64(3)))
+    for bad in (f32(64), bf(32), bf(128), every_second(bf(64)), torch.zeros(64, dtype=torch.float16)):
+        refused("norms", Y.paged_prep, prep, q_norm=bad)
+        refused("norms", Y.paged_prep, prep, k_norm=bad)
+    for bad in (f32(16).double(), bf(16), every_second(f32(16))):
+        refused("frequency|f32", Y.paged_prep, prep, inv_freq=bad)
+
+    att = dict(q=bf(3, 4, 64), k_cache=c, v_cache=c, block_tables=i32(2, 3), lens=i32(2), starts=i32(3), max_new=2,
+               work=torch.zeros(1 << 24, dtype=torch.uint8), out=bf(3, 4, 64), prefix_blocks=i32(2), prefix_len=20)
+    for k in ("lens", "starts", "prefix_blocks", "work"):
+        refused("prefix_attention: dense", Y.prefix_attention, att, **{k: every_second(att[k])})
+
+    adjust = dict(logits=f32(2, 50), out=f32(2, 50), history=i32(2, 4), history_lens=i32(2), prompt_lens=i32(2),
+                  repetition=f32(2), presence=f32(2), frequency=f32(2))
+    for k in ("history_lens", "prompt_lens", "repetition", "presence", "frequency"):
+        refused("logits_adjust: a dense", Y.logits_adjust, adjust, **{k: every_second(adjust[k])})
+        refused("logits_adjust: a dense", Y.logits_adjust, adjust, **{k: adjust[k].double()})

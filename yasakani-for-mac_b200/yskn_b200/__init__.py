@@ -684,7 +684,7 @@ _DT, _FN = {}, {}
 def _types():
     import torch
     _DT.update({torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.int16: DT_BF16})
-    _DT["i32"] = torch.int32
+    _DT["i32"], _DT["i64"] = torch.int32, torch.int64
     # the raw handle at once: building a torch.cuda.Stream object around it takes longer than a launch
     _DT["stream"] = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
         lambda device: torch.cuda.current_stream(device).cuda_stream)
@@ -727,10 +727,12 @@ def batch_plan(lens, new_lens, block_tables, pool, free_count, block_size, lens_
     T, row = slots.numel(), block_tables.stride()
     _need(lens.dtype is i32 and new_lens.dtype is i32 and block_tables.dtype is i32 and pool.dtype is i32 and
           free_count.dtype is i32 and lens_out.dtype is i32 and free_out.dtype is i32 and starts.dtype is i32 and
-          positions.dtype is i32 and requests.dtype is i32 and slots.element_size() == 8 and lens.numel() == B and
+          positions.dtype is i32 and requests.dtype is i32 and slots.dtype is _DT["i64"] and lens.numel() == B and
           new_lens.numel() == B and lens_out.numel() == B and starts.numel() == B + 1 and positions.numel() == T and
-          requests.numel() == T and row[1] == 1,
-          "batch_plan: int32 arrays of the batch, int64 slots and as many positions and requests expected")
+          requests.numel() == T and row[1] == 1 and free_count.numel() and free_out.numel() and
+          lens.is_contiguous() and new_lens.is_contiguous() and pool.is_contiguous() and lens_out.is_contiguous() and
+          starts.is_contiguous() and slots.is_contiguous() and positions.is_contiguous() and requests.is_contiguous(),
+          "batch_plan: dense int32 arrays of the batch, int64 slots and as many positions and requests expected")
     _launch("batch_plan", ARGS["batch_plan"].pack(
         lens.data_ptr(), new_lens.data_ptr(), block_tables.data_ptr(), row[0], pool.data_ptr(), free_count.data_ptr(),
         lens_out.data_ptr(), free_out.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(),
@@ -756,7 +758,11 @@ def paged_prep(q, k, v, slots, positions, query, k_cache, v_cache, inv_freq=None
           vs[2] == 1 and query.is_contiguous(),
           "paged_prep: q, k, v of the caches' heads with dense channels, caches of one shape and strides expected")
     _need(k.dtype is src and v.dtype is src and k_cache.dtype is dt and v_cache.dtype is dt and
-          slots.element_size() == 8 and slots.numel() == T, "paged_prep: types of q, k, v or of the caches differ")
+          slots.dtype is _DT["i64"] and slots.numel() == T and slots.is_contiguous(),
+          "paged_prep: types of q, k, v or of the caches differ, or slots not dense int64")
+    _need((q_norm is None or (_DT.get(q_norm.dtype) == DT_BF16 and q_norm.numel() == D and q_norm.is_contiguous())) and
+          (k_norm is None or (_DT.get(k_norm.dtype) == DT_BF16 and k_norm.numel() == D and k_norm.is_contiguous())),
+          "paged_prep: dense bf16 norms of a head's channels expected")
     rot = n_axes = stride = 0
     packed = b""
     if inv_freq is not None:
@@ -765,8 +771,9 @@ def paged_prep(q, k, v, slots, positions, query, k_cache, v_cache, inv_freq=None
         n_axes, stride = (1, T) if len(ps) == 1 else (ps[0], positions.stride(0))
         packed = bytes(axes) if axes is not None else bytes(rot // 2)
         _need(positions.dtype is _DT["i32"] and ps[-1] == T and positions.stride(-1) == 1 and
-              len(packed) == rot // 2 and len(packed) <= 128,
-              "paged_prep: int32 positions of every token, and an axis of them for each pair expected")
+              len(packed) == rot // 2 and len(packed) <= 128 and _DT.get(inv_freq.dtype) == DT_F32 and
+              inv_freq.is_contiguous(),
+              "paged_prep: int32 positions of every token, and a dense f32 frequency and an axis for each pair expected")
     _launch("paged_prep", ARGS["paged_prep"].pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], slots.data_ptr(),
         positions.data_ptr() if rot else 0, stride, inv_freq.data_ptr() if rot else 0,
@@ -800,10 +807,11 @@ def prefix_attention(q, k_cache, v_cache, block_tables, lens, starts, max_new, w
           qs[2] == 1 and out.is_contiguous() and k_cache.dtype is dt and v_cache.dtype is dt and out.dtype is dt,
           "prefix_attention: q, out and caches of one type and head size with dense channels expected")
     _need(block_tables.dtype is i32 and lens.dtype is i32 and starts.dtype is i32 and lens.numel() == B and
-          starts.numel() == B + 1 and row[1] == 1 and
+          starts.numel() == B + 1 and row[1] == 1 and lens.is_contiguous() and starts.is_contiguous() and
+          work.is_contiguous() and
           (not prefix_len or (prefix_blocks is not None and prefix_blocks.dtype is i32 and
-                              prefix_blocks.numel() * block_size >= prefix_len)),
-          "prefix_attention: int32 tables, lengths and starts of one batch, and the prefix's blocks expected")
+                              prefix_blocks.is_contiguous() and prefix_blocks.numel() * block_size >= prefix_len)),
+          "prefix_attention: dense int32 tables, lengths and starts of one batch, and the prefix's blocks expected")
     gs, gd = (0, 0), 0
     if gate is not None:
         gs, gd = gate.stride(), _dtype(gate)
@@ -847,16 +855,21 @@ def logits_adjust(logits, out, history=None, history_lens=None, prompt_lens=None
     lp = pp = rp = ep = fp = 0
     ok = True
     if history_lens is not None:
-        lp, ok = history_lens.data_ptr(), history_lens.dtype is i32 and history_lens.numel() == M
+        lp = history_lens.data_ptr()
+        ok = history_lens.dtype is i32 and history_lens.numel() == M and history_lens.is_contiguous()
     if prompt_lens is not None:
-        pp, ok = prompt_lens.data_ptr(), ok and prompt_lens.dtype is i32 and prompt_lens.numel() == M
+        pp = prompt_lens.data_ptr()
+        ok = ok and prompt_lens.dtype is i32 and prompt_lens.numel() == M and prompt_lens.is_contiguous()
     if repetition is not None:
-        rp, ok = repetition.data_ptr(), ok and repetition.dtype is f32 and repetition.numel() == M
+        rp = repetition.data_ptr()
+        ok = ok and repetition.dtype is f32 and repetition.numel() == M and repetition.is_contiguous()
     if presence is not None:
-        ep, ok = presence.data_ptr(), ok and presence.dtype is f32 and presence.numel() == M
+        ep = presence.data_ptr()
+        ok = ok and presence.dtype is f32 and presence.numel() == M and presence.is_contiguous()
     if frequency is not None:
-        fp, ok = frequency.data_ptr(), ok and frequency.dtype is f32 and frequency.numel() == M
-    _need(ok, "logits_adjust: a length or penalty for each row expected")
+        fp = frequency.data_ptr()
+        ok = ok and frequency.dtype is f32 and frequency.numel() == M and frequency.is_contiguous()
+    _need(ok, "logits_adjust: a dense int32 length or f32 penalty for each row expected")
     _launch("logits_adjust", ARGS["logits_adjust"].pack(
         logits.data_ptr(), xs[0], 0 if history is None else history.data_ptr(), hs[0], lp, pp, rp, ep, fp,
         0 if bias is None else bias_ids.data_ptr(), 0 if bias is None else bias.data_ptr(),
