@@ -333,3 +333,26 @@ def test_prefix_rows_that_no_token_sees_hold_anything(cuda, case, D, fill):
     assert Y.status() == 0
     near(q, rows, out, starts, new, lens)
     assert torch.equal(out, call(cuda, new, lens, P, 0.0, D=D, seed=case)[2])
+
+
+@pytest.mark.parametrize("n", [1, 20])
+def test_lengths_past_a_table_row_are_reported(cuda, n):
+    import torch
+    import yskn_b200 as Y
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device=cuda)  # noqa: E731
+    c = torch.ones((6, 16, 1, 64), dtype=torch.bfloat16, device=cuda)
+    q = torch.ones((2 * n, 1, 64), dtype=torch.bfloat16, device=cuda)
+    tables, prefix = i32(0, 1, 2, 3).view(2, 2), i32(4, 5)
+    work = torch.empty(Y.prefix_attention_work_bytes(2 * n, 3, n, 1, 1, 64), dtype=torch.uint8, device=cuda)
+
+    def status(lens, starts, P):
+        Y.prefix_attention(q, c, c, tables, i32(*lens), i32(*starts), n, work, torch.empty_like(q),
+                           prefix_blocks=prefix, prefix_len=P)
+        return Y.status()
+
+    for P in (0, 20):  # a table row names 32 rows after the prefix
+        assert status((P + 32, P + 30), (0, n, 2 * n), P) == 0
+        assert status((P + 30, P + 33), (0, n, 2 * n), P) == Y.EINVAL
+        assert status((P + 33, P + 30), (0, n, 2 * n), P) == Y.EINVAL
+        assert status((2 ** 31 - 1, P + 32), (0, n, 2 * n), P) == Y.EINVAL
+        assert status((P + 32, P + 33), (0, n, n), P) == 0  # one without tokens is not read

@@ -845,7 +845,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
       units_of[1] = pa_sum(units_of[1], times(pa_own_units(p, r, nq, true)));
       items = pa_sum(items, times(nq));
       if (r.n > 0) seen = max(seen, (unsigned)pa_visible_prefix(p, r, r.n));
-      if (blockIdx.x == 0 && (__ldg(p.starts + i + 1) - r.s0 != r.n)) raise_device_error(p.err, DERR_RANGE);
+      if (blockIdx.x == 0 && (__ldg(p.starts + i + 1) - r.s0 != r.n ||
+                              (r.n > 0 && r.len > p.prefix_len && r.len - p.prefix_len > p.own_limit)))
+        raise_device_error(p.err, DERR_RANGE);
     }
     unsigned ui[2] = {units_of[0], units_of[1]}, it = items;
 #pragma unroll
