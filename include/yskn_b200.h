@@ -641,7 +641,7 @@ YSKN_B200_API int yskn_b200_paged_prep(const yskn_b200_paged_prep_args* args, vo
 
 /* Attention of the batch's new tokens over the shared prefix and each request's own rows.
  * Request i's tokens are starts[i] .. starts[i + 1] - 1 of `tokens` (rows past
- * starts[batch] are padding), at most max_new, and the last of its lens[i] rows; token t of
+ * starts[batch] are padding), at most max_new (tokens or more: no bound), and the last of its lens[i] rows; token t of
  * n sees the first max(0, len - n + t + 1) rows: below prefix_len in prefix_blocks
  * int32 [ceil(prefix_len / block_size)], from there on in the request's row of
  * block_tables. out = softmax(scale * q k^T) v in binary32 sums, times sigmoid(gate) if

@@ -202,3 +202,13 @@ def test_arrays_that_the_library_reads_by_address_alone():
     for k in ("history_lens", "prompt_lens", "repetition", "presence", "frequency"):
         refused("logits_adjust: a dense", Y.logits_adjust, adjust, **{k: every_second(adjust[k])})
         refused("logits_adjust: a dense", Y.logits_adjust, adjust, **{k: adjust[k].double()})
+
+
+def test_work_bytes_without_a_bound_on_the_new_tokens():
+    """A request has at most all of the call's tokens: a larger max_new says no more than that."""
+    import yskn_b200 as Y
+    for G in (1, 2, 4, 6, 8, 16):
+        for tokens in (1, 3, 200):
+            n = Y.prefix_attention_work_bytes(tokens, 5, tokens, 4 * G, 4, 256)
+            for max_new in (tokens + 1, 357913942, 2 ** 30, 2 ** 31 - 1):
+                assert Y.prefix_attention_work_bytes(tokens, 5, max_new, 4 * G, 4, 256) == n

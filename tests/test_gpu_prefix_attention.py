@@ -356,3 +356,11 @@ def test_lengths_past_a_table_row_are_reported(cuda, n):
         assert status((P + 33, P + 30), (0, n, 2 * n), P) == Y.EINVAL
         assert status((2 ** 31 - 1, P + 32), (0, n, 2 * n), P) == Y.EINVAL
         assert status((P + 32, P + 33), (0, n, n), P) == 0  # one without tokens is not read
+
+
+@pytest.mark.parametrize("G", [1, 2, 4, 6, 8])
+@pytest.mark.parametrize("max_new", [2 ** 31 - 1, 2 ** 30, 357913942])
+def test_no_bound_on_the_new_tokens(cuda, G, max_new):
+    """max_new far above the tokens there are, whose product with G passes 32 bits."""
+    run(cuda, new=(1, 50, 2), own=(30, 300, 2), P=200, n_qh=2 * G, n_kvh=2, max_new=max_new, seed=28)
+    run(cuda, new=(1, 1), own=(30, 300), P=200, n_qh=2 * G, n_kvh=2, max_new=max_new, seed=28)

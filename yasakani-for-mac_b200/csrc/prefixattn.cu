@@ -113,12 +113,13 @@ struct PaWork {
 };
 inline PaWork pa_work(int tokens, int batch, int max_new, int n_qh, int n_kvh, int head) {
   auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+  max_new = std::min(max_new, tokens);  // a request cannot have more
   const int G = n_qh / n_kvh, tpc = PA_ROWS / G, tpi = 2 * tpc;  // tokens per CTA and per item
   const int64_t pre_items = ceil_div(tokens, tpi) * n_kvh;
   // sum of ceil(n_i / tpi) over requests with n_i > 0: at most one more than n_i / tpi each
   const int64_t own_items = (std::min(batch, tokens) + (int64_t)tokens / tpi) * n_kvh;
   const int64_t pre = pre_items + PA_MAX_PAIRS;
-  const int64_t own = own_items + (G * max_new <= PA_THIN_ROWS ? PA_MAX_THIN : PA_MAX_PAIRS);
+  const int64_t own = own_items + ((int64_t)G * max_new <= PA_THIN_ROWS ? PA_MAX_THIN : PA_MAX_PAIRS);
   PaWork w{};
   w.own_half = G * std::min(tpc, max_new);
   w.own_rows = max_new > tpc ? 2 * w.own_half : w.own_half;
@@ -1651,6 +1652,7 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
       !aligned16(a.out) || (a.q_row | a.q_head | a.block_stride | a.token_stride | a.head_stride) % 8 ||
       (a.gate && (a.gate_row | a.gate_head) % (a.gate_dtype == YSKN_DT_F32 ? 4 : 8)))
     return fail(YSKN_EINVAL, "prefix_attention: pointers and strides are multiples of 16 bytes");
+  a.max_new = std::min(a.max_new, a.tokens);  // as pa_work does
   const PaWork w = pa_work(a.tokens, a.batch, a.max_new, n_qh, n_kvh, head);
   if (a.work_bytes < w.bytes) return fail(YSKN_EINVAL, "prefix_attention: workspace too small");
   const int G = n_qh / n_kvh, tpc = PA_ROWS / G;
@@ -1685,7 +1687,7 @@ extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_a
   // quicker than the second launch that joins its parts. Two requests, us whole and cut: of two
   // tokens and one tile 15.5, 19.2, of two tiles 17.3, 14.8; thin with up to 32 and 64 rows 10.3, 14.4
   // and 12.1, 16.1, with 128 15.7, 13.8 (12.2 since a warp's least is 2 units).
-  p.thin = G * a.max_new <= PA_THIN_ROWS && pairs > 1;
+  p.thin = (int64_t)G * a.max_new <= PA_THIN_ROWS && pairs > 1;
   p.tile_shift = p.thin ? PA_THIN_SHIFT : 7;
   p.item_cost = p.thin ? PA_THIN_COST : PA_ITEM_COST;
   const int64_t most_tiles = ceil_div(a.prefix_len, 1 << p.tile_shift) + ceil_div(p.own_limit, 1 << p.tile_shift);
