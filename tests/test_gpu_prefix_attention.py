@@ -364,3 +364,24 @@ def test_no_bound_on_the_new_tokens(cuda, G, max_new):
     """max_new far above the tokens there are, whose product with G passes 32 bits."""
     run(cuda, new=(1, 50, 2), own=(30, 300, 2), P=200, n_qh=2 * G, n_kvh=2, max_new=max_new, seed=28)
     run(cuda, new=(1, 1), own=(30, 300), P=200, n_qh=2 * G, n_kvh=2, max_new=max_new, seed=28)
+
+
+@pytest.mark.parametrize("P", [0, 40, 3000])
+@pytest.mark.parametrize("n_qh,D", [(6, 64), (40, 128)])  # few rows a KV head, and many
+@pytest.mark.parametrize("width", [1, 60])  # of few tiles, and of many
+def test_starts_that_do_not_ascend_are_reported(cuda, P, n_qh, D, width):
+    """More requests with tokens than there are tokens: nothing is computed, every row is zero."""
+    import torch
+    import yskn_b200 as Y
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=cuda)  # noqa: E731
+    T, B = 2, 60
+    c = torch.ones((8, 16, 2, D), dtype=torch.bfloat16, device=cuda)
+    q = torch.ones((T, n_qh, D), dtype=torch.bfloat16, device=cuda)
+    tables = (torch.arange(B * width, device=cuda) % 8).to(torch.int32).view(B, width)
+    work = torch.full((Y.prefix_attention_work_bytes(T, B, 1, n_qh, 2, D),), 255, dtype=torch.uint8, device=cuda)
+    for _ in range(2):
+        out = torch.full((T, n_qh, D), 3.0, dtype=torch.bfloat16, device=cuda)
+        Y.prefix_attention(q, c, c, tables, i32([P + 16 * width] * B), i32([0, 1] * (B // 2) + [0]), 1, work, out,
+                           prefix_blocks=i32([0] * -(-max(P, 1) // 16)), prefix_len=P)
+        assert Y.status() == Y.EINVAL
+        assert bool((out == 0).all())

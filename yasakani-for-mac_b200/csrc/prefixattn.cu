@@ -256,6 +256,7 @@ struct PaSegment {
 struct PaStart {
   int who;           // this pair, or this warp of those that take thin items
   bool thin;         // the latter
+  bool sound;        // false: more items than there is room for, nothing is computed
   int left;          // its units
   int alone;         // no prefix items: each request's items take the prefix too
   int pre_seen;      // rows of the prefix that any token of the call sees
@@ -479,14 +480,14 @@ __device__ __forceinline__ void quarter_sync(int quarter) {
   asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
 }
 
-// Where no join visits every row: zeros for this CTA's share of the tokens that no item holds. One
-// warp; each lane looks at a token.
+// Where no join visits every row: zeros for this CTA's share of the tokens that no item holds (all, where
+// nothing is computed). One warp; each lane looks at a token.
 template <int D>
-__device__ __forceinline__ void zero_unheld(const PrefixAttnParams& p, int lane) {
+__device__ __forceinline__ void zero_unheld(const PrefixAttnParams& p, bool sound, int lane) {
   for (int t0 = blockIdx.x * 32; t0 < p.tokens; t0 += gridDim.x * 32) {
     const int t = t0 + lane;
     bool bare = t < p.tokens;
-    if (bare) {
+    if (bare && sound) {
       const int i = request_of(p.starts, p.batch, t);
       const PaRequest r = i < p.batch ? pa_request(p, i) : PaRequest{};
       bare = t < r.s0 || t >= r.s0 + r.n || pa_tiles(p, r, pa_quotient(t - r.s0, p.tpi_magic), true) == 0;
@@ -902,7 +903,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
         tc = min(max((int)((float)pairs * (float)pre_time / ((float)pre_time + (float)own) + 0.5f), 1), pairs - 1);
       const int warps = 2 * PA_THIN_WARPS * (pairs - tc);
       share_pre = tc > 0 ? (pre + tc - 1) / tc : 0;
-      share_own = warps > 0 ? max((own + warps - 1) / warps, p.whole ? 1 : PA_THIN_LEAST) : 0;
+      share_own = warps > 0 && own > 0 ? max((own + warps - 1) / warps, p.whole ? 1 : PA_THIN_LEAST) : 0;
     }
     const bool thin = pair >= tc;  // this pair's CTAs
     // a CTA's first thin warp, and from each to its next (neighbours are on different SMs: where there
@@ -911,7 +912,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
     if (tid < PA_THIN_WARPS) {
       const int who = who0 + (thin ? tid * ctas : 0), share = thin ? share_own : share_pre;
       const int all = thin ? own : p.thin ? pre : pre + own, t0 = min(all, who * share);
-      PaStart s{who,       thin, min(all, t0 + share) - t0,        alone, (int)seen,
+      PaStart s{who,       thin, sound, min(all, t0 + share) - t0,        alone, (int)seen,
                 pre_items, 0,    p.thin && !thin ? p.batch : 0, 0,     0};
       if (!thin && t0 < pre) {
         s.pre_item = t0 / pre_units;
@@ -954,7 +955,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
   __syncthreads();
   const uint32_t tmem = sh.tmem_slot;
   if (sh.start[0].thin) {
-    if (p.whole && warp == PA_THIN_WARPS - 1) zero_unheld<D>(p, lane);
+    if (p.whole && warp == PA_THIN_WARPS - 1) zero_unheld<D>(p, sh.start[0].sound, lane);
     thin_items<D, DT>(p, sh.start[warp], smem, warp, lane);
   } else {
     PaWalk walk(p, sh.start[0]);
@@ -1158,7 +1159,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
         }
       }
     } else if (warp == 3) {
-      if (walk.alone) zero_unheld<D>(p, lane);
+      if (walk.alone) zero_unheld<D>(p, sh.start[0].sound, lane);
       // ---- V rows past the last visible one, up to the end of the 16-row step, to zero, in the
       // slots that warp 0 names: once for each segment that ends inside a step
       const uint32_t full0 = first_cta(&sh.full[0]);
@@ -1534,7 +1535,7 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
   if (live && (how.x | how.y) > 0 && t >= r.s0 && t < r.s0 + r.n) {
     const int nq = pa_qtiles(p, r), own_qt = nq > 1 ? pa_quotient(t - r.s0, p.tpi_magic) : 0;
     const int kt = pa_tiles(p, r, own_qt, alone);
-    if (kt > 0) {
+    if (kt > 0 && how.y > 0) {
       int b = base.y + p.item_cost;
       if (kvh > 0) b += kvh * (int)pa_own_units(p, r, nq, alone);
       for (int q = 0; q < own_qt; ++q) b += pa_units(pa_tiles(p, r, q, alone), false, p.item_cost);
@@ -1546,7 +1547,7 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
       own_o = reinterpret_cast<const float4*>(p.own_o) + at * (D / 4) + ch * p.own_rows + row;
     }
     if (n_own == 1 && alone) live = false;  // finished where it was computed
-    if (!alone) {
+    if (!alone && how.x > 0) {
       const int qt = pa_quotient(t, p.tpi_magic), it = kvh * p.pre_qtiles + qt, tl = t - qt * p.tpi, rank = tl >= p.tpc;
       const int b = it * pa_units(how.z, false, PA_ITEM_COST) + PA_ITEM_COST, c0 = pair_of(b, how.x);
       n_pre = pair_of(b + how.z - 1, how.x) - c0 + 1;
