@@ -126,3 +126,43 @@ def test_graph_equals_eager(cuda):
 
     for a, b in zip(run(False), run(True)):
         assert torch.equal(a, b)
+
+
+def test_a_stream_that_is_not_the_current_one(cuda):
+    """All of a step runs on the stream it is given: the same steps, held up there, give the same."""
+    import torch
+    import yskn_b200 as Y
+
+    def run(stream):
+        st = _stack(cuda, batch=5, max_tokens=64, capacity=32, n_blocks=24)
+        here = torch.cuda.current_stream(cuda)
+
+        def late():
+            if stream is not None:  # after the inputs, and well after what the current stream does next
+                stream.wait_stream(here)
+                with torch.cuda.stream(stream):
+                    torch.cuda._sleep(4000000)
+
+        prefix = _prefix(cuda, 70)
+        late()
+        st.fill_prefix(prefix, stream)
+        if stream is not None:
+            here.wait_stream(stream)
+        for i in range(5):
+            st.say(i, _prompt(i, 3 + i))
+        st.presence.fill_(0.25)
+        st.new.copy_(st.said)
+        late()
+        st.step(25, 7, stream)
+        if stream is not None:
+            here.wait_stream(stream)
+        st.new.fill_(1)
+        for _ in range(6):
+            late()
+            st.step(5, 1, stream)
+        torch.cuda.synchronize()
+        assert Y.status() == 0
+        return st.text.clone(), st.lens.clone(), st.said.clone(), st.blogits.clone()
+
+    for a, b in zip(run(None), run(torch.cuda.Stream(cuda))):
+        assert torch.equal(a, b)

@@ -76,6 +76,9 @@ class BatchStack(S.Stack):
         """Runs `tokens` (int32, on the device) once as what every request's text follows. Before any
         request: the pool is as at the start."""
         torch, P = self.torch, tokens.numel()
+        if stream is not None:  # torch's operations between the library's calls run on it too
+            with torch.cuda.stream(stream):
+                return self.fill_prefix(tokens)
         table = torch.zeros((1, -(-P // self.block_size)), dtype=torch.int32, device=self.dev)
         lens, lens_out, new = (torch.zeros(1, dtype=torch.int32, device=self.dev) for _ in range(3))
         starts = torch.zeros(2, dtype=torch.int32, device=self.dev)
@@ -83,9 +86,9 @@ class BatchStack(S.Stack):
             n = min(self.max_tokens, P - at)
             new.fill_(n)
             Y.batch_plan(lens, new, table, self.pool, self.free, self.block_size, lens_out, self.free_out, starts,
-                         self.slots[:n], self.pos[:n], self.requests[:n], stream=stream)
+                         self.slots[:n], self.pos[:n], self.requests[:n])
             self.tokens[:n].copy_(tokens[at:at + n])
-            self._layers(n, n, table, lens_out, starts, None, 0, stream)
+            self._layers(n, n, table, lens_out, starts, None, 0)
             lens.copy_(lens_out)
             self.free.copy_(self.free_out)
         self.prefix_len, self.prefix_blocks = P, table[0]
@@ -102,22 +105,25 @@ class BatchStack(S.Stack):
         """Runs self.new[i] tokens of each request i that said them (a negative number ends the
         request): n_tokens in all at most, max_new for one request at most. A request whose tokens or
         blocks do not fit waits (its length in self.lens stays). Those that ran to the end of what they
-        said have their next token appended."""
+        said have their next token appended. Everything runs on `stream` (the current one without it),
+        after what the caller has put there."""
         torch, T, W = self.torch, n_tokens, self.capacity
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self.step(n_tokens, max_new)
         Y.batch_plan(self.lens, self.new, self.tables, self.pool, self.free, self.block_size, self.lens_out,
-                     self.free_out, self.starts, self.slots[:T], self.pos[:T], self.requests[:T], self.prefix_len,
-                     stream=stream)
+                     self.free_out, self.starts, self.slots[:T], self.pos[:T], self.requests[:T], self.prefix_len)
         # token t is its request's text at its position behind the prefix (past the last one: any)
         at = self.requests[:T].clamp(min=0).long() * W + (self.pos[:T] - self.prefix_len).clamp(0, W - 1)
         self.tokens[:T].copy_(self.text.view(-1)[at])
-        self._layers(T, max_new, self.tables, self.lens_out, self.starts, self.prefix_blocks, self.prefix_len, stream)
+        self._layers(T, max_new, self.tables, self.lens_out, self.starts, self.prefix_blocks, self.prefix_len)
         # each request's last token; a request without one answers with a row that is not used
         last = (self.starts[1:] - 1).clamp(min=0).long()
-        Y.linear([self.head], self.bx[last], self.bwork, [self.blogits], inv_rms=self.binv[last], stream=stream)
+        Y.linear([self.head], self.bx[last], self.bwork, [self.blogits], inv_rms=self.binv[last])
         Y.logits_adjust(self.blogits, self.blogits, history=self.text, history_lens=self.said,
                         prompt_lens=self.prompt, repetition=self.repetition, presence=self.presence,
-                        frequency=self.frequency, mask=self.mask, stream=stream)
-        Y.head_select(self.blogits, token=self.btoken, stream=stream)
+                        frequency=self.frequency, mask=self.mask)
+        Y.head_select(self.blogits, token=self.btoken)
         own = self.lens_out - self.prefix_len * (self.lens_out > 0)
         spoke = (self.starts[1:] > self.starts[:-1]) & (own == self.said) & (self.said < W)
         place = self.said.clamp(max=W - 1).long().unsqueeze(1)
@@ -126,28 +132,28 @@ class BatchStack(S.Stack):
         self.lens.copy_(self.lens_out)
         self.free.copy_(self.free_out)
 
-    def _layers(self, T, max_new, tables, lens, starts, prefix_blocks, prefix_len, s):
+    def _layers(self, T, max_new, tables, lens, starts, prefix_blocks, prefix_len):
         """The first T of self.tokens through every layer, into self.bx and self.binv."""
         h, x, inv, proj = self.bh[:T], self.bx[:T], self.binv[:T], self.bproj[:T]
         q, k, v, query, out = self.bq[:T], self.bk[:T], self.bv[:T], self.bquery[:T], self.bout[:T]
         gate, up, m, a_in = self.bg[:T], self.bu[:T], self.bm[:T], self.ba_in[:T]
-        self.embedding.lookup(self.tokens[:T], h, stream=s)
+        self.embedding.lookup(self.tokens[:T], h)
         before = None
         for L in self.L:
-            Y.residual_prepare(h, before, L["in_norm"], S.EPS, x, inv, stream=s)
-            Y.linear([L["q"], L["k"], L["v"]], x, self.bwork, [q, k, v], inv_rms=inv, stream=s)
+            Y.residual_prepare(h, before, L["in_norm"], S.EPS, x, inv)
+            Y.linear([L["q"], L["k"], L["v"]], x, self.bwork, [q, k, v], inv_rms=inv)
             Y.paged_prep(q[:, :, :S.HEAD], k, v, self.slots[:T], self.pos[:T], query, *L["pages"],
-                         inv_freq=self.inv_freq, q_norm=L["q_norm"], k_norm=L["k_norm"], eps=S.EPS, stream=s)
+                         inv_freq=self.inv_freq, q_norm=L["q_norm"], k_norm=L["k_norm"], eps=S.EPS)
             Y.prefix_attention(query, *L["pages"], tables, lens, starts, max_new, self.attn_work, out,
-                               prefix_blocks=prefix_blocks, prefix_len=prefix_len, gate=q[:, :, S.HEAD:], stream=s)
-            Y.widen_bf16(out, a_in, stream=s)
-            Y.linear([L["o"]], a_in, self.bwork, [proj], stream=s)
-            Y.residual_prepare(h, proj, L["post_norm"], S.EPS, x, inv, stream=s)
-            Y.linear([L["gate"], L["up"]], x, self.bwork, [gate, up], inv_rms=inv, stream=s)
-            Y.gated_product(gate, up, m, stream=s)
-            Y.linear([L["down"]], m, self.bwork, [proj], stream=s)
+                               prefix_blocks=prefix_blocks, prefix_len=prefix_len, gate=q[:, :, S.HEAD:])
+            Y.widen_bf16(out, a_in)
+            Y.linear([L["o"]], a_in, self.bwork, [proj])
+            Y.residual_prepare(h, proj, L["post_norm"], S.EPS, x, inv)
+            Y.linear([L["gate"], L["up"]], x, self.bwork, [gate, up], inv_rms=inv)
+            Y.gated_product(gate, up, m)
+            Y.linear([L["down"]], m, self.bwork, [proj])
             before = proj
-        Y.residual_prepare(h, before, self.final_norm, S.EPS, x, inv, stream=s)
+        Y.residual_prepare(h, before, self.final_norm, S.EPS, x, inv)
 
 
 def main():
