@@ -385,3 +385,27 @@ def test_starts_that_do_not_ascend_are_reported(cuda, P, n_qh, D, width):
                            prefix_blocks=i32([0] * -(-max(P, 1) // 16)), prefix_len=P)
         assert Y.status() == Y.EINVAL
         assert bool((out == 0).all())
+
+
+NOTHING = [  # new tokens, lengths and prefix: some tokens see nothing
+    ((1, 1, 1), (30, 0, 1), 40),  # items that are not cut
+    ((1, 2, 1), (3000, 1, 0), 0),  # cut ones
+    ((2,) * 40, tuple([1, 300] * 20), 5000),  # few rows a head, beside prefix items
+    ((4,) * 40, tuple([2, 300, 0, 90] * 10), 5000),  # prefix items
+    ((150, 90), (330, 60), 700),  # many rows, each request by itself
+    ((20, 9), (4, 15), 0),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("case", range(len(NOTHING)))
+def test_tokens_that_see_nothing_give_zeros_whatever_their_gate_holds(cuda, case, dtype):
+    import torch
+    import yskn_b200 as Y
+    new, lens, P = NOTHING[case]
+    g = torch.randn((sum(new), 6, 128), device=cuda).to({"bf16": torch.bfloat16, "f32": torch.float32}[dtype])
+    blind = torch.tensor([n - k + t + 1 <= 0 for n, k in zip(lens, new) for t in range(k)], device=cuda)
+    g[blind] = float("nan")
+    out = call(cuda, new, lens, P, float("nan"), gate=g, seed=case)[2]
+    assert Y.status() == 0 and bool(blind.any())
+    assert bool((out[blind] == 0).all()) and not bool(out[~blind].isnan().any())

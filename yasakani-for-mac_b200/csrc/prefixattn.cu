@@ -458,6 +458,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return y;
 }
+// The gate's factor. (A row that sees nothing is zero whatever its gate holds.)
 __device__ __forceinline__ float gated(float x, float gate) {
   return __fdividef(x, 1.0f + exp2_approx(-1.44269504f * gate));
 }
@@ -750,7 +751,7 @@ __device__ __forceinline__ void thin_items(const PrefixAttnParams& p, const PaSt
             const float4 d = gate_value<DT>(p, gate_load(p, gate + 64 * x + 4));
             const float gs[8] = {a.x, a.y, a.z, a.w, d.x, d.y, d.z, d.w};
 #pragma unroll
-            for (int k = 0; k < 8; ++k) e[k] = gated(e[k], gs[k]);
+            for (int k = 0; k < 8; ++k) e[k] = f == 0.0f ? 0.0f : gated(e[k], gs[k]);
           }
           *reinterpret_cast<uint4*>(out + 64 * x) = make_uint4(Elem<DT>::pack(e[0], e[1]), Elem<DT>::pack(e[2], e[3]),
                                                                Elem<DT>::pack(e[4], e[5]), Elem<DT>::pack(e[6], e[7]));
@@ -1317,7 +1318,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
                       const float4 a = gate_value<DT>(p, g[y / 4]), d = gate_value<DT>(p, g[y / 4 + 1]);
                       const float gs[8] = {a.x, a.y, a.z, a.w, d.x, d.y, d.z, d.w};
 #pragma unroll
-                      for (int k = 0; k < 8; ++k) z[k] = gated(z[k], gs[k]);
+                      for (int k = 0; k < 8; ++k) z[k] = inv == 0.0f ? 0.0f : gated(z[k], gs[k]);
                     }
                     *reinterpret_cast<uint4*>(out + x + y0 + y) =
                         make_uint4(Elem<DT>::pack(z[0], z[1]), Elem<DT>::pack(z[2], z[3]), Elem<DT>::pack(z[4], z[5]),
@@ -1417,7 +1418,7 @@ __device__ __forceinline__ void join_store(const PrefixAttnParams& p, int t, int
                                            uint4 gate) {
   const float inv = s.den == 0.0f ? 0.0f : 1.0f / s.den;
   float v[4] = {s.o.x * inv, s.o.y * inv, s.o.z * inv, s.o.w * inv};
-  if (p.gate) {
+  if (p.gate && inv != 0.0f) {
     const float4 g = gate_value<DT>(p, gate);
     v[0] = gated(v[0], g.x), v[1] = gated(v[1], g.y), v[2] = gated(v[2], g.z), v[3] = gated(v[3], g.w);
   }
