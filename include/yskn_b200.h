@@ -655,7 +655,9 @@ YSKN_B200_API int yskn_b200_paged_prep(const yskn_b200_paged_prep_args* args, vo
  * 64, 128 or 256 channels; blocks of 16, 32, 64 or 128 rows; the cache's strides as in
  * yskn_b200_paged_prep. Pointers and strides are multiples of 16 bytes. A block number outside
  * the cache, a length past what the request's table row can name or a request of more than max_new
- * tokens gives YSKN_EINVAL from yskn_b200_status. work: work_bytes of memory, at least yskn_b200_prefix_attention_work_bytes(), one call's at a time. */
+ * tokens gives YSKN_EINVAL from yskn_b200_status. work: work_bytes of memory, at least
+ * yskn_b200_prefix_attention_work_bytes() (which never falls as tokens, batch or max_new grow, so that
+ * the largest step's serves all), one call's at a time. */
 YSKN_B200_API int64_t yskn_b200_prefix_attention_work_bytes(int tokens, int batch, int max_new, int n_qh, int n_kvh,
                                                             int head);
 typedef struct {

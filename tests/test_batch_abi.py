@@ -212,3 +212,18 @@ def test_work_bytes_without_a_bound_on_the_new_tokens():
             n = Y.prefix_attention_work_bytes(tokens, 5, tokens, 4 * G, 4, 256)
             for max_new in (tokens + 1, 357913942, 2 ** 30, 2 ** 31 - 1):
                 assert Y.prefix_attention_work_bytes(tokens, 5, max_new, 4 * G, 4, 256) == n
+
+
+def test_the_largest_steps_work_bytes_serve_every_smaller_one():
+    import yskn_b200 as Y
+    sizes = (1, 2, 3, 4, 8, 16, 41, 64, 300)
+    for G in (1, 2, 3, 6, 8, 9):
+        for head in (64, 256):
+            need = lambda *a: Y.prefix_attention_work_bytes(*a, 4 * G, 4, head)  # noqa: E731
+            for T in sizes:
+                for B in (1, 7, 64):
+                    for n in sizes:
+                        most = need(T, B, n)
+                        for less in ((max(1, T // 2), B, n), (T, max(1, B // 3), n), (T, B, max(1, n // 2)), (T, B, 1),
+                                     (1, 1, 1)):
+                            assert need(*less) <= most, (G, head, (T, B, n), less)

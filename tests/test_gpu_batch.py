@@ -166,3 +166,18 @@ def test_a_stream_that_is_not_the_current_one(cuda):
 
     for a, b in zip(run(None), run(torch.cuda.Stream(cuda))):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("max_tokens", [2, 5, 16])
+def test_small_steps_of_a_small_loop(cuda, max_tokens):
+    """A step of one token for each request in a loop made for few tokens a step."""
+    import yskn_b200 as Y
+    st = _stack(cuda, batch=2, max_tokens=max_tokens, capacity=32, n_blocks=12)
+    st.fill_prefix(_prefix(cuda, 21))
+    for i in range(2):
+        st.say(i, _prompt(i, 1))
+    for n in range(3):
+        st.new.fill_(1)
+        st.step(2, 1)
+        assert st.lens.tolist() == [22 + n] * 2 and st.said.tolist() == [2 + n] * 2
+    assert Y.status() == 0

@@ -130,6 +130,11 @@ inline PaWork pa_work(int tokens, int batch, int max_new, int n_qh, int n_kvh, i
   w.own_ml = w.pre_o + up(pre * 2 * PA_ROWS * head * 4);
   w.own_o = w.own_ml + up(own * w.own_rows * 8);
   w.bytes = w.own_o + up(own * w.own_rows * head * 4);
+  // Smaller calls fit too: those of few rows a KV head have more places, if smaller ones.
+  if (G <= PA_THIN_ROWS) {
+    const int64_t thin = (own_items + PA_MAX_THIN) * G * std::min(max_new, PA_THIN_ROWS / G);
+    w.bytes = std::max(w.bytes, w.own_ml + up(thin * 8) + up(thin * head * 4));
+  }
   return w;
 }
 
