@@ -592,7 +592,7 @@ YSKN_B200_API int yskn_b200_kv_encode(const float* d_rows, const int32_t* d_row_
  * blocks are back). Written: lens_out [batch] and *free_out (arrays of their own: keep
  * two of each and swap them), starts [batch + 1] (served tokens before each request), and
  * per token slots int64 (block * block_size + place, for yskn_b200_paged_prep), positions
- * and requests int32 [max_tokens], -1 past the last served token. Lengths or a count that
+ * and requests int32 [max_tokens, at most 2^30], -1 past the last served token. Lengths or a count that
  * do not fit their arrays give YSKN_EINVAL from yskn_b200_status. One launch. */
 typedef struct {
   const int32_t *lens, *new_lens; /* [batch] */

@@ -227,3 +227,10 @@ def test_the_largest_steps_work_bytes_serve_every_smaller_one():
                         for less in ((max(1, T // 2), B, n), (T, max(1, B // 3), n), (T, B, max(1, n // 2)), (T, B, 1),
                                      (1, 1, 1)):
                             assert need(*less) <= most, (G, head, (T, B, n), less)
+
+
+def test_plan_of_more_tokens_than_its_places_count():
+    """Places of tokens are 32-bit numbers on the device, those that a CTA rounds up to among them."""
+    good = dict(lens=P, new=P, tables=P, stride=4, pool=P, free=P, lens_out=2 * P, free_out=2 * P, starts=P, slots=P,
+                positions=P, requests=P, batch=2, block=16, prefix=0, width=4, capacity=9, tokens=5)
+    _check("yskn_b200_batch_plan", good, [dict(tokens=2 ** 30 + 1), dict(tokens=2 ** 31 - 1)])
