@@ -181,3 +181,13 @@ def test_small_steps_of_a_small_loop(cuda, max_tokens):
         st.step(2, 1)
         assert st.lens.tolist() == [22 + n] * 2 and st.said.tolist() == [2 + n] * 2
     assert Y.status() == 0
+
+
+def test_a_prefix_larger_than_the_pool_is_refused(cuda):
+    import yskn_b200 as Y
+    st = _stack(cuda, batch=2, max_tokens=64, capacity=32, n_blocks=4)
+    with pytest.raises(Y.YsknError) as e:
+        st.fill_prefix(_prefix(cuda, 65))
+    assert e.value.code == Y.EINVAL and st.prefix_len == 0 and st.free.tolist() == [4]
+    st.fill_prefix(_prefix(cuda, 64))
+    assert st.prefix_len == 64 and st.free.tolist() == [0] and Y.status() == 0

@@ -79,6 +79,8 @@ class BatchStack(S.Stack):
         if stream is not None:  # torch's operations between the library's calls run on it too
             with torch.cuda.stream(stream):
                 return self.fill_prefix(tokens)
+        if -(-P // self.block_size) > self.pool.numel():  # the plan would let the rest wait
+            raise Y.YsknError(Y.EINVAL, "fill_prefix: more tokens than the pool's blocks hold")
         table = torch.zeros((1, -(-P // self.block_size)), dtype=torch.int32, device=self.dev)
         lens, lens_out, new = (torch.zeros(1, dtype=torch.int32, device=self.dev) for _ in range(3))
         starts = torch.zeros(2, dtype=torch.int32, device=self.dev)
