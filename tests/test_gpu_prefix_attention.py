@@ -409,3 +409,32 @@ def test_tokens_that_see_nothing_give_zeros_whatever_their_gate_holds(cuda, case
     out = call(cuda, new, lens, P, float("nan"), gate=g, seed=case)[2]
     assert Y.status() == 0 and bool(blind.any())
     assert bool((out[blind] == 0).all()) and not bool(out[~blind].isnan().any())
+
+
+@pytest.mark.parametrize("own", [12, 15, 16, 17, 63, 64, 65, 127, 128, 129, 191, 192, 193, 255, 256, 257, 600])
+@pytest.mark.parametrize("P", [0, 64, 130])
+def test_own_lengths_of_many_rows_a_head(cuda, own, P):
+    """A tile's edges where items are 256 rows of the tensor cores."""
+    for D in (64, 128, 256):
+        run(cuda, new=(12, 3), own=(own, 3), P=P, D=D, seed=own)
+
+
+def test_long_cache_of_many_rows_a_head(cuda):
+    """Blocks past 2^31 elements into the cache, prefix and own ones, by the tensor maps."""
+    import torch
+    import yskn_b200 as Y
+    D, block, n_blocks, T, P = 256, 128, 70000, 12, 200
+    g = torch.Generator(device=cuda)
+    g.manual_seed(29)
+    kc, vc = (torch.zeros((n_blocks, block, 1, D), dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    for c in (kc, vc):
+        c[-3:].normal_(generator=g)
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device=cuda)  # noqa: E731
+    q = torch.randn((T, 2, D), generator=g, device=cuda).to(torch.bfloat16)
+    out = torch.empty_like(q)
+    work = torch.empty(Y.prefix_attention_work_bytes(T, 1, T, 2, 1, D), dtype=torch.uint8, device=cuda)
+    Y.prefix_attention(q, kc, vc, i32(n_blocks - 1)[None], i32(P + 100), i32(0, T), T, work, out,
+                       prefix_blocks=i32(n_blocks - 3, n_blocks - 2), prefix_len=P)
+    assert Y.status() == 0
+    rows = [torch.cat([c[-3:-1].reshape(-1, 1, D)[:P], c[-1, :100]]) for c in (kc, vc)]
+    near(q, [rows], out, [0, T], (T,), (P + 100,))
