@@ -183,3 +183,18 @@ def test_penalties_of_every_size_round_as_the_division(cuda, rep, wide):
     assert np.array_equal(np.isnan(got), np.isnan(exp))
     bits = ~np.isnan(exp)
     assert np.array_equal(got.view(np.uint32)[bits], exp.view(np.uint32)[bits])
+
+
+def test_a_history_of_no_entries(cuda):
+    """Nothing has been said yet: penalties and all, the logits stay as they are."""
+    import torch
+    import yskn_b200 as Y
+    x = torch.randn((3, 777), device=cuda)
+    out, ones = torch.empty_like(x), torch.ones(3, device=cuda)
+    none = torch.zeros(3, dtype=torch.int32, device=cuda)
+    Y.logits_adjust(x, out, history=torch.zeros((3, 0), dtype=torch.int32, device=cuda), history_lens=none,
+                    prompt_lens=none, repetition=2 * ones, presence=ones, frequency=ones)
+    assert Y.status() == 0 and torch.equal(out, x)
+    Y.logits_adjust(x, out, history=torch.zeros((3, 0), dtype=torch.int32, device=cuda), history_lens=none + 1,
+                    presence=ones)
+    assert Y.status() == Y.EINVAL and torch.equal(out, x)

@@ -839,9 +839,10 @@ def logits_adjust(logits, out, history=None, history_lens=None, prompt_lens=None
     _need(_dtype(logits) == DT_F32 and out.dtype is f32 and out.shape == shape and xs[1] == 1 and os_[1] == 1,
           "logits_adjust: f32 logits and output of one shape with dense rows expected")
     hs = ms = (0, 1)
-    width = n_bias = 0
+    width = n_bias = hp = 0
     if history is not None:
         hs, (rows, width) = history.stride(), history.shape
+        hp = history.data_ptr() or logits.data_ptr()  # one of no entries has no address, and is not read
         _need(history.dtype is i32 and rows == M and hs[1] == 1, "logits_adjust: int32 history rows expected")
     if mask is not None:
         ms, (rows, words) = mask.stride(), mask.shape
@@ -871,6 +872,6 @@ def logits_adjust(logits, out, history=None, history_lens=None, prompt_lens=None
         ok = ok and frequency.dtype is f32 and frequency.numel() == M and frequency.is_contiguous()
     _need(ok, "logits_adjust: a dense int32 length or f32 penalty for each row expected")
     _launch("logits_adjust", ARGS["logits_adjust"].pack(
-        logits.data_ptr(), xs[0], 0 if history is None else history.data_ptr(), hs[0], lp, pp, rp, ep, fp,
+        logits.data_ptr(), xs[0], hp, hs[0], lp, pp, rp, ep, fp,
         0 if bias is None else bias_ids.data_ptr(), 0 if bias is None else bias.data_ptr(),
         0 if mask is None else mask.data_ptr(), ms[0], out.data_ptr(), os_[0], M, V, width, n_bias), out, stream)
