@@ -438,3 +438,23 @@ def test_long_cache_of_many_rows_a_head(cuda):
     assert Y.status() == 0
     rows = [torch.cat([c[-3:-1].reshape(-1, 1, D)[:P], c[-1, :100]]) for c in (kc, vc)]
     near(q, [rows], out, [0, T], (T,), (P + 100,))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("new,lens,P", [((1, 1), (60, 150), 40), ((20, 5), (60, 150), 40), ((4,) * 30, (900,) * 30, 800)])
+def test_gates_of_any_size(cuda, new, lens, P, dtype):
+    """Infinite and large gates: all of the output or none of it."""
+    import torch
+    import yskn_b200 as Y
+    g = torch.zeros((sum(new), 6, 128), device=cuda)
+    for i, x in enumerate((float("inf"), 3e38, 200.0, 89.0, -float("inf"), -3e38, -200.0, -89.0)):
+        g[:, :, i::8] = x
+    g = g.to({"bf16": torch.bfloat16, "f32": torch.float32}[dtype])
+    q, rows, out, starts = call(cuda, new, lens, P, float("nan"), gate=g, seed=30)
+    bare = call(cuda, new, lens, P, float("nan"), seed=30)[2]
+    assert Y.status() == 0
+    for i in range(8):
+        if i < 4:
+            assert torch.equal(out[:, :, i::8], bare[:, :, i::8])
+        else:
+            assert bool((out[:, :, i::8].abs() <= 2.0 ** -25).all())
