@@ -592,8 +592,8 @@ YSKN_B200_API int yskn_b200_kv_encode(const float* d_rows, const int32_t* d_row_
  * blocks are back). Written: lens_out [batch] and *free_out (arrays of their own: keep
  * two of each and swap them), starts [batch + 1] (served tokens before each request), and
  * per token slots int64 (block * block_size + place, for yskn_b200_paged_prep), positions
- * and requests int32 [max_tokens, at most 2^30], -1 past the last served token. Lengths or a count that
- * do not fit their arrays give YSKN_EINVAL from yskn_b200_status. One launch. */
+ * and requests int32 [max_tokens] (at most 2^30), -1 past the last served token. Lengths or a
+ * count that do not fit their arrays give YSKN_EINVAL from yskn_b200_status. One launch. */
 typedef struct {
   const int32_t *lens, *new_lens; /* [batch] */
   int32_t* block_tables;
@@ -641,14 +641,14 @@ YSKN_B200_API int yskn_b200_paged_prep(const yskn_b200_paged_prep_args* args, vo
 
 /* Attention of the batch's new tokens over the shared prefix and each request's own rows.
  * Request i's tokens are starts[i] .. starts[i + 1] - 1 of `tokens` (rows past
- * starts[batch] are padding), at most max_new (tokens or more: no bound), and the last of its lens[i] rows; token t of
- * n sees the first max(0, len - n + t + 1) rows: below prefix_len in prefix_blocks
- * int32 [ceil(prefix_len / block_size)], from there on in the request's row of
+ * starts[batch] are padding), at most max_new (tokens or more: no bound), and the last of its
+ * lens[i] rows; token t of n sees the first max(0, len - n + t + 1) rows: below prefix_len in
+ * prefix_blocks int32 [ceil(prefix_len / block_size)], from there on in the request's row of
  * block_tables. out = softmax(scale * q k^T) v in binary32 sums, times sigmoid(gate) if
  * gate is given, rounded once; a token that sees nothing, padding included, gives zeros.
- * Cache rows that no token sees may hold anything; one that some token of a request sees holds numbers
- * (for the tokens that do not see it its weight is zero, and zero times infinity is NaN). q, gate: element (token, head, channel)
- * at token * row + head * head_stride + channel; out dense [tokens][n_qh][head]; query head
+ * Cache rows that no token sees may hold anything; one that some token sees holds numbers (for the
+ * tokens that do not see it its weight is zero, and zero times infinity is NaN). q, gate: element
+ * (token, head, channel) at token * row + head * head_stride + channel; out dense [tokens][n_qh][head]; query head
  * j reads KV head j / (n_qh / n_kvh), at most 128 query heads each. dtype YSKN_DT_F16 or
  * _BF16 for all of them (the softmax weights are rounded to it for the tensor cores), gate_dtype
  * the same or YSKN_DT_F32 (the gate as a projection leaves it); heads of

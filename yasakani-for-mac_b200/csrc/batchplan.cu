@@ -279,7 +279,8 @@ extern "C" YSKN_B200_API int yskn_b200_batch_plan(const yskn_b200_batch_plan_arg
   if (a.batch < 1 || a.batch > YSKN_PLAN_MAX_BATCH || a.block_size < 1 || a.prefix_len < 0 || a.table_width < 1 ||
       (a.batch > 1 && a.table_stride < a.table_width) || a.pool_capacity < 1 || a.max_tokens < 0)
     return fail(YSKN_EINVAL, "batch_plan: batch outside 1..4096, or a size or stride out of range");
-  if (a.max_tokens > 1 << 30) return fail(YSKN_EINVAL, "batch_plan: more than 2^30 tokens");  // a CTA's last is below 2^31
+  if (a.max_tokens > 1 << 30)  // the last warp's places stay below 2^31
+    return fail(YSKN_EINVAL, "batch_plan: more than 2^30 tokens");
   if (a.lens_out == a.lens || a.free_out == a.free)
     return fail(YSKN_EINVAL, "batch_plan: the new lengths and the new count need arrays of their own");
   PlanParams p{a.lens, a.new_lens, a.block_tables, a.table_stride, a.table_width, a.pool, a.pool_capacity, a.free,

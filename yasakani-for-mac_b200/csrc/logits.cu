@@ -18,7 +18,7 @@
 // the one before, while 16 warps stream the present one, so that the memory does not wait for
 // the counting. (Of 256 rows of 151936 with up to 16384 tokens of history: one logit a thread
 // 255 us; 16-byte accesses, counting and streaming in turn in four CTAs an SM 114; this way
-// 81. Streaming a plain copy and adjusting the history's logits afterwards took 141: two
+// 82. Streaming a plain copy and adjusting the history's logits afterwards took 141: two
 // million scattered 4-byte updates.) Some of nearly every 128 neighbouring tokens are in a
 // long history, so the penalties run for nearly every warp: no division among them (Penalties).
 // A token's count: the top bit for a token of the prompt, the others the count after it, so that
@@ -100,7 +100,7 @@ struct LogitsCount {
 // off by 2^-52 of itself before that, and a quotient of two 24-bit numbers that is normal in binary32
 // lies 2^-49 of itself or more from where binary32's rounding turns, so this is the division's result;
 // infinities, overflow and penalties of any size included. A subnormal quotient half way between two
-// numbers may fall on the other one. (256 rows of 151936: 81.5 us; the division where binary32's
+// numbers may fall on the other one. (256 rows of 151936: 82 us; the division where binary32's
 // product and one Newton step do not hold, as a rare branch, 98.)
 struct Penalties {
   float rep, pres, freq;

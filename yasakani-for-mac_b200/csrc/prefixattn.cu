@@ -81,6 +81,10 @@ constexpr int PA_ITEM_COST = 3;    // an item's fixed cost (Q, the last P V's wa
 // Thin items. Cost, least and time per tile as they served 64 requests best (us behind 32k rows, and
 // without a prefix): costs of 1, 3, 5: 100 and 50, 93 and 46, 81 and 41; times of 10, 14, 18 and 22:
 // 93, 89, 81, 97. A least of 2 rather than 4: two requests 13.7, not 14.8; of 1: 8 requests 17.2, not 15.7.
+// All that at heads of 256 and 6 query heads a KV head. The time per tile at others, us behind 32k rows with 18, 22
+// and 28: heads of 128 with 2, 4, 8 query heads 43, 46, 57, then 41, 45, 56, then 41, 43, 54; heads of 64 36, 36, 51,
+// then 34, 34, 50, then 33, 33, 48; heads of 256 64, 66, 81, then 64, 65, 100, then 68, 69, 96: one number for all
+// costs the smaller heads up to 7 %, a larger one the large heads a fifth.
 constexpr int PA_THIN_ROWS = 8;       // rows of a thin item, at most
 constexpr int PA_THIN_SHIFT = 4;      // its tiles: 16 rows of the cache
 constexpr int PA_THIN_COST = 5;       // its fixed cost in such tiles
