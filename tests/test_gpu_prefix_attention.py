@@ -458,3 +458,22 @@ def test_gates_of_any_size(cuda, new, lens, P, dtype):
             assert torch.equal(out[:, :, i::8], bare[:, :, i::8])
         else:
             assert bool((out[:, :, i::8].abs() <= 2.0 ** -25).all())
+
+
+@pytest.mark.parametrize("P", [0, 3000])
+@pytest.mark.parametrize("n_qh", [6, 40])
+@pytest.mark.parametrize("starts", [(0, 2 ** 31 - 1, -2 ** 31, 1), (2 ** 31 - 1, -2 ** 31, 0, 2), (-2 ** 31, 2 ** 31 - 1, 0, 0),
+                                    (3, 4, 4, 3), (-1, 0, 0, 0), (2 ** 31 - 2, 2 ** 31 - 1, -2 ** 31, 0)])
+def test_starts_of_any_value_are_reported(cuda, P, n_qh, starts):
+    """Tokens that the call does not have, and differences that pass 32 bits."""
+    import torch
+    import yskn_b200 as Y
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=cuda)  # noqa: E731
+    c = torch.ones((8, 16, 2, 64), dtype=torch.bfloat16, device=cuda)
+    q = torch.ones((2, n_qh, 64), dtype=torch.bfloat16, device=cuda)
+    out = torch.full((2, n_qh, 64), 3.0, dtype=torch.bfloat16, device=cuda)
+    work = torch.full((Y.prefix_attention_work_bytes(2, 3, 1, n_qh, 2, 64),), 255, dtype=torch.uint8, device=cuda)
+    Y.prefix_attention(q, c, c, i32([[0, 1, 2, 3]] * 3), i32([P + 60] * 3), i32(starts), 1, work, out,
+                       prefix_blocks=i32([5] * 188), prefix_len=P)
+    assert Y.status() == Y.EINVAL
+    assert bool(torch.isin(out, torch.tensor([0.0, 1.0], dtype=torch.bfloat16, device=cuda)).all())

@@ -207,9 +207,9 @@ struct PaRequest {
 __device__ __forceinline__ PaRequest pa_request(const PrefixAttnParams& p, int i) {
   PaRequest r;
   r.s0 = __ldg(p.starts + i);
-  const int n = __ldg(p.starts + i + 1) - r.s0;
+  const int n = (int)((unsigned)__ldg(p.starts + i + 1) - (unsigned)r.s0);  // whatever the two are
   r.len = __ldg(p.lens + i);
-  r.n = n < 0 || n > p.max_new || r.s0 < 0 || r.s0 + n > p.tokens ? 0 : n;
+  r.n = n < 0 || n > p.max_new || r.s0 < 0 || r.s0 > p.tokens - n ? 0 : n;
   return r;
 }
 // Own rows that the last of the request's first `upto` tokens sees.
@@ -857,7 +857,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
       units_of[1] = pa_sum(units_of[1], times(pa_own_units(p, r, nq, true)));
       items = pa_sum(items, times(nq));
       if (r.n > 0) seen = max(seen, (unsigned)pa_visible_prefix(p, r, r.n));
-      if (blockIdx.x == 0 && (__ldg(p.starts + i + 1) - r.s0 != r.n ||
+      if (blockIdx.x == 0 && (__ldg(p.starts + i + 1) != r.s0 + r.n ||
                               (r.n > 0 && r.len > p.prefix_len && r.len - p.prefix_len > p.own_limit)))
         raise_device_error(p.err, DERR_RANGE);
     }
