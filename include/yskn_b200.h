@@ -705,6 +705,147 @@ typedef struct {
 } yskn_b200_logits_adjust_args;
 YSKN_B200_API int yskn_b200_logits_adjust(const yskn_b200_logits_adjust_args* args, void* stream);
 
+/* ---- Drafted trees, copies of requests, log probabilities ------------------------------
+ * No counterpart in the reference. A draft proposes a tree of tokens for each request of a batch;
+ * one step over all its nodes tells which path the model itself would have taken:
+ *   batch_plan (a new token for each node) -> tree_plan -> per layer paged_prep and tree_attention ->
+ *   head, head_select (the model's choice after each node) -> tree_accept -> cache_compact -> batch_edit.
+ * Node 0 of a request is its next token, known but not in the cache yet; a later node follows one of
+ * those before it. Requests that continue others (beams, several answers) are batch_edit and cache_copy. */
+
+/* Ancestor bits and positions of a step's nodes. Token t is new token t - starts[r] of request r =
+ * requests[t] (as yskn_b200_batch_plan writes them; negative: padding); parents[t] is the new token of
+ * its request that it follows, counted from the request's first, negative for one that follows the
+ * request's cached rows. mask uint32 [tokens][mask_stride], mask_words (1..YSKN_TREE_MAX_WORDS) of them
+ * written: bit j % 32 of word j / 32 is set for j = the node itself and its ancestors. positions
+ * [tokens]: lens[r] - n + the number of its ancestors (lens with the n new rows). Padding gives no
+ * bits and position -1. A parent at or behind its node (taken for none), a node past the mask's bits
+ * (not set) or starts that do not hold t give YSKN_EINVAL from yskn_b200_status. One launch. */
+#define YSKN_TREE_MAX_WORDS 32
+typedef struct {
+  const int32_t *parents, *requests, *starts, *lens; /* [tokens], [tokens], [batch + 1], [batch] */
+  uint32_t* mask;
+  int64_t mask_stride;
+  int32_t* positions;
+  int tokens, batch, mask_words;
+} yskn_b200_tree_plan_args;
+YSKN_B200_API int yskn_b200_tree_plan(const yskn_b200_tree_plan_args* args, void* stream);
+
+/* yskn_b200_prefix_attention where a request's new tokens do not follow one another: new token t sees
+ * every row before the request's new ones, and of those row j <= t if bit j % 32 of word j / 32 of its
+ * mask row is set (uint32 mask [tokens][mask_stride], mask_words of them; bits past them count as
+ * 0, and a request of more new tokens gives YSKN_EINVAL from yskn_b200_status). Everything else as
+ * there, its workspace among it: a row that no bit and no cached row leaves anything gives zeros, and the
+ * new rows hold numbers. */
+typedef struct {
+  yskn_b200_prefix_attention_args attn;
+  const uint32_t* mask;
+  int64_t mask_stride;
+  int mask_words;
+} yskn_b200_tree_attention_args;
+YSKN_B200_API int yskn_b200_tree_attention(const yskn_b200_tree_attention_args* args, void* stream);
+
+/* The accepted path of each request's tree: node 0, then the first node (in index order) whose parent
+ * is the last one and whose token (tokens [tokens]) is the model's choice after it (choice [tokens], as
+ * yskn_b200_head_select writes it; a negative one is no node's), and so on, up to path_width nodes. path
+ * int32 [batch][path_stride]: its nodes, counted from the request's first new token, -1 after
+ * them; accepted [batch]: how many; lens_out [batch]: lens less the new rows that are not on the path (may
+ * be lens); next [batch]: the choice after the last one (-1 for a request without tokens). Starts that
+ * do not ascend within tokens give YSKN_EINVAL from yskn_b200_status and an empty path. One launch. */
+typedef struct {
+  const int32_t *tokens, *parents, *choice; /* [n_tokens] */
+  const int32_t *starts, *lens;             /* [batch + 1], [batch] */
+  int32_t* path;
+  int64_t path_stride;
+  int32_t *accepted, *lens_out, *next; /* [batch] */
+  int batch, n_tokens, path_width;
+} yskn_b200_tree_accept_args;
+YSKN_B200_API int yskn_b200_tree_accept(const yskn_b200_tree_accept_args* args, void* stream);
+
+/* Which rows each request keeps, and whose it continues. Arrays as in yskn_b200_batch_plan (blocks
+ * given back go on top of the pool in the requests' order, new ones come from the top). Request i becomes
+ * the first min(keep[i], lens[source[i]]) rows of request source[i] (source NULL: its own; a negative one:
+ * the request ends, its length 0). Of the requests that continue j, the one that keeps most rows (the
+ * lowest of several) goes on in j's blocks; each other one gets fresh blocks for its own rows
+ * (those after the shared prefix), and the copies that fill them are listed, requests in order:
+ * copies int32 [3][copies_stride], max_copies used: the block to read, the block to write, its rows; -1,
+ * -1, 0 past the last of *n_copies. Such a request is served if the pool and the list hold its blocks
+ * with those of all such requests before it; else it ends (length 0, no blocks). What no one goes on
+ * in goes back to the pool. Written: lens_out [batch], *free_out (arrays of their own), the pool, and
+ * with a source tables_out [batch][tables_out_stride] (an array of its own; entries of the kept
+ * blocks; without a source the tables stay valid and tables_out, copies and n_copies are not used).
+ * Lengths, sources or a count that do not fit their arrays give YSKN_EINVAL from yskn_b200_status. One launch. */
+typedef struct {
+  const int32_t *lens, *keep, *source; /* [batch] */
+  const int32_t* block_tables;
+  int64_t table_stride;
+  int32_t* tables_out;
+  int64_t tables_out_stride;
+  int32_t* pool;
+  const int32_t* free;
+  int32_t *lens_out, *free_out;
+  int32_t* copies;
+  int64_t copies_stride;
+  int32_t* n_copies;
+  int batch, block_size, prefix_len, table_width, pool_capacity, max_copies;
+} yskn_b200_batch_edit_args;
+YSKN_B200_API int yskn_b200_batch_edit(const yskn_b200_batch_edit_args* args, void* stream);
+
+/* Copies blocks within each of n_caches 16-bit caches (host array of device pointers, read before the
+ * call returns, at most YSKN_MAX_CACHES; all of one shape and strides, as in yskn_b200_paged_prep): for
+ * each of the first *count entries (NULL: max_copies) of the list that yskn_b200_batch_edit writes, rows
+ * 0..rows - 1 of every head of block copies[0][e] to block copies[1][e]. Entries without rows are none; a block
+ * outside the caches, or more rows than a block has, is not copied and gives YSKN_EINVAL from
+ * yskn_b200_status. No block is written twice, or written and read, in one call. Pointers and strides are
+ * multiples of 16 bytes, heads of 64, 128 or 256 channels. One launch. */
+#define YSKN_MAX_CACHES 256
+typedef struct {
+  void* const* caches;
+  int64_t block_stride, token_stride, head_stride;
+  const int32_t* copies;
+  int64_t copies_stride;
+  const int32_t* count;
+  int n_caches, n_blocks, block_size, n_kvh, head, max_copies;
+} yskn_b200_cache_copy_args;
+YSKN_B200_API int yskn_b200_cache_copy(const yskn_b200_cache_copy_args* args, void* stream);
+
+/* Makes the rows of accepted paths adjacent in every cache (as in yskn_b200_cache_copy): of request i, whose
+ * starts[i + 1] - starts[i] new rows are the last of its lens[i] (lens with the new rows), new row path[i][k]
+ * goes to the place of new row k, for k = 0, 1, ... up to the first negative entry or path_width. A path
+ * that does not ascend, or a node that the request does not have, ends there, and a block outside the
+ * caches is left alone; both give YSKN_EINVAL from yskn_b200_status. One launch. */
+typedef struct {
+  void* const* caches;
+  int64_t block_stride, token_stride, head_stride;
+  const int32_t* block_tables;
+  int64_t table_stride;
+  const int32_t *lens, *starts;
+  const int32_t* path;
+  int64_t path_stride;
+  int n_caches, n_blocks, block_size, n_kvh, head, batch, table_width, prefix_len, path_width;
+} yskn_b200_cache_compact_args;
+YSKN_B200_API int yskn_b200_cache_compact(const yskn_b200_cache_compact_args* args, void* stream);
+
+/* Log probabilities of f32 logits [rows][vocab] (row stride in elements; any 4-byte alignment): of the
+ * tokens int32 [rows][n_tokens] (row stride token_stride) into logprobs [rows][n_tokens], -inf for one
+ * outside the vocabulary (padding); entropy [rows] (NULL: none) in nats; the n_top (0..YSKN_MAX_TOP) most
+ * likely tokens, equal ones by the lowest number, into top_logprobs and top_ids [rows][n_top], -inf and
+ * -1 past the last token of a logit above -inf. A row of nothing but -inf gives -inf throughout and
+ * entropy 0; one that holds NaN or +inf gives NaN throughout and no tokens (-1). In binary32, the others'
+ * sum kept apart from the likeliest token's 1, so that a sure row keeps its small numbers. One
+ * launch, no workspace. */
+#define YSKN_MAX_TOP 32
+typedef struct {
+  const float* logits;
+  int64_t logits_stride;
+  const int32_t* tokens;
+  int64_t token_stride;
+  float *logprobs, *entropy, *top_logprobs;
+  int32_t* top_ids;
+  int rows, vocab, n_tokens, n_top;
+} yskn_b200_token_logprobs_args;
+YSKN_B200_API int yskn_b200_token_logprobs(const yskn_b200_token_logprobs_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

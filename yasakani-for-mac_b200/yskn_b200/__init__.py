@@ -98,6 +98,13 @@ _SIGNATURES = {
     "yskn_b200_prefix_attention_work_bytes": (_i64, [_i] * 6),
     "yskn_b200_prefix_attention": (_i, [C.c_char_p, _vp]),
     "yskn_b200_logits_adjust": (_i, [C.c_char_p, _vp]),
+    "yskn_b200_tree_plan": (_i, [C.c_char_p, _vp]),
+    "yskn_b200_tree_attention": (_i, [C.c_char_p, _vp]),
+    "yskn_b200_tree_accept": (_i, [C.c_char_p, _vp]),
+    "yskn_b200_batch_edit": (_i, [C.c_char_p, _vp]),
+    "yskn_b200_cache_copy": (_i, [C.c_char_p, _vp]),
+    "yskn_b200_cache_compact": (_i, [C.c_char_p, _vp]),
+    "yskn_b200_token_logprobs": (_i, [C.c_char_p, _vp]),
 }
 
 _lib = None
@@ -677,6 +684,13 @@ ARGS = {
     "paged_prep": struct.Struct("@3P6q2PqP2P3P3q10if128s0P"),
     "prefix_attention": struct.Struct("@P2qP2q2P3q2Pq2PPqP12if0P"),
     "logits_adjust": struct.Struct("@PqPq2P3P2PPqPq4i0P"),
+    "tree_plan": struct.Struct("@5PqP3i0P"),
+    "tree_attention": struct.Struct("@P2qP2q2P3q2Pq2PPqP12if0PPqi0P"),  # prefix_attention's, then the masks
+    "tree_accept": struct.Struct("@6Pq3P3i0P"),
+    "batch_edit": struct.Struct("@4PqPq5PqP6i0P"),
+    "cache_copy": struct.Struct("@P3qPqP6i0P"),
+    "cache_compact": struct.Struct("@P3qPq3Pq9i0P"),
+    "token_logprobs": struct.Struct("@PqPq4P4i0P"),
 }
 _DT, _FN = {}, {}
 
@@ -685,6 +699,7 @@ def _types():
     import torch
     _DT.update({torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.int16: DT_BF16})
     _DT["i32"], _DT["i64"] = torch.int32, torch.int64
+    _DT["device"] = torch.cuda.current_device
     # the raw handle at once: building a torch.cuda.Stream object around it takes longer than a launch
     _DT["stream"] = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
         lambda device: torch.cuda.current_stream(device).cuda_stream)
@@ -788,13 +803,9 @@ def prefix_attention_work_bytes(tokens, batch, max_new, n_qh, n_kvh, head):
     return n
 
 
-def prefix_attention(q, k_cache, v_cache, block_tables, lens, starts, max_new, work, out, prefix_blocks=None,
-                     prefix_len=0, gate=None, scale=None, stream=None):
-    """yskn_b200_prefix_attention: q and gate (of q's type, or f32) [T][n_qh][D] with dense
-    channels, the caches as paged_prep, each request's own blocks in block_tables (int32
-    [batch][width]) and the shared prefix's in prefix_blocks; lens and starts as batch_plan writes them (at most max_new tokens
-    a request) -> out (dense [T][n_qh][D]). scale defaults to 1 / sqrt(D). work: uint8, of
-    prefix_attention_work_bytes(T, batch, max_new, n_qh, n_kvh, D) bytes."""
+def _attention_args(name, q, k_cache, v_cache, block_tables, lens, starts, max_new, work, out, prefix_blocks,
+                    prefix_len, gate, scale):
+    """The checked arguments of prefix_attention, as its struct has them."""
     if not _DT:
         _types()
     i32, dt = _DT["i32"], q.dtype
@@ -805,24 +816,36 @@ def prefix_attention(q, k_cache, v_cache, block_tables, lens, starts, max_new, w
     qs, cs, row = q.stride(), k_cache.stride(), block_tables.stride()
     _need(q.shape == shape and cache[3] == D and v_cache.shape == cache and v_cache.stride() == cs and cs[3] == 1 and
           qs[2] == 1 and out.is_contiguous() and k_cache.dtype is dt and v_cache.dtype is dt and out.dtype is dt,
-          "prefix_attention: q, out and caches of one type and head size with dense channels expected")
+          name + ": q, out and caches of one type and head size with dense channels expected")
     _need(block_tables.dtype is i32 and lens.dtype is i32 and starts.dtype is i32 and lens.numel() == B and
           starts.numel() == B + 1 and row[1] == 1 and lens.is_contiguous() and starts.is_contiguous() and
           work.is_contiguous() and
           (not prefix_len or (prefix_blocks is not None and prefix_blocks.dtype is i32 and
                               prefix_blocks.is_contiguous() and prefix_blocks.numel() * block_size >= prefix_len)),
-          "prefix_attention: dense int32 tables, lengths and starts of one batch, and the prefix's blocks expected")
+          name + ": dense int32 tables, lengths and starts of one batch, and the prefix's blocks expected")
     gs, gd = (0, 0), 0
     if gate is not None:
         gs, gd = gate.stride(), _dtype(gate)
         _need(gate.shape == shape and gs[2] == 1,
-              "prefix_attention: a gate of the queries' shape with dense channels expected")
-    _launch("prefix_attention", ARGS["prefix_attention"].pack(
+              name + ": a gate of the queries' shape with dense channels expected")
+    return (
         q.data_ptr(), qs[0], qs[1], 0 if gate is None else gate.data_ptr(), gs[0], gs[1], k_cache.data_ptr(),
         v_cache.data_ptr(), cs[0], cs[1], cs[2], prefix_blocks.data_ptr() if prefix_len else 0,
         block_tables.data_ptr(), row[0], lens.data_ptr(), starts.data_ptr(), work.data_ptr(),
         work.numel() * work.element_size(), out.data_ptr(), n_blocks, block_size, prefix_len, width, B, T, max_new,
-        n_qh, n_kvh, D, _dtype(q), gd, D ** -0.5 if scale is None else scale), out, stream)
+        n_qh, n_kvh, D, _dtype(q), gd, D ** -0.5 if scale is None else scale)
+
+
+def prefix_attention(q, k_cache, v_cache, block_tables, lens, starts, max_new, work, out, prefix_blocks=None,
+                     prefix_len=0, gate=None, scale=None, stream=None):
+    """yskn_b200_prefix_attention: q and gate (of q's type, or f32) [T][n_qh][D] with dense
+    channels, the caches as paged_prep, each request's own blocks in block_tables (int32
+    [batch][width]) and the shared prefix's in prefix_blocks; lens and starts as batch_plan writes them (at most max_new tokens
+    a request) -> out (dense [T][n_qh][D]). scale defaults to 1 / sqrt(D). work: uint8, of
+    prefix_attention_work_bytes(T, batch, max_new, n_qh, n_kvh, D) bytes."""
+    _launch("prefix_attention", ARGS["prefix_attention"].pack(*_attention_args(
+        "prefix_attention", q, k_cache, v_cache, block_tables, lens, starts, max_new, work, out, prefix_blocks,
+        prefix_len, gate, scale)), out, stream)
 
 
 def logits_adjust(logits, out, history=None, history_lens=None, prompt_lens=None, repetition=None, presence=None,
@@ -875,3 +898,176 @@ def logits_adjust(logits, out, history=None, history_lens=None, prompt_lens=None
         logits.data_ptr(), xs[0], hp, hs[0], lp, pp, rp, ep, fp,
         0 if bias is None else bias_ids.data_ptr(), 0 if bias is None else bias.data_ptr(),
         0 if mask is None else mask.data_ptr(), ms[0], out.data_ptr(), os_[0], M, V, width, n_bias), out, stream)
+
+
+def _on(what, *tensors):
+    """All on the current device, which the call is launched on."""
+    at = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != at:
+            at = -1
+    _need(at >= 0 and at == _DT["device"](), what + ": tensors on the current device expected")
+
+
+def _dense(dtype, *tensors):
+    return all(t.dtype is dtype and t.is_contiguous() for t in tensors)
+
+
+def tree_plan(parents, requests, starts, lens, mask, positions, stream=None):
+    """yskn_b200_tree_plan: for each new token (parents int32 [T]: the new token of its request that it follows,
+    negative for none; requests, starts and lens as batch_plan writes them) the bits of itself and its ancestors
+    (mask int32 [T][words], a bit a new token of its request) and its position (int32 [T])."""
+    if not _DT:
+        _types()
+    i32, T, B = _DT["i32"], parents.numel(), lens.numel()
+    _need(_dense(i32, parents, requests, starts, lens, positions) and mask.dtype is i32 and mask.dim() == 2 and
+          mask.shape[0] == T and mask.stride(1) == 1 and requests.numel() == T and positions.numel() == T and
+          starts.numel() == B + 1, "tree_plan: int32 arrays of one batch and a mask row for each token expected")
+    _on("tree_plan", parents, requests, starts, lens, mask, positions)
+    _launch("tree_plan", ARGS["tree_plan"].pack(
+        parents.data_ptr(), requests.data_ptr(), starts.data_ptr(), lens.data_ptr(), mask.data_ptr(), mask.stride(0),
+        positions.data_ptr(), T, B, mask.shape[1]), parents, stream)
+
+
+def tree_attention(q, k_cache, v_cache, block_tables, lens, starts, max_new, mask, work, out, prefix_blocks=None,
+                   prefix_len=0, gate=None, scale=None, stream=None):
+    """yskn_b200_tree_attention: prefix_attention in which a new token sees, of its request's new rows, only
+    those up to itself whose bit is set in its row of mask (int32 [T][words], as tree_plan writes it)."""
+    args = _attention_args("tree_attention", q, k_cache, v_cache, block_tables, lens, starts, max_new, work, out,
+                           prefix_blocks, prefix_len, gate, scale)
+    _need(mask.dtype is _DT["i32"] and mask.dim() == 2 and mask.shape[0] == q.shape[0] and mask.stride(1) == 1,
+          "tree_attention: an int32 mask row for each token expected")
+    _on("tree_attention", q, k_cache, v_cache, block_tables, lens, starts, mask, work, out, prefix_blocks, gate)
+    _launch("tree_attention", ARGS["tree_attention"].pack(*args, mask.data_ptr(), mask.stride(0), mask.shape[1]), out,
+            stream)
+
+
+def tree_accept(tokens, parents, choice, starts, lens, path, accepted, lens_out, next_token, stream=None):
+    """yskn_b200_tree_accept: of each request's tree (tokens and parents int32 [T]) the path that the model's choices
+    (int32 [T], after each node) take: path (int32 [batch][width], -1 past its end), how many nodes it has,
+    the lengths without the others' rows, and the choice after its last node (int32 [batch] each)."""
+    if not _DT:
+        _types()
+    i32, T, B = _DT["i32"], tokens.numel(), lens.numel()
+    _need(_dense(i32, tokens, parents, choice, starts, lens, accepted, lens_out, next_token) and path.dtype is i32 and
+          path.dim() == 2 and path.shape[0] == B and path.stride(1) == 1 and parents.numel() == T and
+          choice.numel() == T and starts.numel() == B + 1 and accepted.numel() == B and lens_out.numel() == B and
+          next_token.numel() == B, "tree_accept: int32 arrays of one batch and a path row for each request expected")
+    _on("tree_accept", tokens, parents, choice, starts, lens, path, accepted, lens_out, next_token)
+    _launch("tree_accept", ARGS["tree_accept"].pack(
+        tokens.data_ptr(), parents.data_ptr(), choice.data_ptr(), starts.data_ptr(), lens.data_ptr(), path.data_ptr(),
+        path.stride(0), accepted.data_ptr(), lens_out.data_ptr(), next_token.data_ptr(), B, T, path.shape[1]), tokens,
+        stream)
+
+
+def batch_edit(lens, keep, block_tables, pool, free_count, block_size, lens_out, free_out, source=None, tables_out=None,
+               copies=None, n_copies=None, prefix_len=0, stream=None):
+    """yskn_b200_batch_edit: request i keeps its first keep[i] rows, or becomes the first keep[i] rows of request
+    source[i] (int32 [batch]; negative: it ends). Without a source the block tables stay valid; with one the new
+    tables go to tables_out, and the blocks that cache_copy has to copy to copies (int32 [3][n]: block to read,
+    block to write, rows) and their number to n_copies (int32 [1])."""
+    if not _DT:
+        _types()
+    i32 = _DT["i32"]
+    B, width = block_tables.shape
+    _need(_dense(i32, lens, keep, pool, free_count, lens_out, free_out) and block_tables.dtype is i32 and
+          block_tables.stride(1) == 1 and lens.numel() == B and keep.numel() == B and lens_out.numel() == B and
+          free_count.numel() and free_out.numel(), "batch_edit: dense int32 arrays of the batch expected")
+    ts, cs, n, tail = (0, 1), (0, 1), 0, (0, 0, 0, 0)
+    if source is not None:
+        _need(tables_out is not None and copies is not None and n_copies is not None,
+              "batch_edit: a source needs new tables, a list of copies and its count")
+        ts, cs, n = tables_out.stride(), copies.stride(), copies.shape[-1]
+        _need(_dense(i32, source, n_copies) and source.numel() == B and n_copies.numel() and tables_out.dtype is i32 and
+              tables_out.shape == (B, width) and ts[1] == 1 and copies.dtype is i32 and copies.dim() == 2 and
+              copies.shape[0] == 3 and cs[1] == 1,
+              "batch_edit: int32 source, tables of one shape and copies [3][n] expected")
+        tail = (source.data_ptr(), tables_out.data_ptr(), copies.data_ptr(), n_copies.data_ptr())
+        _on("batch_edit", source, tables_out, copies, n_copies)
+    _on("batch_edit", lens, keep, block_tables, pool, free_count, lens_out, free_out)
+    _launch("batch_edit", ARGS["batch_edit"].pack(
+        lens.data_ptr(), keep.data_ptr(), tail[0], block_tables.data_ptr(), block_tables.stride(0), tail[1], ts[0],
+        pool.data_ptr(), free_count.data_ptr(), lens_out.data_ptr(), free_out.data_ptr(), tail[2], cs[0], tail[3], B,
+        block_size, prefix_len, width, pool.numel(), n), lens, stream)
+
+
+class CacheSet:
+    """The K and V caches of a model's layers (16-bit views [n_blocks][block_size][n_kvh][D] of one shape and
+    strides, as paged_prep takes them), for cache_copy and cache_compact. Keeps them alive."""
+
+    def __init__(self, caches):
+        caches = list(caches)
+        _need(len(caches) > 0, "CacheSet: at least one cache expected")
+        first = caches[0]
+        _need(all(c.dim() == 4 and c.element_size() == 2 and c.dtype == first.dtype and c.shape == first.shape and
+                  c.stride() == first.stride() and c.device == first.device for c in caches) and first.stride(3) == 1,
+              "CacheSet: 16-bit caches of one type, shape, strides and device with dense channels expected")
+        self.caches = caches
+        self._addresses = (C.c_void_p * len(caches))(*[c.data_ptr() for c in caches])
+        n_blocks, block_size, n_kvh, head = first.shape
+        s = first.stride()
+        self._head = (C.addressof(self._addresses), s[0], s[1], s[2])
+        self._sizes = (len(caches), n_blocks, block_size, n_kvh, head)
+
+
+def cache_copy(caches, copies, count=None, stream=None):
+    """yskn_b200_cache_copy: in every cache of the CacheSet the blocks that batch_edit lists (copies int32 [3][n]:
+    block to read, block to write, rows), the first *count (int32 [1]) of them or all."""
+    if not _DT:
+        _types()
+    i32 = _DT["i32"]
+    _need(copies.dtype is i32 and copies.dim() == 2 and copies.shape[0] == 3 and copies.stride(1) == 1 and
+          (count is None or (count.dtype is i32 and count.numel())),
+          "cache_copy: int32 copies [3][n] and a count expected")
+    _on("cache_copy", caches.caches[0], copies, count)
+    _launch("cache_copy", ARGS["cache_copy"].pack(
+        *caches._head, copies.data_ptr(), copies.stride(0), 0 if count is None else count.data_ptr(), *caches._sizes,
+        copies.shape[1]), copies, stream)
+
+
+def cache_compact(caches, block_tables, lens, starts, path, prefix_len=0, stream=None):
+    """yskn_b200_cache_compact: in every cache of the CacheSet, of each request's new rows (the last of its lens, as
+    many as its starts say) those on its path (int32 [batch][width], as tree_accept writes it) made adjacent."""
+    if not _DT:
+        _types()
+    i32 = _DT["i32"]
+    B, width = block_tables.shape
+    _need(block_tables.dtype is i32 and block_tables.stride(1) == 1 and _dense(i32, lens, starts) and
+          lens.numel() == B and starts.numel() == B + 1 and path.dtype is i32 and path.dim() == 2 and
+          path.shape[0] == B and path.stride(1) == 1,
+          "cache_compact: int32 tables, lengths, starts and paths of one batch expected")
+    _on("cache_compact", caches.caches[0], block_tables, lens, starts, path)
+    _launch("cache_compact", ARGS["cache_compact"].pack(
+        *caches._head, block_tables.data_ptr(), block_tables.stride(0), lens.data_ptr(), starts.data_ptr(),
+        path.data_ptr(), path.stride(0), *caches._sizes, B, width, prefix_len, path.shape[1]), lens, stream)
+
+
+def token_logprobs(logits, tokens=None, logprobs=None, entropy=None, top_logprobs=None, top_ids=None, stream=None):
+    """yskn_b200_token_logprobs: of f32 logits [M][V] (dense rows, any row stride) the log probabilities of tokens
+    (int32 [M][n]) into logprobs (f32 [M][n]), the entropy (f32 [M]), and the most likely tokens into top_logprobs
+    (f32 [M][k]) and top_ids (int32 [M][k]), k up to 32."""
+    if not _DT:
+        _types()
+    i32, f32 = _DT["i32"], logits.dtype
+    (M, V), s = logits.shape, logits.stride()
+    n = k = stride = 0
+    _need(_DT.get(f32) == DT_F32 and s[1] == 1, "token_logprobs: f32 logits with dense rows expected")
+    _need((tokens is None) == (logprobs is None) and (top_ids is None) == (top_logprobs is None),
+          "token_logprobs: tokens and their output, and both outputs of the most likely ones, go together")
+    if tokens is not None:
+        n, stride = tokens.shape[-1], tokens.stride(0)
+        _need(tokens.dtype is i32 and tokens.shape == (M, n) and (tokens.stride(1) == 1 or n < 2) and
+              logprobs.shape == (M, n) and _dense(f32, logprobs),
+              "token_logprobs: int32 tokens [M][n] and dense f32 log probabilities of their shape expected")
+    if top_ids is not None:
+        k = top_ids.shape[-1]
+        _need(top_ids.shape == (M, k) and top_logprobs.shape == (M, k) and _dense(i32, top_ids) and
+              _dense(f32, top_logprobs),
+              "token_logprobs: dense int32 numbers and f32 log probabilities [M][k] expected")
+    _need(entropy is None or (entropy.shape == (M,) and _dense(f32, entropy)),
+          "token_logprobs: f32 entropy [M] expected")
+    _on("token_logprobs", logits, tokens, logprobs, entropy, top_logprobs, top_ids)
+    _launch("token_logprobs", ARGS["token_logprobs"].pack(
+        logits.data_ptr(), s[0], tokens.data_ptr() if n else 0, stride, logprobs.data_ptr() if n else 0,
+        0 if entropy is None else entropy.data_ptr(), top_logprobs.data_ptr() if k else 0,
+        top_ids.data_ptr() if k else 0, M, V, n, k), logits, stream)
