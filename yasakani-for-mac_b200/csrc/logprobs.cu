@@ -11,13 +11,20 @@
 // What bounds it: one read of the logits (4 bytes each); for few rows, the chain of latencies. A
 // cluster of 1 to 8 CTAs takes a row, one part each; the parts are joined through distributed shared
 // memory, so that there is one launch, no workspace and no counter that a second call could meet.
-// A warp streams slices of 4096 bytes (8 16-byte loads a lane under way at once) by itself: its
-// maximum, its sums, and its list of the 32 largest in registers, one a lane, sorted. A logit is a
-// key: its bits in an order of unsigned numbers, above the complement of its number, so that keys are
-// all different and equal logits go by the lowest number. What exceeds the list's n_top-th key goes to a
-// buffer in shared memory; 32 of them are sorted (bitonic, in registers) and merged into the
-// list at once, since one at a time costs as long a chain of shuffles each. The first slice has no
-// such key: the n_top-th largest of its lanes' maxima serves, which at least n_top logits reach.
+// A warp streams its own run of the part in slices of 4096 bytes, 8 16-byte loads a lane for the next slice under way
+// while it works on one: its maximum and its sums. (512 rows of 151936, without the largest tokens: 67 us with three
+// CTAs an SM that load and work in turn, 53 with two that load ahead; two halves of the slice, four CTAs, 50, but with
+// the largest tokens 70 against 62, and 37 against 25 where a CTA is alone.)
+// A logit is a key: its bits in an order of unsigned numbers, above the complement of its number, so that keys are all
+// different and equal logits go by the lowest number. With m = ceil(n_top / 8), the least of the 8 warps' m-th largest
+// lane maxima so far bounds the keys that can be among the n_top largest: at least n_top logits reach it, and few more
+// (20 of the first 8192 logits, 90 of 151936, for 8 largest). What reaches it goes to the warp's buffer in shared
+// memory; in the end each key of the CTA's buffers counts the keys above it, which is its place. Rows whose largest
+// come late fill a buffer: then 32 keys are sorted (bitonic, in registers) and merged into a list of the warp's 32
+// largest, whose n_top-th is a bound too. (All keys through such lists: 93 us for 512 rows, and the chain of shuffles
+// made one row wait 13.)
+// Measured on the device: one row of 151936 with 20 largest 10.9 us (without them 5.6), 33 rows of 50257 9.2, 256 rows
+// of 151936 with 8 largest 33 (4.7 TB/s), 512 rows 62 (5.0 TB/s; two CTAs of 512 on every SM and a half).
 #include <algorithm>
 
 #include "common.cuh"
@@ -25,9 +32,11 @@
 namespace yskn {
 
 constexpr int LP_WARPS = 8, LP_THREADS = LP_WARPS * 32;
-constexpr int LP_LOADS = 8;                         // 16-byte loads of a lane in a slice
-constexpr int LP_SLICE = LP_LOADS * 32;             // 16-byte groups of a warp's slice
+constexpr int LP_LOADS = 8;              // 16-byte loads of a lane in a slice
+constexpr int LP_SLICE = LP_LOADS * 32;  // 16-byte groups of a warp's slice
+constexpr int LP_RESIDENT = 2;           // CTAs of an SM
 constexpr int LP_MAX_CLUSTER = 8;
+constexpr int LP_LEAST_PART = 7500;      // logits of a CTA where a row has several, at least
 constexpr float LP_LOG2E = 1.44269504088896340736f;
 
 struct LogprobsParams {
@@ -44,11 +53,37 @@ struct LpState {
   float m, rest, e;  // the part's maximum (-inf: nothing above it), R and E
 };
 
-__device__ __forceinline__ float lp_exp(float d) {  // d <= 0, -inf included
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d * LP_LOG2E));
+// Two binary32 operations in one instruction.
+__device__ __forceinline__ float2 lp_add2(float2 a, float2 b) {
+  float2 y;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(y.x), "=f"(y.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return y;
 }
+__device__ __forceinline__ float2 lp_mul2(float2 a, float2 b) {
+  float2 y;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(y.x), "=f"(y.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return y;
+}
+__device__ __forceinline__ float2 lp_fma2(float2 a, float2 b, float2 c) {
+  float2 y;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(y.x), "=f"(y.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return y;
+}
+__device__ __forceinline__ float lp_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lp_exp(float d) { return lp_exp2(d * LP_LOG2E); }  // d <= 0, -inf included
 // Bits whose order as an unsigned number is the logits' order; -0 counts as 0.
 __device__ __forceinline__ uint32_t lp_ordered(float x) {
   const uint32_t b = __float_as_uint(x + 0.0f);
@@ -111,159 +146,222 @@ __device__ __forceinline__ float lp_remote_f32(uint32_t a) {
   return v;
 }
 
+constexpr int LP_BUFFER = 160;  // keys: up to 31 that are left, and 128 that may join them
+
+// A warp's largest keys: `list` descending over the lanes, `bound` the least that may still enter, `held` keys in
+// its buffer.
+struct LpTop {
+  uint64_t list, bound;
+  int held;
+};
+// The buffer's keys into the list, 32 at a time, while there are at least `least`. (Called, not inlined: a copy of
+// it at each place made the kernel wait for instructions.)
+__device__ __noinline__ LpTop lp_flush(LpTop t, uint64_t* buffer, int least, int n_top) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+  while (t.held >= least) {
+    const int at = max(t.held - 32, 0) + lane;  // the last ones
+    const uint64_t v = at < t.held ? buffer[at] : 0;
+    t.held = max(t.held - 32, 0);
+    t.list = lp_merge(t.list, lp_sort_up(v, lane), lane);
+  }
+  __syncwarp();
+  const uint64_t last = __shfl_sync(0xffffffffu, t.list, n_top - 1);
+  t.bound = last > t.bound ? last : t.bound;
+  return t;
+}
+
 struct LpShared {
-  uint64_t buffer[LP_WARPS][64];
-  uint64_t list[LP_WARPS][32];   // each warp's, then each CTA's of the cluster
+  uint64_t buffer[LP_WARPS][LP_BUFFER];
+  alignas(16) uint32_t bound[LP_WARPS];  // each warp's m-th largest lane maximum so far
+  int held[LP_WARPS];  // keys in each buffer; in the end all of the warp's
+  alignas(16) uint64_t keys[LP_WARPS * 64 + 1];  // to be ranked
+  uint64_t list[YSKN_MAX_TOP];   // this CTA's largest
   LpState state[LP_WARPS];
-  uint64_t part_list[32];        // this CTA's, for rank 0
-  LpState part;
+  LpState part;  // this CTA's
 };
 
-// n (1..8) lists and states in shared memory into the first; all threads.
-__device__ __forceinline__ void lp_merge_all(LpShared& sh, int n, bool top, int warp, int lane) {
-  for (int step = 4; step > 0; step >>= 1) {
-    __syncthreads();
-    if (warp < step && warp + step < n) {
-      if (top) {
-        const uint64_t up = sh.list[warp + step][31 - lane];  // descending, so this is ascending
-        sh.list[warp][lane] = lp_merge(sh.list[warp][lane], up, lane);
-      }
-      if (lane == 0) sh.state[warp] = lp_join(sh.state[warp], sh.state[warp + step]);
+// The largest n_top of n different keys in shared memory (a 0 behind them), in order, into `list`, which holds zeros;
+// all threads.
+__device__ __forceinline__ void lp_rank(const uint64_t* keys, int n, uint64_t* list, int n_top, int tid) {
+  for (int i = tid; i < n; i += LP_THREADS) {
+    const uint64_t key = keys[i];
+    int above = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; j += 2) {
+      const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(keys + j);
+      above += (y.x > key) + (y.y > key);
     }
+    if (above < n_top) list[above] = key;
   }
-  __syncthreads();
+}
+// The same of n (1..8) lists of `width` (up to 32) descending keys, zeros at their ends.
+__device__ __forceinline__ void lp_rank_lists(const uint64_t* keys, int n, int width, uint64_t* list, int n_top,
+                                              int tid) {
+  if (tid >= n * width) return;
+  const uint64_t key = keys[tid];
+  if (key == 0) return;
+  int above[LP_MAX_CLUSTER] = {};
+#pragma unroll
+  for (int step = 32; step > 0; step >>= 1)
+#pragma unroll
+    for (int l = 0; l < LP_MAX_CLUSTER; ++l) {
+      const int at = above[l] + step;
+      if (l < n && at <= width && keys[l * width + at - 1] > key) above[l] = at;
+    }
+  int place = 0;
+#pragma unroll
+  for (int l = 0; l < LP_MAX_CLUSTER; ++l) place += above[l];
+  if (place < n_top) list[place] = key;
+}
+// n (1..8) states in shared memory, joined; a whole warp.
+__device__ __forceinline__ LpState lp_whole(const LpState* state, int n, int lane) {
+  LpState t = lane < n ? state[lane] : LpState{-INFINITY, 0.0f, 0.0f};
+#pragma unroll
+  for (int by = 4; by > 0; by >>= 1)
+    t = lp_join(t, LpState{__shfl_down_sync(0xffffffffu, t.m, by), __shfl_down_sync(0xffffffffu, t.rest, by),
+                           __shfl_down_sync(0xffffffffu, t.e, by)});
+  t.m = __shfl_sync(0xffffffffu, t.m, 0);
+  t.rest = __shfl_sync(0xffffffffu, t.rest, 0);
+  t.e = __shfl_sync(0xffffffffu, t.e, 0);
+  return t;
 }
 
 template <bool TOP>
-__global__ void __launch_bounds__(LP_THREADS, 3) token_logprobs_kernel(const __grid_constant__ LogprobsParams p) {
+__global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT)
+    token_logprobs_kernel(const __grid_constant__ LogprobsParams p) {
   __shared__ LpShared sh;
   pdl_begin();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / p.cluster, rank = blockIdx.x - row * p.cluster;
   const float* x = p.logits + row * p.logits_stride;
-  // The row as 16-byte groups: `skew` logits before it fill its first group up. Groups of this part.
-  const int skew = (int)(reinterpret_cast<uintptr_t>(x) >> 2 & 3), end = skew + p.vocab;
-  const float4* groups = reinterpret_cast<const float4*>(x - skew);
-  const int n_groups = (end + 3) >> 2, per = (n_groups + p.cluster - 1) / p.cluster;
+  // The row's whole 16-byte groups, of which this part has [g0, g1) and this warp [w0, w1): all warps some, where
+  // there are 8, so that the least of their bounds is one. Up to three logits before and after them (lanes 0..2 and
+  // 3..5) are a slice of their own of the first part's first warp.
+  const int head = min((int)(-(reinterpret_cast<uintptr_t>(x) >> 2) & 3), p.vocab);
+  const int n_groups = (p.vocab - head) >> 2, tail = p.vocab - head - 4 * n_groups;
+  const float4* groups = reinterpret_cast<const float4*>(x + head);
+  const int per = (n_groups + p.cluster - 1) / p.cluster;
   const int g0 = min(rank * per, n_groups), g1 = min(g0 + per, n_groups);
+  const int w0 = g0 + (int)((int64_t)(g1 - g0) * warp / LP_WARPS);
+  const int w1 = g0 + (int)((int64_t)(g1 - g0) * (warp + 1) / LP_WARPS);
+  bool edges = warp == 0 && rank == 0 && head + tail > 0;
 
   LpState s{-INFINITY, 0.0f, 0.0f};  // m: of the warp; rest and e: of the lane
   const uint64_t lowest = (uint64_t)lp_ordered(-INFINITY) << 32 | 0xffffffffu;  // only logits above -inf pass
-  uint64_t list = 0, bound = lowest;
-  int held = 0;  // keys in the warp's buffer
-  bool fresh = true;
+  LpTop top{0, lowest, 0};
+  uint32_t so_far = 0;  // the lane's largest
   uint64_t* buffer = sh.buffer[warp];
-  auto flush = [&]() {  // the buffer's first 32 into the list
-    __syncwarp();
-    const uint64_t v = lane < held ? buffer[lane] : 0, rest = lane + 32 < held ? buffer[lane + 32] : 0;
-    __syncwarp();
-    buffer[lane] = rest;
-    held = max(held - 32, 0);
-    list = lp_merge(list, lp_sort_up(v, lane), lane);
-    const uint64_t last = __shfl_sync(0xffffffffu, list, p.n_top - 1);
-    bound = last > bound ? last : bound;
-  };
-  for (int g = g0 + warp * LP_SLICE; g < g1; g += LP_WARPS * LP_SLICE) {
-    float v[LP_LOADS][4];
+  if (TOP && lane == 0) sh.held[warp] = 0;
+  const float4 nothing = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+  float4 next[LP_LOADS];  // on their way while a slice is worked on
+  auto load = [&](int g) {
 #pragma unroll
     for (int u = 0; u < LP_LOADS; ++u) {
-      const int at = g + u * 32 + lane, i = 4 * at;
-      float4 y = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-      if (at < g1) {
-        if (i >= skew && i + 4 <= end) {
-          y = __ldcs(groups + at);
-        } else {  // the row's first and last group, of which only its own logits are read
-          const float* z = x - skew + i;
-          if (i >= skew && i < end) y.x = z[0];
-          if (i + 1 >= skew && i + 1 < end) y.y = z[1];
-          if (i + 2 >= skew && i + 2 < end) y.z = z[2];
-          if (i + 3 >= skew && i + 3 < end) y.w = z[3];
-        }
-      }
-      v[u][0] = y.x, v[u][1] = y.y, v[u][2] = y.z, v[u][3] = y.w;
+      const int at = g + u * 32 + lane;
+      next[u] = at < w1 ? __ldcs(groups + at) : nothing;
     }
-    float top4[LP_LOADS], mine = -INFINITY;
+  };
+  load(w0);
+  for (int g = w0;; g += LP_SLICE) {  // once at least, since the warps meet in it
+    float2 v[LP_LOADS][2];
 #pragma unroll
     for (int u = 0; u < LP_LOADS; ++u) {
-      top4[u] = fmaxf(fmaxf(v[u][0], v[u][1]), fmaxf(v[u][2], v[u][3]));
-      mine = fmaxf(mine, top4[u]);
+      v[u][0] = make_float2(next[u].x, next[u].y);
+      v[u][1] = make_float2(next[u].z, next[u].w);
+    }
+    uint32_t first_id = head + 4 * (g + lane);
+    const bool more = g + LP_SLICE < w1;
+    load(g + LP_SLICE);  // nothing, past the end
+    if (g >= w1 && edges) {
+      const int at = lane < 3 ? lane : p.vocab - tail + lane - 3;
+      if (lane < 3 ? lane < head : lane - 3 < tail) v[0][0].x = x[at];
+      first_id = at;
+      edges = false;
+    }
+    float most4[LP_LOADS], mine = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < LP_LOADS; ++u) {
+      most4[u] = fmaxf(fmaxf(v[u][0].x, v[u][0].y), fmaxf(v[u][1].x, v[u][1].y));
+      mine = fmaxf(mine, most4[u]);
+    }
+    if constexpr (TOP) {
+      so_far = max(so_far, mine == mine ? lp_ordered(mine) : 0u);  // (a NaN is no one's bound)
+      auto raise_bound = [&](bool first_time) {
+        uint32_t o = so_far, mth = 0;
+        for (int i = 0; i < p.n_top; i += LP_WARPS) {  // the largest goes, one lane of it
+          mth = __reduce_max_sync(0xffffffffu, o);
+          if (lane == __ffs(__ballot_sync(0xffffffffu, o == mth)) - 1) o = 0;
+        }
+        if (lane == 0) *reinterpret_cast<volatile uint32_t*>(sh.bound + warp) = mth;
+        if (first_time) __syncthreads();  // later an older number of another warp serves as well
+        const uint32_t all = lane < LP_WARPS ? *reinterpret_cast<volatile uint32_t*>(sh.bound + lane) : 0xffffffffu;
+        const uint64_t least = ((uint64_t)__reduce_min_sync(0xffffffffu, all) << 32) - 1;
+        top.bound = least + 1 > top.bound ? least : top.bound;
+      };
+      if (g == w0) raise_bound(true);
+      // What passes (keys from bound + 1 on) is above `edge`, or equal to it and of a number up to edge_id.
+      float edge = lp_value((uint32_t)((top.bound + 1) >> 32));
+      if (__any_sync(0xffffffffu, mine >= edge)) {
+        uint32_t edge_id = ~(uint32_t)(top.bound + 1);
+#pragma unroll
+        for (int u = 0; u < LP_LOADS; ++u) {
+          if (!__any_sync(0xffffffffu, most4[u] >= edge)) continue;
+          if (most4[u] >= edge) {  // one or two lanes, mostly: each takes places by itself
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float y = c == 0 ? v[u][0].x : c == 1 ? v[u][0].y : c == 2 ? v[u][1].x : v[u][1].y;
+              const uint32_t id = first_id + u * 128 + c;
+              if (y > edge || (y == edge && id <= edge_id)) buffer[atomicAdd(sh.held + warp, 1)] = lp_key(y, id);
+            }
+          }
+          __syncwarp();
+          top.held = *reinterpret_cast<volatile int*>(sh.held + warp);
+          if (top.held >= 32) {
+            top = lp_flush(top, buffer, 32, p.n_top);
+            if (lane == 0) *reinterpret_cast<volatile int*>(sh.held + warp) = top.held;
+            __syncwarp();
+            edge = lp_value((uint32_t)((top.bound + 1) >> 32));
+            edge_id = ~(uint32_t)(top.bound + 1);
+          }
+        }
+        raise_bound(false);
+      }
     }
     const uint32_t most = __reduce_max_sync(0xffffffffu, lp_ordered(mine));
     const float now = fmaxf(s.m, lp_value(most));
     // Sums, relative to the largest yet; a new one is left out once, by the first lane that has it.
     if (now > s.m) {
       const unsigned who = __ballot_sync(0xffffffffu, lp_ordered(mine) == most);
-      bool skip = lane == __ffs(who) - 1;
       if (s.m != -INFINITY) {
         const float d = s.m - now, f = lp_exp(d), w = s.rest + (lane == 0 ? 1.0f : 0.0f);  // the old one counts now
         s.e = f == 0.0f ? 0.0f : f * fmaf(w, d, s.e);
         s.rest = f * w;
       }
       s.m = now;
+      bool out = lane == __ffs(who) - 1;
+      auto leave = [&](float& y) {
+        const bool it = out && y == now;
+        y = it ? -INFINITY : y;
+        out = out && !it;
+      };
 #pragma unroll
-      for (int u = 0; u < LP_LOADS; ++u)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float d = v[u][c] - now;
-          const bool out = skip && v[u][c] == now;
-          const float w = out ? 0.0f : lp_exp(d);
-          skip = skip && !out;
-          s.rest += w;
-          s.e = fmaf(w, fmaxf(d, -1e30f), s.e);
-        }
-    } else {
-      const float base = now == -INFINITY ? 0.0f : now;
-      float rest[2] = {s.rest, 0.0f}, e[2] = {s.e, 0.0f};
-#pragma unroll
-      for (int u = 0; u < LP_LOADS; ++u)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float d = v[u][c] - base, w = lp_exp(d);
-          rest[c & 1] += w;
-          e[c & 1] = fmaf(w, fmaxf(d, -1e30f), e[c & 1]);
-        }
-      s.rest = rest[0] + rest[1], s.e = e[0] + e[1];
+      for (int u = 0; u < LP_LOADS; ++u) leave(v[u][0].x), leave(v[u][0].y), leave(v[u][1].x), leave(v[u][1].y);
     }
-    if constexpr (TOP) {
-      if (fresh) {  // at least n_top of the slice's logits reach the n_top-th of the lanes' maxima
-        uint32_t o = lp_ordered(mine);
-        o = mine == mine ? o : 0;  // a NaN is no one's bound
+    const float base = now == -INFINITY ? 0.0f : -now;
+    const float2 base2 = make_float2(base, base), log2e = make_float2(LP_LOG2E, LP_LOG2E);
+    float2 rest = make_float2(s.rest, 0.0f), e = make_float2(s.e, 0.0f);
 #pragma unroll
-        for (int size = 2; size <= 32; size <<= 1)
+    for (int u = 0; u < LP_LOADS; ++u)
 #pragma unroll
-          for (int by = size >> 1; by > 0; by >>= 1) {
-            const uint32_t other = __shfl_xor_sync(0xffffffffu, o, by);
-            o = (o > other) == (((lane & by) == 0) == ((lane & size) == 0)) ? o : other;
-          }
-        // descending in lanes now
-        const uint64_t least = ((uint64_t)__shfl_sync(0xffffffffu, o, p.n_top - 1) << 32) - 1;
-        bound = least + 1 > bound ? least : bound;
-        fresh = false;
+      for (int c = 0; c < 2; ++c) {
+        const float2 d = lp_add2(v[u][c], base2), z = lp_mul2(d, log2e);
+        const float2 w = make_float2(lp_exp2(z.x), lp_exp2(z.y));
+        rest = lp_add2(rest, w);
+        e = lp_fma2(w, make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)), e);  // -inf: 0 times a number
       }
-#pragma unroll
-      for (int u = 0; u < LP_LOADS; ++u) {
-        float edge = lp_value((uint32_t)((bound + 1) >> 32));  // what passes is at least this
-        if (!__any_sync(0xffffffffu, top4[u] >= edge)) continue;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int id = 4 * (g + u * 32 + lane) + c - skew;
-          const uint64_t key = lp_key(v[u][c], id);
-          const bool pass = v[u][c] >= edge && key > bound;
-          const unsigned who = __ballot_sync(0xffffffffu, pass);
-          if (who == 0) continue;
-          if (pass) buffer[held + __popc(who & ((1u << lane) - 1))] = key;
-          held += __popc(who);
-          if (held >= 32) {
-            flush();
-            edge = lp_value((uint32_t)((bound + 1) >> 32));
-          }
-        }
-      }
-    }
-  }
-  if constexpr (TOP) {
-    if (held > 0) flush();
-    sh.list[warp][lane] = list;
+    s.rest = rest.x + rest.y, s.e = e.x + e.y;
+    if (!more && !edges) break;
   }
 #pragma unroll
   for (int by = 16; by > 0; by >>= 1) {
@@ -271,26 +369,46 @@ __global__ void __launch_bounds__(LP_THREADS, 3) token_logprobs_kernel(const __g
     s.e += __shfl_xor_sync(0xffffffffu, s.e, by);
   }
   if (lane == 0) sh.state[warp] = s;
-  lp_merge_all(sh, LP_WARPS, TOP, warp, lane);
-  if (p.cluster > 1) {
-    if (warp == 0) {
-      if (TOP) sh.part_list[lane] = sh.list[0][lane];
-      if (lane == 0) sh.part = sh.state[0];
+  // What the CTA holds, joined: the warps' buffers, and their lists where a buffer has been full.
+  const int listed = TOP ? __popc(__ballot_sync(0xffffffffu, top.list != 0)) : 0;
+  if (TOP && lane == 0) sh.held[warp] = top.held + listed;
+  __syncthreads();
+  if constexpr (TOP) {
+    int at = 0, n = 0;
+#pragma unroll
+    for (int w = 0; w < LP_WARPS; ++w) {
+      if (w == warp) at = n;
+      n += sh.held[w];
     }
+    if (lane < listed) sh.keys[at + lane] = top.list;
+    if (lane < top.held) sh.keys[at + listed + lane] = buffer[lane];
+    if (tid == 0) sh.keys[n] = 0;
+    if (tid < YSKN_MAX_TOP) sh.list[tid] = 0;
+    __syncthreads();
+    lp_rank(sh.keys, n, sh.list, p.n_top, tid);
+  }
+  LpState t = lp_whole(sh.state, LP_WARPS, lane);
+  if (p.cluster > 1) {
+    if (tid == 0) sh.part = t;
     lp_cluster_sync();
     if (rank == 0) {
       if (warp < p.cluster) {
         const uint32_t from = lp_remote(&sh.part, warp);
         if (lane == 0)
           sh.state[warp] = LpState{lp_remote_f32(from), lp_remote_f32(from + 4), lp_remote_f32(from + 8)};
-        if (TOP) sh.list[warp][lane] = lp_remote_u64(lp_remote(&sh.part_list[lane], warp));
+        if (TOP && lane < p.n_top) sh.keys[warp * p.n_top + lane] = lp_remote_u64(lp_remote(&sh.list[lane], warp));
       }
-      lp_merge_all(sh, p.cluster, TOP, warp, lane);
     }
     lp_cluster_sync();  // the others' memory has been read
     if (rank != 0) return;
+    if (TOP) {
+      if (tid < YSKN_MAX_TOP) sh.list[tid] = 0;
+      __syncthreads();
+      lp_rank_lists(sh.keys, p.cluster, p.n_top, sh.list, p.n_top, tid);
+    }
+    t = lp_whole(sh.state, p.cluster, lane);
   }
-  const LpState t = sh.state[0];
+  if (TOP) __syncthreads();
   const bool none = t.m == -INFINITY && t.rest == 0.0f, bad = !(t.m < INFINITY) || !(t.rest < INFINITY);
   const float log_sum = log1pf(t.rest), nan = __int_as_float(0x7fc00000);
   for (int j = tid; j < p.n_tokens; j += LP_THREADS) {
@@ -301,7 +419,7 @@ __global__ void __launch_bounds__(LP_THREADS, 3) token_logprobs_kernel(const __g
   }
   if (tid == 0 && p.entropy) p.entropy[row] = bad ? nan : none ? 0.0f : log_sum - t.e / (1.0f + t.rest);
   if (TOP && tid < p.n_top) {
-    const uint64_t key = sh.list[0][tid];
+    const uint64_t key = sh.list[tid];
     const int64_t at = (int64_t)row * p.n_top + tid;
     const bool any = key != 0 && !bad;
     p.top_logprobs[at] = bad ? nan : any ? (lp_value((uint32_t)(key >> 32)) - t.m) - log_sum : -INFINITY;
@@ -326,9 +444,11 @@ extern "C" YSKN_B200_API int yskn_b200_token_logprobs(const yskn_b200_token_logp
     return fail(YSKN_EINVAL, "token_logprobs: 0..32 top tokens, with both outputs");
   LogprobsParams p{a.logits, a.logits_stride, a.tokens, a.token_stride, a.logprobs, a.entropy, a.top_logprobs,
                    a.top_ids, a.vocab, a.n_tokens, a.n_top, 1};
-  // CTAs of a row: as many as keep about four on each SM, with a slice for every warp of each.
-  while (p.cluster < LP_MAX_CLUSTER && (int64_t)a.rows * p.cluster * 2 <= 4 * 148 &&
-         a.vocab / (p.cluster * 2) >= LP_WARPS * LP_SLICE * 4 / 2)
+  // CTAs of a row: as many as the SMs hold at once, with a slice for every warp of each. us at 151936 logits, 8
+  // largest, with 1, 2, 4, 8: 64 rows 31, 23, 19, 29; 128 rows 25, 22, 29, 43; 256 rows 33, 43, 56, 82; one row with 20 largest
+  // 25, 20, 14, 11; 33 rows of 50257 with 1, 2, 4, 8: 13.6, 11.4, 9.2, 11.4.
+  while (p.cluster < LP_MAX_CLUSTER && (int64_t)a.rows * p.cluster * 2 <= 148 * LP_RESIDENT &&
+         a.vocab / (p.cluster * 2) >= LP_LEAST_PART)
     p.cluster *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = (unsigned)(a.rows * p.cluster);

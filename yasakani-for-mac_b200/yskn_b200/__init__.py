@@ -900,17 +900,24 @@ def logits_adjust(logits, out, history=None, history_lens=None, prompt_lens=None
         0 if mask is None else mask.data_ptr(), ms[0], out.data_ptr(), os_[0], M, V, width, n_bias), out, stream)
 
 
-def _on(what, *tensors):
+def _here(tensors):
     """All on the current device, which the call is launched on."""
     at = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.get_device() != at:
-            at = -1
-    _need(at >= 0 and at == _DT["device"](), what + ": tensors on the current device expected")
+        if t.get_device() != at:
+            return False
+    return at >= 0 and at == _DT["device"]()
 
 
-def _dense(dtype, *tensors):
-    return all(t.dtype is dtype and t.is_contiguous() for t in tensors)
+def _dense(dtype, tensors):
+    for t in tensors:
+        if t.dtype is not dtype or not t.is_contiguous():
+            return False
+    return True
+
+
+def _addresses(tensors):
+    return [t.data_ptr() for t in tensors]
 
 
 def tree_plan(parents, requests, starts, lens, mask, positions, stream=None):
@@ -919,14 +926,15 @@ def tree_plan(parents, requests, starts, lens, mask, positions, stream=None):
     (mask int32 [T][words], a bit a new token of its request) and its position (int32 [T])."""
     if not _DT:
         _types()
-    i32, T, B = _DT["i32"], parents.numel(), lens.numel()
-    _need(_dense(i32, parents, requests, starts, lens, positions) and mask.dtype is i32 and mask.dim() == 2 and
-          mask.shape[0] == T and mask.stride(1) == 1 and requests.numel() == T and positions.numel() == T and
-          starts.numel() == B + 1, "tree_plan: int32 arrays of one batch and a mask row for each token expected")
-    _on("tree_plan", parents, requests, starts, lens, mask, positions)
-    _launch("tree_plan", ARGS["tree_plan"].pack(
-        parents.data_ptr(), requests.data_ptr(), starts.data_ptr(), lens.data_ptr(), mask.data_ptr(), mask.stride(0),
-        positions.data_ptr(), T, B, mask.shape[1]), parents, stream)
+    i32, T, B, (rows, words), row = _DT["i32"], parents.numel(), lens.numel(), mask.shape, mask.stride()
+    flat = (parents, requests, starts, lens, positions)
+    _need(_dense(i32, flat) and mask.dtype is i32 and rows == T and row[1] == 1 and requests.numel() == T and
+          positions.numel() == T and starts.numel() == B + 1,
+          "tree_plan: int32 arrays of one batch and a mask row for each token expected")
+    _need(_here(flat + (mask,)), "tree_plan: tensors on the current device expected")
+    a = _addresses(flat)
+    _launch("tree_plan", ARGS["tree_plan"].pack(a[0], a[1], a[2], a[3], mask.data_ptr(), row[0], a[4], T, B, words),
+            parents, stream)
 
 
 def tree_attention(q, k_cache, v_cache, block_tables, lens, starts, max_new, mask, work, out, prefix_blocks=None,
@@ -935,11 +943,16 @@ def tree_attention(q, k_cache, v_cache, block_tables, lens, starts, max_new, mas
     those up to itself whose bit is set in its row of mask (int32 [T][words], as tree_plan writes it)."""
     args = _attention_args("tree_attention", q, k_cache, v_cache, block_tables, lens, starts, max_new, work, out,
                            prefix_blocks, prefix_len, gate, scale)
-    _need(mask.dtype is _DT["i32"] and mask.dim() == 2 and mask.shape[0] == q.shape[0] and mask.stride(1) == 1,
+    (rows, words), row = mask.shape, mask.stride()
+    _need(mask.dtype is _DT["i32"] and rows == q.shape[0] and row[1] == 1,
           "tree_attention: an int32 mask row for each token expected")
-    _on("tree_attention", q, k_cache, v_cache, block_tables, lens, starts, mask, work, out, prefix_blocks, gate)
-    _launch("tree_attention", ARGS["tree_attention"].pack(*args, mask.data_ptr(), mask.stride(0), mask.shape[1]), out,
-            stream)
+    used = [q, k_cache, v_cache, block_tables, lens, starts, mask, work, out]
+    if prefix_len:
+        used.append(prefix_blocks)
+    if gate is not None:
+        used.append(gate)
+    _need(_here(used), "tree_attention: tensors on the current device expected")
+    _launch("tree_attention", ARGS["tree_attention"].pack(*args, mask.data_ptr(), row[0], words), out, stream)
 
 
 def tree_accept(tokens, parents, choice, starts, lens, path, accepted, lens_out, next_token, stream=None):
@@ -948,16 +961,15 @@ def tree_accept(tokens, parents, choice, starts, lens, path, accepted, lens_out,
     the lengths without the others' rows, and the choice after its last node (int32 [batch] each)."""
     if not _DT:
         _types()
-    i32, T, B = _DT["i32"], tokens.numel(), lens.numel()
-    _need(_dense(i32, tokens, parents, choice, starts, lens, accepted, lens_out, next_token) and path.dtype is i32 and
-          path.dim() == 2 and path.shape[0] == B and path.stride(1) == 1 and parents.numel() == T and
+    i32, T, B, (rows, width), row = _DT["i32"], tokens.numel(), lens.numel(), path.shape, path.stride()
+    flat = (tokens, parents, choice, starts, lens, accepted, lens_out, next_token)
+    _need(_dense(i32, flat) and path.dtype is i32 and rows == B and row[1] == 1 and parents.numel() == T and
           choice.numel() == T and starts.numel() == B + 1 and accepted.numel() == B and lens_out.numel() == B and
           next_token.numel() == B, "tree_accept: int32 arrays of one batch and a path row for each request expected")
-    _on("tree_accept", tokens, parents, choice, starts, lens, path, accepted, lens_out, next_token)
-    _launch("tree_accept", ARGS["tree_accept"].pack(
-        tokens.data_ptr(), parents.data_ptr(), choice.data_ptr(), starts.data_ptr(), lens.data_ptr(), path.data_ptr(),
-        path.stride(0), accepted.data_ptr(), lens_out.data_ptr(), next_token.data_ptr(), B, T, path.shape[1]), tokens,
-        stream)
+    _need(_here(flat + (path,)), "tree_accept: tensors on the current device expected")
+    a = _addresses(flat)
+    _launch("tree_accept", ARGS["tree_accept"].pack(a[0], a[1], a[2], a[3], a[4], path.data_ptr(), row[0], a[5], a[6],
+                                                    a[7], B, T, width), tokens, stream)
 
 
 def batch_edit(lens, keep, block_tables, pool, free_count, block_size, lens_out, free_out, source=None, tables_out=None,
@@ -968,26 +980,27 @@ def batch_edit(lens, keep, block_tables, pool, free_count, block_size, lens_out,
     block to write, rows) and their number to n_copies (int32 [1])."""
     if not _DT:
         _types()
-    i32 = _DT["i32"]
-    B, width = block_tables.shape
-    _need(_dense(i32, lens, keep, pool, free_count, lens_out, free_out) and block_tables.dtype is i32 and
-          block_tables.stride(1) == 1 and lens.numel() == B and keep.numel() == B and lens_out.numel() == B and
-          free_count.numel() and free_out.numel(), "batch_edit: dense int32 arrays of the batch expected")
-    ts, cs, n, tail = (0, 1), (0, 1), 0, (0, 0, 0, 0)
+    i32, (B, width), row = _DT["i32"], block_tables.shape, block_tables.stride()
+    flat = (lens, keep, pool, free_count, lens_out, free_out)
+    _need(_dense(i32, flat) and block_tables.dtype is i32 and row[1] == 1 and lens.numel() == B and
+          keep.numel() == B and lens_out.numel() == B and free_count.numel() and free_out.numel(),
+          "batch_edit: dense int32 arrays of the batch expected")
+    _need(_here(flat + (block_tables,)), "batch_edit: tensors on the current device expected")
+    ts = cs = (0, 1)
+    n, f = 0, (0, 0, 0, 0)
     if source is not None:
+        fork = (source, n_copies, tables_out, copies)
         _need(tables_out is not None and copies is not None and n_copies is not None,
               "batch_edit: a source needs new tables, a list of copies and its count")
-        ts, cs, n = tables_out.stride(), copies.stride(), copies.shape[-1]
-        _need(_dense(i32, source, n_copies) and source.numel() == B and n_copies.numel() and tables_out.dtype is i32 and
-              tables_out.shape == (B, width) and ts[1] == 1 and copies.dtype is i32 and copies.dim() == 2 and
-              copies.shape[0] == 3 and cs[1] == 1,
+        ts, cs, (three, n) = tables_out.stride(), copies.stride(), copies.shape
+        _need(_dense(i32, fork[:2]) and source.numel() == B and n_copies.numel() and tables_out.dtype is i32 and
+              tables_out.shape == (B, width) and ts[1] == 1 and copies.dtype is i32 and three == 3 and cs[1] == 1,
               "batch_edit: int32 source, tables of one shape and copies [3][n] expected")
-        tail = (source.data_ptr(), tables_out.data_ptr(), copies.data_ptr(), n_copies.data_ptr())
-        _on("batch_edit", source, tables_out, copies, n_copies)
-    _on("batch_edit", lens, keep, block_tables, pool, free_count, lens_out, free_out)
+        _need(_here(fork), "batch_edit: tensors on the current device expected")
+        f = _addresses(fork)
+    a = _addresses(flat)
     _launch("batch_edit", ARGS["batch_edit"].pack(
-        lens.data_ptr(), keep.data_ptr(), tail[0], block_tables.data_ptr(), block_tables.stride(0), tail[1], ts[0],
-        pool.data_ptr(), free_count.data_ptr(), lens_out.data_ptr(), free_out.data_ptr(), tail[2], cs[0], tail[3], B,
+        a[0], a[1], f[0], block_tables.data_ptr(), row[0], f[2], ts[0], a[2], a[3], a[4], a[5], f[3], cs[0], f[1], B,
         block_size, prefix_len, width, pool.numel(), n), lens, stream)
 
 
@@ -1003,10 +1016,10 @@ class CacheSet:
                   c.stride() == first.stride() and c.device == first.device for c in caches) and first.stride(3) == 1,
               "CacheSet: 16-bit caches of one type, shape, strides and device with dense channels expected")
         self.caches = caches
-        self._addresses = (C.c_void_p * len(caches))(*[c.data_ptr() for c in caches])
+        self._pointers = (C.c_void_p * len(caches))(*[c.data_ptr() for c in caches])
         n_blocks, block_size, n_kvh, head = first.shape
         s = first.stride()
-        self._head = (C.addressof(self._addresses), s[0], s[1], s[2])
+        self._head = (C.addressof(self._pointers), s[0], s[1], s[2])
         self._sizes = (len(caches), n_blocks, block_size, n_kvh, head)
 
 
@@ -1015,14 +1028,15 @@ def cache_copy(caches, copies, count=None, stream=None):
     block to read, block to write, rows), the first *count (int32 [1]) of them or all."""
     if not _DT:
         _types()
-    i32 = _DT["i32"]
-    _need(copies.dtype is i32 and copies.dim() == 2 and copies.shape[0] == 3 and copies.stride(1) == 1 and
+    i32, (three, n), row = _DT["i32"], copies.shape, copies.stride()
+    _need(copies.dtype is i32 and three == 3 and row[1] == 1 and
           (count is None or (count.dtype is i32 and count.numel())),
           "cache_copy: int32 copies [3][n] and a count expected")
-    _on("cache_copy", caches.caches[0], copies, count)
+    _need(_here((copies, caches.caches[0]) if count is None else (copies, caches.caches[0], count)),
+          "cache_copy: tensors on the current device expected")
     _launch("cache_copy", ARGS["cache_copy"].pack(
-        *caches._head, copies.data_ptr(), copies.stride(0), 0 if count is None else count.data_ptr(), *caches._sizes,
-        copies.shape[1]), copies, stream)
+        *caches._head, copies.data_ptr(), row[0], 0 if count is None else count.data_ptr(), *caches._sizes, n), copies,
+        stream)
 
 
 def cache_compact(caches, block_tables, lens, starts, path, prefix_len=0, stream=None):
@@ -1030,16 +1044,16 @@ def cache_compact(caches, block_tables, lens, starts, path, prefix_len=0, stream
     many as its starts say) those on its path (int32 [batch][width], as tree_accept writes it) made adjacent."""
     if not _DT:
         _types()
-    i32 = _DT["i32"]
-    B, width = block_tables.shape
-    _need(block_tables.dtype is i32 and block_tables.stride(1) == 1 and _dense(i32, lens, starts) and
-          lens.numel() == B and starts.numel() == B + 1 and path.dtype is i32 and path.dim() == 2 and
-          path.shape[0] == B and path.stride(1) == 1,
+    i32, (B, width), (rows, nodes) = _DT["i32"], block_tables.shape, path.shape
+    ts, ps = block_tables.stride(), path.stride()
+    _need(block_tables.dtype is i32 and ts[1] == 1 and _dense(i32, (lens, starts)) and lens.numel() == B and
+          starts.numel() == B + 1 and path.dtype is i32 and rows == B and ps[1] == 1,
           "cache_compact: int32 tables, lengths, starts and paths of one batch expected")
-    _on("cache_compact", caches.caches[0], block_tables, lens, starts, path)
+    _need(_here((lens, starts, block_tables, path, caches.caches[0])),
+          "cache_compact: tensors on the current device expected")
     _launch("cache_compact", ARGS["cache_compact"].pack(
-        *caches._head, block_tables.data_ptr(), block_tables.stride(0), lens.data_ptr(), starts.data_ptr(),
-        path.data_ptr(), path.stride(0), *caches._sizes, B, width, prefix_len, path.shape[1]), lens, stream)
+        *caches._head, block_tables.data_ptr(), ts[0], lens.data_ptr(), starts.data_ptr(), path.data_ptr(), ps[0],
+        *caches._sizes, B, width, prefix_len, nodes), lens, stream)
 
 
 def token_logprobs(logits, tokens=None, logprobs=None, entropy=None, top_logprobs=None, top_ids=None, stream=None):
@@ -1048,26 +1062,34 @@ def token_logprobs(logits, tokens=None, logprobs=None, entropy=None, top_logprob
     (f32 [M][k]) and top_ids (int32 [M][k]), k up to 32."""
     if not _DT:
         _types()
-    i32, f32 = _DT["i32"], logits.dtype
-    (M, V), s = logits.shape, logits.stride()
+    i32, f32, (M, V), row = _DT["i32"], logits.dtype, logits.shape, logits.stride()
     n = k = stride = 0
-    _need(_DT.get(f32) == DT_F32 and s[1] == 1, "token_logprobs: f32 logits with dense rows expected")
+    used = [logits]
+    a = b = e = c = d = 0
+    _need(_DT.get(f32) == DT_F32 and row[1] == 1, "token_logprobs: f32 logits with dense rows expected")
     _need((tokens is None) == (logprobs is None) and (top_ids is None) == (top_logprobs is None),
           "token_logprobs: tokens and their output, and both outputs of the most likely ones, go together")
     if tokens is not None:
-        n, stride = tokens.shape[-1], tokens.stride(0)
-        _need(tokens.dtype is i32 and tokens.shape == (M, n) and (tokens.stride(1) == 1 or n < 2) and
-              logprobs.shape == (M, n) and _dense(f32, logprobs),
+        shape = tokens.shape
+        (rows, n), (stride, step) = shape, tokens.stride()
+        _need(tokens.dtype is i32 and rows == M and (step == 1 or n < 2) and logprobs.shape == shape and
+              logprobs.dtype is f32 and logprobs.is_contiguous(),
               "token_logprobs: int32 tokens [M][n] and dense f32 log probabilities of their shape expected")
+        used += (tokens, logprobs)
+        a, b = tokens.data_ptr(), logprobs.data_ptr()
+    if entropy is not None:
+        _need(entropy.dtype is f32 and entropy.shape == (M,) and entropy.is_contiguous(),
+              "token_logprobs: f32 entropy [M] expected")
+        used.append(entropy)
+        e = entropy.data_ptr()
     if top_ids is not None:
-        k = top_ids.shape[-1]
-        _need(top_ids.shape == (M, k) and top_logprobs.shape == (M, k) and _dense(i32, top_ids) and
-              _dense(f32, top_logprobs),
+        shape = top_ids.shape
+        rows, k = shape
+        _need(rows == M and top_logprobs.shape == shape and top_ids.dtype is i32 and top_ids.is_contiguous() and
+              top_logprobs.dtype is f32 and top_logprobs.is_contiguous(),
               "token_logprobs: dense int32 numbers and f32 log probabilities [M][k] expected")
-    _need(entropy is None or (entropy.shape == (M,) and _dense(f32, entropy)),
-          "token_logprobs: f32 entropy [M] expected")
-    _on("token_logprobs", logits, tokens, logprobs, entropy, top_logprobs, top_ids)
-    _launch("token_logprobs", ARGS["token_logprobs"].pack(
-        logits.data_ptr(), s[0], tokens.data_ptr() if n else 0, stride, logprobs.data_ptr() if n else 0,
-        0 if entropy is None else entropy.data_ptr(), top_logprobs.data_ptr() if k else 0,
-        top_ids.data_ptr() if k else 0, M, V, n, k), logits, stream)
+        used += (top_logprobs, top_ids)
+        c, d = top_logprobs.data_ptr(), top_ids.data_ptr()
+    _need(_here(used), "token_logprobs: tensors on the current device expected")
+    _launch("token_logprobs", ARGS["token_logprobs"].pack(logits.data_ptr(), row[0], a, stride, b, e, c, d, M, V, n, k),
+            logits, stream)
