@@ -14,8 +14,15 @@ then read by every request and never written again. Weights are the stack's seed
 step reads or writes stays on the device and keeps its address, so a decode step (one token
 for each request) can be captured as a CUDA graph.
 
+Where a draft (a small model, n-grams) proposes a tree of tokens for each request, verify runs all of
+its nodes in one step in place of step: tree_plan and tree_attention let a node see its own ancestors
+only, tree_accept finds the path that is the model's own, cache_compact makes that path's rows
+adjacent in every layer and batch_edit gives the other rows' blocks back. fork lets requests
+continue others (beams, several answers to one prompt): batch_edit and cache_copy. With logprobs
+the log probability of each chosen token, its row's entropy and the likeliest tokens are kept.
+
 python -m yskn_b200.batch runs 64 requests behind a prefix on four layers and prints the
-time of a decode step.
+time of a decode step and of a step that verifies eight nodes a request.
 """
 import numpy as np
 
@@ -28,10 +35,12 @@ THETA = 1e7
 
 class BatchStack(S.Stack):
     """batch requests of up to `capacity` own tokens each, steps of up to max_tokens tokens,
-    n_blocks blocks of block_size cache rows shared by the prefix and the requests."""
+    n_blocks blocks of block_size cache rows shared by the prefix and the requests. nodes: of a request's drafted
+    tree, at most, its next token among them (0: verify is not used). logprobs: None, or how many of the likeliest
+    tokens to keep beside the chosen ones' log probabilities."""
 
     def __init__(self, device, layers=4, vocab=S.VOCAB, batch=64, max_tokens=512, capacity=512, n_blocks=1024,
-                 block_size=64, bits=8, seed=1):
+                 block_size=64, bits=8, seed=1, nodes=0, logprobs=None):
         super().__init__(device, vocab=vocab, ctx=0, bits=bits, seed=seed, kinds=["attn"] * layers)
         torch = self.torch
         self.batch, self.max_tokens, self.capacity, self.block_size = batch, max_tokens, capacity, block_size
@@ -71,6 +80,26 @@ class BatchStack(S.Stack):
         n = max(Y.prefix_attention_work_bytes(T, batch, T, S.N_QH, S.N_KVH, S.HEAD),
                 Y.prefix_attention_work_bytes(T, 1, T, S.N_QH, S.N_KVH, S.HEAD))
         self.attn_work = torch.empty(n, dtype=torch.uint8, device=device)
+        # all layers' caches; copies of requests
+        self.caches = Y.CacheSet([c for L in self.L for c in L["pages"]])
+        self.tables_out, self.copies, self.n_copies = i32(batch, self.tables.shape[1]), i32(3, n_blocks), i32(1)
+        self.whole = i32(batch).fill_(2 ** 31 - 1)
+        # chosen tokens' log probabilities, by request
+        self.logprobs = logprobs
+        rows = lambda n: (f32(n, 1), f32(n), f32(n, logprobs or 0), i32(n, logprobs or 0))  # noqa: E731
+        if logprobs is not None:
+            self.logprob, self.entropy, self.top_logprobs, self.top_ids = rows(batch)
+        # drafted trees: node j of request i is draft[i][j] behind node draft_parents[i][j]; node 0 its next token
+        self.nodes = nodes
+        if nodes:
+            self.draft_tokens, self.draft_parents = i32(batch, nodes), i32(batch, nodes).fill_(-1)
+            self.parents, self.tree, self.tree_pos = i32(T), i32(T, -(-nodes // 32)), i32(T)
+            self.path, self.accepted, self.keep, self.next = i32(batch, nodes), i32(batch), i32(batch), i32(batch)
+            self.tlogits, self.choice = f32(T, vocab), i32(T)
+            self.bwork = torch.empty(max(self.bwork.numel(), Y.linear_work_bytes([self.head], T)), dtype=torch.uint8,
+                                     device=device)
+            if logprobs is not None:  # by node
+                self.node_logprob, self.node_entropy, self.node_top_logprobs, self.node_top_ids = rows(T)
 
     def fill_prefix(self, tokens, stream=None):
         """Runs `tokens` (int32, on the device) once as what every request's text follows. Before any
@@ -126,6 +155,8 @@ class BatchStack(S.Stack):
                         prompt_lens=self.prompt, repetition=self.repetition, presence=self.presence,
                         frequency=self.frequency, mask=self.mask)
         Y.head_select(self.blogits, token=self.btoken)
+        if self.logprobs is not None:
+            self._score(self.blogits, self.btoken, self.logprob, self.entropy, self.top_logprobs, self.top_ids)
         own = self.lens_out - self.prefix_len * (self.lens_out > 0)
         spoke = (self.starts[1:] > self.starts[:-1]) & (own == self.said) & (self.said < W)
         place = self.said.clamp(max=W - 1).long().unsqueeze(1)
@@ -134,8 +165,83 @@ class BatchStack(S.Stack):
         self.lens.copy_(self.lens_out)
         self.free.copy_(self.free_out)
 
-    def _layers(self, T, max_new, tables, lens, starts, prefix_blocks, prefix_len):
-        """The first T of self.tokens through every layer, into self.bx and self.binv."""
+    def _score(self, logits, token, logprob, entropy, top_logprobs, top_ids):
+        """The tokens' log probabilities (after penalties, biases and masks) and their rows' likeliest tokens."""
+        most = dict(top_logprobs=top_logprobs, top_ids=top_ids) if self.logprobs else {}
+        Y.token_logprobs(logits, token.unsqueeze(1), logprob, entropy, **most)
+
+    def draft(self, request, tokens, parents):
+        """The request's drafted tree: node j + 1 is tokens[j] behind node parents[j] <= j (node 0 is the request's
+        next token, said but not run yet). The next verify that gives it 1 + len(tokens) new tokens runs it."""
+        n = len(tokens)
+        if n >= self.nodes or len(parents) != n or any(not 0 <= p <= j for j, p in enumerate(parents)):
+            raise Y.YsknError(Y.EINVAL, "draft: %d nodes at most, each behind an earlier one" % max(self.nodes - 1, 0))
+        dev, t = self.dev, self.torch
+        self.draft_tokens[request, 1:n + 1] = t.tensor(tokens, dtype=t.int32, device=dev)
+        self.draft_parents[request, 1:n + 1] = t.tensor(parents, dtype=t.int32, device=dev)
+
+    def verify(self, n_tokens, stream=None):
+        """Runs the trees of the requests that have drafted some: self.new[i] nodes of request i (0: none; 1: its next
+        token alone), n_tokens in all at most. The tokens of each accepted path and the model's choice behind it are
+        appended; the cache keeps the path's rows. Choices are the largest logits, without penalties and masks (which
+        what a node's ancestors say would change), of requests that have run all they said but the last token."""
+        torch, T, W = self.torch, n_tokens, self.capacity
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self.verify(n_tokens)
+        Y.batch_plan(self.lens, self.new, self.tables, self.pool, self.free, self.block_size, self.lens_out,
+                     self.free_out, self.starts, self.slots[:T], self.pos[:T], self.requests[:T], self.prefix_len)
+        request = self.requests[:T].clamp(min=0).long()
+        node = (torch.arange(T, device=self.dev) - self.starts[request]).clamp(0, self.nodes - 1)
+        said = self.text.gather(1, (self.said - 1).clamp(min=0).long().unsqueeze(1))[:, 0]
+        self.tokens[:T].copy_(torch.where(node > 0, self.draft_tokens[request, node], said[request]))
+        self.parents[:T].copy_(self.draft_parents[request, node])
+        Y.tree_plan(self.parents[:T], self.requests[:T], self.starts, self.lens_out, self.tree[:T], self.tree_pos[:T])
+        self._layers(T, self.nodes, self.tables, self.lens_out, self.starts, self.prefix_blocks, self.prefix_len,
+                     self.tree_pos[:T], self.tree[:T])
+        logits, choice = self.tlogits[:T], self.choice[:T]
+        Y.linear([self.head], self.bx[:T], self.bwork, [logits], inv_rms=self.binv[:T])
+        Y.head_select(logits, token=choice)
+        if self.logprobs is not None:
+            self._score(logits, choice, self.node_logprob[:T], self.node_entropy[:T], self.node_top_logprobs[:T],
+                        self.node_top_ids[:T])
+        Y.tree_accept(self.tokens[:T], self.parents[:T], choice, self.starts, self.lens_out, self.path, self.accepted,
+                      self.keep, self.next)
+        Y.cache_compact(self.caches, self.tables, self.lens_out, self.starts, self.path, self.prefix_len)
+        Y.batch_edit(self.lens_out, self.keep, self.tables, self.pool, self.free_out, self.block_size, self.lens,
+                     self.free, prefix_len=self.prefix_len)
+        # the path's tokens behind node 0, then the choice after its last node
+        at = self.starts[:-1, None].long() + self.path[:, 1:].clamp(min=0)
+        took = torch.cat([self.tokens[at.clamp(max=T - 1)], self.next.unsqueeze(1)], 1)
+        count = self.accepted.long().unsqueeze(1)
+        col = torch.arange(W, device=self.dev).unsqueeze(0) - self.said.unsqueeze(1)
+        new = torch.where(col == count - 1, self.next.unsqueeze(1), took.gather(1, col.clamp(0, self.nodes - 1)))
+        self.text.copy_(torch.where((col >= 0) & (col < count), new, self.text))
+        self.said.copy_((self.said + self.accepted).clamp(max=W))
+
+    def fork(self, source, stream=None):
+        """Request i becomes a copy of request source[i] (int32 on the device; itself: it goes on; negative: it ends):
+        cache, text and controls. Of those that continue one request the first goes on in its blocks, the others get
+        copies; one whose copy the pool does not hold keeps the text and has to run it again (its lens is 0)."""
+        torch = self.torch
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self.fork(source)
+        Y.batch_edit(self.lens, self.whole, self.tables, self.pool, self.free, self.block_size, self.lens_out,
+                     self.free_out, source=source, tables_out=self.tables_out, copies=self.copies,
+                     n_copies=self.n_copies, prefix_len=self.prefix_len)
+        Y.cache_copy(self.caches, self.copies, self.n_copies)
+        self.tables.copy_(self.tables_out)
+        self.lens.copy_(self.lens_out)
+        self.free.copy_(self.free_out)
+        of, live = source.clamp(min=0).long(), (source >= 0)
+        for t in (self.text, self.prompt, self.repetition, self.presence, self.frequency, self.mask):
+            t.copy_(t[of])
+        self.said.copy_(self.said[of] * live)
+
+    def _layers(self, T, max_new, tables, lens, starts, prefix_blocks, prefix_len, positions=None, tree=None):
+        """The first T of self.tokens through every layer, into self.bx and self.binv; where they are trees' nodes,
+        with their positions and masks."""
         h, x, inv, proj = self.bh[:T], self.bx[:T], self.binv[:T], self.bproj[:T]
         q, k, v, query, out = self.bq[:T], self.bk[:T], self.bv[:T], self.bquery[:T], self.bout[:T]
         gate, up, m, a_in = self.bg[:T], self.bu[:T], self.bm[:T], self.ba_in[:T]
@@ -144,10 +250,13 @@ class BatchStack(S.Stack):
         for L in self.L:
             Y.residual_prepare(h, before, L["in_norm"], S.EPS, x, inv)
             Y.linear([L["q"], L["k"], L["v"]], x, self.bwork, [q, k, v], inv_rms=inv)
-            Y.paged_prep(q[:, :, :S.HEAD], k, v, self.slots[:T], self.pos[:T], query, *L["pages"],
-                         inv_freq=self.inv_freq, q_norm=L["q_norm"], k_norm=L["k_norm"], eps=S.EPS)
-            Y.prefix_attention(query, *L["pages"], tables, lens, starts, max_new, self.attn_work, out,
-                               prefix_blocks=prefix_blocks, prefix_len=prefix_len, gate=q[:, :, S.HEAD:])
+            Y.paged_prep(q[:, :, :S.HEAD], k, v, self.slots[:T], self.pos[:T] if positions is None else positions,
+                         query, *L["pages"], inv_freq=self.inv_freq, q_norm=L["q_norm"], k_norm=L["k_norm"], eps=S.EPS)
+            rest = dict(prefix_blocks=prefix_blocks, prefix_len=prefix_len, gate=q[:, :, S.HEAD:])
+            if tree is None:
+                Y.prefix_attention(query, *L["pages"], tables, lens, starts, max_new, self.attn_work, out, **rest)
+            else:
+                Y.tree_attention(query, *L["pages"], tables, lens, starts, max_new, tree, self.attn_work, out, **rest)
             Y.widen_bf16(out, a_in)
             Y.linear([L["o"]], a_in, self.bwork, [proj])
             Y.residual_prepare(h, proj, L["post_norm"], S.EPS, x, inv)
@@ -162,7 +271,7 @@ def main():
     import torch
     dev = torch.device("cuda:0")
     batch, prefix = 64, 2000
-    st = BatchStack(dev, batch=batch)
+    st = BatchStack(dev, batch=batch, nodes=8)
     gen = torch.Generator(device=dev)
     gen.manual_seed(3)
     stream = torch.cuda.Stream(dev)
@@ -191,6 +300,18 @@ def main():
     ms = t0.elapsed_time(t1) / steps
     print("%d requests behind %d shared tokens, %d attention layers: %.3f ms a step, %.0f tokens/s"
           % (batch, prefix, st.layers, ms, batch * 1e3 / ms))
+    # random drafts: what a step that verifies them takes, not what it saves
+    for i in range(batch):
+        st.draft(i, [(53 * i + 7 * j) % st.vocab for j in range(7)], [0, 0, 1, 1, 2, 3, 4])
+    st.new.fill_(8)
+    with torch.cuda.stream(stream):
+        st.verify(8 * batch, stream)
+        t0.record()
+        st.verify(8 * batch, stream)
+        t1.record()
+        torch.cuda.synchronize()
+    Y.check(Y.status(stream), "verify")
+    print("trees of 8 nodes: %.3f ms a step" % t0.elapsed_time(t1))
     print("request 0:", st.text[0, :int(st.said[0])].tolist()[:16], "...")
 
 
