@@ -90,7 +90,7 @@ def test_cache_moves():
               dict(block_size=0), dict(n_kvh=0), dict(head=96), dict(head=8), dict(block=4), dict(token=4),
               dict(head_stride=4)]
     refused("cache_copy", COPY, shapes + [dict(copies=None), dict(max_copies=0), dict(copies_stride=8),
-                                          dict(block_size=2 ** 20 + 1)])
+                                          dict(block_size=2 ** 31 - 1, n_kvh=2 ** 20)])
     refused("cache_compact", COMPACT,
             shapes + [{k: None} for k in ("tables", "lens", "starts", "path")] +
             [dict(batch=0), dict(width=0), dict(prefix=-1), dict(path_width=0), dict(stride=3), dict(path_stride=4)])

@@ -1,22 +1,28 @@
 // Rows moved inside the layers' paged 16-bit caches: whole blocks copied for requests that continue
 // others, and the rows of accepted paths made adjacent. All layers' K and V caches in one launch.
 //
-// What bounds both: bytes, each read once and written once. cache_copy: a unit is one head of one block of
-// one cache (rows x D, 32 KB at 64 rows of 256 channels); a CTA takes units in turn, 8 16-byte loads a
-// thread under way before the first store. cache_compact: a warp takes one head of one request's path
-// in one cache. Row base + path[k] goes to base + k, and path[k] >= k, in ascending order: a row that is
-// written (k) was a source only for smaller k (path[k'] = k means k' <= k), so that a warp that loads
-// a run of rows before it stores them, run after run, never reads a row that it has overwritten.
+// What bounds both: bytes, each read once and written once; for short paths, latency.
+// cache_copy: a warp copies a piece, 4 KB of one head of one block of one cache (8 rows of 256 channels, 8 16-byte
+// loads a lane before the first store). Many more CTAs than the SMs hold, each a few pieces, so that the SMs keep
+// busy whatever rows the blocks hold: 256 copies of 1 to 64 rows in 16 caches 88 us (6.4 TB/s; whole blocks 6.7), as
+// many CTAs as are resident 96, and one CTA a head of a block with the next one's loads ahead of its stores 104 to 117.
+// cache_compact: a warp takes one head of one request's path in four caches: the path and the blocks are looked up
+// once, and three rows in each cache are under way at once (64 paths of 6 nodes in 32 caches 7.4 us; one cache and
+// four rows a warp 12.0). Row base + path[k] goes to base + k, and path[k] >= k, in ascending order: a row that is
+// written (k) was a source only for smaller k (path[k'] = k means k' <= k), so that a warp that loads a run of rows
+// before it stores them, run after run, never reads a row that it has overwritten.
 #include <algorithm>
 
 #include "paged.cuh"
 
 namespace yskn {
 
-constexpr int MOVE_THREADS = 256;
+constexpr int MOVE_THREADS = 128;
 constexpr int MOVE_WARPS = MOVE_THREADS / 32;
-constexpr int MOVE_LOADS = 8;   // 16-byte loads of a thread under way
-constexpr int MOVE_RUN = 4;     // the same in cache_compact
+constexpr int COPY_LOADS = 8;   // 16-byte loads of a lane under way
+constexpr int COPY_CTAS = 80;   // of an SM's share of a long list, most of them waiting
+constexpr int MOVE_RUN = 3;     // rows of a path that a lane moves at once
+constexpr int MOVE_CACHES = 4;  // in so many caches
 
 struct MoveCaches {
   uint16_t* base[YSKN_MAX_CACHES];
@@ -37,38 +43,33 @@ struct CopyParams {
 __global__ void __launch_bounds__(MOVE_THREADS) cache_copy_kernel(const __grid_constant__ CopyParams p) {
   pdl_begin();
   const MoveCaches& c = p.c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = p.count ? min(max(__ldg(p.count), 0), p.max_copies) : p.max_copies;
-  const int per = c.n_caches * c.n_kvh;  // units of an entry
-  for (int64_t u = blockIdx.x; u < (int64_t)n * per; u += gridDim.x) {
-    const int e = (int)(u / per), rest = (int)(u - (int64_t)e * per);
+  const int at_once = 32 >> c.unit_shift, sub = lane >> c.unit_shift, unit = lane & (c.units - 1);
+  const int step = at_once * COPY_LOADS, steps = (c.block_size + step - 1) / step;  // rows of a piece; pieces of a head
+  const int per = c.n_caches * c.n_kvh * steps;                                     // and of an entry
+  const int64_t pieces = (int64_t)n * per;
+  for (int64_t u = (int64_t)blockIdx.x * MOVE_WARPS + warp; u < pieces; u += (int64_t)gridDim.x * MOVE_WARPS) {
+    const int e = (int)(u / per), rest = (int)(u - (int64_t)e * per), head = rest / steps;
+    const int first = (rest - head * steps) * step, cache = head / c.n_kvh, h = head - cache * c.n_kvh;
     const int from = __ldg(p.copies + e), to = __ldg(p.copies + e + p.copies_stride);
     const int rows = __ldg(p.copies + e + 2 * p.copies_stride);
-    if (rows <= 0) continue;
+    if (rows <= first) continue;
     if (from < 0 || from >= c.n_blocks || to < 0 || to >= c.n_blocks || rows > c.block_size) {
-      if (threadIdx.x == 0) raise_device_error(p.err, DERR_RANGE);
+      if (lane == 0) raise_device_error(p.err, DERR_RANGE);
       continue;
     }
-    const int cache = rest / c.n_kvh, h = rest - cache * c.n_kvh;
-    uint16_t* base = c.base[cache] + h * c.stride.head;
+    uint16_t* base = c.base[cache] + h * c.stride.head + (first + sub) * c.stride.token + unit * 8;
     const uint16_t* src = base + from * c.stride.block;
     uint16_t* dst = base + to * c.stride.block;
-    const int all = rows << c.unit_shift;
-    for (int i0 = threadIdx.x; i0 < all; i0 += MOVE_THREADS * MOVE_LOADS) {
-      uint4 v[MOVE_LOADS];
+    const int64_t by = at_once * c.stride.token;
+    uint4 v[COPY_LOADS];
 #pragma unroll
-      for (int x = 0; x < MOVE_LOADS; ++x) {
-        const int i = i0 + x * MOVE_THREADS;
-        if (i < all)
-          v[x] = __ldcs(reinterpret_cast<const uint4*>(src + (i >> c.unit_shift) * c.stride.token) +
-                        (i & (c.units - 1)));
-      }
+    for (int x = 0; x < COPY_LOADS; ++x)
+      if (first + x * at_once + sub < rows) v[x] = __ldcs(reinterpret_cast<const uint4*>(src + x * by));
 #pragma unroll
-      for (int x = 0; x < MOVE_LOADS; ++x) {
-        const int i = i0 + x * MOVE_THREADS;
-        if (i < all)
-          __stcs(reinterpret_cast<uint4*>(dst + (i >> c.unit_shift) * c.stride.token) + (i & (c.units - 1)), v[x]);
-      }
-    }
+    for (int x = 0; x < COPY_LOADS; ++x)
+      if (first + x * at_once + sub < rows) __stcs(reinterpret_cast<uint4*>(dst + x * by), v[x]);
   }
 }
 
@@ -82,27 +83,28 @@ struct CompactParams {
   unsigned* err;
 };
 
-__global__ void __launch_bounds__(MOVE_THREADS) cache_compact_kernel(const __grid_constant__ CompactParams p) {
+__global__ void __launch_bounds__(MOVE_THREADS, 3) cache_compact_kernel(const __grid_constant__ CompactParams p) {
   pdl_begin();
   const MoveCaches& c = p.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per = c.n_caches * c.n_kvh;  // units of a request
+  const int groups = (c.n_caches + MOVE_CACHES - 1) / MOVE_CACHES, per = groups * c.n_kvh;  // units of a request
   const int at_once = 32 >> c.unit_shift, sub = lane >> c.unit_shift, unit = lane & (c.units - 1);
   const int64_t units = (int64_t)p.batch * per;
   for (int64_t u = (int64_t)blockIdx.x * MOVE_WARPS + warp; u < units; u += (int64_t)gridDim.x * MOVE_WARPS) {
     const int r = (int)(u / per), rest = (int)(u - (int64_t)r * per);
-    const int cache = rest / c.n_kvh, h = rest - cache * c.n_kvh;
+    const int group = rest / c.n_kvh, h = rest - group * c.n_kvh;
+    const int cache0 = group * MOVE_CACHES, caches = min(MOVE_CACHES, c.n_caches - cache0);
     const int s0 = __ldg(p.starts + r), n = (int)((unsigned)__ldg(p.starts + r + 1) - (unsigned)s0);
     const int len = __ldg(p.lens + r);
-    const long long base = (long long)len - n - p.prefix_len;  // own row of the first new one
-    if (n == 0) continue;
     const int32_t* table = p.tables + (int64_t)r * p.table_stride;
     const int32_t* path = p.path + (int64_t)r * p.path_stride;
+    const long long base = (long long)len - n - p.prefix_len;  // own row of the first new one
+    if (n == 0) continue;
     // the same in all lanes; a block of this lane's outside the caches
     bool wrong = n < 0 || base < 0 || (base + n - 1) / c.block_size >= p.table_width, lost = false;
     // This lane's element of own row `row`, or -1.
     auto place = [&](long long row) -> int64_t {
-      const int b = (int)(row / c.block_size), block = __ldg(table + b);
+      const int b = (int)((unsigned)row / (unsigned)c.block_size), block = __ldg(table + b);
       if (block < 0 || block >= c.n_blocks) {
         lost = true;
         return -1;
@@ -120,24 +122,28 @@ __global__ void __launch_bounds__(MOVE_THREADS) cache_compact_kernel(const __gri
       const unsigned bad = __ballot_sync(0xffffffffu, lane < run && node >= 0 && (node <= prior || node >= n));
       const int stop = min(ends ? __ffs(ends) - 1 : 32, bad ? __ffs(bad) - 1 : 32);
       if (bad && __ffs(bad) - 1 == stop) wrong = true;
-      uint4 v[MOVE_RUN];
-      int64_t to[MOVE_RUN];
+      uint4 v[MOVE_CACHES][MOVE_RUN];
+      int64_t from[MOVE_RUN], to[MOVE_RUN];
 #pragma unroll
       for (int x = 0; x < MOVE_RUN; ++x) {
-        const int k = x * at_once + sub, from = __shfl_sync(0xffffffffu, node, k & 31);
+        const int k = x * at_once + sub, source = __shfl_sync(0xffffffffu, node, k & 31);
         to[x] = -1;
-        if (k < stop && from != k0 + k) {
-          const int64_t src = place(base + from), dst = place(base + k0 + k);
-          if (src >= 0 && dst >= 0) {
-            to[x] = dst;
-            v[x] = *reinterpret_cast<const uint4*>(c.base[cache] + src);
-          }
+        if (k < stop && source != k0 + k) {
+          from[x] = place(base + source), to[x] = place(base + k0 + k);
+          if (from[x] < 0) to[x] = -1;
         }
       }
+#pragma unroll
+      for (int y = 0; y < MOVE_CACHES; ++y)
+#pragma unroll
+        for (int x = 0; x < MOVE_RUN; ++x)
+          if (y < caches && to[x] >= 0) v[y][x] = *reinterpret_cast<const uint4*>(c.base[cache0 + y] + from[x]);
       __syncwarp();
 #pragma unroll
-      for (int x = 0; x < MOVE_RUN; ++x)
-        if (to[x] >= 0) *reinterpret_cast<uint4*>(c.base[cache] + to[x]) = v[x];
+      for (int y = 0; y < MOVE_CACHES; ++y)
+#pragma unroll
+        for (int x = 0; x < MOVE_RUN; ++x)
+          if (y < caches && to[x] >= 0) *reinterpret_cast<uint4*>(c.base[cache0 + y] + to[x]) = v[y][x];
       __syncwarp();
       if (stop < run) break;
       before = __shfl_sync(0xffffffffu, node, run - 1);
@@ -182,12 +188,13 @@ extern "C" YSKN_B200_API int yskn_b200_cache_copy(const yskn_b200_cache_copy_arg
     return fail(YSKN_EINVAL, std::string("cache_copy: ") + what);
   if (!a.copies || a.max_copies < 1 || a.copies_stride < a.max_copies)
     return fail(YSKN_EINVAL, "cache_copy: no list of copies, or a stride below its width");
-  if (a.block_size > 1 << 20 || (int64_t)a.n_caches * a.n_kvh > INT32_MAX / 2)
-    return fail(YSKN_EINVAL, "cache_copy: blocks of more than 2^20 rows, or too many heads");
+  const int at_once = COPY_LOADS * (32 >> p.c.unit_shift);  // rows of a piece
+  const int64_t pieces = (int64_t)a.n_caches * a.n_kvh * ceil_div(a.block_size, at_once);  // of an entry
+  if (pieces > INT32_MAX) return fail(YSKN_EINVAL, "cache_copy: more rows, heads and caches than 2^31 pieces");
   p.copies = a.copies, p.copies_stride = a.copies_stride, p.count = a.count, p.max_copies = a.max_copies;
   p.err = device_error_word();
-  const int64_t units = (int64_t)a.max_copies * a.n_caches * a.n_kvh;
-  const unsigned grid = (unsigned)std::min<int64_t>(units, 148 * 6);
+  const int64_t ctas = ceil_div(a.max_copies * pieces, MOVE_WARPS);
+  const unsigned grid = (unsigned)std::min<int64_t>(ctas, 148 * COPY_CTAS);
   return cuda_fail(launch_pdl(cache_copy_kernel, grid, MOVE_THREADS, 0, reinterpret_cast<cudaStream_t>(stream), p),
                    "cache_copy_kernel");
 }
@@ -208,8 +215,8 @@ extern "C" YSKN_B200_API int yskn_b200_cache_compact(const yskn_b200_cache_compa
   p.path = a.path, p.path_stride = a.path_stride;
   p.batch = a.batch, p.table_width = a.table_width, p.prefix_len = a.prefix_len, p.path_width = a.path_width;
   p.err = device_error_word();
-  const int64_t units = ceil_div((int64_t)a.batch * a.n_caches * a.n_kvh, MOVE_WARPS);
-  const unsigned grid = (unsigned)std::min<int64_t>(units, 148 * 8);
+  const int64_t units = ceil_div((int64_t)a.batch * ceil_div(a.n_caches, MOVE_CACHES) * a.n_kvh, MOVE_WARPS);
+  const unsigned grid = (unsigned)std::min<int64_t>(units, 148 * 16);
   return cuda_fail(launch_pdl(cache_compact_kernel, grid, MOVE_THREADS, 0, reinterpret_cast<cudaStream_t>(stream), p),
                    "cache_compact_kernel");
 }
