@@ -732,11 +732,11 @@ typedef struct {
 YSKN_B200_API int yskn_b200_tree_plan(const yskn_b200_tree_plan_args* args, void* stream);
 
 /* yskn_b200_prefix_attention where a request's new tokens do not follow one another: new token t sees
- * every row before the request's new ones, and of those row j <= t if bit j % 32 of word j / 32 of its
- * mask row is set (uint32 mask [tokens][mask_stride], mask_words of them; bits past them count as
- * 0, and a request of more new tokens gives YSKN_EINVAL from yskn_b200_status). Everything else as
- * there, its workspace among it: a row that no bit and no cached row leaves anything gives zeros, and the
- * new rows hold numbers. */
+ * every row before the request's new ones (the whole prefix among them), and of those row j <= t if bit
+ * j % 32 of word j / 32 of its mask row is set (uint32 mask [tokens][mask_stride], mask_words of them).
+ * Everything else as there, its workspace and its size among it; a token that sees nothing gives zeros, and
+ * new rows that a token does not see may hold anything. A request of more new tokens than mask bits, or
+ * whose lens do not hold the prefix and its new tokens, gives zeros and YSKN_EINVAL from yskn_b200_status. */
 typedef struct {
   yskn_b200_prefix_attention_args attn;
   const uint32_t* mask;

@@ -43,14 +43,28 @@ def _started(cuda, sizes, P=75, **kw):
     return st
 
 
+def _choices(monkeypatch, forced):
+    """The selection answers forced[row] for those rows of a verification: the model's own choice is as good as a coin's
+    where two logits are about equal, and other orders of sums move them by 0.2 here."""
+    import yskn_b200 as Y
+    select = Y.head_select
+
+    def chosen(logits, token=None, **kw):
+        select(logits, token=token, **kw)
+        for row, t in forced.items():
+            token[row] = t
+
+    monkeypatch.setattr(Y, "head_select", chosen)
+
+
 @pytest.mark.parametrize("P", [0, 75])
-def test_verified_trees_equal_steps(cuda, P):
+def test_verified_trees_equal_steps(cuda, P, monkeypatch):
     import torch
     import yskn_b200 as Y
-    sizes, steps = [3, 19, 14], 7
+    sizes, right = [3, 19, 14], [4, 1, 0]
     one = _started(cuda, sizes, P)
     logits = [one.blogits.clone()]
-    for _ in range(steps):
+    for _ in range(6):
         one.new.fill_(1)
         one.step(3, 1)
         logits.append(one.blogits.clone())
@@ -58,23 +72,26 @@ def test_verified_trees_equal_steps(cuda, P):
 
     st = _started(cuda, sizes, P)
     # the true continuation's first 4, 1 and 0 tokens, each among others that are not the model's
-    right, trees = [4, 1, 0], []
+    forced, nodes = {}, []
     for i, n in enumerate(sizes):
-        true, tokens, parents, last = text[i][n + 1:n + 1 + right[i]], [], [], 0
-        for t in true:  # two wrong siblings, then the right one; a wrong child under one of the wrong ones
+        tokens, parents, path = [], [], [0]
+        for t in text[i][n + 1:n + 1 + right[i]]:  # two wrong ones, the right one, and the right one under a wrong one
             tokens += [(t + 1) % VOCAB, (t + 2) % VOCAB, t]
-            parents += [last, last, last]
+            parents += [path[-1]] * 3
+            path.append(len(tokens))
             tokens.append(t)
-            parents.append(len(tokens) - 2)  # the right token under a wrong one
-            last = len(tokens) - 1
+            parents.append(len(tokens) - 2)
         tokens.append((text[i][n + 1 + right[i]] + 5) % VOCAB)  # where the draft goes wrong
-        parents.append(last)
+        parents.append(path[-1])
         st.draft(i, tokens, parents)
-        trees.append((tokens, parents))
         st.new[i] = 1 + len(tokens)
-    total = int(st.new.sum())
+        first = int(st.new[:i].sum())
+        forced.update({first + node: text[i][n + 1 + k] for k, node in enumerate(path)})
+        nodes.append([first + node for node in path])
     before = st.free.item()
-    st.verify(total)
+    _choices(monkeypatch, forced)
+    st.verify(int(st.new.sum()))
+    monkeypatch.undo()
     assert Y.status() == 0
     assert st.accepted.tolist() == [1 + r for r in right]
     assert st.said.tolist() == [n + 2 + r for n, r in zip(sizes, right)]
@@ -82,17 +99,13 @@ def test_verified_trees_equal_steps(cuda, P):
     held = [-(-(n + 1 + r) // 16) - -(-n // 16) for n, r in zip(sizes, right)]
     assert st.free.item() == before - sum(held)
     for i, n in enumerate(sizes):
-        assert st.text[i, :n + 1 + right[i]].tolist() == text[i][:n + 1 + right[i]]
-    # every node on the path has the logits of the step that its token was said in, and the token behind the path
-    # is one that these leave room for (two of about equal logits may change places)
-    starts = st.starts.tolist()
-    for i, n in enumerate(sizes):
-        for k, node in enumerate(st.path[i].tolist()[:1 + right[i]]):
-            assert _close(st.tlogits[starts[i] + node], logits[1 + k][i]) <= TOL, (i, k)
-        row, last = st.tlogits[starts[i] + node], logits[1 + k][i]
-        said = st.text[i, n + 1 + right[i]].item()
-        assert said == int(row.argmax()) and last.max() - last[said] <= 2 * (row - last).abs().max()
-        st.text[i, n + 1 + right[i]] = text[i][n + 1 + right[i]]
+        assert st.text[i, :n + 2 + right[i]].tolist() == text[i][:n + 2 + right[i]]
+        # every node on the path has the logits of the step that its token was said in, and they leave room for what
+        # was chosen there
+        for k, node in enumerate(nodes[i]):
+            row, step = st.tlogits[node], logits[1 + k][i]
+            assert _close(row, step) <= TOL, (i, k)
+            assert row.max() - row[text[i][n + 1 + k]] <= 2 * (row - step).abs().max()
     # and the cache is as those steps left it
     st.new.fill_(1)
     st.step(3, 1)
@@ -101,28 +114,20 @@ def test_verified_trees_equal_steps(cuda, P):
     assert Y.status() == 0
 
 
-def test_wrong_rows_in_the_cache_would_show(cuda):
+def test_wrong_rows_in_the_cache_would_show(cuda, monkeypatch):
     """The tolerance tells a cache with the path's rows left where they were from a packed one."""
     import yskn_b200 as Y
-    sizes, P = [9], 40  # whose first choices are far from their seconds: 0.7, where logits differ by 0.2
-    one = _started(cuda, sizes, P)
-    for _ in range(3):
-        one.new.fill_(1)
-        one.step(1, 1)
-    text = one.text.tolist()[0]
-    compact = Y.cache_compact
     far = []
     for packed in (True, False):
-        st = _started(cuda, sizes, P)
-        st.draft(0, [(text[10] + 1) % VOCAB, (text[10] + 2) % VOCAB, text[10], text[11]], [0, 0, 0, 3])
+        st = _started(cuda, [9], 40)
+        st.draft(0, [1, 2, 3, 4], [0, 0, 0, 3])
         st.new.fill_(5)
-        try:
-            if not packed:
-                Y.cache_compact = lambda *a, **k: None
-            st.verify(5)
-        finally:
-            Y.cache_compact = compact
-        assert st.accepted.tolist() == [3]
+        _choices(monkeypatch, {0: 3, 3: 4, 4: 5})
+        if not packed:
+            monkeypatch.setattr(Y, "cache_compact", lambda *a, **k: None)
+        st.verify(5)
+        monkeypatch.undo()
+        assert st.accepted.tolist() == [3] and st.text[0, 10:13].tolist() == [3, 4, 5]
         st.new.fill_(1)
         st.step(1, 1)
         far.append(st.blogits[0].clone())

@@ -167,7 +167,8 @@ def test_many_requests_and_long_contexts(cuda):
 
 
 def test_a_chains_mask_is_the_plain_order(cuda):
-    """Every earlier row's bit set: the bits of prefix_attention, item for item."""
+    """Every earlier row's bit set: what prefix_attention gives, whose error is bounded like this one's: each half a step
+    of the result and of the weights, and little else."""
     import torch
     import yskn_b200 as Y
     B, n, ctx, D, hq, hk, bs = 3, 21, 150, 128, 6, 2, 64
@@ -184,36 +185,45 @@ def test_a_chains_mask_is_the_plain_order(cuda):
     Y.tree_attention(q, kc, vc, tables, lens, starts, n, torch.full((B * n, 1), -1, dtype=torch.int32, device=cuda),
                      work, b)
     torch.cuda.synchronize()
-    assert torch.equal(a, b)
+    most = vc.float().abs().max()  # a weighted mean of values: A is at most this
+    assert bool(((a.float() - b.float()).abs() <= 2 * (2.0 ** -8 * (a.float().abs() + most) + 2.0 ** -10 * most)).all())
 
 
-def test_scores_of_masked_rows_may_be_anything(cuda):
-    """Keys of infinities and NaN in rows that a token does not see change nothing for it."""
+@pytest.mark.parametrize("hq,hk,n,ctx", [(6, 2, 20, 50), (2, 2, 4, 50), (24, 4, 40, 0), (8, 1, 33, 200)])
+def test_hidden_rows_may_hold_anything(cuda, hq, hk, n, ctx):
+    """Keys and values of infinities and NaN in new rows that a token does not see change no bit of its result."""
     import torch
     import yskn_b200 as Y
-    for hq, hk, n in ((6, 2, 20), (2, 2, 4)):
-        D, bs, ctx = 64, 16, 50
-        g = torch.Generator(device=cuda)
-        g.manual_seed(n)
-        rnd = lambda *s: torch.randn(s, generator=g, device=cuda).bfloat16()  # noqa: E731
-        q, kc, vc = rnd(n, hq, D), rnd(6, bs, hk, D), rnd(6, bs, hk, D)
-        tables = torch.arange(6, dtype=torch.int32, device=cuda).view(1, 6)
-        lens = torch.tensor([ctx + n], dtype=torch.int32, device=cuda)
-        starts = torch.tensor([0, n], dtype=torch.int32, device=cuda)
-        mask = torch.tensor([[1 | 1 << t] for t in range(n)], dtype=torch.int32, device=cuda)  # a star
-        work = torch.empty(Y.prefix_attention_work_bytes(n, 1, n, hq, hk, D), dtype=torch.uint8, device=cuda)
-        outs = []
-        for bad in (None, float("nan"), float("inf"), -float("inf")):
-            k2 = kc.clone()
-            if bad is not None:
-                row = ctx + n - 2
+    D, bs = 64, 16
+    g = torch.Generator(device=cuda)
+    g.manual_seed(n)
+    rnd = lambda *s: torch.randn(s, generator=g, device=cuda).bfloat16()  # noqa: E731
+    blocks = -(-(ctx + n) // bs)
+    q, kc, vc = rnd(n, hq, D), rnd(blocks, bs, hk, D), rnd(blocks, bs, hk, D)
+    tables = torch.arange(blocks, dtype=torch.int32, device=cuda).view(1, blocks)
+    lens = torch.tensor([ctx + n], dtype=torch.int32, device=cuda)
+    starts = torch.tensor([0, n], dtype=torch.int32, device=cuda)
+    mask = torch.zeros((n, 2), dtype=torch.int64, device=cuda)  # a star, all of whose nodes see node 0 and themselves
+    for t in range(n):
+        mask[t, 0] |= 1
+        mask[t, t // 32] |= 1 << t % 32
+    mask = torch.where(mask >= 2 ** 31, mask - 2 ** 32, mask).to(torch.int32)
+    work = torch.empty(Y.prefix_attention_work_bytes(n, 1, n, hq, hk, D), dtype=torch.uint8, device=cuda)
+    outs, hidden = [], [n - 2, 1]
+    for bad in (None, float("nan"), float("inf"), -float("inf")):
+        k2, v2 = kc.clone(), vc.clone()
+        if bad is not None:
+            for j in hidden:
+                row = ctx + j
                 k2[row // bs, row % bs] = bad
-            out = torch.empty_like(q)
-            Y.tree_attention(q, k2, vc, tables, lens, starts, n, mask, work, out)
-            torch.cuda.synchronize()
-            outs.append(out)
-        others = [t for t in range(n) if t != n - 2]
-        assert all(torch.equal(outs[0][others], o[others]) for o in outs[1:])
+                v2[row // bs, row % bs] = bad
+        out = torch.empty_like(q)
+        Y.tree_attention(q, k2, v2, tables, lens, starts, n, mask, work, out)
+        torch.cuda.synchronize()
+        outs.append(out)
+    others = [t for t in range(n) if t not in hidden]
+    assert all(torch.equal(outs[0][others], o[others]) for o in outs[1:])
+    assert all(bool(o[hidden].isnan().any()) for o in outs[1:3])  # those that see it, see it
     assert Y.status() == 0
 
 

@@ -32,10 +32,6 @@
 // itself. Everything is summed in a fixed order: the same call gives the same bits. The lengths stay
 // on the device: every CTA forms the prefix sum of the requests' units itself.
 //
-// Trees of drafted tokens (TREE; yskn_b200_tree_attention): the same, but of its request's new rows a token sees
-// those of its mask only. Its bits leave a row's weight out beside the bound on its tile, in the tiles
-// that hold new rows: one or two of a request's last.
-//
 // prefix_attention_kernel: persistent, clusters of two CTAs (a pair of SMs), 12 warps each. The
 // pair works on 256 rows with tcgen05.mma.cta_group::2: each CTA holds its 128 rows of Q, S, P and
 // O, and half of each K tile (64 of its 128 rows) and V tile (half of the channels). With one
@@ -69,8 +65,7 @@
 #include <cmath>
 #include <type_traits>
 
-#include "paged.cuh"
-#include "tcgen05.cuh"
+#include "attention.cuh"
 
 namespace yskn {
 
@@ -172,10 +167,6 @@ struct PrefixAttnParams {
   float c;     // |scale| log2 e
   uint32_t negate_q;
   int4* work_per;  // for the join: units per pair of prefix items and of own ones, prefix tiles (-1: alone), own units
-  const uint32_t* mask;  // trees: [tokens][mask_stride], mask_words used
-  int64_t mask_stride;
-  int mask_words;
-  int64_t least_before;  // rows before a request's new ones, at least (trees: the prefix; else any number)
   int2* work_base;        // [batch] own items, and units of all items, before each request's own
   // per place: (m, l) of each row; o as [D / 4][rows][4], so that a warp's rows are adjacent
   float2 *pre_ml, *own_ml;
@@ -217,8 +208,7 @@ __device__ __forceinline__ PaRequest pa_request(const PrefixAttnParams& p, int i
   r.s0 = __ldg(p.starts + i);
   const int n = (int)((unsigned)__ldg(p.starts + i + 1) - (unsigned)r.s0);  // whatever the two are
   r.len = __ldg(p.lens + i);
-  const bool wrong = n < 0 || n > p.max_new || r.s0 < 0 || r.s0 > p.tokens - n || r.len < p.least_before + n;
-  r.n = wrong ? 0 : n;
+  r.n = n < 0 || n > p.max_new || r.s0 < 0 || r.s0 > p.tokens - n ? 0 : n;
   return r;
 }
 // Own rows that the last of the request's first `upto` tokens sees.
@@ -252,14 +242,6 @@ __device__ __forceinline__ unsigned pa_own_units(const PrefixAttnParams& p, cons
   return u;
 }
 
-// Bits of token t's mask from new row `at` on (32 of them, those of rows before the new ones set).
-__device__ __forceinline__ uint32_t tree_bits(const PrefixAttnParams& p, int64_t t, int at) {
-  const uint32_t* row = p.mask + t * p.mask_stride;
-  const int w = at >> 5;
-  auto word = [&](int i) { return i < 0 ? 0xffffffffu : i < p.mask_words ? __ldg(row + i) : 0u; };
-  return __funnelshift_r(word(w), word(w + 1), at & 31);
-}
-
 struct PaSegment {
   bool prefix, whole;   // prefix item; all that its rows see
   int kvh, tok0, ntok;  // KV head, first token and whole tokens
@@ -270,10 +252,6 @@ struct PaSegment {
   int first;            // rows of the sequence that token tok0 sees, one more for each token (prefix
                         // items: as if its last token saw what the longest request does)
   int64_t place;        // of its partial result
-  // Own row of the request's first new one (own items).
-  __device__ int first_new(const PrefixAttnParams& p) const {
-    return first - 1 - (tok0 - __ldg(p.starts + req)) - p.prefix_len;
-  }
   // Rows of the prefix that any of its tokens sees.
   __device__ int pre_keys(const PrefixAttnParams& p) const { return min(first + ntok - 1, p.prefix_len); }
   // Rows of tile kt that the rows on its axis leave it.
@@ -377,121 +355,6 @@ struct PaWalk {
   }
 };
 
-// B operand whose N runs along the swizzled rows (V: rows are keys, MMA K), in columns of LINE
-// bytes `stride` bytes apart, 8-key groups 8 LINE bytes apart. Swizzle span 128 or 64 bytes.
-template <int LINE>
-__device__ __forceinline__ uint64_t mn_desc(uint32_t saddr, uint32_t stride) {
-  return (uint64_t)((saddr >> 4) & 0x3fff) | ((uint64_t)(stride >> 4) << 16) | ((uint64_t)(8 * LINE >> 4) << 32) |
-         (1ull << 46) | ((LINE == 128 ? 2ull : 4ull) << 61);
-}
-// kind::f16 with f32 accumulators, M = 256: type of both operands, N, B's major axis, A's sign.
-__device__ __forceinline__ uint32_t pa_idesc(int dt, int n, uint32_t b_mn, uint32_t negate_a) {
-  const uint32_t t = dt == YSKN_DT_BF16 ? 1u : 0u;
-  return (1u << 4) | (t << 7) | (t << 10) | (negate_a << 13) | (b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
-         ((uint32_t)(2 * PA_ROWS >> 4) << 24);
-}
-// A and B by the low words of their descriptors (the high words are the same throughout), which
-// leaves one 32-bit addition per operand and step to the issuing thread.
-__device__ __forceinline__ void umma2_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc,
-                                         uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\t"
-      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(accumulate));
-}
-__device__ __forceinline__ void umma2_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc,
-                                         uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b), "r"(hi), "r"(idesc), "r"(accumulate));
-}
-// One lane of a converged warp.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t one;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
-  return one != 0;
-}
-// Arrives on the barrier at this place in both CTAs once the MMAs issued so far are done.
-__device__ __forceinline__ void umma2_commit(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-          smem_u32(bar)),
-      "h"((uint16_t)3)
-      : "memory");
-}
-
-// ---- the pair: addresses and barriers of its first CTA
-__device__ __forceinline__ uint32_t first_cta(const void* p) {
-  uint32_t a;
-  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
-  return a;
-}
-// What these two announce is in TMEM or comes by TMA, so that they order no memory of their own
-// (cluster-scope release and acquire here cost hundreds of clocks each: 16 prompt chunks 1439 us, now 986).
-__device__ __forceinline__ void arrive_first(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void expect_first(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-// After stores to this CTA's shared memory that the first CTA's MMAs read.
-__device__ __forceinline__ void release_first(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// TMA into this CTA's shared memory, counted on a barrier of the pair's first CTA.
-__device__ __forceinline__ void pair_load_3d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
-      "%5}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
-      : "memory");
-}
-__device__ __forceinline__ void pair_load_5d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z,
-                                             int w, int v) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
-      "%5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v)
-      : "memory");
-}
-
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
-// Two binary32 operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 y;
-  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(y.x), "=f"(y.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return y;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 y;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\t"
-      "mov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(y.x), "=f"(y.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return y;
-}
-// The gate's factor. (A row that sees nothing is zero whatever its gate holds.)
-__device__ __forceinline__ float gated(float x, float gate) {
-  return __fdividef(x, 1.0f + exp2_approx(-1.44269504f * gate));
-}
 // Four of the output gate's channels from element `at` on, as they are stored, and as f32: apart, so
 // that several loads are under way before the first is waited for.
 __device__ __forceinline__ uint4 gate_load(const PrefixAttnParams& p, int64_t at) {
@@ -629,7 +492,7 @@ struct ThinCursor {
   }
 };
 
-template <int D, int DT, bool TREE>
+template <int D, int DT>
 __device__ __forceinline__ void thin_items(const PrefixAttnParams& p, const PaStart& start, uint8_t* smem, int warp,
                                            int lane) {
   constexpr int C = D / 64, CHUNKS = 2 * C;  // chunks of a slice's K; of K and V
@@ -682,7 +545,6 @@ __device__ __forceinline__ void thin_items(const PrefixAttnParams& p, const PaSt
   for (int taken = 0; taken < from.found;) {
     const PaSegment& seg = queue[taken % PA_THIN_QUEUE];
     const int n_rows = seg.ntok * p.G, sees = seg.first + tl;  // rows of the sequence that row g sees
-    const int first_new = TREE ? seg.first_new(p) : 0;
     float o[C][4][4];
 #pragma unroll
     for (int x = 0; x < C * 16; ++x) o[x / 16][x / 4 % 4][x % 4] = 0.0f;
@@ -719,14 +581,6 @@ __device__ __forceinline__ void thin_items(const PrefixAttnParams& p, const PaSt
       for (int x = 0; x < 4; ++x) {
         z[x] = (s[x >> 1][x & 1] + s[2 + (x >> 1)][x & 1]) * c;
         if ((x & 1) + 8 * (x >> 1) >= seen) z[x] = -INFINITY;
-      }
-      if constexpr (TREE) {
-        if (!pre && first + (1 << PA_THIN_SHIFT) > first_new) {
-          const uint32_t bits = g < n_rows ? tree_bits(p, seg.tok0 + tl, first - first_new) >> 2 * t : 0;
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            if (!(bits >> ((x & 1) + 8 * (x >> 1)) & 1)) z[x] = -INFINITY;
-        }
       }
       float top = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -833,7 +687,7 @@ struct PaShared {
 };
 static_assert(sizeof(PaShared) <= 3072, "shared memory beside the ring");
 
-template <int D, int DT, bool TREE>
+template <int D, int DT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
     prefix_attention_kernel(const __grid_constant__ CUtensorMap map_q_pre, const __grid_constant__ CUtensorMap map_q_own,
                             const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -996,7 +850,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
   const uint32_t tmem = sh.tmem_slot;
   if (sh.start[0].thin) {
     if (p.whole && warp == PA_THIN_WARPS - 1) zero_unheld<D>(p, sh.start[0].sound, lane);
-    thin_items<D, DT, TREE>(p, sh.start[warp], smem, warp, lane);
+    thin_items<D, DT>(p, sh.start[warp], smem, warp, lane);
   } else {
     PaWalk walk(p, sh.start[0]);
     PaSegment seg;
@@ -1107,7 +961,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
     } else if (warp == 1) {
       // ---- MMAs: one thread of the first CTA
       if (rank == 0 && elect_one()) {
-        const uint32_t id_qk = pa_idesc(DT, PA_KEYS, 0, p.negate_q), id_pv = pa_idesc(DT, D, 1, 0);
+        const uint32_t id_qk = pair_idesc(DT, PA_KEYS, 0, p.negate_q), id_pv = pair_idesc(DT, D, 1, 0);
         int s = 0, g = 0, n_seg = 0;  // ring place, tiles issued, segments
         uint32_t turn = 0;
         bool ok = true;
@@ -1247,8 +1101,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
         // on either axis, and the least of the warp's rows
         const int lim_pre = min(lim, p.prefix_len), lim_own = min(max(lim - p.prefix_len, 0), seg.keys);
         const int least_pre = __reduce_min_sync(0xffffffffu, valid ? lim_pre : INT32_MAX);
-        const int first_new = TREE && !seg.prefix ? seg.first_new(p) : INT32_MAX;
-        const int least_own = min((int)__reduce_min_sync(0xffffffffu, valid ? lim_own : INT32_MAX), first_new);
+        const int least_own = __reduce_min_sync(0xffffffffu, valid ? lim_own : INT32_MAX);
         float m = -INFINITY, l = 0.0f;
         for (int kt = seg.key0; kt < seg.key1; ++kt, ++g) {
           const int b = g & 1;
@@ -1269,18 +1122,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PA_THREADS, 1)
 #pragma unroll
               for (int x = 0; x < 64; ++x)
                 if (x >= see) s[x >> 5][x & 31] = 0xff800000u;  // -inf
-              if constexpr (TREE) {
-                if (!pre) {
-                  const int at = from + half * 64 - first_new;
-#pragma unroll
-                  for (int y = 0; y < 2; ++y) {
-                    const uint32_t bits = valid ? tree_bits(p, seg.tok0 + tl, at + 32 * y) : 0;
-#pragma unroll
-                    for (int x = 0; x < 32; ++x)
-                      if (!(bits >> x & 1)) s[y][x] = 0xff800000u;
-                  }
-                }
-              }
             }
             auto val = [&](int x) { return __uint_as_float(s[x >> 5][x & 31]); };
             float t[4] = {val(0), val(1), val(2), val(3)};
@@ -1638,36 +1479,18 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const __grid_consta
   }
 }
 
-template <int D, int DT, bool TREE>
+template <int D, int DT>
 static int launch_prefix_attention(const CUtensorMap (&maps)[4], const PrefixAttnParams& p, int grid, cudaStream_t st) {
   static SmemOptIn opt_in;
-  if (cudaError_t e = opt_in(prefix_attention_kernel<D, DT, TREE>, PaShape<D>::SMEM))
+  if (cudaError_t e = opt_in(prefix_attention_kernel<D, DT>, PaShape<D>::SMEM))
     return cuda_fail(e, "prefix_attention_kernel attributes");
-  if (cudaError_t e = launch_pdl(prefix_attention_kernel<D, DT, TREE>, grid, PA_THREADS, PaShape<D>::SMEM, st, maps[0],
+  if (cudaError_t e = launch_pdl(prefix_attention_kernel<D, DT>, grid, PA_THREADS, PaShape<D>::SMEM, st, maps[0],
                                  maps[1], maps[2], maps[3], p))
     return cuda_fail(e, "prefix_attention_kernel");
   if (p.whole) return YSKN_OK;
   const int64_t warps = ceil_div((int64_t)p.tokens * p.G, 8) * (D / 16 / p.join_span) * p.join_split;
   return cuda_fail(launch_pdl(prefix_combine_kernel<D, DT>, dim3((unsigned)ceil_div(warps, 8), p.n_kvh), 256, 0, st, p),
                    "prefix_combine_kernel");
-}
-
-// 16-bit tensor of 3 to 5 axes with swizzled boxes of 64 channels (128-byte lines) or 32 (64). Strides in elements.
-static int paged_map(const char* name, CUtensorMap* map, const void* base, int dt, int rank, const int64_t* dims,
-                     const int64_t* strides, const int* box) {
-  EncodeTiled fn = encode_fn();
-  if (!fn) return fail(YSKN_ECUDA, "cuTensorMapEncodeTiled is not available");
-  cuuint64_t d[5], s[4];
-  cuuint32_t b[5], one[5] = {1, 1, 1, 1, 1};
-  for (int i = 0; i < rank; ++i) d[i] = (cuuint64_t)dims[i], b[i] = (cuuint32_t)box[i];
-  for (int i = 0; i + 1 < rank; ++i) s[i] = (cuuint64_t)(dims[i + 1] == 1 ? dims[0] : strides[i]) * 2;
-  const CUresult r = fn(map, dt == YSKN_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                        rank, const_cast<void*>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        box[0] == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(YSKN_EINVAL, std::string(name) + ": strides that a tensor map cannot hold");
-  return YSKN_OK;
 }
 
 }  // namespace yskn
@@ -1682,35 +1505,14 @@ extern "C" YSKN_B200_API int64_t yskn_b200_prefix_attention_work_bytes(int token
   return pa_work(tokens, batch, max_new, n_qh, n_kvh, head).bytes;
 }
 
-// The call `name`, with the tree's masks where there are some.
-static int attention(const char* name, yskn_b200_prefix_attention_args a, const uint32_t* mask, int64_t mask_stride,
-                     int mask_words, void* stream) {
-  auto refuse = [&](const char* what) { return fail(YSKN_EINVAL, std::string(name) + ": " + what); };
-  if (!a.q || !a.k_cache || !a.v_cache || !a.block_tables || !a.lens || !a.starts || !a.work || !a.out ||
-      (a.prefix_len > 0 && !a.prefix_blocks))
-    return refuse("null argument");
+extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_attention_args* args, void* stream) {
+  if (!args) return fail(YSKN_EINVAL, "prefix_attention: null argument");
+  yskn_b200_prefix_attention_args a = *args;
+  if (const char* what = attention_refusal(a)) return fail(YSKN_EINVAL, std::string("prefix_attention: ") + what);
   const int head = a.head, n_qh = a.n_qh, n_kvh = a.n_kvh, block_size = a.block_size, dtype = a.dtype;
-  if (head != 64 && head != 128 && head != 256)
-    return refuse("heads of 64, 128 or 256 channels");
-  if (!is_16bit(dtype) || (a.gate && a.gate_dtype != dtype && a.gate_dtype != YSKN_DT_F32))
-    return refuse("queries and cache are f16 or bf16, the gate of their type or f32");
-  if (a.tokens < 1 || a.batch < 1 || a.max_new < 1 || n_kvh < 1 || n_qh < 1 || n_qh % n_kvh || n_qh / n_kvh > PA_ROWS ||
-      a.prefix_len < 0 || a.table_width < 1 || (a.batch > 1 && a.table_stride < a.table_width) || a.n_blocks < 1)
-    return refuse("empty shape, heads not a multiple, or a stride below its width");
-  if (block_size != 16 && block_size != 32 && block_size != 64 && block_size != 128)
-    return refuse("blocks of 16, 32, 64 or 128 rows");
-  if (a.tokens == 1) a.q_row = a.gate_row = 0;  // strides that nothing steps over may be anything
-  if (n_qh == 1) a.q_head = a.gate_head = 0;
-  if (n_kvh == 1) a.head_stride = 0;
-  if (a.n_blocks == 1) a.block_stride = 0;
-  if (!aligned16(a.q) || !aligned16(a.gate) || !aligned16(a.k_cache) || !aligned16(a.v_cache) || !aligned16(a.work) ||
-      !aligned16(a.out) || (a.q_row | a.q_head | a.block_stride | a.token_stride | a.head_stride) % 8 ||
-      (a.gate && (a.gate_row | a.gate_head) % (a.gate_dtype == YSKN_DT_F32 ? 4 : 8)))
-    return refuse("pointers and strides are multiples of 16 bytes");
   a.max_new = std::min(a.max_new, a.tokens);  // as pa_work does
-  if (mask) a.max_new = (int)std::min<int64_t>(a.max_new, 32ll * mask_words);
   const PaWork w = pa_work(a.tokens, a.batch, a.max_new, n_qh, n_kvh, head);
-  if (a.work_bytes < w.bytes) return refuse("workspace too small");
+  if (a.work_bytes < w.bytes) return fail(YSKN_EINVAL, "prefix_attention: workspace too small");
   const int G = n_qh / n_kvh, tpc = PA_ROWS / G;
   int dev = 0, sms = 2 * PA_MAX_PAIRS;
   cudaGetDevice(&dev);
@@ -1725,8 +1527,6 @@ static int attention(const char* name, yskn_b200_prefix_attention_args a, const 
   p.prefix_blocks = a.prefix_blocks;
   p.tables = a.block_tables, p.table_stride = a.table_stride;
   p.lens = a.lens, p.starts = a.starts;
-  p.mask = mask, p.mask_stride = mask_stride, p.mask_words = mask_words;
-  p.least_before = mask ? a.prefix_len : -(int64_t(1) << 40);
   p.n_blocks = a.n_blocks, p.prefix_len = a.prefix_len;
   p.block_shift = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : 7;
   p.own_limit = (int)std::min<int64_t>((int64_t)a.table_width * block_size, INT32_MAX - PA_KEYS);
@@ -1739,7 +1539,7 @@ static int attention(const char* name, yskn_b200_prefix_attention_args a, const 
   const int64_t items = (int64_t)p.pre_qtiles * n_kvh;
   if (items * pa_units(pre_tiles, false, PA_ITEM_COST) >= (int64_t)PA_MANY ||
       (int64_t)a.tokens * n_qh * head > INT32_MAX || a.tokens >= 1 << 24 || n_kvh > 65535)
-    return refuse("too much work");
+    return fail(YSKN_EINVAL, "prefix_attention: too much work");
   p.shared_items = a.prefix_len > 0 ? (int)items : 0;
   // Few items of few tiles: each by one pair of SMs (a thin one by one warp) from end to end, which is
   // quicker than the second launch that joins its parts. Two requests, us whole and cut: of two
@@ -1785,36 +1585,21 @@ static int attention(const char* name, yskn_b200_prefix_attention_args a, const 
                         block_size < v_rows || head <= 128 ? 1 : head / 128, 1, 1};
   CUtensorMap maps[4] = {};
   if (!p.thin || p.shared_items > 0) {  // thin items need no map
-    if (int rc = paged_map(name, &maps[0], a.q, dtype, 3, q_dims, q_strides, box_pre)) return rc;
-    if (int rc = paged_map(name, &maps[2], a.k_cache, dtype, 5, c_dims, c_strides, box_k)) return rc;
-    if (int rc = paged_map(name, &maps[3], a.v_cache, dtype, 5, c_dims, c_strides, box_v)) return rc;
+    if (int rc = paged_map("prefix_attention", &maps[0], a.q, dtype, 3, q_dims, q_strides, box_pre)) return rc;
+    if (int rc = paged_map("prefix_attention", &maps[2], a.k_cache, dtype, 5, c_dims, c_strides, box_k)) return rc;
+    if (int rc = paged_map("prefix_attention", &maps[3], a.v_cache, dtype, 5, c_dims, c_strides, box_v)) return rc;
     maps[1] = maps[0];
     if (!p.thin)
-      if (int rc = paged_map(name, &maps[1], a.q, dtype, 3, q_dims, q_strides, box_own)) return rc;
+      if (int rc = paged_map("prefix_attention", &maps[1], a.q, dtype, 3, q_dims, q_strides, box_own)) return rc;
   }
   const int grid = 2 * pairs;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   auto run = [&](auto d) {
     constexpr int D = decltype(d)::value;
-    if (mask)
-      return dtype == YSKN_DT_BF16 ? launch_prefix_attention<D, YSKN_DT_BF16, true>(maps, p, grid, st)
-                                   : launch_prefix_attention<D, YSKN_DT_F16, true>(maps, p, grid, st);
-    return dtype == YSKN_DT_BF16 ? launch_prefix_attention<D, YSKN_DT_BF16, false>(maps, p, grid, st)
-                                 : launch_prefix_attention<D, YSKN_DT_F16, false>(maps, p, grid, st);
+    return dtype == YSKN_DT_BF16 ? launch_prefix_attention<D, YSKN_DT_BF16>(maps, p, grid, st)
+                                 : launch_prefix_attention<D, YSKN_DT_F16>(maps, p, grid, st);
   };
   if (head == 64) return run(std::integral_constant<int, 64>{});
   if (head == 128) return run(std::integral_constant<int, 128>{});
   return run(std::integral_constant<int, 256>{});
-}
-
-extern "C" YSKN_B200_API int yskn_b200_prefix_attention(const yskn_b200_prefix_attention_args* args, void* stream) {
-  if (!args) return fail(YSKN_EINVAL, "prefix_attention: null argument");
-  return attention("prefix_attention", *args, nullptr, 0, 0, stream);
-}
-
-extern "C" YSKN_B200_API int yskn_b200_tree_attention(const yskn_b200_tree_attention_args* args, void* stream) {
-  if (!args || !args->mask) return fail(YSKN_EINVAL, "tree_attention: null argument");
-  if (args->mask_words < 1 || (args->attn.tokens > 1 && args->mask_stride < args->mask_words))
-    return fail(YSKN_EINVAL, "tree_attention: no mask words, or a stride below them");
-  return attention("tree_attention", args->attn, args->mask, args->mask_stride, args->mask_words, stream);
 }
