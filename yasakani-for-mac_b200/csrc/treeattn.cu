@@ -74,7 +74,7 @@ struct TaShape {
 // those of the own items', own_rows each; a place more for each cut, of which there is one a pair at most.
 struct TaWork {
   int64_t base, ml, o, bytes;  // byte offsets
-  int own_half, own_rows;      // rows of a CTA and of the pair in an own item's place
+  int own_rows;                // of an own item's place
   int64_t own_items;           // own items that there is room for
   int pre_items;
 };
@@ -82,8 +82,7 @@ inline TaWork ta_work(int tokens, int batch, int max_new, int prefix_len, int n_
   auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
   const int G = n_qh / n_kvh, tpc = TA_ROWS / G, tpi = 2 * tpc;  // tokens per CTA and per item
   TaWork w{};
-  w.own_half = G * std::min(tpc, max_new);
-  w.own_rows = max_new > tpc ? 2 * w.own_half : w.own_half;
+  w.own_rows = G * std::min(tpi, max_new);
   // sum of ceil(n_i / tpi) over requests with n_i > 0: at most one more than n_i / tpi each
   w.own_items = (std::min(batch, tokens) + (int64_t)tokens / tpi) * n_kvh;
   w.pre_items = prefix_len > 0 ? (int)(ceil_div(tokens, tpi) * n_kvh) : 0;
@@ -123,7 +122,7 @@ struct TreeAttnParams {
   int2* base;  // [batch] own items, and units of all items, before each request's own
   float2* ml;  // (m, l) of each row of results
   float* o;
-  int own_half, own_rows;
+  int own_rows;
   long long own_items;  // more of them (starts that do not ascend), or 2^30 units, is an error: nothing is computed
   uint16_t* out;        // [tokens][n_qh][D]
   unsigned* err;
@@ -167,6 +166,9 @@ struct TaSegment {
   int key0, key1;       // key tiles [key0, key1)
   int pre;              // the item's first tiles that are the prefix's
   int own;              // own rows
+  // The item's tokens are halved between the CTAs: the first one of a CTA, and how many.
+  __device__ int first_of(int rank) const { return rank ? (ntok + 1) >> 1 : 0; }
+  __device__ int tokens_of(int rank) const { return rank ? ntok >> 1 : (ntok + 1) >> 1; }
   // Rows of tile kt.
   __device__ int rows_of(const TreeAttnParams& p, int kt) const {
     return min(TA_KEYS, kt < pre ? p.prefix_len - kt * TA_KEYS : own - (kt - pre) * TA_KEYS);
@@ -588,13 +590,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TA_THREADS, 1)
         for (int i = 0; i < n_list; ++i, ++n_seg) {
           const TaSegment seg = sh.list[i];
           if (n_seg > 0 && !(ok = ok && mbar_wait(&sh.q_empty, (n_seg - 1) & 1, abort_flag))) break;
-          const bool prefix = seg.req < 0, any = seg.ntok > rank * p.tpc;
+          const bool prefix = seg.req < 0, any = seg.tokens_of(rank) > 0;
           const int box = prefix ? p.tpc : min(p.tpc, p.max_new);
           expect_first(bar, any ? (uint32_t)(box * p.G * 128 * Shape::CHUNKS) : 0u);
           if (any)
             for (int d = 0; d < Shape::CHUNKS; ++d)
               pair_load_3d(sQ + d * TA_ROWS * 128, prefix ? &map_q_pre : &map_q_own, bar, d * 64, seg.kvh * p.G,
-                           seg.tok0 + rank * p.tpc);
+                           seg.tok0 + seg.first_of(rank));
         }
         if (!ok) {
           const long long t0 = clock64();
@@ -638,7 +640,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TA_THREADS, 1)
       const float c = fabsf(p.c);
       for (int i = 0; i < n_list; ++i) {
         const TaSegment seg = sh.list[i];
-        const bool valid = row < min(p.tpc, seg.ntok - rank * p.tpc) * p.G;
+        const bool valid = row < seg.tokens_of(rank) * p.G;
         const bool live = __any_sync(0xffffffffu, valid);  // a warp without rows only keeps the barriers going
         float m = -INFINITY, l = 0.0f;
         for (int kt = seg.key0; kt < seg.key1; ++kt, ++g) {
@@ -720,7 +722,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TA_THREADS, 1)
           ta_quarter_sync(quarter);
           l += sh.half[0][half ^ 1][row];
           const int rows = seg.req < 0 ? 2 * TA_ROWS : p.own_rows;
-          const int at = rank * (seg.req < 0 ? TA_ROWS : p.own_half) + row;  // of the place
+          const int at = seg.first_of(rank) * p.G + row;  // of the place
           float4* o = reinterpret_cast<float4*>(p.o + (int64_t)seg.row0 * D) + at;
           for (int x = half * (D / 2); x < (half + 1) * (D / 2); x += 32) {
             uint32_t v[32];
@@ -953,22 +955,22 @@ __global__ void __launch_bounds__(128 * (1 + S), S == 0 ? TJ_RESIDENT : 1)
     int64_t pre_row = 0, own_row = 0;
     if (valid && sound) {
       if (pre_units > 0) {
-        const int each = ta_units(p.pre_tiles), qt = ta_quotient(t, p.tpi_magic), in = t - qt * p.tpi;
+        const int each = ta_units(p.pre_tiles), qt = ta_quotient(t, p.tpi_magic);
         const int item = kvh * (p.pre_items / p.n_kvh) + qt, b = item * each + TA_COST, c0 = b / per;
         n_pre = (b + p.pre_tiles - 1) / per - c0 + 1;
         pre_row = (int64_t)(item + c0) * 2 * TA_ROWS;
-        pre_in = in < p.tpc ? in * p.G + gh : TA_ROWS + (in - p.tpc) * p.G + gh;
+        pre_in = (t - qt * p.tpi) * p.G + gh;
       }
       const int tiles = ta_tiles(p, rq, alone);
       n = n_pre;
       if (tiles > 0) {
-        const int each = ta_units(tiles), qt = ta_quotient(self, p.tpi_magic), in = self - qt * p.tpi;
+        const int each = ta_units(tiles), qt = ta_quotient(self, p.tpi_magic);
         const int item = kvh * ta_items(p, rq) + qt;
         const int b = base.y + item * each + TA_COST, c0 = b / per;
         const int pre_rows = pre_units > 0 ? (p.pre_items + (pre_units + per - 1) / per) * 2 * TA_ROWS : 0;
         n += (b + tiles - 1) / per - c0 + 1;
         own_row = pre_rows + (int64_t)(base.x + item + c0 - pre_units / per) * p.own_rows;
-        own_in = in < p.tpc ? in * p.G + gh : p.own_half + (in - p.tpc) * p.G + gh;
+        own_in = (self - qt * p.tpi) * p.G + gh;
       }
     }
     const int most = (int)__reduce_max_sync(0xffffffffu, n);
@@ -1133,7 +1135,7 @@ extern "C" YSKN_B200_API int yskn_b200_tree_attention(const yskn_b200_tree_atten
   p.how = reinterpret_cast<int4*>(work);
   p.base = reinterpret_cast<int2*>(work + w.base);
   p.ml = reinterpret_cast<float2*>(work + w.ml), p.o = reinterpret_cast<float*>(work + w.o);
-  p.own_half = w.own_half, p.own_rows = w.own_rows, p.own_items = w.own_items;
+  p.own_rows = w.own_rows, p.own_items = w.own_items;
   p.out = reinterpret_cast<uint16_t*>(a.out), p.err = device_error_word();
   // The cache's 64-channel columns are an axis of their own, so that one box holds several columns of its rows in the
   // order of the ring's slots; where a slot takes several boxes (blocks shorter than it), a box is one column.
