@@ -30,10 +30,11 @@
 // ring holds does not cover the memory's latency; the tensor cores need 1.1); results, 1 KB a row and segment both
 // ways, where they have few (a segment of one tile and 252 rows 4.9 us, without its stores 2.8); set-up, 8 us.
 // Everything is summed in a fixed order: the same call gives the same bits.
-// us a call, and with a mask on prefix_attention's kernel instead: one request of 60 nodes and 2000 rows 24.6, 29.7; of
-// 32 nodes and 8000 rows 24.0, 43.7; 8 of 60 nodes and up to 8000 rows 60, 100; 64 of 16 nodes and up to 1000 rows 69,
-// 119; 32 of 32 nodes behind 4096 rows with up to 4096 of their own 156, 151. (One CTA with 128 rows instead of the
-// pair: 25, 37, 72, 67 and 180: its ring holds 1.25 tiles instead of 2.5.)
+// us a call, and with a mask on prefix_attention's kernel instead: one request of 60 nodes and 2000 rows 20.4, 29.7; of
+// 32 nodes and 8000 rows 23.0, 43.7; 8 of 60 nodes and up to 8000 rows 60, 100; 64 of 16 nodes and up to 1000 rows 67,
+// 119; 32 of 32 nodes behind 4096 rows with up to 4096 of their own 152, 151. (One CTA with 128 rows instead of the
+// pair, whose ring holds 1.25 tiles instead of 2.5: 25, 37, 72, 67 and 180, where the pair then took 25, 24, 60, 69 and
+// 156, still with the join by one group and an item's rows not halved between the CTAs.)
 // Every mbarrier wait is bounded; after a timeout the softmax warps go through their remaining tiles without waiting,
 // so that the halves' named barriers still match, and both CTAs meet before either leaves.
 #include <algorithm>
@@ -775,21 +776,22 @@ __device__ __forceinline__ float4 ta_four(uint2 v) {
 // every fourth 16-byte unit of the quarter from qd on. The new rows first: a few visible ones of each row at a time,
 // keys and values asked for together, the scores of the quarters added up through shared memory. Then the row's
 // segments. What bounds it is the chain of dependent loads (the token's request, its table, its rows; the segments),
-// and instructions where there are many rows (64 requests of 16 nodes: 25 of 69 us). Where there are few rows, which
-// then have many segments, S = 3 more groups of 4 warps take every third segment beside the group for the new rows,
-// which does not wait for the first kernel (one request of 32 nodes and 8000 rows: all by one group 33 us, so 24).
+// and instructions where there are many rows (64 requests of 16 nodes: 25 of 67 us). Where there are few rows, which
+// then have many segments (SPLIT), four more warps take the segments beside those for the new rows, which do not wait
+// for the first kernel. By one group, by two, by four (a CTA an SM then): one request of 60 nodes and 2000 rows 24, 20,
+// 25 us; of 32 nodes and 8000 rows 33, 23, 22; 16 of 16 nodes and 1500 rows, more rows than the rule's, 27, 30, 30.
 // (A warp for all heads of a token, whose lanes share the keys and values: fewer instructions, but 200 registers, and
 // 64 requests 89 us where this takes 69.)
-constexpr int TJ_RESIDENT = 5;  // CTAs an SM without more groups (4 to 8: within 4 %)
+constexpr int TJ_RESIDENT = 5;  // CTAs an SM of one group (4 to 8: within 4 %)
 
-template <int D, int DT, int S>
-__global__ void __launch_bounds__(128 * (1 + S), S == 0 ? TJ_RESIDENT : 1)
+template <int D, int DT, bool SPLIT>
+__global__ void __launch_bounds__(SPLIT ? 256 : 128, SPLIT ? 2 : TJ_RESIDENT)
     tree_join_kernel(const __grid_constant__ TreeAttnParams p) {
   constexpr int NJ = D / 64;            // 16-byte units (4 channels) of a lane
-  constexpr int ONCE = S == 0 ? 2 : 4;  // new rows, or segments, asked for at once: what registers hold
+  constexpr int ONCE = SPLIT ? 4 : 2;   // new rows, or segments, asked for at once: what registers hold
   __shared__ __align__(16) float s_part[2][4][8][4];  // a warp's part of each score
   __shared__ bool s_sound;
-  __shared__ float s_state[S > 0 ? S : 1][4][2 + 4 * NJ][32];  // what the other groups have
+  __shared__ float s_state[4][2 + 4 * NJ][32];  // what the second group has
   const int lane = threadIdx.x & 31, group = threadIdx.x >> 7, part = threadIdx.x >> 5 & 3;
   const int r = lane & 7, qd = lane >> 3;
   const int idx = blockIdx.x * 8 + r, kvh = blockIdx.y, t = ta_quotient(idx, p.g_magic), gh = idx - t * p.G;
@@ -943,9 +945,9 @@ __global__ void __launch_bounds__(128 * (1 + S), S == 0 ? TJ_RESIDENT : 1)
     }
   }
   bool sound = true;
-  if (S == 0 || group > 0) {
+  if (!SPLIT || group > 0) {
     pdl_begin();  // the first kernel's results
-    // ---- the row's segments (every S-th): n_pre of its prefix item, then those of its own
+    // ---- the row's segments: n_pre of its prefix item, then those of its own
     const int4 how = *p.how;
     const int2 base = valid ? p.base[req] : make_int2(0, 0);
     const int per = how.x, pre_units = max(how.y, 0);
@@ -974,14 +976,13 @@ __global__ void __launch_bounds__(128 * (1 + S), S == 0 ? TJ_RESIDENT : 1)
       }
     }
     const int most = (int)__reduce_max_sync(0xffffffffu, n);
-    constexpr int STEP = S == 0 ? 1 : S;
-    for (int x0 = S == 0 ? 0 : group - 1; x0 < most; x0 += STEP * ONCE) {
+    for (int x0 = 0; x0 < most; x0 += ONCE) {
       float2 ml[ONCE];
       float4 y[ONCE][NJ];
       float now = m;
 #pragma unroll
       for (int u = 0; u < ONCE; ++u) {
-        const int x = x0 + u * STEP;
+        const int x = x0 + u;
         const bool pre = x < n_pre;
         const int rows = pre ? 2 * TA_ROWS : p.own_rows, in = pre ? pre_in : own_in;
         const int64_t row = pre ? pre_row + (int64_t)x * rows : own_row + (int64_t)(x - n_pre) * rows;
@@ -1014,9 +1015,9 @@ __global__ void __launch_bounds__(128 * (1 + S), S == 0 ? TJ_RESIDENT : 1)
         }
       }
     }
-    if constexpr (S > 0) {
+    if constexpr (SPLIT) {
       if (threadIdx.x == 128) s_sound = sound;
-      float(&mine)[2 + 4 * NJ][32] = s_state[group - 1][part];
+      float(&mine)[2 + 4 * NJ][32] = s_state[part];
       mine[0][lane] = m, mine[1][lane] = l;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
@@ -1025,25 +1026,21 @@ __global__ void __launch_bounds__(128 * (1 + S), S == 0 ? TJ_RESIDENT : 1)
       }
     }
   }
-  if constexpr (S > 0) {
+  if constexpr (SPLIT) {
     __syncthreads();
     if (group > 0 || !live) return;
+    const float(&other)[2 + 4 * NJ][32] = s_state[part];
+    const float top = other[0][lane], now = fmaxf(m, top);
+    const float keep = exp2_approx(m - now), w = top == -INFINITY ? 0.0f : exp2_approx(top - now);
+    if (m != -INFINITY) {
+      l *= keep;
+      scale_by(keep);
+    }
+    l = fmaf(other[1][lane], w, l);
 #pragma unroll
-    for (int x = 0; x < S; ++x) {
-      const float(&other)[2 + 4 * NJ][32] = s_state[x][part];
-      const float top = other[0][lane], now = fmaxf(m, top);
-      const float keep = exp2_approx(m - now), w = top == -INFINITY ? 0.0f : exp2_approx(top - now);
-      if (m != -INFINITY) {
-        l *= keep;
-        scale_by(keep);
-      }
-      m = now;
-      l = fmaf(other[1][lane], w, l);
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        o[j][0].x = fmaf(other[2 + 4 * j][lane], w, o[j][0].x), o[j][0].y = fmaf(other[3 + 4 * j][lane], w, o[j][0].y);
-        o[j][1].x = fmaf(other[4 + 4 * j][lane], w, o[j][1].x), o[j][1].y = fmaf(other[5 + 4 * j][lane], w, o[j][1].y);
-      }
+    for (int j = 0; j < NJ; ++j) {
+      o[j][0].x = fmaf(other[2 + 4 * j][lane], w, o[j][0].x), o[j][0].y = fmaf(other[3 + 4 * j][lane], w, o[j][0].y);
+      o[j][1].x = fmaf(other[4 + 4 * j][lane], w, o[j][1].x), o[j][1].y = fmaf(other[5 + 4 * j][lane], w, o[j][1].y);
     }
     sound = s_sound;
   }
@@ -1076,13 +1073,11 @@ static int launch_tree_attention(const CUtensorMap (&maps)[4], const TreeAttnPar
                                  maps[1], maps[2], maps[3], p))
     return cuda_fail(e, "tree_attention_kernel");
   const dim3 grid((unsigned)ceil_div((int64_t)p.tokens * p.G, 8), p.n_kvh);
-  // Groups for the segments: more where the rows alone do not fill the SMs.
-  auto join = [&](auto s) {
-    constexpr int S = decltype(s)::value;
-    return cuda_fail(launch_pdl(tree_join_kernel<D, DT, S>, grid, 128 * (1 + S), 0, st, p), "tree_join_kernel");
+  auto join = [&](auto split) {  // a second group where the rows alone do not fill the SMs
+    constexpr bool SPLIT = decltype(split)::value;
+    return cuda_fail(launch_pdl(tree_join_kernel<D, DT, SPLIT>, grid, SPLIT ? 256 : 128, 0, st, p), "tree_join_kernel");
   };
-  return (int64_t)grid.x * grid.y <= 2 * 148 ? join(std::integral_constant<int, 3>{})
-                                             : join(std::integral_constant<int, 0>{});
+  return (int64_t)grid.x * grid.y <= 2 * 148 ? join(std::true_type{}) : join(std::false_type{});
 }
 
 }  // namespace yskn
