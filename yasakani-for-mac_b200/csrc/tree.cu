@@ -9,7 +9,8 @@
 // What bounds both: latency, a chain as long as the tree is deep (a few KB move). A warp takes a
 // node (tree_plan) or a request (tree_accept). What the chain reads is loaded before it, 64 nodes in
 // two registers a lane, and followed by shuffles; only parents past the 64th node are followed
-// through the cache. A lane holds one word of the node's bits.
+// through the cache. A lane holds one word of the node's bits. Both calls, in a captured chain: a tree of 60 nodes
+// 3.6 us, 256 of up to 64 nodes 6.0.
 #include "common.cuh"
 
 namespace yskn {
