@@ -272,3 +272,16 @@ def test_graphs_and_streams(cuda):
         for a, b in zip(eager, run(kind)):
             assert torch.equal(a, b), kind
     assert np.isfinite(eager[4].cpu().numpy()).all()
+
+
+def test_a_fork_of_a_request_that_is_not_there_ends(cuda):
+    import torch
+    import yskn_b200 as Y
+    st = _started(cuda, [3, 19, 14])
+    st.fork(torch.tensor([1, 3, 2 ** 31 - 1], dtype=torch.int32, device=cuda))
+    torch.cuda.synchronize()
+    assert Y.status() == Y.EINVAL and Y.status() == 0
+    assert st.lens.tolist() == [94, 0, 0] and st.said.tolist() == [20, 0, 0] and st.free.item() == 40 - 5 - 2
+    st.new.copy_(torch.tensor([1, 0, 0], dtype=torch.int32))
+    st.step(3, 1)
+    assert st.lens.tolist() == [95, 0, 0] and st.said.tolist() == [21, 0, 0] and Y.status() == 0

@@ -220,8 +220,8 @@ class BatchStack(S.Stack):
         self.said.copy_((self.said + self.accepted).clamp(max=W))
 
     def fork(self, source, stream=None):
-        """Request i becomes a copy of request source[i] (int32 on the device; itself: it goes on; negative: it ends):
-        cache, text and controls. Of those that continue one request the first goes on in its blocks, the others get
+        """Request i becomes a copy of request source[i] (int32 [batch] on the device; itself: it goes on; negative: it
+        ends): cache, text and controls. Of those that continue one request the first goes on in its blocks, the others get
         copies; one whose copy the pool does not hold keeps the text and has to run it again (its lens is 0)."""
         torch = self.torch
         if stream is not None:
@@ -234,7 +234,8 @@ class BatchStack(S.Stack):
         self.tables.copy_(self.tables_out)
         self.lens.copy_(self.lens_out)
         self.free.copy_(self.free_out)
-        of, live = source.clamp(min=0).long(), (source >= 0)
+        # (a source outside the batch ends the request too, and is an error that the status tells)
+        of, live = source.clamp(0, self.batch - 1).long(), (source >= 0) & (source < self.batch)
         for t in (self.text, self.prompt, self.repetition, self.presence, self.frequency, self.mask):
             t.copy_(t[of])
         self.said.copy_(self.said[of] * live)
