@@ -285,3 +285,32 @@ def test_a_fork_of_a_request_that_is_not_there_ends(cuda):
     st.new.copy_(torch.tensor([1, 0, 0], dtype=torch.int32))
     st.step(3, 1)
     assert st.lens.tolist() == [95, 0, 0] and st.said.tolist() == [21, 0, 0] and Y.status() == 0
+
+
+def test_calls_that_do_not_fit_the_loop(cuda):
+    import yskn_b200 as Y
+    st = _started(cuda, [3, 5])
+    for request in (-1, 2):
+        with pytest.raises(Y.YsknError):
+            st.draft(request, [1], [0])
+    for n in (0, 97):
+        with pytest.raises(Y.YsknError):
+            st.verify(n)
+    with pytest.raises(Y.YsknError):
+        _stack(cuda, batch=1, max_tokens=4, capacity=16, n_blocks=4).verify(1)
+
+
+def test_a_tree_of_more_nodes_than_the_loop_has_is_an_error(cuda):
+    import torch
+    import yskn_b200 as Y
+    st = _stack(cuda, batch=2, max_tokens=64, capacity=64, n_blocks=16, nodes=3)
+    for i in range(2):
+        st.say(i, _prompt(i, 5))
+    st.new.copy_(st.said)
+    st.step(10, 5)
+    st.draft(1, [3, 4], [0, 0])
+    st.new.copy_(torch.tensor([7, 3], dtype=torch.int32))
+    st.verify(10)
+    torch.cuda.synchronize()
+    assert Y.status() == Y.EINVAL and Y.status() == 0
+    assert 1 <= st.said[1].item() - 6 <= 3 and st.lens[1].item() == st.said[1].item() - 1

@@ -174,8 +174,10 @@ class BatchStack(S.Stack):
         """The request's drafted tree: node j + 1 is tokens[j] behind node parents[j] <= j (node 0 is the request's
         next token, said but not run yet). The next verify that gives it 1 + len(tokens) new tokens runs it."""
         n = len(tokens)
-        if n >= self.nodes or len(parents) != n or any(not 0 <= p <= j for j, p in enumerate(parents)):
-            raise Y.YsknError(Y.EINVAL, "draft: %d nodes at most, each behind an earlier one" % max(self.nodes - 1, 0))
+        if (not 0 <= request < self.batch or n >= self.nodes or len(parents) != n or
+                any(not 0 <= p <= j for j, p in enumerate(parents))):
+            raise Y.YsknError(Y.EINVAL, "draft: a request of the batch, and %d nodes at most, each behind an earlier one"
+                              % max(self.nodes - 1, 0))
         dev, t = self.dev, self.torch
         self.draft_tokens[request, 1:n + 1] = t.tensor(tokens, dtype=t.int32, device=dev)
         self.draft_parents[request, 1:n + 1] = t.tensor(parents, dtype=t.int32, device=dev)
@@ -186,6 +188,8 @@ class BatchStack(S.Stack):
         appended; the cache keeps the path's rows. Choices are the largest logits, without penalties and masks (which
         what a node's ancestors say would change), of requests that have run all they said but the last token."""
         torch, T, W = self.torch, n_tokens, self.capacity
+        if not self.nodes or not 0 < T <= self.max_tokens:
+            raise Y.YsknError(Y.EINVAL, "verify: a loop made for trees, and 1..%d tokens" % self.max_tokens)
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.verify(n_tokens)
