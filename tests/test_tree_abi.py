@@ -197,3 +197,7 @@ def test_the_binding_refuses_what_the_c_entry_cannot_see():
         no(Y.token_logprobs, lp, **{k: None})
     no(Y.token_logprobs, lp, logits=f32(50, 2).t())
     no(Y.token_logprobs, lp, logprobs=f32(3, 2).t())
+
+
+def test_batch_edit_writes_lengths_to_an_array_of_their_own():
+    refused("batch_edit", BATCH_EDIT, [dict(keep=2 * P), dict(source=2 * P), dict(keep=2 * P, source=None)])

@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(EDIT_THREADS) batch_edit_kernel(const __grid_c
     int stay = kept, need = 0;
     if (FORK) {
       const unsigned long long heir = s_heir[i];
-      stay = heir ? edit_blocks(p, (int)(heir >> 32) - 1) : 0;
+      stay = heir ? edit_blocks(p, (int)((heir >> 32) - 1)) : 0;
       if (source[k] >= 0 && (unsigned)s_heir[source[k]] != ~(unsigned)i) need = kept;
     }
     wrong |= old > p.prefix_len && (old - p.prefix_len - 1) / p.block_size >= p.table_width;
@@ -220,7 +220,8 @@ extern "C" YSKN_B200_API int yskn_b200_batch_edit(const yskn_b200_batch_edit_arg
   if (fork && (a.max_copies < 1 || a.copies_stride < a.max_copies ||
                (a.batch > 1 && a.tables_out_stride < a.table_width)))
     return fail(YSKN_EINVAL, "batch_edit: an empty list of copies, or a stride below its width");
-  if (a.lens_out == a.lens || a.free_out == a.free || (fork && a.tables_out == a.block_tables))
+  if (a.lens_out == a.lens || a.lens_out == a.keep || a.lens_out == a.source || a.free_out == a.free ||
+      (fork && a.tables_out == a.block_tables))
     return fail(YSKN_EINVAL, "batch_edit: the new lengths, count and tables need arrays of their own");
   EditParams p{a.lens,         a.keep,       a.source,        a.block_tables, a.table_stride, a.tables_out,
                a.tables_out_stride, a.pool,  a.free,          a.lens_out,     a.free_out,     a.copies,
