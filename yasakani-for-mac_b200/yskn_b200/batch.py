@@ -176,7 +176,7 @@ class BatchStack(S.Stack):
         n = len(tokens)
         if (not 0 <= request < self.batch or n >= self.nodes or len(parents) != n or
                 any(not 0 <= p <= j for j, p in enumerate(parents))):
-            raise Y.YsknError(Y.EINVAL, "draft: a request of the batch, and %d nodes at most, each behind an earlier one"
+            raise Y.YsknError(Y.EINVAL, "draft: a request of the batch, %d nodes at most, each behind an earlier one"
                               % max(self.nodes - 1, 0))
         dev, t = self.dev, self.torch
         self.draft_tokens[request, 1:n + 1] = t.tensor(tokens, dtype=t.int32, device=dev)
@@ -225,8 +225,8 @@ class BatchStack(S.Stack):
 
     def fork(self, source, stream=None):
         """Request i becomes a copy of request source[i] (int32 [batch] on the device; itself: it goes on; negative: it
-        ends): cache, text and controls. Of those that continue one request the first goes on in its blocks, the others get
-        copies; one whose copy the pool does not hold keeps the text and has to run it again (its lens is 0)."""
+        ends): cache, text and controls. Of those that continue one request the first goes on in its blocks, the others
+        get copies; one whose copy the pool does not hold keeps the text and has to run it again (its lens is 0)."""
         torch = self.torch
         if stream is not None:
             with torch.cuda.stream(stream):
