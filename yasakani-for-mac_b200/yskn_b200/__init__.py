@@ -699,7 +699,7 @@ def _types():
     import torch
     _DT.update({torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16, torch.int16: DT_BF16})
     _DT["i32"], _DT["i64"] = torch.int32, torch.int64
-    _DT["device"] = torch.cuda.current_device
+    _DT["device"] = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
     # the raw handle at once: building a torch.cuda.Stream object around it takes longer than a launch
     _DT["stream"] = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
         lambda device: torch.cuda.current_stream(device).cuda_stream)
@@ -900,24 +900,28 @@ def logits_adjust(logits, out, history=None, history_lens=None, prompt_lens=None
         0 if mask is None else mask.data_ptr(), ms[0], out.data_ptr(), os_[0], M, V, width, n_bias), out, stream)
 
 
-def _here(tensors):
+def _here(name, tensors):
     """All on the current device, which the call is launched on."""
     at = tensors[0].get_device()
     for t in tensors:
         if t.get_device() != at:
-            return False
-    return at >= 0 and at == _DT["device"]()
+            at = -1
+    if at < 0 or at != _DT["device"]():
+        raise YsknError(EINVAL, name + ": tensors on the current device expected")
 
 
-def _dense(dtype, tensors):
+def _flat(name, dtype, tensors):
+    """The addresses of dense arrays of one type on the current device."""
+    at, out = tensors[0].get_device(), []
     for t in tensors:
         if t.dtype is not dtype or not t.is_contiguous():
-            return False
-    return True
-
-
-def _addresses(tensors):
-    return [t.data_ptr() for t in tensors]
+            raise YsknError(EINVAL, "%s: dense arrays of %s expected" % (name, dtype))
+        if t.get_device() != at:
+            at = -1
+        out.append(t.data_ptr())
+    if at < 0 or at != _DT["device"]():
+        raise YsknError(EINVAL, name + ": tensors on the current device expected")
+    return out
 
 
 def tree_plan(parents, requests, starts, lens, mask, positions, stream=None):
@@ -927,14 +931,11 @@ def tree_plan(parents, requests, starts, lens, mask, positions, stream=None):
     if not _DT:
         _types()
     i32, T, B, (rows, words), row = _DT["i32"], parents.numel(), lens.numel(), mask.shape, mask.stride()
-    flat = (parents, requests, starts, lens, positions)
-    _need(_dense(i32, flat) and mask.dtype is i32 and rows == T and row[1] == 1 and requests.numel() == T and
-          positions.numel() == T and starts.numel() == B + 1,
-          "tree_plan: int32 arrays of one batch and a mask row for each token expected")
-    _need(_here(flat + (mask,)), "tree_plan: tensors on the current device expected")
-    a = _addresses(flat)
-    _launch("tree_plan", ARGS["tree_plan"].pack(a[0], a[1], a[2], a[3], mask.data_ptr(), row[0], a[4], T, B, words),
-            parents, stream)
+    if not (mask.dtype is i32 and mask.get_device() == parents.get_device() and rows == T and row[1] == 1 and
+            requests.numel() == T and positions.numel() == T and starts.numel() == B + 1):
+        raise YsknError(EINVAL, "tree_plan: int32 arrays of one batch and a mask row for each token expected")
+    a, b, c, d, e = _flat("tree_plan", i32, (parents, requests, starts, lens, positions))
+    _launch("tree_plan", ARGS["tree_plan"].pack(a, b, c, d, mask.data_ptr(), row[0], e, T, B, words), parents, stream)
 
 
 def tree_attention(q, k_cache, v_cache, block_tables, lens, starts, max_new, mask, work, out, prefix_blocks=None,
@@ -951,7 +952,7 @@ def tree_attention(q, k_cache, v_cache, block_tables, lens, starts, max_new, mas
         used.append(prefix_blocks)
     if gate is not None:
         used.append(gate)
-    _need(_here(used), "tree_attention: tensors on the current device expected")
+    _here("tree_attention", used)
     _launch("tree_attention", ARGS["tree_attention"].pack(*args, mask.data_ptr(), row[0], words), out, stream)
 
 
@@ -962,14 +963,14 @@ def tree_accept(tokens, parents, choice, starts, lens, path, accepted, lens_out,
     if not _DT:
         _types()
     i32, T, B, (rows, width), row = _DT["i32"], tokens.numel(), lens.numel(), path.shape, path.stride()
-    flat = (tokens, parents, choice, starts, lens, accepted, lens_out, next_token)
-    _need(_dense(i32, flat) and path.dtype is i32 and rows == B and row[1] == 1 and parents.numel() == T and
-          choice.numel() == T and starts.numel() == B + 1 and accepted.numel() == B and lens_out.numel() == B and
-          next_token.numel() == B, "tree_accept: int32 arrays of one batch and a path row for each request expected")
-    _need(_here(flat + (path,)), "tree_accept: tensors on the current device expected")
-    a = _addresses(flat)
-    _launch("tree_accept", ARGS["tree_accept"].pack(a[0], a[1], a[2], a[3], a[4], path.data_ptr(), row[0], a[5], a[6],
-                                                    a[7], B, T, width), tokens, stream)
+    if not (path.dtype is i32 and path.get_device() == tokens.get_device() and rows == B and row[1] == 1 and
+            parents.numel() == T and choice.numel() == T and starts.numel() == B + 1 and accepted.numel() == B and
+            lens_out.numel() == B and next_token.numel() == B):
+        raise YsknError(EINVAL, "tree_accept: int32 arrays of one batch and a path row for each request expected")
+    a, b, c, d, e, f, g, h = _flat("tree_accept", i32, (tokens, parents, choice, starts, lens, accepted, lens_out,
+                                                        next_token))
+    _launch("tree_accept", ARGS["tree_accept"].pack(a, b, c, d, e, path.data_ptr(), row[0], f, g, h, B, T, width),
+            tokens, stream)
 
 
 def batch_edit(lens, keep, block_tables, pool, free_count, block_size, lens_out, free_out, source=None, tables_out=None,
@@ -981,27 +982,27 @@ def batch_edit(lens, keep, block_tables, pool, free_count, block_size, lens_out,
     if not _DT:
         _types()
     i32, (B, width), row = _DT["i32"], block_tables.shape, block_tables.stride()
-    flat = (lens, keep, pool, free_count, lens_out, free_out)
-    _need(_dense(i32, flat) and block_tables.dtype is i32 and row[1] == 1 and lens.numel() == B and
-          keep.numel() == B and lens_out.numel() == B and free_count.numel() and free_out.numel(),
-          "batch_edit: dense int32 arrays of the batch expected")
-    _need(_here(flat + (block_tables,)), "batch_edit: tensors on the current device expected")
-    ts = cs = (0, 1)
-    n, f = 0, (0, 0, 0, 0)
-    if source is not None:
-        fork = (source, n_copies, tables_out, copies)
-        _need(tables_out is not None and copies is not None and n_copies is not None,
-              "batch_edit: a source needs new tables, a list of copies and its count")
-        ts, cs, (three, n) = tables_out.stride(), copies.stride(), copies.shape
-        _need(_dense(i32, fork[:2]) and source.numel() == B and n_copies.numel() and tables_out.dtype is i32 and
-              tables_out.shape == (B, width) and ts[1] == 1 and copies.dtype is i32 and three == 3 and cs[1] == 1,
-              "batch_edit: int32 source, tables of one shape and copies [3][n] expected")
-        _need(_here(fork), "batch_edit: tensors on the current device expected")
-        f = _addresses(fork)
-    a = _addresses(flat)
+    if not (block_tables.dtype is i32 and block_tables.get_device() == lens.get_device() and row[1] == 1 and
+            lens.numel() == B and keep.numel() == B and lens_out.numel() == B and free_count.numel() and
+            free_out.numel()):
+        raise YsknError(EINVAL, "batch_edit: dense int32 arrays of the batch expected")
+    a, b, c, d, e, f = _flat("batch_edit", i32, (lens, keep, pool, free_count, lens_out, free_out))
+    if source is None:
+        _launch("batch_edit", ARGS["batch_edit"].pack(a, b, 0, block_tables.data_ptr(), row[0], 0, 0, c, d, e, f, 0, 0,
+                                                      0, B, block_size, prefix_len, width, pool.numel(), 0),
+                lens, stream)
+        return
+    _need(tables_out is not None and copies is not None and n_copies is not None,
+          "batch_edit: a source needs new tables, a list of copies and its count")
+    ts, cs, (three, n) = tables_out.stride(), copies.stride(), copies.shape
+    if not (tables_out.dtype is i32 and tables_out.shape == block_tables.shape and ts[1] == 1 and
+            copies.dtype is i32 and three == 3 and cs[1] == 1 and source.numel() == B and n_copies.numel() and
+            tables_out.get_device() == copies.get_device() == lens.get_device()):
+        raise YsknError(EINVAL, "batch_edit: int32 source, tables of one shape and copies [3][n] expected")
+    g, h = _flat("batch_edit", i32, (source, n_copies))
     _launch("batch_edit", ARGS["batch_edit"].pack(
-        a[0], a[1], f[0], block_tables.data_ptr(), row[0], f[2], ts[0], a[2], a[3], a[4], a[5], f[3], cs[0], f[1], B,
-        block_size, prefix_len, width, pool.numel(), n), lens, stream)
+        a, b, g, block_tables.data_ptr(), row[0], tables_out.data_ptr(), ts[0], c, d, e, f, copies.data_ptr(), cs[0],
+        h, B, block_size, prefix_len, width, pool.numel(), n), lens, stream)
 
 
 class CacheSet:
@@ -1032,8 +1033,7 @@ def cache_copy(caches, copies, count=None, stream=None):
     _need(copies.dtype is i32 and three == 3 and row[1] == 1 and
           (count is None or (count.dtype is i32 and count.numel())),
           "cache_copy: int32 copies [3][n] and a count expected")
-    _need(_here((copies, caches.caches[0]) if count is None else (copies, caches.caches[0], count)),
-          "cache_copy: tensors on the current device expected")
+    _here("cache_copy", (copies, caches.caches[0]) if count is None else (copies, caches.caches[0], count))
     _launch("cache_copy", ARGS["cache_copy"].pack(
         *caches._head, copies.data_ptr(), row[0], 0 if count is None else count.data_ptr(), *caches._sizes, n), copies,
         stream)
@@ -1046,14 +1046,14 @@ def cache_compact(caches, block_tables, lens, starts, path, prefix_len=0, stream
         _types()
     i32, (B, width), (rows, nodes) = _DT["i32"], block_tables.shape, path.shape
     ts, ps = block_tables.stride(), path.stride()
-    _need(block_tables.dtype is i32 and ts[1] == 1 and _dense(i32, (lens, starts)) and lens.numel() == B and
-          starts.numel() == B + 1 and path.dtype is i32 and rows == B and ps[1] == 1,
+    _need(block_tables.dtype is i32 and ts[1] == 1 and lens.numel() == B and starts.numel() == B + 1 and
+          path.dtype is i32 and rows == B and ps[1] == 1,
           "cache_compact: int32 tables, lengths, starts and paths of one batch expected")
-    _need(_here((lens, starts, block_tables, path, caches.caches[0])),
-          "cache_compact: tensors on the current device expected")
+    _here("cache_compact", (block_tables, path, caches.caches[0]))
+    a, b = _flat("cache_compact", i32, (lens, starts))
     _launch("cache_compact", ARGS["cache_compact"].pack(
-        *caches._head, block_tables.data_ptr(), ts[0], lens.data_ptr(), starts.data_ptr(), path.data_ptr(), ps[0],
-        *caches._sizes, B, width, prefix_len, nodes), lens, stream)
+        *caches._head, block_tables.data_ptr(), ts[0], a, b, path.data_ptr(), ps[0], *caches._sizes, B, width,
+        prefix_len, nodes), lens, stream)
 
 
 def token_logprobs(logits, tokens=None, logprobs=None, entropy=None, top_logprobs=None, top_ids=None, stream=None):
@@ -1090,6 +1090,6 @@ def token_logprobs(logits, tokens=None, logprobs=None, entropy=None, top_logprob
               "token_logprobs: dense int32 numbers and f32 log probabilities [M][k] expected")
         used += (top_logprobs, top_ids)
         c, d = top_logprobs.data_ptr(), top_ids.data_ptr()
-    _need(_here(used), "token_logprobs: tensors on the current device expected")
+    _here("token_logprobs", used)
     _launch("token_logprobs", ARGS["token_logprobs"].pack(logits.data_ptr(), row[0], a, stride, b, e, c, d, M, V, n, k),
             logits, stream)
