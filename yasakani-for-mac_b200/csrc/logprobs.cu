@@ -135,15 +135,11 @@ __device__ __forceinline__ uint32_t lp_remote(const void* p, int rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
   return a;
 }
-__device__ __forceinline__ uint64_t lp_remote_u64(uint32_t a) {
-  uint64_t v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
-  return v;
+__device__ __forceinline__ void lp_put_u64(uint32_t a, uint64_t v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
-__device__ __forceinline__ float lp_remote_f32(uint32_t a) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
+__device__ __forceinline__ void lp_put_f32(uint32_t a, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
 }
 
 constexpr int LP_BUFFER = 160;  // keys: up to 31 that are left, and 128 that may join them
@@ -178,7 +174,13 @@ struct LpShared {
   alignas(16) uint64_t keys[LP_WARPS * 64 + 1];  // to be ranked
   uint64_t list[YSKN_MAX_TOP];   // this CTA's largest
   LpState state[LP_WARPS];
-  LpState part;  // this CTA's
+  // in the cluster's first CTA: what the others have put there, and the row's largest
+  LpState parts[LP_MAX_CLUSTER];
+  uint64_t lists[LP_MAX_CLUSTER * YSKN_MAX_TOP];
+  uint64_t row_list[YSKN_MAX_TOP];
+  // the first tokens and their logits, asked for ahead of the row
+  int id[LP_THREADS];
+  float logit[LP_THREADS];
 };
 
 // The largest n_top of n different keys in shared memory (a 0 behind them), in order, into `list`, which holds zeros;
@@ -232,6 +234,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT)
     token_logprobs_kernel(const __grid_constant__ LogprobsParams p) {
   __shared__ LpShared sh;
   pdl_begin();
+  if (p.cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA has begun
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / p.cluster, rank = blockIdx.x - row * p.cluster;
   const float* x = p.logits + row * p.logits_stride;
@@ -263,6 +266,14 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT)
     }
   };
   load(w0);
+  if (rank == 0 && tid < p.n_tokens) {  // behind the row, their two loads would be its last 1.2 us
+    const int id = p.tokens[row * p.token_stride + tid];
+    sh.id[tid] = id;
+    if ((unsigned)id < (unsigned)p.vocab)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(sh.logit + tid)),
+                   "l"(__cvta_generic_to_global(x + id))
+                   : "memory");
+  }
   for (int g = w0;; g += LP_SLICE) {  // once at least, since the warps meet in it
     float2 v[LP_LOADS][2];
 #pragma unroll
@@ -383,43 +394,37 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT)
     if (lane < listed) sh.keys[at + lane] = top.list;
     if (lane < top.held) sh.keys[at + listed + lane] = buffer[lane];
     if (tid == 0) sh.keys[n] = 0;
-    if (tid < YSKN_MAX_TOP) sh.list[tid] = 0;
+    if (tid < YSKN_MAX_TOP) sh.list[tid] = sh.row_list[tid] = 0;
     __syncthreads();
     lp_rank(sh.keys, n, sh.list, p.n_top, tid);
   }
   LpState t = lp_whole(sh.state, LP_WARPS, lane);
   if (p.cluster > 1) {
-    if (tid == 0) sh.part = t;
+    if (TOP) __syncthreads();  // the list is whole
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the first CTA has begun
+    if (tid == 0) {
+      const uint32_t to = lp_remote(sh.parts + rank, 0);
+      lp_put_f32(to, t.m), lp_put_f32(to + 4, t.rest), lp_put_f32(to + 8, t.e);
+    }
+    if (TOP && tid < p.n_top) lp_put_u64(lp_remote(sh.lists + rank * p.n_top + tid, 0), sh.list[tid]);
     lp_cluster_sync();
-    if (rank == 0) {
-      if (warp < p.cluster) {
-        const uint32_t from = lp_remote(&sh.part, warp);
-        if (lane == 0)
-          sh.state[warp] = LpState{lp_remote_f32(from), lp_remote_f32(from + 4), lp_remote_f32(from + 8)};
-        if (TOP && lane < p.n_top) sh.keys[warp * p.n_top + lane] = lp_remote_u64(lp_remote(&sh.list[lane], warp));
-      }
-    }
-    lp_cluster_sync();  // the others' memory has been read
     if (rank != 0) return;
-    if (TOP) {
-      if (tid < YSKN_MAX_TOP) sh.list[tid] = 0;
-      __syncthreads();
-      lp_rank_lists(sh.keys, p.cluster, p.n_top, sh.list, p.n_top, tid);
-    }
-    t = lp_whole(sh.state, p.cluster, lane);
+    if (TOP) lp_rank_lists(sh.lists, p.cluster, p.n_top, sh.row_list, p.n_top, tid);
+    t = lp_whole(sh.parts, p.cluster, lane);
   }
   if (TOP) __syncthreads();
   const bool none = t.m == -INFINITY && t.rest == 0.0f, bad = !(t.m < INFINITY) || !(t.rest < INFINITY);
   const float log_sum = log1pf(t.rest), nan = __int_as_float(0x7fc00000);
+  asm volatile("cp.async.wait_all;" ::: "memory");  // each thread its own
   for (int j = tid; j < p.n_tokens; j += LP_THREADS) {
-    const int id = p.tokens[row * p.token_stride + j];
+    const int id = j < LP_THREADS ? sh.id[j] : p.tokens[row * p.token_stride + j];
     float y = -INFINITY;
-    if ((unsigned)id < (unsigned)p.vocab && !none) y = (x[id] - t.m) - log_sum;
+    if ((unsigned)id < (unsigned)p.vocab && !none) y = ((j < LP_THREADS ? sh.logit[j] : x[id]) - t.m) - log_sum;
     p.logprobs[(int64_t)row * p.n_tokens + j] = bad ? nan : y;
   }
   if (tid == 0 && p.entropy) p.entropy[row] = bad ? nan : none ? 0.0f : log_sum - t.e / (1.0f + t.rest);
   if (TOP && tid < p.n_top) {
-    const uint64_t key = sh.list[tid];
+    const uint64_t key = p.cluster > 1 ? sh.row_list[tid] : sh.list[tid];
     const int64_t at = (int64_t)row * p.n_top + tid;
     const bool any = key != 0 && !bad;
     p.top_logprobs[at] = bad ? nan : any ? (lp_value((uint32_t)(key >> 32)) - t.m) - log_sum : -INFINITY;
