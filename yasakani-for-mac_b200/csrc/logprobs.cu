@@ -254,6 +254,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT)
   const uint64_t lowest = (uint64_t)lp_ordered(-INFINITY) << 32 | 0xffffffffu;  // only logits above -inf pass
   LpTop top{0, lowest, 0};
   uint32_t so_far = 0;  // the lane's largest
+  bool raise = true;    // the bound may be lower than it could
   uint64_t* buffer = sh.buffer[warp];
   if (TOP && lane == 0) sh.held[warp] = 0;
   const float4 nothing = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
@@ -281,13 +282,13 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT)
       v[u][0] = make_float2(next[u].x, next[u].y);
       v[u][1] = make_float2(next[u].z, next[u].w);
     }
-    uint32_t first_id = head + 4 * (g + lane);
+    uint32_t first_id = head + 4 * (g + lane), in_group = 4;
     const bool more = g + LP_SLICE < w1;
     load(g + LP_SLICE);  // nothing, past the end
     if (g >= w1 && edges) {
       const int at = lane < 3 ? lane : p.vocab - tail + lane - 3;
       if (lane < 3 ? lane < head : lane - 3 < tail) v[0][0].x = x[at];
-      first_id = at;
+      first_id = at, in_group = 1;
       edges = false;
     }
     float most4[LP_LOADS], mine = -INFINITY;
@@ -298,33 +299,37 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT)
     }
     if constexpr (TOP) {
       so_far = max(so_far, mine == mine ? lp_ordered(mine) : 0u);  // (a NaN is no one's bound)
-      auto raise_bound = [&](bool first_time) {
+      if (raise) {
         uint32_t o = so_far, mth = 0;
         for (int i = 0; i < p.n_top; i += LP_WARPS) {  // the largest goes, one lane of it
           mth = __reduce_max_sync(0xffffffffu, o);
           if (lane == __ffs(__ballot_sync(0xffffffffu, o == mth)) - 1) o = 0;
         }
         if (lane == 0) *reinterpret_cast<volatile uint32_t*>(sh.bound + warp) = mth;
-        if (first_time) __syncthreads();  // later an older number of another warp serves as well
+        if (g == w0) __syncthreads();  // later an older number of another warp serves as well
         const uint32_t all = lane < LP_WARPS ? *reinterpret_cast<volatile uint32_t*>(sh.bound + lane) : 0xffffffffu;
         const uint64_t least = ((uint64_t)__reduce_min_sync(0xffffffffu, all) << 32) - 1;
         top.bound = least + 1 > top.bound ? least : top.bound;
-      };
-      if (g == w0) raise_bound(true);
+      }
       // What passes (keys from bound + 1 on) is above `edge`, or equal to it and of a number up to edge_id.
       float edge = lp_value((uint32_t)((top.bound + 1) >> 32));
-      if (__any_sync(0xffffffffu, mine >= edge)) {
-        uint32_t edge_id = ~(uint32_t)(top.bound + 1);
+      raise = __any_sync(0xffffffffu, mine >= edge);  // for the next slice: this one's may change it
+      if (raise) {
+        uint32_t edge_id = ~(uint32_t)(top.bound + 1), hits = 0;  // this lane's groups that pass
 #pragma unroll
-        for (int u = 0; u < LP_LOADS; ++u) {
-          if (!__any_sync(0xffffffffu, most4[u] >= edge)) continue;
-          if (most4[u] >= edge) {  // one or two lanes, mostly: each takes places by itself
+        for (int u = 0; u < LP_LOADS; ++u) hits |= most4[u] >= edge ? 1u << u : 0u;
+        do {  // once, mostly, for one or two lanes: each takes places by itself
+          if (hits) {
+            // (read again: a loop over registers would have to be unrolled, and its code fetched)
+            const uint32_t id = first_id + (__ffs(hits) - 1) * 128;
+            hits &= hits - 1;
+            float y[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const float y = c == 0 ? v[u][0].x : c == 1 ? v[u][0].y : c == 2 ? v[u][1].x : v[u][1].y;
-              const uint32_t id = first_id + u * 128 + c;
-              if (y > edge || (y == edge && id <= edge_id)) buffer[atomicAdd(sh.held + warp, 1)] = lp_key(y, id);
-            }
+            for (int c = 0; c < 4; ++c) y[c] = c < in_group ? x[id + c] : -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (y[c] > edge || (y[c] == edge && id + c <= edge_id))
+                buffer[atomicAdd(sh.held + warp, 1)] = lp_key(y[c], id + c);
           }
           __syncwarp();
           top.held = *reinterpret_cast<volatile int*>(sh.held + warp);
@@ -335,8 +340,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT)
             edge = lp_value((uint32_t)((top.bound + 1) >> 32));
             edge_id = ~(uint32_t)(top.bound + 1);
           }
-        }
-        raise_bound(false);
+        } while (__any_sync(0xffffffffu, hits != 0));
       }
     }
     const uint32_t most = __reduce_max_sync(0xffffffffu, lp_ordered(mine));
