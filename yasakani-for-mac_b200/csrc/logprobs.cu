@@ -23,8 +23,11 @@
 // come late fill a buffer: then 32 keys are sorted (bitonic, in registers) and merged into a list of the warp's 32
 // largest, whose n_top-th is a bound too. (All keys through such lists: 93 us for 512 rows, and the chain of shuffles
 // made one row wait 13.)
-// Measured on the device: one row of 151936 with 20 largest 10.9 us (without them 5.6), 33 rows of 50257 9.2, 256 rows
-// of 151936 with 8 largest 33 (4.7 TB/s), 512 rows 62 (5.0 TB/s; two CTAs of 512 on every SM and a half).
+// The passing logits are read again, from the cache, by a rolled loop: 32 copies of its code for the slice's registers
+// took 62 us for 512 rows instead of 59.8, and one row, where each CTA runs the code once and waits for it, 10.6.
+// Measured on the device: one row of 151936 with 20 largest 9.0 us (without them 4.9), 33 rows of 50257 7.8, 256 rows
+// of 151936 with 8 largest 31.8 (4.9 TB/s), 512 rows 59.8 (5.2 TB/s, without the largest 52.5; two CTAs of 512 on every
+// SM and a half).
 #include <algorithm>
 
 #include "common.cuh"
@@ -454,8 +457,8 @@ extern "C" YSKN_B200_API int yskn_b200_token_logprobs(const yskn_b200_token_logp
   LogprobsParams p{a.logits, a.logits_stride, a.tokens, a.token_stride, a.logprobs, a.entropy, a.top_logprobs,
                    a.top_ids, a.vocab, a.n_tokens, a.n_top, 1};
   // CTAs of a row: as many as the SMs hold at once, with a slice for every warp of each. us at 151936 logits, 8
-  // largest, with 1, 2, 4, 8: 64 rows 31, 23, 19, 29; 128 rows 25, 22, 29, 43; 256 rows 33, 43, 56, 82; one row with 20 largest
-  // 25, 20, 14, 11; 33 rows of 50257 with 1, 2, 4, 8: 13.6, 11.4, 9.2, 11.4.
+  // largest, with 1, 2, 4, 8: 64 rows (20 largest) 24.6, 18.6, 15.9, 25; 128 rows 21.7, 20.4, 25, 37; 256 rows 31.9,
+  // 40, 49, 71; one row with 20 largest 22, 16.6, 11.5, 9.0; 33 rows of 50257 with 1, 2, 4, 8: 11.8, 9.6, 7.8, 10.2.
   while (p.cluster < LP_MAX_CLUSTER && (int64_t)a.rows * p.cluster * 2 <= 148 * LP_RESIDENT &&
          a.vocab / (p.cluster * 2) >= LP_LEAST_PART)
     p.cluster *= 2;
