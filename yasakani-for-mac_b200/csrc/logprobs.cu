@@ -11,10 +11,10 @@
 // What bounds it: one read of the logits (4 bytes each); for few rows, the chain of latencies. A
 // cluster of 1 to 8 CTAs takes a row, one part each; the parts are joined through distributed shared
 // memory, so that there is one launch, no workspace and no counter that a second call could meet.
-// A warp streams its own run of the part in slices of 4096 bytes, 8 16-byte loads a lane for the next slice under way
+// A warp streams its own run of the part in slices, 8 or 10 16-byte loads a lane for the next slice under way
 // while it works on one: its maximum and its sums. (512 rows of 151936, without the largest tokens: 67 us with three
-// CTAs an SM that load and work in turn, 53 with two that load ahead; two halves of the slice, four CTAs, 50, but with
-// the largest tokens 70 against 62, and 37 against 25 where a CTA is alone.)
+// CTAs an SM that load and work in turn, 52.5 with two that load 8 ahead; half the slice, four CTAs, 49.9, but with
+// the largest tokens 74 against 60, and 12.2 against 9.0 for one row.)
 // A logit is a key: its bits in an order of unsigned numbers, above the complement of its number, so that keys are all
 // different and equal logits go by the lowest number. With m = ceil(n_top / 8), the least of the 8 warps' m-th largest
 // lane maxima so far bounds the keys that can be among the n_top largest: at least n_top logits reach it, and few more
@@ -25,18 +25,19 @@
 // made one row wait 13.)
 // The passing logits are read again, from the cache, by a rolled loop: 32 copies of its code for the slice's registers
 // took 62 us for 512 rows instead of 59.8, and one row, where each CTA runs the code once and waits for it, 10.6.
-// Measured on the device: one row of 151936 with 20 largest 9.0 us (without them 4.9), 33 rows of 50257 7.8, 256 rows
-// of 151936 with 8 largest 31.8 (4.9 TB/s), 512 rows 59.8 (5.2 TB/s, without the largest 52.5; two CTAs of 512 on every
+// Measured on the device: one row of 151936 with 20 largest 8.2 us (without them 4.7), 33 rows of 50257 7.8, 256 rows
+// of 151936 with 8 largest 30.8 (5.1 TB/s), 512 rows 57.9 (5.4 TB/s, without the largest 50.4; two CTAs of 512 on every
 // SM and a half).
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
 namespace yskn {
 
 constexpr int LP_WARPS = 8, LP_THREADS = LP_WARPS * 32;
-constexpr int LP_LOADS = 8;              // 16-byte loads of a lane in a slice
-constexpr int LP_SLICE = LP_LOADS * 32;  // 16-byte groups of a warp's slice
+// 16-byte loads of a lane in a slice, one of the two: a slice is 32 times as many 16-byte groups.
+constexpr int LP_FEW = 8, LP_MANY = 10;
 constexpr int LP_RESIDENT = 2;           // CTAs of an SM
 constexpr int LP_MAX_CLUSTER = 8;
 constexpr int LP_LEAST_PART = 7500;      // logits of a CTA where a row has several, at least
@@ -232,9 +233,10 @@ __device__ __forceinline__ LpState lp_whole(const LpState* state, int n, int lan
   return t;
 }
 
-template <bool TOP>
+template <bool TOP, int LOADS>
 __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT)
     token_logprobs_kernel(const __grid_constant__ LogprobsParams p) {
+  constexpr int SLICE = LOADS * 32;
   __shared__ LpShared sh;
   pdl_begin();
   if (p.cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA has begun
@@ -261,10 +263,10 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT)
   uint64_t* buffer = sh.buffer[warp];
   if (TOP && lane == 0) sh.held[warp] = 0;
   const float4 nothing = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-  float4 next[LP_LOADS];  // on their way while a slice is worked on
+  float4 next[LOADS];  // on their way while a slice is worked on
   auto load = [&](int g) {
 #pragma unroll
-    for (int u = 0; u < LP_LOADS; ++u) {
+    for (int u = 0; u < LOADS; ++u) {
       const int at = g + u * 32 + lane;
       next[u] = at < w1 ? __ldcs(groups + at) : nothing;
     }
@@ -278,25 +280,25 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT)
                    "l"(__cvta_generic_to_global(x + id))
                    : "memory");
   }
-  for (int g = w0;; g += LP_SLICE) {  // once at least, since the warps meet in it
-    float2 v[LP_LOADS][2];
+  for (int g = w0;; g += SLICE) {  // once at least, since the warps meet in it
+    float2 v[LOADS][2];
 #pragma unroll
-    for (int u = 0; u < LP_LOADS; ++u) {
+    for (int u = 0; u < LOADS; ++u) {
       v[u][0] = make_float2(next[u].x, next[u].y);
       v[u][1] = make_float2(next[u].z, next[u].w);
     }
     uint32_t first_id = head + 4 * (g + lane), in_group = 4;
-    const bool more = g + LP_SLICE < w1;
-    load(g + LP_SLICE);  // nothing, past the end
+    const bool more = g + SLICE < w1;
+    load(g + SLICE);  // nothing, past the end
     if (g >= w1 && edges) {
       const int at = lane < 3 ? lane : p.vocab - tail + lane - 3;
       if (lane < 3 ? lane < head : lane - 3 < tail) v[0][0].x = x[at];
       first_id = at, in_group = 1;
       edges = false;
     }
-    float most4[LP_LOADS], mine = -INFINITY;
+    float most4[LOADS], mine = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < LP_LOADS; ++u) {
+    for (int u = 0; u < LOADS; ++u) {
       most4[u] = fmaxf(fmaxf(v[u][0].x, v[u][0].y), fmaxf(v[u][1].x, v[u][1].y));
       mine = fmaxf(mine, most4[u]);
     }
@@ -320,7 +322,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT)
       if (raise) {
         uint32_t edge_id = ~(uint32_t)(top.bound + 1), hits = 0;  // this lane's groups that pass
 #pragma unroll
-        for (int u = 0; u < LP_LOADS; ++u) hits |= most4[u] >= edge ? 1u << u : 0u;
+        for (int u = 0; u < LOADS; ++u) hits |= most4[u] >= edge ? 1u << u : 0u;
         do {  // once, mostly, for one or two lanes: each takes places by itself
           if (hits) {
             // (read again: a loop over registers would have to be unrolled, and its code fetched)
@@ -364,13 +366,13 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT)
         out = out && !it;
       };
 #pragma unroll
-      for (int u = 0; u < LP_LOADS; ++u) leave(v[u][0].x), leave(v[u][0].y), leave(v[u][1].x), leave(v[u][1].y);
+      for (int u = 0; u < LOADS; ++u) leave(v[u][0].x), leave(v[u][0].y), leave(v[u][1].x), leave(v[u][1].y);
     }
     const float base = now == -INFINITY ? 0.0f : -now;
     const float2 base2 = make_float2(base, base), log2e = make_float2(LP_LOG2E, LP_LOG2E);
     float2 rest = make_float2(s.rest, 0.0f), e = make_float2(s.e, 0.0f);
 #pragma unroll
-    for (int u = 0; u < LP_LOADS; ++u)
+    for (int u = 0; u < LOADS; ++u)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const float2 d = lp_add2(v[u][c], base2), z = lp_mul2(d, log2e);
@@ -462,6 +464,11 @@ extern "C" YSKN_B200_API int yskn_b200_token_logprobs(const yskn_b200_token_logp
   while (p.cluster < LP_MAX_CLUSTER && (int64_t)a.rows * p.cluster * 2 <= 148 * LP_RESIDENT &&
          a.vocab / (p.cluster * 2) >= LP_LEAST_PART)
     p.cluster *= 2;
+  // The slice whose last one of a warp's run is emptiest by fewest groups, the larger of two alike. us with 8, 10 loads
+  // where 10 leave no more empty: one row of 151936 with 20 largest 9.0, 8.2, 256 rows 31.8, 30.9, 512 rows 60.0, 57.9;
+  // where 8 leave less: 33 rows of 50257 7.8, 8.4, 512 rows of 32000 19.6, 20.9, of 2000 9.4, 10.0. (11 and more spill.)
+  const int run = (int)ceil_div(ceil_div(a.vocab / 4, p.cluster), LP_WARPS);
+  const bool many = ceil_div(run, LP_MANY * 32) * LP_MANY <= ceil_div(run, LP_FEW * 32) * LP_FEW;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = (unsigned)(a.rows * p.cluster);
   cfg.blockDim = LP_THREADS;
@@ -473,7 +480,11 @@ extern "C" YSKN_B200_API int yskn_b200_token_logprobs(const yskn_b200_token_logp
   attr[1].val.clusterDim.x = (unsigned)p.cluster, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cuda_fail(a.n_top > 0 ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<true>, p)
-                               : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<false>, p),
-                   "token_logprobs_kernel");
+  auto launch = [&](auto loads) {
+    constexpr int LOADS = decltype(loads)::value;
+    return cuda_fail(a.n_top > 0 ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<true, LOADS>, p)
+                                 : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<false, LOADS>, p),
+                     "token_logprobs_kernel");
+  };
+  return many ? launch(std::integral_constant<int, LP_MANY>{}) : launch(std::integral_constant<int, LP_FEW>{});
 }
