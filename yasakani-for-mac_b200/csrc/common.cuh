@@ -55,9 +55,10 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
-// Opts a kernel into more than 48 KB of dynamic shared memory, once per device (the attribute
-// belongs to the device's context). One static object per kernel.
+// Opts a kernel into more than 48 KB of dynamic shared memory (or sets another attribute of it), once
+// per device (the attribute belongs to the device's context). One static object per kernel.
 struct SmemOptIn {
+  cudaFuncAttribute attribute = cudaFuncAttributeMaxDynamicSharedMemorySize;
   std::atomic<uint64_t> done{0};
   template <typename K>
   cudaError_t operator()(K* kernel, int bytes) {
@@ -65,7 +66,7 @@ struct SmemOptIn {
     if (cudaError_t e = cudaGetDevice(&dev)) return e;
     const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
     if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, attribute, bytes);
     if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
     return e;
   }

@@ -782,6 +782,10 @@ __device__ __forceinline__ float4 ta_four(uint2 v) {
 // 25 us; of 32 nodes and 8000 rows 33, 23, 22; 16 of 16 nodes and 1500 rows, more rows than the rule's, 27, 30, 30.
 // (A warp for all heads of a token, whose lanes share the keys and values: fewer instructions, but 200 registers, and
 // 64 requests 89 us where this takes 69.)
+// Per cent of the largest shared memory, a hint: the join needs few KB of it, and the rest caches the rows that a
+// token's heads share. Without it the join runs with what the first kernel has asked for, all of it: one request of 60
+// nodes 20.2 us, with 15 to 65 per cent 18.5; 64 of 16 nodes 64.1, with up to 35 per cent 61.9.
+constexpr int TJ_CARVE = 35;
 constexpr int TJ_RESIDENT = 5;  // CTAs an SM of one group (4 to 8: within 4 %)
 
 template <int D, int DT, bool SPLIT>
@@ -1076,6 +1080,9 @@ static int launch_tree_attention(const CUtensorMap (&maps)[4], const TreeAttnPar
   const dim3 grid((unsigned)ceil_div((int64_t)p.tokens * p.G, 8), p.n_kvh);
   auto join = [&](auto split) {  // a second group where the rows alone do not fill the SMs
     constexpr bool SPLIT = decltype(split)::value;
+    static SmemOptIn carve{cudaFuncAttributePreferredSharedMemoryCarveout};
+    if (cudaError_t e = carve(tree_join_kernel<D, DT, SPLIT>, TJ_CARVE))
+      return cuda_fail(e, "tree_join_kernel attributes");
     return cuda_fail(launch_pdl(tree_join_kernel<D, DT, SPLIT>, grid, SPLIT ? 256 : 128, 0, st, p), "tree_join_kernel");
   };
   return (int64_t)grid.x * grid.y <= 2 * 148 ? join(std::true_type{}) : join(std::false_type{});
