@@ -6,11 +6,12 @@
 // loads a lane before the first store). Many more CTAs than the SMs hold, each a few pieces, so that the SMs keep
 // busy whatever rows the blocks hold: 256 copies of 1 to 64 rows in 16 caches 88 us (6.4 TB/s; whole blocks 6.7), as
 // many CTAs as are resident 96, and one CTA a head of a block with the next one's loads ahead of its stores 104 to 117.
-// cache_compact: a warp takes one head of one request's path in four caches: the path and the blocks are looked up
-// once, and three rows in each cache are under way at once (64 paths of 6 nodes in 32 caches 7.4 us; one cache and
-// four rows a warp 12.0). Row base + path[k] goes to base + k, and path[k] >= k, in ascending order: a row that is
-// written (k) was a source only for smaller k (path[k'] = k means k' <= k), so that a warp that loads a run of rows
-// before it stores them, run after run, never reads a row that it has overwritten.
+// cache_compact: a warp takes one head of one request's path in three caches: the path and the blocks are looked up
+// once, and three rows in each cache are under way at once (64 paths of 6 nodes in 32 caches 7.2 us, 64 of 12 in 64
+// caches 35; in four caches, with three CTAs an SM, 8.0 and 40; in two, with six, 7.4 and 37; in one 11.4 and 50).
+// Row base + path[k] goes to base + k, and path[k] >= k, in ascending order: a row that is written (k) was a source
+// only for smaller k (path[k'] = k means k' <= k), so that a warp that loads a run of rows before it stores them, run
+// after run, never reads a row that it has overwritten.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -22,7 +23,7 @@ constexpr int MOVE_WARPS = MOVE_THREADS / 32;
 constexpr int COPY_LOADS = 8;   // 16-byte loads of a lane under way
 constexpr int COPY_CTAS = 80;   // of an SM's share of a long list, most of them waiting
 constexpr int MOVE_RUN = 3;     // rows of a path that a lane moves at once
-constexpr int MOVE_CACHES = 4;  // in so many caches
+constexpr int MOVE_CACHES = 3;  // in so many caches
 
 struct MoveCaches {
   uint16_t* base[YSKN_MAX_CACHES];
@@ -83,7 +84,7 @@ struct CompactParams {
   unsigned* err;
 };
 
-__global__ void __launch_bounds__(MOVE_THREADS, 3) cache_compact_kernel(const __grid_constant__ CompactParams p) {
+__global__ void __launch_bounds__(MOVE_THREADS, 5) cache_compact_kernel(const __grid_constant__ CompactParams p) {
   pdl_begin();
   const MoveCaches& c = p.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -98,6 +99,11 @@ __global__ void __launch_bounds__(MOVE_THREADS, 3) cache_compact_kernel(const __
     const int len = __ldg(p.lens + r);
     const int32_t* table = p.tables + (int64_t)r * p.table_stride;
     const int32_t* path = p.path + (int64_t)r * p.path_stride;
+    // Lane l: node k0 + l of the path, for the run from k0 on; the first asked for beside the lengths.
+    auto nodes = [&](int k0) {
+      return lane < min(at_once * MOVE_RUN, p.path_width - k0) ? __ldg(path + k0 + lane) : -1;
+    };
+    int node = nodes(0);
     const long long base = (long long)len - n - p.prefix_len;  // own row of the first new one
     if (n == 0) continue;
     // the same in all lanes; a block of this lane's outside the caches
@@ -113,9 +119,7 @@ __global__ void __launch_bounds__(MOVE_THREADS, 3) cache_compact_kernel(const __
     };
     int before = -1;  // the node before this run's first
     for (int k0 = 0; !wrong && k0 < p.path_width; k0 += at_once * MOVE_RUN) {
-      // Lane l: node k0 + l of the path; how many of the run are in order.
-      const int run = min(at_once * MOVE_RUN, p.path_width - k0);
-      const int node = lane < run ? __ldg(path + k0 + lane) : -1;
+      const int run = min(at_once * MOVE_RUN, p.path_width - k0);  // how many of them are in order:
       int prior = __shfl_up_sync(0xffffffffu, node, 1);
       if (lane == 0) prior = before;
       const unsigned ends = __ballot_sync(0xffffffffu, lane >= run || node < 0);
@@ -147,6 +151,7 @@ __global__ void __launch_bounds__(MOVE_THREADS, 3) cache_compact_kernel(const __
       __syncwarp();
       if (stop < run) break;
       before = __shfl_sync(0xffffffffu, node, run - 1);
+      node = nodes(k0 + run);
     }
     if (__any_sync(0xffffffffu, wrong || lost) && lane == 0) raise_device_error(p.err, DERR_RANGE);
   }

@@ -30,11 +30,11 @@
 // ring holds does not cover the memory's latency; the tensor cores need 1.1); results, 1 KB a row and segment both
 // ways, where they have few (a segment of one tile and 252 rows 4.9 us, without its stores 2.8); set-up, 8 us.
 // Everything is summed in a fixed order: the same call gives the same bits.
-// us a call, and with a mask on prefix_attention's kernel instead: one request of 60 nodes and 2000 rows 20.4, 29.7; of
-// 32 nodes and 8000 rows 23.0, 43.7; 8 of 60 nodes and up to 8000 rows 60, 100; 64 of 16 nodes and up to 1000 rows 67,
-// 119; 32 of 32 nodes behind 4096 rows with up to 4096 of their own 152, 151. (One CTA with 128 rows instead of the
+// us a call, and with a mask on prefix_attention's kernel instead: one request of 60 nodes and 2000 rows 18.5, 29.7; of
+// 32 nodes and 8000 rows 22, 43.7; 8 of 60 nodes and up to 8000 rows 58, 100; 64 of 16 nodes and up to 1000 rows 62,
+// 119; 32 of 32 nodes behind 4096 rows with up to 4096 of their own 146, 151. (One CTA with 128 rows instead of the
 // pair, whose ring holds 1.25 tiles instead of 2.5: 25, 37, 72, 67 and 180, where the pair then took 25, 24, 60, 69 and
-// 156, still with the join by one group and an item's rows not halved between the CTAs.)
+// 156, with a slower join and an item's rows not halved between the CTAs.)
 // Every mbarrier wait is bounded; after a timeout the softmax warps go through their remaining tiles without waiting,
 // so that the halves' named barriers still match, and both CTAs meet before either leaves.
 #include <algorithm>
@@ -776,7 +776,7 @@ __device__ __forceinline__ float4 ta_four(uint2 v) {
 // every fourth 16-byte unit of the quarter from qd on. The new rows first: a few visible ones of each row at a time,
 // keys and values asked for together, the scores of the quarters added up through shared memory. Then the row's
 // segments. What bounds it is the chain of dependent loads (the token's request, its table, its rows; the segments),
-// and instructions where there are many rows (64 requests of 16 nodes: 25 of 67 us). Where there are few rows, which
+// and instructions where there are many rows (64 requests of 16 nodes: 17 of 62 us, of which new rows 8). Where there are few rows, which
 // then have many segments (SPLIT), four more warps take the segments beside those for the new rows, which do not wait
 // for the first kernel. By one group, by two, by four (a CTA an SM then): one request of 60 nodes and 2000 rows 24, 20,
 // 25 us; of 32 nodes and 8000 rows 33, 23, 22; 16 of 16 nodes and 1500 rows, more rows than the rule's, 27, 30, 30.
