@@ -466,7 +466,7 @@ extern "C" YSKN_B200_API int yskn_b200_token_logprobs(const yskn_b200_token_logp
     p.cluster *= 2;
   // The slice whose last one of a warp's run is emptiest by fewest groups, the larger of two alike. us with 8, 10 loads
   // where 10 leave no more empty: one row of 151936 with 20 largest 9.0, 8.2, 256 rows 31.8, 30.9, 512 rows 60.0, 57.9;
-  // where 8 leave less: 33 rows of 50257 7.8, 8.4, 512 rows of 32000 19.6, 20.9, of 2000 9.4, 10.0. (11 and more spill.)
+  // where 8 leave less: 33 rows of 50257 7.8, 8.4, 512 rows of 32000 19.6, 20.9, of 2000 9.4, 10.0. (11 spill.)
   const int run = (int)ceil_div(ceil_div(a.vocab / 4, p.cluster), LP_WARPS);
   const bool many = ceil_div(run, LP_MANY * 32) * LP_MANY <= ceil_div(run, LP_FEW * 32) * LP_FEW;
   cudaLaunchConfig_t cfg = {};

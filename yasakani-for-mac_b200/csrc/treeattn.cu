@@ -776,9 +776,9 @@ __device__ __forceinline__ float4 ta_four(uint2 v) {
 // every fourth 16-byte unit of the quarter from qd on. The new rows first: a few visible ones of each row at a time,
 // keys and values asked for together, the scores of the quarters added up through shared memory. Then the row's
 // segments. What bounds it is the chain of dependent loads (the token's request, its table, its rows; the segments),
-// and instructions where there are many rows (64 requests of 16 nodes: 17 of 62 us, of which new rows 8). Where there are few rows, which
-// then have many segments (SPLIT), four more warps take the segments beside those for the new rows, which do not wait
-// for the first kernel. By one group, by two, by four (a CTA an SM then): one request of 60 nodes and 2000 rows 24, 20,
+// and instructions where there are many rows (64 requests of 16 nodes: 17 of 62 us, of which new rows 8). Where there
+// are few rows, which then have many segments (SPLIT), four more warps take the segments beside those for the new rows,
+// which do not wait for the first kernel. By one group, by two, by four (a CTA an SM then): one request of 60 nodes and 2000 rows 24, 20,
 // 25 us; of 32 nodes and 8000 rows 33, 23, 22; 16 of 16 nodes and 1500 rows, more rows than the rule's, 27, 30, 30.
 // (A warp for all heads of a token, whose lanes share the keys and values: fewer instructions, but 200 registers, and
 // 64 requests 89 us where this takes 69.)
@@ -786,7 +786,9 @@ __device__ __forceinline__ float4 ta_four(uint2 v) {
 // token's heads share. Without it the join runs with what the first kernel has asked for, all of it: one request of 60
 // nodes 20.2 us, with 15 to 65 per cent 18.5; 64 of 16 nodes 64.1, with up to 35 per cent 61.9.
 constexpr int TJ_CARVE = 35;
-constexpr int TJ_RESIDENT = 5;  // CTAs an SM of one group (4 to 8: within 4 %)
+// CTAs an SM of one group. 4, 5, 6, 7: 64 requests of 16 nodes 65, 62, 63, 69 us, 32 of 32 behind 4096 rows 149, 146,
+// 149, 152.
+constexpr int TJ_RESIDENT = 5;
 
 template <int D, int DT, bool SPLIT>
 __global__ void __launch_bounds__(SPLIT ? 256 : 128, SPLIT ? 2 : TJ_RESIDENT)
