@@ -16,17 +16,18 @@
 // CTAs an SM that load and work in turn, 52.5 with two that load 8 ahead; half the slice, four CTAs, 49.9, but with
 // the largest tokens 74 against 60, and 12.2 against 9.0 for one row.)
 // A logit is a key: its bits in an order of unsigned numbers, above the complement of its number, so that keys are all
-// different and equal logits go by the lowest number. With m = ceil(n_top / 8), the least of the 8 warps' m-th largest
-// lane maxima so far bounds the keys that can be among the n_top largest: at least n_top logits reach it, and few more
-// (20 of the first 8192 logits, 90 of 151936, for 8 largest). What reaches it goes to the warp's buffer in shared
-// memory; in the end each key of the CTA's buffers counts the keys above it, which is its place. Rows whose largest
-// come late fill a buffer: then 32 keys are sorted (bitonic, in registers) and merged into a list of the warp's 32
+// different and equal logits go by the lowest number. A bound holds most keys off that cannot be among the n_top
+// largest: n_top of the 32 groups of 8 lanes have a logit that reaches it. (The 8 largest of 151936: 9 of the first 8192
+// logits reach it, 35 in all.) What reaches it goes to the warp's buffer in shared memory; in the end each key of the
+// CTA's buffers counts the keys above it, which is its place. Rows whose largest come late fill a buffer: then 32 keys
+// are sorted (bitonic, in registers) and merged into a list of the warp's 32
 // largest, whose n_top-th is a bound too. (All keys through such lists: 93 us for 512 rows, and the chain of shuffles
 // made one row wait 13.)
 // The passing logits are read again, from the cache, by a rolled loop: 32 copies of its code for the slice's registers
-// took 62 us for 512 rows instead of 59.8, and one row, where each CTA runs the code once and waits for it, 10.6.
-// Measured on the device: one row of 151936 with 20 largest 8.2 us (without them 4.7), 33 rows of 50257 7.8, 256 rows
-// of 151936 with 8 largest 30.8 (5.1 TB/s), 512 rows 57.9 (5.4 TB/s, without the largest 50.4; two CTAs of 512 on every
+// took 62 us for 512 rows instead of 59.8, and one row, where each CTA runs the code once and waits for it, 10.6 instead
+// of 9.0.
+// Measured on the device: one row of 151936 with 20 largest 7.9 us (without them 4.7), 33 rows of 50257 7.5, 256 rows
+// of 151936 with 8 largest 29.8 (5.2 TB/s), 512 rows 56.1 (5.5 TB/s, without the largest 50.4; two CTAs of 512 on every
 // SM and a half).
 #include <algorithm>
 #include <type_traits>
@@ -130,6 +131,15 @@ __device__ __forceinline__ uint64_t lp_merge(uint64_t list, uint64_t up, int lan
   return lp_bitonic_down(list > up ? list : up, lane);
 }
 
+__device__ __forceinline__ uint4 lp_shared_u32x4(const uint32_t* p) {
+  uint4 y;
+  asm volatile("ld.volatile.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+               : "r"((uint32_t)__cvta_generic_to_shared(p))
+               : "memory");
+  return y;
+}
+
 // ---- the cluster
 __device__ __forceinline__ void lp_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -146,6 +156,10 @@ __device__ __forceinline__ void lp_put_f32(uint32_t a, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
 }
 
+// Up to so many largest the bound is the groups' n_top-th largest logit; for more, where that is nearly the groups' least,
+// the least of the warps' ceil(n_top / 8)-th largest lane maxima. us by groups, by warps: 512 rows with 8 largest 56.1,
+// 57.7, with one 52.9, 57.7; 64 rows with 20 14.5, 15.9, one row 7.9, 8.2; 300 rows with 32 71, 56.5.
+constexpr int LP_BINNED = 24;
 constexpr int LP_BUFFER = 160;  // keys: up to 31 that are left, and 128 that may join them
 
 // A warp's largest keys: `list` descending over the lanes, `bound` the least that may still enter, `held` keys in
@@ -173,7 +187,7 @@ __device__ __noinline__ LpTop lp_flush(LpTop t, uint64_t* buffer, int least, int
 
 struct LpShared {
   uint64_t buffer[LP_WARPS][LP_BUFFER];
-  alignas(16) uint32_t bound[LP_WARPS];  // each warp's m-th largest lane maximum so far
+  alignas(16) uint32_t bound[32];  // of each 8 lanes the largest so far, or each warp's m-th largest lane maximum
   int held[LP_WARPS];  // keys in each buffer; in the end all of the warp's
   alignas(16) uint64_t keys[LP_WARPS * 64 + 1];  // to be ranked
   uint64_t list[YSKN_MAX_TOP];   // this CTA's largest
@@ -305,16 +319,34 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT)
     if constexpr (TOP) {
       so_far = max(so_far, mine == mine ? lp_ordered(mine) : 0u);  // (a NaN is no one's bound)
       if (raise) {
-        uint32_t o = so_far, mth = 0;
-        for (int i = 0; i < p.n_top; i += LP_WARPS) {  // the largest goes, one lane of it
-          mth = __reduce_max_sync(0xffffffffu, o);
-          if (lane == __ffs(__ballot_sync(0xffffffffu, o == mth)) - 1) o = 0;
+        uint32_t least;
+        if (p.n_top <= LP_BINNED) {
+          uint32_t most = so_far;
+#pragma unroll
+          for (int by = 1; by < 8; by <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, by));
+          if ((lane & 7) == 0) *reinterpret_cast<volatile uint32_t*>(sh.bound + warp * 4 + (lane >> 3)) = most;
+          if (g == w0) __syncthreads();  // later older numbers of the other warps serve as well: they only grow
+          const uint32_t own = *reinterpret_cast<volatile uint32_t*>(sh.bound + lane);
+          int reach = 0;
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const uint4 y = lp_shared_u32x4(sh.bound + j);
+            reach += (y.x >= own) + (y.y >= own) + (y.z >= own) + (y.w >= own);
+          }
+          least = __reduce_max_sync(0xffffffffu, reach >= p.n_top ? own : 0u);
+        } else {
+          uint32_t o = so_far, mth = 0;
+          for (int i = 0; i < p.n_top; i += LP_WARPS) {  // the largest goes, one lane of it
+            mth = __reduce_max_sync(0xffffffffu, o);
+            if (lane == __ffs(__ballot_sync(0xffffffffu, o == mth)) - 1) o = 0;
+          }
+          if (lane == 0) *reinterpret_cast<volatile uint32_t*>(sh.bound + warp) = mth;
+          if (g == w0) __syncthreads();
+          least = lane < LP_WARPS ? *reinterpret_cast<volatile uint32_t*>(sh.bound + lane) : 0xffffffffu;
+          least = __reduce_min_sync(0xffffffffu, least);
         }
-        if (lane == 0) *reinterpret_cast<volatile uint32_t*>(sh.bound + warp) = mth;
-        if (g == w0) __syncthreads();  // later an older number of another warp serves as well
-        const uint32_t all = lane < LP_WARPS ? *reinterpret_cast<volatile uint32_t*>(sh.bound + lane) : 0xffffffffu;
-        const uint64_t least = ((uint64_t)__reduce_min_sync(0xffffffffu, all) << 32) - 1;
-        top.bound = least + 1 > top.bound ? least : top.bound;
+        const uint64_t below = ((uint64_t)least << 32) - 1;
+        top.bound = below + 1 > top.bound ? below : top.bound;
       }
       // What passes (keys from bound + 1 on) is above `edge`, or equal to it and of a number up to edge_id.
       float edge = lp_value((uint32_t)((top.bound + 1) >> 32));
