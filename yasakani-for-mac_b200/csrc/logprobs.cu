@@ -17,15 +17,14 @@
 // the largest tokens 74 against 60, and 12.2 against 9.0 for one row.)
 // A logit is a key: its bits in an order of unsigned numbers, above the complement of its number, so that keys are all
 // different and equal logits go by the lowest number. A bound holds most keys off that cannot be among the n_top
-// largest: n_top of the 32 groups of 8 lanes have a logit that reaches it. (The 8 largest of 151936: 9 of the first 8192
-// logits reach it, 35 in all.) What reaches it goes to the warp's buffer in shared memory; in the end each key of the
-// CTA's buffers counts the keys above it, which is its place. Rows whose largest come late fill a buffer: then 32 keys
-// are sorted (bitonic, in registers) and merged into a list of the warp's 32
-// largest, whose n_top-th is a bound too. (All keys through such lists: 93 us for 512 rows, and the chain of shuffles
-// made one row wait 13.)
+// largest: n_top of the 32 groups of 8 lanes have a logit that reaches it. (The 8 largest of 151936: 9 of the first
+// 8192 logits reach it, 35 in all.) What reaches it goes to the warp's buffer in shared memory; in the end each key of
+// the CTA's buffers counts the keys above it, which is its place. Rows whose largest come late fill a buffer: then 32
+// keys are sorted (bitonic, in registers) and merged into a list of the warp's 32 largest, whose n_top-th is a bound
+// too. (All keys through such lists: 93 us for 512 rows, and the chain of shuffles made one row wait 13.)
 // The passing logits are read again, from the cache, by a rolled loop: 32 copies of its code for the slice's registers
-// took 62 us for 512 rows instead of 59.8, and one row, where each CTA runs the code once and waits for it, 10.6 instead
-// of 9.0.
+// took 62 us for 512 rows instead of 59.8, and one row, where each CTA runs the code once and waits for it, 10.6
+// instead of 9.0.
 // Measured on the device: one row of 151936 with 20 largest 7.9 us (without them 4.7), 33 rows of 50257 7.5, 256 rows
 // of 151936 with 8 largest 29.8 (5.2 TB/s), 512 rows 56.1 (5.5 TB/s, without the largest 50.4; two CTAs of 512 on every
 // SM and a half).
@@ -156,9 +155,9 @@ __device__ __forceinline__ void lp_put_f32(uint32_t a, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
 }
 
-// Up to so many largest the bound is the groups' n_top-th largest logit; for more, where that is nearly the groups' least,
-// the least of the warps' ceil(n_top / 8)-th largest lane maxima. us by groups, by warps: 512 rows with 8 largest 56.1,
-// 57.7, with one 52.9, 57.7; 64 rows with 20 14.5, 15.9, one row 7.9, 8.2; 300 rows with 32 71, 56.5.
+// Up to so many largest the bound is the groups' n_top-th largest logit; for more, where that is nearly the groups'
+// least, the least of the warps' ceil(n_top / 8)-th largest lane maxima. us by groups, by warps: 512 rows with 8
+// largest 56.1, 57.7, with one 52.9, 57.7; 64 rows with 20 14.5, 15.9, one row 7.9, 8.2; 300 rows with 32 71, 56.5.
 constexpr int LP_BINNED = 24;
 constexpr int LP_BUFFER = 160;  // keys: up to 31 that are left, and 128 that may join them
 
@@ -258,7 +257,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_RESIDENT)
   const int row = blockIdx.x / p.cluster, rank = blockIdx.x - row * p.cluster;
   const float* x = p.logits + row * p.logits_stride;
   // The row's whole 16-byte groups, of which this part has [g0, g1) and this warp [w0, w1): all warps some, where
-  // there are 8, so that the least of their bounds is one. Up to three logits before and after them (lanes 0..2 and
+  // there are 8, so that each has a part of the bound. Up to three logits before and after them (lanes 0..2 and
   // 3..5) are a slice of their own of the first part's first warp.
   const int head = min((int)(-(reinterpret_cast<uintptr_t>(x) >> 2) & 3), p.vocab);
   const int n_groups = (p.vocab - head) >> 2, tail = p.vocab - head - 4 * n_groups;
