@@ -206,3 +206,26 @@ def test_same_bits_each_time_on_another_stream_and_in_a_graph(cuda):
     for p, q, r in zip(a, b, c):
         assert torch.equal(p, q) and torch.equal(p, r)
     assert (a[3][:, 0] == t[:, 0]).all()
+
+
+@pytest.mark.parametrize("k", [1, 8, 20, 23, 24, 25])
+def test_largest_in_few_places(cuda, k):
+    """Both bounds where they hold off least: the largest in one lane's places, in eight lanes', in one warp's run, at
+    the row's ends, few logits above -inf, and rows of two numbers; in one part and in several."""
+    rng = np.random.default_rng(k)
+    for V, M in ((50257, 6), (151936, 6), (9001, 300)):
+        x = rows(k, M, V)
+        x[0, 4 * 17::1024] += 30
+        x[1, (np.arange(V) // 4 % 32) < 8] += 25
+        x[2, V // 3:V // 3 + 900] += 25
+        x[3, :7] += 40
+        x[3, -9:] += 40
+        keep = rng.choice(V, k + 1, replace=False)
+        x[4] = np.where(np.isin(np.arange(V), keep), x[4], -np.inf)
+        x[5] = np.where(rng.random(V) < 0.3, np.float32(2.5), np.float32(-1.0))
+        if M > 6:
+            x[6:] = np.sort(x[6:], axis=1)
+        check(cuda, x[:7] if M > 6 else x, [[0, V - 1]] * min(M, 7), k)
+        if M > 6:  # one CTA a row, and all rows' numbers
+            _, _, _, ids = call(cuda, x, [[0]] * M, k)
+            assert [i.tolist() for i in ids] == [order(r.astype(np.float64), k) for r in x]
