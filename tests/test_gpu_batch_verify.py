@@ -1,0 +1,121 @@
+"""Verified trees of requests that are behind their text (yskn_b200/batch.py): nothing of theirs changes."""
+import pytest
+
+from test_gpu_batch_tree import _prompt, _stack, _started
+
+pytestmark = pytest.mark.gpu
+
+
+def _i32(cuda, *a):
+    import torch
+    return torch.tensor(a, dtype=torch.int32, device=cuda)
+
+
+def _pages(st, request):
+    """All layers' rows of the request's own blocks, as long as its length says."""
+    import torch
+    own = max(st.lens[request].item() - st.prefix_len, 0)
+    blocks = st.tables[request, :-(-own // st.block_size)].long()
+    return [c[blocks].reshape(-1, *c.shape[2:])[:own].clone() for c in st.caches.caches] + [torch.tensor(own)]
+
+
+def test_a_fork_that_the_pool_does_not_hold_waits_in_verify(cuda):
+    """Its copy has no rows (length 0) and its whole text: the last token alone, at the text's beginning, is no answer."""
+    import torch
+    import yskn_b200 as Y
+    from test_gpu_batch_tree import _prefix
+    st = _stack(cuda, batch=3, max_tokens=64, capacity=48, n_blocks=5, nodes=4)
+    st.fill_prefix(_prefix(cuda, 16))
+    st.say(0, _prompt(0, 20))
+    st.say(2, _prompt(2, 3))
+    st.new.copy_(st.said)
+    st.step(23, 20)
+    assert st.free.item() == 1  # too few for the copy, enough for a token or two
+    st.fork(_i32(cuda, 0, 0, 2))
+    assert st.lens.tolist() == [36, 0, 19] and st.said.tolist() == [21, 21, 4]
+    text = st.text.clone()
+    for i in range(3):
+        st.draft(i, [5, 6], [0, 1])
+    st.new.copy_(_i32(cuda, 3, 3, 3))
+    st.verify(9)
+    acc = st.accepted.tolist()
+    assert Y.status() == 0 and acc[1] == 0 and min(acc[0], acc[2]) >= 1
+    assert st.lens.tolist() == [36 + acc[0], 0, 19 + acc[2]] and st.said.tolist() == [21 + acc[0], 21, 4 + acc[2]]
+    assert torch.equal(st.text[1], text[1]) and st.free.item() == 1
+
+
+@pytest.mark.parametrize("P", [0, 75])
+def test_requests_that_are_behind_their_text_wait(cuda, P):
+    """Nothing run, some of a prompt run, nothing said, all run: none of them has one token left; the one that has goes
+    on, and an ending one ends."""
+    import torch
+    import yskn_b200 as Y
+    st = _started(cuda, [3, 19, 14, 5, 7, 2], P)
+    st.say(0, _prompt(9, 12))      # a longer prompt: 3 of 12 run
+    st.said[1] = 19                # all run
+    st.new.copy_(_i32(cuda, 0, 0, -1, 0, 0, -1))
+    st.step(6, 1)                  # requests 2 and 5 end
+    st.say(2, _prompt(8, 10))      # nothing run
+    st.said[5] = 0                 # nothing said
+    text, said, lens, free = st.text.clone(), st.said.tolist(), st.lens.tolist(), st.free.item()
+    pages = [_pages(st, i) for i in (0, 1, 3)]
+    for i in range(6):
+        st.draft(i, [5, 6], [0, 0])
+    st.new.copy_(_i32(cuda, 3, 3, 1, 3, -1, 3))
+    st.verify(18)
+    acc = st.accepted.tolist()
+    assert Y.status() == 0 and acc[:3] == [0, 0, 0] and acc[3] >= 1 and acc[4:] == [0, 0]
+    said[3] += acc[3]
+    own = [P + n if n else 0 for n in (3, 19, 0, 5 + acc[3], 0, 0)]
+    assert st.said.tolist() == said and st.lens.tolist() == own
+    assert all(torch.equal(st.text[i], text[i]) for i in (0, 1, 2, 4, 5))
+    assert torch.equal(st.text[3, :6], text[3, :6])
+    for i, before in zip((0, 1), pages):
+        assert all(torch.equal(a, b) for a, b in zip(before, _pages(st, i)))
+    assert all(torch.equal(a[:5], b[:5]) for a, b in zip(pages[2][:-1], _pages(st, 3)[:-1]))
+    held = lambda n: -(-n // 16)  # noqa: E731
+    assert st.free.item() == free + held(7) - held(5 + acc[3]) + held(5)
+    # and those behind are served by step, which runs what they said
+    st.new.copy_(_i32(cuda, 9, 0, 10, 0, 0, 0))
+    st.step(19, 10)
+    assert Y.status() == 0 and st.said.tolist()[:3] == [13, 19, 11] and st.lens.tolist()[:3] == [P + 12, P + 19, P + 10]
+
+
+def test_a_captured_fork_and_verify_keep_a_request_that_did_not_fit(cuda):
+    """Nobody on the host sees the length between the two."""
+    import torch
+    import yskn_b200 as Y
+    got = []
+    for captured in (False, True):
+        st = _stack(cuda, batch=2, max_tokens=64, capacity=48, n_blocks=5, nodes=4)
+        st.say(0, _prompt(0, 40))
+        st.new.copy_(_i32(cuda, 40, 0))
+        st.step(40, 40)
+        st.draft(0, [5, 6], [0, 1])
+        st.draft(1, [5, 6], [0, 1])
+        st.new.fill_(3)
+        source, stream = _i32(cuda, 0, 0), torch.cuda.Stream(cuda)
+        torch.cuda.synchronize()
+        if captured:
+            warm = _stack(cuda, batch=2, max_tokens=64, capacity=48, n_blocks=5, nodes=4)
+            warm.say(0, [1])
+            warm.new.fill_(1)
+            warm.step(2, 1)
+            warm.fork(source, stream)
+            warm.verify(6, stream)
+            torch.cuda.synchronize()
+            assert Y.status() == 0
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                st.fork(source, stream)
+                st.verify(6, stream)
+            g.replay()
+        else:
+            st.fork(source, stream)
+            st.verify(6, stream)
+        torch.cuda.synchronize()
+        assert Y.status() == 0
+        assert st.lens[1].item() == 0 and st.said[1].item() == 41 and st.accepted[1].item() == 0
+        assert torch.equal(st.text[1, :41], st.text[0, :41]) and not bool(st.text[1, 41:].any())
+        got.append([st.text.clone(), st.said.clone(), st.lens.clone(), st.free.clone()])
+    assert all(torch.equal(a, b) for a, b in zip(*got))

@@ -185,15 +185,19 @@ class BatchStack(S.Stack):
     def verify(self, n_tokens, stream=None):
         """Runs the trees of the requests that have drafted some: self.new[i] nodes of request i (0: none; 1: its next
         token alone), n_tokens in all at most. The tokens of each accepted path and the model's choice behind it are
-        appended; the cache keeps the path's rows. Choices are the largest logits, without penalties and masks (which
-        what a node's ancestors say would change), of requests that have run all they said but the last token."""
+        appended; the cache keeps the path's rows. A request that has not run all it said but the last token waits, as
+        one whose rows do not fit does: a prompt that step has not run to its end, a fork whose copy did not fit.
+        Choices are the largest logits, without penalties and masks (which what a node's ancestors say would
+        change)."""
         torch, T, W = self.torch, n_tokens, self.capacity
         if not self.nodes or not 0 < T <= self.max_tokens:
             raise Y.YsknError(Y.EINVAL, "verify: a loop made for trees, and 1..%d tokens" % self.max_tokens)
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.verify(n_tokens)
-        Y.batch_plan(self.lens, self.new, self.tables, self.pool, self.free, self.block_size, self.lens_out,
+        own = self.lens - self.prefix_len * (self.lens > 0)
+        new = torch.where((own == self.said - 1) | (self.new < 0), self.new, 0)
+        Y.batch_plan(self.lens, new, self.tables, self.pool, self.free, self.block_size, self.lens_out,
                      self.free_out, self.starts, self.slots[:T], self.pos[:T], self.requests[:T], self.prefix_len)
         request = self.requests[:T].clamp(min=0).long()
         node = (torch.arange(T, device=self.dev) - self.starts[request]).clamp(0, self.nodes - 1)
