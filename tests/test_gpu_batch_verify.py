@@ -1,7 +1,8 @@
-"""Verified trees of requests that are behind their text (yskn_b200/batch.py): nothing of theirs changes."""
+"""Verified trees of requests that are behind their text, of which nothing changes, or at its end
+(yskn_b200/batch.py)."""
 import pytest
 
-from test_gpu_batch_tree import _prompt, _stack, _started
+from test_gpu_batch_tree import _choices, _prompt, _stack, _started
 
 pytestmark = pytest.mark.gpu
 
@@ -119,3 +120,45 @@ def test_a_captured_fork_and_verify_keep_a_request_that_did_not_fit(cuda):
         assert torch.equal(st.text[1, :41], st.text[0, :41]) and not bool(st.text[1, 41:].any())
         got.append([st.text.clone(), st.said.clone(), st.lens.clone(), st.free.clone()])
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("capacity,said", [(20, 18), (20, 19), (20, 20), (20, 14), (33, 30), (31, 29)])
+def test_paths_end_where_the_text_does(cuda, capacity, said, monkeypatch):
+    """A chain of 7 right drafts near the end of a text whose last block has more rows than it has tokens."""
+    import yskn_b200 as Y
+    st = _stack(cuda, batch=2, max_tokens=64, capacity=capacity, n_blocks=12, nodes=8)
+    rows = 16 * -(-capacity // 16)
+    st.say(0, _prompt(0, said - 1))
+    st.say(1, _prompt(1, 3))
+    st.new.copy_(st.said)
+    st.step(said + 2, said - 1)
+    assert st.said.tolist() == [said, 4]
+    n = min(8, rows - said + 1)  # what the table holds
+    chain = [100 + j for j in range(n - 1)]
+    st.draft(0, chain, list(range(n - 1)))
+    st.draft(1, [100, 101], [0, 1])
+    st.new.copy_(_i32(cuda, n, 3))
+    # the model's choice after node j is node j + 1's token; after the last one 777
+    _choices(monkeypatch, {**{j: t for j, t in enumerate(chain + [777])}, n: 100, n + 1: 101, n + 2: 55})
+    st.verify(n + 3)
+    monkeypatch.undo()
+    took = min(n, capacity - said + 1)  # rows up to the text's last token
+    text = _prompt(0, said - 1) + st.text[0, said - 1:said].tolist() + chain + [777]
+    assert Y.status() == 0
+    assert st.accepted.tolist() == [took, 3]
+    assert st.path[0].tolist() == list(range(took)) + [-1] * (8 - took)
+    assert st.next[0].item() == (chain + [777])[took - 1]
+    assert st.said.tolist() == [min(said + took, capacity), 7] and st.lens.tolist() == [said - 1 + took, 6]
+    assert st.text[0, :st.said[0].item()].tolist() == text[:min(said + took, capacity)]
+    assert st.text[1, 4:7].tolist() == [100, 101, 55]
+    assert st.free.item() == 12 - -(-(said - 1 + took) // 16) - 1
+    # the text full: verify leaves it alone from here on
+    before = st.text.clone()
+    for _ in range(3):
+        lens = st.lens[0].item()
+        st.new.copy_(_i32(cuda, 1, 0))
+        st.verify(1)
+        assert Y.status() == 0 and st.said[0].item() <= capacity and st.lens[0].item() <= capacity
+        if lens == capacity:
+            assert st.accepted.tolist() == [0, 0] and st.lens[0].item() == capacity
+            assert (st.text[0] == before[0]).all()

@@ -186,7 +186,8 @@ class BatchStack(S.Stack):
         """Runs the trees of the requests that have drafted some: self.new[i] nodes of request i (0: none; 1: its next
         token alone), n_tokens in all at most. The tokens of each accepted path and the model's choice behind it are
         appended; the cache keeps the path's rows. A request that has not run all it said but the last token waits, as
-        one whose rows do not fit does: a prompt that step has not run to its end, a fork whose copy did not fit.
+        one whose rows do not fit does: a prompt that step has not run to its end, a fork whose copy did not fit. Paths
+        end where the text does, with its last token run and nothing behind it.
         Choices are the largest logits, without penalties and masks (which what a node's ancestors say would
         change)."""
         torch, T, W = self.torch, n_tokens, self.capacity
@@ -213,7 +214,9 @@ class BatchStack(S.Stack):
         if self.logprobs is not None:
             self._score(logits, choice, self.node_logprob[:T], self.node_entropy[:T], self.node_top_logprobs[:T],
                         self.node_top_ids[:T])
-        Y.tree_accept(self.tokens[:T], self.parents[:T], choice, self.starts, self.lens_out, self.path, self.accepted,
+        # (a node behind the text's last place follows none, so that no path has it)
+        fits = torch.where(self.tree_pos[:T] - self.prefix_len < W, self.parents[:T], -1)
+        Y.tree_accept(self.tokens[:T], fits, choice, self.starts, self.lens_out, self.path, self.accepted,
                       self.keep, self.next)
         Y.cache_compact(self.caches, self.tables, self.lens_out, self.starts, self.path, self.prefix_len)
         Y.batch_edit(self.lens_out, self.keep, self.tables, self.pool, self.free_out, self.block_size, self.lens,
