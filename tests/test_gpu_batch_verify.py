@@ -1,8 +1,14 @@
-"""Verified trees of requests that are behind their text, of which nothing changes, or at its end
-(yskn_b200/batch.py)."""
+"""Verified trees of requests that are behind their text, at its end, or under controls (yskn_b200/batch.py): what the
+loop one token at a time would have done, nothing lost.
+
+Everything here is whole numbers held equal, but for the adjusted logits: the unadjusted ones have the same bits in a
+second loop (same calls, same inputs), to which the formula is applied in 64 bits; the call rounds each of its four steps
+once, and a quotient by the repetition, so that with u = 2^-24 the result is off by at most 4 u times the largest
+intermediate value."""
+import numpy as np
 import pytest
 
-from test_gpu_batch_tree import _choices, _prompt, _stack, _started
+from test_gpu_batch_tree import VOCAB, _choices, _prompt, _stack, _started
 
 pytestmark = pytest.mark.gpu
 
@@ -162,3 +168,92 @@ def test_paths_end_where_the_text_does(cuda, capacity, said, monkeypatch):
         if lens == capacity:
             assert st.accepted.tolist() == [0, 0] and st.lens[0].item() == capacity
             assert (st.text[0] == before[0]).all()
+
+
+def _controls(st, cuda, seed):
+    """A penalty or two for each request, and masks that allow half the tokens (all of request 2's)."""
+    import torch
+    rng = np.random.default_rng(seed)
+    B = st.batch
+    st.repetition.copy_(torch.tensor([1.0, 1.7, 1.3, 0.8][:B]))
+    st.presence.copy_(torch.tensor([0.0, 0.5, -0.25, 1.5][:B]))
+    st.frequency.copy_(torch.tensor([0.0, 0.25, 0.75, -0.5][:B]))
+    mask = rng.integers(0, 2 ** 32, (B, VOCAB // 32), dtype=np.uint32)
+    if B > 2:
+        mask[2] = 0xffffffff
+    st.mask.copy_(torch.from_numpy(mask.view(np.int32)))
+    return (mask[:, np.arange(VOCAB) // 32] >> (np.arange(VOCAB) % 32).astype(np.uint32)) & 1 == 1
+
+
+@pytest.mark.parametrize("P", [0, 75])
+def test_controls_of_every_node(cuda, P):
+    """Each node's logits under its request's controls, by the request's text and what the node's ancestors say (its own
+    token among them; often one that the text has, or an ancestor)."""
+    import torch
+    import yskn_b200 as Y
+    sizes = [3, 19, 14, 5]
+    trees = [([7, 7, 9], [0, 1, 1]), (_prompt(1, 6) + [7, 7], [0, 0, 1, 3, 4, 4, 6, 7]), ([], []),
+             ([50, 50, 50, 51], [0, 1, 2, 3])]
+    T = sum(1 + len(t) for t, _ in trees)
+    loops = []
+    for controlled in (False, True):
+        st = _started(cuda, sizes, P)
+        for i, (tokens, parents) in enumerate(trees):
+            st.draft(i, tokens, parents)
+            st.new[i] = 1 + len(tokens)
+        allowed = _controls(st, cuda, 3) if controlled else None
+        text = [st.text[i, :st.said[i].item()].tolist() for i in range(4)]
+        st.verify(T + 2)  # and two places that hold no token
+        assert Y.status() == 0
+        loops.append((st, text))
+    (plain, text), (st, _) = loops
+    raw, got, t = plain.tlogits[:T].double().cpu().numpy(), st.tlogits[:T].cpu().numpy(), 0
+    u = 2.0 ** -24
+    for i, (tokens, parents) in enumerate(trees):
+        said = [[]]
+        for tok, p in zip(tokens, parents):
+            said.append(said[p] + [tok])
+        r, pres, freq = (x[i].item() for x in (st.repetition, st.presence, st.frequency))
+        for path in said:
+            history, x = text[i] + path, raw[t].copy()
+            seen, count = np.zeros(VOCAB, bool), np.zeros(VOCAB)
+            seen[history] = True
+            np.add.at(count, history[sizes[i]:], 1)  # behind the prompt
+            x = np.where(seen, np.where(x > 0, x / r, x * r), x)
+            most = np.maximum(np.abs(raw[t]), np.abs(x))
+            x = x - freq * count
+            most = np.maximum(most, np.abs(freq * count) + np.abs(x))
+            x = x - np.where(count > 0, pres, 0.0)
+            most = np.maximum(most, np.abs(x) + abs(pres))
+            assert np.array_equal(np.isneginf(got[t]), ~allowed[i]), (i, path)
+            ok = allowed[i]
+            assert (np.abs(got[t][ok] - x[ok]) <= 4 * u * most[ok]).all(), (i, path)
+            assert st.choice[t].item() == int(got[t].argmax())  # of the adjusted ones, the first of equal ones
+            t += 1
+    for i in range(4):  # no token that the mask forbids has been said
+        assert all(allowed[i][tok] for tok in st.text[i, sizes[i] + 1:st.said[i].item()].tolist())
+
+
+@pytest.mark.parametrize("seed", [1, 2])
+def test_one_node_alone_is_a_step_under_controls(cuda, seed):
+    """Without drafts: the choice of verify is that of step, whose penalties and masks it has."""
+    import yskn_b200 as Y
+    sizes, P = [3, 19, 14, 5], 75
+    one, st = _started(cuda, sizes, P, logprobs=3), _started(cuda, sizes, P, logprobs=3)
+    for s in (one, st):
+        allowed = _controls(s, cuda, seed)
+        s.new.fill_(1)
+    one.step(4, 1)
+    st.verify(4)
+    assert Y.status() == 0 and st.accepted.tolist() == [1] * 4
+    a, b = one.blogits.cpu().numpy(), st.tlogits[:4].cpu().numpy()
+    assert np.array_equal(np.isneginf(a), np.isneginf(b)) and np.array_equal(np.isneginf(a), ~allowed)
+    for i in range(4):
+        ok, chose = allowed[i], int(b[i].argmax())
+        off = 2 * np.abs(a[i][ok] - b[i][ok]).max()  # the two orders of sums
+        assert off < 1.0 and a[i].max() - a[i][chose] <= off and st.next[i].item() == chose
+        assert st.text[i, sizes[i] + 1].item() == chose and ok[chose]
+    # the log probability is that of the adjusted logits, as in step
+    lse = np.log(np.exp(b.astype(np.float64)).sum(1))
+    want = b[np.arange(4), st.choice[:4].tolist()] - lse
+    assert np.abs(st.node_logprob[:4, 0].cpu().numpy() - want).max() <= 1e-5

@@ -188,8 +188,8 @@ class BatchStack(S.Stack):
         appended; the cache keeps the path's rows. A request that has not run all it said but the last token waits, as
         one whose rows do not fit does: a prompt that step has not run to its end, a fork whose copy did not fit. Paths
         end where the text does, with its last token run and nothing behind it.
-        Choices are the largest logits, without penalties and masks (which what a node's ancestors say would
-        change)."""
+        Choices are those that steps with the request's controls as they are would make: a node's penalties count what
+        its ancestors and itself say, and the request's mask holds for every node."""
         torch, T, W = self.torch, n_tokens, self.capacity
         if not self.nodes or not 0 < T <= self.max_tokens:
             raise Y.YsknError(Y.EINVAL, "verify: a loop made for trees, and 1..%d tokens" % self.max_tokens)
@@ -210,6 +210,7 @@ class BatchStack(S.Stack):
                      self.tree_pos[:T], self.tree[:T])
         logits, choice = self.tlogits[:T], self.choice[:T]
         Y.linear([self.head], self.bx[:T], self.bwork, [logits], inv_rms=self.binv[:T])
+        self._adjust_nodes(logits, request)
         Y.head_select(logits, token=choice)
         if self.logprobs is not None:
             self._score(logits, choice, self.node_logprob[:T], self.node_entropy[:T], self.node_top_logprobs[:T],
@@ -229,6 +230,23 @@ class BatchStack(S.Stack):
         new = torch.where(col == count - 1, self.next.unsqueeze(1), took.gather(1, col.clamp(0, self.nodes - 1)))
         self.text.copy_(torch.where((col >= 0) & (col < count), new, self.text))
         self.said.copy_((self.said + self.accepted).clamp(max=W))
+
+    def _adjust_nodes(self, logits, request):
+        """The controls of each node's request on its logits: its history is the request's text, then the tokens from
+        node 1 on of the path that leads to it, its own the last."""
+        torch, T, N = self.torch, logits.shape[0], self.nodes
+        first = self.starts[:-1].long()[request].clamp(max=T - 1)
+        node = torch.arange(N, device=self.dev).unsqueeze(0)
+        at = (first.unsqueeze(1) + node).clamp(max=T - 1)  # of each node of the same tree
+        depth = self.tree_pos[:T] - self.tree_pos[first]  # of each token; what follows no one here has 0
+        sees = (self.tree[:T].gather(1, (node >> 5).expand(T, N)) >> (node & 31)) & 1 == 1
+        said, end = self.said[request], self.capacity + N  # a history's last place: for what it does not hold
+        history = torch.cat([self.text, self.text.new_zeros(self.batch, N + 1)], 1)[request]
+        place = torch.where(sees & (depth[at] > 0), said.unsqueeze(1) - 1 + depth[at], end)
+        history.scatter_(1, place.clamp(0, end).long(), self.tokens[at])
+        Y.logits_adjust(logits, logits, history=history[:, :end], history_lens=said + depth.clamp(min=0),
+                        prompt_lens=self.prompt[request], repetition=self.repetition[request],
+                        presence=self.presence[request], frequency=self.frequency[request], mask=self.mask[request])
 
     def fork(self, source, stream=None):
         """Request i becomes a copy of request source[i] (int32 [batch] on the device; itself: it goes on; negative: it
