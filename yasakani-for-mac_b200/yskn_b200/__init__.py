@@ -814,20 +814,22 @@ def _attention_args(name, q, k_cache, v_cache, block_tables, lens, starts, max_n
     n_blocks, block_size, n_kvh, _ = cache
     B, width = block_tables.shape
     qs, cs, row = q.stride(), k_cache.stride(), block_tables.stride()
-    _need(q.shape == shape and cache[3] == D and v_cache.shape == cache and v_cache.stride() == cs and cs[3] == 1 and
-          qs[2] == 1 and out.is_contiguous() and k_cache.dtype is dt and v_cache.dtype is dt and out.dtype is dt,
-          name + ": q, out and caches of one type and head size with dense channels expected")
-    _need(block_tables.dtype is i32 and lens.dtype is i32 and starts.dtype is i32 and lens.numel() == B and
-          starts.numel() == B + 1 and row[1] == 1 and lens.is_contiguous() and starts.is_contiguous() and
-          work.is_contiguous() and
-          (not prefix_len or (prefix_blocks is not None and prefix_blocks.dtype is i32 and
-                              prefix_blocks.is_contiguous() and prefix_blocks.numel() * block_size >= prefix_len)),
-          name + ": dense int32 tables, lengths and starts of one batch, and the prefix's blocks expected")
+    # (not by _need: the messages would be put together at each call)
+    if not (q.shape == shape and cache[3] == D and v_cache.shape == cache and v_cache.stride() == cs and cs[3] == 1 and
+            qs[2] == 1 and out.is_contiguous() and k_cache.dtype is dt and v_cache.dtype is dt and out.dtype is dt):
+        raise YsknError(EINVAL, name + ": q, out and caches of one type and head size with dense channels expected")
+    if not (block_tables.dtype is i32 and lens.dtype is i32 and starts.dtype is i32 and lens.numel() == B and
+            starts.numel() == B + 1 and row[1] == 1 and lens.is_contiguous() and starts.is_contiguous() and
+            work.is_contiguous() and
+            (not prefix_len or (prefix_blocks is not None and prefix_blocks.dtype is i32 and
+                                prefix_blocks.is_contiguous() and prefix_blocks.numel() * block_size >= prefix_len))):
+        raise YsknError(EINVAL, name + ": dense int32 tables, lengths and starts of one batch, and the prefix's blocks "
+                        "expected")
     gs, gd = (0, 0), 0
     if gate is not None:
         gs, gd = gate.stride(), _dtype(gate)
-        _need(gate.shape == shape and gs[2] == 1,
-              name + ": a gate of the queries' shape with dense channels expected")
+        if not (gate.shape == shape and gs[2] == 1):
+            raise YsknError(EINVAL, name + ": a gate of the queries' shape with dense channels expected")
     return (
         q.data_ptr(), qs[0], qs[1], 0 if gate is None else gate.data_ptr(), gs[0], gs[1], k_cache.data_ptr(),
         v_cache.data_ptr(), cs[0], cs[1], cs[2], prefix_blocks.data_ptr() if prefix_len else 0,
