@@ -1,6 +1,6 @@
 """Attention of drafted trees (yskn_b200_tree_attention) over its arguments: scales of either sign and zero, masks and
-largest requests wider than the trees, gates in f32 with strides and of any size. Few rows are joined by two groups of
-warps a CTA, many by one; both are taken.
+largest requests wider than the trees, gates in f32 with strides and of any size, starts that overlap. Few rows are
+joined by two groups of warps a CTA, many by one; both are taken.
 
 Tolerance as in test_gpu_tree_attention.py, whose run() takes the scale into it. A gate's factor 1 / (1 + exp(-g)), one
 approximate exponential, sum and quotient in binary32, is off by at most 2^-20 of itself."""
@@ -139,3 +139,31 @@ def test_tokens_that_see_nothing_give_zeros_whatever_their_gate_holds(cuda, D, h
     gate[10] = -float("inf")
     out = c.run(gate)
     assert Y.status() == 0 and bool((out[9:11] == 0).all()) and not bool(out.isnan().any())
+
+
+@pytest.mark.parametrize("P", [0, 130])
+def test_requests_that_overlap_stay_inside_the_workspace(cuda, P):
+    """Starts that go back again name 12 items of 16 tokens a KV head, where six requests of 64 tokens in all have 10
+    places: nothing is computed, every row is zero, and the status says so."""
+    import torch
+    import yskn_b200 as Y
+    T, B, G, hk, D, bs = 64, 6, 16, 2, 64, 16
+    g = torch.Generator(device=cuda)
+    g.manual_seed(1)
+    rnd = lambda *s: torch.randn(s, generator=g, device=cuda).bfloat16()  # noqa: E731
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=cuda)  # noqa: E731
+    q, kc, vc = rnd(T, G * hk, D), rnd(60, bs, hk, D), rnd(60, bs, hk, D)
+    n = Y.prefix_attention_work_bytes(T, B, T, G * hk, hk, D)
+    buffer = torch.full((n + 4096,), 91, dtype=torch.uint8, device=cuda)
+    out, mask = torch.full_like(q, 3.0), torch.full((T, 2), -1, dtype=torch.int32, device=cuda)
+    tables, prefix = torch.arange(48, device=cuda).int().view(B, 8), torch.arange(48, 57, device=cuda).int()
+    args = (q, kc, vc, tables, i32([P + 100] * B))
+
+    def attend(starts):
+        Y.tree_attention(*args, i32(starts), T, mask, buffer[:n], out, prefix_blocks=prefix, prefix_len=P)
+        torch.cuda.synchronize()
+        assert bool((buffer[n:] == 91).all())
+        return Y.status()
+
+    assert attend([0, 64, 0, 64, 0, 64, 0]) == Y.EINVAL and bool((out == 0).all())
+    assert attend([0, 64, 64, 64, 64, 64, 64]) == 0 and bool(out.float().isfinite().all()) and bool((out != 0).any())
