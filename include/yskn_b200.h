@@ -771,9 +771,9 @@ YSKN_B200_API int yskn_b200_tree_accept(const yskn_b200_tree_accept_args* args, 
  * copies int32 [3][copies_stride], max_copies used: the block to read, the block to write, its rows; -1,
  * -1, 0 past the last of *n_copies. Such a request is served if the pool and the list hold its blocks
  * with those of all such requests before it; else it ends (length 0, no blocks). What no one goes on
- * in goes back to the pool. Written: lens_out [batch], *free_out (arrays of their own, not keep), the pool, and
- * with a source tables_out [batch][tables_out_stride] (an array of its own; entries of the kept
- * blocks; without a source the tables stay valid and tables_out, copies and n_copies are not used).
+ * in goes back to the pool. Written: lens_out [batch], *free_out, the pool, and with a source *n_copies, copies and
+ * tables_out [batch][tables_out_stride] (entries of the kept blocks; without a source the tables stay valid and
+ * tables_out, copies and n_copies are not used); all arrays of their own, of which no other one is a part.
  * Lengths, sources or a count that do not fit their arrays give YSKN_EINVAL from yskn_b200_status. One launch. */
 typedef struct {
   const int32_t *lens, *keep, *source; /* [batch] */

@@ -229,9 +229,17 @@ extern "C" YSKN_B200_API int yskn_b200_batch_edit(const yskn_b200_batch_edit_arg
   if (fork && (a.max_copies < 1 || a.copies_stride < a.max_copies ||
                (a.batch > 1 && a.tables_out_stride < a.table_width)))
     return fail(YSKN_EINVAL, "batch_edit: an empty list of copies, or a stride below its width");
-  if (a.lens_out == a.lens || a.lens_out == a.keep || a.lens_out == a.source || a.free_out == a.free ||
-      (fork && a.tables_out == a.block_tables))
-    return fail(YSKN_EINVAL, "batch_edit: the new lengths, count and tables need arrays of their own");
+  // Every CTA reads the lengths, sources and count, the first one writes: dense arrays by all their bytes. (Tables may be
+  // interleaved.)
+  const int64_t row = 4ll * a.batch;
+  const Span in[] = {{a.lens, row}, {a.keep, row}, {a.source, row}, {a.free, 4}};
+  const Span out[] = {{a.lens_out, row}, {a.free_out, 4}, {a.pool, 4ll * a.pool_capacity}, {fork ? a.n_copies : nullptr, 4}};
+  bool meet = fork && a.tables_out == a.block_tables;
+  for (int i = 0; i < 4; ++i) {
+    for (const Span& s : in) meet = meet || out[i].meets(s);
+    for (int j = 0; j < i; ++j) meet = meet || out[i].meets(out[j]);
+  }
+  if (meet) return fail(YSKN_EINVAL, "batch_edit: the new lengths, counts, tables and the pool need arrays of their own");
   EditParams p{};
   p.lens = a.lens, p.keep = a.keep, p.source = a.source;
   p.tables = a.block_tables, p.table_stride = a.table_stride;

@@ -72,6 +72,16 @@ struct SmemOptIn {
   }
 };
 
+// An array of a call, for looking whether an output meets another one: its first byte and how many (none: no array).
+struct Span {
+  const void* at;
+  int64_t bytes;
+  bool meets(const Span& o) const {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(at), b = reinterpret_cast<uintptr_t>(o.at);
+    return at && o.at && a < b + (uintptr_t)o.bytes && b < a + (uintptr_t)bytes;
+  }
+};
+
 // Thread-local error message (src/c_api.cpp:11-14 keeps one per thread as well).
 int fail(int code, const std::string& msg);
 int cuda_fail(cudaError_t e, const char* where);
