@@ -119,6 +119,12 @@ extern "C" YSKN_B200_API int yskn_b200_tree_plan(const yskn_b200_tree_plan_args*
   if (a.tokens < 1 || a.tokens > 1 << 30 || a.batch < 1 || a.mask_words < 1 || a.mask_words > YSKN_TREE_MAX_WORDS ||
       (a.tokens > 1 && a.mask_stride < a.mask_words))
     return fail(YSKN_EINVAL, "tree_plan: empty shape, 1..32 mask words, or a stride below them");
+  // Each warp reads its tree's parents and its request's lengths: not where others have written.
+  const Span parents{a.parents, 4ll * a.tokens}, starts{a.starts, 4ll * a.batch + 4}, lens{a.lens, 4ll * a.batch};
+  const Span mask{a.mask, 4ll * ((a.tokens - 1) * a.mask_stride + a.mask_words)}, positions{a.positions, 4ll * a.tokens};
+  for (const Span& in : {parents, starts, lens})
+    if (positions.meets(in) || mask.meets(in) || mask.meets(positions))
+      return fail(YSKN_EINVAL, "tree_plan: the masks and positions need arrays of their own");
   TreePlanParams p{a.parents, a.requests, a.starts,  a.lens,  a.mask,       a.mask_stride,
                    a.positions, a.tokens, a.batch, a.mask_words, device_error_word()};
   return cuda_fail(launch_pdl(tree_plan_kernel, (unsigned)ceil_div(a.tokens, TREE_WARPS), TREE_WARPS * 32, 0,
@@ -134,6 +140,18 @@ extern "C" YSKN_B200_API int yskn_b200_tree_accept(const yskn_b200_tree_accept_a
   if (a.batch < 1 || a.batch > 1 << 30 || a.n_tokens < 1 || a.n_tokens > 1 << 30 || a.path_width < 1 ||
       (a.batch > 1 && a.path_stride < a.path_width))
     return fail(YSKN_EINVAL, "tree_accept: empty shape, or a stride below the path's width");
+  // A warp reads its request's length alone, so that the new one may take its place; the rest others read too.
+  const int64_t row = 4ll * a.batch, nodes = 4ll * a.n_tokens;
+  const Span lens{a.lens, row}, in[] = {{a.tokens, nodes}, {a.parents, nodes}, {a.choice, nodes}, {a.starts, row + 4}};
+  const Span path{a.path, 4ll * ((a.batch - 1) * a.path_stride + a.path_width)};
+  const Span out[] = {path, {a.accepted, row}, {a.next, row}, {a.lens_out, row}};
+  bool meet = false;
+  for (int i = 0; i < 4; ++i) {
+    for (const Span& s : in) meet = meet || out[i].meets(s);
+    for (int j = 0; j < i; ++j) meet = meet || out[i].meets(out[j]);
+    meet = meet || (out[i].meets(lens) && !(i == 3 && a.lens_out == a.lens));
+  }
+  if (meet) return fail(YSKN_EINVAL, "tree_accept: paths, counts and lengths need arrays of their own");
   TreeAcceptParams p{a.tokens,   a.parents,  a.choice, a.starts, a.lens,     a.path,       a.path_stride,
                      a.accepted, a.lens_out, a.next,   a.batch,  a.n_tokens, a.path_width, device_error_word()};
   return cuda_fail(launch_pdl(tree_accept_kernel, (unsigned)ceil_div(a.batch, TREE_WARPS), TREE_WARPS * 32, 0,
