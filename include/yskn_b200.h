@@ -655,7 +655,8 @@ YSKN_B200_API int yskn_b200_paged_prep(const yskn_b200_paged_prep_args* args, vo
  * 64, 128 or 256 channels; blocks of 16, 32, 64 or 128 rows; the cache's strides as in
  * yskn_b200_paged_prep. Pointers and strides are multiples of 16 bytes. A block number outside
  * the cache, a length past what the request's table row can name or a request of more than max_new
- * tokens gives YSKN_EINVAL from yskn_b200_status. work: work_bytes of memory, at least
+ * tokens gives YSKN_EINVAL from yskn_b200_status. The softmax weights are rounded to the cache's type where
+ * matrix instructions take them, all sums are binary32. work: work_bytes of memory, at least
  * yskn_b200_prefix_attention_work_bytes() (which never falls as tokens, batch or max_new grow, so that
  * the largest step's serves all), one call's at a time. */
 YSKN_B200_API int64_t yskn_b200_prefix_attention_work_bytes(int tokens, int batch, int max_new, int n_qh, int n_kvh,
@@ -736,8 +737,10 @@ YSKN_B200_API int yskn_b200_tree_plan(const yskn_b200_tree_plan_args* args, void
  * every row before the request's new ones (the whole prefix among them), and of those row j <= t if bit
  * j % 32 of word j / 32 of its mask row is set (uint32 mask [tokens][mask_stride], mask_words of them).
  * Everything else as there, its workspace and its size among it; a token that sees nothing gives zeros, and
- * new rows that a token does not see may hold anything. A request of more new tokens than mask bits, or
- * whose lens do not hold the prefix and its new tokens, gives zeros and YSKN_EINVAL from yskn_b200_status. */
+ * new rows that a token does not see may hold anything. The work on new rows grows with how many each token
+ * sees: a draft without branches needs no mask, and from some 16 nodes on prefix_attention is faster. A
+ * request of more new tokens than mask bits, or whose lens do not hold the prefix and its new tokens, gives
+ * zeros and YSKN_EINVAL from yskn_b200_status. */
 typedef struct {
   yskn_b200_prefix_attention_args attn;
   const uint32_t* mask;

@@ -13,8 +13,9 @@
 // heirs (atomic maxima of (k, i) in shared memory: no two are equal, so the order changes nothing) and the
 // sums over the whole batch, then its warps take pieces of 64 entries of the new tables, and of the
 // pool's and the list's ends. Nothing that any CTA reads is written: the stack is read below its old count
-// and written above it, the tables and lengths go to other arrays. 64 requests that keep fewer rows 3.5 us, 1024 of
-// which a third continue others 6.6 (with a division for each request's blocks, where a shift does, 7.2).
+// and written above it, the tables and lengths go to other arrays. 64 requests that keep fewer rows 3.5 us in a captured
+// graph, 1024 of which a third continue others 6.6 (with a division for each request's blocks, where a shift does, 7.2);
+// calls by themselves, which the host bounds, 6.3 and 8.5.
 #include <algorithm>
 
 #include "common.cuh"

@@ -33,7 +33,10 @@ __device__ __forceinline__ void raise_device_error(unsigned* word, unsigned bits
 // first statement, pdl_begin(), waits for that kernel's completion and memory (before any
 // access to memory) and then lets the next kernel of the stream be scheduled early, so a
 // following operator loads its tables while this kernel runs. Both are no-ops in a kernel
-// launched without the attribute.
+// launched without the attribute. What a kernel may touch before pdl_begin() is what neither the
+// kernel before it in the same call writes nor, since that one lets it start only after its own
+// pdl_begin(), any kernel before that: the inputs of a call of two kernels, in its second
+// (tree_join_kernel, which says so). No launch may come between the two.
 __device__ __forceinline__ void pdl_begin() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");

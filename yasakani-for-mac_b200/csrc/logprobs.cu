@@ -17,8 +17,8 @@
 // the largest tokens 74 against 60, and 12.2 against 9.0 for one row.)
 // A logit is a key: its bits in an order of unsigned numbers, above the complement of its number, so that keys are all
 // different and equal logits go by the lowest number. A bound holds most keys off that cannot be among the n_top
-// largest: n_top of the 32 groups of 8 lanes have a logit that reaches it. (The 8 largest of 151936: 9 of the first
-// 8192 logits reach it, 35 in all.) What reaches it goes to the warp's buffer in shared memory; in the end each key of
+// largest: n_top of the 32 groups of 8 lanes have a logit that reaches it. (The 8 largest of 151936 normal ones: 9 of the
+// 10240 in the warps' first slices reach it, 30 in all.) What reaches it goes to the warp's buffer in shared memory; in the end each key of
 // the CTA's buffers counts the keys above it, which is its place. Rows whose largest come late fill a buffer: then 32
 // keys are sorted (bitonic, in registers) and merged into a list of the warp's 32 largest, whose n_top-th is a bound
 // too. (All keys through such lists: 93 us for 512 rows, and the chain of shuffles made one row wait 13.)

@@ -30,11 +30,16 @@
 // ring holds does not cover the memory's latency; the tensor cores need 1.1); results, 1 KB a row and segment both
 // ways, where they have few (a segment of one tile and 252 rows 4.9 us, without its stores 2.8); set-up, 8 us.
 // Everything is summed in a fixed order: the same call gives the same bits.
-// us a call, and with a mask on prefix_attention's kernel instead: one request of 60 nodes and 2000 rows 18.5, 29.7; of
-// 32 nodes and 8000 rows 22, 43.7; 8 of 60 nodes and up to 8000 rows 58, 100; 64 of 16 nodes and up to 1000 rows 62,
-// 119; 32 of 32 nodes behind 4096 rows with up to 4096 of their own 146, 151. (One CTA with 128 rows instead of the
-// pair, whose ring holds 1.25 tiles instead of 2.5: 25, 37, 72, 67 and 180, where the pair then took 25, 24, 60, 69 and
-// 156, with a slower join and an item's rows not halved between the CTAs.)
+// Rounded to 16 bits: the weights over the rows before the new ones, as the tensor cores take them (the type of V; 32-bit
+// ones would be tf32, at half the rate, with V widened on the way), and the result. m, l, o, the joins and the new rows'
+// weights are binary32, l the sum of the unrounded weights. Error against 64 bits 0.0021 to 0.0023 of the norm in bf16,
+// where the result's rounding alone gives 0.0017, 0.00028 and 0.00021 in f16.
+// us in a captured graph, and with a mask on prefix_attention's kernel instead: one request of 60 nodes and 2000 rows
+// 18.5, 29.7; of 32 nodes and 8000 rows 22, 43.7; 8 of 60 nodes and up to 8000 rows 58, 100; 64 of 16 nodes and up to
+// 1000 rows 62, 119; 32 of 32 nodes behind 4096 rows with up to 4096 of their own 146, 151. Calls one after another, each
+// on inputs of its own, take 20 for the first and, at the clocks of a long run, 170 to 176 for the last. (One CTA with 128
+// rows instead of the pair, whose ring holds 1.25 tiles instead of 2.5: 25, 37, 72, 67 and 180, where the pair then took
+// 25, 24, 60, 69 and 156, with a slower join and an item's rows not halved between the CTAs.)
 // Every mbarrier wait is bounded; after a timeout the softmax warps go through their remaining tiles without waiting,
 // so that the halves' named barriers still match, and both CTAs meet before either leaves.
 #include <algorithm>
@@ -782,6 +787,11 @@ __device__ __forceinline__ float4 ta_four(uint2 v) {
 // 25 us; of 32 nodes and 8000 rows 33, 23, 22; 16 of 16 nodes and 1500 rows, more rows than the rule's, 27, 30, 30.
 // (A warp for all heads of a token, whose lanes share the keys and values: fewer instructions, but 200 registers, and
 // 64 requests 89 us where this takes 69.)
+// Its new rows' work grows with what a node sees, and each query head reads it again: a tree's few ancestors, not a long
+// chain (us behind 2000 rows, a chain of 8, 16, 32, 60, 128: 14.5, 18, 29, 45, 105, prefix_attention 23, 24, 28, 34, 33).
+// It reads the call's inputs before pdl_begin(), and the first group of SPLIT never waits: it starts only once every CTA
+// of tree_attention_kernel has passed its own pdl_begin(), so that what came before the call is done and in memory; the
+// first kernel's results, and all writes, come after the wait. Nothing may be launched between the two.
 // Per cent of the largest shared memory, a hint: the join needs few KB of it, and the rest caches the rows that a
 // token's heads share. Without it the join runs with what the first kernel has asked for, all of it: one request of 60
 // nodes 20.2 us, with 15 to 65 per cent 18.5; 64 of 16 nodes 64.1, with up to 35 per cent 61.9.
