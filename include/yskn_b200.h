@@ -722,7 +722,7 @@ YSKN_B200_API int yskn_b200_logits_adjust(const yskn_b200_logits_adjust_args* ar
  * [tokens]: lens[r] - n + the number of its ancestors (lens with the n new rows). Padding gives no
  * bits and position -1. A parent at or behind its node (taken for none), a node past the mask's bits
  * (not set) or starts that do not hold t give YSKN_EINVAL from yskn_b200_status. The mask and the positions
- * have no part in common with each other, the parents, starts or lens. One launch. */
+ * have no part in common with the parents, starts or lens. One launch. */
 #define YSKN_TREE_MAX_WORDS 32
 typedef struct {
   const int32_t *parents, *requests, *starts, *lens; /* [tokens], [tokens], [batch + 1], [batch] */
@@ -756,7 +756,7 @@ YSKN_B200_API int yskn_b200_tree_attention(const yskn_b200_tree_attention_args* 
  * them; accepted [batch]: how many; lens_out [batch]: lens less the new rows that are not on the path (may
  * be lens); next [batch]: the choice after the last one (-1 for a request without tokens). Starts that
  * do not ascend within tokens give YSKN_EINVAL from yskn_b200_status and an empty path. What is written has no
- * part in common with the inputs (but lens_out, if it is lens) or with one another. One launch. */
+ * part in common with the inputs, but that accepted, lens_out or next may be lens. One launch. */
 typedef struct {
   const int32_t *tokens, *parents, *choice; /* [n_tokens] */
   const int32_t *starts, *lens;             /* [batch + 1], [batch] */

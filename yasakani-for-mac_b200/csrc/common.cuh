@@ -84,6 +84,13 @@ struct Span {
     return at && o.at && a < b + (uintptr_t)o.bytes && b < a + (uintptr_t)bytes;
   }
 };
+// The same of `rows` (1 or more) rows of `width` bytes, `stride` bytes (no less than width) from one to the next, of
+// which what lies between them is no part.
+inline bool rows_meet(const void* at, int64_t rows, int64_t stride, int64_t width, const Span& o) {
+  const int64_t behind = (int64_t)(reinterpret_cast<uintptr_t>(o.at) - reinterpret_cast<uintptr_t>(at)) - width;
+  const int64_t r = behind < 0 ? 0 : rows > 1 ? behind / stride + 1 : 1;  // the first row that ends behind o's first byte
+  return r < rows && Span{reinterpret_cast<const uint8_t*>(at) + (r > 0 ? r * stride : 0), width}.meets(o);
+}
 
 // Thread-local error message (src/c_api.cpp:11-14 keeps one per thread as well).
 int fail(int code, const std::string& msg);

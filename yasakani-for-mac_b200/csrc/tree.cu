@@ -121,9 +121,9 @@ extern "C" YSKN_B200_API int yskn_b200_tree_plan(const yskn_b200_tree_plan_args*
     return fail(YSKN_EINVAL, "tree_plan: empty shape, 1..32 mask words, or a stride below them");
   // Each warp reads its tree's parents and its request's lengths: not where others have written.
   const Span parents{a.parents, 4ll * a.tokens}, starts{a.starts, 4ll * a.batch + 4}, lens{a.lens, 4ll * a.batch};
-  const Span mask{a.mask, 4ll * ((a.tokens - 1) * a.mask_stride + a.mask_words)}, positions{a.positions, 4ll * a.tokens};
+  const Span positions{a.positions, 4ll * a.tokens};
   for (const Span& in : {parents, starts, lens})
-    if (positions.meets(in) || mask.meets(in) || mask.meets(positions))
+    if (positions.meets(in) || rows_meet(a.mask, a.tokens, 4 * a.mask_stride, 4ll * a.mask_words, in))
       return fail(YSKN_EINVAL, "tree_plan: the masks and positions need arrays of their own");
   TreePlanParams p{a.parents, a.requests, a.starts,  a.lens,  a.mask,       a.mask_stride,
                    a.positions, a.tokens, a.batch, a.mask_words, device_error_word()};
@@ -140,16 +140,14 @@ extern "C" YSKN_B200_API int yskn_b200_tree_accept(const yskn_b200_tree_accept_a
   if (a.batch < 1 || a.batch > 1 << 30 || a.n_tokens < 1 || a.n_tokens > 1 << 30 || a.path_width < 1 ||
       (a.batch > 1 && a.path_stride < a.path_width))
     return fail(YSKN_EINVAL, "tree_accept: empty shape, or a stride below the path's width");
-  // A warp reads its request's length alone, so that the new one may take its place; the rest others read too.
+  // Other warps read these; its request's length a warp reads alone, so that a result may take that one's place.
   const int64_t row = 4ll * a.batch, nodes = 4ll * a.n_tokens;
-  const Span lens{a.lens, row}, in[] = {{a.tokens, nodes}, {a.parents, nodes}, {a.choice, nodes}, {a.starts, row + 4}};
-  const Span path{a.path, 4ll * ((a.batch - 1) * a.path_stride + a.path_width)};
-  const Span out[] = {path, {a.accepted, row}, {a.next, row}, {a.lens_out, row}};
+  const Span in[] = {{a.tokens, nodes}, {a.parents, nodes}, {a.choice, nodes}, {a.starts, row + 4}, {a.lens, row}};
   bool meet = false;
-  for (int i = 0; i < 4; ++i) {
-    for (const Span& s : in) meet = meet || out[i].meets(s);
-    for (int j = 0; j < i; ++j) meet = meet || out[i].meets(out[j]);
-    meet = meet || (out[i].meets(lens) && !(i == 3 && a.lens_out == a.lens));
+  for (const Span& s : in) {
+    for (const int32_t* out : {a.accepted, a.lens_out, a.next})
+      meet = meet || (out != a.lens && Span{out, row}.meets(s));
+    meet = meet || rows_meet(a.path, a.batch, 4 * a.path_stride, 4ll * a.path_width, s);
   }
   if (meet) return fail(YSKN_EINVAL, "tree_accept: paths, counts and lengths need arrays of their own");
   TreeAcceptParams p{a.tokens,   a.parents,  a.choice, a.starts, a.lens,     a.path,       a.path_stride,
